@@ -163,7 +163,7 @@ def _window_inputs(case, g):
     q = _normal(g, (int(n.sum()), case["heads"], d), dt, 1.5)
     k = _normal(g, (int(m.sum()), case["kv_heads"], d), dt)
     v = _normal(g, (int(m.sum()), case["kv_heads"], dv), dt)
-    return dict(q=q, k=k, v=v, cu_q=cu_q, cu_k=cu_k, max_q=int(n.max()))
+    return dict(q=q, k=k, v=v, cu_q=cu_q, cu_k=cu_k)
 
 
 def _attend_inputs(case, g):
@@ -264,8 +264,8 @@ def _window_own(case, s):
     import streaming_attention_b200 as sa
     if case["form"] == "dense":
         return sa.sliding_window_attention(s["q"], s["k"], s["v"], window=case["window"], sinks=case["sinks"])
-    return sa.sliding_window_attention_packed(s["q"], s["k"], s["v"], s["cu_q"], s["cu_k"], s["max_q"],
-                                              window=case["window"], sinks=case["sinks"])
+    return sa.sliding_window_attention_packed(s["q"], s["k"], s["v"], s["cu_q"], s["cu_k"], window=case["window"],
+                                              sinks=case["sinks"])
 
 
 def _cache_of(case, s):
