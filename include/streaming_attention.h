@@ -323,6 +323,101 @@ int sa_flash_causal_attention(const float* q, const float* k, const float* v, in
                               int d, int dv, float scale, float* out, void* workspace,
                               size_t workspace_bytes, void* stream);
 
+/* ---- serving: windowed attention, a paged 4-bit cache, page plans, norm + rotation ----
+ * No counterpart in the reference.  dtype is an SA_REP_* code, of every tensor
+ * of elements in the call; strides are in elements and the last dimension is
+ * contiguous.  The kernels check the contents of device-side index arrays
+ * (offsets, slots, page tables, lengths): what is out of range is skipped and
+ * recorded in the device's error word, which sa_serving_status reads.  No call
+ * allocates or needs a workspace; all may be captured into a graph. */
+
+/* Synchronises `stream`, then returns SA_OK, or what the serving calls on this
+ * device recorded first since the last read (SA_ERR_INVALID_ARG for bad index
+ * contents, SA_ERR_TIMEOUT for a bounded wait that gave up) and clears it. */
+int sa_serving_status(void* stream);
+
+/* Attention with a sliding window and first tokens that stay visible:
+ *   out_i = softmax over visible j of (scale q_i.k_j), times v_j,
+ *   visible: j <= p and (j > p - window or j < sinks), p = m - n + i;
+ * window 0 means no end.  A query that sees nothing gives zeros.  Query head h
+ * reads key head h / (heads / kv_heads).
+ * Dense (cu_q == cu_k == NULL): q [batch, heads, n, d], k [batch, kv_heads, m,
+ * d], v [.., m, dv], out like q with dv; strides = {q_b, q_h, q_n, k_b, k_h,
+ * k_n, v_b, v_h, v_n, o_b, o_h, o_n}.  Packed: cu_q, cu_k [batch + 1] are the
+ * requests' first rows in q / out (n rows in all) and k / v (m rows in all),
+ * p counts within the request, the *_b strides are 0; rows behind
+ * cu_q[batch] stay as they were.  d, dv <= 256. */
+int sa_window_attention(const void* q, const void* k, const void* v, void* out, const int64_t* strides, int batch,
+                        int heads, int kv_heads, int64_t n, int64_t m, int d, int dv, int64_t window, int64_t sinks,
+                        float scale, int dtype, const int32_t* cu_q, const int32_t* cu_k, void* stream);
+
+/* The cache: pages of page_size (16, 32, 64, 128 or 256) tokens; dp = d filled
+ * up to 32, 64, 128 or 256 (d <= 256); byte b of a row holds column 2 b in its
+ * low and 2 b + 1 in its high half:
+ *   k_codes  uint8 [pages, heads, page_size, dp / 2]
+ *   v_codes  uint8 [pages, heads, page_size / 4, dp / 2, 4]   (last: the token within four)
+ *   k_params, v_params  bfloat16 [pages, heads, page_size, 2]: scale, least value
+ * all contiguous and 16-byte aligned.  A row x is held as least = bf16(min x),
+ * scale = bf16((max x - min x) / 15), code = clamp(rint((x - least) / scale), 0,
+ * 15), and stands for scale * code + least; a row that holds NaN, an infinity
+ * or a least value that bfloat16 cannot hold stands for NaN.
+ * Slot = page * page_size + token within the page; negative: none. */
+
+/* Quantises k, v [tokens, heads, d] (strides {k_t, k_h, v_t, v_h}) into their
+ * slots [tokens]; each slot at most once per call. */
+int sa_kv4_append(void* k_codes, void* k_params, void* v_codes, void* v_params, int64_t pages, int heads,
+                  int page_size, int d, const void* k, const void* v, const int64_t* strides, const int32_t* slots,
+                  int64_t tokens, int dtype, void* stream);
+
+/* The values that the slots hold, k, v [tokens, heads, d] contiguous; zeros
+ * for a negative slot. */
+int sa_kv4_read(const void* k_codes, const void* k_params, const void* v_codes, const void* v_params, int64_t pages,
+                int heads, int page_size, int d, void* k, void* v, const int32_t* slots, int64_t tokens, int dtype,
+                void* stream);
+
+/* Attention of each request's n newest tokens over the cache: q [requests, n,
+ * heads, d] (strides {q_r, q_n, q_h}), out contiguous; request r holds
+ * lengths[r] tokens (the new ones among them) in pages tables[r, 0..] (width
+ * entries a row), query i stands at lengths[r] - n + i, visible as in
+ * sa_window_attention.  Tokens behind a bad page id count as hidden. */
+int sa_kv4_attend(const void* k_codes, const void* k_params, const void* v_codes, const void* v_params, int64_t pages,
+                  int kv_heads, int page_size, int d, const void* q, void* out, const int64_t* strides,
+                  const int32_t* tables, const int32_t* lengths, int requests, int n, int heads, int width,
+                  int64_t window, int64_t sinks, float scale, int dtype, void* stream);
+
+/* Room for fresh[r] (>= 0) new tokens of each of `requests` requests (at most
+ * 16384): pages are taken in request order from the end of the free_count[0]
+ * entries of free_pages and entered in tables [requests, width] (in place;
+ * entries of pages held before stay).  lengths_out = lengths + fresh; offsets
+ * [requests + 1] is the running sum of fresh; positions / slots [max_tokens]
+ * give each packed new token's position in its request and its slot, -1 behind
+ * the last token and where there is no page (per_request > 0: token i of
+ * request r stands at r * per_request + i instead, max_tokens is requests *
+ * per_request, and -1 fills the rows of requests with fewer new tokens); free_out[0] is what is left.
+ * Page ids are below free_size.  No output overlaps an input. */
+int sa_plan_kv_pages(const int32_t* lengths, const int32_t* fresh, int32_t* tables, const int32_t* free_pages,
+                     const int32_t* free_count, int requests, int width, int free_size, int page_size, int max_tokens,
+                     int per_request, int32_t* lengths_out, int32_t* offsets, int32_t* positions, int32_t* slots, int32_t* free_out,
+                     void* stream);
+
+/* Returns the pages of the requests with drop[r] != 0 to the free list and
+ * empties those requests (all in place). */
+int sa_release_kv_pages(int32_t* lengths, int32_t* tables, const uint8_t* drop, int32_t* free_pages,
+                        int32_t* free_count, int requests, int width, int free_size, int page_size, void* stream);
+
+/* Root-mean-square norm of each head's row and its rotation by the token's
+ * position, one pass: y = x / sqrt(mean(x^2) + eps) * weight (NULL: ones);
+ * (y_a, y_b) -> (y_a cos - y_b sin, y_b cos + y_a sin) with angle
+ * positions[t] * frequencies[i] (float64 [half]) and (a, b) = (i, i + half) or,
+ * interleaved, (2 i, 2 i + 1).  q [tokens, heads, d], k [tokens, kv_heads, d];
+ * strides = {q_t, q_h, k_t, k_h, qo_t, qo_h, ko_t, ko_h}; out may be the input
+ * itself.  A token of negative position is left out: its output rows are zeroed
+ * (zero_skipped != 0) or stay as they were.  d <= 256. */
+int sa_qk_norm_rotary(const void* q, const void* k, void* q_out, void* k_out, const int32_t* positions,
+                      const void* q_weight, const void* k_weight, const double* frequencies, const int64_t* strides,
+                      int64_t tokens, int heads, int kv_heads, int d, int half, float eps, int interleaved,
+                      int zero_skipped, int dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -71,6 +71,17 @@ SIGNATURES = {
     "sa_flash_causal_attention": [_vp, _vp, _vp, _i64, _i64, _i32, _i32, _f32, _vp, _vp, _sz, _vp],
     "sa_article_segment_mean": [_vp, _vp, _vp, _i64, _i64, _i32, _i32, _i32, _i32, _i32, _f32, _i32, _i32, _f32,
                                 _vp, _vp, _sz, _vp],
+    "sa_serving_status": [_vp],
+    "sa_window_attention": [_vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i64, _i64, _i32, _i32, _i64, _i64, _f32, _i32,
+                            _vp, _vp, _vp],
+    "sa_kv4_append": [_vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _i64, _i32, _vp],
+    "sa_kv4_read": [_vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _vp, _vp, _vp, _i64, _i32, _vp],
+    "sa_kv4_attend": [_vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32,
+                      _i64, _i64, _f32, _i32, _vp],
+    "sa_plan_kv_pages": [_vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _vp],
+    "sa_release_kv_pages": [_vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _vp],
+    "sa_qk_norm_rotary": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _f32, _i32, _i32,
+                          _i32, _vp],
     "sa_stream_query": [_vp, _i32, _i32, _i32, _f32, _vp, _vp, _vp, _vp, _i64, _vp, _vp, _vp, _i64, _f32, _vp, _vp,
                         _vp, _sz, _vp],
 }

@@ -1,0 +1,101 @@
+"""What the serving entry points share: argument checks, strides, the launch
+and the device's error word."""
+
+from __future__ import annotations
+
+import ctypes
+from typing import Optional, Tuple
+
+import torch
+
+from . import _lib
+from . import fast as _fast
+
+Tensor = torch.Tensor
+
+DTYPES = {torch.float32: _lib.REP_DTYPES["float32"], torch.float16: _lib.REP_DTYPES["float16"],
+          torch.bfloat16: _lib.REP_DTYPES["bfloat16"]}
+MAX_DIM = 256
+
+
+def dtype_code(*ts: Tensor) -> int:
+    """The SA_REP_* code of the tensors' one element type."""
+    dt = ts[0].dtype
+    if dt not in DTYPES:
+        raise ValueError(f"unsupported dtype {dt}: float32, float16 and bfloat16 are accepted")
+    for t in ts[1:]:
+        if t.dtype != dt:
+            raise ValueError(f"all inputs must have one dtype, got {dt} and {t.dtype}")
+    return DTYPES[dt]
+
+
+def device_of(*ts: Tensor) -> torch.device:
+    """The CUDA device that all tensors are on."""
+    dev = ts[0].device
+    for t in ts:
+        if not t.is_cuda:
+            raise ValueError("the B200 kernels require CUDA tensors")
+        if t.device != dev:
+            raise ValueError("all tensors must be on the same device")
+    return dev
+
+
+def int32(t: Tensor, shape: Tuple[int, ...], what: str) -> Tensor:
+    """Checks a contiguous int32 index tensor of the given shape."""
+    if t.dtype != torch.int32:
+        raise ValueError(f"{what} must be int32, got {t.dtype}")
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{what} must have shape {list(shape)}, got {list(t.shape)}")
+    return t.contiguous()
+
+
+def rows(t: Tensor) -> Tensor:
+    """t, or a copy of it, with a contiguous last dimension."""
+    return t if t.shape[-1] <= 1 or t.stride(-1) == 1 else t.contiguous()
+
+
+def strides(*values: int):
+    return (ctypes.c_int64 * len(values))(*values)
+
+
+def ptr(t: Optional[Tensor]) -> Optional[int]:
+    return None if t is None else t.data_ptr()
+
+
+def check_window(window: Optional[int], sinks: int) -> Tuple[int, int]:
+    """Window (0: without end) and first tokens as the C ABI takes them."""
+    if window is not None and window <= 0:
+        raise ValueError("window must be positive, or None for no end")
+    if sinks < 0:
+        raise ValueError("sinks must be non-negative")
+    return (0 if window is None else int(window)), int(sinks)
+
+
+def launch(dev: torch.device, name: str, *args) -> None:
+    """Calls a serving entry point on the current stream of `dev`."""
+    if dev.index == torch.cuda.current_device():
+        _launch(dev, name, args)
+    else:
+        with torch.cuda.device(dev):
+            _launch(dev, name, args)
+
+
+def _launch(dev: torch.device, name: str, args) -> None:
+    lib = _lib.load()
+    rc = getattr(lib, name)(*args, torch.cuda.current_stream(dev).cuda_stream)
+    if rc:
+        _lib.check(rc, name)
+    if _fast._CHECK_STATUS and not torch.cuda.is_current_stream_capturing():
+        check_serving_status(dev)
+
+
+def check_serving_status(device: Optional[torch.device] = None) -> None:
+    """Raises for what the serving kernels recorded on `device` since the last
+    such call: offsets, slots, page ids or lengths out of range (ValueError; the
+    kernels skip what they point at) or a bounded wait that gave up (SAError).
+    Synchronises the current stream.  With SA_CHECK_STATUS=1 every serving call
+    does this itself."""
+    dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+    with torch.cuda.device(dev):
+        rc = _lib.load().sa_serving_status(torch.cuda.current_stream(dev).cuda_stream)
+    _lib.check(rc, "serving status")

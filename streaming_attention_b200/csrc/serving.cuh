@@ -1,0 +1,147 @@
+// Shared by the serving kernels (windowed attention, the 4-bit cache, page
+// plans, norm + rotation): element types, the visible key ranges of a sliding
+// window with first tokens, and the error word.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "sa_common.cuh"
+
+namespace sa {
+
+// Codes of the error word that name bad contents of device-side index arrays
+// (the kernels skip what they point at); sa_workspace_status reports them as
+// SA_ERR_INVALID_ARG.
+constexpr int kBadFirst = 400, kBadLast = 499;
+constexpr int kBadPage = 400;     // a page id outside the cache
+constexpr int kBadSlot = 401;     // a slot outside the cache
+constexpr int kBadLength = 402;   // a request longer than its row of the page table
+constexpr int kBadOffsets = 403;  // offsets that are not monotone or leave the tensors
+constexpr int kNoPages = 404;     // the list of free pages ran out
+constexpr int kNoRows = 405;      // more new tokens than the outputs hold
+
+__device__ __forceinline__ void report(int* status, int code, long long index) {
+  if (status && atomicCAS(status, 0, code) == 0) *reinterpret_cast<volatile long long*>(status + 2) = index;
+}
+
+// Element types (the SA_REP_* codes).
+template <int DT>
+struct Elem;
+template <>
+struct Elem<SA_REP_FLOAT32> {
+  using T = float;
+};
+template <>
+struct Elem<SA_REP_FLOAT16> {
+  using T = __half;
+};
+template <>
+struct Elem<SA_REP_BFLOAT16> {
+  using T = __nv_bfloat16;
+};
+
+__device__ __forceinline__ float to_f32(float x) { return x; }
+__device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <typename T>
+__device__ __forceinline__ T from_f32(float x);
+template <>
+__device__ __forceinline__ float from_f32<float>(float x) {
+  return x;
+}
+template <>
+__device__ __forceinline__ __half from_f32<__half>(float x) {
+  return __float2half_rn(x);
+}
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) {
+  return __float2bfloat16_rn(x);
+}
+
+__host__ inline int elem_size(int dtype) { return dtype == SA_REP_FLOAT32 ? 4 : 2; }
+
+// What the window kernels take.  Strides are in elements.  Dense: request b's
+// rows start at b * *_b.  Packed (cu_q != nullptr): *_b is 0, n and m are the
+// tensors' row counts and request b's rows are cu_q[b] .. cu_q[b + 1].
+struct WindowArgs {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* out;
+  int64_t q_b, q_h, q_n, k_b, k_h, k_n, v_b, v_h, v_n, o_b, o_h, o_n;
+  int batch, heads, kv_heads;
+  int64_t n, m;
+  int d, dv;
+  int64_t window;   // keys p - window + 1 .. p of the query at position p
+  int64_t sinks;    // and keys 0 .. sinks - 1
+  float scale;
+  int dtype;
+  const int32_t* cu_q;
+  const int32_t* cu_k;
+  int* status;
+};
+
+// One request of a (dense or packed) batch: first rows and row counts.
+struct Request {
+  int64_t q0, k0, n, m;
+};
+
+// Offsets that are out of order or out of range are clamped (and reported).
+__device__ __forceinline__ Request request_of(const WindowArgs& a, int b) {
+  Request r{0, 0, a.n, a.m};
+  if (a.cu_q) {
+    int64_t q0 = a.cu_q[b], q1 = a.cu_q[b + 1], k0 = a.cu_k[b], k1 = a.cu_k[b + 1];
+    if (q0 < 0 || q1 < q0 || q1 > a.n || k0 < 0 || k1 < k0 || k1 > a.m) {
+      report(a.status, kBadOffsets, b);
+      return Request{0, 0, 0, 0};
+    }
+    r = Request{q0, k0, q1 - q0, k1 - k0};
+  }
+  return r;
+}
+
+// Tile t of a batch of query tiles of `rows` rows.  Dense: t = b * tiles + i.
+// Packed: request b owns tiles cu_q[b] / rows + b onwards -- a start that is
+// strictly monotone in b and leaves room for its ceil(n_b / rows) tiles, so a
+// binary search over cu_q finds the request and the grid needs no request's
+// length: n / rows + batch tiles in all.
+__device__ __forceinline__ int tile_request(const WindowArgs& a, int64_t t, int rows, int64_t* tile) {
+  if (!a.cu_q) {
+    const int64_t per = (a.n + rows - 1) / rows;
+    *tile = t % per;
+    return (int)(t / per);
+  }
+  int lo = 0, hi = a.batch - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if ((int64_t)max(a.cu_q[mid], 0) / rows + mid <= t)
+      lo = mid;
+    else
+      hi = mid - 1;
+  }
+  *tile = t - ((int64_t)max(a.cu_q[lo], 0) / rows + lo);
+  return lo;
+}
+__host__ inline int64_t tile_count(const WindowArgs& a, int rows) {
+  return a.cu_q ? a.n / rows + a.batch : ceil_div(a.n, rows) * a.batch;
+}
+
+// The keys that any of the queries at positions p0 .. p1 sees, as two ranges:
+// first tokens [0, first) and window [begin, end); first <= begin.
+struct KeyRanges {
+  int64_t first, begin, end;
+};
+__host__ __device__ inline KeyRanges key_ranges(int64_t p0, int64_t p1, int64_t m, int64_t window, int64_t sinks) {
+  KeyRanges r;
+  r.end = p1 + 1 < m ? p1 + 1 : m;
+  if (r.end < 0) r.end = 0;
+  r.begin = p0 - window + 1 > 0 ? p0 - window + 1 : 0;
+  if (r.begin > r.end) r.begin = r.end;
+  r.first = sinks < r.begin ? sinks : r.begin;
+  return r;
+}
+
+int launch_window_simt(const WindowArgs& a, cudaStream_t s);
+
+}  // namespace sa
