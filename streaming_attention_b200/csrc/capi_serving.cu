@@ -3,6 +3,7 @@
 // checked here; the contents of device-side index arrays (offsets, slots, page
 // tables, lengths) are checked in the kernels, which skip what is out of range
 // and record it in the error word of sa_serving_status.
+#include <stdlib.h>
 #include <string.h>
 
 #include "kv4.cuh"
@@ -127,6 +128,8 @@ int sa_window_attention(const void* q, const void* k, const void* v, void* out, 
                      strides[4], strides[5], strides[6], strides[7], strides[8], strides[9], strides[10], strides[11],
                      batch,      heads,      kv_heads,   n,          m,          d,          dv,
                      window > 0 ? window : (int64_t)1 << 40, sinks, scale, dtype, cu_q, cu_k, status_word()};
+  const char* simt = getenv("SA_FORCE_SIMT");
+  if (window_tc_takes(a) && !(simt && simt[0] == '1')) return launch_window_tc(a, (cudaStream_t)stream);
   return launch_window_simt(a, (cudaStream_t)stream);
 }
 

@@ -143,5 +143,7 @@ __host__ __device__ inline KeyRanges key_ranges(int64_t p0, int64_t p1, int64_t 
 }
 
 int launch_window_simt(const WindowArgs& a, cudaStream_t s);
+bool window_tc_takes(const WindowArgs& a);
+int launch_window_tc(const WindowArgs& a, cudaStream_t s);
 
 }  // namespace sa

@@ -42,6 +42,19 @@ def _check_heads(heads: int, kv_heads: int) -> None:
         raise ValueError(f"the query heads ({heads}) must be a multiple of the key heads ({kv_heads})")
 
 
+def _on_borders(t: Tensor) -> Tensor:
+    """t, or a copy of it, as the kernels read it: a contiguous last dimension
+    and, for 16-bit types of widths the tensor cores take, rows that start on
+    16-byte borders (TMA) and are no repeats of one another."""
+    d = t.shape[-1]
+    t = S.rows(t)
+    if t.dtype == torch.float32 or d > 128 or (t.data_ptr() % 16 == 0 and all(
+            n <= 1 or (st > 0 and st % 8 == 0) for n, st in zip(t.shape[:-1], t.stride()[:-1]))):
+        return t
+    wide = torch.empty(t.shape[:-1] + ((d + 7) // 8 * 8,), device=t.device, dtype=t.dtype)[..., :d]
+    return wide.copy_(t)
+
+
 @torch.no_grad()
 def sliding_window_attention(q: Tensor, k: Tensor, v: Tensor, *, window: Optional[int], sinks: int = 0,
                              scale: Optional[float] = None) -> Tensor:
@@ -70,7 +83,7 @@ def sliding_window_attention(q: Tensor, k: Tensor, v: Tensor, *, window: Optiona
     out = torch.empty((b, heads, n, dv), device=dev, dtype=q.dtype)
     if out.numel():
         _check_heads(heads, kv_heads)
-        q, k, v = S.rows(q), S.rows(k), S.rows(v)
+        q, k, v = _on_borders(q), _on_borders(k), _on_borders(v)
         S.launch(dev, "sa_window_attention", q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
                  S.strides(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *out.stride()[:3]), b, heads, kv_heads,
                  n, m, d, dv, w, s, _scale(scale, d), code, None, None)
@@ -107,7 +120,7 @@ def sliding_window_attention_packed(q: Tensor, k: Tensor, v: Tensor, cu_q: Tenso
         raise ValueError(f"out must be [{t},{heads},{dv}] like q, its last dimension contiguous")
     if out.numel():
         _check_heads(heads, kv_heads)
-        q, k, v = S.rows(q), S.rows(k), S.rows(v)
+        q, k, v = _on_borders(q), _on_borders(k), _on_borders(v)
         S.launch(dev, "sa_window_attention", q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
                  S.strides(0, q.stride(1), q.stride(0), 0, k.stride(1), k.stride(0), 0, v.stride(1), v.stride(0), 0,
                            out.stride(1), out.stride(0)), cu_q.shape[0] - 1, heads, kv_heads, t, rows, d, dv, w, s,

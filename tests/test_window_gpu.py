@@ -178,18 +178,23 @@ def test_window_packed_equals_dense(dev):
 @pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
 @pytest.mark.parametrize("d", [64, 128])
 def test_window_hidden_keys_do_not_matter(dtype, bad, d, dev):
-    """NaN and infinities in keys and values that a query does not see."""
+    """NaN and infinities in keys and values that a query does not see: its result
+    stays within the roundings of the definition over what it sees (the rows that
+    share a tile with such a value are computed in another way, without rounded
+    probabilities, so they need not be the same bits)."""
     g = R.rng(12)
     n, window, sinks = 260, 50, 2
     q, k, v = (_make((1, 2, n, d), dtype, g).to(dev) for _ in range(3))
-    clean = sa.sliding_window_attention(q, k, v, window=window, sinks=sinks)
     k2, v2 = k.clone(), v.clone()
     k2[:, :, 100] = bad          # seen by the queries 100 .. 149 alone
     v2[:, :, 100] = bad
     got = sa.sliding_window_attention(q, k2, v2, window=window, sinks=sinks)
-    keep = torch.ones(n, dtype=torch.bool, device=dev)
+    keep = torch.ones(n, dtype=torch.bool)
     keep[100:150] = False
-    assert torch.equal(got[:, :, keep], clean[:, :, keep])
+    ref, spread, score = R.attention(*(x[0].cpu().double() for x in (q, k, v)), R.visible(n, n, window, sinks), d ** -0.5)
+    bound = R.attention_bound(ref, spread, score, d, window + sinks, dtype, _p_half(dtype))
+    R.assert_close(got[0][:, keep.to(dev)], ref[:, keep], bound[:, keep])
+    assert not torch.isfinite(got[:, :, 100:150]).any()
 
 
 @pytest.mark.parametrize("dtype", [F32, F16, BF16], ids=["f32", "f16", "bf16"])
