@@ -108,9 +108,9 @@ __device__ __forceinline__ Request request_of(const WindowArgs& a, int b) {
 // length: n / rows + batch tiles in all.
 __device__ __forceinline__ int tile_request(const WindowArgs& a, int64_t t, int rows, int64_t* tile) {
   if (!a.cu_q) {
-    const int64_t per = (a.n + rows - 1) / rows;
-    *tile = t % per;
-    return (int)(t / per);
+    const uint32_t per = (uint32_t)((a.n + rows - 1) / rows), u = (uint32_t)t;   // the grid has less than 2^31 tiles
+    *tile = u % per;
+    return (int)(u / per);
   }
   int lo = 0, hi = a.batch - 1;
   while (lo < hi) {

@@ -93,6 +93,32 @@ __device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, c
   return __all_sync(0xffffffffu, r);
 }
 
+// mbar_wait for a whole converged warp that reads the clock only after 256
+// tries: a try suspends the warp by itself for a while, and %globaltimer is slow
+// to read, which a wait that is merely not over yet should not pay for.
+__device__ __forceinline__ bool mbar_wait_warp_lazy(uint64_t* bar, uint32_t parity, const Abort& ab, int code) {
+  bool r = false;
+  uint64_t t0 = 0;
+  for (uint32_t it = 1;; ++it) {
+    if (mbar_try_wait(bar, parity)) {
+      r = true;
+      break;
+    }
+    if ((it & 255) == 0) {
+      if (*ab.cta) break;
+      const uint64_t now = globaltimer_ns();
+      if (t0 == 0) {
+        t0 = now;
+      } else if (now - t0 > ab.limit_ns) {
+        *ab.cta = 1;
+        if (ab.global_status) atomicCAS(ab.global_status, 0, code);
+        break;
+      }
+    }
+  }
+  return __all_sync(0xffffffffu, r);
+}
+
 // ---------------------------------------------------------------------------
 // TMA (no multicast anywhere in this library)
 // ---------------------------------------------------------------------------

@@ -18,8 +18,12 @@
 // with sk = first (the filling columns lie below every row's window), or, where
 // window and first tokens touch, F = begin = 0 and sk = sinks.
 //
-// Warps: 0 loads (TMA), 1 issues the products (converged, one elected lane),
-// 2..5 and 6..9 are the softmax of query tile 0 and 1, one row per thread.
+// One CTA per SM works through query tile pairs (persistent: a pair's set-up,
+// first loads and stores run under its neighbours' products; as one CTA per pair
+// they took 40 % of the time).  Warps: 0 plans the pairs and loads (TMA), 1
+// issues the products (converged, one elected lane), 2..5 and 6..9 are the
+// softmax of query tile 0 and 1, one row per thread, 64 of its 128 scores in
+// registers at a time.
 // TMEM: S0 S1 O0 O1 of 128 columns each; P, in 16 bits, overwrites the first
 // half of its S.  The issue order per key tile is PV0 S0' PV1 S1', so that one
 // tile's softmax runs under the other's products; the commit of S(j + 1) also
@@ -53,13 +57,16 @@ constexpr int kSeam = 16;      // rows of a box of the seam tile
 constexpr int kThreads = 320;
 constexpr float kMove = 8.0f;
 
-constexpr int kErrQ = 501, kErrFull = 502, kErrP = 503, kErrS = 504, kErrEmpty = 505, kErrO = 506, kErrDrain = 507;
+constexpr int kErrQ = 501, kErrFull = 502, kErrP = 503, kErrS = 504, kErrEmpty = 505, kErrO = 506, kErrDrain = 507,
+              kErrPlan = 508;
 
 struct WindowTcParams {
   WindowArgs a;
   int group, pack, blocks;   // query heads per key head, heads per tile, tiles of heads per key head
+  int pack_log;              // pack = 1 << pack_log
   int rows_per_cta;          // queries of a CTA (2 * kRows / pack)
   int vec_out;               // out rows take 16-byte stores
+  uint32_t tiles, items;     // query tile pairs of one tile of heads, and of all
   uint64_t wait_ns;
 };
 
@@ -87,10 +94,66 @@ __device__ __forceinline__ Columns columns_of(int64_t p0, int64_t p1, int64_t m,
   return c;
 }
 
+// A query tile pair, in shared memory: each role reads what it needs, so that
+// nothing of it takes registers (or, worse, local memory) where it is not used.
+struct PairPlan {
+  int live;        // 0: no queries (skipped), -1: no pairs are left
+  int b, hk, g0;   // request, key head, first query head of the tile within the group
+  int q_row, nq;   // first query's row in q, queries
+  int k_row, m;    // first key's row in k, keys of the request
+  int p0;          // position of the first query
+  int tiles, total, fill, sk;
+  int base;        // column V >= fill is row base + V of k
+  int hi;          // hi of the first query; query i's is hi + i
+  int lo[2], last[2];   // columns that query tile t needs: lo[t] (or below sk) .. last[t]
+};
+
+__device__ __forceinline__ PairPlan plan_pair(const WindowTcParams& p, uint32_t item) {
+  const WindowArgs& a = p.a;
+  PairPlan c;
+  const uint32_t y = item / p.tiles;
+  int64_t tile;
+  c.b = tile_request(a, item - y * p.tiles, p.rows_per_cta, &tile);
+  const Request rq = request_of(a, c.b);
+  const int64_t i0 = tile * p.rows_per_cta;
+  c.live = tile >= 0 && i0 < rq.n;
+  c.hk = y / p.blocks;
+  c.g0 = (y % p.blocks) * p.pack;
+  c.q_row = (int)(rq.q0 + i0);
+  c.nq = (int)min((int64_t)p.rows_per_cta, rq.n - i0);
+  c.k_row = (int)rq.k0;
+  c.m = (int)rq.m;
+  const int64_t p0 = rq.m - rq.n + i0;
+  c.p0 = (int)p0;
+  const Columns cols = columns_of(p0, p0 + c.nq - 1, rq.m, a.window, a.sinks);
+  c.tiles = (cols.total + kCols - 1) / kCols;
+  c.total = cols.total;
+  c.fill = cols.fill;
+  c.sk = cols.sk;
+  c.base = (int)(rq.k0 + cols.begin) - cols.fill;
+  c.hi = (int)(p0 - cols.begin) + cols.fill;
+  const int tq = kRows >> p.pack_log, window = (int)min(a.window, (int64_t)1 << 30);
+  c.last[0] = c.hi + min(tq, c.nq) - 1;
+  c.last[1] = c.nq > tq ? c.hi + c.nq - 1 : -1;
+  c.lo[0] = c.hi - window + 1;
+  c.lo[1] = c.lo[0] + tq;
+  return c;
+}
+
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// Ties 32 loaded registers to this point of the program: what follows uses them
+// after the wait that stands before.
+__device__ __forceinline__ void tie32(float (&v)[32]) {
+  asm volatile("" : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]),
+               "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15]));
+  asm volatile("" : "+f"(v[16]), "+f"(v[17]), "+f"(v[18]), "+f"(v[19]), "+f"(v[20]), "+f"(v[21]), "+f"(v[22]),
+               "+f"(v[23]), "+f"(v[24]), "+f"(v[25]), "+f"(v[26]), "+f"(v[27]), "+f"(v[28]), "+f"(v[29]), "+f"(v[30]),
+               "+f"(v[31]));
 }
 
 __device__ __forceinline__ uint64_t pack2(float a, float b) {
@@ -112,6 +175,40 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   return r;
 }
 
+// 2^x of two values on the FMA and integer pipes: x = n + f with n whole and
+// |f| <= 1/2, 2^f as a polynomial of least relative error on that interval
+// (a reweighted least-squares fit: degree 3 is 7.5e-5 off, a fiftieth of
+// bfloat16's half step; degree 4 2.7e-6, a hundredth and less of float16's),
+// n added to the exponent.  Below 2^-125 the result stays at 2^-125.
+template <int DT>
+__device__ __forceinline__ void exp2_poly(uint64_t x2, float& a, float& b) {
+  float x, y;
+  unpack2(x2, x, y);
+  // a NaN stays one (as the largest float at the end: its products are not finite either)
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x) : "f"(-125.0f));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(y) : "f"(-125.0f));
+  x2 = pack2(x, y);
+  const uint64_t magic = pack2(12582912.0f, 12582912.0f), unmagic = pack2(-12582912.0f, -12582912.0f);
+  const uint64_t t = add2(x2, magic);
+  const uint64_t f = fma2(add2(t, unmagic), pack2(-1.0f, -1.0f), x2);
+  uint64_t r;
+  if (DT == SA_REP_BFLOAT16) {
+    r = fma2(pack2(0.0551716610789299f, 0.0551716610789299f), f, pack2(0.2426111251115799f, 0.2426111251115799f));
+    r = fma2(r, f, pack2(0.6932609677314758f, 0.6932609677314758f));
+    r = fma2(r, f, pack2(0.9999280571937561f, 0.9999280571937561f));
+  } else {
+    r = fma2(pack2(0.009570101276040077f, 0.009570101276040077f), f, pack2(0.05591785907745361f, 0.05591785907745361f));
+    r = fma2(r, f, pack2(0.240247443318367f, 0.240247443318367f));
+    r = fma2(r, f, pack2(0.6931217908859253f, 0.6931217908859253f));
+    r = fma2(r, f, pack2(0.9999992847442627f, 0.9999992847442627f));
+  }
+  float tx, ty;
+  unpack2(t, tx, ty);
+  unpack2(r, x, y);
+  a = __uint_as_float(__float_as_uint(x) + (__float_as_uint(tx) << 23));
+  b = __uint_as_float(__float_as_uint(y) + (__float_as_uint(ty) << 23));
+}
+
 // Two floats as 16-bit values, the first in the low half.
 template <int DT>
 __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
@@ -123,9 +220,76 @@ __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
   return r;
 }
 
+// Which pairs of a chunk's 16 take the polynomial: 4, so that the special
+// function unit (16 a clock) and the FMA pipe finish together.
+__host__ __device__ constexpr bool poly_pair(int e) { return e % 4 == 1; }
+
 // The x lowest bits set (x may be anything).
 __device__ __forceinline__ uint32_t low_bits(int x) {
   return x >= 32 ? 0xffffffffu : (x <= 0 ? 0u : (1u << x) - 1u);
+}
+
+// Hidden scores (bit 0) become -inf.
+__device__ __forceinline__ void hide(float (&s)[32], uint32_t on) {
+#pragma unroll
+  for (int e = 0; e < 32; ++e) s[e] = (on >> e) & 1u ? s[e] : -INFINITY;
+}
+
+__device__ __forceinline__ float max32(const float (&s)[32]) {
+  float t[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+  for (int e = 4; e < 32; ++e) t[e & 3] = fmaxf(t[e & 3], s[e]);
+  return fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
+}
+
+// P of a chunk: 2^(s c2 + off), summed and, in 16 bits, stored to TMEM.  Hidden
+// scores (-inf) need the exact zero of ex2.
+template <int DT>
+__device__ __forceinline__ void exp_chunk(float (&s)[32], bool all_on, uint64_t c22, uint64_t off2, uint64_t (&sum2)[2],
+                                          uint32_t to) {
+  uint32_t pk[16];
+  if (all_on) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const uint64_t z = fma2(pack2(s[2 * e], s[2 * e + 1]), c22, off2);
+      float x, y;
+      if (poly_pair(e)) {
+        exp2_poly<DT>(z, x, y);
+      } else {
+        unpack2(z, x, y);
+        x = ex2(x);
+        y = ex2(y);
+      }
+      sum2[e & 1] = add2(sum2[e & 1], pack2(x, y));
+      pk[e] = pack16<DT>(x, y);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      float x, y;
+      unpack2(fma2(pack2(s[2 * e], s[2 * e + 1]), c22, off2), x, y);
+      x = ex2(x);
+      y = ex2(y);
+      sum2[e & 1] = add2(sum2[e & 1], pack2(x, y));
+      pk[e] = pack16<DT>(x, y);
+    }
+  }
+  tmem_st16(to, pk);
+}
+
+// O of a row times alpha, in TMEM (rare: kept out of the way of the tile loop's code).
+__device__ __noinline__ void scale_row(uint32_t to, int dv, float alpha) {
+#pragma unroll 1
+  for (int c = 0; c < dv; c += 16) {
+    float o[16];
+    tmem_ld16(to + c, o);
+    tmem_wait_ld();
+    uint32_t os[16];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) os[e] = __float_as_uint(o[e] * alpha);
+    tmem_st16(to + c, os);
+  }
+  tmem_wait_st();
 }
 
 // One output row from its visible keys alone, in float32 by one thread.
@@ -170,18 +334,21 @@ template <int DC, int VC>   // 64-column chunks of the head widths
 struct Layout {
   static constexpr uint32_t kQ = DC * kRows * 128;                              // one query tile
   static constexpr uint32_t kSlot = (DC > VC ? DC : VC) * kCols * 128;          // one K or V tile
-  static constexpr int kSlots = DC == 2 || VC == 2 ? 5 : 8;
+  static constexpr int kSlots = DC == 2 || VC == 2 ? 4 : 8;
   static constexpr uint32_t kRing = 2 * kQ;
-  static constexpr uint32_t kBars = kRing + kSlots * kSlot;
-  static constexpr uint32_t kBytes = kBars + (2 * kSlots + 8) * 8 + 16 + 1024;
+  static constexpr uint32_t kPitch = 80;                                        // a row's 32 columns, staged
+  static constexpr uint32_t kStage = kRing + kSlots * kSlot;
+  static constexpr uint32_t kBars = kStage + 8 * 32 * kPitch;
+  static constexpr uint32_t kBytes = kBars + (2 * kSlots + 16) * 8 + 16 + 2 * sizeof(PairPlan) + 1024;
   static_assert(kBytes <= 227 * 1024, "shared memory");
 };
 
 template <int DT, int DC, int VC>
 __global__ void __launch_bounds__(kThreads, 1)
 window_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
-                 const __grid_constant__ CUtensorMap tm_ks, const __grid_constant__ CUtensorMap tm_v,
-                 const __grid_constant__ CUtensorMap tm_vs, const __grid_constant__ WindowTcParams p) {
+                 const __grid_constant__ CUtensorMap tm_ks, const __grid_constant__ CUtensorMap tm_kw,
+                 const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_vs,
+                 const __grid_constant__ CUtensorMap tm_vw, const __grid_constant__ WindowTcParams p) {
   using L = Layout<DC, VC>;
   using T = typename Elem<DT>::T;
   constexpr int kSlots = L::kSlots;
@@ -191,40 +358,20 @@ window_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::kBars);
   uint64_t* empty = full + kSlots;
   uint64_t* sfull = empty + kSlots;   // [2]
-  uint64_t* pfull = sfull + 2;        // [2]
-  uint64_t* qfull = pfull + 2;
-  uint64_t* ofull = qfull + 1;
-  uint64_t* drain = ofull + 1;
+  uint64_t* pfull = sfull + 2;        // [2 query tiles][2 halves of the key tile]
+  uint64_t* ofull = pfull + 4;        // [2]
+  uint64_t* qfull = ofull + 2;
+  uint64_t* qempty = qfull + 1;
+  uint64_t* plan_full = qempty + 1;   // [2]
+  uint64_t* plan_empty = plan_full + 2;   // [2]
+  uint64_t* drain = plan_empty + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   int* abort_word = reinterpret_cast<int*>(tmem_slot + 1);
+  PairPlan* plans = reinterpret_cast<PairPlan*>(tmem_slot + 4);   // [2]
 
   const WindowArgs& a = p.a;
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
-  int64_t tile;
-  const int b = tile_request(a, blockIdx.x, p.rows_per_cta, &tile);
-  const Request rq = request_of(a, b);
-  const int64_t i0 = tile * p.rows_per_cta;
-  if (tile < 0 || i0 >= rq.n) return;
-  const int hk = blockIdx.y / p.blocks, g0 = (blockIdx.y % p.blocks) * p.pack;
-  const int tq = kRows / p.pack;                               // queries of a tile
-  const int nq = (int)min((int64_t)p.rows_per_cta, rq.n - i0);
-  const int64_t p0 = rq.m - rq.n + i0;
-  const Columns cols = columns_of(p0, p0 + nq - 1, rq.m, a.window, a.sinks);
-  const int tiles = (cols.total + kCols - 1) / kCols;
-  const int window = (int)min(a.window, (int64_t)1 << 30);
-  // the columns that query tile t needs: below hi_t, and from lo_t on or below sk
-  const int hi0 = (int)(p0 + min(tq, nq) - 1 - cols.begin) + cols.fill;
-  const int hi1 = nq > tq ? (int)(p0 + nq - 1 - cols.begin) + cols.fill : -1;
-  const int lo0 = (int)(p0 - cols.begin) + cols.fill - window + 1;
-  const int lo1 = lo0 + tq;
-  auto needed = [&](int t, int j) {
-    const int v0 = j * kCols;
-    return v0 <= (t ? hi1 : hi0) && (v0 + kCols > (t ? lo1 : lo0) || v0 < cols.sk);
-  };
-  // columns of tile j that a product takes: a multiple of 32
-  auto width = [&](int j) { return min(kCols, (cols.total - j * kCols + 31) & ~31); };
-
   if (threadIdx.x == 0) {
     for (int s = 0; s < kSlots; ++s) {
       mbar_init(&full[s], 1);
@@ -232,13 +379,18 @@ window_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
     }
     for (int t = 0; t < 2; ++t) {
       mbar_init(&sfull[t], 1);
-      mbar_init(&pfull[t], 4);
+      mbar_init(&pfull[2 * t], 4);
+      mbar_init(&pfull[2 * t + 1], 4);
+      mbar_init(&ofull[t], 1);
+      mbar_init(&plan_full[t], 1);
+      mbar_init(&plan_empty[t], 9);   // the issuer and eight softmax warps
     }
     mbar_init(qfull, 1);
-    mbar_init(ofull, 1);
+    mbar_init(qempty, 1);
     mbar_init(drain, 1);
     *abort_word = 0;
     fence_mbar_init();
+    fence_proxy_async_smem();
   }
   if (warp == 1) {
     tmem_alloc(tmem_slot, 512);
@@ -252,40 +404,66 @@ window_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
   const uint32_t tS[2] = {tmem, tmem + 128}, tO[2] = {tmem + 256, tmem + 384};
 
   if (warp == 0) {
-    // ------------------------------------------------------------ loads
-    if (lane == 0 && tiles > 0) {
-      const int qb = a.cu_q ? 0 : b;
-      mbar_arrive_expect_tx(qfull, 2 * L::kQ);
-      for (int t = 0; t < 2; ++t)
-        for (int c = 0; c < DC; ++c)
-          tma_load_5d(smem + t * L::kQ + c * (kRows * 128), &tm_q, qfull, c * 64, g0, (int)(rq.q0 + i0) + t * tq, hk, qb);
-      int issued = 0;
-      for (int u = 0; u < 2 * tiles; ++u) {   // K of a tile, then its V
-        const int s = u % kSlots, j = u >> 1;
-        if (u >= kSlots && !mbar_wait(&empty[s], ((u / kSlots) - 1) & 1, ab, kErrEmpty)) break;
-        const bool isv = u & 1;
-        const int chunks = isv ? VC : DC;
-        uint8_t* dst = smem + L::kRing + s * L::kSlot;
-        mbar_arrive_expect_tx(&full[s], chunks * kCols * 128);
-        const int v0 = j * kCols;
-        if (v0 >= cols.fill) {
-          const int row = (int)(rq.k0 + cols.begin) + v0 - cols.fill;
-          for (int c = 0; c < chunks; ++c)
-            tma_load_4d(dst + c * (kCols * 128), isv ? &tm_v : &tm_k, &full[s], c * 64, row, hk, qb);
+    // ------------------------------------------------------------ plans and loads
+    if (lane == 0) {
+      int u = 0, pairs = 0;   // ring loads and pairs so far
+      bool ok = true;
+#pragma unroll 1
+      for (uint32_t item = blockIdx.x; ok; item += gridDim.x) {
+        PairPlan c;
+        c.live = -1;
+        if (item < p.items) c = plan_pair(p, item);
+        if (c.live == 0) continue;
+        const int ps = pairs & 1;
+        if (pairs >= 2 && !mbar_wait(&plan_empty[ps], ((pairs >> 1) - 1) & 1, ab, kErrPlan)) break;
+        plans[ps] = c;
+        mbar_arrive(&plan_full[ps]);
+        if (c.live < 0) break;
+        if (pairs >= 1 && !mbar_wait(qempty, (pairs - 1) & 1, ab, kErrEmpty)) break;
+        ++pairs;
+        const int kb = a.cu_q ? 0 : c.b, tq = kRows >> p.pack_log;
+        if (c.tiles > 0) {
+          mbar_arrive_expect_tx(qfull, 2 * L::kQ);
+          for (int t = 0; t < 2; ++t)
+            for (int j = 0; j < DC; ++j)
+              tma_load_5d(smem + t * L::kQ + j * (kRows * 128), &tm_q, qfull, j * 64, c.g0, c.q_row + t * tq, c.hk, kb);
         } else {
-          for (int r = 0; r < kCols; r += kSeam) {
-            const int v = v0 + r;
-            const int row = (int)rq.k0 + (v < cols.fill ? v : (int)cols.begin + v - cols.fill);
-            for (int c = 0; c < chunks; ++c)
-              tma_load_4d(dst + c * (kCols * 128) + r * 128, isv ? &tm_vs : &tm_ks, &full[s], c * 64, row, hk, qb);
+          mbar_arrive(qfull);
+        }
+#pragma unroll 1
+        for (int i = 0; i < 2 * c.tiles; ++i, ++u) {   // K of a key tile, then its V
+          const int s = u % kSlots, v0 = (i >> 1) * kCols;
+          if (u >= kSlots && !mbar_wait(&empty[s], ((u / kSlots) - 1) & 1, ab, kErrEmpty)) {
+            ok = false;
+            break;
+          }
+          const bool isv = i & 1;
+          const int chunks = isv ? VC : DC;
+          uint8_t* dst = smem + L::kRing + s * L::kSlot;
+          mbar_arrive_expect_tx(&full[s], chunks * kCols * 128);
+#pragma unroll 1
+          for (int j = 0; j < chunks; ++j, dst += kCols * 128) {
+            if (v0 >= c.fill) {
+              tma_load_4d(dst, isv ? &tm_v : &tm_k, &full[s], j * 64, c.base + v0, c.hk, kb);
+            } else if (c.fill == kSeam) {
+              tma_load_4d(dst, isv ? &tm_vs : &tm_ks, &full[s], j * 64, c.k_row, c.hk, kb);
+              tma_load_4d(dst + kSeam * 128, isv ? &tm_vw : &tm_kw, &full[s], j * 64, c.base + kSeam, c.hk, kb);
+            } else {
+#pragma unroll 1
+              for (int r = 0; r < kCols; r += kSeam) {
+                const int v = v0 + r;
+                tma_load_4d(dst + r * 128, isv ? &tm_vs : &tm_ks, &full[s], j * 64, v < c.fill ? c.k_row + v : c.base + v,
+                            c.hk, kb);
+              }
+            }
           }
         }
-        ++issued;
       }
       // never leave with copies in flight
-      for (int u = max(0, issued - kSlots); u <= issued; ++u) {
-        uint64_t* bar = u < issued ? &full[u % kSlots] : qfull;
-        const int parity = u < issued ? (u / kSlots) & 1 : 0;
+      for (int i = max(0, u - kSlots); i <= u; ++i) {
+        if (i == u && pairs == 0) break;
+        uint64_t* bar = i < u ? &full[i % kSlots] : qfull;
+        const int parity = i < u ? (i / kSlots) & 1 : (pairs - 1) & 1;
         const uint64_t t0 = globaltimer_ns();
         while (!mbar_try_wait(bar, parity)) {
           if (globaltimer_ns() - t0 > 1000000000ull) {
@@ -298,35 +476,58 @@ window_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
     __syncwarp();
   } else if (warp == 1) {
     // ------------------------------------------------------------ products
-    if (tiles > 0) {
-      bool ok = mbar_wait_warp(qfull, 0, ab, kErrQ);
-      const int ksteps = (a.d + 15) >> 4;
-      const uint32_t id_pv = idesc_f16(kRows, (a.dv + 15) & ~15, DT == SA_REP_BFLOAT16, false, true);
-      int done[2] = {0, 0};   // products P V issued per query tile
+    const int ksteps = (a.d + 15) >> 4;
+    const uint32_t id_pv = idesc_f16(kRows, (a.dv + 15) & ~15, DT == SA_REP_BFLOAT16, false, true);
+    int u = 0;                                       // ring loads before this pair
+    int count_p[2][2] = {{0, 0}, {0, 0}};            // halves of P waited for
+    bool ok = true;
+#pragma unroll 1
+    for (int pair = 0; ok; ++pair) {
+      ok = mbar_wait_warp_lazy(&plan_full[pair & 1], (pair >> 1) & 1, ab, kErrPlan);
+      if (!ok) break;
+      const PairPlan& c = plans[pair & 1];
+      if (c.live < 0) break;
+      const int tiles = c.tiles, total = c.total, sk = c.sk, lo[2] = {c.lo[0], c.lo[1]}, last[2] = {c.last[0], c.last[1]};
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&plan_empty[pair & 1]);
+      auto needed = [&](int t, int j) { return j * kCols <= last[t] && (j * kCols + kCols > lo[t] || j * kCols < sk); };
+      // columns of tile j that a product takes: a multiple of 32
+      auto width = [&](int j) { return min(kCols, (total - j * kCols + 31) & ~31); };
+      ok = mbar_wait_warp_lazy(qfull, pair & 1, ab, kErrQ);
+      bool begun[2] = {false, false};
+#pragma unroll 1
       for (int j = 0; ok && j <= tiles; ++j) {
-        const int us = 2 * j, uv = 2 * j - 1;   // ring positions of K(j) and V(j - 1)
+        const int us = u + 2 * j, uv = us - 1;   // ring positions of K(j) and V(j - 1)
         bool waited_k = false, waited_v = false;
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
           if (ok && j > 0 && needed(t, j - 1)) {
-            if (!waited_v) ok = mbar_wait_warp(&full[uv % kSlots], (uv / kSlots) & 1, ab, kErrFull);
+            if (!waited_v) ok = mbar_wait_warp_lazy(&full[uv % kSlots], (uv / kSlots) & 1, ab, kErrFull);
             waited_v = true;
-            if (ok) ok = mbar_wait_warp(&pfull[t], done[t] & 1, ab, kErrP);
-            if (ok) {
-              tc_fence_after();
-              const int steps = width(j - 1) >> 4;
-              if (elect_one()) {
-                const uint64_t vd = sdesc_sw128(smem_u32(smem + L::kRing + (uv % kSlots) * L::kSlot), kCols * 128, 1024);
-                for (int kk = 0; kk < steps; ++kk)
-                  mma_f16_ts(tO[t], tS[t] + kk * 8, vd + (uint64_t)((kk * 16 * 128) >> 4), id_pv,
-                             (done[t] > 0 || kk > 0) ? 1u : 0u);
+            const int steps = width(j - 1) >> 4;
+            const uint64_t vd = sdesc_sw128(smem_u32(smem + L::kRing + (uv % kSlots) * L::kSlot), kCols * 128, 1024);
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {   // keys 0..63 of the tile, then the rest
+              if (ok && half * 4 < steps) {
+                ok = mbar_wait_warp_lazy(&pfull[2 * t + half], count_p[t][half] & 1, ab, kErrP);
+                ++count_p[t][half];
+                tc_fence_after();
+                if (ok && elect_one()) {
+                  // unrolled: descriptors that are constants apart stay in uniform registers
+#pragma unroll
+                  for (int kk = half * 4; kk < half * 4 + 4; ++kk)
+                    if (kk < steps)
+                      mma_f16_ts(tO[t], tS[t] + kk * 8, vd + (uint64_t)((kk * 16 * 128) >> 4), id_pv,
+                                 (begun[t] || kk > 0) ? 1u : 0u);
+                  if ((half == 1 || steps <= 4) && j - 1 == last[t] / kCols) mma_commit(&ofull[t]);
+                }
+                __syncwarp();
               }
-              __syncwarp();
-              ++done[t];
             }
+            begun[t] = true;
           }
           if (ok && j < tiles && needed(t, j)) {
-            if (!waited_k) ok = mbar_wait_warp(&full[us % kSlots], (us / kSlots) & 1, ab, kErrFull);
+            if (!waited_k) ok = mbar_wait_warp_lazy(&full[us % kSlots], (us / kSlots) & 1, ab, kErrFull);
             waited_k = true;
             if (ok) {
               tc_fence_after();
@@ -334,9 +535,10 @@ window_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
               if (elect_one()) {
                 const uint64_t qd = sdesc_sw128(smem_u32(smem + t * L::kQ), 16, 1024);
                 const uint64_t kd = sdesc_sw128(smem_u32(smem + L::kRing + (us % kSlots) * L::kSlot), 16, 1024);
-                for (int kk = 0; kk < ksteps; ++kk) {
+#pragma unroll
+                for (int kk = 0; kk < DC * 4; ++kk) {
                   const uint64_t at = (uint64_t)(((kk >> 2) * (kRows * 128) + (kk & 3) * 32) >> 4);
-                  mma_f16_ss(tS[t], qd + at, kd + at, id_s, kk > 0 ? 1u : 0u);
+                  if (kk < ksteps) mma_f16_ss(tS[t], qd + at, kd + at, id_s, kk > 0 ? 1u : 0u);
                 }
                 mma_commit(&sfull[t]);
               }
@@ -347,163 +549,199 @@ window_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
         if (ok && elect_one()) {
           if (j > 0) mma_commit(&empty[uv % kSlots]);
           if (j < tiles) mma_commit(&empty[us % kSlots]);
+          // the queries' last product (or, without keys, nothing) is issued
+          if (j == tiles - 1 || tiles == 0) mma_commit(qempty);
         }
         __syncwarp();
       }
-      if (ok && elect_one()) mma_commit(ofull);
-      if (elect_one()) mma_commit(drain);
-      const uint64_t t0 = globaltimer_ns();
-      while (!mbar_try_wait(drain, 0)) {
-        if (globaltimer_ns() - t0 > 2000000000ull) {
-          if (a.status) atomicCAS(a.status, 0, kErrDrain);
-          break;
-        }
-      }
-      __syncwarp();
+      u += 2 * tiles;
     }
+    if (elect_one()) mma_commit(drain);
+    const uint64_t t0 = globaltimer_ns();
+    while (!mbar_try_wait(drain, 0)) {
+      if (globaltimer_ns() - t0 > 2000000000ull) {
+        if (a.status) atomicCAS(a.status, 0, kErrDrain);
+        break;
+      }
+    }
+    __syncwarp();
   } else {
     // ------------------------------------------------------------ softmax rows
     const int t = (warp - 2) >> 2;
     const int quarter = warp & 3;
     const int row = quarter * 32 + lane;
-    const int qi = t * tq + row / p.pack;                    // query of the CTA
-    const int h = hk * p.group + g0 + (row & (p.pack - 1));
-    const bool valid = qi < nq;
+    const int tq = kRows >> p.pack_log;                      // queries of a tile
+    const int qi = t * tq + (row >> p.pack_log);             // query of the pair
     const uint32_t at = (uint32_t)(quarter * 32) << 16;
-    const int hi = valid ? (int)(p0 + qi - cols.begin) + cols.fill : -1;
-    const int lo = hi - window + 1;
-    const bool flip = a.scale < 0.0f;
-    const float c2 = fabsf(a.scale) * 1.4426950408889634f;
-    float m = -INFINITY, l = 0.0f;
+    const float c2 = a.scale * 1.4426950408889634f;          // log2(e); not negative (window_tc_takes)
+    const uint32_t ts = tS[t] + at;
+    uint8_t* stage = smem + L::kStage + (warp - 2) * 32 * L::kPitch;
+    int count = 0, outs = 0;   // score tiles and outputs so far
     bool ok = true;
-    int done = 0;
-    for (int j = 0; ok && j < tiles; ++j) {
-      if (!needed(t, j)) continue;
-      if (!mbar_wait_warp(&sfull[t], done & 1, ab, kErrS)) {
-        ok = false;
-        break;
-      }
-      tc_fence_after();
-      const int w = width(j), v0 = j * kCols;
-      float s[4][32];
-#pragma unroll
-      for (int c = 0; c < 4; ++c)
-        if (c * 32 < w) tmem_ld32(tS[t] + at + c * 32, s[c]);
-      tmem_wait_ld();
-      if (flip) {
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-#pragma unroll
-          for (int e = 0; e < 32; ++e) s[c][e] = -s[c][e];
-      }
-      const bool all_on = v0 + w - 1 <= hi && (v0 >= lo || v0 + w <= cols.sk);
-      if (!__all_sync(0xffffffffu, all_on)) {
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const int vc = v0 + c * 32;
-          const uint32_t on = low_bits(hi - vc + 1) & (~low_bits(lo - vc) | low_bits(cols.sk - vc));
-#pragma unroll
-          for (int e = 0; e < 32; ++e) s[c][e] = (on >> e) & 1u ? s[c][e] : -INFINITY;
+#pragma unroll 1
+    for (int pair = 0; ok; ++pair) {
+      ok = mbar_wait_warp_lazy(&plan_full[pair & 1], (pair >> 1) & 1, ab, kErrPlan);
+      if (!ok) break;
+      const PairPlan& c = plans[pair & 1];
+      if (c.live < 0) break;
+      // rows behind the last query count as that query: they need no masks of their own
+      const int hi = c.hi + min(qi, c.nq - 1);
+      const int lo = hi - (int)min(a.window, (int64_t)1 << 30) + 1;
+      const int total = c.total, sk = c.sk, tlo = c.lo[t], tlast = c.last[t];
+      float m = -INFINITY, l = 0.0f;
+      int done = 0;
+#pragma unroll 1
+      for (int v0 = 0; v0 <= tlast; v0 += kCols) {
+        if (v0 + kCols <= tlo && v0 >= sk) continue;   // as the issuer's needed()
+        if (!mbar_wait_warp_lazy(&sfull[t], count & 1, ab, kErrS)) {
+          ok = false;
+          break;
         }
-      }
-      float tm[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-      for (int c = 0; c < 4; ++c)
-        if (c * 32 < w) {
-#pragma unroll
-          for (int e = 0; e < 32; ++e) tm[e & 3] = fmaxf(tm[e & 3], s[c][e]);
-        }
-      const float top = fmaxf(fmaxf(tm[0], tm[1]), fmaxf(tm[2], tm[3])) * c2;
-      const bool move = top > m + kMove;
-      if (__any_sync(0xffffffffu, move)) {
-        const float to = move ? top : m;
-        const float alpha = move ? ex2(m - to) : 1.0f;   // m = -inf: 0
-        m = to;
-        l *= alpha;
-        if (done > 0) {   // the products of this row's earlier tiles have ended (sfull)
-#pragma unroll
-          for (int c = 0; c < VC * 2; ++c)
-            if (c * 32 < a.dv) {
-              float o[32];
-              tmem_ld32(tO[t] + at + c * 32, o);
-              tmem_wait_ld();
-              uint32_t os[32];
-#pragma unroll
-              for (int e = 0; e < 32; ++e) os[e] = __float_as_uint(o[e] * alpha);
-              tmem_st32(tO[t] + at + c * 32, os);
-            }
-        }
-      }
-      const float off = kShift - (m == -INFINITY ? 0.0f : m);
-      const uint64_t off2 = pack2(off, off), c22 = pack2(c2, c2);
-      uint64_t sum2[2] = {0, 0};
-#pragma unroll
-      for (int c = 0; c < 4; ++c)
-        if (c * 32 < w) {
-          uint32_t pk[16];
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            float x, y;
-            unpack2(fma2(pack2(s[c][2 * e], s[c][2 * e + 1]), c22, off2), x, y);
-            x = ex2(x);
-            y = ex2(y);
-            sum2[e & 1] = add2(sum2[e & 1], pack2(x, y));
-            pk[e] = pack16<DT>(x, y);
+        ++count;
+        tc_fence_after();
+        // columns of a last, narrower tile that its product left out hold an earlier tile's numbers: hidden like others
+        const int w = min(kCols, (total - v0 + 31) & ~31);
+        // a tile that all rows of the warp see whole needs no mask
+        const bool all_on = __all_sync(0xffffffffu, v0 + kCols - 1 <= hi && (v0 >= lo || v0 + kCols <= sk));
+        auto hide_chunk = [&](float (&x)[32], int i) {
+          const int vc = v0 + i * 32;
+          hide(x, low_bits(hi - vc + 1) & (~low_bits(lo - vc) | low_bits(sk - vc)) & low_bits(w - i * 32));
+        };
+        // the upper 64 columns are read for their maximum, then again for their
+        // exponentials: 64 scores in registers, not 128 (which spill)
+        float s0[32], s1[32];
+        float top;
+        {
+          float b0[32], b1[32];
+          tmem_ld32(ts + 64, b0);
+          tmem_ld32(ts + 96, b1);
+          tmem_wait_ld();
+          tie32(b0);
+          tie32(b1);
+          tmem_ld32(ts, s0);
+          if (!all_on) {
+            hide_chunk(b0, 2);
+            hide_chunk(b1, 3);
           }
-          tmem_st16(tS[t] + at + c * 16, pk);
+          top = fmaxf(max32(b0), max32(b1));
         }
-      float x0, x1, x2, x3;
-      unpack2(sum2[0], x0, x1);
-      unpack2(sum2[1], x2, x3);
-      l += (x0 + x1) + (x2 + x3);
-      tmem_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&pfull[t]);
-      ++done;
-    }
-    if (ok && tiles > 0 && done > 0) ok = mbar_wait_warp(ofull, 0, ab, kErrO);
-    if (ok) {
-      tc_fence_after();
-      const int64_t ooff = b * a.o_b + (int64_t)h * a.o_h + (rq.q0 + i0 + qi) * a.o_n;
-      T* orow = static_cast<T*>(a.out) + (valid ? ooff : 0);
-      bool fine = true;
-#pragma unroll
-      for (int c = 0; c < VC * 2; ++c) {
-        if (c * 32 >= a.dv) break;
-        float o[32];
-        if (done > 0) {
-          tmem_ld32(tO[t] + at + c * 32, o);
+        tmem_ld32(ts + 32, s1);
+        tmem_wait_ld();
+        tie32(s0);
+        tie32(s1);
+        if (!all_on) {
+          hide_chunk(s0, 0);
+          hide_chunk(s1, 1);
+        }
+        top = fmaxf(top, fmaxf(max32(s0), max32(s1))) * c2;
+        const bool move = top > m + kMove;
+        if (__any_sync(0xffffffffu, move)) {
+          const float to = move ? top : m;
+          const float alpha = move ? ex2(m - to) : 1.0f;   // m = -inf: 0
+          m = to;
+          l *= alpha;
+          if (done > 0)   // the products of this row's earlier tiles have ended (sfull)
+            scale_row(tO[t] + at, a.dv, alpha);
+        }
+        const float off = kShift - (m == -INFINITY ? 0.0f : m);
+        const uint64_t off2 = pack2(off, off), c22 = pack2(c2, c2);
+        uint64_t sum2[2] = {0, 0};
+        // the first 64 keys' products start under the rest's exponentials
+        auto hand_over = [&](int half) {
+          tmem_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&pfull[2 * t + half]);
+        };
+        exp_chunk<DT>(s0, all_on, c22, off2, sum2, ts);
+        tmem_ld32(ts + 64, s0);
+        exp_chunk<DT>(s1, all_on, c22, off2, sum2, ts + 16);
+        tmem_ld32(ts + 96, s1);
+        hand_over(0);
+        if (w > 64) {
+          tmem_wait_ld();
+          tie32(s0);
+          tie32(s1);
+          if (!all_on) {
+            hide_chunk(s0, 2);
+            hide_chunk(s1, 3);
+          }
+          exp_chunk<DT>(s0, all_on, c22, off2, sum2, ts + 32);
+          exp_chunk<DT>(s1, all_on, c22, off2, sum2, ts + 48);
+          hand_over(1);
+        } else {
           tmem_wait_ld();
         }
-        const float inv = 1.0f / l;
-        uint32_t pk[16];
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const float x = l == 0.0f ? 0.0f : o[2 * e] * inv, y = l == 0.0f ? 0.0f : o[2 * e + 1] * inv;
-          fine &= c * 32 + 2 * e >= a.dv || fabsf(x) < INFINITY;
-          fine &= c * 32 + 2 * e + 1 >= a.dv || fabsf(y) < INFINITY;
-          pk[e] = pack16<DT>(x, y);
+        float x0, x1, x2, x3;
+        unpack2(sum2[0], x0, x1);
+        unpack2(sum2[1], x2, x3);
+        l += (x0 + x1) + (x2 + x3);
+        ++done;
+      }
+      if (ok && done > 0) {
+        ok = mbar_wait_warp_lazy(&ofull[t], outs & 1, ab, kErrO);
+        ++outs;
+      }
+      if (!ok) break;
+      tc_fence_after();
+      const int h0 = c.hk * p.group + c.g0, nq = c.nq;
+      const int64_t obase = c.b * a.o_b + (int64_t)h0 * a.o_h + c.q_row * a.o_n;
+      // 32 columns at a time pass through shared memory, so that neighbouring
+      // lanes store neighbouring pieces of a row (16 bytes; the pitch keeps the
+      // banks apart)
+      T* out = static_cast<T*>(a.out) + obase;
+      const float inv = 1.0f / l;
+      bool fine = true;
+#pragma unroll 1
+      for (int c0 = 0; c0 < a.dv && t * tq < nq; c0 += 32) {
+        float o[32];
+        if (done > 0) {
+          tmem_ld32(tO[t] + at + c0, o);
+          tmem_wait_ld();
         }
-        if (valid) {
-          if (p.vec_out && c * 32 + 32 <= a.dv) {
+        tie32(o);
+        float big = 0.0f;
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              reinterpret_cast<uint4*>(orow + c * 32)[e] = make_uint4(pk[4 * e], pk[4 * e + 1], pk[4 * e + 2], pk[4 * e + 3]);
-          } else {
+        for (int e = 0; e < 32; ++e) {
+          o[e] = l == 0.0f ? 0.0f : o[e] * inv;
+          // 0 * x is 0, NaN where x is not finite
+          big = c0 + e < a.dv ? fmaf(o[e], 0.0f, big) : big;
+        }
+        fine &= big == 0.0f;
 #pragma unroll
-            for (int e = 0; e < 32; ++e)
-              if (c * 32 + e < a.dv) {
-                const uint16_t bits = (uint16_t)(pk[e >> 1] >> (16 * (e & 1)));
-                reinterpret_cast<uint16_t*>(orow)[c * 32 + e] = bits;
-              }
+        for (int e = 0; e < 32; e += 8)
+          *reinterpret_cast<uint4*>(stage + lane * L::kPitch + e * 2) =
+              make_uint4(pack16<DT>(o[e], o[e + 1]), pack16<DT>(o[e + 2], o[e + 3]), pack16<DT>(o[e + 4], o[e + 5]),
+                         pack16<DT>(o[e + 6], o[e + 7]));
+        __syncwarp();
+        const int width = min(32, a.dv - c0);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {   // 8 rows of four pieces
+          const int r = i * 8 + (lane >> 2), piece = lane & 3;
+          const int rr = quarter * 32 + r, rqi = t * tq + (rr >> p.pack_log);
+          T* to = out + (int64_t)(rr & (p.pack - 1)) * a.o_h + rqi * a.o_n + c0 + piece * 8;
+          if (rqi < nq && piece * 8 < width) {
+            if (p.vec_out) {
+              *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(stage + r * L::kPitch + piece * 16);
+            } else {
+#pragma unroll 1
+              for (int e = 0; e < min(8, width - piece * 8); ++e)
+                to[e] = *reinterpret_cast<const T*>(stage + r * L::kPitch + piece * 16 + e * 2);
+            }
           }
         }
+        __syncwarp();
       }
-      if (valid && !fine)
-        row_again<DT>(a, b * a.q_b + (int64_t)h * a.q_h + (rq.q0 + i0 + qi) * a.q_n,
-                      b * a.k_b + (int64_t)hk * a.k_h + rq.k0 * a.k_n, b * a.v_b + (int64_t)hk * a.v_h + rq.k0 * a.v_n, ooff,
-                      p0 + qi, rq.m);
+      if (qi < nq && !fine) {
+        const int g = row & (p.pack - 1), h = h0 + g;
+        row_again<DT>(a, c.b * a.q_b + (int64_t)h * a.q_h + (c.q_row + qi) * a.q_n,
+                      c.b * a.k_b + (int64_t)c.hk * a.k_h + c.k_row * a.k_n,
+                      c.b * a.v_b + (int64_t)c.hk * a.v_h + c.k_row * a.v_n, obase + (int64_t)g * a.o_h + qi * a.o_n,
+                      c.p0 + qi, c.m);
+      }
+      tc_fence_before();   // O has been read: the next pair's products may overwrite it
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&plan_empty[pair & 1]);
     }
   }
   tc_fence_before();
@@ -560,7 +798,7 @@ int launch_one(const CUtensorMap* maps, const WindowTcParams& p, dim3 grid, cuda
   auto kern = window_tc_kernel<DT, DC, VC>;
   const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Layout<DC, VC>::kBytes);
   if (e != cudaSuccess) return set_error(SA_ERR_CUDA, "window_tc smem attribute: %s", cudaGetErrorString(e));
-  kern<<<grid, kThreads, Layout<DC, VC>::kBytes, s>>>(maps[0], maps[1], maps[2], maps[3], maps[4], p);
+  kern<<<grid, kThreads, Layout<DC, VC>::kBytes, s>>>(maps[0], maps[1], maps[2], maps[3], maps[4], maps[5], maps[6], p);
   return check_launch("window_tc_kernel");
 }
 
@@ -579,9 +817,10 @@ bool aligned(const void* base, int64_t size1, int64_t s1, int64_t size2, int64_t
 }  // namespace
 
 // Whether the tensor-core kernel takes these tensors: 16-bit elements, head
-// widths up to 128, rows on 16-byte borders (TMA) and no repeated rows.
+// widths up to 128, rows on 16-byte borders (TMA), no repeated rows, and a scale
+// that is not negative (the running maximum is taken before the scale).
 bool window_tc_takes(const WindowArgs& a) {
-  if (a.dtype == SA_REP_FLOAT32 || a.d > 128 || a.dv > 128 || a.m == 0) return false;
+  if (a.dtype == SA_REP_FLOAT32 || a.d > 128 || a.dv > 128 || a.m == 0 || a.m >= (1 << 30) || a.n >= (1 << 30) || !(a.scale >= 0.0f)) return false;
   return aligned(a.q, a.n, a.q_n, a.heads, a.q_h, a.cu_q ? 1 : a.batch, a.q_b) &&
          aligned(a.k, a.m, a.k_n, a.kv_heads, a.k_h, a.cu_q ? 1 : a.batch, a.k_b) &&
          aligned(a.v, a.m, a.v_n, a.kv_heads, a.v_h, a.cu_q ? 1 : a.batch, a.v_b);
@@ -592,29 +831,40 @@ int launch_window_tc(const WindowArgs& a, cudaStream_t s) {
   p.a = a;
   p.group = a.heads / a.kv_heads;
   p.pack = 1;
-  while (p.pack < 32 && p.group % (2 * p.pack) == 0) p.pack *= 2;
+  while (p.pack < 32 && p.group % (2 * p.pack) == 0) {
+    p.pack *= 2;
+    ++p.pack_log;
+  }
   p.blocks = p.group / p.pack;
   p.rows_per_cta = 2 * kRows / p.pack;
-  p.vec_out = ((uintptr_t)a.out & 15) == 0 && (a.o_n & 7) == 0 && (a.o_h & 7) == 0 && (a.o_b & 7) == 0;
+  p.vec_out = ((uintptr_t)a.out & 15) == 0 && (a.o_n & 7) == 0 && (a.o_h & 7) == 0 && (a.o_b & 7) == 0 &&
+              (a.dv & 7) == 0;
   p.wait_ns = wait_limit_ns();
   const bool bf16 = a.dtype == SA_REP_BFLOAT16;
   const int64_t batch = a.cu_q ? 1 : a.batch;
-  CUtensorMap maps[5];
+  CUtensorMap maps[7];   // q; k in boxes of a tile, of the seam's 16 rows and of the rows behind them; v likewise
   const int64_t qd[5] = {a.d, p.group, a.n, a.kv_heads, batch};
   const int64_t qs[4] = {a.q_h, a.q_n, a.q_h * p.group, a.q_b};
   const int qb[5] = {64, p.pack, kRows / p.pack, 1, 1};
   int rc = encode(&maps[0], bf16, a.q, 5, qd, qs, qb);
-  for (int i = 0; !rc && i < 4; ++i) {
-    const bool isv = i >= 2;
+  for (int i = 0; !rc && i < 6; ++i) {
+    const bool isv = i >= 3;
     const int64_t kd[4] = {isv ? a.dv : a.d, a.m, a.kv_heads, batch};
     const int64_t ks[3] = {isv ? a.v_n : a.k_n, isv ? a.v_h : a.k_h, isv ? a.v_b : a.k_b};
-    const int kb[4] = {64, i & 1 ? kSeam : kCols, 1, 1};
+    const int rows[3] = {kCols, kSeam, kCols - kSeam};
+    const int kb[4] = {64, rows[i % 3], 1, 1};
     rc = encode(&maps[1 + i], bf16, isv ? a.v : a.k, 4, kd, ks, kb);
   }
   if (rc) return rc;
-  const int64_t tiles = tile_count(a, p.rows_per_cta);
-  if (tiles > 2147483647LL || a.heads / p.pack > 65535) return set_error(SA_ERR_UNSUPPORTED, "window attention: grid too large");
-  dim3 grid((unsigned)tiles, (unsigned)(a.heads / p.pack));
+  const int64_t tiles = tile_count(a, p.rows_per_cta), items = tiles * (a.heads / p.pack);
+  if (items > 2147483647LL) return set_error(SA_ERR_UNSUPPORTED, "window attention: grid too large");
+  p.tiles = (uint32_t)tiles;
+  p.items = (uint32_t)items;
+  int dev = 0, sms = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  if (e != cudaSuccess) return set_error(SA_ERR_CUDA, "window_tc device query: %s", cudaGetErrorString(e));
+  dim3 grid((unsigned)(items < sms ? items : sms));
   return bf16 ? launch_dims<SA_REP_BFLOAT16>(maps, p, grid, s) : launch_dims<SA_REP_FLOAT16>(maps, p, grid, s);
 }
 
