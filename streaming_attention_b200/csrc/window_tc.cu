@@ -175,40 +175,6 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   return r;
 }
 
-// 2^x of two values on the FMA and integer pipes: x = n + f with n whole and
-// |f| <= 1/2, 2^f as a polynomial of least relative error on that interval
-// (a reweighted least-squares fit: degree 3 is 7.5e-5 off, a fiftieth of
-// bfloat16's half step; degree 4 2.7e-6, a hundredth and less of float16's),
-// n added to the exponent.  Below 2^-125 the result stays at 2^-125.
-template <int DT>
-__device__ __forceinline__ void exp2_poly(uint64_t x2, float& a, float& b) {
-  float x, y;
-  unpack2(x2, x, y);
-  // a NaN stays one (as the largest float at the end: its products are not finite either)
-  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x) : "f"(-125.0f));
-  asm("max.NaN.f32 %0, %0, %1;" : "+f"(y) : "f"(-125.0f));
-  x2 = pack2(x, y);
-  const uint64_t magic = pack2(12582912.0f, 12582912.0f), unmagic = pack2(-12582912.0f, -12582912.0f);
-  const uint64_t t = add2(x2, magic);
-  const uint64_t f = fma2(add2(t, unmagic), pack2(-1.0f, -1.0f), x2);
-  uint64_t r;
-  if (DT == SA_REP_BFLOAT16) {
-    r = fma2(pack2(0.0551716610789299f, 0.0551716610789299f), f, pack2(0.2426111251115799f, 0.2426111251115799f));
-    r = fma2(r, f, pack2(0.6932609677314758f, 0.6932609677314758f));
-    r = fma2(r, f, pack2(0.9999280571937561f, 0.9999280571937561f));
-  } else {
-    r = fma2(pack2(0.009570101276040077f, 0.009570101276040077f), f, pack2(0.05591785907745361f, 0.05591785907745361f));
-    r = fma2(r, f, pack2(0.240247443318367f, 0.240247443318367f));
-    r = fma2(r, f, pack2(0.6931217908859253f, 0.6931217908859253f));
-    r = fma2(r, f, pack2(0.9999992847442627f, 0.9999992847442627f));
-  }
-  float tx, ty;
-  unpack2(t, tx, ty);
-  unpack2(r, x, y);
-  a = __uint_as_float(__float_as_uint(x) + (__float_as_uint(tx) << 23));
-  b = __uint_as_float(__float_as_uint(y) + (__float_as_uint(ty) << 23));
-}
-
 // Two floats as 16-bit values, the first in the low half.
 template <int DT>
 __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
@@ -219,10 +185,6 @@ __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
     asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
-
-// Which pairs of a chunk's 16 take the polynomial: 4, so that the special
-// function unit (16 a clock) and the FMA pipe finish together.
-__host__ __device__ constexpr bool poly_pair(int e) { return e % 4 == 1; }
 
 // The x lowest bits set (x may be anything).
 __device__ __forceinline__ uint32_t low_bits(int x) {
@@ -242,37 +204,20 @@ __device__ __forceinline__ float max32(const float (&s)[32]) {
   return fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
 }
 
-// P of a chunk: 2^(s c2 + off), summed and, in 16 bits, stored to TMEM.  Hidden
-// scores (-inf) need the exact zero of ex2.
+// P of a chunk: 2^(s c2 + off), summed and, in 16 bits, stored to TMEM.  (A third
+// of the exponentials as a polynomial on the FMA pipe, which a loop of softmax
+// alone gains 15 % from, cost 3 % here: the loop waits more than it computes.)
 template <int DT>
-__device__ __forceinline__ void exp_chunk(float (&s)[32], bool all_on, uint64_t c22, uint64_t off2, uint64_t (&sum2)[2],
-                                          uint32_t to) {
+__device__ __forceinline__ void exp_chunk(float (&s)[32], uint64_t c22, uint64_t off2, uint64_t (&sum2)[2], uint32_t to) {
   uint32_t pk[16];
-  if (all_on) {
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      const uint64_t z = fma2(pack2(s[2 * e], s[2 * e + 1]), c22, off2);
-      float x, y;
-      if (poly_pair(e)) {
-        exp2_poly<DT>(z, x, y);
-      } else {
-        unpack2(z, x, y);
-        x = ex2(x);
-        y = ex2(y);
-      }
-      sum2[e & 1] = add2(sum2[e & 1], pack2(x, y));
-      pk[e] = pack16<DT>(x, y);
-    }
-  } else {
-#pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      float x, y;
-      unpack2(fma2(pack2(s[2 * e], s[2 * e + 1]), c22, off2), x, y);
-      x = ex2(x);
-      y = ex2(y);
-      sum2[e & 1] = add2(sum2[e & 1], pack2(x, y));
-      pk[e] = pack16<DT>(x, y);
-    }
+  for (int e = 0; e < 16; ++e) {
+    float x, y;
+    unpack2(fma2(pack2(s[2 * e], s[2 * e + 1]), c22, off2), x, y);
+    x = ex2(x);
+    y = ex2(y);
+    sum2[e & 1] = add2(sum2[e & 1], pack2(x, y));
+    pk[e] = pack16<DT>(x, y);
   }
   tmem_st16(to, pk);
 }
@@ -653,9 +598,9 @@ window_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
           __syncwarp();
           if (lane == 0) mbar_arrive(&pfull[2 * t + half]);
         };
-        exp_chunk<DT>(s0, all_on, c22, off2, sum2, ts);
+        exp_chunk<DT>(s0, c22, off2, sum2, ts);
         tmem_ld32(ts + 64, s0);
-        exp_chunk<DT>(s1, all_on, c22, off2, sum2, ts + 16);
+        exp_chunk<DT>(s1, c22, off2, sum2, ts + 16);
         tmem_ld32(ts + 96, s1);
         hand_over(0);
         if (w > 64) {
@@ -666,8 +611,8 @@ window_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
             hide_chunk(s0, 2);
             hide_chunk(s1, 3);
           }
-          exp_chunk<DT>(s0, all_on, c22, off2, sum2, ts + 32);
-          exp_chunk<DT>(s1, all_on, c22, off2, sum2, ts + 48);
+          exp_chunk<DT>(s0, c22, off2, sum2, ts + 32);
+          exp_chunk<DT>(s1, c22, off2, sum2, ts + 48);
           hand_over(1);
         } else {
           tmem_wait_ld();

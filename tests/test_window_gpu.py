@@ -23,10 +23,7 @@ def dev():
 
 
 def _p_half(dtype):
-    """The rounding of a probability to 16 bits, and a 32nd of it for the
-    exponentials that a polynomial takes: bfloat16's is 7.5e-5 = 0.019 2^-8 off,
-    float16's 2.7e-6 = 0.006 2^-11."""
-    return 0.0 if dtype == F32 else R.HALF[dtype] * (1 + 2.0 ** -5)
+    return 0.0 if dtype == F32 else R.HALF[dtype]
 
 
 def _make(shape, dtype, g, scale=1.0):
