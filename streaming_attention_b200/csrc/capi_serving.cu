@@ -236,6 +236,8 @@ int sa_kv4_attend(const void* k_codes, const void* k_params, const void* v_codes
   if (window < 0 || sinks < 0) return set_error(SA_ERR_INVALID_ARG, "window and sinks must be non-negative");
   if (requests > 65535) return set_error(SA_ERR_UNSUPPORTED, "more than 65535 requests in one call");
   if ((int64_t)n * heads > 65535) return set_error(SA_ERR_UNSUPPORTED, "more than 65535 query rows per request");
+  if (((int64_t)width << a.c.page_shift) > 2147483647LL)
+    return set_error(SA_ERR_UNSUPPORTED, "a row of the page table covers 2^31 tokens or more");
   if (requests == 0 || n == 0) return SA_OK;
   if (!q || !out || !strides || !lengths || (width > 0 && !tables)) return set_error(SA_ERR_INVALID_ARG, "null pointer");
   a.q = q;

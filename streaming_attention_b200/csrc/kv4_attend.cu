@@ -4,10 +4,34 @@
 //   query i of n stands at position length - n + i; visible as in the windowed
 //   attention (serving.cuh); nothing visible gives zeros.
 //
-// One CTA per (query head and token, request), four warps; a warp takes every
-// fourth visible token, a lane the columns lane, lane + 32, ...; each warp
-// keeps a running maximum, sum and float32 output, joined at the end.
+// Bound by the cache's bytes (d / 2 + 4 of a key and of a value), so codes go
+// from global memory to registers and from there to the matrix units, with no
+// shared memory between (mma.sync m16n8k16: eight query rows fill its n, where
+// a tcgen05 tile would hold 128 rows, nearly all empty).
+//
+// A warp takes blocks of 16 tokens.  With x = scale 8 + least the value of a
+// code is s (code - 8) + x, and code - 8 is exact in bfloat16, so
+//   S = s_k (K_codes Q^T) + x_k sum(Q)         tokens x rows
+//   O = V_codes^T (p s_v)^T + sum(p x_v)       columns x rows
+// with scales and offsets in float32 on either side of the products.  Q is
+// bfloat16 as it is, float16 as two and float32 as three bfloat16 pieces (exact,
+// or to 24 bits); p s_v is split into two pieces (16 bits; three for float32).
+//
+// Fragments.  Lane (g = lane / 4, c = lane % 4).  Row r < 8 of the token axis is
+// token 2 r of the block and row r + 8 token 2 r + 1: the cache keeps four
+// tokens' bytes of a value column pair in one word, and that word is then a
+// whole A fragment of V^T (tokens 4 c .. 4 c + 3, columns 2 b and 2 b + 1); a word
+// of a key row is half the A fragments of two k steps, with the contraction's
+// columns in the order of its nibbles (Q is loaded to match).  S comes out as
+// tokens x rows and is turned by movmatrix for the second product.
+//
+// The visible blocks of a (request, key head) are dealt out to the warps of a
+// cluster of CTAs, which join their maxima, sums and outputs through (distributed)
+// shared memory in a fixed order: one launch, the same bits every time.
+#include <cooperative_groups.h>
 #include <math.h>
+
+#include <algorithm>
 
 #include "kv4.cuh"
 
@@ -15,101 +39,481 @@ namespace sa {
 
 namespace {
 
-constexpr int kWarps = 4;
-constexpr int kCols = 8;   // columns per lane: d <= 256
+namespace cg = cooperative_groups;
 
-template <int DT>
-__global__ void __launch_bounds__(kWarps * 32) attend_kernel(const Kv4AttendArgs a) {
-  using T = typename Elem<DT>::T;
-  __shared__ float o_s[kWarps][256];
-  __shared__ float m_s[kWarps], l_s[kWarps];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int h = blockIdx.x % a.heads, i = blockIdx.x / a.heads, r = blockIdx.y;
-  const int hk = h / (a.heads / a.c.heads);
-  const int64_t length = max(a.lengths[r], 0);
-  const int64_t cap = (int64_t)a.width << a.c.page_shift;
-  if (length > cap && threadIdx.x == 0) report(a.status, kBadLength, r);
-  const int64_t p = length - a.n + i;
-  const KeyRanges kr = key_ranges(p, p, min(length, cap), a.window, a.sinks);
-  const T* q = static_cast<const T*>(a.q) + r * a.q_r + i * a.q_n + h * a.q_h;
-  float qv[kCols], acc[kCols];
+constexpr int kWarps = 8;
+constexpr int kThreads = kWarps * 32;
+constexpr float kMove = 8.0f;     // how far a maximum may be passed before it is moved (base 2)
+constexpr float kShift = -12.0f;  // p <= 2^-4: 2^16 values of 1e34 still sum below float32's limit
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+// Two codes (bits 0..3 and 16..19 of w) less 8, as bfloat16: 128 + code by its
+// bits, less 136; both exact.
+__device__ __forceinline__ uint32_t codes(uint32_t w) {
+  uint32_t x = (w & 0x000f000fu) | 0x43004300u, r;
+  asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(x), "r"(0x3f803f80u), "r"(0xc308c308u));
+  return r;
+}
+
+__device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                    uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+  return r;
+}
+
+__device__ __forceinline__ float2 params(uint32_t w) {   // scale, least
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+
+// What a lane holds of one block.
+template <int DP>
+struct Block {
+  static constexpr int kK = DP / 32;                  // words of one key row's share
+  static constexpr int kV = DP / 16;                  // words of V: one a 16-column tile
+  uint32_t k0[kK], k1[kK], v[kV];
+  uint2 kp, vp;                                       // params of tokens 2 g and 2 g + 1
+};
+
+template <int N>
+__device__ __forceinline__ void load_words(uint32_t (&x)[N], const uint8_t* p) {
+  if constexpr (N % 4 == 0) {
 #pragma unroll
-  for (int c = 0; c < kCols; ++c) {
-    qv[c] = lane + 32 * c < a.c.d ? to_f32(q[lane + 32 * c]) * a.scale : 0.0f;
-    acc[c] = 0.0f;
+    for (int i = 0; i < N / 4; ++i) {
+      const uint4 y = __ldg(reinterpret_cast<const uint4*>(p) + i);
+      x[4 * i] = y.x;
+      x[4 * i + 1] = y.y;
+      x[4 * i + 2] = y.z;
+      x[4 * i + 3] = y.w;
+    }
+  } else if constexpr (N == 2) {
+    const uint2 y = __ldg(reinterpret_cast<const uint2*>(p));
+    x[0] = y.x;
+    x[1] = y.y;
+  } else {
+    x[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
   }
-  float m = -INFINITY, l = 0.0f;
-  const int bytes = a.c.dp >> 1;
-  for (int part = 0; part < 2; ++part) {
-    const int64_t jb = part ? kr.begin : 0, je = part ? kr.end : kr.first;
-    for (int64_t j = jb + warp; j < je; j += kWarps) {
-      const int page = a.tables[(int64_t)r * a.width + (j >> a.c.page_shift)];
-      if (page < 0 || page >= a.c.pages) {
-        if (lane == 0) report(a.status, kBadPage, page);
-        continue;
-      }
-      const int off = (int)(j & ((1 << a.c.page_shift) - 1));
-      const int64_t cell = ((int64_t)page * a.c.heads + hk) << a.c.page_shift;
-      const __nv_bfloat16* kp = a.c.k_params + 2 * (cell + off);
-      const __nv_bfloat16* vp = a.c.v_params + 2 * (cell + off);
-      const float ks = __bfloat162float(kp[0]), km = __bfloat162float(kp[1]);
-      const float vs = __bfloat162float(vp[0]), vm = __bfloat162float(vp[1]);
-      float dot = 0.0f;
+}
+
+// cell: index of the block's first token in [pages, heads, page].
+template <int DP>
+__device__ __forceinline__ void load_block(Block<DP>& b, const Kv4Cache& c, int64_t cell, int g, int cc) {
+  const uint8_t* k = c.k_codes + (cell + 2 * g) * (DP / 2) + cc * (DP / 8);
+  load_words(b.k0, k);
+  load_words(b.k1, k + DP / 2);
+  // token group cc of the block; 16-byte pieces of neighbouring lanes g are neighbours
+  const uint8_t* v = c.v_codes + (cell + 4 * cc) * (DP / 2);
+  if constexpr (DP >= 64) {
 #pragma unroll
-      for (int c = 0; c < kCols; ++c) {
-        const int col = lane + 32 * c;
-        if (col < a.c.d) {
-          const uint32_t byte = a.c.k_codes[(cell + off) * bytes + (col >> 1)];
-          dot = fmaf(qv[c], fmaf((float)((byte >> (4 * (col & 1))) & 15), ks, km), dot);
+    for (int q = 0; q < DP / 64; ++q) {
+      const uint4 y = __ldg(reinterpret_cast<const uint4*>(v + q * 128) + g);
+      b.v[4 * q] = y.x;
+      b.v[4 * q + 1] = y.y;
+      b.v[4 * q + 2] = y.z;
+      b.v[4 * q + 3] = y.w;
+    }
+  } else {
+    const uint2 y = __ldg(reinterpret_cast<const uint2*>(v) + g);
+    b.v[0] = y.x;
+    b.v[1] = y.y;
+  }
+  b.kp = __ldg(reinterpret_cast<const uint2*>(c.k_params + 2 * (cell + 2 * g)));
+  b.vp = __ldg(reinterpret_cast<const uint2*>(c.v_params + 2 * (cell + 2 * g)));
+}
+
+// Byte column b of O's tile t (16 columns): lane g holds columns 2 b and 2 b + 1.
+template <int DP>
+__device__ __forceinline__ int byte_column(int t, int g) {
+  return DP >= 64 ? (t >> 2) * 32 + g * 4 + (t & 3) : g * 2 + t;
+}
+
+template <int DT, int DP, int NT>
+struct Shape {
+  static constexpr int kQ = DT == SA_REP_BFLOAT16 ? 1 : (DT == SA_REP_FLOAT16 ? 2 : 3);   // pieces of q
+  static constexpr int kP = DT == SA_REP_FLOAT32 ? 3 : 2;                                 // pieces of p s_v
+  static constexpr int kRows = 8 * NT;
+  // registers of O, Q and two blocks in a lane: where two CTAs an SM would spill (much), one
+  static constexpr int kHeld = NT * (DP / 4 + kQ * DP / 8) + DP / 4 + 8;
+  static constexpr int kPerSm = kHeld <= 104 ? 2 : 1;
+  static constexpr int kPitch = DP + 4;   // a row of O in shared memory
+  static constexpr int kSmem = (kWarps * kRows * kPitch + 2 * kWarps * kRows + 2 * kRows) * 4;
+};
+
+template <int DT, int DP, int NT>
+__global__ void __launch_bounds__(kThreads, (Shape<DT, DP, NT>::kPerSm)) attend_kernel(const Kv4AttendArgs a) {
+  using T = typename Elem<DT>::T;
+  using S = Shape<DT, DP, NT>;
+  constexpr int kKS = DP / 16;   // k steps of the first product, 16-column tiles of the second
+  extern __shared__ float smem[];
+  float* sm_o = smem;                                   // [warps][rows][pitch]
+  float* sm_m = smem + kWarps * S::kRows * S::kPitch;   // [warps][rows]
+  float* sm_l = sm_m + kWarps * S::kRows;
+  float* part_m = sm_l + kWarps * S::kRows;             // [rows]: this CTA's
+  float* part_l = part_m + S::kRows;
+
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int g = lane >> 2, cc = lane & 3;
+  const int group = a.heads / a.c.heads;
+  const int rows = a.n * group;
+  const int tiles = (rows + S::kRows - 1) / S::kRows;
+  const int hk = blockIdx.y / tiles, row0 = (blockIdx.y % tiles) * S::kRows;
+  const int r = blockIdx.z;
+  const int splits = gridDim.x;
+
+  const int cap = a.width << a.c.page_shift;
+  int length = max(a.lengths[r], 0);
+  if (length > cap && threadIdx.x == 0) report(a.status, kBadLength, r);
+  const int window = (int)min(a.window, (int64_t)1 << 30), sinks = (int)min(a.sinks, (int64_t)1 << 30);
+  // positions of this tile's rows (rows behind the last count as the last)
+  auto position = [&](int row) { return length - a.n + min(row0 + row, rows - 1) / group; };
+  const int p_lo = position(0), p_hi = position(S::kRows - 1);
+  const KeyRanges kr = key_ranges(p_lo, p_hi, min(length, cap), window, sinks);
+  const int sink_blocks = (int)((kr.first + 15) >> 4);
+  const int win_begin = max((int)(kr.begin >> 4), sink_blocks), win_end = (int)((kr.end + 15) >> 4);
+  const int blocks = sink_blocks + max(win_end - win_begin, 0);
+  const float sc = a.scale * 1.4426950408889634f;   // log2(e): scores in base 2
+
+  // Q: fragments of this lane's row g (of each n tile) and the sums of the rows 2 cc, 2 cc + 1
+  uint32_t qf[NT][S::kQ][kKS][2];
+  float qsum[NT][2];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    const int row = row0 + nt * 8 + g;
+    const bool in = row < rows;
+    const int i = in ? row / group : 0, h = hk * group + (in ? row - i * group : 0);
+    const T* q = static_cast<const T*>(a.q) + r * a.q_r + i * a.q_n + h * a.q_h;
+    float sum = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kKS / 2; ++w) {
+      float x[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int col = cc * (DP / 4) + w * 8 + e;
+        x[e] = in && col < a.c.d ? to_f32(q[col]) : 0.0f;
+        sum += x[e];
+      }
+#pragma unroll
+      for (int s = 0; s < S::kQ; ++s) {
+        float hi[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          hi[e] = __bfloat162float(__float2bfloat16_rn(x[e]));
+          x[e] -= hi[e];
         }
+        qf[nt][s][2 * w][0] = pack_bf16(hi[0], hi[4]);
+        qf[nt][s][2 * w][1] = pack_bf16(hi[1], hi[5]);
+        qf[nt][s][2 * w + 1][0] = pack_bf16(hi[2], hi[6]);
+        qf[nt][s][2 * w + 1][1] = pack_bf16(hi[3], hi[7]);
+      }
+    }
+    sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+    sum += __shfl_xor_sync(0xffffffffu, sum, 2);   // row g's sum, in its four lanes
+    qsum[nt][0] = __shfl_sync(0xffffffffu, sum, 8 * cc);
+    qsum[nt][1] = __shfl_sync(0xffffffffu, sum, 8 * cc + 4);
+  }
+
+  float o[NT][kKS][4];
+  float m[NT][2], l[NT][2], z[NT][2];   // of rows 2 cc and 2 cc + 1
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+    for (int t = 0; t < kKS; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[nt][t][e] = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      m[nt][e] = -INFINITY;
+      l[nt][e] = z[nt][e] = 0.0f;
+    }
+  }
+
+  // block u of this warp is block first + u * step of the visible ones
+  const int first = blockIdx.x * kWarps + warp, step = splits * kWarps;
+  const int mine = first < blocks ? (blocks - first + step - 1) / step : 0;
+  auto token_of = [&](int u) {
+    const int v = first + u * step;
+    return (v < sink_blocks ? v : win_begin + v - sink_blocks) << 4;
+  };
+  const int32_t* table = a.tables + (int64_t)r * a.width;
+  // page ids of the next 32 blocks, one a lane
+  int page_of = 0;
+  auto fetch_pages = [&](int u0) {
+    const int u = u0 + lane;
+    page_of = u < mine ? __ldg(table + (token_of(u) >> a.c.page_shift)) : 0;
+    if (u < mine && (page_of < 0 || page_of >= a.c.pages)) {
+      report(a.status, kBadPage, page_of);
+      page_of = -1;   // its tokens count as hidden
+    }
+  };
+  const int page_mask = (1 << a.c.page_shift) - 1;
+  auto load = [&](Block<DP>& b, int u) -> bool {   // false: nothing there
+    if (u >= mine) return false;
+    if ((u & 31) == 0) fetch_pages(u);
+    const int page = __shfl_sync(0xffffffffu, page_of, u & 31);
+    if (page < 0) return false;
+    const int64_t cell = (((int64_t)page * a.c.heads + hk) << a.c.page_shift) + (token_of(u) & page_mask);
+    load_block(b, a.c, cell, g, cc);
+    return true;
+  };
+
+  auto work = [&](const Block<DP>& b, int token) {
+    float s[NT][4];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[nt][e] = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kKS / 2; ++w) {
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const uint32_t a0 = codes(b.k0[w] >> (8 * half)), a1 = codes(b.k1[w] >> (8 * half));
+        const uint32_t a2 = codes(b.k0[w] >> (8 * half + 4)), a3 = codes(b.k1[w] >> (8 * half + 4));
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int q = 0; q < S::kQ; ++q)
+            mma(s[nt], a0, a1, a2, a3, qf[nt][q][2 * w + half][0], qf[nt][q][2 * w + half][1]);
+      }
+    }
+    const float2 ka = params(b.kp.x), kb = params(b.kp.y), va = params(b.vp.x), vb = params(b.vp.y);
+    const float k_s[2] = {ka.x * sc, kb.x * sc}, k_x[2] = {fmaf(8.0f, ka.x, ka.y) * sc, fmaf(8.0f, kb.x, kb.y) * sc};
+    const float v_s[2] = {va.x, vb.x}, v_x[2] = {fmaf(8.0f, va.x, va.y), fmaf(8.0f, vb.x, vb.y)};
+    // every row sees the whole block
+    const bool all_on = token + 15 <= p_lo && (token > p_hi - window || token + 16 <= sinks);
+    uint32_t on = 0xffffffffu;   // bit 4 nt + e: s[nt][e]
+    if (!all_on) {
+      on = 0;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int j = token + 2 * g + (e >> 1), p = position(nt * 8 + 2 * cc + (e & 1));
+          if (j <= p && (j > p - window || j < sinks) && j < cap) on |= 1u << (4 * nt + e);
+        }
+    }
+    bool move = false;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float x = fmaf(k_s[e >> 1], s[nt][e], k_x[e >> 1] * qsum[nt][e & 1]);
+        s[nt][e] = (on >> (4 * nt + e)) & 1u ? x : -INFINITY;
+        move |= s[nt][e] > m[nt][e & 1] + kMove;
+      }
+    if (__any_sync(0xffffffffu, move)) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float top = fmaxf(s[nt][e], s[nt][e + 2]);
+#pragma unroll
+          for (int d = 4; d < 32; d *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+          if (top > m[nt][e] + kMove) {
+            const float alpha = ex2(m[nt][e] - top);   // from -inf: 0
+            m[nt][e] = top;
+            l[nt][e] *= alpha;
+            z[nt][e] *= alpha;
+#pragma unroll
+            for (int t = 0; t < kKS; ++t) {
+              o[nt][t][e] *= alpha;
+              o[nt][t][e + 2] *= alpha;
+            }
+          }
+        }
+    }
+    uint32_t pf[NT][S::kP][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      float ps[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float mm = m[nt][e & 1] == -INFINITY ? 0.0f : m[nt][e & 1];
+        const float p = ex2(s[nt][e] - mm + kShift);
+        const bool seen = (on >> (4 * nt + e)) & 1u;   // hidden tokens' scales may be anything
+        l[nt][e & 1] += p;
+        z[nt][e & 1] = seen ? fmaf(p, v_x[e >> 1], z[nt][e & 1]) : z[nt][e & 1];
+        ps[e] = seen ? p * v_s[e >> 1] : 0.0f;
       }
 #pragma unroll
-      for (int s = 16; s >= 1; s >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, s);
-      const float m_new = fmaxf(m, dot);
-      const float alpha = m_new == -INFINITY ? 1.0f : expf(m - m_new);
-      const float e = m_new == -INFINITY ? 0.0f : expf(dot - m_new);
-      m = m_new;
-      l = l * alpha + e;
-#pragma unroll
-      for (int c = 0; c < kCols; ++c) {
-        const int col = lane + 32 * c;
-        if (col < a.c.d) {
-          const uint32_t byte = a.c.v_codes[cell * bytes + ((int64_t)(off >> 2) * bytes + (col >> 1)) * 4 + (off & 3)];
-          acc[c] = fmaf(e, fmaf((float)((byte >> (4 * (col & 1))) & 15), vs, vm), acc[c] * alpha);
+      for (int q = 0; q < S::kP; ++q) {
+        const uint32_t x = pack_bf16(ps[0], ps[1]), y = pack_bf16(ps[2], ps[3]);
+        pf[nt][q][0] = transpose8(x);
+        pf[nt][q][1] = transpose8(y);
+        if (q + 1 < S::kP) {
+          ps[0] -= __uint_as_float(x << 16);
+          ps[1] -= __uint_as_float(x & 0xffff0000u);
+          ps[2] -= __uint_as_float(y << 16);
+          ps[3] -= __uint_as_float(y & 0xffff0000u);
         }
       }
     }
-  }
-  if (lane == 0) {
-    m_s[warp] = m;
-    l_s[warp] = l;
-  }
 #pragma unroll
-  for (int c = 0; c < kCols; ++c) o_s[warp][lane + 32 * c] = acc[c];
-  __syncthreads();
-  float top = -INFINITY, sum = 0.0f;
-  for (int w = 0; w < kWarps; ++w) top = fmaxf(top, m_s[w]);
-  for (int w = 0; w < kWarps; ++w) sum += m_s[w] == -INFINITY ? 0.0f * l_s[w] : l_s[w] * expf(m_s[w] - top);
-  T* o = static_cast<T*>(a.out) + (((int64_t)r * a.n + i) * a.heads + h) * a.c.d;
-  for (int c = threadIdx.x; c < a.c.d; c += kWarps * 32) {
-    float x = 0.0f;
-    for (int w = 0; w < kWarps; ++w)
-      if (m_s[w] != -INFINITY) x += o_s[w][c] * expf(m_s[w] - top);
-    o[c] = from_f32<T>(sum == 0.0f ? 0.0f : x / sum);
+    for (int t = 0; t < kKS; ++t) {
+      const uint32_t w = b.v[t];
+      const uint32_t a0 = codes(w), a1 = codes(w >> 4), a2 = codes(w >> 8), a3 = codes(w >> 12);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int q = 0; q < S::kP; ++q) mma(o[nt][t], a0, a1, a2, a3, pf[nt][q][0], pf[nt][q][1]);
+    }
+  };
+
+  {
+    Block<DP> b0, b1;
+    bool in0 = load(b0, 0);
+    for (int u = 0; u < mine; u += 2) {
+      const bool in1 = load(b1, u + 1);
+      if (in0) work(b0, token_of(u));
+      in0 = load(b0, u + 2);
+      if (in1) work(b1, token_of(u + 1));
+    }
   }
+
+  // join the warps
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      float x = l[nt][e], y = z[nt][e];
+#pragma unroll
+      for (int d = 4; d < 32; d *= 2) {
+        x += __shfl_xor_sync(0xffffffffu, x, d);
+        y += __shfl_xor_sync(0xffffffffu, y, d);
+      }
+      const int row = nt * 8 + 2 * cc + e;
+      if (g == 0) {
+        sm_m[warp * S::kRows + row] = m[nt][e];
+        sm_l[warp * S::kRows + row] = x;
+      }
+      float* to = sm_o + (warp * S::kRows + row) * S::kPitch;
+#pragma unroll
+      for (int t = 0; t < kKS; ++t) {
+        const int col = 2 * byte_column<DP>(t, g);
+        *reinterpret_cast<float2*>(to + col) = make_float2(o[nt][t][e] + y, o[nt][t][e + 2] + y);
+      }
+    }
+  __syncthreads();
+  // warp 0's place takes the CTA's: each thread a (row, column), warps in order
+  for (int x = threadIdx.x; x < S::kRows * DP; x += kThreads) {
+    const int row = x / DP, col = x - row * DP;
+    float top = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) top = fmaxf(top, sm_m[w * S::kRows + row]);
+    float sum = 0.0f, total = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const float mw = sm_m[w * S::kRows + row];
+      const float f = mw == -INFINITY ? 0.0f : ex2(mw - top);
+      sum = fmaf(f, sm_o[(w * S::kRows + row) * S::kPitch + col], sum);
+      total = fmaf(f, sm_l[w * S::kRows + row], total);
+    }
+    sm_o[row * S::kPitch + col] = sum;
+    if (col == 0) {
+      part_m[row] = top;
+      part_l[row] = total;
+    }
+  }
+  cg::cluster_group cluster = cg::this_cluster();
+  if (splits > 1)
+    cluster.sync();
+  else
+    __syncthreads();
+  // and the cluster's CTAs, each a share of the columns
+  const int share = S::kRows * DP / splits;
+  for (int x = blockIdx.x * share + threadIdx.x; x < (blockIdx.x + 1) * share; x += kThreads) {
+    const int row = x / DP, col = x - row * DP;
+    float top = -INFINITY, sum = 0.0f, total = 0.0f;
+    for (int s = 0; s < splits; ++s) top = fmaxf(top, splits > 1 ? *cluster.map_shared_rank(part_m + row, s) : part_m[row]);
+    for (int s = 0; s < splits; ++s) {
+      const float ms = splits > 1 ? *cluster.map_shared_rank(part_m + row, s) : part_m[row];
+      const float ls = splits > 1 ? *cluster.map_shared_rank(part_l + row, s) : part_l[row];
+      const float os = splits > 1 ? *cluster.map_shared_rank(sm_o + row * S::kPitch + col, s) : sm_o[row * S::kPitch + col];
+      const float f = ms == -INFINITY ? 0.0f : ex2(ms - top);
+      sum = fmaf(f, os, sum);
+      total = fmaf(f, ls, total);
+    }
+    if (row0 + row < rows && col < a.c.d) {
+      const int i = (row0 + row) / group, h = hk * group + (row0 + row) - i * group;
+      T* out = static_cast<T*>(a.out) + (((int64_t)r * a.n + i) * a.heads + h) * a.c.d;
+      out[col] = from_f32<T>(total == 0.0f ? 0.0f : sum / total);
+    }
+  }
+  if (splits > 1) cluster.sync();   // nobody leaves while its shared memory is read
+}
+
+template <int DT, int DP, int NT>
+int launch_one(const Kv4AttendArgs& a, cudaStream_t s) {
+  using S = Shape<DT, DP, NT>;
+  auto kern = attend_kernel<DT, DP, NT>;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
+  if (e != cudaSuccess) return set_error(SA_ERR_CUDA, "kv4 attend smem attribute: %s", cudaGetErrorString(e));
+  const int64_t rows = (int64_t)a.n * (a.heads / a.c.heads);
+  const int64_t y = a.c.heads * ceil_div(rows, S::kRows);
+  if (y > 65535) return set_error(SA_ERR_UNSUPPORTED, "kv4 attend: grid too large");
+  // CTAs per (request, key head): while a warp keeps at least four blocks of the
+  // longest request the table allows and the grid has room for less than six
+  // rounds
+  const int64_t longest = std::min<int64_t>((int64_t)a.width << a.c.page_shift, a.window + std::min(a.sinks, a.window) + a.n);
+  int splits = 1;
+  while (splits < 8 && longest >= (int64_t)splits * 2 * kWarps * 16 * 4 && y * a.requests * splits < 148 * S::kPerSm * 6) splits *= 2;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)splits, (unsigned)y, (unsigned)a.requests);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = S::kSmem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)splits;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  e = cudaLaunchKernelEx(&cfg, kern, a);
+  if (e != cudaSuccess) return set_error(SA_ERR_CUDA, "kv4 attend_kernel: %s", cudaGetErrorString(e));
+  return check_launch("kv4 attend_kernel");
+}
+
+// Two tiles of eight rows where the registers hold them and there are that many rows.
+template <int DT, int DP>
+int launch_rows(const Kv4AttendArgs& a, cudaStream_t s) {
+  if constexpr (DT != SA_REP_FLOAT32 && DP <= 128)
+    if (a.n * (a.heads / a.c.heads) > 8) return launch_one<DT, DP, 2>(a, s);
+  return launch_one<DT, DP, 1>(a, s);
+}
+
+template <int DT>
+int launch_dim(const Kv4AttendArgs& a, cudaStream_t s) {
+  if (a.c.dp == 32) return launch_rows<DT, 32>(a, s);
+  if (a.c.dp == 64) return launch_rows<DT, 64>(a, s);
+  if (a.c.dp == 128) return launch_rows<DT, 128>(a, s);
+  return launch_rows<DT, 256>(a, s);
 }
 
 }  // namespace
 
 int launch_kv4_attend(const Kv4AttendArgs& a, cudaStream_t s) {
-  dim3 grid((unsigned)(a.heads * a.n), (unsigned)a.requests);
-  if (a.dtype == SA_REP_FLOAT32)
-    attend_kernel<SA_REP_FLOAT32><<<grid, kWarps * 32, 0, s>>>(a);
-  else if (a.dtype == SA_REP_FLOAT16)
-    attend_kernel<SA_REP_FLOAT16><<<grid, kWarps * 32, 0, s>>>(a);
-  else
-    attend_kernel<SA_REP_BFLOAT16><<<grid, kWarps * 32, 0, s>>>(a);
-  return check_launch("kv4 attend_kernel");
+  if (a.dtype == SA_REP_FLOAT32) return launch_dim<SA_REP_FLOAT32>(a, s);
+  if (a.dtype == SA_REP_FLOAT16) return launch_dim<SA_REP_FLOAT16>(a, s);
+  return launch_dim<SA_REP_BFLOAT16>(a, s);
 }
 
 }  // namespace sa
