@@ -9,11 +9,15 @@
 // shared memory between (mma.sync m16n8k16: eight query rows fill its n, where
 // a tcgen05 tile would hold 128 rows, nearly all empty).
 //
-// A warp takes blocks of 16 tokens.  With x = scale 8 + least the value of a
-// code is s (code - 8) + x, and code - 8 is exact in bfloat16, so
+// A warp takes blocks of 16 tokens.  A code's bits, moved to the top of a
+// bfloat16's mantissa under the exponent of 16, are 16 + code: a shift and one
+// logical operation for two codes, exact.  With x = least - 16 scale the value is
+// s (16 + code) + x, so
 //   S = s_k (K_codes Q^T) + x_k sum(Q)         tokens x rows
 //   O = V_codes^T (p s_v)^T + sum(p x_v)       columns x rows
-// with scales and offsets in float32 on either side of the products.  Q is
+// with scales and offsets in float32 on either side of the products.  What bounds
+// it beside the bytes is instructions (550 a block at first, taking 8 off each
+// code and choosing by mask everywhere; 301 us where the bytes take 94).  Q is
 // bfloat16 as it is, float16 as two and float32 as three bfloat16 pieces (exact,
 // or to 24 bits); p s_v is split into two pieces (16 bits; three for float32).
 //
@@ -32,6 +36,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "kv4.cuh"
 
@@ -58,12 +63,11 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   return r;
 }
 
-// Two codes (bits 0..3 and 16..19 of w) less 8, as bfloat16: 128 + code by its
-// bits, less 136; both exact.
+// Two codes, nibble i of each half of w, plus 16, as bfloat16.
+template <int I>
 __device__ __forceinline__ uint32_t codes(uint32_t w) {
-  uint32_t x = (w & 0x000f000fu) | 0x43004300u, r;
-  asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(x), "r"(0x3f803f80u), "r"(0xc308c308u));
-  return r;
+  const uint32_t x = I == 0 ? w << 3 : w >> (4 * I - 3);
+  return (x & 0x00780078u) | 0x41804180u;
 }
 
 __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -94,50 +98,88 @@ struct Block {
   uint2 kp, vp;                                       // params of tokens 2 g and 2 g + 1
 };
 
+// Blocks on their way: each lane has a queue of kDepth slots of its own in shared
+// memory, filled by cp.async and read by that lane alone (no barriers).  A slot's
+// pieces of 16 (or 8, 4) bytes lie a warp's width apart.
+constexpr int kDepth = 4;
+
+template <int DP>
+struct Queue {
+  static constexpr int kPiece = DP >= 128 ? 16 : DP / 8;     // bytes of a key row's piece
+  static constexpr int kPieces = (DP / 8) / kPiece;          // pieces of a key row's share
+  static constexpr int kVPiece = DP >= 64 ? 16 : 8;
+  static constexpr int kVPieces = (DP / 4) / kVPiece;
+  static constexpr int kSlot = 32 * (2 * (DP / 8) + DP / 4 + 16);   // bytes of a warp's slot
+};
+
 template <int N>
-__device__ __forceinline__ void load_words(uint32_t (&x)[N], const uint8_t* p) {
-  if constexpr (N % 4 == 0) {
-#pragma unroll
-    for (int i = 0; i < N / 4; ++i) {
-      const uint4 y = __ldg(reinterpret_cast<const uint4*>(p) + i);
-      x[4 * i] = y.x;
-      x[4 * i + 1] = y.y;
-      x[4 * i + 2] = y.z;
-      x[4 * i + 3] = y.w;
-    }
-  } else if constexpr (N == 2) {
-    const uint2 y = __ldg(reinterpret_cast<const uint2*>(p));
+__device__ __forceinline__ void copy_async(uint32_t to, const uint8_t* from) {
+  if constexpr (N == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(to), "l"(from), "n"(N) : "memory");
+}
+
+template <int N>
+__device__ __forceinline__ void take(uint32_t* x, const uint8_t* p) {
+  if constexpr (N == 16) {
+    const uint4 y = *reinterpret_cast<const uint4*>(p);
+    x[0] = y.x;
+    x[1] = y.y;
+    x[2] = y.z;
+    x[3] = y.w;
+  } else if constexpr (N == 8) {
+    const uint2 y = *reinterpret_cast<const uint2*>(p);
     x[0] = y.x;
     x[1] = y.y;
   } else {
-    x[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
+    x[0] = *reinterpret_cast<const uint32_t*>(p);
   }
 }
 
-// cell: index of the block's first token in [pages, heads, page].
+// The addresses of a lane's share of the cache's first block.
+struct Lanes {
+  const uint8_t* k;
+  const uint8_t* v;
+  const uint8_t* kp;
+  const uint8_t* vp;
+};
+
+// off: bytes of codes from there to the block, a multiple of 8 DP (params take
+// off * 8 / DP bytes); slot: the warp's slot, lane: this lane.
 template <int DP>
-__device__ __forceinline__ void load_block(Block<DP>& b, const Kv4Cache& c, int64_t cell, int g, int cc) {
-  const uint8_t* k = c.k_codes + (cell + 2 * g) * (DP / 2) + cc * (DP / 8);
-  load_words(b.k0, k);
-  load_words(b.k1, k + DP / 2);
-  // token group cc of the block; 16-byte pieces of neighbouring lanes g are neighbours
-  const uint8_t* v = c.v_codes + (cell + 4 * cc) * (DP / 2);
-  if constexpr (DP >= 64) {
+__device__ __forceinline__ void send_block(const Lanes& at, int64_t off, uint32_t slot, int lane) {
+  using Q = Queue<DP>;
+  uint32_t to = slot + lane * Q::kPiece;
 #pragma unroll
-    for (int q = 0; q < DP / 64; ++q) {
-      const uint4 y = __ldg(reinterpret_cast<const uint4*>(v + q * 128) + g);
-      b.v[4 * q] = y.x;
-      b.v[4 * q + 1] = y.y;
-      b.v[4 * q + 2] = y.z;
-      b.v[4 * q + 3] = y.w;
-    }
-  } else {
-    const uint2 y = __ldg(reinterpret_cast<const uint2*>(v) + g);
-    b.v[0] = y.x;
-    b.v[1] = y.y;
-  }
-  b.kp = __ldg(reinterpret_cast<const uint2*>(c.k_params + 2 * (cell + 2 * g)));
-  b.vp = __ldg(reinterpret_cast<const uint2*>(c.v_params + 2 * (cell + 2 * g)));
+  for (int row = 0; row < 2; ++row)
+#pragma unroll
+    for (int i = 0; i < Q::kPieces; ++i, to += 32 * Q::kPiece)
+      copy_async<Q::kPiece>(to, at.k + off + row * (DP / 2) + i * Q::kPiece);
+  to = slot + 32 * 2 * (DP / 8) + lane * Q::kVPiece;
+  // 16-byte pieces of neighbouring lanes g are neighbours
+#pragma unroll
+  for (int i = 0; i < Q::kVPieces; ++i, to += 32 * Q::kVPiece) copy_async<Q::kVPiece>(to, at.v + off + i * 128);
+  const int64_t poff = (int64_t)((uint64_t)off / (DP / 8));
+  to = slot + 32 * (2 * (DP / 8) + DP / 4) + lane * 8;
+  copy_async<8>(to, at.kp + poff);
+  copy_async<8>(to + 32 * 8, at.vp + poff);
+}
+
+template <int DP>
+__device__ __forceinline__ void take_block(Block<DP>& b, const uint8_t* slot, int lane) {
+  using Q = Queue<DP>;
+  const uint8_t* from = slot + lane * Q::kPiece;
+#pragma unroll
+  for (int i = 0; i < Q::kPieces; ++i, from += 32 * Q::kPiece) take<Q::kPiece>(b.k0 + i * Q::kPiece / 4, from);
+#pragma unroll
+  for (int i = 0; i < Q::kPieces; ++i, from += 32 * Q::kPiece) take<Q::kPiece>(b.k1 + i * Q::kPiece / 4, from);
+  from = slot + 32 * 2 * (DP / 8) + lane * Q::kVPiece;
+#pragma unroll
+  for (int i = 0; i < Q::kVPieces; ++i, from += 32 * Q::kVPiece) take<Q::kVPiece>(b.v + i * Q::kVPiece / 4, from);
+  from = slot + 32 * (2 * (DP / 8) + DP / 4) + lane * 8;
+  b.kp = *reinterpret_cast<const uint2*>(from);
+  b.vp = *reinterpret_cast<const uint2*>(from + 32 * 8);
 }
 
 // Byte column b of O's tile t (16 columns): lane g holds columns 2 b and 2 b + 1.
@@ -151,11 +193,15 @@ struct Shape {
   static constexpr int kQ = DT == SA_REP_BFLOAT16 ? 1 : (DT == SA_REP_FLOAT16 ? 2 : 3);   // pieces of q
   static constexpr int kP = DT == SA_REP_FLOAT32 ? 3 : 2;                                 // pieces of p s_v
   static constexpr int kRows = 8 * NT;
-  // registers of O, Q and two blocks in a lane: where two CTAs an SM would spill (much), one
-  static constexpr int kHeld = NT * (DP / 4 + kQ * DP / 8) + DP / 4 + 8;
-  static constexpr int kPerSm = kHeld <= 104 ? 2 : 1;
+  // registers of O, Q and a block in a lane: where two CTAs an SM would spill, one
+  static constexpr int kHeld = NT * (DP / 4 + kQ * DP / 8) + DP / 8;
+  static constexpr int kPerSm = kHeld <= 96 ? 2 : 1;
   static constexpr int kPitch = DP + 4;   // a row of O in shared memory
-  static constexpr int kSmem = (kWarps * kRows * kPitch + 2 * kWarps * kRows + 2 * kRows) * 4;
+  // the queues, later the warps' O; then m, l and factors of warps (and CTAs), m, l
+  static constexpr int kQueues = kWarps * kDepth * Queue<DP>::kSlot;
+  static constexpr int kJoin = kWarps * kRows * kPitch * 4;
+  static constexpr int kFirst = kQueues > kJoin ? kQueues : kJoin;
+  static constexpr int kSmem = kFirst + (3 * kWarps * kRows + 2 * kRows) * 4;
 };
 
 template <int DT, int DP, int NT>
@@ -163,11 +209,12 @@ __global__ void __launch_bounds__(kThreads, (Shape<DT, DP, NT>::kPerSm)) attend_
   using T = typename Elem<DT>::T;
   using S = Shape<DT, DP, NT>;
   constexpr int kKS = DP / 16;   // k steps of the first product, 16-column tiles of the second
-  extern __shared__ float smem[];
-  float* sm_o = smem;                                   // [warps][rows][pitch]
-  float* sm_m = smem + kWarps * S::kRows * S::kPitch;   // [warps][rows]
+  extern __shared__ __align__(16) uint8_t smem[];
+  float* sm_o = reinterpret_cast<float*>(smem);                // [warps][rows][pitch]
+  float* sm_m = reinterpret_cast<float*>(smem + S::kFirst);    // [warps][rows]
   float* sm_l = sm_m + kWarps * S::kRows;
-  float* part_m = sm_l + kWarps * S::kRows;             // [rows]: this CTA's
+  float* sm_f = sm_l + kWarps * S::kRows;
+  float* part_m = sm_f + kWarps * S::kRows;                    // [rows]: this CTA's
   float* part_l = part_m + S::kRows;
 
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -265,17 +312,37 @@ __global__ void __launch_bounds__(kThreads, (Shape<DT, DP, NT>::kPerSm)) attend_
     }
   };
   const int page_mask = (1 << a.c.page_shift) - 1;
-  auto load = [&](Block<DP>& b, int u) -> bool {   // false: nothing there
-    if (u >= mine) return false;
-    if ((u & 31) == 0) fetch_pages(u);
-    const int page = __shfl_sync(0xffffffffu, page_of, u & 31);
-    if (page < 0) return false;
-    const int64_t cell = (((int64_t)page * a.c.heads + hk) << a.c.page_shift) + (token_of(u) & page_mask);
-    load_block(b, a.c, cell, g, cc);
-    return true;
+  const int page_step = a.c.heads << a.c.page_shift;   // cells of a page, all heads
+  const int64_t cell0 = (int64_t)hk << a.c.page_shift;
+  const Lanes at{a.c.k_codes + (cell0 + 2 * g) * (DP / 2) + cc * (DP / 8),
+                 a.c.v_codes + (cell0 + 4 * cc) * (DP / 2) + g * (DP >= 64 ? 16 : 8),
+                 reinterpret_cast<const uint8_t*>(a.c.k_params + 2 * (cell0 + 2 * g)),
+                 reinterpret_cast<const uint8_t*>(a.c.v_params + 2 * (cell0 + 2 * g))};
+  uint8_t* queue = smem + warp * kDepth * Queue<DP>::kSlot;
+  const uint32_t queue_u32 = static_cast<uint32_t>(__cvta_generic_to_shared(queue));
+  uint32_t sent = 0;   // bit of a slot: a block is in it
+  auto send = [&](int u) {
+    const int slot = u % kDepth;
+    sent &= ~(1u << slot);
+    if (u < mine) {
+      if ((u & 31) == 0) fetch_pages(u);
+      const int page = __shfl_sync(0xffffffffu, page_of, u & 31);
+      if (page >= 0) {
+        send_block<DP>(at, ((int64_t)page * page_step + (token_of(u) & page_mask)) * (DP / 2),
+                       queue_u32 + slot * Queue<DP>::kSlot, lane);
+        sent |= 1u << slot;
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
   };
 
-  auto work = [&](const Block<DP>& b, int token) {
+  // off: what is added to a score before 2^x; the maximum is moved where a score passes kMove + kShift
+  float off[NT][2];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) off[nt][0] = off[nt][1] = INFINITY;   // no maximum yet: the first score moves it
+
+  auto work = [&](const Block<DP>& b, int token, auto whole) {
+    constexpr bool kWhole = decltype(whole)::value;   // every row sees the whole block
     float s[NT][4];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
@@ -283,25 +350,21 @@ __global__ void __launch_bounds__(kThreads, (Shape<DT, DP, NT>::kPerSm)) attend_
       for (int e = 0; e < 4; ++e) s[nt][e] = 0.0f;
 #pragma unroll
     for (int w = 0; w < kKS / 2; ++w) {
+      uint32_t f[2][4] = {{codes<0>(b.k0[w]), codes<0>(b.k1[w]), codes<1>(b.k0[w]), codes<1>(b.k1[w])},
+                          {codes<2>(b.k0[w]), codes<2>(b.k1[w]), codes<3>(b.k0[w]), codes<3>(b.k1[w])}};
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const uint32_t a0 = codes(b.k0[w] >> (8 * half)), a1 = codes(b.k1[w] >> (8 * half));
-        const uint32_t a2 = codes(b.k0[w] >> (8 * half + 4)), a3 = codes(b.k1[w] >> (8 * half + 4));
+      for (int half = 0; half < 2; ++half)
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int q = 0; q < S::kQ; ++q)
-            mma(s[nt], a0, a1, a2, a3, qf[nt][q][2 * w + half][0], qf[nt][q][2 * w + half][1]);
-      }
+            mma(s[nt], f[half][0], f[half][1], f[half][2], f[half][3], qf[nt][q][2 * w + half][0], qf[nt][q][2 * w + half][1]);
     }
     const float2 ka = params(b.kp.x), kb = params(b.kp.y), va = params(b.vp.x), vb = params(b.vp.y);
-    const float k_s[2] = {ka.x * sc, kb.x * sc}, k_x[2] = {fmaf(8.0f, ka.x, ka.y) * sc, fmaf(8.0f, kb.x, kb.y) * sc};
-    const float v_s[2] = {va.x, vb.x}, v_x[2] = {fmaf(8.0f, va.x, va.y), fmaf(8.0f, vb.x, vb.y)};
-    // every row sees the whole block
-    const bool all_on = token + 15 <= p_lo && (token > p_hi - window || token + 16 <= sinks);
-    uint32_t on = 0xffffffffu;   // bit 4 nt + e: s[nt][e]
-    if (!all_on) {
-      on = 0;
+    const float k_s[2] = {ka.x * sc, kb.x * sc}, k_x[2] = {fmaf(-16.0f, ka.x, ka.y) * sc, fmaf(-16.0f, kb.x, kb.y) * sc};
+    const float v_s[2] = {va.x, vb.x}, v_x[2] = {fmaf(-16.0f, va.x, va.y), fmaf(-16.0f, vb.x, vb.y)};
+    uint32_t on = 0;   // bit 4 nt + e: s[nt][e] is seen
+    if (!kWhole) {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -315,9 +378,9 @@ __global__ void __launch_bounds__(kThreads, (Shape<DT, DP, NT>::kPerSm)) attend_
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const float x = fmaf(k_s[e >> 1], s[nt][e], k_x[e >> 1] * qsum[nt][e & 1]);
-        s[nt][e] = (on >> (4 * nt + e)) & 1u ? x : -INFINITY;
-        move |= s[nt][e] > m[nt][e & 1] + kMove;
+        s[nt][e] = fmaf(k_s[e >> 1], s[nt][e], k_x[e >> 1] * qsum[nt][e & 1]);
+        if (!kWhole) s[nt][e] = (on >> (4 * nt + e)) & 1u ? s[nt][e] : -INFINITY;
+        move |= s[nt][e] + off[nt][e & 1] > kMove + kShift;
       }
     if (__any_sync(0xffffffffu, move)) {
 #pragma unroll
@@ -330,6 +393,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<DT, DP, NT>::kPerSm)) attend_
           if (top > m[nt][e] + kMove) {
             const float alpha = ex2(m[nt][e] - top);   // from -inf: 0
             m[nt][e] = top;
+            off[nt][e] = kShift - top;
             l[nt][e] *= alpha;
             z[nt][e] *= alpha;
 #pragma unroll
@@ -346,9 +410,9 @@ __global__ void __launch_bounds__(kThreads, (Shape<DT, DP, NT>::kPerSm)) attend_
       float ps[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const float mm = m[nt][e & 1] == -INFINITY ? 0.0f : m[nt][e & 1];
-        const float p = ex2(s[nt][e] - mm + kShift);
-        const bool seen = (on >> (4 * nt + e)) & 1u;   // hidden tokens' scales may be anything
+        // without a maximum yet nothing has been seen: every score is -inf (or NaN)
+        const float p = ex2(kWhole || m[nt][e & 1] != -INFINITY ? s[nt][e] + off[nt][e & 1] : s[nt][e]);
+        const bool seen = kWhole || ((on >> (4 * nt + e)) & 1u);   // hidden tokens' scales may be anything
         l[nt][e & 1] += p;
         z[nt][e & 1] = seen ? fmaf(p, v_x[e >> 1], z[nt][e & 1]) : z[nt][e & 1];
         ps[e] = seen ? p * v_s[e >> 1] : 0.0f;
@@ -369,24 +433,32 @@ __global__ void __launch_bounds__(kThreads, (Shape<DT, DP, NT>::kPerSm)) attend_
 #pragma unroll
     for (int t = 0; t < kKS; ++t) {
       const uint32_t w = b.v[t];
-      const uint32_t a0 = codes(w), a1 = codes(w >> 4), a2 = codes(w >> 8), a3 = codes(w >> 12);
+      const uint32_t a0 = codes<0>(w), a1 = codes<1>(w), a2 = codes<2>(w), a3 = codes<3>(w);
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int q = 0; q < S::kP; ++q) mma(o[nt][t], a0, a1, a2, a3, pf[nt][q][0], pf[nt][q][1]);
     }
   };
+  auto go = [&](const Block<DP>& b, int token) {
+    if (token + 15 <= p_lo && (token > p_hi - window || token + 16 <= sinks))
+      work(b, token, std::true_type{});
+    else
+      work(b, token, std::false_type{});
+  };
 
-  {
-    Block<DP> b0, b1;
-    bool in0 = load(b0, 0);
-    for (int u = 0; u < mine; u += 2) {
-      const bool in1 = load(b1, u + 1);
-      if (in0) work(b0, token_of(u));
-      in0 = load(b0, u + 2);
-      if (in1) work(b1, token_of(u + 1));
+  for (int u = 0; u < kDepth - 1; ++u) send(u);
+  for (int u = 0; u < mine; ++u) {
+    send(u + kDepth - 1);
+    asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 1) : "memory");
+    if ((sent >> (u % kDepth)) & 1u) {
+      Block<DP> b;
+      take_block<DP>(b, queue + (u % kDepth) * Queue<DP>::kSlot, lane);
+      go(b, token_of(u));
     }
   }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  __syncthreads();   // the queues' memory takes the outputs
 
   // join the warps
 #pragma unroll
@@ -412,25 +484,36 @@ __global__ void __launch_bounds__(kThreads, (Shape<DT, DP, NT>::kPerSm)) attend_
       }
     }
   __syncthreads();
-  // warp 0's place takes the CTA's: each thread a (row, column), warps in order
-  for (int x = threadIdx.x; x < S::kRows * DP; x += kThreads) {
-    const int row = x / DP, col = x - row * DP;
-    float top = -INFINITY;
+  if (threadIdx.x < S::kRows) {   // what each warp's sums count for
+    const int row = threadIdx.x;
+    float top = -INFINITY, total = 0.0f;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) top = fmaxf(top, sm_m[w * S::kRows + row]);
-    float sum = 0.0f, total = 0.0f;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
       const float mw = sm_m[w * S::kRows + row];
       const float f = mw == -INFINITY ? 0.0f : ex2(mw - top);
-      sum = fmaf(f, sm_o[(w * S::kRows + row) * S::kPitch + col], sum);
+      sm_f[w * S::kRows + row] = f;
       total = fmaf(f, sm_l[w * S::kRows + row], total);
     }
-    sm_o[row * S::kPitch + col] = sum;
-    if (col == 0) {
-      part_m[row] = top;
-      part_l[row] = total;
+    part_m[row] = top;
+    part_l[row] = total;
+  }
+  __syncthreads();
+  // warp 0's place takes the CTA's: each thread a row's four columns, warps in order
+  for (int x = threadIdx.x; x < S::kRows * DP / 4; x += kThreads) {
+    const int row = x / (DP / 4), col = (x - row * (DP / 4)) * 4;
+    float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const float f = sm_f[w * S::kRows + row];
+      const float4 y = *reinterpret_cast<const float4*>(sm_o + (w * S::kRows + row) * S::kPitch + col);
+      sum.x = fmaf(f, y.x, sum.x);
+      sum.y = fmaf(f, y.y, sum.y);
+      sum.z = fmaf(f, y.z, sum.z);
+      sum.w = fmaf(f, y.w, sum.w);
     }
+    *reinterpret_cast<float4*>(sm_o + row * S::kPitch + col) = sum;
   }
   cg::cluster_group cluster = cg::this_cluster();
   if (splits > 1)
