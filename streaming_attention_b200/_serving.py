@@ -21,12 +21,13 @@ MAX_DIM = 256
 def dtype_code(*ts: Tensor) -> int:
     """The SA_REP_* code of the tensors' one element type."""
     dt = ts[0].dtype
-    if dt not in DTYPES:
+    code = DTYPES.get(dt)
+    if code is None:
         raise ValueError(f"unsupported dtype {dt}: float32, float16 and bfloat16 are accepted")
     for t in ts[1:]:
         if t.dtype != dt:
             raise ValueError(f"all inputs must have one dtype, got {dt} and {t.dtype}")
-    return DTYPES[dt]
+    return code
 
 
 def device_of(*ts: Tensor) -> torch.device:
@@ -44,18 +45,21 @@ def int32(t: Tensor, shape: Tuple[int, ...], what: str) -> Tensor:
     """Checks a contiguous int32 index tensor of the given shape."""
     if t.dtype != torch.int32:
         raise ValueError(f"{what} must be int32, got {t.dtype}")
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise ValueError(f"{what} must have shape {list(shape)}, got {list(t.shape)}")
-    return t.contiguous()
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def rows(t: Tensor) -> Tensor:
     """t, or a copy of it, with a contiguous last dimension."""
-    return t if t.shape[-1] <= 1 or t.stride(-1) == 1 else t.contiguous()
+    return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.detach().contiguous()
+
+
+_ARRAYS = {n: ctypes.c_int64 * n for n in (3, 4, 8, 12)}
 
 
 def strides(*values: int):
-    return (ctypes.c_int64 * len(values))(*values)
+    return _ARRAYS[len(values)](*values)
 
 
 def ptr(t: Optional[Tensor]) -> Optional[int]:
@@ -71,6 +75,14 @@ def check_window(window: Optional[int], sinks: int) -> Tuple[int, int]:
     return (0 if window is None else int(window)), int(sinks)
 
 
+def _raw_stream(index: int) -> int:
+    return torch.cuda.current_stream(index).cuda_stream
+
+
+# the current stream's handle without a Stream object around it (2 us a call), where torch has it
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _raw_stream)
+
+
 def launch(dev: torch.device, name: str, *args) -> None:
     """Calls a serving entry point on the current stream of `dev`."""
     if dev.index == torch.cuda.current_device():
@@ -81,8 +93,7 @@ def launch(dev: torch.device, name: str, *args) -> None:
 
 
 def _launch(dev: torch.device, name: str, args) -> None:
-    lib = _lib.load()
-    rc = getattr(lib, name)(*args, torch.cuda.current_stream(dev).cuda_stream)
+    rc = getattr(_lib.load(), name)(*args, _raw_stream(dev.index))
     if rc:
         _lib.check(rc, name)
     if _fast._CHECK_STATUS and not torch.cuda.is_current_stream_capturing():

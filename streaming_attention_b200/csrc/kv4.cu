@@ -139,9 +139,205 @@ __global__ void __launch_bounds__(kThreads) read_kernel(const Kv4ReadArgs a) {
   }
 }
 
+// Rows on 16-byte borders of widths that are multiples of 8: a lane holds eight
+// columns (four bytes of codes), 1 << LOG lanes a row, and takes four neighbouring
+// tokens t0 .. t0 + 3 of one head.  Keys: each row's bytes are contiguous.
+// Values: where four tokens fill a word group of the cache (slots 4 m .. 4 m + 3),
+// the lane that finds the first of them among its own transposes their bytes
+// and stores 16 at once; its neighbours leave those tokens to it.  Other tokens
+// store single bytes.
+template <int DT, int LOG>
+__global__ void __launch_bounds__(kThreads) append_vec_kernel(const Kv4AppendArgs a) {
+  using T = typename Elem<DT>::T;
+  constexpr int kLanes = 1 << LOG;
+  const int lane = threadIdx.x & 31, li = lane & (kLanes - 1);
+  int64_t item = ((int64_t)blockIdx.x * kThreads + threadIdx.x) >> LOG;   // (k or v, quad of tokens, head)
+  const int64_t items = ((a.tokens + 3) >> 2) * a.c.heads;
+  const bool isv = item >= items;
+  if (isv) item -= items;
+  const int h = (int)(item % a.c.heads);
+  const int64_t t0 = item < items ? (item / a.c.heads) * 4 : a.tokens;
+  const int c0 = li * 8, bytes = a.c.dp >> 1, page_mask = (1 << a.c.page_shift) - 1;
+  const bool in = c0 < a.c.d;
+  auto slot_of = [&](int64_t t) -> int { return t >= 0 && t < a.tokens ? __ldg(a.slots + t) : -1; };
+  // opens(t): tokens t .. t + 3 fill a word group
+  auto opens = [&](int64_t t) {
+    const int s = slot_of(t);
+    return s >= 0 && (s & 3) == 0 && (s >> a.c.page_shift) < a.c.pages && slot_of(t + 1) == s + 1 && slot_of(t + 2) == s + 2 &&
+           slot_of(t + 3) == s + 3;
+  };
+  int64_t from = t0;     // the group this lane stores whole: tokens from .. from + 3
+  bool whole = false;
+  int taken = 0;         // bit i: token t0 + i belongs to a group
+  if (isv) {
+#pragma unroll
+    for (int i = -3; i < 4; ++i)
+      if (opens(t0 + i)) {
+        if (i >= 0) {
+          whole = true;
+          from = t0 + i;
+        }
+        taken |= i >= 0 ? 15 << i : 15 >> -i;
+      }
+  }
+  // codes of token t, as four bytes, and its params
+  auto code_row = [&](int64_t t, __nv_bfloat162& sm) -> uint32_t {
+    float x[8];
+    const bool here = in && t < a.tokens;
+    if (here)
+      load8(x, (isv ? static_cast<const T*>(a.v) + t * a.v_t + h * a.v_h : static_cast<const T*>(a.k) + t * a.k_t + h * a.k_h) + c0);
+    float lo = INFINITY, hi = -INFINITY;
+    bool bad = false;
+    if (here)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        bad |= !(fabsf(x[e]) < INFINITY);
+        lo = fminf(lo, x[e]);
+        hi = fmaxf(hi, x[e]);
+      }
+    if (bad) lo = -INFINITY, hi = INFINITY;   // spreads to the row
+#pragma unroll
+    for (int d = 1; d < kLanes; d *= 2) {
+      lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, d));
+      hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, d));
+    }
+    sm.x = __float2bfloat16_rn((float)(((double)hi - (double)lo) / 15.0));
+    sm.y = __float2bfloat16_rn(lo);
+    if (!(fabsf(__bfloat162float(sm.y)) < INFINITY)) sm.x = sm.y = __float2bfloat16_rn(NAN);
+    const float scale = __bfloat162float(sm.x), least = __bfloat162float(sm.y);
+    uint32_t w = 0;
+    if (here)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) w |= code_of(x[e], least, scale) << (4 * e);
+    return w;
+  };
+  // single tokens (every key; values outside whole groups)
+#pragma unroll 1
+  for (int i = 0; i < 4; ++i) {
+    const int64_t t = t0 + i;
+    const int slot = slot_of(t);
+    bool put = slot >= 0 && !((taken >> i) & 1);
+    if (put && (slot >> a.c.page_shift) >= a.c.pages) {
+      if (li == 0) report(a.status, kBadSlot, t);
+      put = false;
+    }
+    if (!__any_sync(0xffffffffu, put)) continue;
+    __nv_bfloat162 sm;
+    const uint32_t w = code_row(t, sm);
+    if (!put) continue;
+    const int64_t cell = (((int64_t)(slot >> a.c.page_shift) * a.c.heads + h) << a.c.page_shift);
+    const int off = slot & page_mask;
+    if (li == 0) *reinterpret_cast<__nv_bfloat162*>((isv ? a.c.v_params : a.c.k_params) + 2 * (cell + off)) = sm;
+    if (c0 >= a.c.dp) continue;
+    if (!isv) {
+      *reinterpret_cast<uint32_t*>(a.c.k_codes + (cell + off) * bytes + li * 4) = w;
+    } else {
+      uint8_t* to = a.c.v_codes + cell * bytes + ((int64_t)(off >> 2) * bytes + li * 4) * 4 + (off & 3);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) to[4 * e] = (uint8_t)(w >> (8 * e));
+    }
+  }
+  if (__any_sync(0xffffffffu, whole)) {
+    uint32_t w[4], sm[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      __nv_bfloat162 x;
+      w[i] = code_row(from + i, x);
+      sm[i] = *reinterpret_cast<const uint32_t*>(&x);
+    }
+    if (whole) {
+      const int slot = slot_of(from);
+      const int64_t cell = (((int64_t)(slot >> a.c.page_shift) * a.c.heads + h) << a.c.page_shift) + (slot & page_mask);
+      if (li == 0) *reinterpret_cast<uint4*>(a.c.v_params + 2 * cell) = make_uint4(sm[0], sm[1], sm[2], sm[3]);
+      // byte e of the four words side by side
+      const uint32_t l0 = __byte_perm(w[0], w[1], 0x5140), h0 = __byte_perm(w[2], w[3], 0x5140);
+      const uint32_t l1 = __byte_perm(w[0], w[1], 0x7362), h1 = __byte_perm(w[2], w[3], 0x7362);
+      if (c0 < a.c.dp)
+        *reinterpret_cast<uint4*>(a.c.v_codes + cell * bytes + li * 16) =
+            make_uint4(__byte_perm(l0, h0, 0x5410), __byte_perm(l0, h0, 0x7632), __byte_perm(l1, h1, 0x5410),
+                       __byte_perm(l1, h1, 0x7632));
+    }
+  }
+}
+
+// 1 << LOG lanes a row, eight columns a lane.
+template <int DT, int LOG>
+__global__ void __launch_bounds__(kThreads) read_vec_kernel(const Kv4ReadArgs a) {
+  using T = typename Elem<DT>::T;
+  const int lane = threadIdx.x & 31, li = lane & ((1 << LOG) - 1);
+  const int64_t row = ((int64_t)blockIdx.x * kThreads + threadIdx.x) >> LOG;
+  if (row >= a.tokens * a.c.heads * 2 || li * 8 >= a.c.d) return;
+  // k's rows, then v's: neighbouring groups write neighbouring rows
+  const bool isv = row >= a.tokens * a.c.heads;
+  const int64_t u = isv ? row - a.tokens * a.c.heads : row;
+  const int h = (int)(u % a.c.heads);
+  const int64_t t = u / a.c.heads;
+  const int slot = __ldg(a.slots + t);
+  T* o = static_cast<T*>(isv ? a.v : a.k) + u * a.c.d + li * 8;
+  const int bytes = a.c.dp >> 1;
+  float x[8];
+  if (slot < 0 || (slot >> a.c.page_shift) >= a.c.pages) {
+    if (slot >= 0 && li == 0) report(a.status, kBadSlot, t);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = 0.0f;
+  } else {
+    const int off = slot & ((1 << a.c.page_shift) - 1);
+    const int64_t cell = (((int64_t)(slot >> a.c.page_shift) * a.c.heads + h) << a.c.page_shift);
+    const uint32_t p = *reinterpret_cast<const uint32_t*>((isv ? a.c.v_params : a.c.k_params) + 2 * (cell + off));
+    const float scale = __uint_as_float(p << 16), least = __uint_as_float(p & 0xffff0000u);
+    uint32_t w;
+    if (!isv) {
+      w = *reinterpret_cast<const uint32_t*>(a.c.k_codes + (cell + off) * bytes + li * 4);
+    } else {
+      // four columns' words of four tokens: this token's byte of each
+      const uint4 y = *reinterpret_cast<const uint4*>(a.c.v_codes + cell * bytes + ((int64_t)(off >> 2) * bytes + li * 4) * 4);
+      const int sel = (off & 3) | (((off & 3) + 4) << 4);
+      w = __byte_perm(__byte_perm(y.x, y.y, sel), __byte_perm(y.z, y.w, sel), 0x5410);
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = fmaf((float)((w >> (4 * e)) & 15u), scale, least);
+  }
+  store8(o, x);
+}
+
+// log2 of the lanes that hold a row of dp columns, eight each.
+int row_lanes_log(int dp) { return dp == 32 ? 2 : (dp == 64 ? 3 : (dp == 128 ? 4 : 5)); }
+
+template <int DT>
+int append_vec(const Kv4AppendArgs& a, cudaStream_t s) {
+  const int log = row_lanes_log(a.c.dp);
+  const int64_t ctas = ceil_div((((a.tokens + 3) >> 2) * a.c.heads * 2) << log, kThreads);
+  if (ctas > 2147483647LL) return set_error(SA_ERR_UNSUPPORTED, "kv4 append: too many rows");
+  const unsigned g = (unsigned)ctas;
+  if (log == 2) append_vec_kernel<DT, 2><<<g, kThreads, 0, s>>>(a);
+  else if (log == 3) append_vec_kernel<DT, 3><<<g, kThreads, 0, s>>>(a);
+  else if (log == 4) append_vec_kernel<DT, 4><<<g, kThreads, 0, s>>>(a);
+  else append_vec_kernel<DT, 5><<<g, kThreads, 0, s>>>(a);
+  return check_launch("kv4 append_vec_kernel");
+}
+
+template <int DT>
+int read_vec(const Kv4ReadArgs& a, cudaStream_t s) {
+  const int log = row_lanes_log(a.c.dp);
+  const int64_t ctas = ceil_div((a.tokens * a.c.heads * 2) << log, kThreads);
+  if (ctas > 2147483647LL) return set_error(SA_ERR_UNSUPPORTED, "kv4 read: too many rows");
+  const unsigned g = (unsigned)ctas;
+  if (log == 2) read_vec_kernel<DT, 2><<<g, kThreads, 0, s>>>(a);
+  else if (log == 3) read_vec_kernel<DT, 3><<<g, kThreads, 0, s>>>(a);
+  else if (log == 4) read_vec_kernel<DT, 4><<<g, kThreads, 0, s>>>(a);
+  else read_vec_kernel<DT, 5><<<g, kThreads, 0, s>>>(a);
+  return check_launch("kv4 read_vec_kernel");
+}
+
 }  // namespace
 
 int launch_kv4_append(const Kv4AppendArgs& a, int dtype, cudaStream_t s) {
+  const int elem = elem_size(dtype);
+  if (a.c.d % 8 == 0 && rows_aligned(a.k, elem, a.k_t, a.k_h) && rows_aligned(a.v, elem, a.v_t, a.v_h)) {
+    if (dtype == SA_REP_FLOAT32) return append_vec<SA_REP_FLOAT32>(a, s);
+    if (dtype == SA_REP_FLOAT16) return append_vec<SA_REP_FLOAT16>(a, s);
+    return append_vec<SA_REP_BFLOAT16>(a, s);
+  }
   const int64_t ctas = ceil_div(a.tokens * a.c.heads * 2, kThreads / 32);
   if (ctas > 2147483647LL) return set_error(SA_ERR_UNSUPPORTED, "kv4 append: too many rows");
   if (dtype == SA_REP_FLOAT32)
@@ -154,6 +350,11 @@ int launch_kv4_append(const Kv4AppendArgs& a, int dtype, cudaStream_t s) {
 }
 
 int launch_kv4_read(const Kv4ReadArgs& a, int dtype, cudaStream_t s) {
+  if (a.c.d % 8 == 0 && (((uintptr_t)a.k | (uintptr_t)a.v) & 15) == 0) {
+    if (dtype == SA_REP_FLOAT32) return read_vec<SA_REP_FLOAT32>(a, s);
+    if (dtype == SA_REP_FLOAT16) return read_vec<SA_REP_FLOAT16>(a, s);
+    return read_vec<SA_REP_BFLOAT16>(a, s);
+  }
   const int64_t ctas = ceil_div(a.tokens * a.c.heads * 2, kThreads / 32);
   if (ctas > 2147483647LL) return set_error(SA_ERR_UNSUPPORTED, "kv4 read: too many rows");
   if (dtype == SA_REP_FLOAT32)

@@ -59,6 +59,42 @@ __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) {
   return __float2bfloat16_rn(x);
 }
 
+// Eight elements of a row, 16-byte aligned (32 bytes of float32).
+template <typename T>
+__device__ __forceinline__ void load8(float (&x)[8], const T* p) {
+  if constexpr (sizeof(T) == 4) {
+    const float4 a = *reinterpret_cast<const float4*>(p), b = *(reinterpret_cast<const float4*>(p) + 1);
+    x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+  } else {
+    union {
+      uint4 w;
+      T e[8];
+    } u;
+    u.w = *reinterpret_cast<const uint4*>(p);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = to_f32(u.e[i]);
+  }
+}
+template <typename T>
+__device__ __forceinline__ void store8(T* p, const float (&x)[8]) {
+  if constexpr (sizeof(T) == 4) {
+    *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
+    *(reinterpret_cast<float4*>(p) + 1) = make_float4(x[4], x[5], x[6], x[7]);
+  } else {
+    union {
+      uint4 w;
+      T e[8];
+    } u;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) u.e[i] = from_f32<T>(x[i]);
+    *reinterpret_cast<uint4*>(p) = u.w;
+  }
+}
+// Whether every row of a tensor with these strides starts on a 16-byte border.
+__host__ inline bool rows_aligned(const void* p, int elem, int64_t s0, int64_t s1) {
+  return (((uintptr_t)p | (uintptr_t)(s0 * elem) | (uintptr_t)(s1 * elem)) & 15) == 0;
+}
+
 __host__ inline int elem_size(int dtype) { return dtype == SA_REP_FLOAT32 ? 4 : 2; }
 
 // What the window kernels take.  Strides are in elements.  Dense: request b's

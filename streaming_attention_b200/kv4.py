@@ -19,8 +19,7 @@ scale and a least value in bfloat16 (layout in include/streaming_attention.h):
 from __future__ import annotations
 
 import math
-from dataclasses import dataclass
-from typing import Optional, Tuple
+from typing import NamedTuple, Optional, Tuple
 
 import torch
 
@@ -38,8 +37,7 @@ def _check_page_size(page_size: int) -> None:
         raise ValueError(f"page_size must be one of {PAGE_SIZES}, got {page_size}")
 
 
-@dataclass(frozen=True)
-class PagePlan:
+class PagePlan(NamedTuple):
     """What ``plan_kv_pages`` gives: the lengths with the new tokens, the packed
     new tokens' first rows per request [R+1], each row's position and slot (-1
     where no token stands), the page tables and how many pages stay free [1]."""
@@ -51,7 +49,6 @@ class PagePlan:
     free_count: Tensor
 
 
-@torch.no_grad()
 def plan_kv_pages(lengths: Tensor, new: Tensor, tables: Tensor, free_pages: Tensor, free_count: Tensor, *,
                   page_size: int, max_tokens: Optional[int] = None, per_request: Optional[int] = None) -> PagePlan:
     """Makes room for ``new[r]`` tokens of each request behind its ``lengths[r]``
@@ -72,7 +69,7 @@ def plan_kv_pages(lengths: Tensor, new: Tensor, tables: Tensor, free_pages: Tens
     new = S.int32(new, (r,), "new")
     if free_pages.ndim != 1:
         raise ValueError("free_pages must be [F]")
-    free_pages = S.int32(free_pages, tuple(free_pages.shape), "free_pages")
+    free_pages = S.int32(free_pages, free_pages.shape, "free_pages")
     free_count = S.int32(free_count, (1,), "free_count")
     if (max_tokens is None) == (per_request is None):
         raise ValueError("give either max_tokens or per_request")
@@ -82,18 +79,15 @@ def plan_kv_pages(lengths: Tensor, new: Tensor, tables: Tensor, free_pages: Tens
         max_tokens = r * per_request
     elif max_tokens < 0:
         raise ValueError("max_tokens must be non-negative")
-    # one allocation for the outputs, each starting at a multiple of 16 bytes
-    up = lambda x: (x + 3) & ~3  # noqa: E731
-    sizes = (r, r + 1, max_tokens, max_tokens, 1)
-    lens, offsets, positions, slots, free = torch.empty(
-        sum(up(x) for x in sizes), device=dev, dtype=torch.int32).split([up(x) for x in sizes])
+    # one allocation for the outputs
+    lens, offsets, positions, slots, free = lengths.new_empty(2 * r + 2 + 2 * max_tokens).split(
+        (r, r + 1, max_tokens, max_tokens, 1))
     S.launch(dev, "sa_plan_kv_pages", lengths.data_ptr(), new.data_ptr(), tables.data_ptr(), free_pages.data_ptr(),
              free_count.data_ptr(), r, width, free_pages.shape[0], page_size, max_tokens, per_request or 0, lens.data_ptr(),
              offsets.data_ptr(), positions.data_ptr(), slots.data_ptr(), free.data_ptr())
-    return PagePlan(lens[:r], offsets[:r + 1], positions[:max_tokens], slots[:max_tokens], tables, free[:1])
+    return PagePlan(lens, offsets, positions, slots, tables, free)
 
 
-@torch.no_grad()
 def release_kv_pages(lengths: Tensor, tables: Tensor, drop: Tensor, free_pages: Tensor, free_count: Tensor, *,
                      page_size: int) -> None:
     """Ends the requests with ``drop[r]`` (bool [R]): their pages go back to the
@@ -108,7 +102,7 @@ def release_kv_pages(lengths: Tensor, tables: Tensor, drop: Tensor, free_pages: 
         raise ValueError(f"drop must be bool [{r}]")
     S.int32(lengths, (r,), "lengths")
     S.int32(tables, (r, width), "tables")
-    S.int32(free_pages, tuple(free_pages.shape), "free_pages")
+    S.int32(free_pages, free_pages.shape, "free_pages")
     S.int32(free_count, (1,), "free_count")
     for t in (lengths, tables, free_pages, free_count):
         if not t.is_contiguous():
@@ -167,7 +161,6 @@ class Kv4Cache:
                    torch.zeros((num_pages, kv_heads, page_size // 4, half, 4), **u8),
                    torch.zeros((num_pages, kv_heads, page_size, 2), **b16), dim)
 
-    @torch.no_grad()
     def append(self, k: Tensor, v: Tensor, slots: Tensor) -> None:
         """Quantises k and v [T,Hkv,D] into ``slots`` (int32 [T]); a negative slot
         leaves its token out, and no slot may be given twice in one call."""
@@ -182,7 +175,6 @@ class Kv4Cache:
         S.launch(self.device, "sa_kv4_append", *self._args, k.data_ptr(), v.data_ptr(),
                  S.strides(*k.stride()[:2], *v.stride()[:2]), slots.data_ptr(), k.shape[0], code)
 
-    @torch.no_grad()
     def read(self, slots: Tensor, dtype: torch.dtype = torch.float32) -> Tuple[Tensor, Tensor]:
         """The keys and values [T,Hkv,D] that ``slots`` (int32 [T]) stand for, in
         ``dtype``; zeros for a negative slot."""
@@ -191,7 +183,7 @@ class Kv4Cache:
             raise ValueError(f"unsupported dtype {dtype}: float32, float16 and bfloat16 are accepted")
         if slots.ndim != 1:
             raise ValueError("slots must be [T]")
-        slots = S.int32(slots, tuple(slots.shape), "slots")
+        slots = S.int32(slots, slots.shape, "slots")
         t = slots.shape[0]
         k = torch.empty((t, self.kv_heads, self.dim), device=self.device, dtype=dtype)
         v = torch.empty((t, self.kv_heads, self.dim), device=self.device, dtype=dtype)
@@ -200,7 +192,6 @@ class Kv4Cache:
                      S.DTYPES[dtype])
         return k, v
 
-    @torch.no_grad()
     def attend(self, q: Tensor, tables: Tensor, lengths: Tensor, *, window: Optional[int] = None, sinks: int = 0,
                scale: Optional[float] = None) -> Tensor:
         """Attention of each request's newest tokens over its cached ones.
@@ -221,7 +212,7 @@ class Kv4Cache:
             raise ValueError(f"q must have head width {self.dim} and a multiple of {self.kv_heads} heads")
         if tables.ndim != 2 or tables.shape[0] != r:
             raise ValueError(f"tables must be [{r},W]")
-        tables = S.int32(tables, tuple(tables.shape), "tables")
+        tables = S.int32(tables, tables.shape, "tables")
         lengths = S.int32(lengths, (r,), "lengths")
         out = torch.empty((r, n, heads, d), device=self.device, dtype=q.dtype)
         if out.numel():

@@ -30,7 +30,6 @@ def rotary_frequencies(dim: int, *, base: float = 10000.0, device=None) -> Tenso
     return base ** (-2.0 * i / max(dim, 1))
 
 
-@torch.no_grad()
 def qk_norm_rotary(q: Tensor, k: Tensor, positions: Tensor, q_weight: Optional[Tensor], k_weight: Optional[Tensor],
                    frequencies: Tensor, *, eps: float = 1e-6, interleaved: bool = False,
                    out: Optional[Tuple[Tensor, Tensor]] = None) -> Tuple[Tensor, Tensor]:
@@ -50,8 +49,9 @@ def qk_norm_rotary(q: Tensor, k: Tensor, positions: Tensor, q_weight: Optional[T
     code = S.dtype_code(q, k, *given)
     if not 1 <= d <= S.MAX_DIM:
         raise ValueError(f"the head width must lie in [1, {S.MAX_DIM}]")
-    if any(tuple(x.shape) != (d,) for x in given):
-        raise ValueError(f"q_weight and k_weight must be [{d}]")
+    for w in given:
+        if w.shape != (d,):
+            raise ValueError(f"q_weight and k_weight must be [{d}]")
     if heads + kv_heads == 0:
         raise ValueError("at least one head is needed")
     if frequencies.dtype != torch.float64 or frequencies.ndim != 1 or 2 * frequencies.shape[0] > d:
@@ -59,11 +59,11 @@ def qk_norm_rotary(q: Tensor, k: Tensor, positions: Tensor, q_weight: Optional[T
     positions = S.int32(positions, (t,), "positions")
     fresh = out is None
     if fresh:
-        out = (torch.empty((t, heads, d), device=dev, dtype=q.dtype),
-               torch.empty((t, kv_heads, d), device=dev, dtype=q.dtype))
-    for o, x in zip(out, (q, k)):
-        if o.shape != x.shape or o.dtype != x.dtype or o.device != dev or (d > 1 and o.stride(-1) != 1):
-            raise ValueError("out must match q and k, its last dimension contiguous")
+        out = q.new_empty((t, heads, d)), k.new_empty((t, kv_heads, d))
+    else:
+        for o, x in zip(out, (q, k)):
+            if o.shape != x.shape or o.dtype != x.dtype or o.device != dev or (d > 1 and o.stride(-1) != 1):
+                raise ValueError("out must match q and k, its last dimension contiguous")
     if t:
         q, k, frequencies = S.rows(q), S.rows(k), frequencies.contiguous()
         q_weight, k_weight = (None if w is None else w.contiguous() for w in (q_weight, k_weight))

@@ -48,14 +48,14 @@ def _on_borders(t: Tensor) -> Tensor:
     16-byte borders (TMA) and are no repeats of one another."""
     d = t.shape[-1]
     t = S.rows(t)
-    if t.dtype == torch.float32 or d > 128 or (t.data_ptr() % 16 == 0 and all(
-            n <= 1 or (st > 0 and st % 8 == 0) for n, st in zip(t.shape[:-1], t.stride()[:-1]))):
+    if t.dtype == torch.float32 or d > 128:
+        return t
+    if t.data_ptr() % 16 == 0 and all(st > 0 and st % 8 == 0 or n <= 1 for n, st in zip(t.shape, t.stride()[:-1])):
         return t
     wide = torch.empty(t.shape[:-1] + ((d + 7) // 8 * 8,), device=t.device, dtype=t.dtype)[..., :d]
-    return wide.copy_(t)
+    return wide.copy_(t.detach())
 
 
-@torch.no_grad()
 def sliding_window_attention(q: Tensor, k: Tensor, v: Tensor, *, window: Optional[int], sinks: int = 0,
                              scale: Optional[float] = None) -> Tensor:
     """Windowed attention of [N,D] or [B,H,N,D] queries over [M,D] or [B,Hkv,M,D]
@@ -90,7 +90,6 @@ def sliding_window_attention(q: Tensor, k: Tensor, v: Tensor, *, window: Optiona
     return out[0, 0] if single else out
 
 
-@torch.no_grad()
 def sliding_window_attention_packed(q: Tensor, k: Tensor, v: Tensor, cu_q: Tensor, cu_k: Tensor, *,
                                     window: Optional[int], sinks: int = 0, scale: Optional[float] = None,
                                     out: Optional[Tensor] = None) -> Tensor:
@@ -112,8 +111,8 @@ def sliding_window_attention_packed(q: Tensor, k: Tensor, v: Tensor, cu_q: Tenso
     rows, kv_heads, dv = v.shape
     if cu_q.ndim != 1 or cu_q.shape[0] < 1:
         raise ValueError("cu_q must be [R+1]")
-    cu_q = S.int32(cu_q, tuple(cu_q.shape), "cu_q")
-    cu_k = S.int32(cu_k, tuple(cu_q.shape), "cu_k")
+    cu_q = S.int32(cu_q, cu_q.shape, "cu_q")
+    cu_k = S.int32(cu_k, cu_q.shape, "cu_k")
     if out is None:
         out = torch.zeros((t, heads, dv), device=dev, dtype=q.dtype)
     elif tuple(out.shape) != (t, heads, dv) or out.dtype != q.dtype or out.device != dev or (dv > 1 and out.stride(-1) != 1):

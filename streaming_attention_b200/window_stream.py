@@ -75,7 +75,6 @@ class StreamingWindowAttention:
         self.free_count.copy_(plan.free_count)
         return plan, q, k
 
-    @torch.no_grad()
     def prefill(self, q: Tensor, k: Tensor, v: Tensor, new: Tensor) -> Tensor:
         """Prompts of requests that hold nothing yet: ``new`` (int32
         [max_requests]) tokens of each, packed in request order in q [T,H,D], k
@@ -85,7 +84,6 @@ class StreamingWindowAttention:
         return sliding_window_attention_packed(q, k, v, plan.offsets, plan.offsets, window=self.window,
                                                sinks=self.sinks, scale=self.scale)
 
-    @torch.no_grad()
     def decode(self, q: Tensor, k: Tensor, v: Tensor) -> Tensor:
         """The next token of every request: q [max_requests,H,D], k and v
         [max_requests,Hkv,D], one row for each request; a request that holds
@@ -95,7 +93,6 @@ class StreamingWindowAttention:
         _, q, _ = self._step(q, k, v, (self.lengths > 0).to(torch.int32), per_request=1)
         return self.cache.attend(q, self.tables, self.lengths, window=self.window, sinks=self.sinks, scale=self.scale)
 
-    @torch.no_grad()
     def release(self, drop: Tensor) -> None:
         """Ends the requests with drop[r] (bool [max_requests])."""
         release_kv_pages(self.lengths, self.tables, drop, self.free_pages, self.free_count,
