@@ -29,10 +29,12 @@ constexpr int kMaxPairs = 4;   // byte columns per lane: dp <= 256
 // The code of x, decided as in exact arithmetic.
 __device__ __forceinline__ uint32_t code_of(float x, float least, float scale) {
   if (!(scale > 0.0f)) return 0;
-  const float t = __fdiv_rn(x - least, scale);
+  const float d = x - least;
+  const float t = __fdiv_rn(d, scale);
   const float r = rintf(t);
-  // |t - exact| is a few 2^-24 of t: far from k + 1/2 the rounding stands
-  if (t > -1.0f && t < 16.0f && fabsf(fabsf(t - r) - 0.5f) < 1e-4f) {
+  // |t - exact| is a few 2^-24 of t: far from k + 1/2 the rounding stands, where
+  // the difference did not overflow
+  if ((t > -1.0f && t < 16.0f && fabsf(fabsf(t - r) - 0.5f) < 1e-4f) || !(fabsf(d) < INFINITY)) {
     const double e = rint(((double)x - (double)least) / (double)scale);
     return (uint32_t)fmin(fmax(e, 0.0), 15.0);
   }
@@ -139,6 +141,51 @@ __global__ void __launch_bounds__(kThreads) read_kernel(const Kv4ReadArgs a) {
   }
 }
 
+// The codes of eight values, a nibble each.  The quotient, as a product with the
+// reciprocal clamped by saturation, is less than 3e-6 off.  Where one of the eight
+// lies within 1e-5 of a border b = k + 1/2 (often: ties are common among bfloat16
+// values) the sign of x - least - b scale decides, which float32 gives exactly:
+// b scale has 13 bits, the difference x - least is kept with its rounding error,
+// and near the border the subtraction is exact.  Whole numbers stay floats until
+// four of them make 16 bits, so that nearly all of it runs on the FMA pipe.
+__device__ __forceinline__ uint32_t codes_of(const float (&x)[8], float least, float scale) {
+  const float inv = scale > 0.0f ? 1.0f / (15.0f * scale) : 0.0f;   // 0 or infinite where 15 scale over- or underflows
+  constexpr float kWhole = 12582912.0f;   // 1.5 2^23: sums with it round to whole numbers
+  bool near = false;
+  float c[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float u = __saturatef((x[e] - least) * inv);
+    c[e] = fmaf(u, 15.0f, kWhole) - kWhole;
+    near |= fabsf(fmaf(u, 15.0f, -c[e])) > 0.49999f;
+  }
+  if (scale > 0.0f && !(inv > 0.0f && inv < INFINITY)) {
+    uint32_t w = 0;
+#pragma unroll 1
+    for (int e = 0; e < 8; ++e) {
+      float y = x[0];
+#pragma unroll
+      for (int i = 1; i < 8; ++i) y = e == i ? x[i] : y;   // keeps x in registers
+      w |= code_of(y, least, scale) << (4 * e);
+    }
+    return w;
+  }
+  if (near) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float d = x[e] - least, t = d - x[e];
+      const float lost = (x[e] - (d - t)) - (least + t);   // x - least = d + lost, exactly
+      const float b = c[e] + copysignf(0.5f, fmaf(__saturatef(d * inv), 15.0f, -c[e]));
+      const float side = fmaf(-b, scale, d) + lost;
+      const float even = 2.0f * (fmaf(b, 0.5f, kWhole) - kWhole);   // the even one of b - 1/2, b + 1/2: b / 2 is 1/4 from it
+      c[e] = fminf(fmaxf(side == 0.0f ? even : b + copysignf(0.5f, side), 0.0f), 15.0f);
+    }
+  }
+  const float lo = fmaf(c[3], 4096.0f, fmaf(c[2], 256.0f, fmaf(c[1], 16.0f, c[0]))) + kWhole;
+  const float hi = fmaf(c[7], 4096.0f, fmaf(c[6], 256.0f, fmaf(c[5], 16.0f, c[4]))) + kWhole;
+  return __byte_perm(__float_as_uint(lo), __float_as_uint(hi), 0x5410);
+}
+
 // Rows on 16-byte borders of widths that are multiples of 8: a lane holds eight
 // columns (four bytes of codes), 1 << LOG lanes a row, and takes four neighbouring
 // tokens t0 .. t0 + 3 of one head.  Keys: each row's bytes are contiguous.
@@ -151,34 +198,37 @@ __global__ void __launch_bounds__(kThreads) append_vec_kernel(const Kv4AppendArg
   using T = typename Elem<DT>::T;
   constexpr int kLanes = 1 << LOG;
   const int lane = threadIdx.x & 31, li = lane & (kLanes - 1);
-  int64_t item = ((int64_t)blockIdx.x * kThreads + threadIdx.x) >> LOG;   // (k or v, quad of tokens, head)
-  const int64_t items = ((a.tokens + 3) >> 2) * a.c.heads;
+  uint32_t item = (uint32_t)(((int64_t)blockIdx.x * kThreads + threadIdx.x) >> LOG);   // (k or v, quad of tokens, head)
+  const uint32_t items = (uint32_t)((a.tokens + 3) >> 2) * a.c.heads;
   const bool isv = item >= items;
   if (isv) item -= items;
-  const int h = (int)(item % a.c.heads);
-  const int64_t t0 = item < items ? (item / a.c.heads) * 4 : a.tokens;
+  const uint32_t quad = item / (uint32_t)a.c.heads;
+  const int h = (int)(item - quad * a.c.heads);
+  const int64_t t0 = item < items ? (int64_t)quad * 4 : a.tokens;
   const int c0 = li * 8, bytes = a.c.dp >> 1, page_mask = (1 << a.c.page_shift) - 1;
   const bool in = c0 < a.c.d;
   auto slot_of = [&](int64_t t) -> int { return t >= 0 && t < a.tokens ? __ldg(a.slots + t) : -1; };
-  // opens(t): tokens t .. t + 3 fill a word group
-  auto opens = [&](int64_t t) {
-    const int s = slot_of(t);
-    return s >= 0 && (s & 3) == 0 && (s >> a.c.page_shift) < a.c.pages && slot_of(t + 1) == s + 1 && slot_of(t + 2) == s + 2 &&
-           slot_of(t + 3) == s + 3;
-  };
   int64_t from = t0;     // the group this lane stores whole: tokens from .. from + 3
   bool whole = false;
   int taken = 0;         // bit i: token t0 + i belongs to a group
   if (isv) {
+    // bit j: token t0 - 3 + j is followed by the next slot; opens a word group of the cache
+    uint32_t next = 0, first = 0;
+    int s0 = slot_of(t0 - 3);
 #pragma unroll
-    for (int i = -3; i < 4; ++i)
-      if (opens(t0 + i)) {
-        if (i >= 0) {
-          whole = true;
-          from = t0 + i;
-        }
-        taken |= i >= 0 ? 15 << i : 15 >> -i;
-      }
+    for (int j = 0; j < 9; ++j) {
+      const int s1 = slot_of(t0 - 2 + j);
+      if (s0 >= 0 && s1 == s0 + 1) next |= 1u << j;
+      if (s0 >= 0 && (s0 & 3) == 0 && (s0 >> a.c.page_shift) < a.c.pages) first |= 1u << j;
+      s0 = s1;
+    }
+    const uint32_t opens = first & next & (next >> 1) & (next >> 2) & 127u;   // j: tokens t0 - 3 + j .. t0 + j
+#pragma unroll
+    for (int j = 0; j < 7; ++j)
+      if ((opens >> j) & 1u) taken |= j < 3 ? 15 >> (3 - j) : 15 << (j - 3);
+    whole = (opens >> 3) != 0;
+    from = t0 + __ffs(opens >> 3) - (whole ? 1 : 0);
+    taken &= 15;
   }
   // codes of token t, as four bytes, and its params
   auto code_row = [&](int64_t t, __nv_bfloat162& sm) -> uint32_t {
@@ -186,16 +236,15 @@ __global__ void __launch_bounds__(kThreads) append_vec_kernel(const Kv4AppendArg
     const bool here = in && t < a.tokens;
     if (here)
       load8(x, (isv ? static_cast<const T*>(a.v) + t * a.v_t + h * a.v_h : static_cast<const T*>(a.k) + t * a.k_t + h * a.k_h) + c0);
-    float lo = INFINITY, hi = -INFINITY;
-    bool bad = false;
+    float lo = INFINITY, hi = -INFINITY, odd = 0.0f;
     if (here)
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        bad |= !(fabsf(x[e]) < INFINITY);
+        odd = fmaf(x[e], 0.0f, odd);   // NaN once a value is not finite
         lo = fminf(lo, x[e]);
         hi = fmaxf(hi, x[e]);
       }
-    if (bad) lo = -INFINITY, hi = INFINITY;   // spreads to the row
+    if (odd != 0.0f) lo = -INFINITY, hi = INFINITY;   // spreads to the row
 #pragma unroll
     for (int d = 1; d < kLanes; d *= 2) {
       lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, d));
@@ -205,15 +254,12 @@ __global__ void __launch_bounds__(kThreads) append_vec_kernel(const Kv4AppendArg
     sm.y = __float2bfloat16_rn(lo);
     if (!(fabsf(__bfloat162float(sm.y)) < INFINITY)) sm.x = sm.y = __float2bfloat16_rn(NAN);
     const float scale = __bfloat162float(sm.x), least = __bfloat162float(sm.y);
-    uint32_t w = 0;
-    if (here)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) w |= code_of(x[e], least, scale) << (4 * e);
-    return w;
+    return here ? codes_of(x, least, scale) : 0u;
   };
   // single tokens (every key; values outside whole groups)
+  const bool singles = __any_sync(0xffffffffu, taken != 15);
 #pragma unroll 1
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; singles && i < 4; ++i) {
     const int64_t t = t0 + i;
     const int slot = slot_of(t);
     bool put = slot >= 0 && !((taken >> i) & 1);
@@ -265,15 +311,16 @@ template <int DT, int LOG>
 __global__ void __launch_bounds__(kThreads) read_vec_kernel(const Kv4ReadArgs a) {
   using T = typename Elem<DT>::T;
   const int lane = threadIdx.x & 31, li = lane & ((1 << LOG) - 1);
-  const int64_t row = ((int64_t)blockIdx.x * kThreads + threadIdx.x) >> LOG;
-  if (row >= a.tokens * a.c.heads * 2 || li * 8 >= a.c.d) return;
+  const uint32_t row = (uint32_t)(((int64_t)blockIdx.x * kThreads + threadIdx.x) >> LOG);
+  const uint32_t each = (uint32_t)a.tokens * a.c.heads;
+  if (row >= 2 * each || li * 8 >= a.c.d) return;
   // k's rows, then v's: neighbouring groups write neighbouring rows
-  const bool isv = row >= a.tokens * a.c.heads;
-  const int64_t u = isv ? row - a.tokens * a.c.heads : row;
-  const int h = (int)(u % a.c.heads);
-  const int64_t t = u / a.c.heads;
+  const bool isv = row >= each;
+  const uint32_t u = isv ? row - each : row;
+  const uint32_t t = u / (uint32_t)a.c.heads;
+  const int h = (int)(u - t * a.c.heads);
   const int slot = __ldg(a.slots + t);
-  T* o = static_cast<T*>(isv ? a.v : a.k) + u * a.c.d + li * 8;
+  T* o = static_cast<T*>(isv ? a.v : a.k) + (int64_t)u * a.c.d + li * 8;
   const int bytes = a.c.dp >> 1;
   float x[8];
   if (slot < 0 || (slot >> a.c.page_shift) >= a.c.pages) {
@@ -333,7 +380,7 @@ int read_vec(const Kv4ReadArgs& a, cudaStream_t s) {
 
 int launch_kv4_append(const Kv4AppendArgs& a, int dtype, cudaStream_t s) {
   const int elem = elem_size(dtype);
-  if (a.c.d % 8 == 0 && rows_aligned(a.k, elem, a.k_t, a.k_h) && rows_aligned(a.v, elem, a.v_t, a.v_h)) {
+  if (a.c.d % 8 == 0 && a.tokens * a.c.heads < (1 << 30) && rows_aligned(a.k, elem, a.k_t, a.k_h) && rows_aligned(a.v, elem, a.v_t, a.v_h)) {
     if (dtype == SA_REP_FLOAT32) return append_vec<SA_REP_FLOAT32>(a, s);
     if (dtype == SA_REP_FLOAT16) return append_vec<SA_REP_FLOAT16>(a, s);
     return append_vec<SA_REP_BFLOAT16>(a, s);
@@ -350,7 +397,7 @@ int launch_kv4_append(const Kv4AppendArgs& a, int dtype, cudaStream_t s) {
 }
 
 int launch_kv4_read(const Kv4ReadArgs& a, int dtype, cudaStream_t s) {
-  if (a.c.d % 8 == 0 && (((uintptr_t)a.k | (uintptr_t)a.v) & 15) == 0) {
+  if (a.c.d % 8 == 0 && a.tokens * a.c.heads < (1 << 30) && (((uintptr_t)a.k | (uintptr_t)a.v) & 15) == 0) {
     if (dtype == SA_REP_FLOAT32) return read_vec<SA_REP_FLOAT32>(a, s);
     if (dtype == SA_REP_FLOAT16) return read_vec<SA_REP_FLOAT16>(a, s);
     return read_vec<SA_REP_BFLOAT16>(a, s);

@@ -9,11 +9,14 @@
 // float64, so that far positions lose nothing.  Bound by the rows' bytes.
 //
 // Rows on 16-byte borders of widths (and halves) that are multiples of 8: a lane
-// holds eight columns of a row and the cosines and sines of their angles, which
-// serve every head of the token; lanes (1, 2, .. 32 to a row) sum squares and
-// trade partners by shuffles, four rows' loads in flight; no shared memory.  A
-// warp takes some of a token's heads: all of them where tokens abound.
+// holds eight columns of a row and, for every head of the token, what they are
+// multiplied with: out_a = r (x_a (w_a cos) - x_b (w_b sin)).  Lanes (1, 2, .. 32 to
+// a row) sum squares and trade the rows' bits by shuffles, four rows' loads in
+// flight; no shared memory.  A warp takes some of a token's heads: all of them
+// where tokens abound.
 // Others: one CTA per token, angles in shared memory, element by element.
+#include <type_traits>
+
 #include "serving.cuh"
 
 namespace sa {
@@ -93,94 +96,133 @@ __global__ void __launch_bounds__(kRotThreads) rotary_kernel(const RotaryArgs a)
   }
 }
 
+// Eight elements' bits.
+template <typename T>
+struct Bits {
+  static constexpr int kWords = sizeof(T) * 2;
+  uint32_t w[kWords];
+};
+
+template <typename T>
+__device__ __forceinline__ void floats(float (&x)[8], const Bits<T>& b) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    if constexpr (sizeof(T) == 4) {
+      x[e] = __uint_as_float(b.w[e]);
+    } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+      x[e] = __uint_as_float(e & 1 ? b.w[e >> 1] & 0xffff0000u : b.w[e >> 1] << 16);
+    } else {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&b.w[e >> 1]));
+      x[e] = e & 1 ? f.y : f.x;
+    }
+  }
+}
+
 // log2 of the lanes to a row; a warp takes `span` rows (heads of q, then of k) of a token.
 template <int DT, int LOG>
 __global__ void __launch_bounds__(kRotThreads) rotary_vec_kernel(const RotaryArgs a, int spans, int span) {
   using T = typename Elem<DT>::T;
   constexpr int kLanes = 1 << LOG, kRowsAtOnce = 32 >> LOG, kAhead = 4;
   const int lane = threadIdx.x & 31, li = lane & (kLanes - 1), sub = lane >> LOG;
-  const int64_t w = (int64_t)blockIdx.x * (kRotThreads / 32) + (threadIdx.x >> 5);
-  const int64_t t = w / spans;
+  const uint32_t w = blockIdx.x * (kRotThreads / 32) + (threadIdx.x >> 5);
+  const uint32_t t32 = w / (uint32_t)spans;
+  const int64_t t = t32;
   if (t >= a.tokens) return;
-  const int first = (int)(w - t * spans) * span, rows = min(first + span, a.heads + a.kv_heads);
+  const int first = (int)(w - t32 * spans) * span, rows = min(first + span, a.heads + a.kv_heads);
   const int position = a.positions[t];
-  if (position < 0 && !a.zero_skipped) return;
   const int c0 = li * 8;
   const bool in = c0 < a.d;              // a row may take fewer lanes than it has
+  if (position < 0) {
+    if (a.zero_skipped && in) {
+      const float none[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+      for (int row = first + sub; row < rows; row += kRowsAtOnce)
+        store8((row < a.heads ? static_cast<T*>(a.q_out) + t * a.qo_t + row * a.qo_h
+                              : static_cast<T*>(a.k_out) + t * a.ko_t + (row - a.heads) * a.ko_h) + c0, none);
+    }
+    return;
+  }
   const bool turned = c0 < 2 * a.half;   // whole lanes are: half is a multiple of 8 (of 4 where interleaved)
-  const int shift = a.interleaved ? 0 : a.half >> 3;
-  const bool second = !a.interleaved && c0 >= a.half;
+  const int shift = a.half >> 3;
+  const bool second = c0 >= a.half;
   const int partner = turned && !a.interleaved ? (second ? lane - shift : lane + shift) : lane;
-  float cs[8], sn[8], wq[8], wk[8];
+  float cs[8], sn[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     cs[e] = 1.0f;
     sn[e] = 0.0f;
-    wq[e] = wk[e] = 1.0f;
   }
-  auto load = [&](float (&x)[8], int row) {
-    if (in && row < rows)
-      load8(x, (row < a.heads ? static_cast<const T*>(a.q) + t * a.q_t + row * a.q_h
-                              : static_cast<const T*>(a.k) + t * a.k_t + (row - a.heads) * a.k_h) + c0);
-    else
-      for (int e = 0; e < 8; ++e) x[e] = 0.0f;
-  };
-  float x[kAhead][8];
-  if (position >= 0)
+  if (turned) {
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) load(x[i], first + i * kRowsAtOnce + sub);
-  if (turned && position >= 0) {
-    if (a.interleaved) {
-#pragma unroll
-      for (int e = 0; e < 8; e += 2) {
-        const double turns = (double)position * a.frequencies[(c0 + e) >> 1] * 0.15915494309189533577;
-        float s, c;
-        sincospif(2.0f * (float)(turns - rint(turns)), &s, &c);
-        cs[e] = cs[e + 1] = c;
-        sn[e] = -s;
-        sn[e + 1] = s;
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const double turns = (double)position * a.frequencies[c0 + e - (second ? a.half : 0)] * 0.15915494309189533577;
-        float s;
-        sincospif(2.0f * (float)(turns - rint(turns)), &s, &cs[e]);
-        sn[e] = second ? s : -s;
-      }
+    for (int e = 0; e < 8; ++e) {
+      const int i = a.interleaved ? (c0 + e) >> 1 : c0 + e - (second ? a.half : 0);
+      const double turns = (double)position * a.frequencies[i] * 0.15915494309189533577;
+      float s;
+      sincospif(2.0f * (float)(turns - rint(turns)), &s, &cs[e]);
+      sn[e] = (a.interleaved ? (e & 1) != 0 : second) ? s : -s;
     }
   }
-  if (in && a.q_weight) load8(wq, static_cast<const T*>(a.q_weight) + c0);
-  if (in && a.k_weight) load8(wk, static_cast<const T*>(a.k_weight) + c0);
   const float inv_d = 1.0f / (float)a.d;
-  for (int r0 = first; r0 < rows; r0 += kAhead * kRowsAtOnce) {
+#pragma unroll 1
+  for (int part = 0; part < 2; ++part) {   // queries, then keys
+    const int lo = part ? max(first, a.heads) - a.heads : first, hi = part ? rows - a.heads : min(rows, a.heads);
+    if (lo >= hi) continue;
+    const T* from = (part ? static_cast<const T*>(a.k) + t * a.k_t : static_cast<const T*>(a.q) + t * a.q_t) + c0;
+    T* to = (part ? static_cast<T*>(a.k_out) + t * a.ko_t : static_cast<T*>(a.q_out) + t * a.qo_t) + c0;
+    const int64_t from_h = part ? a.k_h : a.q_h, to_h = part ? a.ko_h : a.qo_h;
+    auto load = [&](Bits<T>& x, int row) {
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) {
-      const int row = r0 + i * kRowsAtOnce + sub;
-      const bool isq = row < a.heads;
-      float y[8];
-      if (position >= 0) {
+      for (int i = 0; i < Bits<T>::kWords; i += 4) {
+        uint4 y = make_uint4(0, 0, 0, 0);
+        if (in && row < hi) y = *(reinterpret_cast<const uint4*>(from + row * from_h) + i / 4);
+        x.w[i] = y.x;
+        x.w[i + 1] = y.y;
+        x.w[i + 2] = y.z;
+        x.w[i + 3] = y.w;
+      }
+    };
+    Bits<T> x[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) load(x[i], lo + i * kRowsAtOnce + sub);
+    // own[e] = w_e cos, other[e] = w_partner (-+ sin)
+    float own[8], other[8];
+    const T* weight = static_cast<const T*>(part ? a.k_weight : a.q_weight);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) own[e] = 1.0f;
+    if (weight && in) load8(own, weight + c0);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) other[e] = a.interleaved ? own[e ^ 1] : __shfl_sync(0xffffffffu, own[e], partner);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      own[e] *= cs[e];
+      other[e] *= sn[e];
+    }
+#pragma unroll 1
+    for (int r0 = lo; r0 < hi; r0 += kAhead * kRowsAtOnce) {
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        const int row = r0 + i * kRowsAtOnce + sub;
+        float y[8], z[8];
+        floats(y, x[i]);
         float ss = 0.0f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) ss = fmaf(x[i][e], x[i][e], ss);
+        for (int e = 0; e < 8; ++e) ss = fmaf(y[e], y[e], ss);
 #pragma unroll
         for (int d = 1; d < kLanes; d *= 2) ss += __shfl_xor_sync(0xffffffffu, ss, d);
-        const float r = 1.0f / sqrtf(fmaf(ss, inv_d, a.eps));
+        if (a.interleaved) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) y[e] = x[i][e] * r * (isq ? wq[e] : wk[e]);
+          for (int e = 0; e < 8; ++e) z[e] = y[e ^ 1];
+        } else {
+          Bits<T> b;
+#pragma unroll
+          for (int e = 0; e < Bits<T>::kWords; ++e) b.w[e] = __shfl_sync(0xffffffffu, x[i].w[e], partner);
+          floats(z, b);
+        }
         load(x[i], row + kAhead * kRowsAtOnce);
-        float z[8];
+        const float r = rsqrtf(fmaf(ss, inv_d, a.eps));
 #pragma unroll
-        for (int e = 0; e < 8; ++e) z[e] = a.interleaved ? y[e ^ 1] : __shfl_sync(0xffffffffu, y[e], partner);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) y[e] = fmaf(y[e], cs[e], z[e] * sn[e]);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) y[e] = 0.0f;
+        for (int e = 0; e < 8; ++e) y[e] = r * fmaf(y[e], own[e], z[e] * other[e]);
+        if (in && row < hi) store8(to + row * to_h, y);
       }
-      if (in && row < rows)
-        store8((isq ? static_cast<T*>(a.q_out) + t * a.qo_t + row * a.qo_h
-                    : static_cast<T*>(a.k_out) + t * a.ko_t + (row - a.heads) * a.ko_h) + c0, y);
     }
   }
 }
@@ -198,7 +240,7 @@ int launch_vec(const RotaryArgs& a, cudaStream_t s) {
   span = (span + (32 >> log) - 1) / (32 >> log) * (32 >> log);   // whole warps of rows
   spans = (rows + span - 1) / span;
   const int64_t ctas = ceil_div(a.tokens * spans, kRotThreads / 32);
-  if (ctas > 2147483647LL) return set_error(SA_ERR_UNSUPPORTED, "rotary: grid too large");
+  if (ctas > (1 << 28)) return set_error(SA_ERR_UNSUPPORTED, "rotary: grid too large");
   const unsigned g = (unsigned)ctas;
   if (log == 0) rotary_vec_kernel<DT, 0><<<g, kRotThreads, 0, s>>>(a, spans, span);
   else if (log == 1) rotary_vec_kernel<DT, 1><<<g, kRotThreads, 0, s>>>(a, spans, span);

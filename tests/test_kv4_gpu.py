@@ -72,6 +72,21 @@ def test_append_borders_and_extremes(dev):
         _check_rows(cache, k, v, slots)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("d", [32, 33, 128])
+def test_append_rows_of_the_whole_range(dtype, d, dev):
+    """Differences of values that float32 cannot hold, scales whose reciprocals it cannot."""
+    g = R.rng(d)
+    u = torch.rand(40, 1, d, generator=g, dtype=torch.float64) * 2 - 1
+    level = torch.cat([torch.full((10,), 3.38e38, dtype=torch.float64), torch.full((10,), 1.6e38, dtype=torch.float64),
+                       10.0 ** torch.linspace(-41, -36, 20, dtype=torch.float64)])
+    k = (u * level[:, None, None]).to(dtype)
+    cache = sa.Kv4Cache.empty(3, 1, d, page_size=16, device=dev)
+    slots = torch.arange(40)
+    cache.append(k.to(dev), (-k).to(dev), slots.to(torch.int32).to(dev))
+    _check_rows(cache, k, -k, slots)
+
+
 def test_append_many_near_borders(dev):
     """Rows whose quotients sit within float32 rounding of a border."""
     g = R.rng(9)
