@@ -329,7 +329,7 @@ int sa_flash_causal_attention(const float* q, const float* k, const float* v, in
  * contiguous.  The kernels check the contents of device-side index arrays
  * (offsets, slots, page tables, lengths): what is out of range is skipped and
  * recorded in the device's error word, which sa_serving_status reads.  No call
- * allocates or needs a workspace; all may be captured into a graph. */
+ * allocates; all may be captured into a graph. */
 
 /* Synchronises `stream`, then returns SA_OK, or what the serving calls on this
  * device recorded first since the last read (SA_ERR_INVALID_ARG for bad index
@@ -346,10 +346,17 @@ int sa_serving_status(void* stream);
  * k_n, v_b, v_h, v_n, o_b, o_h, o_n}.  Packed: cu_q, cu_k [batch + 1] are the
  * requests' first rows in q / out (n rows in all) and k / v (m rows in all),
  * p counts within the request, the *_b strides are 0; rows behind
- * cu_q[batch] stay as they were.  d, dv <= 256. */
+ * cu_q[batch] stay as they were.  d, dv <= 256.
+ * Tensor cores: float16 / bfloat16 of d, dv <= 128 on 16-byte borders; dense
+ * contiguous float32 (3xTF32) of d <= 64, dv <= 128 and long enough given a workspace of
+ * sa_window_attention_workspace_size bytes (256-byte aligned; 0: none is used).
+ * CUDA cores otherwise. */
+int sa_window_attention_workspace_size(int batch, int heads, int kv_heads, int64_t n, int64_t m, int d, int dv,
+                                       int64_t window, int64_t sinks, int dtype, size_t* bytes);
 int sa_window_attention(const void* q, const void* k, const void* v, void* out, const int64_t* strides, int batch,
                         int heads, int kv_heads, int64_t n, int64_t m, int d, int dv, int64_t window, int64_t sinks,
-                        float scale, int dtype, const int32_t* cu_q, const int32_t* cu_k, void* stream);
+                        float scale, int dtype, const int32_t* cu_q, const int32_t* cu_k, void* workspace,
+                        size_t workspace_bytes, void* stream);
 
 /* The cache: pages of page_size (16, 32, 64, 128 or 256) tokens; dp = d filled
  * up to 32, 64, 128 or 256 (d <= 256); byte b of a row holds column 2 b in its

@@ -15,12 +15,14 @@
 #include <cuda.h>
 #include <stdarg.h>
 
+#include <algorithm>
 #include <atomic>
 #include <stdio.h>
 #include <stdlib.h>
 #include <string.h>
 
 #include "sa_common.cuh"
+#include "serving.cuh"
 
 namespace sa {
 
@@ -59,6 +61,7 @@ int launch_segment_mean(const float* k, const float* v, int64_t bh, int64_t n, i
 int launch_fill(float* dst, int64_t count, float value, cudaStream_t s);
 int launch_flash_tc(const CUtensorMap* maps, const float* q, float* out, int* status, int64_t bh, int64_t n, int d,
                     int dv, float scale, cudaStream_t stream);
+int launch_window_tf32(const CUtensorMap* maps, const WindowArgs& w, cudaStream_t stream);
 int launch_flash_simt(const float* q, const float* k, const float* v, int64_t bh, int64_t n, int d, int dv,
                       float scale, float* out, cudaStream_t s);
 
@@ -609,6 +612,40 @@ int fast_attention_run(const float* q, const float* k, const float* v, int64_t b
   }
   if (!rc) stage_mark(4, s);
   return rc;
+}
+
+// The float32 windowed attention on the tensor cores: workspace bytes (0: not
+// taken) of n queries over m keys.  It splits all of K and V first, which the CUDA
+// cores' kernel does not: taken where a query tile sees some hundred keys, and
+// either there are queries enough or most keys are seen.
+size_t window_tf32_bytes(int64_t batch, int heads, int kv_heads, int64_t n, int64_t m, int d, int dv, int64_t window,
+                         int64_t sinks) {
+  if (batch * heads > 65535 || m >= (1 << 30) || n == 0) return 0;
+  const int64_t seen = window == 0 || window >= m ? m : std::min(m, window + std::min(sinks, m) + n);
+  if (seen < 256 || (n < 64 && 4 * seen < m)) return 0;
+  return plan_flash(batch * kv_heads, m, d, dv).total;
+}
+
+int window_tf32_run(const WindowArgs& a, void* workspace, size_t workspace_bytes, cudaStream_t s) {
+  const int64_t bkv = (int64_t)a.batch * a.kv_heads;
+  const Workspace w = plan_flash(bkv, a.m, a.d, a.dv);
+  int rc = check_workspace(w, workspace, workspace_bytes);
+  if (rc) return rc;
+  char* ws = static_cast<char*>(workspace);
+  float* khi = reinterpret_cast<float*>(ws + w.khi);
+  float* klo = reinterpret_cast<float*>(ws + w.klo);
+  float* vthi = reinterpret_cast<float*>(ws + w.vthi);
+  float* vtlo = reinterpret_cast<float*>(ws + w.vtlo);
+  rc = launch_split(static_cast<const float*>(a.k), bkv * a.m, a.d, w.dp, khi, klo, s);
+  if (!rc) rc = launch_split_t(static_cast<const float*>(a.v), bkv, a.m, a.dv, w.dvp, w.n_pad, vthi, vtlo, s);
+  if (rc) return rc;
+  CUtensorMap maps[4];
+  rc = encode_map_3d(&maps[0], khi, w.dp, a.m, bkv, 64, CU_TENSOR_MAP_SWIZZLE_128B);
+  if (!rc) rc = encode_map_3d(&maps[1], klo, w.dp, a.m, bkv, 64, CU_TENSOR_MAP_SWIZZLE_128B);
+  if (!rc) rc = encode_map(&maps[2], vthi, a.m, w.n_pad, w.dvp, bkv, w.dvp, CU_TENSOR_MAP_SWIZZLE_128B);
+  if (!rc) rc = encode_map(&maps[3], vtlo, a.m, w.n_pad, w.dvp, bkv, w.dvp, CU_TENSOR_MAP_SWIZZLE_128B);
+  if (rc) return rc;
+  return launch_window_tf32(maps, a, s);
 }
 
 }  // namespace sa

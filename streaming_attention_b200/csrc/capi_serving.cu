@@ -109,9 +109,21 @@ int sa_serving_status(void* stream) {
   return set_error(SA_ERR_TIMEOUT, "a bounded device-side wait gave up (wait code %d)", code);
 }
 
+int sa_window_attention_workspace_size(int batch, int heads, int kv_heads, int64_t n, int64_t m, int d, int dv,
+                                       int64_t window, int64_t sinks, int dtype, size_t* bytes) {
+  if (!bytes) return set_error(SA_ERR_INVALID_ARG, "null output pointer");
+  int rc = check_dtype(dtype);
+  if (!rc) rc = check_heads(heads, kv_heads);
+  if (rc) return rc;
+  if (batch < 0 || n < 0 || m < 0 || d <= 0 || dv <= 0 || window < 0 || sinks < 0) return set_error(SA_ERR_INVALID_ARG, "bad sizes");
+  *bytes = dtype == SA_REP_FLOAT32 ? window_tf32_bytes(batch, heads, kv_heads, n, m, d, dv, window, sinks) : 0;
+  return SA_OK;
+}
+
 int sa_window_attention(const void* q, const void* k, const void* v, void* out, const int64_t* strides, int batch,
                         int heads, int kv_heads, int64_t n, int64_t m, int d, int dv, int64_t window, int64_t sinks,
-                        float scale, int dtype, const int32_t* cu_q, const int32_t* cu_k, void* stream) {
+                        float scale, int dtype, const int32_t* cu_q, const int32_t* cu_k, void* workspace,
+                        size_t workspace_bytes, void* stream) {
   int rc = check_dtype(dtype);
   if (!rc) rc = check_heads(heads, kv_heads);
   if (rc) return rc;
@@ -130,6 +142,12 @@ int sa_window_attention(const void* q, const void* k, const void* v, void* out, 
                      window > 0 ? window : (int64_t)1 << 40, sinks, scale, dtype, cu_q, cu_k, status_word()};
   const char* simt = getenv("SA_FORCE_SIMT");
   if (window_tc_takes(a) && !(simt && simt[0] == '1')) return launch_window_tc(a, (cudaStream_t)stream);
+  // float32 on the tensor cores: contiguous tensors and a workspace
+  if (dtype == SA_REP_FLOAT32 && !cu_q && workspace && a.status && a.q_n == d && a.q_h == n * d && a.q_b == heads * a.q_h &&
+      a.k_n == d && a.k_h == m * d && a.k_b == kv_heads * a.k_h && a.v_n == dv && a.v_h == m * dv &&
+      a.v_b == kv_heads * a.v_h && a.o_n == dv && a.o_h == n * dv && a.o_b == heads * a.o_h &&
+      window_tf32_bytes(batch, heads, kv_heads, n, m, d, dv, window, sinks) > 0)
+    return window_tf32_run(a, workspace, workspace_bytes, (cudaStream_t)stream);
   return launch_window_simt(a, (cudaStream_t)stream);
 }
 

@@ -28,10 +28,17 @@
 // the next product restarts the TMEM chain.  The running sum l adds each tile's 32
 // values pairwise before the running add.  Scores are kept in base-2 units (the query is scaled by
 // scale * log2(e), as FlashAttention-2 does), so p = 2^(s - m) is one ex2.
+//
+// kWin: the float32 windowed attention with first tokens and grouped heads
+// (serving.cuh) on the same tiles: a CTA walks the tiles of 64 keys that hold the
+// first tokens, then those of its rows' windows; p = 2^(s - m - 24), so that sums
+// of values near float32's largest stay below it; rows that come out non-finite
+// are computed again from their visible keys (window_row.cuh).
 #include <math.h>
 
 #include "sa_common.cuh"
 #include "tc_util.cuh"
+#include "window_row.cuh"
 
 namespace sa {
 
@@ -63,6 +70,7 @@ struct FlashParams {
   int d, dv;
   float scale;
   uint64_t wait_ns;  // limit of one bounded wait
+  WindowArgs w;      // kWin only: dense, contiguous float32
 };
 
 template <int DP, int DVP>
@@ -83,7 +91,12 @@ struct FLayout {
   static constexpr uint32_t kSmemBytes = kBars + (2 * kStages + 10) * 8 + 64 + 1024;
 };
 
-template <int DP, int DVP>
+// The x lowest bits set (x may be anything).
+__device__ __forceinline__ uint32_t low_bits(int64_t x) {
+  return x >= 32 ? 0xffffffffu : (x <= 0 ? 0u : (1u << x) - 1u);
+}
+
+template <int DP, int DVP, bool kWin>
 __global__ void __launch_bounds__(kThreads, 1)
 flash_tc_kernel(const __grid_constant__ CUtensorMap tm_kh, const __grid_constant__ CUtensorMap tm_kl,
                 const __grid_constant__ CUtensorMap tm_vh, const __grid_constant__ CUtensorMap tm_vl,
@@ -113,7 +126,19 @@ flash_tc_kernel(const __grid_constant__ CUtensorMap tm_kh, const __grid_constant
   const int64_t qt = n_qt - 1 - blockIdx.x;     // heavy (late) query tiles first
   const int64_t q0 = qt * kRowsQ;
   const int64_t q_last = min(q0 + kRowsQ, p.n) - 1;
-  const int T = (int)((q_last + kTile) / kTile);  // key tiles 0 .. q_last
+  int T = (int)((q_last + kTile) / kTile);  // key tiles 0 .. q_last
+  int hk = (int)h;                          // the sequence of keys
+  int sink_tiles = 0, win_tile = 0;         // kWin: tile t >= sink_tiles is key tile win_tile + t - sink_tiles
+  const int64_t back = kWin ? p.w.m - p.n : 0;   // position of query 0
+  if constexpr (kWin) {
+    const int b = (int)h / p.w.heads, hh = (int)h - b * p.w.heads;
+    hk = b * p.w.kv_heads + hh / (p.w.heads / p.w.kv_heads);
+    const KeyRanges kr = key_ranges(back + q0, back + q_last, p.w.m, p.w.window, p.w.sinks);
+    sink_tiles = (int)((kr.first + kTile - 1) / kTile);
+    win_tile = max((int)(kr.begin / kTile), sink_tiles);
+    T = sink_tiles + max((int)((kr.end + kTile - 1) / kTile) - win_tile, 0);
+  }
+  auto key_tile = [&](int t) { return !kWin || t < sink_tiles ? t : win_tile + t - sink_tiles; };
 
   // Query-row threads start loading their 32-column chunk of the query row now,
   // so that the loads' latency overlaps the set-up below: 16-byte loads when
@@ -175,19 +200,19 @@ flash_tc_kernel(const __grid_constant__ CUtensorMap tm_kh, const __grid_constant
       for (int t = 0; t < T; ++t) {
         const int s = t % kStages;
         if (t >= kStages && !mbar_wait(&empty[s], ((t / kStages) - 1) & 1, ab, kErrWaitEmpty)) break;
-        const int row0 = t * kTile;
+        const int row0 = key_tile(t) * kTile;
         mbar_arrive_expect_tx(&full[s], L::kStage);
         uint8_t* st = smem + s * L::kStage;
 #pragma unroll
         for (int a = 0; a < DP / 32; ++a) {
-          tma_load_3d(st + a * (2 * kTile * 128), &tm_kh, &full[s], a * 32, row0, (int)h);
-          tma_load_3d(st + a * (2 * kTile * 128) + kTile * 128, &tm_kl, &full[s], a * 32, row0, (int)h);
+          tma_load_3d(st + a * (2 * kTile * 128), &tm_kh, &full[s], a * 32, row0, hk);
+          tma_load_3d(st + a * (2 * kTile * 128) + kTile * 128, &tm_kl, &full[s], a * 32, row0, hk);
         }
 #pragma unroll
         for (int a = 0; a < kTile / 32; ++a) {
           uint8_t* vd = st + 2 * L::kKT + a * (2 * DVP * 128);
-          tma_load_3d(vd, &tm_vh, &full[s], row0 + a * 32, 0, (int)h);
-          tma_load_3d(vd + DVP * 128, &tm_vl, &full[s], row0 + a * 32, 0, (int)h);
+          tma_load_3d(vd, &tm_vh, &full[s], row0 + a * 32, 0, hk);
+          tma_load_3d(vd + DVP * 128, &tm_vl, &full[s], row0 + a * 32, 0, hk);
         }
         ++issued;
       }
@@ -319,11 +344,15 @@ flash_tc_kernel(const __grid_constant__ CUtensorMap tm_kh, const __grid_constant
       const int b = t & 1;
       if (ok && !mbar_wait_warp(&sfull[b], (t >> 1) & 1, ab, kErrWaitS)) ok = false;
       const uint32_t tS = lane_addr + L::kS0 + 128 * b + half * 32;
-      const int64_t col0 = (int64_t)t * kTile + half * 32;
+      const int64_t col0 = (int64_t)key_tile(t) * kTile + half * 32;
       // causal mask: key col0 + j is visible to row i when j <= lim
-      const int64_t rel = i - col0;
+      const int64_t rel = back + i - col0;
       const int lim = !valid || rel < 0 ? -1 : (rel > 31 ? 31 : (int)rel);
-      const bool all_on = lim >= 31;
+      uint32_t on = 0;   // kWin: bit j
+      if constexpr (kWin) {
+        on = low_bits(lim + 1) & (~low_bits(rel - p.w.window + 1) | low_bits(p.w.sinks - col0));
+      }
+      const bool all_on = kWin ? on == 0xffffffffu : lim >= 31;
       float sv[32];
       float pm = -INFINITY;
       if (ok) {
@@ -341,7 +370,7 @@ flash_tc_kernel(const __grid_constant__ CUtensorMap tm_kh, const __grid_constant
         } else {
 #pragma unroll
           for (int j = 0; j < 32; ++j) {
-            sv[j] = j <= lim ? sv[j] + s2[j] : -INFINITY;
+            sv[j] = (kWin ? ((on >> j) & 1u) != 0 : j <= lim) ? sv[j] + s2[j] : -INFINITY;
             pm = fmaxf(pm, sv[j]);
           }
         }
@@ -409,7 +438,8 @@ flash_tc_kernel(const __grid_constant__ CUtensorMap tm_kh, const __grid_constant
       }
       // masked scores are -inf: ex2 gives exactly 0 there (m is finite for a
       // valid row; an invalid row has every p = 0 below)
-      const float mm = valid ? m : 0.0f;
+      // (kWin: a row that has seen nothing yet has no m)
+      const float mm = kWin ? (m == -INFINITY ? 24.0f : m + 24.0f) : (valid ? m : 0.0f);
       uint32_t hi[32], lo[32];
       float ps[16];
 #pragma unroll
@@ -436,9 +466,14 @@ flash_tc_kernel(const __grid_constant__ CUtensorMap tm_kh, const __grid_constant
     lsum[half * 128 + row] = l;
     asm volatile("bar.sync 1, 256;" ::: "memory");
     const float l_all = lsum[row] + lsum[128 + row];
-    if (ok && mbar_wait_warp(ofull, 0, ab, kErrWaitO)) {
+    if (ok && (!kWin || T > 0)) ok = mbar_wait_warp(ofull, 0, ab, kErrWaitO);
+    bool fine = true;
+    if (kWin && T == 0) {   // no key is visible to any row of the tile
+      if (valid && half == 0)
+        for (int c = 0; c < p.dv; ++c) p.out[(h * p.n + i) * (int64_t)p.dv + c] = 0.0f;
+    } else if (ok) {
       tc_fence_after();
-      const float dmax = fmaxf(l_all, 1.0e-20f);
+      const float dmax = kWin ? (l_all == 0.0f ? 1.0f : l_all) : fmaxf(l_all, 1.0e-20f);
       float* orow = p.out + (h * p.n + (valid ? i : 0)) * (int64_t)p.dv;
 #pragma unroll
       for (int cchunk = 0; cchunk < DVP / 32; ++cchunk) {
@@ -458,9 +493,24 @@ flash_tc_kernel(const __grid_constant__ CUtensorMap tm_kh, const __grid_constant
 #pragma unroll
           for (int j = 0; j < 32; ++j) {
             const int col = cchunk * 32 + j;
-            if (col < p.dv) orow[col] = __fdiv_rn(master[DVP == 32 ? 0 : cchunk >> 1][j] + ov[j], dmax);
+            if (col < p.dv) {
+              const float x = __fdiv_rn(master[DVP == 32 ? 0 : cchunk >> 1][j] + ov[j], dmax);
+              if constexpr (kWin) fine &= fabsf(x) < INFINITY;
+              orow[col] = x;
+            }
           }
         }
+      }
+    }
+    if constexpr (kWin) {
+      // once both halves of a row are written (a failed wait or not: the pair meets in any case)
+      xmax[half * 128 + row] = fine ? 0.0f : 1.0f;
+      __threadfence_block();
+      asm volatile("bar.sync %0, 64;" ::"r"(bar_id) : "memory");
+      if (ok && half == 0 && valid && (!fine || xmax[128 + row] != 0.0f)) {
+        const int b = (int)h / p.w.heads, hh = (int)h - b * p.w.heads, kv = hk - b * p.w.kv_heads;
+        row_again<SA_REP_FLOAT32>(p.w, b * p.w.q_b + hh * p.w.q_h + i * p.w.q_n, b * p.w.k_b + kv * p.w.k_h,
+                                  b * p.w.v_b + kv * p.w.v_h, b * p.w.o_b + hh * p.w.o_h + i * p.w.o_n, back + i, p.w.m);
       }
     }
   }
@@ -472,15 +522,29 @@ flash_tc_kernel(const __grid_constant__ CUtensorMap tm_kh, const __grid_constant
   }
 }
 
-template <int DP, int DVP>
+template <int DP, int DVP, bool kWin>
 int launch_flash(const CUtensorMap* maps, const FlashParams& prm, int64_t bh, cudaStream_t stream) {
   using L = FLayout<DP, DVP>;
-  auto kern = flash_tc_kernel<DP, DVP>;
+  auto kern = flash_tc_kernel<DP, DVP, kWin>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L::kSmemBytes);
   if (e != cudaSuccess) return set_error(SA_ERR_CUDA, "flash_tc smem attribute: %s", cudaGetErrorString(e));
   dim3 grid((unsigned)((prm.n + kRowsQ - 1) / kRowsQ), (unsigned)bh);
   kern<<<grid, kThreads, L::kSmemBytes, stream>>>(maps[0], maps[1], maps[2], maps[3], prm);
   return check_launch("flash_tc_kernel");
+}
+
+template <bool kWin>
+int launch_flash_dims(const CUtensorMap* maps, const FlashParams& prm, int64_t bh, cudaStream_t stream) {
+  const int d = prm.d, dv = prm.dv;
+  const int dp = d <= 32 ? 32 : (d <= 64 ? 64 : 0);
+  const int dvp = dv <= 32 ? 32 : (dv <= 64 ? 64 : (dv <= 128 ? 128 : 0));
+  if (dp == 32 && dvp == 32) return launch_flash<32, 32, kWin>(maps, prm, bh, stream);
+  if (dp == 32 && dvp == 64) return launch_flash<32, 64, kWin>(maps, prm, bh, stream);
+  if (dp == 32 && dvp == 128) return launch_flash<32, 128, kWin>(maps, prm, bh, stream);
+  if (dp == 64 && dvp == 32) return launch_flash<64, 32, kWin>(maps, prm, bh, stream);
+  if (dp == 64 && dvp == 64) return launch_flash<64, 64, kWin>(maps, prm, bh, stream);
+  if (dp == 64 && dvp == 128) return launch_flash<64, 128, kWin>(maps, prm, bh, stream);
+  return set_error(SA_ERR_UNSUPPORTED, "tensor-core flash: d=%d dv=%d not supported", d, dv);
 }
 
 }  // namespace
@@ -492,16 +556,17 @@ int launch_flash_tc(const CUtensorMap* maps, const float* q, float* out, int* st
   if (bh == 0 || n == 0) return SA_OK;
   if (bh > 65535 || (n + kRowsQ - 1) / kRowsQ > 2147483647LL)
     return set_error(SA_ERR_UNSUPPORTED, "grid too large for the tensor-core flash kernel");
-  const FlashParams prm{q, out, status, n, d, dv, scale, wait_limit_ns()};
-  const int dp = d <= 32 ? 32 : (d <= 64 ? 64 : 0);
-  const int dvp = dv <= 32 ? 32 : (dv <= 64 ? 64 : (dv <= 128 ? 128 : 0));
-  if (dp == 32 && dvp == 32) return launch_flash<32, 32>(maps, prm, bh, stream);
-  if (dp == 32 && dvp == 64) return launch_flash<32, 64>(maps, prm, bh, stream);
-  if (dp == 32 && dvp == 128) return launch_flash<32, 128>(maps, prm, bh, stream);
-  if (dp == 64 && dvp == 32) return launch_flash<64, 32>(maps, prm, bh, stream);
-  if (dp == 64 && dvp == 64) return launch_flash<64, 64>(maps, prm, bh, stream);
-  if (dp == 64 && dvp == 128) return launch_flash<64, 128>(maps, prm, bh, stream);
-  return set_error(SA_ERR_UNSUPPORTED, "tensor-core flash: d=%d dv=%d not supported", d, dv);
+  const FlashParams prm{q, out, status, n, d, dv, scale, wait_limit_ns(), {}};
+  return launch_flash_dims<false>(maps, prm, bh, stream);
+}
+
+// The windowed form: q, out [batch * heads, n, *], the maps over [batch * kv_heads, m, *].
+int launch_window_tf32(const CUtensorMap* maps, const WindowArgs& w, cudaStream_t stream) {
+  const int64_t bh = (int64_t)w.batch * w.heads;
+  if (bh > 65535) return set_error(SA_ERR_UNSUPPORTED, "grid too large for the tensor-core flash kernel");
+  const FlashParams prm{static_cast<const float*>(w.q), static_cast<float*>(w.out), w.status, w.n, w.d, w.dv, w.scale,
+                        wait_limit_ns(), w};
+  return launch_flash_dims<true>(maps, prm, bh, stream);
 }
 
 }  // namespace sa

@@ -11,8 +11,8 @@
 // Rows on 16-byte borders of widths (and halves) that are multiples of 8: a lane
 // holds eight columns of a row and, for every head of the token, what they are
 // multiplied with: out_a = r (x_a (w_a cos) - x_b (w_b sin)).  Lanes (1, 2, .. 32 to
-// a row) sum squares and trade the rows' bits by shuffles, four rows' loads in
-// flight; no shared memory.  A warp takes some of a token's heads: all of them
+// a row) sum squares and trade the rows' bits by shuffles, two rows' loads in
+// flight (and a third CTA an SM for it); no shared memory.  A warp takes some of a token's heads: all of them
 // where tokens abound.
 // Others: one CTA per token, angles in shared memory, element by element.
 #include <type_traits>
@@ -120,9 +120,9 @@ __device__ __forceinline__ void floats(float (&x)[8], const Bits<T>& b) {
 
 // log2 of the lanes to a row; a warp takes `span` rows (heads of q, then of k) of a token.
 template <int DT, int LOG>
-__global__ void __launch_bounds__(kRotThreads) rotary_vec_kernel(const RotaryArgs a, int spans, int span) {
+__global__ void __launch_bounds__(kRotThreads, DT == SA_REP_FLOAT32 ? 2 : 3) rotary_vec_kernel(const RotaryArgs a, int spans, int span) {
   using T = typename Elem<DT>::T;
-  constexpr int kLanes = 1 << LOG, kRowsAtOnce = 32 >> LOG, kAhead = 4;
+  constexpr int kLanes = 1 << LOG, kRowsAtOnce = 32 >> LOG, kAhead = 2;
   const int lane = threadIdx.x & 31, li = lane & (kLanes - 1), sub = lane >> LOG;
   const uint32_t w = blockIdx.x * (kRotThreads / 32) + (threadIdx.x >> 5);
   const uint32_t t32 = w / (uint32_t)spans;
@@ -233,7 +233,7 @@ int launch_vec(const RotaryArgs& a, cudaStream_t s) {
   while ((8 << log) < a.d) ++log;
   // rows of a token to a warp: all of them, or as few as its lanes hold in flight
   // once while the grid has less than 16 warps an SM
-  const int rows = a.heads + a.kv_heads, at_once = 4 * (32 >> log);
+  const int rows = a.heads + a.kv_heads, at_once = 2 * (32 >> log);
   int spans = 1;
   while (a.tokens * spans < 148 * 16 && (rows + spans - 1) / spans > at_once) ++spans;
   int span = (rows + spans - 1) / spans;

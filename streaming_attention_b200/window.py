@@ -14,11 +14,13 @@ their product with v (the operand type of the tensor cores).
 
 from __future__ import annotations
 
+import ctypes
 import math
 from typing import Optional
 
 import torch
 
+from . import _lib
 from . import _serving as S
 
 Tensor = torch.Tensor
@@ -40,6 +42,12 @@ def _check_dims(q: Tensor, k: Tensor, v: Tensor) -> None:
 def _check_heads(heads: int, kv_heads: int) -> None:
     if kv_heads == 0 or heads % kv_heads != 0:
         raise ValueError(f"the query heads ({heads}) must be a multiple of the key heads ({kv_heads})")
+
+
+def _workspace_size(*sizes: int) -> int:
+    nbytes = ctypes.c_size_t(0)
+    _lib.check(_lib.load().sa_window_attention_workspace_size(*sizes, ctypes.byref(nbytes)), "window workspace size")
+    return nbytes.value
 
 
 def _on_borders(t: Tensor) -> Tensor:
@@ -83,10 +91,17 @@ def sliding_window_attention(q: Tensor, k: Tensor, v: Tensor, *, window: Optiona
     out = torch.empty((b, heads, n, dv), device=dev, dtype=q.dtype)
     if out.numel():
         _check_heads(heads, kv_heads)
+        ws = None
+        if code == _lib.REP_DTYPES["float32"]:
+            size = _workspace_size(b, heads, kv_heads, n, m, d, dv, w, s, code)
+            if size:
+                ws = torch.empty(size, device=dev, dtype=torch.uint8)
+                q, k, v = (t.detach().contiguous() for t in (q, k, v))
         q, k, v = _on_borders(q), _on_borders(k), _on_borders(v)
         S.launch(dev, "sa_window_attention", q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
                  S.strides(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *out.stride()[:3]), b, heads, kv_heads,
-                 n, m, d, dv, w, s, _scale(scale, d), code, None, None)
+                 n, m, d, dv, w, s, _scale(scale, d), code, None, None,
+                 None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel())
     return out[0, 0] if single else out
 
 
@@ -123,5 +138,5 @@ def sliding_window_attention_packed(q: Tensor, k: Tensor, v: Tensor, cu_q: Tenso
         S.launch(dev, "sa_window_attention", q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
                  S.strides(0, q.stride(1), q.stride(0), 0, k.stride(1), k.stride(0), 0, v.stride(1), v.stride(0), 0,
                            out.stride(1), out.stride(0)), cu_q.shape[0] - 1, heads, kv_heads, t, rows, d, dv, w, s,
-                 _scale(scale, d), code, cu_q.data_ptr(), cu_k.data_ptr())
+                 _scale(scale, d), code, cu_q.data_ptr(), cu_k.data_ptr(), None, 0)
     return out

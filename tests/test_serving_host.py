@@ -18,7 +18,7 @@ def _strides(n):
 
 def _window(**kw):
     a = dict(q=P, k=P, v=P, out=P, strides=_strides(12), batch=1, heads=4, kv_heads=2, n=8, m=8, d=64, dv=64, window=4, sinks=0,
-             scale=1.0, dtype=2, cu_q=None, cu_k=None, stream=None)
+             scale=1.0, dtype=2, cu_q=None, cu_k=None, ws=None, ws_bytes=0, stream=None)
     a.update(kw)
     return _lib.load().sa_window_attention(*a.values())
 
@@ -48,7 +48,6 @@ def test_cache_arguments(kw, rc):
     lib, c = _lib.load(), _cache(**kw)
     assert lib.sa_kv4_append(*c.values(), P, P, _strides(4), P, 3, 0, None) == rc
     assert lib.sa_kv4_read(*c.values(), P, P, P, 3, 0, None) == rc
-    c["heads"] = c["heads"]
     assert lib.sa_kv4_attend(*c.values(), P, P, _strides(3), P, P, 1, 1, 4, 2, 0, 0, 1.0, 0, None) == rc
 
 
