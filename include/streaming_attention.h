@@ -346,7 +346,7 @@ int sa_serving_status(void* stream);
  * k_n, v_b, v_h, v_n, o_b, o_h, o_n}.  Packed: cu_q, cu_k [batch + 1] are the
  * requests' first rows in q / out (n rows in all) and k / v (m rows in all),
  * p counts within the request, the *_b strides are 0; rows behind
- * cu_q[batch] stay as they were.  d, dv <= 256.
+ * cu_q[batch] stay as they were, or are zeroed (zero_behind != 0).  d, dv <= 256.
  * Tensor cores: float16 / bfloat16 of d, dv <= 128 on 16-byte borders; dense
  * contiguous float32 (3xTF32) of d <= 64, dv <= 128 and long enough given a workspace of
  * sa_window_attention_workspace_size bytes (256-byte aligned; 0: none is used).
@@ -355,7 +355,7 @@ int sa_window_attention_workspace_size(int batch, int heads, int kv_heads, int64
                                        int64_t window, int64_t sinks, int dtype, size_t* bytes);
 int sa_window_attention(const void* q, const void* k, const void* v, void* out, const int64_t* strides, int batch,
                         int heads, int kv_heads, int64_t n, int64_t m, int d, int dv, int64_t window, int64_t sinks,
-                        float scale, int dtype, const int32_t* cu_q, const int32_t* cu_k, void* workspace,
+                        float scale, int dtype, const int32_t* cu_q, const int32_t* cu_k, int zero_behind, void* workspace,
                         size_t workspace_bytes, void* stream);
 
 /* The cache: pages of page_size (16, 32, 64, 128 or 256) tokens; dp = d filled

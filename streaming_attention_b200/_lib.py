@@ -75,7 +75,7 @@ SIGNATURES = {
     "sa_window_attention_workspace_size": [_i32, _i32, _i32, _i64, _i64, _i32, _i32, _i64, _i64, _i32,
                                            ctypes.POINTER(_sz)],
     "sa_window_attention": [_vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i64, _i64, _i32, _i32, _i64, _i64, _f32, _i32,
-                            _vp, _vp, _vp, _sz, _vp],
+                            _vp, _vp, _i32, _vp, _sz, _vp],
     "sa_kv4_append": [_vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _i64, _i32, _vp],
     "sa_kv4_read": [_vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _vp, _vp, _vp, _i64, _i32, _vp],
     "sa_kv4_attend": [_vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32,

@@ -30,14 +30,17 @@ def dtype_code(*ts: Tensor) -> int:
     return code
 
 
-def device_of(*ts: Tensor) -> torch.device:
+def device_of(first: Tensor, *others: Tensor) -> torch.device:
     """The CUDA device that all tensors are on."""
-    dev = ts[0].device
-    for t in ts:
-        if not t.is_cuda:
-            raise ValueError("the B200 kernels require CUDA tensors")
+    dev = first.device
+    for t in others:
         if t.device != dev:
+            for x in (first, *others):
+                if not x.is_cuda:
+                    raise ValueError("the B200 kernels require CUDA tensors")
             raise ValueError("all tensors must be on the same device")
+    if dev.type != "cuda":
+        raise ValueError("the B200 kernels require CUDA tensors")
     return dev
 
 
@@ -85,15 +88,11 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _raw_stream)
 
 def launch(dev: torch.device, name: str, *args) -> None:
     """Calls a serving entry point on the current stream of `dev`."""
-    if dev.index == torch.cuda.current_device():
-        _launch(dev, name, args)
-    else:
+    index = dev.index
+    if index != torch.cuda.current_device():
         with torch.cuda.device(dev):
-            _launch(dev, name, args)
-
-
-def _launch(dev: torch.device, name: str, args) -> None:
-    rc = getattr(_lib.load(), name)(*args, _raw_stream(dev.index))
+            return launch(dev, name, *args)
+    rc = getattr(_lib.load(), name)(*args, _raw_stream(index))
     if rc:
         _lib.check(rc, name)
     if _fast._CHECK_STATUS and not torch.cuda.is_current_stream_capturing():

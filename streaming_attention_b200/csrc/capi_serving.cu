@@ -122,7 +122,7 @@ int sa_window_attention_workspace_size(int batch, int heads, int kv_heads, int64
 
 int sa_window_attention(const void* q, const void* k, const void* v, void* out, const int64_t* strides, int batch,
                         int heads, int kv_heads, int64_t n, int64_t m, int d, int dv, int64_t window, int64_t sinks,
-                        float scale, int dtype, const int32_t* cu_q, const int32_t* cu_k, void* workspace,
+                        float scale, int dtype, const int32_t* cu_q, const int32_t* cu_k, int zero_behind, void* workspace,
                         size_t workspace_bytes, void* stream) {
   int rc = check_dtype(dtype);
   if (!rc) rc = check_heads(heads, kv_heads);
@@ -139,7 +139,7 @@ int sa_window_attention(const void* q, const void* k, const void* v, void* out, 
   const WindowArgs a{q,          k,          v,          out,        strides[0], strides[1], strides[2],  strides[3],
                      strides[4], strides[5], strides[6], strides[7], strides[8], strides[9], strides[10], strides[11],
                      batch,      heads,      kv_heads,   n,          m,          d,          dv,
-                     window > 0 ? window : (int64_t)1 << 40, sinks, scale, dtype, cu_q, cu_k, status_word()};
+                     window > 0 ? window : (int64_t)1 << 40, sinks, scale, dtype, cu_q, cu_k, status_word(), zero_behind};
   const char* simt = getenv("SA_FORCE_SIMT");
   if (window_tc_takes(a) && !(simt && simt[0] == '1')) return launch_window_tc(a, (cudaStream_t)stream);
   // float32 on the tensor cores: contiguous tensors and a workspace

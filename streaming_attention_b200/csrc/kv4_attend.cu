@@ -11,7 +11,8 @@
 //
 // A warp takes blocks of 16 tokens.  A code's bits, moved to the top of a
 // bfloat16's mantissa under the exponent of 16, are 16 + code: a shift and one
-// logical operation for two codes, exact.  With x = least - 16 scale the value is
+// logical operation for two codes, exact (float32 takes 24 off again: the sums'
+// errors grow with the offset).  With x = least - 16 scale the value is
 // s (16 + code) + x, so
 //   S = s_k (K_codes Q^T) + x_k sum(Q)         tokens x rows
 //   O = V_codes^T (p s_v)^T + sum(p x_v)       columns x rows
@@ -63,11 +64,13 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   return r;
 }
 
-// Two codes, nibble i of each half of w, plus 16, as bfloat16.
-template <int I>
+// Two codes, nibble i of each half of w, plus kOffset, as bfloat16.
+template <int I, int kOffset>
 __device__ __forceinline__ uint32_t codes(uint32_t w) {
-  const uint32_t x = I == 0 ? w << 3 : w >> (4 * I - 3);
-  return (x & 0x00780078u) | 0x41804180u;
+  uint32_t x = I == 0 ? w << 3 : w >> (4 * I - 3);
+  x = (x & 0x00780078u) | 0x41804180u;
+  if (kOffset == -8) asm("add.rn.bf16x2 %0, %0, %1;" : "+r"(x) : "r"(0xc1c0c1c0u));   // - 24
+  return x;
 }
 
 __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -208,6 +211,8 @@ template <int DT, int DP, int NT>
 __global__ void __launch_bounds__(kThreads, (Shape<DT, DP, NT>::kPerSm)) attend_kernel(const Kv4AttendArgs a) {
   using T = typename Elem<DT>::T;
   using S = Shape<DT, DP, NT>;
+  // codes enter the products plus 16; less 8 for float32, whose sums that shift would cost two bits
+  constexpr int kOff = DT == SA_REP_FLOAT32 ? -8 : 16;
   constexpr int kKS = DP / 16;   // k steps of the first product, 16-column tiles of the second
   extern __shared__ __align__(16) uint8_t smem[];
   float* sm_o = reinterpret_cast<float*>(smem);                // [warps][rows][pitch]
@@ -350,8 +355,8 @@ __global__ void __launch_bounds__(kThreads, (Shape<DT, DP, NT>::kPerSm)) attend_
       for (int e = 0; e < 4; ++e) s[nt][e] = 0.0f;
 #pragma unroll
     for (int w = 0; w < kKS / 2; ++w) {
-      uint32_t f[2][4] = {{codes<0>(b.k0[w]), codes<0>(b.k1[w]), codes<1>(b.k0[w]), codes<1>(b.k1[w])},
-                          {codes<2>(b.k0[w]), codes<2>(b.k1[w]), codes<3>(b.k0[w]), codes<3>(b.k1[w])}};
+      uint32_t f[2][4] = {{codes<0, kOff>(b.k0[w]), codes<0, kOff>(b.k1[w]), codes<1, kOff>(b.k0[w]), codes<1, kOff>(b.k1[w])},
+                          {codes<2, kOff>(b.k0[w]), codes<2, kOff>(b.k1[w]), codes<3, kOff>(b.k0[w]), codes<3, kOff>(b.k1[w])}};
 #pragma unroll
       for (int half = 0; half < 2; ++half)
 #pragma unroll
@@ -361,8 +366,8 @@ __global__ void __launch_bounds__(kThreads, (Shape<DT, DP, NT>::kPerSm)) attend_
             mma(s[nt], f[half][0], f[half][1], f[half][2], f[half][3], qf[nt][q][2 * w + half][0], qf[nt][q][2 * w + half][1]);
     }
     const float2 ka = params(b.kp.x), kb = params(b.kp.y), va = params(b.vp.x), vb = params(b.vp.y);
-    const float k_s[2] = {ka.x * sc, kb.x * sc}, k_x[2] = {fmaf(-16.0f, ka.x, ka.y) * sc, fmaf(-16.0f, kb.x, kb.y) * sc};
-    const float v_s[2] = {va.x, vb.x}, v_x[2] = {fmaf(-16.0f, va.x, va.y), fmaf(-16.0f, vb.x, vb.y)};
+    const float k_s[2] = {ka.x * sc, kb.x * sc}, k_x[2] = {fmaf(-(float)kOff, ka.x, ka.y) * sc, fmaf(-(float)kOff, kb.x, kb.y) * sc};
+    const float v_s[2] = {va.x, vb.x}, v_x[2] = {fmaf(-(float)kOff, va.x, va.y), fmaf(-(float)kOff, vb.x, vb.y)};
     uint32_t on = 0;   // bit 4 nt + e: s[nt][e] is seen
     if (!kWhole) {
 #pragma unroll
@@ -433,7 +438,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<DT, DP, NT>::kPerSm)) attend_
 #pragma unroll
     for (int t = 0; t < kKS; ++t) {
       const uint32_t w = b.v[t];
-      const uint32_t a0 = codes<0>(w), a1 = codes<1>(w), a2 = codes<2>(w), a3 = codes<3>(w);
+      const uint32_t a0 = codes<0, kOff>(w), a1 = codes<1, kOff>(w), a2 = codes<2, kOff>(w), a3 = codes<3, kOff>(w);
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll

@@ -51,6 +51,10 @@ __device__ __forceinline__ float from_f32<float>(float x) {
   return x;
 }
 template <>
+__device__ __forceinline__ uint16_t from_f32<uint16_t>(float) {   // bits of 0 alone
+  return 0;
+}
+template <>
 __device__ __forceinline__ __half from_f32<__half>(float x) {
   return __float2half_rn(x);
 }
@@ -116,7 +120,22 @@ struct WindowArgs {
   const int32_t* cu_q;
   const int32_t* cu_k;
   int* status;
+  int zero_behind;   // packed: write zeros to the rows behind the last request
 };
+
+// Zeros for the rows of out that belong to no request, dealt out to the grid's
+// threads (`threads` of each CTA, this one the `thread`-th).
+template <typename T>
+__device__ __forceinline__ void zero_rows_behind(const WindowArgs& a, int64_t thread, int64_t threads) {
+  if (!a.cu_q || !a.zero_behind) return;
+  const int64_t lead = min(max((int64_t)a.cu_q[0], (int64_t)0), a.n);   // and before the first
+  const int64_t first = min(max((int64_t)a.cu_q[a.batch], lead), a.n), width = (int64_t)a.heads * a.dv;
+  const int64_t cta = blockIdx.x + (int64_t)blockIdx.y * gridDim.x, ctas = (int64_t)gridDim.x * gridDim.y;
+  for (int64_t e = cta * threads + thread; e < (lead + a.n - first) * width; e += ctas * threads) {
+    const int64_t r = e / width, rest = e - r * width, h = rest / a.dv, row = r < lead ? r : first + r - lead;
+    static_cast<T*>(a.out)[h * a.o_h + row * a.o_n + rest - h * a.dv] = from_f32<T>(0.0f);
+  }
+}
 
 // One request of a (dense or packed) batch: first rows and row counts.
 struct Request {

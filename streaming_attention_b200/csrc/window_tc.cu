@@ -475,6 +475,7 @@ window_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
     __syncwarp();
   } else {
     // ------------------------------------------------------------ softmax rows
+    zero_rows_behind<T>(a, threadIdx.x - 64, kThreads - 64);
     const int t = (warp - 2) >> 2;
     const int quarter = warp & 3;
     const int row = quarter * 32 + lane;

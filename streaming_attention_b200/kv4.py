@@ -123,18 +123,20 @@ class Kv4Cache:
         if k_codes.ndim != 4:
             raise ValueError("k_codes must be [P,Hkv,page,Dp/2]")
         pages, heads, page, half = k_codes.shape
-        _check_page_size(page)
+        if page not in PAGE_SIZES:
+            _check_page_size(page)
         if pages == 0 or heads == 0:
             raise ValueError("the cache needs at least one page and one head")
         if half != self.padded_dim(dim) // 2:
             raise ValueError(f"a row of codes of dim {dim} takes {self.padded_dim(dim) // 2} bytes, got {half}")
         self.device = S.device_of(k_codes, k_params, v_codes, v_params)
-        for t, shape, dt, what in ((k_codes, (pages, heads, page, half), torch.uint8, "k_codes"),
+        params = (pages, heads, page, 2)
+        for t, shape, dt, what in ((k_codes, None, torch.uint8, "k_codes"),
                                    (v_codes, (pages, heads, page // 4, half, 4), torch.uint8, "v_codes"),
-                                   (k_params, (pages, heads, page, 2), torch.bfloat16, "k_params"),
-                                   (v_params, (pages, heads, page, 2), torch.bfloat16, "v_params")):
-            if tuple(t.shape) != shape or t.dtype != dt or not t.is_contiguous():
-                raise ValueError(f"{what} must be contiguous {dt} {list(shape)}")
+                                   (k_params, params, torch.bfloat16, "k_params"),
+                                   (v_params, params, torch.bfloat16, "v_params")):
+            if t.dtype != dt or (shape is not None and t.shape != shape) or not t.is_contiguous():
+                raise ValueError(f"{what} must be contiguous {dt} {list(shape or k_codes.shape)}")
         self.k_codes, self.k_params, self.v_codes, self.v_params = k_codes, k_params, v_codes, v_params
         self.dim, self.kv_heads, self.page_size, self.num_pages = int(dim), heads, page, pages
         self._args = (k_codes.data_ptr(), k_params.data_ptr(), v_codes.data_ptr(), v_params.data_ptr(), pages, heads,

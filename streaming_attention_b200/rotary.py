@@ -40,21 +40,23 @@ def qk_norm_rotary(q: Tensor, k: Tensor, positions: Tensor, q_weight: Optional[T
     ones.  A token of negative position is left out: its rows of a given ``out``
     pair stay as they were (``out=(q, k)`` works in place), of a new one are
     zero."""
-    if q.ndim != 3 or k.ndim != 3 or q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2]:
+    if q.ndim != 3 or k.ndim != 3:
         raise ValueError("q and k must be [T,H,D] and [T,Hkv,D]")
     t, heads, d = q.shape
-    kv_heads = k.shape[1]
+    kt, kv_heads, kd = k.shape
+    if kt != t or kd != d:
+        raise ValueError("q and k must be [T,H,D] and [T,Hkv,D]")
     given = [x for x in (q_weight, k_weight) if x is not None]
     dev = S.device_of(q, k, positions, frequencies, *given)
     code = S.dtype_code(q, k, *given)
     if not 1 <= d <= S.MAX_DIM:
         raise ValueError(f"the head width must lie in [1, {S.MAX_DIM}]")
     for w in given:
-        if w.shape != (d,):
+        if w.ndim != 1 or w.size(0) != d:
             raise ValueError(f"q_weight and k_weight must be [{d}]")
     if heads + kv_heads == 0:
         raise ValueError("at least one head is needed")
-    if frequencies.dtype != torch.float64 or frequencies.ndim != 1 or 2 * frequencies.shape[0] > d:
+    if frequencies.dtype != torch.float64 or frequencies.ndim != 1 or 2 * frequencies.size(0) > d:
         raise ValueError(f"frequencies must be float64 [R] with 2 R <= {d}")
     positions = S.int32(positions, (t,), "positions")
     fresh = out is None
@@ -70,5 +72,5 @@ def qk_norm_rotary(q: Tensor, k: Tensor, positions: Tensor, q_weight: Optional[T
         S.launch(dev, "sa_qk_norm_rotary", q.data_ptr(), k.data_ptr(), out[0].data_ptr(), out[1].data_ptr(),
                  positions.data_ptr(), S.ptr(q_weight), S.ptr(k_weight), frequencies.data_ptr(),
                  S.strides(*q.stride()[:2], *k.stride()[:2], *out[0].stride()[:2], *out[1].stride()[:2]), t, heads,
-                 kv_heads, d, frequencies.shape[0], float(eps), int(interleaved), int(fresh), code)
+                 kv_heads, d, frequencies.size(0), float(eps), int(interleaved), int(fresh), code)
     return out[0], out[1]

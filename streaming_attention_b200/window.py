@@ -88,7 +88,7 @@ def sliding_window_attention(q: Tensor, k: Tensor, v: Tensor, *, window: Optiona
         raise ValueError("q, k and v must have the same batch size")
     if m < n:
         raise ValueError(f"fewer keys ({m}) than queries ({n})")
-    out = torch.empty((b, heads, n, dv), device=dev, dtype=q.dtype)
+    out = q.new_empty((b, heads, n, dv))
     if out.numel():
         _check_heads(heads, kv_heads)
         ws = None
@@ -100,7 +100,7 @@ def sliding_window_attention(q: Tensor, k: Tensor, v: Tensor, *, window: Optiona
         q, k, v = _on_borders(q), _on_borders(k), _on_borders(v)
         S.launch(dev, "sa_window_attention", q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
                  S.strides(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *out.stride()[:3]), b, heads, kv_heads,
-                 n, m, d, dv, w, s, _scale(scale, d), code, None, None,
+                 n, m, d, dv, w, s, _scale(scale, d), code, None, None, 0,
                  None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel())
     return out[0, 0] if single else out
 
@@ -112,8 +112,8 @@ def sliding_window_attention_packed(q: Tensor, k: Tensor, v: Tensor, cu_q: Tenso
     [S,Hkv,D], v [S,Hkv,Dv]; ``cu_q`` and ``cu_k`` (int32 [R+1], on the device)
     are the requests' first rows, so that request r has rows cu_q[r]..cu_q[r+1]
     of q and cu_k[r]..cu_k[r+1] of k and v, its queries at the last of its
-    positions.  No length is read on the host.  Rows behind cu_q[R] are left as
-    they were in ``out`` ([T,H,Dv], made as zeros if not given)."""
+    positions.  No length is read on the host.  Rows of no request (behind
+    cu_q[R]) are left as they were in ``out`` ([T,H,Dv]); in a new one they are zero."""
     dev = S.device_of(q, k, v, cu_q, cu_k)
     if not q.ndim == k.ndim == v.ndim == 3:
         raise ValueError("q, k and v must be [T,H,D], [S,Hkv,D], [S,Hkv,Dv]")
@@ -128,8 +128,9 @@ def sliding_window_attention_packed(q: Tensor, k: Tensor, v: Tensor, cu_q: Tenso
         raise ValueError("cu_q must be [R+1]")
     cu_q = S.int32(cu_q, cu_q.shape, "cu_q")
     cu_k = S.int32(cu_k, cu_q.shape, "cu_k")
-    if out is None:
-        out = torch.zeros((t, heads, dv), device=dev, dtype=q.dtype)
+    fresh = out is None
+    if fresh:
+        out = q.new_empty((t, heads, dv)) if cu_q.size(0) > 1 else q.new_zeros((t, heads, dv))
     elif tuple(out.shape) != (t, heads, dv) or out.dtype != q.dtype or out.device != dev or (dv > 1 and out.stride(-1) != 1):
         raise ValueError(f"out must be [{t},{heads},{dv}] like q, its last dimension contiguous")
     if out.numel():
@@ -138,5 +139,5 @@ def sliding_window_attention_packed(q: Tensor, k: Tensor, v: Tensor, cu_q: Tenso
         S.launch(dev, "sa_window_attention", q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
                  S.strides(0, q.stride(1), q.stride(0), 0, k.stride(1), k.stride(0), 0, v.stride(1), v.stride(0), 0,
                            out.stride(1), out.stride(0)), cu_q.shape[0] - 1, heads, kv_heads, t, rows, d, dv, w, s,
-                 _scale(scale, d), code, cu_q.data_ptr(), cu_k.data_ptr(), None, 0)
+                 _scale(scale, d), code, cu_q.data_ptr(), cu_k.data_ptr(), int(fresh), None, 0)
     return out

@@ -18,7 +18,7 @@ def _strides(n):
 
 def _window(**kw):
     a = dict(q=P, k=P, v=P, out=P, strides=_strides(12), batch=1, heads=4, kv_heads=2, n=8, m=8, d=64, dv=64, window=4, sinks=0,
-             scale=1.0, dtype=2, cu_q=None, cu_k=None, ws=None, ws_bytes=0, stream=None)
+             scale=1.0, dtype=2, cu_q=None, cu_k=None, zero=0, ws=None, ws_bytes=0, stream=None)
     a.update(kw)
     return _lib.load().sa_window_attention(*a.values())
 
