@@ -244,6 +244,51 @@ __global__ void __launch_bounds__(kThreads, (Shape<DT, DP, NT>::kPerSm)) attend_
   const int blocks = sink_blocks + max(win_end - win_begin, 0);
   const float sc = a.scale * 1.4426950408889634f;   // log2(e): scores in base 2
 
+  // block u of this warp is block first + u * step of the visible ones
+  const int first = blockIdx.x * kWarps + warp, step = splits * kWarps;
+  const int mine = first < blocks ? (blocks - first + step - 1) / step : 0;
+  auto token_of = [&](int u) {
+    const int v = first + u * step;
+    return (v < sink_blocks ? v : win_begin + v - sink_blocks) << 4;
+  };
+  const int32_t* table = a.tables + (int64_t)r * a.width;
+  // page ids of the next 32 blocks, one a lane
+  int page_of = 0;
+  auto fetch_pages = [&](int u0) {
+    const int u = u0 + lane;
+    page_of = u < mine ? __ldg(table + (token_of(u) >> a.c.page_shift)) : 0;
+    if (u < mine && (page_of < 0 || page_of >= a.c.pages)) {
+      report(a.status, kBadPage, page_of);
+      page_of = -1;   // its tokens count as hidden
+    }
+  };
+  const int page_mask = (1 << a.c.page_shift) - 1;
+  const int page_step = a.c.heads << a.c.page_shift;   // cells of a page, all heads
+  const int64_t cell0 = (int64_t)hk << a.c.page_shift;
+  const Lanes at{a.c.k_codes + (cell0 + 2 * g) * (DP / 2) + cc * (DP / 8),
+                 a.c.v_codes + (cell0 + 4 * cc) * (DP / 2) + g * (DP >= 64 ? 16 : 8),
+                 reinterpret_cast<const uint8_t*>(a.c.k_params + 2 * (cell0 + 2 * g)),
+                 reinterpret_cast<const uint8_t*>(a.c.v_params + 2 * (cell0 + 2 * g))};
+  uint8_t* queue = smem + warp * kDepth * Queue<DP>::kSlot;
+  const uint32_t queue_u32 = static_cast<uint32_t>(__cvta_generic_to_shared(queue));
+  uint32_t sent = 0;   // bit of a slot: a block is in it
+  auto send = [&](int u) {
+    const int slot = u % kDepth;
+    sent &= ~(1u << slot);
+    if (u < mine) {
+      if ((u & 31) == 0) fetch_pages(u);
+      const int page = __shfl_sync(0xffffffffu, page_of, u & 31);
+      if (page >= 0) {
+        send_block<DP>(at, ((int64_t)page * page_step + (token_of(u) & page_mask)) * (DP / 2),
+                       queue_u32 + slot * Queue<DP>::kSlot, lane);
+        sent |= 1u << slot;
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  // the first blocks come in under the queries' set-up
+  for (int u = 0; u < kDepth - 1; ++u) send(u);
+
   // Q: fragments of this lane's row g (of each n tile) and the sums of the rows 2 cc, 2 cc + 1
   uint32_t qf[NT][S::kQ][kKS][2];
   float qsum[NT][2];
@@ -297,49 +342,6 @@ __global__ void __launch_bounds__(kThreads, (Shape<DT, DP, NT>::kPerSm)) attend_
       l[nt][e] = z[nt][e] = 0.0f;
     }
   }
-
-  // block u of this warp is block first + u * step of the visible ones
-  const int first = blockIdx.x * kWarps + warp, step = splits * kWarps;
-  const int mine = first < blocks ? (blocks - first + step - 1) / step : 0;
-  auto token_of = [&](int u) {
-    const int v = first + u * step;
-    return (v < sink_blocks ? v : win_begin + v - sink_blocks) << 4;
-  };
-  const int32_t* table = a.tables + (int64_t)r * a.width;
-  // page ids of the next 32 blocks, one a lane
-  int page_of = 0;
-  auto fetch_pages = [&](int u0) {
-    const int u = u0 + lane;
-    page_of = u < mine ? __ldg(table + (token_of(u) >> a.c.page_shift)) : 0;
-    if (u < mine && (page_of < 0 || page_of >= a.c.pages)) {
-      report(a.status, kBadPage, page_of);
-      page_of = -1;   // its tokens count as hidden
-    }
-  };
-  const int page_mask = (1 << a.c.page_shift) - 1;
-  const int page_step = a.c.heads << a.c.page_shift;   // cells of a page, all heads
-  const int64_t cell0 = (int64_t)hk << a.c.page_shift;
-  const Lanes at{a.c.k_codes + (cell0 + 2 * g) * (DP / 2) + cc * (DP / 8),
-                 a.c.v_codes + (cell0 + 4 * cc) * (DP / 2) + g * (DP >= 64 ? 16 : 8),
-                 reinterpret_cast<const uint8_t*>(a.c.k_params + 2 * (cell0 + 2 * g)),
-                 reinterpret_cast<const uint8_t*>(a.c.v_params + 2 * (cell0 + 2 * g))};
-  uint8_t* queue = smem + warp * kDepth * Queue<DP>::kSlot;
-  const uint32_t queue_u32 = static_cast<uint32_t>(__cvta_generic_to_shared(queue));
-  uint32_t sent = 0;   // bit of a slot: a block is in it
-  auto send = [&](int u) {
-    const int slot = u % kDepth;
-    sent &= ~(1u << slot);
-    if (u < mine) {
-      if ((u & 31) == 0) fetch_pages(u);
-      const int page = __shfl_sync(0xffffffffu, page_of, u & 31);
-      if (page >= 0) {
-        send_block<DP>(at, ((int64_t)page * page_step + (token_of(u) & page_mask)) * (DP / 2),
-                       queue_u32 + slot * Queue<DP>::kSlot, lane);
-        sent |= 1u << slot;
-      }
-    }
-    asm volatile("cp.async.commit_group;" ::: "memory");
-  };
 
   // off: what is added to a score before 2^x; the maximum is moved where a score passes kMove + kShift
   float off[NT][2];
@@ -452,7 +454,6 @@ __global__ void __launch_bounds__(kThreads, (Shape<DT, DP, NT>::kPerSm)) attend_
       work(b, token, std::false_type{});
   };
 
-  for (int u = 0; u < kDepth - 1; ++u) send(u);
   for (int u = 0; u < mine; ++u) {
     send(u + kDepth - 1);
     asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 1) : "memory");
@@ -558,11 +559,11 @@ int launch_one(const Kv4AttendArgs& a, cudaStream_t s) {
   const int64_t y = a.c.heads * ceil_div(rows, S::kRows);
   if (y > 65535) return set_error(SA_ERR_UNSUPPORTED, "kv4 attend: grid too large");
   // CTAs per (request, key head): while a warp keeps at least four blocks of the
-  // longest request the table allows and the grid has room for less than six
+  // longest request the table allows and the grid has less than three
   // rounds
   const int64_t longest = std::min<int64_t>((int64_t)a.width << a.c.page_shift, a.window + std::min(a.sinks, a.window) + a.n);
   int splits = 1;
-  while (splits < 8 && longest >= (int64_t)splits * 2 * kWarps * 16 * 4 && y * a.requests * splits < 148 * S::kPerSm * 6) splits *= 2;
+  while (splits < 8 && longest >= (int64_t)splits * 2 * kWarps * 16 * 4 && y * a.requests * splits < 148 * S::kPerSm * 3) splits *= 2;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)splits, (unsigned)y, (unsigned)a.requests);
   cfg.blockDim = dim3(kThreads);
