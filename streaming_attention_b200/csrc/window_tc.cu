@@ -20,14 +20,14 @@
 //
 // One CTA per SM works through query tile pairs (persistent: a pair's set-up,
 // first loads and stores run under its neighbours' products; as one CTA per pair
-// they took 40 % of the time).  Warps: 0 plans the pairs and loads (TMA), 1
-// issues the products (converged, one elected lane), 2..5 and 6..9 are the
-// softmax of query tile 0 and 1, one row per thread, 64 of its 128 scores in
-// registers at a time.
-// TMEM: S0 S1 O0 O1 of 128 columns each; P, in 16 bits, overwrites the first
-// half of its S.  The issue order per key tile is PV0 S0' PV1 S1', so that one
-// tile's softmax runs under the other's products; the commit of S(j + 1) also
-// says that PV(j) has ended, so that a row may then scale its O.
+// they took 40 % of the time).  Warps: 0 plans the pairs and loads (TMA), 1 and 2
+// issue the products of query tile 0 and 1 (converged, one elected lane), 3..6
+// and 7..10 are their softmax, one row per thread, a tile's 64 scores in
+// registers (more, of 128 columns, spilled: beside 220 KB of shared memory that
+// goes to L2).  TMEM: of each query tile two S of 64 columns and O of 128; P, in 16
+// bits, overwrites the first half of its S.  A tile's issuer goes P V(j), S(j + 2),
+// so that the next scores are there while a softmax runs; with one S of 128
+// columns each waited for the other (184 us for the 8192-token prompt).
 //
 // Softmax in base 2 with a lazily moved maximum: m follows a tile's maximum
 // only when that is more than kMove above it, so O is scaled rarely.  P is
@@ -53,9 +53,9 @@ namespace {
 using namespace tc;
 
 constexpr int kRows = 128;     // rows of a query tile
-constexpr int kCols = 128;     // keys of a key tile
+constexpr int kCols = 64;      // keys of a key tile
 constexpr int kSeam = 16;      // rows of a box of the seam tile
-constexpr int kThreads = 320;
+constexpr int kThreads = 352;
 constexpr float kMove = 8.0f;
 
 constexpr int kErrQ = 501, kErrFull = 502, kErrP = 503, kErrS = 504, kErrEmpty = 505, kErrO = 506, kErrDrain = 507,
@@ -241,7 +241,8 @@ __device__ __noinline__ void scale_row(uint32_t to, int dv, float alpha) {
 template <int DC, int VC>   // 64-column chunks of the head widths
 struct Layout {
   static constexpr uint32_t kQ = DC * kRows * 128;                              // one query tile
-  static constexpr uint32_t kSlot = (DC > VC ? DC : VC) * kCols * 128;          // one K or V tile
+  static constexpr uint32_t kTile = (DC > VC ? DC : VC) * kCols * 128;          // one K or V tile
+  static constexpr uint32_t kSlot = 2 * kTile;                                  // a group of the ring
   static constexpr int kSlots = DC == 2 || VC == 2 ? 4 : 8;
   static constexpr uint32_t kRing = 2 * kQ;
   static constexpr uint32_t kPitch = 80;                                        // a row's 32 columns, staged
@@ -265,15 +266,14 @@ window_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::kBars);
   uint64_t* empty = full + kSlots;
-  uint64_t* sfull = empty + kSlots;   // [2]
-  uint64_t* pfull = sfull + 2;        // [2 query tiles][2 halves of the key tile]
-  uint64_t* ofull = pfull + 4;        // [2]
-  uint64_t* qfull = ofull + 2;
+  uint64_t* sfull = empty + kSlots;   // [2 query tiles][2 score buffers]
+  uint64_t* pfull = sfull + 4;        // likewise
+  uint64_t* qfull = pfull + 4;
   uint64_t* qempty = qfull + 1;
-  uint64_t* plan_full = qempty + 1;   // [2]
+  uint64_t* plan_full = qempty + 1;       // [2]
   uint64_t* plan_empty = plan_full + 2;   // [2]
-  uint64_t* drain = plan_empty + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  uint64_t* drain = plan_empty + 2;       // [2]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 2);
   int* abort_word = reinterpret_cast<int*>(tmem_slot + 1);
   PairPlan* plans = reinterpret_cast<PairPlan*>(tmem_slot + 4);   // [2]
 
@@ -283,19 +283,19 @@ window_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
   if (threadIdx.x == 0) {
     for (int s = 0; s < kSlots; ++s) {
       mbar_init(&full[s], 1);
-      mbar_init(&empty[s], 1);
+      mbar_init(&empty[s], 2);   // both issuers
     }
-    for (int t = 0; t < 2; ++t) {
-      mbar_init(&sfull[t], 1);
-      mbar_init(&pfull[2 * t], 4);
-      mbar_init(&pfull[2 * t + 1], 4);
-      mbar_init(&ofull[t], 1);
-      mbar_init(&plan_full[t], 1);
-      mbar_init(&plan_empty[t], 9);   // the issuer and eight softmax warps
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(&sfull[i], 1);
+      mbar_init(&pfull[i], 4);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&plan_full[i], 1);
+      mbar_init(&plan_empty[i], 10);   // two issuers and eight softmax warps
+      mbar_init(&drain[i], 1);
     }
     mbar_init(qfull, 1);
-    mbar_init(qempty, 1);
-    mbar_init(drain, 1);
+    mbar_init(qempty, 2);
     *abort_word = 0;
     fence_mbar_init();
     fence_proxy_async_smem();
@@ -338,30 +338,36 @@ window_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
         } else {
           mbar_arrive(qfull);
         }
+        // group 0: K of tiles 0 and 1; group g: V of tile g - 1 and K of tile g + 1
 #pragma unroll 1
-        for (int i = 0; i < 2 * c.tiles; ++i, ++u) {   // K of a key tile, then its V
-          const int s = u % kSlots, v0 = (i >> 1) * kCols;
+        for (int g = 0; c.tiles > 0 && g <= c.tiles; ++g, ++u) {
+          const int s = u % kSlots;
           if (u >= kSlots && !mbar_wait(&empty[s], ((u / kSlots) - 1) & 1, ab, kErrEmpty)) {
             ok = false;
             break;
           }
-          const bool isv = i & 1;
-          const int chunks = isv ? VC : DC;
-          uint8_t* dst = smem + L::kRing + s * L::kSlot;
-          mbar_arrive_expect_tx(&full[s], chunks * kCols * 128);
+          const int second = g == 0 ? 1 : g + 1;   // the key tile of the second half, if there is one
+          const bool two = second < c.tiles;
+          mbar_arrive_expect_tx(&full[s], ((g == 0 ? DC : VC) + (two ? DC : 0)) * kCols * 128);
 #pragma unroll 1
-          for (int j = 0; j < chunks; ++j, dst += kCols * 128) {
-            if (v0 >= c.fill) {
-              tma_load_4d(dst, isv ? &tm_v : &tm_k, &full[s], j * 64, c.base + v0, c.hk, kb);
-            } else if (c.fill == kSeam) {
-              tma_load_4d(dst, isv ? &tm_vs : &tm_ks, &full[s], j * 64, c.k_row, c.hk, kb);
-              tma_load_4d(dst + kSeam * 128, isv ? &tm_vw : &tm_kw, &full[s], j * 64, c.base + kSeam, c.hk, kb);
-            } else {
+          for (int half = 0; half < (two ? 2 : 1); ++half) {
+            const bool isv = g > 0 && half == 0;
+            const int v0 = (half ? second : (g == 0 ? 0 : g - 1)) * kCols;
+            uint8_t* dst = smem + L::kRing + s * L::kSlot + half * L::kTile;
 #pragma unroll 1
-              for (int r = 0; r < kCols; r += kSeam) {
-                const int v = v0 + r;
-                tma_load_4d(dst + r * 128, isv ? &tm_vs : &tm_ks, &full[s], j * 64, v < c.fill ? c.k_row + v : c.base + v,
-                            c.hk, kb);
+            for (int j = 0; j < (isv ? VC : DC); ++j, dst += kCols * 128) {
+              if (v0 >= c.fill) {
+                tma_load_4d(dst, isv ? &tm_v : &tm_k, &full[s], j * 64, c.base + v0, c.hk, kb);
+              } else if (c.fill == kSeam) {
+                tma_load_4d(dst, isv ? &tm_vs : &tm_ks, &full[s], j * 64, c.k_row, c.hk, kb);
+                tma_load_4d(dst + kSeam * 128, isv ? &tm_vw : &tm_kw, &full[s], j * 64, c.base + kSeam, c.hk, kb);
+              } else {
+#pragma unroll 1
+                for (int r = 0; r < kCols; r += kSeam) {
+                  const int v = v0 + r;
+                  tma_load_4d(dst + r * 128, isv ? &tm_vs : &tm_ks, &full[s], j * 64,
+                              v < c.fill ? c.k_row + v : c.base + v, c.hk, kb);
+                }
               }
             }
           }
@@ -382,12 +388,14 @@ window_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
       }
     }
     __syncwarp();
-  } else if (warp == 1) {
-    // ------------------------------------------------------------ products
+  } else if (warp <= 2) {
+    // ------------------------------------------------------------ products of query tile t
     const int ksteps = (a.d + 15) >> 4;
     const uint32_t id_pv = idesc_f16(kRows, (a.dv + 15) & ~15, DT == SA_REP_BFLOAT16, false, true);
-    int u = 0;                                       // ring loads before this pair
-    int count_p[2][2] = {{0, 0}, {0, 0}};            // halves of P waited for
+    const int t = warp - 1;
+    const uint32_t q_smem = smem_u32(smem + t * L::kQ), ring = smem_u32(smem + L::kRing);
+    int u = 0;                 // ring groups before this pair
+    int count_p[2] = {0, 0};   // P tiles waited for in each buffer
     bool ok = true;
 #pragma unroll 1
     for (int pair = 0; ok; ++pair) {
@@ -395,78 +403,76 @@ window_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
       if (!ok) break;
       const PairPlan& c = plans[pair & 1];
       if (c.live < 0) break;
-      const int tiles = c.tiles, total = c.total, sk = c.sk, lo[2] = {c.lo[0], c.lo[1]}, last[2] = {c.last[0], c.last[1]};
+      const int tiles = c.tiles, total = c.total, sk = c.sk, lo = c.lo[t], last = c.last[t];
       __syncwarp();
       if (lane == 0) mbar_arrive(&plan_empty[pair & 1]);
-      auto needed = [&](int t, int j) { return j * kCols <= last[t] && (j * kCols + kCols > lo[t] || j * kCols < sk); };
+      auto needed = [&](int j) { return j * kCols <= last && (j * kCols + kCols > lo || j * kCols < sk); };
       // columns of tile j that a product takes: a multiple of 32
       auto width = [&](int j) { return min(kCols, (total - j * kCols + 31) & ~31); };
+      // S of tile j into buffer j & 1 (called by one lane)
+      auto scores = [&](int j) {
+        const int group = u + (j < 2 ? 0 : j - 1);
+        const uint64_t qd = sdesc_sw128(q_smem, 16, 1024);
+        const uint64_t kd = sdesc_sw128(ring + (group % kSlots) * L::kSlot + (j == 0 ? 0 : L::kTile), 16, 1024);
+        const uint32_t id_s = idesc_f16(kRows, width(j), DT == SA_REP_BFLOAT16, false, false);
+        const uint32_t to = tS[t] + (j & 1) * kCols;
+        // unrolled: descriptors that are constants apart stay in uniform registers
+#pragma unroll
+        for (int kk = 0; kk < DC * 4; ++kk)
+          if (kk < ksteps)
+            mma_f16_ss(to, qd + (uint64_t)(((kk >> 2) * (kRows * 128) + (kk & 3) * 32) >> 4),
+                       kd + (uint64_t)(((kk >> 2) * (kCols * 128) + (kk & 3) * 32) >> 4), id_s, kk > 0 ? 1u : 0u);
+      };
       ok = mbar_wait_warp_lazy(qfull, pair & 1, ab, kErrQ);
-      bool begun[2] = {false, false};
+      if (ok && tiles > 0) ok = mbar_wait_warp_lazy(&full[u % kSlots], (u / kSlots) & 1, ab, kErrFull);
+      if (!ok) break;
+      tc_fence_after();
+      if (elect_one()) {
 #pragma unroll 1
-      for (int j = 0; ok && j <= tiles; ++j) {
-        const int us = u + 2 * j, uv = us - 1;   // ring positions of K(j) and V(j - 1)
-        bool waited_k = false, waited_v = false;
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          if (ok && j > 0 && needed(t, j - 1)) {
-            if (!waited_v) ok = mbar_wait_warp_lazy(&full[uv % kSlots], (uv / kSlots) & 1, ab, kErrFull);
-            waited_v = true;
-            const int steps = width(j - 1) >> 4;
-            const uint64_t vd = sdesc_sw128(smem_u32(smem + L::kRing + (uv % kSlots) * L::kSlot), kCols * 128, 1024);
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {   // keys 0..63 of the tile, then the rest
-              if (ok && half * 4 < steps) {
-                ok = mbar_wait_warp_lazy(&pfull[2 * t + half], count_p[t][half] & 1, ab, kErrP);
-                ++count_p[t][half];
-                tc_fence_after();
-                if (ok && elect_one()) {
-                  // unrolled: descriptors that are constants apart stay in uniform registers
-#pragma unroll
-                  for (int kk = half * 4; kk < half * 4 + 4; ++kk)
-                    if (kk < steps)
-                      mma_f16_ts(tO[t], tS[t] + kk * 8, vd + (uint64_t)((kk * 16 * 128) >> 4), id_pv,
-                                 (begun[t] || kk > 0) ? 1u : 0u);
-                  if ((half == 1 || steps <= 4) && j - 1 == last[t] / kCols) mma_commit(&ofull[t]);
-                }
-                __syncwarp();
-              }
-            }
-            begun[t] = true;
+        for (int j = 0; j < min(tiles, 2); ++j)
+          if (needed(j)) {
+            scores(j);
+            mma_commit(&sfull[2 * t + j]);
           }
-          if (ok && j < tiles && needed(t, j)) {
-            if (!waited_k) ok = mbar_wait_warp_lazy(&full[us % kSlots], (us / kSlots) & 1, ab, kErrFull);
-            waited_k = true;
-            if (ok) {
-              tc_fence_after();
-              const uint32_t id_s = idesc_f16(kRows, width(j), DT == SA_REP_BFLOAT16, false, false);
-              if (elect_one()) {
-                const uint64_t qd = sdesc_sw128(smem_u32(smem + t * L::kQ), 16, 1024);
-                const uint64_t kd = sdesc_sw128(smem_u32(smem + L::kRing + (us % kSlots) * L::kSlot), 16, 1024);
-#pragma unroll
-                for (int kk = 0; kk < DC * 4; ++kk) {
-                  const uint64_t at = (uint64_t)(((kk >> 2) * (kRows * 128) + (kk & 3) * 32) >> 4);
-                  if (kk < ksteps) mma_f16_ss(tS[t], qd + at, kd + at, id_s, kk > 0 ? 1u : 0u);
-                }
-                mma_commit(&sfull[t]);
-              }
-              __syncwarp();
-            }
-          }
+        if (tiles > 0) mma_commit(&empty[u % kSlots]);
+        if (tiles <= 2) mma_commit(qempty);
+      }
+      __syncwarp();
+      bool begun = false;
+#pragma unroll 1
+      for (int j = 0; j < tiles; ++j) {
+        const int group = u + j + 1, buf = j & 1;
+        const bool pv = needed(j), next = j + 2 < tiles && needed(j + 2);
+        ok = mbar_wait_warp_lazy(&full[group % kSlots], (group / kSlots) & 1, ab, kErrFull);
+        if (ok && pv) {
+          ok = mbar_wait_warp_lazy(&pfull[2 * t + buf], count_p[buf] & 1, ab, kErrP);
+          ++count_p[buf];
         }
-        if (ok && elect_one()) {
-          if (j > 0) mma_commit(&empty[uv % kSlots]);
-          if (j < tiles) mma_commit(&empty[us % kSlots]);
-          // the queries' last product (or, without keys, nothing) is issued
-          if (j == tiles - 1 || tiles == 0) mma_commit(qempty);
+        if (!ok) break;
+        tc_fence_after();
+        if (elect_one()) {
+          if (pv) {
+            const int steps = width(j) >> 4;
+            const uint64_t vd = sdesc_sw128(ring + (group % kSlots) * L::kSlot, kCols * 128, 1024);
+#pragma unroll
+            for (int kk = 0; kk < kCols / 16; ++kk)
+              if (kk < steps)
+                mma_f16_ts(tO[t], tS[t] + buf * kCols + kk * 8, vd + (uint64_t)((kk * 16 * 128) >> 4), id_pv,
+                           (begun || kk > 0) ? 1u : 0u);
+          }
+          if (next) scores(j + 2);
+          if (pv || next) mma_commit(&sfull[2 * t + buf]);
+          mma_commit(&empty[group % kSlots]);
+          if (j + 3 == tiles) mma_commit(qempty);   // the queries' last product is issued
         }
         __syncwarp();
+        begun |= pv;
       }
-      u += 2 * tiles;
+      u += tiles > 0 ? tiles + 1 : 0;
     }
-    if (elect_one()) mma_commit(drain);
+    if (elect_one()) mma_commit(&drain[t]);
     const uint64_t t0 = globaltimer_ns();
-    while (!mbar_try_wait(drain, 0)) {
+    while (!mbar_try_wait(&drain[t], 0)) {
       if (globaltimer_ns() - t0 > 2000000000ull) {
         if (a.status) atomicCAS(a.status, 0, kErrDrain);
         break;
@@ -475,17 +481,16 @@ window_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
     __syncwarp();
   } else {
     // ------------------------------------------------------------ softmax rows
-    zero_rows_behind<T>(a, threadIdx.x - 64, kThreads - 64);
-    const int t = (warp - 2) >> 2;
+    zero_rows_behind<T>(a, threadIdx.x - 96, kThreads - 96);
+    const int t = (warp - 3) >> 2;
     const int quarter = warp & 3;
     const int row = quarter * 32 + lane;
     const int tq = kRows >> p.pack_log;                      // queries of a tile
     const int qi = t * tq + (row >> p.pack_log);             // query of the pair
     const uint32_t at = (uint32_t)(quarter * 32) << 16;
     const float c2 = a.scale * 1.4426950408889634f;          // log2(e); not negative (window_tc_takes)
-    const uint32_t ts = tS[t] + at;
-    uint8_t* stage = smem + L::kStage + (warp - 2) * 32 * L::kPitch;
-    int count = 0, outs = 0;   // score tiles and outputs so far
+    uint8_t* stage = smem + L::kStage + (warp - 3) * 32 * L::kPitch;
+    int count[2] = {0, 0};   // what the issuer has committed to each score buffer's barrier
     bool ok = true;
 #pragma unroll 1
     for (int pair = 0; ok; ++pair) {
@@ -496,100 +501,70 @@ window_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
       // rows behind the last query count as that query: they need no masks of their own
       const int hi = c.hi + min(qi, c.nq - 1);
       const int lo = hi - (int)min(a.window, (int64_t)1 << 30) + 1;
-      const int total = c.total, sk = c.sk, tlo = c.lo[t], tlast = c.last[t];
+      const int tiles = c.tiles, total = c.total, sk = c.sk, tlo = c.lo[t], tlast = c.last[t];
       float m = -INFINITY, l = 0.0f;
       int done = 0;
+      auto needed = [&](int j) {   // as the issuer's
+        return j < tiles && j * kCols <= tlast && (j * kCols + kCols > tlo || j * kCols < sk);
+      };
+      // step j of the issuer: P V of tile j, then S of tile j + 2 into the same
+      // buffer, then a commit; so the commit that brings S(j) says that P V of tile
+      // j - 2 has ended, and the two behind the last tile that all have
 #pragma unroll 1
-      for (int v0 = 0; v0 <= tlast; v0 += kCols) {
-        if (v0 + kCols <= tlo && v0 >= sk) continue;   // as the issuer's needed()
-        if (!mbar_wait_warp_lazy(&sfull[t], count & 1, ab, kErrS)) {
-          ok = false;
-          break;
-        }
-        ++count;
+      for (int j = 0; j < tiles + 2; ++j) {
+        const int buf = j & 1;
+        const bool here = needed(j);
+        if (!here && (j < 2 || !needed(j - 2))) continue;
+        ok = mbar_wait_warp_lazy(&sfull[2 * t + buf], count[buf] & 1, ab, kErrS);
+        if (!ok) break;
+        ++count[buf];
+        if (!here) continue;
         tc_fence_after();
         // columns of a last, narrower tile that its product left out hold an earlier tile's numbers: hidden like others
-        const int w = min(kCols, (total - v0 + 31) & ~31);
+        const int v0 = j * kCols, w = min(kCols, (total - v0 + 31) & ~31);
+        const uint32_t ts = tS[t] + at + buf * kCols;
         // a tile that all rows of the warp see whole needs no mask
         const bool all_on = __all_sync(0xffffffffu, v0 + kCols - 1 <= hi && (v0 >= lo || v0 + kCols <= sk));
-        auto hide_chunk = [&](float (&x)[32], int i) {
-          const int vc = v0 + i * 32;
-          hide(x, low_bits(hi - vc + 1) & (~low_bits(lo - vc) | low_bits(sk - vc)) & low_bits(w - i * 32));
-        };
-        // the upper 64 columns are read for their maximum, then again for their
-        // exponentials: 64 scores in registers, not 128 (which spill)
         float s0[32], s1[32];
-        float top;
-        {
-          float b0[32], b1[32];
-          tmem_ld32(ts + 64, b0);
-          tmem_ld32(ts + 96, b1);
-          tmem_wait_ld();
-          tie32(b0);
-          tie32(b1);
-          tmem_ld32(ts, s0);
-          if (!all_on) {
-            hide_chunk(b0, 2);
-            hide_chunk(b1, 3);
-          }
-          top = fmaxf(max32(b0), max32(b1));
-        }
+        tmem_ld32(ts, s0);
         tmem_ld32(ts + 32, s1);
         tmem_wait_ld();
         tie32(s0);
         tie32(s1);
         if (!all_on) {
-          hide_chunk(s0, 0);
-          hide_chunk(s1, 1);
+          auto seen = [&](int v) { return low_bits(hi - v + 1) & (~low_bits(lo - v) | low_bits(sk - v)) & low_bits(v0 + w - v); };
+          hide(s0, seen(v0));
+          hide(s1, seen(v0 + 32));
         }
-        top = fmaxf(top, fmaxf(max32(s0), max32(s1))) * c2;
+        const float top = fmaxf(max32(s0), max32(s1)) * c2;
         const bool move = top > m + kMove;
         if (__any_sync(0xffffffffu, move)) {
           const float to = move ? top : m;
           const float alpha = move ? ex2(m - to) : 1.0f;   // m = -inf: 0
           m = to;
           l *= alpha;
-          if (done > 0)   // the products of this row's earlier tiles have ended (sfull)
+          if (done > 0) {
+            // the product of the tile before may still run: its step's commit ends the wait (and is not used up)
+            if (needed(j - 1)) ok = mbar_wait_warp_lazy(&sfull[2 * t + (buf ^ 1)], count[buf ^ 1] & 1, ab, kErrO);
+            if (!ok) break;
+            tc_fence_after();
             scale_row(tO[t] + at, a.dv, alpha);
+          }
         }
         const float off = kShift - (m == -INFINITY ? 0.0f : m);
         const uint64_t off2 = pack2(off, off), c22 = pack2(c2, c2);
         uint64_t sum2[2] = {0, 0};
-        // the first 64 keys' products start under the rest's exponentials
-        auto hand_over = [&](int half) {
-          tmem_wait_st();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&pfull[2 * t + half]);
-        };
         exp_chunk<DT>(s0, c22, off2, sum2, ts);
-        tmem_ld32(ts + 64, s0);
         exp_chunk<DT>(s1, c22, off2, sum2, ts + 16);
-        tmem_ld32(ts + 96, s1);
-        hand_over(0);
-        if (w > 64) {
-          tmem_wait_ld();
-          tie32(s0);
-          tie32(s1);
-          if (!all_on) {
-            hide_chunk(s0, 2);
-            hide_chunk(s1, 3);
-          }
-          exp_chunk<DT>(s0, c22, off2, sum2, ts + 32);
-          exp_chunk<DT>(s1, c22, off2, sum2, ts + 48);
-          hand_over(1);
-        } else {
-          tmem_wait_ld();
-        }
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&pfull[2 * t + buf]);
         float x0, x1, x2, x3;
         unpack2(sum2[0], x0, x1);
         unpack2(sum2[1], x2, x3);
         l += (x0 + x1) + (x2 + x3);
         ++done;
-      }
-      if (ok && done > 0) {
-        ok = mbar_wait_warp_lazy(&ofull[t], outs & 1, ab, kErrO);
-        ++outs;
       }
       if (!ok) break;
       tc_fence_after();
