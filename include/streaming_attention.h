@@ -347,7 +347,8 @@ int sa_serving_status(void* stream);
  * requests' first rows in q / out (n rows in all) and k / v (m rows in all),
  * p counts within the request, the *_b strides are 0; rows behind
  * cu_q[batch] stay as they were, or are zeroed (zero_behind != 0).  d, dv <= 256.
- * Tensor cores: float16 / bfloat16 of d, dv <= 128 on 16-byte borders; dense
+ * Tensor cores: float16 / bfloat16 of d, dv <= 128 on 16-byte borders (few
+ * queries over many keys: split over the SMs, given the workspace); dense
  * contiguous float32 (3xTF32) of d <= 64, dv <= 128 and long enough given a workspace of
  * sa_window_attention_workspace_size bytes (256-byte aligned; 0: none is used).
  * CUDA cores otherwise. */

@@ -116,7 +116,22 @@ int sa_window_attention_workspace_size(int batch, int heads, int kv_heads, int64
   if (!rc) rc = check_heads(heads, kv_heads);
   if (rc) return rc;
   if (batch < 0 || n < 0 || m < 0 || d <= 0 || dv <= 0 || window < 0 || sinks < 0) return set_error(SA_ERR_INVALID_ARG, "bad sizes");
-  *bytes = dtype == SA_REP_FLOAT32 ? window_tf32_bytes(batch, heads, kv_heads, n, m, d, dv, window, sinks) : 0;
+  *bytes = 0;
+  if (batch == 0 || n == 0 || m < n) return SA_OK;
+  if (dtype == SA_REP_FLOAT32) {
+    *bytes = window_tf32_bytes(batch, heads, kv_heads, n, m, d, dv, window, sinks);
+  } else if (d <= 128 && dv <= 128) {
+    WindowArgs a{};
+    a.batch = batch;
+    a.heads = heads;
+    a.kv_heads = kv_heads;
+    a.n = n;
+    a.m = m;
+    a.dv = dv;
+    a.window = window > 0 ? window : (int64_t)1 << 40;
+    a.sinks = sinks;
+    *bytes = window_tc_bytes(a);
+  }
   return SA_OK;
 }
 
@@ -141,7 +156,7 @@ int sa_window_attention(const void* q, const void* k, const void* v, void* out, 
                      batch,      heads,      kv_heads,   n,          m,          d,          dv,
                      window > 0 ? window : (int64_t)1 << 40, sinks, scale, dtype, cu_q, cu_k, status_word(), zero_behind};
   const char* simt = getenv("SA_FORCE_SIMT");
-  if (window_tc_takes(a) && !(simt && simt[0] == '1')) return launch_window_tc(a, (cudaStream_t)stream);
+  if (window_tc_takes(a) && !(simt && simt[0] == '1')) return launch_window_tc(a, workspace, workspace_bytes, (cudaStream_t)stream);
   // float32 on the tensor cores: contiguous tensors and a workspace
   if (dtype == SA_REP_FLOAT32 && !cu_q && workspace && a.status && a.q_n == d && a.q_h == n * d && a.q_b == heads * a.q_h &&
       a.k_n == d && a.k_h == m * d && a.k_b == kv_heads * a.k_h && a.v_n == dv && a.v_h == m * dv &&

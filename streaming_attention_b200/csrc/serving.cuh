@@ -199,7 +199,8 @@ __host__ __device__ inline KeyRanges key_ranges(int64_t p0, int64_t p1, int64_t 
 
 int launch_window_simt(const WindowArgs& a, cudaStream_t s);
 bool window_tc_takes(const WindowArgs& a);
-int launch_window_tc(const WindowArgs& a, cudaStream_t s);
+size_t window_tc_bytes(const WindowArgs& a);
+int launch_window_tc(const WindowArgs& a, void* workspace, size_t workspace_bytes, cudaStream_t s);
 size_t window_tf32_bytes(int64_t batch, int heads, int kv_heads, int64_t n, int64_t m, int d, int dv, int64_t window,
                          int64_t sinks);
 int window_tf32_run(const WindowArgs& a, void* workspace, size_t workspace_bytes, cudaStream_t s);

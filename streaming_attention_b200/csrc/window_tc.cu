@@ -29,6 +29,9 @@
 // so that the next scores are there while a softmax runs; with one S of 128
 // columns each waited for the other (184 us for the 8192-token prompt).
 //
+// Where a dense call has few pairs and many keys, a pair's key tiles are dealt
+// into parts that run as items of their own and are joined by join_kernel.
+//
 // Softmax in base 2 with a lazily moved maximum: m follows a tile's maximum
 // only when that is more than kMove above it, so O is scaled rarely.  P is
 // 2^(x - m + kShift): bfloat16 takes kShift = -24 (float32's range, so that
@@ -41,6 +44,8 @@
 // visible keys alone (row_again): what a query does not see cannot reach it.
 #include <cuda.h>
 #include <math.h>
+
+#include <algorithm>
 
 #include "serving.cuh"
 #include "tc_util.cuh"
@@ -67,7 +72,10 @@ struct WindowTcParams {
   int pack_log;              // pack = 1 << pack_log
   int rows_per_cta;          // queries of a CTA (2 * kRows / pack)
   int vec_out;               // out rows take 16-byte stores
-  uint32_t tiles, items;     // query tile pairs of one tile of heads, and of all
+  uint32_t tiles, items;     // query tile pairs of one tile of heads, and work items (pairs times splits) of all
+  int splits;                // parts that a pair's keys are dealt into
+  float* part;               // splits > 1: [row][split][pitch], O (not divided), m, l
+  int pitch;
   uint64_t wait_ns;
 };
 
@@ -103,7 +111,9 @@ struct PairPlan {
   int q_row, nq;   // first query's row in q, queries
   int k_row, m;    // first key's row in k, keys of the request
   int p0;          // position of the first query
-  int tiles, total, fill, sk;
+  int j0, tiles;   // first key tile, key tiles
+  int split;
+  int total, fill, sk;
   int base;        // column V >= fill is row base + V of k
   int hi;          // hi of the first query; query i's is hi + i
   int lo[2], last[2];   // columns that query tile t needs: lo[t] (or below sk) .. last[t]
@@ -112,6 +122,9 @@ struct PairPlan {
 __device__ __forceinline__ PairPlan plan_pair(const WindowTcParams& p, uint32_t item) {
   const WindowArgs& a = p.a;
   PairPlan c;
+  const uint32_t whole = item / (uint32_t)p.splits;
+  c.split = (int)(item - whole * p.splits);
+  item = whole;
   const uint32_t y = item / p.tiles;
   int64_t tile;
   c.b = tile_request(a, item - y * p.tiles, p.rows_per_cta, &tile);
@@ -127,7 +140,9 @@ __device__ __forceinline__ PairPlan plan_pair(const WindowTcParams& p, uint32_t 
   const int64_t p0 = rq.m - rq.n + i0;
   c.p0 = (int)p0;
   const Columns cols = columns_of(p0, p0 + c.nq - 1, rq.m, a.window, a.sinks);
-  c.tiles = (cols.total + kCols - 1) / kCols;
+  const int64_t all = (cols.total + kCols - 1) / kCols;
+  c.j0 = (int)(all * c.split / p.splits);
+  c.tiles = (int)(all * (c.split + 1) / p.splits) - c.j0;
   c.total = cols.total;
   c.fill = cols.fill;
   c.sk = cols.sk;
@@ -352,7 +367,7 @@ window_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
 #pragma unroll 1
           for (int half = 0; half < (two ? 2 : 1); ++half) {
             const bool isv = g > 0 && half == 0;
-            const int v0 = (half ? second : (g == 0 ? 0 : g - 1)) * kCols;
+            const int v0 = (c.j0 + (half ? second : (g == 0 ? 0 : g - 1))) * kCols;
             uint8_t* dst = smem + L::kRing + s * L::kSlot + half * L::kTile;
 #pragma unroll 1
             for (int j = 0; j < (isv ? VC : DC); ++j, dst += kCols * 128) {
@@ -404,11 +419,13 @@ window_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
       const PairPlan& c = plans[pair & 1];
       if (c.live < 0) break;
       const int tiles = c.tiles, total = c.total, sk = c.sk, lo = c.lo[t], last = c.last[t];
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&plan_empty[pair & 1]);
-      auto needed = [&](int j) { return j * kCols <= last && (j * kCols + kCols > lo || j * kCols < sk); };
+      const int start = c.j0 * kCols;
+      auto needed = [&](int j) {
+        const int v = start + j * kCols;
+        return v <= last && (v + kCols > lo || v < sk);
+      };
       // columns of tile j that a product takes: a multiple of 32
-      auto width = [&](int j) { return min(kCols, (total - j * kCols + 31) & ~31); };
+      auto width = [&](int j) { return min(kCols, (total - start - j * kCols + 31) & ~31); };
       // S of tile j into buffer j & 1 (called by one lane)
       auto scores = [&](int j) {
         const int group = u + (j < 2 ? 0 : j - 1);
@@ -423,6 +440,8 @@ window_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
             mma_f16_ss(to, qd + (uint64_t)(((kk >> 2) * (kRows * 128) + (kk & 3) * 32) >> 4),
                        kd + (uint64_t)(((kk >> 2) * (kCols * 128) + (kk & 3) * 32) >> 4), id_s, kk > 0 ? 1u : 0u);
       };
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&plan_empty[pair & 1]);
       ok = mbar_wait_warp_lazy(qfull, pair & 1, ab, kErrQ);
       if (ok && tiles > 0) ok = mbar_wait_warp_lazy(&full[u % kSlots], (u / kSlots) & 1, ab, kErrFull);
       if (!ok) break;
@@ -501,11 +520,12 @@ window_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
       // rows behind the last query count as that query: they need no masks of their own
       const int hi = c.hi + min(qi, c.nq - 1);
       const int lo = hi - (int)min(a.window, (int64_t)1 << 30) + 1;
-      const int tiles = c.tiles, total = c.total, sk = c.sk, tlo = c.lo[t], tlast = c.last[t];
+      const int tiles = c.tiles, total = c.total, sk = c.sk, tlo = c.lo[t], tlast = c.last[t], start = c.j0 * kCols;
       float m = -INFINITY, l = 0.0f;
       int done = 0;
       auto needed = [&](int j) {   // as the issuer's
-        return j < tiles && j * kCols <= tlast && (j * kCols + kCols > tlo || j * kCols < sk);
+        const int v = start + j * kCols;
+        return j < tiles && v <= tlast && (v + kCols > tlo || v < sk);
       };
       // step j of the issuer: P V of tile j, then S of tile j + 2 into the same
       // buffer, then a commit; so the commit that brings S(j) says that P V of tile
@@ -521,7 +541,7 @@ window_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
         if (!here) continue;
         tc_fence_after();
         // columns of a last, narrower tile that its product left out hold an earlier tile's numbers: hidden like others
-        const int v0 = j * kCols, w = min(kCols, (total - v0 + 31) & ~31);
+        const int v0 = start + j * kCols, w = min(kCols, (total - v0 + 31) & ~31);
         const uint32_t ts = tS[t] + at + buf * kCols;
         // a tile that all rows of the warp see whole needs no mask
         const bool all_on = __all_sync(0xffffffffu, v0 + kCols - 1 <= hi && (v0 >= lo || v0 + kCols <= sk));
@@ -574,6 +594,28 @@ window_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
       // lanes store neighbouring pieces of a row (16 bytes; the pitch keeps the
       // banks apart)
       T* out = static_cast<T*>(a.out) + obase;
+      if (p.splits > 1) {   // this part's O, maximum and sum, for join_kernel
+        const int64_t h = h0 + (row & (p.pack - 1)), r = (c.b * (int64_t)a.heads + h) * a.n + c.q_row + qi;
+        float* to = p.part + (r * p.splits + c.split) * p.pitch;
+#pragma unroll 1
+        for (int c0 = 0; c0 < a.dv; c0 += 16) {
+          float o[16];
+          if (done > 0) {
+            tmem_ld16(tO[t] + at + c0, o);
+            tmem_wait_ld();
+          }
+#pragma unroll
+          for (int e = 0; e < 16; e += 4)
+            if (qi < nq && c0 + e < p.pitch - 4)
+              *reinterpret_cast<float4*>(to + c0 + e) =
+                  done > 0 ? make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        }
+        if (qi < nq) *reinterpret_cast<float2*>(to + p.pitch - 4) = make_float2(m, l);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&plan_empty[pair & 1]);
+        continue;
+      }
       const float inv = 1.0f / l;
       bool fine = true;
 #pragma unroll 1
@@ -636,6 +678,47 @@ window_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
   }
 }
 
+// Joins the parts of rows whose keys were split: a warp takes a row (query, head).
+template <int DT>
+__global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ WindowTcParams p) {
+  using T = typename Elem<DT>::T;
+  const WindowArgs& a = p.a;
+  const int lane = threadIdx.x & 31;
+  const int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (r >= (int64_t)a.batch * a.heads * a.n) return;
+  const int64_t bh = r / a.n, i = r - bh * a.n, b = bh / a.heads, h = bh - b * a.heads;
+  const float* part = p.part + r * p.splits * p.pitch;
+  const float2 ml = lane < p.splits ? *reinterpret_cast<const float2*>(part + lane * p.pitch + p.pitch - 4)
+                                    : make_float2(-INFINITY, 0.0f);
+  float top = ml.x;
+#pragma unroll
+  for (int d = 1; d < 32; d *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+  const float f = ml.x == -INFINITY ? 0.0f : ex2(ml.x - top);
+  float total = f * ml.y;
+#pragma unroll
+  for (int d = 1; d < 32; d *= 2) total += __shfl_xor_sync(0xffffffffu, total, d);
+  T* out = static_cast<T*>(a.out) + b * a.o_b + h * a.o_h + i * a.o_n;
+  bool fine = true;
+  for (int c0 = 0; c0 < a.dv; c0 += 32) {
+    const int c = c0 + lane;
+    float sum = 0.0f;
+    for (int s = 0; s < p.splits; ++s) {
+      const float fs = __shfl_sync(0xffffffffu, f, s);
+      if (c < a.dv) sum = fmaf(fs, part[s * p.pitch + c], sum);
+    }
+    const float x = total == 0.0f ? 0.0f : sum / total;
+    if (c < a.dv) {
+      fine &= fabsf(x) < INFINITY;
+      out[c] = from_f32<T>(x);
+    }
+  }
+  if (!__all_sync(0xffffffffu, fine) && lane == 0) {
+    const int64_t hk = h / p.group;
+    row_again<DT>(a, b * a.q_b + h * a.q_h + i * a.q_n, b * a.k_b + hk * a.k_h, b * a.v_b + hk * a.v_h,
+                  b * a.o_b + h * a.o_h + i * a.o_n, a.m - a.n + i, a.m);
+  }
+}
+
 // ---------------------------------------------------------------- host side
 
 using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
@@ -692,6 +775,19 @@ int launch_dims(const CUtensorMap* maps, const WindowTcParams& p, dim3 grid, cud
   return p.a.dv <= 64 ? launch_one<DT, 2, 1>(maps, p, grid, s) : launch_one<DT, 2, 2>(maps, p, grid, s);
 }
 
+void shape_of(const WindowArgs& a, WindowTcParams& p) {
+  p.group = a.heads / a.kv_heads;
+  p.pack = 1;
+  while (p.pack < 32 && p.group % (2 * p.pack) == 0) {
+    p.pack *= 2;
+    ++p.pack_log;
+  }
+  p.blocks = p.group / p.pack;
+  p.rows_per_cta = 2 * kRows / p.pack;
+}
+
+int part_pitch(int dv) { return (dv + 3) / 4 * 4 + 4; }
+
 bool aligned(const void* base, int64_t size1, int64_t s1, int64_t size2, int64_t s2, int64_t size3, int64_t s3) {
   const bool ok = ((uintptr_t)base & 15) == 0;
   auto fits = [](int64_t size, int64_t s) { return size <= 1 || (s > 0 && (s & 7) == 0 && s < ((int64_t)1 << 38)); };
@@ -710,20 +806,38 @@ bool window_tc_takes(const WindowArgs& a) {
          aligned(a.v, a.m, a.v_n, a.kv_heads, a.v_h, a.cu_q ? 1 : a.batch, a.v_b);
 }
 
-int launch_window_tc(const WindowArgs& a, cudaStream_t s) {
+// Parts of each pair's keys, for a dense call whose pairs fill less than half of
+// the SMs: at most 32 (a lane each in the join), at least four tiles to a part,
+// and from 48 tiles on.  A tile takes 0.85 us, the join's launch and workspace 11 us
+// of the caller's time: 8192 keys 105 us whole and 39 split, 4096 57 and 39, 1024 28
+// and 39.
+int window_tc_splits(const WindowArgs& a) {
+  if (a.cu_q) return 1;
+  WindowTcParams p{};
+  shape_of(a, p);
+  const int64_t pairs = ceil_div(a.n, p.rows_per_cta) * a.batch * (a.heads / p.pack);
+  const int64_t rows = std::min<int64_t>(a.n, p.rows_per_cta), span = std::min<int64_t>(a.window, a.m) + rows;
+  const int64_t tiles = ceil_div(std::min<int64_t>(a.m, span + std::min<int64_t>(a.sinks, a.m)), kCols);
+  const int64_t splits = std::min<int64_t>(std::min<int64_t>(148 / std::max<int64_t>(pairs, 1), tiles / 4), 32);
+  return splits < 2 || tiles < 48 ? 1 : (int)splits;
+}
+
+size_t window_tc_bytes(const WindowArgs& a) {
+  const int splits = window_tc_splits(a);
+  return splits > 1 ? (size_t)a.batch * a.heads * a.n * splits * part_pitch(a.dv) * sizeof(float) : 0;
+}
+
+int launch_window_tc(const WindowArgs& a, void* workspace, size_t workspace_bytes, cudaStream_t s) {
   WindowTcParams p{};
   p.a = a;
-  p.group = a.heads / a.kv_heads;
-  p.pack = 1;
-  while (p.pack < 32 && p.group % (2 * p.pack) == 0) {
-    p.pack *= 2;
-    ++p.pack_log;
-  }
-  p.blocks = p.group / p.pack;
-  p.rows_per_cta = 2 * kRows / p.pack;
+  shape_of(a, p);
   p.vec_out = ((uintptr_t)a.out & 15) == 0 && (a.o_n & 7) == 0 && (a.o_h & 7) == 0 && (a.o_b & 7) == 0 &&
               (a.dv & 7) == 0;
   p.wait_ns = wait_limit_ns();
+  p.pitch = part_pitch(a.dv);
+  // without a workspace the keys are not split
+  p.splits = workspace && workspace_bytes >= window_tc_bytes(a) ? window_tc_splits(a) : 1;
+  p.part = static_cast<float*>(workspace);
   const bool bf16 = a.dtype == SA_REP_BFLOAT16;
   const int64_t batch = a.cu_q ? 1 : a.batch;
   CUtensorMap maps[7];   // q; k in boxes of a tile, of the seam's 16 rows and of the rows behind them; v likewise
@@ -740,7 +854,7 @@ int launch_window_tc(const WindowArgs& a, cudaStream_t s) {
     rc = encode(&maps[1 + i], bf16, isv ? a.v : a.k, 4, kd, ks, kb);
   }
   if (rc) return rc;
-  const int64_t tiles = tile_count(a, p.rows_per_cta), items = tiles * (a.heads / p.pack);
+  const int64_t tiles = tile_count(a, p.rows_per_cta), items = tiles * (a.heads / p.pack) * p.splits;
   if (items > 2147483647LL) return set_error(SA_ERR_UNSUPPORTED, "window attention: grid too large");
   p.tiles = (uint32_t)tiles;
   p.items = (uint32_t)items;
@@ -749,7 +863,14 @@ int launch_window_tc(const WindowArgs& a, cudaStream_t s) {
   if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
   if (e != cudaSuccess) return set_error(SA_ERR_CUDA, "window_tc device query: %s", cudaGetErrorString(e));
   dim3 grid((unsigned)(items < sms ? items : sms));
-  return bf16 ? launch_dims<SA_REP_BFLOAT16>(maps, p, grid, s) : launch_dims<SA_REP_FLOAT16>(maps, p, grid, s);
+  rc = bf16 ? launch_dims<SA_REP_BFLOAT16>(maps, p, grid, s) : launch_dims<SA_REP_FLOAT16>(maps, p, grid, s);
+  if (rc || p.splits == 1) return rc;
+  const unsigned join = (unsigned)ceil_div((int64_t)a.batch * a.heads * a.n, 8);
+  if (bf16)
+    join_kernel<SA_REP_BFLOAT16><<<join, 256, 0, s>>>(p);
+  else
+    join_kernel<SA_REP_FLOAT16><<<join, 256, 0, s>>>(p);
+  return check_launch("window join_kernel");
 }
 
 }  // namespace sa

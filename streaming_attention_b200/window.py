@@ -92,11 +92,12 @@ def sliding_window_attention(q: Tensor, k: Tensor, v: Tensor, *, window: Optiona
     if out.numel():
         _check_heads(heads, kv_heads)
         ws = None
-        if code == _lib.REP_DTYPES["float32"]:
+        if q.dtype == torch.float32 or (n * heads <= 4096 and m > 2900):   # 16-bit: few rows have their many keys split
             size = _workspace_size(b, heads, kv_heads, n, m, d, dv, w, s, code)
             if size:
                 ws = torch.empty(size, device=dev, dtype=torch.uint8)
-                q, k, v = (t.detach().contiguous() for t in (q, k, v))
+                if q.dtype == torch.float32:
+                    q, k, v = (t.detach().contiguous() for t in (q, k, v))
         q, k, v = _on_borders(q), _on_borders(k), _on_borders(v)
         S.launch(dev, "sa_window_attention", q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
                  S.strides(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *out.stride()[:3]), b, heads, kv_heads,

@@ -63,6 +63,10 @@ SHAPES = [
     (1, 2, 2, 70, 150, 256, 256, 64, 5),
     (1, 2, 1, 130, 260, 192, 100, 65, 40),
     (1, 16, 2, 2, 1500, 128, 128, 1000, 20),
+    (1, 2, 1, 1, 4100, 128, 128, None, 0),          # few queries, many keys: the keys are split
+    (2, 4, 4, 3, 4211, 64, 96, 3900, 300),
+    (1, 8, 2, 70, 4000, 80, 33, None, 0),
+    (3, 1, 1, 40, 4700, 48, 48, 3300, 1000),
 ]
 
 
@@ -195,6 +199,35 @@ def test_window_hidden_keys_do_not_matter(dtype, bad, d, dev):
     bound = R.attention_bound(ref, spread, score, d, window + sinks, dtype, _p_half(dtype))
     R.assert_close(got[0][:, keep.to(dev)], ref[:, keep], bound[:, keep])
     assert not torch.isfinite(got[:, :, 100:150]).any()
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16], ids=["f32", "f16", "bf16"])
+def test_window_split_keys_hide_and_repeat(dtype, dev):
+    """Few queries over many keys (16-bit types split them over the SMs): hidden NaN
+    and infinities, the same bits twice and in a replayed graph, on another stream."""
+    g = R.rng(21)
+    q, k, v = _make((1, 4, 2, 64), dtype, g, 1.5).to(dev), *(_make((1, 2, 5000, 64), dtype, g).to(dev) for _ in range(2))
+    clean = k.clone(), v.clone()
+    k[:, :, 4999], v[:, :, 4999] = float("nan"), float("inf")      # seen by the last query alone
+    k[:, :, 700], v[:, :, 700] = float("inf"), float("nan")        # by none
+    f = lambda: sa.sliding_window_attention(q, k, v, window=4000, sinks=5)  # noqa: E731
+    out = f()
+    _check(q[:, :, :1], clean[0][:, :, :4999], clean[1][:, :, :4999], out[:, :, :1], 4000, 5)
+    assert not torch.isfinite(out[:, :, 1]).any()
+    k.copy_(clean[0])
+    v.copy_(clean[1])
+    first = f()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = f()
+    graph.replay()
+    side = torch.cuda.Stream(dev)
+    side.wait_stream(torch.cuda.current_stream(dev))
+    with torch.cuda.stream(side):
+        other = f()
+    again = f()
+    torch.cuda.synchronize()
+    assert torch.equal(first, captured) and torch.equal(first, other) and torch.equal(first, again)
 
 
 @pytest.mark.parametrize("dtype", [F32, F16, BF16], ids=["f32", "f16", "bf16"])
