@@ -18,8 +18,8 @@ namespace sa {
 
 namespace {
 
-constexpr int kPlanThreads = 256;
-constexpr int kPlanTokens = 4 * kPlanThreads;   // per CTA
+constexpr int kPlanThreads = 1024;              // a batch of 1000 requests is summed in one round (256 threads: 13 us)
+constexpr int kPlanTokens = 2 * kPlanThreads;   // per CTA
 constexpr int kPlanMaxRequests = 16384;
 
 struct PlanArgs {
@@ -86,12 +86,16 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs a) {
       part_pages[warp] = y;
     }
     __syncthreads();
-    x += carry_new;
-    y += carry_pages;
-    for (int w = 0; w < warp; ++w) {
-      x += part_new[w];
-      y += part_pages[w];
+    // the warps before: each lane takes one, summed by shuffles
+    long long xb = lane < warp ? part_new[lane] : 0;
+    int yb = lane < warp ? part_pages[lane] : 0;
+#pragma unroll
+    for (int o = 16; o >= 1; o >>= 1) {
+      xb += __shfl_xor_sync(0xffffffffu, xb, o);
+      yb += __shfl_xor_sync(0xffffffffu, yb, o);
     }
+    x += carry_new + xb;
+    y += carry_pages + yb;
     if (r < a.requests) {
       sum_new[r] = (int32_t)min(x - (long long)add, 2147483647LL);
       sum_pages[r] = y - pages;

@@ -107,7 +107,8 @@ def release_kv_pages(lengths: Tensor, tables: Tensor, drop: Tensor, free_pages: 
     for t in (lengths, tables, free_pages, free_count):
         if not t.is_contiguous():
             raise ValueError("lengths, tables, free_pages and free_count are updated in place: they must be contiguous")
-    S.launch(dev, "sa_release_kv_pages", lengths.data_ptr(), tables.data_ptr(), drop.contiguous().data_ptr(),
+    drop = drop.contiguous()
+    S.launch(dev, "sa_release_kv_pages", lengths.data_ptr(), tables.data_ptr(), drop.data_ptr(),
              free_pages.data_ptr(), free_count.data_ptr(), r, width, free_pages.shape[0], page_size)
 
 
