@@ -33,7 +33,8 @@
 // (serving.cuh) on the same tiles: a CTA walks the tiles of 64 keys that hold the
 // first tokens, then those of its rows' windows; p = 2^(s - m - 24), so that sums
 // of values near float32's largest stay below it; rows that come out non-finite
-// are computed again from their visible keys (window_row.cuh).
+// are computed again from their visible keys (window_row.cuh).  16 heads x 4096 of
+// 64, window 512: 118 us and 17 us of splits, 1159 us on the CUDA cores.
 #include <math.h>
 
 #include "sa_common.cuh"

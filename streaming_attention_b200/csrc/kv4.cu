@@ -15,6 +15,9 @@
 //   v_codes [pages, heads, page / 4, dp / 2, 4]  four tokens' bytes of a column pair share a word: the pairs
 //                                                along the token axis that the product P V contracts
 //   k_params, v_params [pages, heads, page, 2]   scale, least
+// 20011 tokens of 8 heads of 128 (bfloat16): the write 68 us (104 MB; bound by the
+// instructions that find the codes, 69 % of the issue slots), the read of the same
+// to float32 48 us (186 MB, 3.9 TB/s).
 #include <math.h>
 
 #include "kv4.cuh"

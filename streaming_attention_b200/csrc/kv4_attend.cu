@@ -17,8 +17,11 @@
 //   S = s_k (K_codes Q^T) + x_k sum(Q)         tokens x rows
 //   O = V_codes^T (p s_v)^T + sum(p x_v)       columns x rows
 // with scales and offsets in float32 on either side of the products.  What bounds
-// it beside the bytes is instructions (550 a block at first, taking 8 off each
-// code and choosing by mask everywhere; 301 us where the bytes take 94).  Q is
+// it beside the bytes (94 us of 64 requests x 6000..12000 tokens x 8 heads, 611 MB) is
+// instructions: 480 a block and 301 us with every code centred, masks in every
+// block and register double buffers; 212 us now (2.9 TB/s, the integer pipe 60 %
+// busy).  Float16 operands (five integer operations for eight codes in place of
+// eight) took 245: their scales cost more than they saved.  Q is
 // bfloat16 as it is, float16 as two and float32 as three bfloat16 pieces (exact,
 // or to 24 bits); p s_v is split into two pieces (16 bits; three for float32).
 //
@@ -560,7 +563,7 @@ int launch_one(const Kv4AttendArgs& a, cudaStream_t s) {
   if (y > 65535) return set_error(SA_ERR_UNSUPPORTED, "kv4 attend: grid too large");
   // CTAs per (request, key head): while a warp keeps at least four blocks of the
   // longest request the table allows and the grid has less than three
-  // rounds
+  // rounds (the batch above: 232 us with six, 231 with one)
   const int64_t longest = std::min<int64_t>((int64_t)a.width << a.c.page_shift, a.window + std::min(a.sinks, a.window) + a.n);
   int splits = 1;
   while (splits < 8 && longest >= (int64_t)splits * 2 * kWarps * 16 * 4 && y * a.requests * splits < 148 * S::kPerSm * 3) splits *= 2;

@@ -53,6 +53,16 @@ def attention_bound(ref, spread, score, dim, keys, dtype, p_half):
     return HALF[dtype] * (ref.abs() + rel * spread) + rel * spread + (2.0 ** -25 if dtype == torch.float16 else 1e-37)
 
 
+def code_span(dtype):
+    """How much larger the terms of a score over 4-bit codes are than |q k|, at most,
+    for rows that are not far off zero.  A value is s c' + x, c' the code plus an
+    offset, and both products are summed on their own.  Rows of roughly normal values
+    of deviation 1 have s = 5 / 15 and mean |k| = 0.8: float32 takes c' = code - 8, so
+    8 s + |x| <= 2.7 + 0.5 = 4 * 0.8; 16-bit types take c' = code + 16, so 31 s + |x| <=
+    10.3 + 7.8 + 0.5 < 24 * 0.8."""
+    return 4 if dtype == torch.float32 else 24
+
+
 def assert_close(got, ref, bound):
     got = got.double().cpu()
     assert got.shape == ref.shape, (got.shape, ref.shape)

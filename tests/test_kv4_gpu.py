@@ -220,10 +220,8 @@ def _check_attend(out, q, ks, vs, lengths, window, sinks, scale=None):
         k, v = (y.repeat_interleave(per, 1).transpose(0, 1) for y in (ks[r], vs[r]))
         sees = R.visible(n, x, window, sinks)
         ref, spread, score = R.attention(q[r].cpu().double().transpose(0, 1), k, v, sees, sc)
-        # the scores' codes are summed around their middle: |q| times (8 scale + |least + 8 scale|) bounds every term,
-        # at most 4 times the dot product's own magnitude for rows that are not far off zero
         R.assert_close(out[r].transpose(0, 1), ref,
-                       R.attention_bound(ref, spread, 4 * score, d, x, out.dtype, P_HALF[out.dtype]))
+                       R.attention_bound(ref, spread, R.code_span(out.dtype) * score, d, x, out.dtype, P_HALF[out.dtype]))
 
 
 ATTEND = [

@@ -336,7 +336,7 @@ def test_prompt_and_decode_through_the_cache(dtype, graph, dev):
             kk, vv = (y.repeat_interleave(heads // hkv, 1).transpose(0, 1) for y in (hk, hv))
             ref, spread, score = R.attention(qr.double().cpu().transpose(0, 1), kk, vv, R.visible(1, lens[r], window, sinks), d ** -0.5)
             R.assert_close(out[r:r + 1].transpose(0, 1), ref,
-                           R.attention_bound(ref, spread, 4 * score, d, lens[r], dtype, 0.0 if dtype == F32 else 2.0 ** -16))
+                           R.attention_bound(ref, spread, R.code_span(dtype) * score, d, lens[r], dtype, 0.0 if dtype == F32 else 2.0 ** -16))
         assert layer.lengths.tolist() == lens
         if step == 2:
             before = layer.free_count.item()
