@@ -70,12 +70,13 @@ def ptr(t: Optional[Tensor]) -> Optional[int]:
 
 
 def check_window(window: Optional[int], sinks: int) -> Tuple[int, int]:
-    """Window (0: without end) and first tokens as the C ABI takes them."""
+    """Window (0: without end) and first tokens as the C ABI takes them; what lies
+    beyond every position (2^31) hides and shows no more than that does."""
     if window is not None and window <= 0:
         raise ValueError("window must be positive, or None for no end")
     if sinks < 0:
         raise ValueError("sinks must be non-negative")
-    return (0 if window is None else int(window)), int(sinks)
+    return (0 if window is None else min(int(window), 1 << 40)), min(int(sinks), 1 << 40)
 
 
 def _raw_stream(index: int) -> int:

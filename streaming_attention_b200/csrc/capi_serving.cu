@@ -6,6 +6,8 @@
 #include <stdlib.h>
 #include <string.h>
 
+#include <algorithm>
+
 #include "kv4.cuh"
 #include "serving.cuh"
 
@@ -49,6 +51,11 @@ int check_heads(int heads, int kv_heads) {
     return set_error(SA_ERR_INVALID_ARG, "the query heads must be a positive multiple of the key heads");
   return SA_OK;
 }
+
+// A window (0: without end) and first tokens, held where sums with positions
+// (below 2^31) cannot pass 64 bits.
+int64_t window_of(int64_t window) { return window > 0 ? std::min(window, (int64_t)1 << 40) : (int64_t)1 << 40; }
+int64_t sinks_of(int64_t sinks) { return std::min(sinks, (int64_t)1 << 40); }
 
 int page_shift_of(int page_size) {
   for (int s = 4; s <= 8; ++s)
@@ -119,7 +126,7 @@ int sa_window_attention_workspace_size(int batch, int heads, int kv_heads, int64
   *bytes = 0;
   if (batch == 0 || n == 0 || m < n) return SA_OK;
   if (dtype == SA_REP_FLOAT32) {
-    *bytes = window_tf32_bytes(batch, heads, kv_heads, n, m, d, dv, window, sinks);
+    *bytes = window_tf32_bytes(batch, heads, kv_heads, n, m, d, dv, window, sinks_of(sinks));
   } else if (d <= 128 && dv <= 128) {
     WindowArgs a{};
     a.batch = batch;
@@ -128,8 +135,8 @@ int sa_window_attention_workspace_size(int batch, int heads, int kv_heads, int64
     a.n = n;
     a.m = m;
     a.dv = dv;
-    a.window = window > 0 ? window : (int64_t)1 << 40;
-    a.sinks = sinks;
+    a.window = window_of(window);
+    a.sinks = sinks_of(sinks);
     *bytes = window_tc_bytes(a);
   }
   return SA_OK;
@@ -154,14 +161,14 @@ int sa_window_attention(const void* q, const void* k, const void* v, void* out, 
   const WindowArgs a{q,          k,          v,          out,        strides[0], strides[1], strides[2],  strides[3],
                      strides[4], strides[5], strides[6], strides[7], strides[8], strides[9], strides[10], strides[11],
                      batch,      heads,      kv_heads,   n,          m,          d,          dv,
-                     window > 0 ? window : (int64_t)1 << 40, sinks, scale, dtype, cu_q, cu_k, status_word(), zero_behind};
+                     window_of(window), sinks_of(sinks), scale, dtype, cu_q, cu_k, status_word(), zero_behind};
   const char* simt = getenv("SA_FORCE_SIMT");
   if (window_tc_takes(a) && !(simt && simt[0] == '1')) return launch_window_tc(a, workspace, workspace_bytes, (cudaStream_t)stream);
   // float32 on the tensor cores: contiguous tensors and a workspace
   if (dtype == SA_REP_FLOAT32 && !cu_q && workspace && a.status && a.q_n == d && a.q_h == n * d && a.q_b == heads * a.q_h &&
       a.k_n == d && a.k_h == m * d && a.k_b == kv_heads * a.k_h && a.v_n == dv && a.v_h == m * dv &&
       a.v_b == kv_heads * a.v_h && a.o_n == dv && a.o_h == n * dv && a.o_b == heads * a.o_h &&
-      window_tf32_bytes(batch, heads, kv_heads, n, m, d, dv, window, sinks) > 0)
+      window_tf32_bytes(batch, heads, kv_heads, n, m, d, dv, window, sinks_of(sinks)) > 0)
     return window_tf32_run(a, workspace, workspace_bytes, (cudaStream_t)stream);
   return launch_window_simt(a, (cudaStream_t)stream);
 }
@@ -284,8 +291,8 @@ int sa_kv4_attend(const void* k_codes, const void* k_params, const void* v_codes
   a.n = n;
   a.heads = heads;
   a.width = width;
-  a.window = window > 0 ? window : (int64_t)1 << 40;
-  a.sinks = sinks;
+  a.window = window_of(window);
+  a.sinks = sinks_of(sinks);
   a.scale = scale;
   a.dtype = dtype;
   a.status = status_word();

@@ -322,6 +322,17 @@ def test_attend_strides_scale_and_streams(dev):
     assert torch.equal(out, other) and torch.equal(out, again)
 
 
+def test_attend_window_of_any_size(dev):
+    """Windows and first tokens beyond every position are what no window is."""
+    cache, tables, lens, ks, vs = _filled(dev, [90, 300], 2, 64, 32, F32, 16)
+    q = torch.randn(2, 2, 4, 64, generator=R.rng(17)).to(BF16).to(dev)
+    whole = cache.attend(q, tables, lens)
+    for window, sinks in ((2 ** 32 + 1, 0), (2 ** 63 - 1, 2 ** 63 - 1), (2 ** 64 + 3, 0), (1, 2 ** 63 - 1)):
+        out = cache.attend(q, tables, lens, window=window, sinks=sinks)
+        _check_attend(out, q, ks, vs, [90, 300], None, 0)
+        assert sinks or torch.equal(out, whole)
+
+
 def test_attend_two_graphs_and_growing_lengths(dev):
     """Two captured calls replayed in turn and at once; lengths and tables change between replays."""
     cache, tables, lens, ks, vs = _filled(dev, [400, 120], 2, 128, 16, F32, 12)

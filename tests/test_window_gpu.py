@@ -285,6 +285,18 @@ def test_window_graph_replay(dev):
         assert torch.equal(out, sa.sliding_window_attention(q, k, v, window=100, sinks=1))
 
 
+@pytest.mark.parametrize("dtype,n", [(F32, 20), (F32, 300), (BF16, 20), (BF16, 300)])
+def test_window_of_any_size(dtype, n, dev):
+    """Windows and first tokens beyond every position are what no window is."""
+    g = R.rng(21)
+    q, k, v = (_make((1, 2, n, 64), dtype, g).to(dev) for _ in range(3))
+    whole = sa.sliding_window_attention(q, k, v, window=None)
+    for window, sinks in ((2 ** 32 + 1, 0), (2 ** 62, 2 ** 62), (2 ** 63 + 5, 0), (1, 2 ** 63 - 1), (1, 2 ** 64 + 1)):
+        out = sa.sliding_window_attention(q, k, v, window=window, sinks=sinks)
+        _check(q.cpu(), k.cpu(), v.cpu(), out, None, 0)
+        assert sinks or torch.equal(out, whole)
+
+
 def test_window_empty(dev):
     z = lambda *s: torch.zeros(*s, device=dev)  # noqa: E731
     assert sa.sliding_window_attention(z(2, 4, 0, 64), z(2, 4, 9, 64), z(2, 4, 9, 64), window=3).shape == (2, 4, 0, 64)
