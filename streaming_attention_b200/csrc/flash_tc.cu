@@ -27,7 +27,7 @@
 // registers (the row's columns of this half) with round-to-nearest adds, and
 // the next product restarts the TMEM chain.  The running sum l adds each tile's 32
 // values pairwise before the running add.  Scores are kept in base-2 units (the query is scaled by
-// scale * log2(e), as FlashAttention-2 does), so p = 2^(s - m) is one ex2.
+// scale * log2(e)), so p = 2^(s - m) is one ex2.
 //
 // kWin: the float32 windowed attention with first tokens and grouped heads
 // (serving.cuh) on the same tiles: a CTA walks the tiles of 64 keys that hold the

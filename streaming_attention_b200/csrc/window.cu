@@ -9,7 +9,9 @@
 // One CTA per (64-query tile, query head), 256 threads: four threads per query
 // row, each scoring 8 of a 32-key tile and accumulating a quarter of the value
 // columns (float32 throughout, online softmax).  Only tiles that hold a visible
-// key are read: the first tokens' tiles, then the window's.
+// key are read: the first tokens' tiles, then the window's.  Bound by the FMA pipe
+// and its shared-memory operands: 2 x 8 heads x 4096 of 64 with a window of 512
+// 1159 us, where the tensor cores' form takes 134.
 #include <math.h>
 
 #include "serving.cuh"

@@ -27,7 +27,8 @@
 // goes to L2).  TMEM: of each query tile two S of 64 columns and O of 128; P, in 16
 // bits, overwrites the first half of its S.  A tile's issuer goes P V(j), S(j + 2),
 // so that the next scores are there while a softmax runs; with one S of 128
-// columns each waited for the other (184 us for the 8192-token prompt).
+// columns each waited for the other (32 heads x 8192 of 128, window 1024: 184 us, and
+// 174 so; 129 GFLOP, 44 % of the measured GEMM rate, bound by that chain).
 //
 // Where a dense call has few pairs and many keys, a pair's key tiles are dealt
 // into parts that run as items of their own and are joined by join_kernel.
