@@ -278,8 +278,18 @@ flash_tc_kernel(const __grid_constant__ CUtensorMap tm_kh, const __grid_constant
 #pragma unroll
         for (int kk = 0; kk < DP / 8; ++kk) {
           const uint64_t bk = kd + (uint64_t)(((kk >> 2) * (2 * kTile * 128) + (kk & 3) * 32) >> 4);
-          mma_tf32_ts(dS, tmem + L::kQhi + kk * 8, bk, idesc_qk, kk > 0 ? 1u : 0u);
-          mma_tf32_ts(dS, tmem + L::kQlo + kk * 8, bk, idesc_qk, 1u);
+          if constexpr (kWin) {   // the small products first: sums are truncated at their own size
+            mma_tf32_ts(dS, tmem + L::kQlo + kk * 8, bk, idesc_qk, kk > 0 ? 1u : 0u);
+          } else {
+            mma_tf32_ts(dS, tmem + L::kQhi + kk * 8, bk, idesc_qk, kk > 0 ? 1u : 0u);
+            mma_tf32_ts(dS, tmem + L::kQlo + kk * 8, bk, idesc_qk, 1u);
+          }
+        }
+        if constexpr (kWin) {
+#pragma unroll
+          for (int kk = 0; kk < DP / 8; ++kk)
+            mma_tf32_ts(dS, tmem + L::kQhi + kk * 8, kd + (uint64_t)(((kk >> 2) * (2 * kTile * 128) + (kk & 3) * 32) >> 4),
+                        idesc_qk, 1u);
         }
         mma_commit(&sfull[b]);
       }

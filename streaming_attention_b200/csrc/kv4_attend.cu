@@ -351,13 +351,16 @@ __global__ void __launch_bounds__(kThreads, (Shape<DT, DP, NT>::kPerSm)) attend_
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) off[nt][0] = off[nt][1] = INFINITY;   // no maximum yet: the first score moves it
 
+  // float32: the matrix units truncate as they add, so their sums stay short (a
+  // block) and apart by size, and longer ones are added outside, rounded
+  constexpr bool kApart = DT == SA_REP_FLOAT32;
   auto work = [&](const Block<DP>& b, int token, auto whole) {
     constexpr bool kWhole = decltype(whole)::value;   // every row sees the whole block
-    float s[NT][4];
+    float s[NT][4], low[NT][4];   // low: the products of Q's lower pieces, added at the end
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) s[nt][e] = 0.0f;
+      for (int e = 0; e < 4; ++e) s[nt][e] = low[nt][e] = 0.0f;
 #pragma unroll
     for (int w = 0; w < kKS / 2; ++w) {
       uint32_t f[2][4] = {{codes<0, kOff>(b.k0[w]), codes<0, kOff>(b.k1[w]), codes<1, kOff>(b.k0[w]), codes<1, kOff>(b.k1[w])},
@@ -368,7 +371,8 @@ __global__ void __launch_bounds__(kThreads, (Shape<DT, DP, NT>::kPerSm)) attend_
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int q = 0; q < S::kQ; ++q)
-            mma(s[nt], f[half][0], f[half][1], f[half][2], f[half][3], qf[nt][q][2 * w + half][0], qf[nt][q][2 * w + half][1]);
+            mma(kApart && q > 0 ? low[nt] : s[nt], f[half][0], f[half][1], f[half][2], f[half][3], qf[nt][q][2 * w + half][0],
+                qf[nt][q][2 * w + half][1]);
     }
     const float2 ka = params(b.kp.x), kb = params(b.kp.y), va = params(b.vp.x), vb = params(b.vp.y);
     const float k_s[2] = {ka.x * sc, kb.x * sc}, k_x[2] = {fmaf(-(float)kOff, ka.x, ka.y) * sc, fmaf(-(float)kOff, kb.x, kb.y) * sc};
@@ -388,6 +392,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<DT, DP, NT>::kPerSm)) attend_
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
+        if (kApart) s[nt][e] += low[nt][e];
         s[nt][e] = fmaf(k_s[e >> 1], s[nt][e], k_x[e >> 1] * qsum[nt][e & 1]);
         if (!kWhole) s[nt][e] = (on >> (4 * nt + e)) & 1u ? s[nt][e] : -INFINITY;
         move |= s[nt][e] + off[nt][e & 1] > kMove + kShift;
@@ -445,9 +450,16 @@ __global__ void __launch_bounds__(kThreads, (Shape<DT, DP, NT>::kPerSm)) attend_
       const uint32_t w = b.v[t];
       const uint32_t a0 = codes<0, kOff>(w), a1 = codes<1, kOff>(w), a2 = codes<2, kOff>(w), a3 = codes<3, kOff>(w);
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+      for (int nt = 0; nt < NT; ++nt) {
+        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        float (&to)[4] = kApart ? sum : o[nt][t];
 #pragma unroll
-        for (int q = 0; q < S::kP; ++q) mma(o[nt][t], a0, a1, a2, a3, pf[nt][q][0], pf[nt][q][1]);
+        for (int q = S::kP - 1; q >= 0; --q) mma(to, a0, a1, a2, a3, pf[nt][q][0], pf[nt][q][1]);
+        if (kApart) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[nt][t][e] += sum[e];
+        }
+      }
     }
   };
   auto go = [&](const Block<DP>& b, int token) {
