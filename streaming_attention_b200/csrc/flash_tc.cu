@@ -52,6 +52,11 @@ constexpr int kTile = 64;
 constexpr int kThreads = 320;
 constexpr float kRescale = 12.0f;   // base-2 units: p <= 4096
 constexpr int kFold = 16;           // key tiles per TMEM accumulation chain
+// A window's rows have few tiles, and the matrix units truncate as they add.
+template <bool kWin>
+__host__ __device__ constexpr int fold_of() {
+  return kWin ? 4 : kFold;
+}
 
 constexpr int kErrWaitQ = 301, kErrWaitFull = 302, kErrWaitP = 304, kErrWaitS = 305,
               kErrWaitEmpty = 306, kErrWaitO = 307, kErrDrain = 308, kErrWaitPV = 309;
@@ -249,7 +254,7 @@ flash_tc_kernel(const __grid_constant__ CUtensorMap tm_kh, const __grid_constant
         for (int kk = 0; kk < kTile / 8; ++kk) {
           const uint64_t bh_ = vd + (uint64_t)(((kk >> 2) * (2 * DVP * 128) + (kk & 3) * 32) >> 4);
           // the accumulator restarts after every fold (tiles tp % kFold == 0)
-          mma_tf32_ts(tmem + L::kO, ph + kk * 8, bh_, idesc_pv, (tp % kFold || kk > 0) ? 1u : 0u);
+          mma_tf32_ts(tmem + L::kO, ph + kk * 8, bh_, idesc_pv, (tp % fold_of<kWin>() || kk > 0) ? 1u : 0u);
           if (L::kPVStack) {
             mma_tf32_ts(tmem + L::kO, pl + kk * 8, bh_, idesc_pv, 1u);
           } else {
@@ -402,7 +407,7 @@ flash_tc_kernel(const __grid_constant__ CUtensorMap tm_kh, const __grid_constant
       }
       // fold O into the master (every kFold tiles), or rescale it where a row
       // of this warp moved its m; both first wait for the products of tile t-1
-      const bool fold = t > 0 && t % kFold == 0;
+      const bool fold = t > 0 && t % fold_of<kWin>() == 0;
       if (t > 0 && (fold || __any_sync(0xffffffffu, move))) {
         const int tp = t - 1;
         if (!mbar_wait_warp(&sfree[tp & 1], (tp >> 1) & 1, ab, kErrWaitPV)) {
