@@ -26,7 +26,10 @@
 // registers (more, of 128 columns, spilled: beside 220 KB of shared memory that
 // goes to L2).  TMEM: of each query tile two S of 64 columns and O of 128; P, in 16
 // bits, overwrites the first half of its S.  A tile's issuer goes P V(j), S(j + 2),
-// so that the next scores are there while a softmax runs; with one S of 128
+// so that the next scores are there while a softmax runs (their commit says too
+// that P V(j) has ended; one without scores behind it has a barrier of its own,
+// since a parity wait must have seen each phase of its barrier before the next
+// ends: scores' commits are all answered by a P, these by a later one); with one S of 128
 // columns each waited for the other (32 heads x 8192 of 128, window 1024: 184 us, and
 // 174 so; 129 GFLOP, 44 % of the measured GEMM rate, bound by that chain).
 //
@@ -264,7 +267,7 @@ struct Layout {
   static constexpr uint32_t kPitch = 80;                                        // a row's 32 columns, staged
   static constexpr uint32_t kStage = kRing + kSlots * kSlot;
   static constexpr uint32_t kBars = kStage + 8 * 32 * kPitch;
-  static constexpr uint32_t kBytes = kBars + (2 * kSlots + 16) * 8 + 16 + 2 * sizeof(PairPlan) + 1024;
+  static constexpr uint32_t kBytes = kBars + (2 * kSlots + 20) * 8 + 16 + 2 * sizeof(PairPlan) + 1024;
   static_assert(kBytes <= 227 * 1024, "shared memory");
 };
 
@@ -284,7 +287,8 @@ window_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
   uint64_t* empty = full + kSlots;
   uint64_t* sfull = empty + kSlots;   // [2 query tiles][2 score buffers]
   uint64_t* pfull = sfull + 4;        // likewise
-  uint64_t* qfull = pfull + 4;
+  uint64_t* ofull = pfull + 4;        // likewise: a P V that no scores follow in its buffer has ended
+  uint64_t* qfull = ofull + 4;
   uint64_t* qempty = qfull + 1;
   uint64_t* plan_full = qempty + 1;       // [2]
   uint64_t* plan_empty = plan_full + 2;   // [2]
@@ -304,6 +308,7 @@ window_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
     for (int i = 0; i < 4; ++i) {
       mbar_init(&sfull[i], 1);
       mbar_init(&pfull[i], 4);
+      mbar_init(&ofull[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&plan_full[i], 1);
@@ -481,7 +486,12 @@ window_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
                            (begun || kk > 0) ? 1u : 0u);
           }
           if (next) scores(j + 2);
-          if (pv || next) mma_commit(&sfull[2 * t + buf]);
+          // every commit to sfull is of scores, whose P the issuer waits for before the next; one to ofull
+          // is waited for by the softmax before it makes the P of a later tile in the buffer
+          if (next)
+            mma_commit(&sfull[2 * t + buf]);
+          else if (pv)
+            mma_commit(&ofull[2 * t + buf]);
           mma_commit(&empty[group % kSlots]);
           if (j + 3 == tiles) mma_commit(qempty);   // the queries' last product is issued
         }
@@ -510,7 +520,7 @@ window_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
     const uint32_t at = (uint32_t)(quarter * 32) << 16;
     const float c2 = a.scale * 1.4426950408889634f;          // log2(e); not negative (window_tc_takes)
     uint8_t* stage = smem + L::kStage + (warp - 3) * 32 * L::kPitch;
-    int count[2] = {0, 0};   // what the issuer has committed to each score buffer's barrier
+    int count[2] = {0, 0}, ended[2] = {0, 0};   // commits waited for in each buffer: scores, P V alone
     bool ok = true;
 #pragma unroll 1
     for (int pair = 0; ok; ++pair) {
@@ -530,16 +540,21 @@ window_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
       };
       // step j of the issuer: P V of tile j, then S of tile j + 2 into the same
       // buffer, then a commit; so the commit that brings S(j) says that P V of tile
-      // j - 2 has ended, and the two behind the last tile that all have
+      // j - 2 has ended; where there is no S(j), that P V has a commit of its own
 #pragma unroll 1
       for (int j = 0; j < tiles + 2; ++j) {
         const int buf = j & 1;
         const bool here = needed(j);
-        if (!here && (j < 2 || !needed(j - 2))) continue;
+        if (!here) {
+          if (j < 2 || !needed(j - 2)) continue;
+          ok = mbar_wait_warp_lazy(&ofull[2 * t + buf], ended[buf] & 1, ab, kErrO);
+          if (!ok) break;
+          ++ended[buf];
+          continue;
+        }
         ok = mbar_wait_warp_lazy(&sfull[2 * t + buf], count[buf] & 1, ab, kErrS);
         if (!ok) break;
         ++count[buf];
-        if (!here) continue;
         tc_fence_after();
         // columns of a last, narrower tile that its product left out hold an earlier tile's numbers: hidden like others
         const int v0 = start + j * kCols, w = min(kCols, (total - v0 + 31) & ~31);
@@ -566,7 +581,11 @@ window_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
           l *= alpha;
           if (done > 0) {
             // the product of the tile before may still run: its step's commit ends the wait (and is not used up)
-            if (needed(j - 1)) ok = mbar_wait_warp_lazy(&sfull[2 * t + (buf ^ 1)], count[buf ^ 1] & 1, ab, kErrO);
+            if (needed(j - 1)) {
+              const bool more = needed(j + 1);
+              ok = mbar_wait_warp_lazy(more ? &sfull[2 * t + (buf ^ 1)] : &ofull[2 * t + (buf ^ 1)],
+                                       (more ? count[buf ^ 1] : ended[buf ^ 1]) & 1, ab, kErrO);
+            }
             if (!ok) break;
             tc_fence_after();
             scale_row(tO[t] + at, a.dv, alpha);
