@@ -3,6 +3,7 @@
 // checked here; the contents of device-side index arrays (offsets, slots, page
 // tables, lengths) are checked in the kernels, which skip what is out of range
 // and record it in the error word of sa_serving_status.
+#include <stddef.h>
 #include <stdlib.h>
 #include <string.h>
 
@@ -28,8 +29,14 @@ int launch_rotary(const void* q, const void* k, void* q_out, void* k_out, const 
 namespace {
 
 // The error word: one per device, zero at load, set by the first kernel that
-// finds something wrong and cleared when it is read.
-__device__ int g_serving_status[4];
+// finds something wrong and cleared when it is read.  Its index is stored as 8
+// bytes behind it (report), so the type carries the alignment.
+struct alignas(16) StatusWord {
+  int code[2];
+  long long index;
+};
+static_assert(alignof(StatusWord) % alignof(long long) == 0 && offsetof(StatusWord, index) == 2 * sizeof(int), "report() stores the index as one 8-byte word");
+__device__ StatusWord g_serving_status;
 
 int* status_word() {
   void* p = nullptr;
