@@ -518,7 +518,7 @@ window_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
     const int tq = kRows >> p.pack_log;                      // queries of a tile
     const int qi = t * tq + (row >> p.pack_log);             // query of the pair
     const uint32_t at = (uint32_t)(quarter * 32) << 16;
-    const float c2 = a.scale * 1.4426950408889634f;          // log2(e); not negative (window_tc_takes)
+    const float c2 = a.scale * 1.4426950408889634f;          // log2(e); positive (window_tc_takes)
     uint8_t* stage = smem + L::kStage + (warp - 3) * 32 * L::kPitch;
     int count[2] = {0, 0}, ended[2] = {0, 0};   // commits waited for in each buffer: scores, P V alone
     bool ok = true;
@@ -817,10 +817,11 @@ bool aligned(const void* base, int64_t size1, int64_t s1, int64_t size2, int64_t
 }  // namespace
 
 // Whether the tensor-core kernel takes these tensors: 16-bit elements, head
-// widths up to 128, rows on 16-byte borders (TMA), no repeated rows, and a scale
-// that is not negative (the running maximum is taken before the scale).
+// widths up to 128, rows on 16-byte borders (TMA), no repeated rows, and a positive
+// scale (the running maximum is taken before the scale, and a hidden score, -inf,
+// has to stay that when it is scaled).
 bool window_tc_takes(const WindowArgs& a) {
-  if (a.dtype == SA_REP_FLOAT32 || a.d > 128 || a.dv > 128 || a.m == 0 || a.m >= (1 << 30) || a.n >= (1 << 30) || !(a.scale >= 0.0f)) return false;
+  if (a.dtype == SA_REP_FLOAT32 || a.d > 128 || a.dv > 128 || a.m == 0 || a.m >= (1 << 30) || a.n >= (1 << 30) || !(a.scale > 0.0f)) return false;
   return aligned(a.q, a.n, a.q_n, a.heads, a.q_h, a.cu_q ? 1 : a.batch, a.q_b) &&
          aligned(a.k, a.m, a.k_n, a.kv_heads, a.k_h, a.cu_q ? 1 : a.batch, a.k_b) &&
          aligned(a.v, a.m, a.v_n, a.kv_heads, a.v_h, a.cu_q ? 1 : a.batch, a.v_b);
