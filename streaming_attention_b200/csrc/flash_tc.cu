@@ -32,7 +32,7 @@
 // kWin: the float32 windowed attention with first tokens and grouped heads
 // (serving.cuh) on the same tiles: a CTA walks the tiles of 64 keys that hold the
 // first tokens, then those of its rows' windows; p = 2^(s - m - 24), so that sums
-// of values near float32's largest stay below it; rows that come out non-finite
+// of values near float32's largest stay below it; columns that come out non-finite
 // are computed again from their visible keys (window_row.cuh).  16 heads x 4096 of
 // 64, window 512: 121 us and 17 us of splits, 1159 us on the CUDA cores.
 #include <math.h>
@@ -525,10 +525,14 @@ flash_tc_kernel(const __grid_constant__ CUtensorMap tm_kh, const __grid_constant
       xmax[half * 128 + row] = fine ? 0.0f : 1.0f;
       __threadfence_block();
       asm volatile("bar.sync %0, 64;" ::"r"(bar_id) : "memory");
-      if (ok && half == 0 && valid && (!fine || xmax[128 + row] != 0.0f)) {
+      const bool again = valid && (!fine || xmax[128 + row] != 0.0f);
+#pragma unroll 1
+      for (unsigned left = ok && half == 0 ? __ballot_sync(0xffffffffu, again) : 0; left; left &= left - 1) {
         const int b = (int)h / p.w.heads, hh = (int)h - b * p.w.heads, kv = hk - b * p.w.kv_heads;
-        row_again<SA_REP_FLOAT32>(p.w, b * p.w.q_b + hh * p.w.q_h + i * p.w.q_n, b * p.w.k_b + kv * p.w.k_h,
-                                  b * p.w.v_b + kv * p.w.v_h, b * p.w.o_b + hh * p.w.o_h + i * p.w.o_n, back + i, p.w.m);
+        const int64_t at = q0 + quarter * 32 + __ffs(left) - 1;
+        repair_row<SA_REP_FLOAT32>(p.w, b * p.w.q_b + hh * p.w.q_h + at * p.w.q_n, b * p.w.k_b + kv * p.w.k_h,
+                                   b * p.w.v_b + kv * p.w.v_h, b * p.w.o_b + hh * p.w.o_h + at * p.w.o_n, back + at, p.w.m,
+                                   nullptr);
       }
     }
   }

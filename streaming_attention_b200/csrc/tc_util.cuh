@@ -66,18 +66,34 @@ struct Abort {
   volatile int* cta;     // shared memory: nonzero once any role of this CTA gave up
   int* global_status;    // device memory: first error code of the launch
   uint64_t limit_ns;     // how long one wait may take before the CTA gives up
+  // whether cta[1] counts on while a warp of the CTA does work of any length that
+  // others may be waiting behind: a wait starts anew when it has
+  bool beats = false;
 };
+
+// Whether a wait that began at t0 is over its limit (t0 and `seen`, the beat then, move on).
+__device__ __forceinline__ bool over_limit(const Abort& ab, uint64_t& t0, int& seen) {
+  const uint64_t now = globaltimer_ns();
+  if (now - t0 <= ab.limit_ns) return false;
+  if (ab.beats && ab.cta[1] != seen) {
+    seen = ab.cta[1];
+    t0 = now;
+    return false;
+  }
+  return true;
+}
 
 // Waits for the given phase parity; gives up after ab.limit_ns (or at once if
 // the CTA is already aborting), records `code` and returns false.
 __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, const Abort& ab, int code) {
   if (mbar_try_wait(bar, parity)) return true;
-  const uint64_t t0 = globaltimer_ns();
+  uint64_t t0 = globaltimer_ns();
+  int seen = 0;
   for (uint32_t it = 0;; ++it) {
     if (mbar_try_wait(bar, parity)) return true;
     if ((it & 63) == 63) {
       if (*ab.cta) return false;
-      if (globaltimer_ns() - t0 > ab.limit_ns) {
+      if (over_limit(ab, t0, seen)) {
         *ab.cta = 1;
         if (ab.global_status) atomicCAS(ab.global_status, 0, code);
         return false;
@@ -99,6 +115,7 @@ __device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, c
 __device__ __forceinline__ bool mbar_wait_warp_lazy(uint64_t* bar, uint32_t parity, const Abort& ab, int code) {
   bool r = false;
   uint64_t t0 = 0;
+  int seen = 0;
   for (uint32_t it = 1;; ++it) {
     if (mbar_try_wait(bar, parity)) {
       r = true;
@@ -106,10 +123,9 @@ __device__ __forceinline__ bool mbar_wait_warp_lazy(uint64_t* bar, uint32_t pari
     }
     if ((it & 255) == 0) {
       if (*ab.cta) break;
-      const uint64_t now = globaltimer_ns();
       if (t0 == 0) {
-        t0 = now;
-      } else if (now - t0 > ab.limit_ns) {
+        t0 = globaltimer_ns();
+      } else if (over_limit(ab, t0, seen)) {
         *ab.cta = 1;
         if (ab.global_status) atomicCAS(ab.global_status, 0, code);
         break;

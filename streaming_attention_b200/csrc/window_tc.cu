@@ -44,8 +44,9 @@
 // row's usual largest).
 //
 // A product with a hidden key's value is 0 * v, NaN where v is NaN or infinite.
-// Rows that come out non-finite are computed again by one thread from the
-// visible keys alone (row_again): what a query does not see cannot reach it.
+// Columns that come out non-finite are computed again by the row's warp from the
+// visible keys alone (repair_row): what a query does not see cannot reach it.
+// The bounded waits of the CTA's other warps are renewed as long as that goes on.
 #include <cuda.h>
 #include <math.h>
 
@@ -317,7 +318,7 @@ window_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
     }
     mbar_init(qfull, 1);
     mbar_init(qempty, 2);
-    *abort_word = 0;
+    abort_word[0] = abort_word[1] = 0;   // [1] counts on while a warp repairs rows
     fence_mbar_init();
     fence_proxy_async_smem();
   }
@@ -329,7 +330,7 @@ window_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  const Abort ab{abort_word, a.status, p.wait_ns};
+  const Abort ab{abort_word, a.status, p.wait_ns, true};
   const uint32_t tS[2] = {tmem, tmem + 128}, tO[2] = {tmem + 256, tmem + 384};
 
   if (warp == 0) {
@@ -678,12 +679,13 @@ window_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
         }
         __syncwarp();
       }
-      if (qi < nq && !fine) {
-        const int g = row & (p.pack - 1), h = h0 + g;
-        row_again<DT>(a, c.b * a.q_b + (int64_t)h * a.q_h + (c.q_row + qi) * a.q_n,
-                      c.b * a.k_b + (int64_t)c.hk * a.k_h + c.k_row * a.k_n,
-                      c.b * a.v_b + (int64_t)c.hk * a.v_h + c.k_row * a.v_n, obase + (int64_t)g * a.o_h + qi * a.o_n,
-                      c.p0 + qi, c.m);
+#pragma unroll 1
+      for (unsigned left = __ballot_sync(0xffffffffu, qi < nq && !fine); left; left &= left - 1) {
+        const int rr = quarter * 32 + __ffs(left) - 1, rqi = t * tq + (rr >> p.pack_log), g = rr & (p.pack - 1);
+        repair_row<DT>(a, c.b * a.q_b + (int64_t)(h0 + g) * a.q_h + (c.q_row + rqi) * a.q_n,
+                       c.b * a.k_b + (int64_t)c.hk * a.k_h + c.k_row * a.k_n,
+                       c.b * a.v_b + (int64_t)c.hk * a.v_h + c.k_row * a.v_n, obase + (int64_t)g * a.o_h + rqi * a.o_n,
+                       c.p0 + rqi, c.m, abort_word + 1);
       }
       tc_fence_before();   // O has been read: the next pair's products may overwrite it
       __syncwarp();
@@ -732,10 +734,11 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Windo
       out[c] = from_f32<T>(x);
     }
   }
-  if (!__all_sync(0xffffffffu, fine) && lane == 0) {
+  if (!__all_sync(0xffffffffu, fine)) {
     const int64_t hk = h / p.group;
-    row_again<DT>(a, b * a.q_b + h * a.q_h + i * a.q_n, b * a.k_b + hk * a.k_h, b * a.v_b + hk * a.v_h,
-                  b * a.o_b + h * a.o_h + i * a.o_n, a.m - a.n + i, a.m);
+    __syncwarp();
+    repair_row<DT>(a, b * a.q_b + h * a.q_h + i * a.q_n, b * a.k_b + hk * a.k_h, b * a.v_b + hk * a.v_h,
+                   b * a.o_b + h * a.o_h + i * a.o_n, a.m - a.n + i, a.m, nullptr);
   }
 }
 

@@ -8,6 +8,7 @@ import torch
 
 import serving_ref as R
 import streaming_attention_b200 as sa
+from streaming_attention_b200 import _lib
 
 pytestmark = pytest.mark.gpu
 
@@ -53,3 +54,73 @@ def test_scale_of_zero(dtype, dev):
             else:
                 os.environ["SA_FORCE_SIMT"] = old
         assert torch.equal(out, plain)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16], ids=["f32", "f16", "bf16"])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+@pytest.mark.parametrize("n,m", [(700, 700), (3, 5000)], ids=["whole", "split"])
+def test_one_bad_column_is_one_bad_column(dtype, bad, n, m, dev):
+    """A value that is not finite in one column of one key: the queries that see it
+    have it there and nowhere else; the others are as if it were not there."""
+    g = torch.Generator(dev).manual_seed(2)
+    q, k, v = (_make(g, dev, dtype, 1, 4, n, 64), *(_make(g, dev, dtype, 1, 2, m, 64) for _ in range(2)))
+    for at, window, sinks in ((2, 150, 4), (5, 150, 4), (m - 130, 150, 4), (m - 2, None, 0)):
+        w = v.clone()
+        w[:, :, at, 37] = bad
+        out = sa.sliding_window_attention(q, k, w, window=window, sinks=sinks)
+        ref, bound = _bound(q[0], k[0], v[0], window, sinks, 0.125, dtype)
+        sees = R.visible(n, m, window, sinks)[:, at]
+        cols = torch.arange(64) != 37
+        R.assert_close(out[0][..., cols.to(dev)], ref[..., cols], bound[..., cols])
+        R.assert_close(out[0][:, ~sees.to(dev)], ref[:, ~sees], bound[:, ~sees])
+        hit = out[0, :, sees.to(dev), 37].float().cpu()
+        assert (torch.isnan(hit) if bad != bad else hit == bad).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16], ids=["f32", "f16", "bf16"])
+def test_keys_that_are_not_finite_make_their_readers_nan(dtype, dev):
+    g = torch.Generator(dev).manual_seed(3)
+    q, k, v = (_make(g, dev, dtype, 1, 2, 400, 128 if dtype != F32 else 64) for _ in range(3))
+    ref, bound = _bound(q[0], k[0], v[0], 60, 0, q.shape[-1] ** -0.5, dtype)
+    for bad in (float("nan"), float("inf"), float("-inf")):
+        w = k.clone()
+        w[:, :, 200, 5] = bad
+        w[:, :, 200, 6] = -bad
+        q[..., 5:7] = 1.0
+        ref, bound = _bound(q[0], k[0], v[0], 60, 0, q.shape[-1] ** -0.5, dtype)
+        out = sa.sliding_window_attention(q, w, v, window=60, sinks=0)[0]
+        assert torch.isnan(out[:, 200:260]).all()
+        for rows in (slice(0, 200), slice(260, None)):
+            R.assert_close(out[:, rows], ref[:, rows], bound[:, rows])
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=["f16", "bf16"])
+def test_repairs_of_any_length_end_no_wait(dtype, dev):
+    """A hidden NaN beside the first tokens makes every row of the call one to repair,
+    each over two thousand keys.  That takes many times the limit that the waits
+    have here, and the CTA's other warps wait behind it: all rows come out."""
+    g = torch.Generator(dev).manual_seed(4)
+    heads, n, m, window = 320, 256, 2400, 2000
+    q, k, v = _make(g, dev, dtype, 1, heads, n, 64), *(_make(g, dev, dtype, 1, heads, m, 64) for _ in range(2))
+    bad = v.clone()
+    bad[:, :, 5] = float("nan")
+    sa.sliding_window_attention(q, k, v, window=window, sinks=4)
+    lib = _lib.load()
+    try:
+        _lib.check(lib.sa_set_wait_limit_ns(1000000), "limit")
+        out = sa.sliding_window_attention(q, k, bad, window=window, sinks=4)
+        torch.cuda.synchronize(dev)
+    finally:
+        lib.sa_set_wait_limit_ns(0)
+    for h in (0, 147, 148, 319):
+        R.assert_close(out[0, h:h + 1], *_bound(q[0, h:h + 1], k[0, h:h + 1], v[0, h:h + 1], window, 4, 0.125, dtype))
+    assert torch.isfinite(out).all()
+
+
+def test_a_bad_first_token_of_a_long_prompt(dev):
+    """Every query sees it, so every row is NaN, and that is found at once."""
+    g = torch.Generator(dev).manual_seed(5)
+    q, k, v = (_make(g, dev, BF16, 1, h, 16384, 128) for h in (8, 2, 2))
+    k[:, :, 0], v[:, :, 0] = float("nan"), float("nan")
+    assert torch.isnan(sa.sliding_window_attention(q, k, v, window=None)).all()
+    assert torch.isnan(sa.sliding_window_attention(q, k, v, window=512, sinks=1)).all()
