@@ -345,8 +345,10 @@ int sa_serving_status(void* stream);
  * d], v [.., m, dv], out like q with dv; strides = {q_b, q_h, q_n, k_b, k_h,
  * k_n, v_b, v_h, v_n, o_b, o_h, o_n}.  Packed: cu_q, cu_k [batch + 1] are the
  * requests' first rows in q / out (n rows in all) and k / v (m rows in all),
- * p counts within the request, the *_b strides are 0; rows behind
- * cu_q[batch] stay as they were, or are zeroed (zero_behind != 0).  d, dv <= 256.
+ * p counts within the request, the *_b strides are 0; a request whose offsets
+ * are out of order or range is reported and skipped.  Rows of no request, those
+ * between a skipped one's offsets too, stay as they were or are zeroed
+ * (zero_behind != 0).  d, dv <= 256.
  * Tensor cores: float16 / bfloat16 of d, dv <= 128 on 16-byte borders (few
  * queries over many keys: split over the SMs, given the workspace); dense
  * contiguous float32 (3xTF32) of d <= 64, dv <= 128 and long enough given a workspace of

@@ -120,21 +120,14 @@ struct WindowArgs {
   const int32_t* cu_q;
   const int32_t* cu_k;
   int* status;
-  int zero_behind;   // packed: write zeros to the rows behind the last request
+  int zero_behind;   // packed: write zeros to the rows that no request writes
 };
 
-// Zeros for the rows of out that belong to no request, dealt out to the grid's
-// threads (`threads` of each CTA, this one the `thread`-th).
-template <typename T>
-__device__ __forceinline__ void zero_rows_behind(const WindowArgs& a, int64_t thread, int64_t threads) {
-  if (!a.cu_q || !a.zero_behind) return;
-  const int64_t lead = min(max((int64_t)a.cu_q[0], (int64_t)0), a.n);   // and before the first
-  const int64_t first = min(max((int64_t)a.cu_q[a.batch], lead), a.n), width = (int64_t)a.heads * a.dv;
-  const int64_t cta = blockIdx.x + (int64_t)blockIdx.y * gridDim.x, ctas = (int64_t)gridDim.x * gridDim.y;
-  for (int64_t e = cta * threads + thread; e < (lead + a.n - first) * width; e += ctas * threads) {
-    const int64_t r = e / width, rest = e - r * width, h = rest / a.dv, row = r < lead ? r : first + r - lead;
-    static_cast<T*>(a.out)[h * a.o_h + row * a.o_n + rest - h * a.dv] = from_f32<T>(0.0f);
-  }
+// Packed: whether request b's offsets are out of order or out of range.  Such a
+// request counts as empty.
+__device__ __forceinline__ bool offsets_refused(const WindowArgs& a, int64_t b) {
+  const int64_t q0 = a.cu_q[b], q1 = a.cu_q[b + 1], k0 = a.cu_k[b], k1 = a.cu_k[b + 1];
+  return q0 < 0 || q1 < q0 || q1 > a.n || k0 < 0 || k1 < k0 || k1 > a.m;
 }
 
 // One request of a (dense or packed) batch: first rows and row counts.
@@ -142,18 +135,11 @@ struct Request {
   int64_t q0, k0, n, m;
 };
 
-// Offsets that are out of order or out of range are clamped (and reported).
 __device__ __forceinline__ Request request_of(const WindowArgs& a, int b) {
-  Request r{0, 0, a.n, a.m};
-  if (a.cu_q) {
-    int64_t q0 = a.cu_q[b], q1 = a.cu_q[b + 1], k0 = a.cu_k[b], k1 = a.cu_k[b + 1];
-    if (q0 < 0 || q1 < q0 || q1 > a.n || k0 < 0 || k1 < k0 || k1 > a.m) {
-      report(a.status, kBadOffsets, b);
-      return Request{0, 0, 0, 0};
-    }
-    r = Request{q0, k0, q1 - q0, k1 - k0};
-  }
-  return r;
+  if (!a.cu_q) return Request{0, 0, a.n, a.m};
+  if (offsets_refused(a, b)) return Request{0, 0, 0, 0};
+  const int64_t q0 = a.cu_q[b], k0 = a.cu_k[b];
+  return Request{q0, k0, a.cu_q[b + 1] - q0, a.cu_k[b + 1] - k0};
 }
 
 // Tile t of a batch of query tiles of `rows` rows.  Dense: t = b * tiles + i.
@@ -180,6 +166,76 @@ __device__ __forceinline__ int tile_request(const WindowArgs& a, int64_t t, int 
 }
 __host__ inline int64_t tile_count(const WindowArgs& a, int rows) {
   return a.cu_q ? a.n / rows + a.batch : ceil_div(a.n, rows) * a.batch;
+}
+
+// Packed: reports the requests whose offsets are refused and writes zeros to the
+// rows of out that no request writes, `tile_rows` rows to a query tile:
+// - those before the first offset and behind the largest, dealt out to the grid's
+//   threads (whole warps, `threads` of each CTA, this one the `thread`-th);
+// - those between a refused request's offsets, by the CTA that finds it;
+// - where an offset steps back, the tiles that tile_request then gives to another
+//   request, likewise.
+// Offsets go from the first to the last of them in steps, and a step back passes
+// rows that one forward has passed before: so that is every row.  (Rows that two
+// steps forward pass hold one's result or the other's, or zeros.)  `beat` as in
+// repair_row.
+template <typename T>
+__device__ __forceinline__ void zero_unwritten_rows(const WindowArgs& a, int tile_rows, int64_t thread, int64_t threads,
+                                                    int* beat) {
+  if (!a.cu_q) return;
+  const int64_t cta = blockIdx.x + (int64_t)blockIdx.y * gridDim.x, ctas = (int64_t)gridDim.x * gridDim.y;
+  const int64_t width = (int64_t)a.heads * a.dv;
+  const int lane = threadIdx.x & 31;
+  auto zero = [&](int64_t first, int64_t e) {   // element e of the rows from `first` on
+    const int64_t r = e / width, rest = e - r * width, h = rest / a.dv;
+    static_cast<T*>(a.out)[h * a.o_h + (first + r) * a.o_n + rest - h * a.dv] = from_f32<T>(0.0f);
+  };
+  auto zero_rows = [&](int64_t x, int64_t y) {   // by this CTA
+    int turn = 0;
+    for (int64_t e = thread; e < (y - x) * width; e += threads) {
+      zero(x, e);
+      if (beat && (++turn & 1023) == 0) atomicAdd(beat, 1);
+    }
+  };
+  bool back = false;
+  for (int64_t b0 = cta; b0 < a.batch; b0 += 32 * ctas) {
+    const int64_t b = b0 + lane * ctas;
+    const bool bad = b < a.batch && offsets_refused(a, b);
+    if (bad) report(a.status, kBadOffsets, b);
+#pragma unroll 1
+    for (unsigned left = __ballot_sync(0xffffffffu, bad); a.zero_behind && left; left &= left - 1) {
+      const int64_t at = b0 + (__ffs(left) - 1) * ctas;
+      const int64_t x = a.cu_q[at], y = a.cu_q[at + 1];
+      back |= y < x;
+      zero_rows(max(x, (int64_t)0), min(y, a.n));
+    }
+  }
+  if (!a.zero_behind) return;
+#pragma unroll 1
+  for (int b = 0; back && b < a.batch; ++b) {
+    const Request r = request_of(a, b);
+    const int64_t first = r.q0 / tile_rows + b, tiles = (r.n + tile_rows - 1) / tile_rows;
+    if (beat) atomicAdd(beat, 1);
+#pragma unroll 1
+    for (int64_t i0 = 0; i0 < tiles; i0 += 32) {
+      int64_t tile;
+      const bool lost = i0 + lane < tiles && tile_request(a, first + i0 + lane, tile_rows, &tile) != b;
+#pragma unroll 1
+      for (unsigned left = __ballot_sync(0xffffffffu, lost); left; left &= left - 1) {
+        const int64_t x = (i0 + __ffs(left) - 1) * tile_rows;
+        zero_rows(r.q0 + x, r.q0 + min(x + tile_rows, r.n));
+      }
+    }
+  }
+  const int64_t lead = min(max((int64_t)a.cu_q[0], (int64_t)0), a.n);
+  int64_t behind = min(max((int64_t)a.cu_q[a.batch], lead), a.n);
+  if (behind < a.n) {   // behind the largest of them, should that not be the last
+    int top = 0;
+    for (int b = lane; b <= a.batch; b += 32) top = max(top, a.cu_q[b]);
+    behind = min(max(behind, (int64_t)__reduce_max_sync(0xffffffffu, top)), a.n);
+  }
+  for (int64_t e = cta * threads + thread; e < (lead + a.n - behind) * width; e += ctas * threads)
+    zero(e < lead * width ? 0 : behind - lead, e);
 }
 
 // The keys that any of the queries at positions p0 .. p1 sees, as two ranges:

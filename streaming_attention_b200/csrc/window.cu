@@ -51,9 +51,9 @@ __global__ void __launch_bounds__(kWThreads) window_simt_kernel(const WindowArgs
   const int tid = threadIdx.x;
   const int qi = tid >> 2, cg = tid & 3;
   if (a.dtype == SA_REP_FLOAT32)
-    zero_rows_behind<float>(a, tid, kWThreads);
+    zero_unwritten_rows<float>(a, kWQ, tid, kWThreads, nullptr);
   else
-    zero_rows_behind<uint16_t>(a, tid, kWThreads);   // zero has the same bits in both 16-bit types
+    zero_unwritten_rows<uint16_t>(a, kWQ, tid, kWThreads, nullptr);   // zero has the same bits in both 16-bit types
   const int h = blockIdx.y, hk = h / (a.heads / a.kv_heads);
   int64_t tile;
   const int b = tile_request(a, blockIdx.x, kWQ, &tile);

@@ -512,7 +512,7 @@ window_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
     __syncwarp();
   } else {
     // ------------------------------------------------------------ softmax rows
-    zero_rows_behind<T>(a, threadIdx.x - 96, kThreads - 96);
+    zero_unwritten_rows<T>(a, p.rows_per_cta, threadIdx.x - 96, kThreads - 96, abort_word + 1);
     const int t = (warp - 3) >> 2;
     const int quarter = warp & 3;
     const int row = quarter * 32 + lane;

@@ -115,8 +115,10 @@ def sliding_window_attention_packed(q: Tensor, k: Tensor, v: Tensor, cu_q: Tenso
     [S,Hkv,D], v [S,Hkv,Dv]; ``cu_q`` and ``cu_k`` (int32 [R+1], on the device)
     are the requests' first rows, so that request r has rows cu_q[r]..cu_q[r+1]
     of q and cu_k[r]..cu_k[r+1] of k and v, its queries at the last of its
-    positions.  No length is read on the host.  Rows of no request (behind
-    cu_q[R]) are left as they were in ``out`` ([T,H,Dv]); in a new one they are zero."""
+    positions.  No length is read on the host: a request whose offsets are out of
+    order or range is skipped, and reported by ``check_serving_status``.  Rows of
+    no request (behind cu_q[R]) and of a skipped one are left as they were in
+    ``out`` ([T,H,Dv]); in a new one they are zero."""
     dev = S.device_of(q, k, v, cu_q, cu_k)
     if not q.ndim == k.ndim == v.ndim == 3:
         raise ValueError("q, k and v must be [T,H,D], [S,Hkv,D], [S,Hkv,Dv]")

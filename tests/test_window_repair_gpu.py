@@ -8,7 +8,7 @@ import torch
 
 import serving_ref as R
 import streaming_attention_b200 as sa
-from streaming_attention_b200 import _lib
+from streaming_attention_b200 import _lib, fast
 
 pytestmark = pytest.mark.gpu
 
@@ -124,3 +124,88 @@ def test_a_bad_first_token_of_a_long_prompt(dev):
     k[:, :, 0], v[:, :, 0] = float("nan"), float("nan")
     assert torch.isnan(sa.sliding_window_attention(q, k, v, window=None)).all()
     assert torch.isnan(sa.sliding_window_attention(q, k, v, window=512, sinks=1)).all()
+
+
+# ------------------------------------------------- offsets out of order or range
+
+@pytest.fixture
+def unchecked(monkeypatch):
+    """Calls as they are without SA_CHECK_STATUS: nothing raises until somebody asks."""
+    monkeypatch.setattr(fast, "_CHECK_STATUS", False)
+
+
+def _fill_pool(dev, nbytes):
+    """What the allocator hands out next is not zero."""
+    x = torch.full((nbytes,), 0x3C, dtype=torch.uint8, device=dev)
+    del x
+
+
+BAD_OFFSETS = [
+    # cu_q, cu_k of 40 rows; which rows of a new result are zero
+    ([0, 10, 30, 55], [0, 10, 30, 40], range(30, 40)),
+    ([0, 10, 30, 40], [0, 10, 50, 40], range(10, 40)),
+    ([-4, 10, 30, 36], [0, 10, 30, 40], [*range(10), *range(36, 40)]),
+    ([0, 10, 20, 5], [0, 10, 20, 40], range(20, 40)),
+    ([8, 50, 60, 70], [0, 10, 20, 30], range(40)),
+    ([3, 12, 12, 12], [0, 41, 41, 41], range(40)),
+    ([30, 40, 40, 20], [0, 40, 40, 40], range(30)),
+]
+
+
+@pytest.mark.parametrize("dtype,d", [(F32, 64), (F16, 64), (BF16, 128), (BF16, 200)])
+@pytest.mark.parametrize("case", range(len(BAD_OFFSETS)))
+def test_every_row_of_a_new_result_is_written(case, dtype, d, unchecked, dev):
+    """Requests with bad offsets are skipped and reported, the others right, and no
+    row of a new result is what the allocator gave; a given one keeps its rows."""
+    cu_q, cu_k, zero = BAD_OFFSETS[case]
+    g = torch.Generator(dev).manual_seed(case)
+    q, k, v = (_make(g, dev, dtype, 40, h, d) for h in (4, 2, 2))
+    to = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    f = lambda **kw: sa.sliding_window_attention_packed(q, k, v, to(cu_q), to(cu_k), window=7, sinks=1, **kw)  # noqa: E731
+    _fill_pool(dev, q.numel() * q.element_size())
+    out = f()
+    with pytest.raises(ValueError, match="offsets of request"):
+        sa.check_serving_status(dev)
+    given = f(out=torch.full_like(q, 7.0))
+    with pytest.raises(ValueError, match="offsets of request"):
+        sa.check_serving_status(dev)
+    zero = torch.tensor(sorted(zero), dtype=torch.long, device=dev)
+    assert (out[zero] == 0).all() and (given[zero] == 7.0).all()
+    seen = set(zero.tolist())
+    for a, b, c, e in zip(cu_q, cu_q[1:], cu_k, cu_k[1:]):
+        if 0 <= a <= b <= 40 and 0 <= c <= e <= 40 and b > a:
+            ref, bound = _bound(q[a:b].transpose(0, 1), k[c:e].transpose(0, 1), v[c:e].transpose(0, 1), 7, 1, d ** -0.5, dtype)
+            for x in (out, given):
+                R.assert_close(x[a:b].transpose(0, 1), ref, bound)
+            seen |= set(range(a, b))
+    assert seen == set(range(40))
+
+
+@pytest.mark.parametrize("dtype,d", [(F32, 64), (BF16, 64)], ids=["f32", "bf16"])
+def test_offsets_that_step_back_over_many_tiles(dtype, d, unchecked, dev):
+    """Requests behind a step back take tiles of the long one before it."""
+    n = 4000
+    cu = torch.tensor([0, n, 50, 51, 52, 53, 54, 54, 60], dtype=torch.int32, device=dev)
+    g = torch.Generator(dev).manual_seed(8)
+    q, k, v = (_make(g, dev, dtype, n, 1, d) for _ in range(3))
+    _fill_pool(dev, q.numel() * q.element_size())
+    out = sa.sliding_window_attention_packed(q, k, v, cu, cu, window=30)[:, 0]
+    with pytest.raises(ValueError, match="offsets of request"):
+        sa.check_serving_status(dev)
+    ref, bound = (x[0].to(dev) for x in _bound(*(x.transpose(0, 1) for x in (q, k, v)), 30, 0, d ** -0.5, dtype))
+    right = ((out.double() - ref).abs() <= bound).all(1)
+    right[50:60] = True          # claimed twice
+    assert (right | (out == 0).all(1)).all() and torch.isfinite(out).all() and right.sum() > 100
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+def test_prefill_with_fewer_rows_than_new_tokens(dtype, unchecked, dev):
+    """The request that the rows end in, and those behind it, are reported; their rows are zero."""
+    layer = sa.StreamingWindowAttention(4, 2, 64, max_requests=3, max_length=64, window=20, sinks=1, page_size=16, device=dev)
+    g = torch.Generator(dev).manual_seed(9)
+    q, k, v = (_make(g, dev, dtype, 40, h, 64) for h in (4, 2, 2))
+    _fill_pool(dev, q.numel() * q.element_size())
+    out = layer.prefill(q, k, v, torch.tensor([10, 35, 20], dtype=torch.int32, device=dev))
+    with pytest.raises(ValueError):
+        sa.check_serving_status(dev)
+    assert (out[10:] == 0).all() and torch.isfinite(out).all() and (out[:10] != 0).any()
