@@ -11,16 +11,27 @@
 //
 // A warp takes blocks of 16 tokens.  A code's bits, moved to the top of a
 // bfloat16's mantissa under the exponent of 16, are 16 + code: a shift and one
-// logical operation for two codes, exact (float32 takes 24 off again: the sums'
-// errors grow with the offset).  With x = least - 16 scale the value is
+// logical operation for two codes, exact.  With x = least - 16 scale the value is
 // s (16 + code) + x, so
 //   S = s_k (K_codes Q^T) + x_k sum(Q)         tokens x rows
 //   O = V_codes^T (p s_v)^T + sum(p x_v)       columns x rows
-// with scales and offsets in float32 on either side of the products.  What bounds
-// it beside the bytes (94 us of 64 requests x 6000..12000 tokens x 8 heads, 611 MB) is
-// instructions: 480 a block and 301 us with every code centred, masks in every
-// block and register double buffers; 212 us now (2.9 TB/s, the integer pipe 60 %
-// busy).  Float16 operands (five integer operations for eight codes in place of
+// with scales and offsets in float32 on either side of the products.
+//
+// Sums.  The matrix units truncate as they add, and over a long cache the output
+// is small against its parts, whose mean cancels: with one chain of products over
+// a request the error of nearly equal weights passed that of a float16 result's
+// own rounding at 12000 tokens and reached 2 % at 131072.  So a block's products
+// start from zero and are added to O outside, rounded; and where the result keeps
+// more than 8 bits the codes of V are centred (16 + code less 24), which takes
+// their mean out of the sums.  Nearly equal weights, 131072 / 1048576 tokens: an error
+// of 1.7e-4 / 3.2e-4 not centred, which is little beside bfloat16's rounding (1.6e-3)
+// and not beside float16's (2.1e-4); centred it does not show there.  Full batch as
+// below: bfloat16 212 us with one chain, 228 so, 238 centred too; float16 247, 254,
+// 262.  Float32 centres K as well and keeps the products of lower pieces apart.
+//
+// What bounds it beside the bytes (94 us of 64 requests x 6000..12000 tokens x 8
+// heads, 611 MB) is instructions: 480 a block and 301 us with every code centred,
+// masks in every block and register double buffers; 228 us now (2.7 TB/s).  Float16 operands (five integer operations for eight codes in place of
 // eight) took 245: their scales cost more than they saved.  Q is
 // bfloat16 as it is, float16 as two and float32 as three bfloat16 pieces (exact,
 // or to 24 bits); p s_v is split into two pieces (16 bits; three for float32).
@@ -83,6 +94,16 @@ __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uin
       "{%0, %1, %2, %3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// The same from a sum of zero.
+__device__ __forceinline__ void mma_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                          uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%10, %10, %10, %10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
 }
 
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
@@ -214,8 +235,9 @@ template <int DT, int DP, int NT>
 __global__ void __launch_bounds__(kThreads, (Shape<DT, DP, NT>::kPerSm)) attend_kernel(const Kv4AttendArgs a) {
   using T = typename Elem<DT>::T;
   using S = Shape<DT, DP, NT>;
-  // codes enter the products plus 16; less 8 for float32, whose sums that shift would cost two bits
+  // codes of K and V enter the products plus 16, or, where the sums need the bits, less 8
   constexpr int kOff = DT == SA_REP_FLOAT32 ? -8 : 16;
+  constexpr int kOffV = DT == SA_REP_BFLOAT16 ? 16 : -8;
   constexpr int kKS = DP / 16;   // k steps of the first product, 16-column tiles of the second
   extern __shared__ __align__(16) uint8_t smem[];
   float* sm_o = reinterpret_cast<float*>(smem);                // [warps][rows][pitch]
@@ -351,8 +373,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<DT, DP, NT>::kPerSm)) attend_
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) off[nt][0] = off[nt][1] = INFINITY;   // no maximum yet: the first score moves it
 
-  // float32: the matrix units truncate as they add, so their sums stay short (a
-  // block) and apart by size, and longer ones are added outside, rounded
+  // float32: the scores' sums are kept apart by size
   constexpr bool kApart = DT == SA_REP_FLOAT32;
   auto work = [&](const Block<DP>& b, int token, auto whole) {
     constexpr bool kWhole = decltype(whole)::value;   // every row sees the whole block
@@ -376,7 +397,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<DT, DP, NT>::kPerSm)) attend_
     }
     const float2 ka = params(b.kp.x), kb = params(b.kp.y), va = params(b.vp.x), vb = params(b.vp.y);
     const float k_s[2] = {ka.x * sc, kb.x * sc}, k_x[2] = {fmaf(-(float)kOff, ka.x, ka.y) * sc, fmaf(-(float)kOff, kb.x, kb.y) * sc};
-    const float v_s[2] = {va.x, vb.x}, v_x[2] = {fmaf(-(float)kOff, va.x, va.y), fmaf(-(float)kOff, vb.x, vb.y)};
+    const float v_s[2] = {va.x, vb.x}, v_x[2] = {fmaf(-(float)kOffV, va.x, va.y), fmaf(-(float)kOffV, vb.x, vb.y)};
     uint32_t on = 0;   // bit 4 nt + e: s[nt][e] is seen
     if (!kWhole) {
 #pragma unroll
@@ -448,17 +469,15 @@ __global__ void __launch_bounds__(kThreads, (Shape<DT, DP, NT>::kPerSm)) attend_
 #pragma unroll
     for (int t = 0; t < kKS; ++t) {
       const uint32_t w = b.v[t];
-      const uint32_t a0 = codes<0, kOff>(w), a1 = codes<1, kOff>(w), a2 = codes<2, kOff>(w), a3 = codes<3, kOff>(w);
+      const uint32_t a0 = codes<0, kOffV>(w), a1 = codes<1, kOffV>(w), a2 = codes<2, kOffV>(w), a3 = codes<3, kOffV>(w);
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        float (&to)[4] = kApart ? sum : o[nt][t];
+        float sum[4];
+        mma_first(sum, a0, a1, a2, a3, pf[nt][S::kP - 1][0], pf[nt][S::kP - 1][1]);
 #pragma unroll
-        for (int q = S::kP - 1; q >= 0; --q) mma(to, a0, a1, a2, a3, pf[nt][q][0], pf[nt][q][1]);
-        if (kApart) {
+        for (int q = S::kP - 2; q >= 0; --q) mma(sum, a0, a1, a2, a3, pf[nt][q][0], pf[nt][q][1]);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) o[nt][t][e] += sum[e];
-        }
+        for (int e = 0; e < 4; ++e) o[nt][t][e] += sum[e];
       }
     }
   };

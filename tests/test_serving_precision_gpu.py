@@ -1,0 +1,83 @@
+"""How precise the attentions are, as root mean squares over the whole output: an
+error that grows with the length of the context shows here long before it passes
+the bounds for single elements."""
+
+import math
+
+import pytest
+import torch
+
+import streaming_attention_b200 as sa
+
+pytestmark = pytest.mark.gpu
+
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+
+
+@pytest.fixture(scope="module")
+def dev():
+    assert torch.cuda.is_available(), "GPU tests need a CUDA device"
+    return torch.device("cuda:0")
+
+
+def _rms(x):
+    return x.double().pow(2).mean().sqrt().item()
+
+
+def _long_cache(length, heads, dim, dev):
+    """A cache of one request: random codes, scales and least values as rows of roughly normal values have them."""
+    g = torch.Generator(dev).manual_seed(length)
+    page = 64
+    pages = -(-length // page)
+    half = sa.Kv4Cache.padded_dim(dim) // 2
+    u8 = lambda *s: torch.randint(0, 256, s, generator=g, device=dev, dtype=torch.uint8)  # noqa: E731
+
+    def params():
+        scale = 0.25 + 0.15 * torch.rand((pages, heads, page, 1), generator=g, device=dev)
+        return torch.cat([scale, -7.5 * scale + 0.3 * torch.randn(scale.shape, generator=g, device=dev)], -1).to(BF16)
+
+    return sa.Kv4Cache(u8(pages, heads, page, half), params(), u8(pages, heads, page // 4, half, 4), params(), dim)
+
+
+def _attention64(cache, q, length):
+    """q [H,D] over the whole cache: the result, and sum p (least + 8 scale), the mean that the codes' sums are added to."""
+    per = q.shape[0] // cache.kv_heads
+    qd = q.double().reshape(cache.kv_heads, per, -1) / math.sqrt(cache.dim)
+    parts = [torch.arange(a, min(length, a + 65536), device=q.device, dtype=torch.int32) for a in range(0, length, 65536)]
+    w = torch.softmax(torch.cat([torch.einsum("gpd,tgd->gpt", qd, cache.read(s)[0].double()) for s in parts], -1), -1)
+    out = sum(torch.einsum("gpt,tgd->gpd", w[..., s[0]:s[-1] + 1], cache.read(s)[1].double()) for s in parts)
+    page = cache.page_size
+    par = torch.cat([cache.v_params[s.long() // page, :, s.long() % page].double() for s in parts])
+    mean = torch.einsum("gpt,tg->gp", w, par[..., 1] + 8 * par[..., 0])
+    return out.reshape(q.shape), mean
+
+
+# requests that share the one cache, so that each request's blocks go to few warps
+ATTEND = [(2000, 4, 64), (12000, 8, 64), (40000, 8, 64), (131072, 8, 64), (40000, 1, 2), (300000, 1, 2)]
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16], ids=["f32", "f16", "bf16"])
+@pytest.mark.parametrize("spread", [0.02, 1.5], ids=["equal", "normal"])
+@pytest.mark.parametrize("length,heads,requests", ATTEND)
+def test_cache_attention_keeps_its_precision_over_long_caches(length, heads, requests, spread, dtype, dev):
+    """Beside the output's own rounding the error is at most `own`, per unit of p:
+    16 bits: a block's truncated sums (4 2^-23 of its parts) and sqrt(blocks of a
+    warp) rounded additions (2^-24 each) of sums no larger than the parts, which
+    are scale |code + offset|: 0.33 * 23.5 in bfloat16, 0.33 * 4 in float16.
+    float32: the additions of the centred sums, which are as large as the result
+    and the mean beside it; and 2^-20 for scores and probabilities of 24 bits."""
+    cache = _long_cache(length, heads, 128, dev)
+    q = (torch.randn(heads * 4, 128, generator=torch.Generator(dev).manual_seed(1), device=dev) * spread).to(dtype)
+    tables = torch.arange(cache.num_pages, dtype=torch.int32, device=dev).expand(requests, -1).contiguous()
+    lens = torch.full((requests,), length, dtype=torch.int32, device=dev)
+    out = cache.attend(q.expand(requests, -1, -1), tables, lens)
+    assert (out == out[:1]).all()
+    ref, mean = _attention64(cache, q, length)
+    adds = math.sqrt(length / 16 / 16)      # at least 16 warps to a request
+    size, rounding = _rms(ref), _rms(ref.to(dtype).double() - ref)
+    if dtype == F32:
+        own = size * 2.0 ** -20 + adds * 2.0 ** -24 * (_rms(mean) + size)
+    else:
+        own = 0.33 * (23.5 if dtype == BF16 else 4.0) * (4 * 2.0 ** -23 + adds * 2.0 ** -24)
+    err = _rms(out[0].double() - ref)
+    assert err <= math.hypot(rounding, own) * 1.02, (err / size, rounding / size, own / size)
