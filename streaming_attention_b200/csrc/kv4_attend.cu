@@ -259,11 +259,12 @@ __global__ void __launch_bounds__(kThreads, (Shape<DT, DP, NT>::kPerSm)) attend_
   const int cap = a.width << a.c.page_shift;
   int length = max(a.lengths[r], 0);
   if (length > cap && threadIdx.x == 0) report(a.status, kBadLength, r);
-  const int window = (int)min(a.window, (int64_t)1 << 30), sinks = (int)min(a.sinks, (int64_t)1 << 30);
+  // as int: positions lie below 2^31 - 1, so differences of two are less than the largest
+  const int window = (int)min(a.window, (int64_t)2147483647), sinks = (int)min(a.sinks, (int64_t)2147483647);
   // positions of this tile's rows (rows behind the last count as the last)
   auto position = [&](int row) { return length - a.n + min(row0 + row, rows - 1) / group; };
   const int p_lo = position(0), p_hi = position(S::kRows - 1);
-  const KeyRanges kr = key_ranges(p_lo, p_hi, min(length, cap), window, sinks);
+  const KeyRanges kr = key_ranges(p_lo, p_hi, min(length, cap), a.window, a.sinks);
   const int sink_blocks = (int)((kr.first + 15) >> 4);
   const int win_begin = max((int)(kr.begin >> 4), sink_blocks), win_end = (int)((kr.end + 15) >> 4);
   const int blocks = sink_blocks + max(win_end - win_begin, 0);
@@ -405,7 +406,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<DT, DP, NT>::kPerSm)) attend_
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int j = token + 2 * g + (e >> 1), p = position(nt * 8 + 2 * cc + (e & 1));
-          if (j <= p && (j > p - window || j < sinks) && j < cap) on |= 1u << (4 * nt + e);
+          if (j <= p && (p - j < window || j < sinks) && j < cap) on |= 1u << (4 * nt + e);
         }
     }
     bool move = false;
@@ -482,7 +483,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<DT, DP, NT>::kPerSm)) attend_
     }
   };
   auto go = [&](const Block<DP>& b, int token) {
-    if (token + 15 <= p_lo && (token > p_hi - window || token + 16 <= sinks))
+    if (token + 15 <= p_lo && (p_hi - token < window || token + 16 <= sinks))
       work(b, token, std::true_type{});
     else
       work(b, token, std::false_type{});
