@@ -594,9 +594,11 @@ int launch_one(const Kv4AttendArgs& a, cudaStream_t s) {
   const int64_t y = a.c.heads * ceil_div(rows, S::kRows);
   if (y > 65535) return set_error(SA_ERR_UNSUPPORTED, "kv4 attend: grid too large");
   // CTAs per (request, key head): while a warp keeps at least four blocks of the
-  // longest request the table allows and the grid has less than three
-  // rounds (the batch above: 232 us with six, 231 with one)
-  const int64_t longest = std::min<int64_t>((int64_t)a.width << a.c.page_shift, a.window + std::min(a.sinks, a.window) + a.n);
+  // longest request the table allows, of what window and first tokens show of it
+  // (8192 first tokens and a window of 64 of one request: 65 us as one CTA, 20 as
+  // eight), and the grid has less than three rounds (the batch above as it was at
+  // 212 us: 232 with six, 231 with one)
+  const int64_t longest = std::min<int64_t>((int64_t)a.width << a.c.page_shift, a.window + a.sinks + a.n);
   int splits = 1;
   while (splits < 8 && longest >= (int64_t)splits * 2 * kWarps * 16 * 4 && y * a.requests * splits < 148 * S::kPerSm * 3) splits *= 2;
   cudaLaunchConfig_t cfg{};

@@ -6,7 +6,9 @@ import math
 import pytest
 import torch
 
+import serving_ref as R
 import streaming_attention_b200 as sa
+from test_kv4_gpu import _check_attend, _filled
 
 pytestmark = pytest.mark.gpu
 
@@ -29,3 +31,13 @@ def test_windows_past_2_30_tokens(window, sinks, at):
     w = others / (page * math.exp(top) + others)      # what the other tokens weigh
     # their sum, of 2^30 equal terms by 64 warps of eight lanes, is off by far less than a hundredth
     assert (out.double() - (3 - 4 * w)).abs().max() <= 2 ** -8 * 3 + 0.01 * 4 * w
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+def test_many_first_tokens_and_a_short_window(dtype):
+    """They count for how many CTAs share a request as a long window does."""
+    dev, length = torch.device("cuda:0"), 9000
+    cache, tables, lens, ks, vs = _filled(dev, [length], 2, 64, 64, torch.float32, 30)
+    q = torch.randn(1, 2, 8, 64, generator=R.rng(31)).to(dtype).to(dev)
+    for window, sinks in ((1, length), (64, 6000), (3, 4097)):
+        _check_attend(cache.attend(q, tables, lens, window=window, sinks=sinks), q, ks, vs, [length], window, sinks)
