@@ -116,11 +116,19 @@ class Kv4Cache:
     """The cache's storage.  ``Kv4Cache.empty`` makes one; the constructor takes
     the four tensors (k_codes uint8 [P,Hkv,page,Dp/2], k_params bfloat16
     [P,Hkv,page,2], v_codes uint8 [P,Hkv,page/4,Dp/2,4], v_params bfloat16
-    [P,Hkv,page,2]; Dp is ``dim`` filled up to 32, 64, 128 or 256)."""
+    [P,Hkv,page,2]; Dp is ``dim`` filled up to 32, 64, 128 or 256).  They are
+    attributes of those names and may be replaced between calls, all four where
+    the pages change; a captured call keeps those it was captured with."""
 
     def __init__(self, k_codes: Tensor, k_params: Tensor, v_codes: Tensor, v_params: Tensor, dim: int) -> None:
         if not 1 <= dim <= S.MAX_DIM:
             raise ValueError(f"dim must lie in [1, {S.MAX_DIM}]")
+        self.k_codes, self.k_params, self.v_codes, self.v_params, self.dim = k_codes, k_params, v_codes, v_params, int(dim)
+        self._bind()
+
+    def _bind(self) -> None:
+        """Checks the four tensors as they are now and keeps what the calls need of them."""
+        held = k_codes, k_params, v_codes, v_params = self.k_codes, self.k_params, self.v_codes, self.v_params
         if k_codes.ndim != 4:
             raise ValueError("k_codes must be [P,Hkv,page,Dp/2]")
         pages, heads, page, half = k_codes.shape
@@ -128,9 +136,9 @@ class Kv4Cache:
             _check_page_size(page)
         if pages == 0 or heads == 0:
             raise ValueError("the cache needs at least one page and one head")
-        if half != self.padded_dim(dim) // 2:
-            raise ValueError(f"a row of codes of dim {dim} takes {self.padded_dim(dim) // 2} bytes, got {half}")
-        self.device = S.device_of(k_codes, k_params, v_codes, v_params)
+        if half != self.padded_dim(self.dim) // 2:
+            raise ValueError(f"a row of codes of dim {self.dim} takes {self.padded_dim(self.dim) // 2} bytes, got {half}")
+        device = S.device_of(k_codes, k_params, v_codes, v_params)
         params = (pages, heads, page, 2)
         for t, shape, dt, what in ((k_codes, None, torch.uint8, "k_codes"),
                                    (v_codes, (pages, heads, page // 4, half, 4), torch.uint8, "v_codes"),
@@ -138,10 +146,17 @@ class Kv4Cache:
                                    (v_params, params, torch.bfloat16, "v_params")):
             if t.dtype != dt or (shape is not None and t.shape != shape) or not t.is_contiguous():
                 raise ValueError(f"{what} must be contiguous {dt} {list(shape or k_codes.shape)}")
-        self.k_codes, self.k_params, self.v_codes, self.v_params = k_codes, k_params, v_codes, v_params
-        self.dim, self.kv_heads, self.page_size, self.num_pages = int(dim), heads, page, pages
-        self._args = (k_codes.data_ptr(), k_params.data_ptr(), v_codes.data_ptr(), v_params.data_ptr(), pages, heads,
-                      page, self.dim)
+        self.device, self.kv_heads, self.page_size, self.num_pages = device, heads, page, pages
+        self._held, self._args = held, tuple(t.data_ptr() for t in held) + (pages, heads, page, self.dim)
+
+    def _storage(self):
+        """Pointers and sizes for a call: the tensors may have been replaced, or their
+        memory, since the last one."""
+        a, (k, kp, v, vp) = self._args, self._held
+        if (self.k_codes is not k or self.k_params is not kp or self.v_codes is not v or self.v_params is not vp or
+                k.data_ptr() != a[0] or kp.data_ptr() != a[1] or v.data_ptr() != a[2] or vp.data_ptr() != a[3]):
+            self._bind()
+        return self._args
 
     @staticmethod
     def padded_dim(dim: int) -> int:
@@ -167,6 +182,7 @@ class Kv4Cache:
     def append(self, k: Tensor, v: Tensor, slots: Tensor) -> None:
         """Quantises k and v [T,Hkv,D] into ``slots`` (int32 [T]); a negative slot
         leaves its token out, and no slot may be given twice in one call."""
+        cache = self._storage()
         S.device_of(self.k_codes, k, v, slots)
         code = S.dtype_code(k, v)
         if k.ndim != 3 or k.shape[1:] != (self.kv_heads, self.dim) or v.shape != k.shape:
@@ -175,12 +191,13 @@ class Kv4Cache:
         if k.shape[0] == 0:
             return
         k, v = S.rows(k), S.rows(v)
-        S.launch(self.device, "sa_kv4_append", *self._args, k.data_ptr(), v.data_ptr(),
+        S.launch(self.device, "sa_kv4_append", *cache, k.data_ptr(), v.data_ptr(),
                  S.strides(*k.stride()[:2], *v.stride()[:2]), slots.data_ptr(), k.shape[0], code)
 
     def read(self, slots: Tensor, dtype: torch.dtype = torch.float32) -> Tuple[Tensor, Tensor]:
         """The keys and values [T,Hkv,D] that ``slots`` (int32 [T]) stand for, in
         ``dtype``; zeros for a negative slot."""
+        cache = self._storage()
         S.device_of(self.k_codes, slots)
         if dtype not in S.DTYPES:
             raise ValueError(f"unsupported dtype {dtype}: float32, float16 and bfloat16 are accepted")
@@ -191,7 +208,7 @@ class Kv4Cache:
         k = torch.empty((t, self.kv_heads, self.dim), device=self.device, dtype=dtype)
         v = torch.empty((t, self.kv_heads, self.dim), device=self.device, dtype=dtype)
         if t:
-            S.launch(self.device, "sa_kv4_read", *self._args, k.data_ptr(), v.data_ptr(), slots.data_ptr(), t,
+            S.launch(self.device, "sa_kv4_read", *cache, k.data_ptr(), v.data_ptr(), slots.data_ptr(), t,
                      S.DTYPES[dtype])
         return k, v
 
@@ -204,6 +221,7 @@ class Kv4Cache:
         are appended before.  Query i of N stands at lengths[r] - N + i and sees
         as in ``sliding_window_attention``; a query that sees nothing (a request
         of length 0, or shorter than N) gives zeros.  Returns q's shape and dtype."""
+        cache = self._storage()
         S.device_of(self.k_codes, q, tables, lengths)
         code = S.dtype_code(q)
         w, s = S.check_window(window, sinks)
@@ -220,7 +238,7 @@ class Kv4Cache:
         out = torch.empty((r, n, heads, d), device=self.device, dtype=q.dtype)
         if out.numel():
             q4 = S.rows(q4)
-            S.launch(self.device, "sa_kv4_attend", *self._args, q4.data_ptr(), out.data_ptr(),
+            S.launch(self.device, "sa_kv4_attend", *cache, q4.data_ptr(), out.data_ptr(),
                      S.strides(*q4.stride()[:3]), tables.data_ptr(), lengths.data_ptr(), r, n, heads, tables.shape[1],
                      w, s, float(1.0 / math.sqrt(d) if scale is None else scale), code)
         return out[:, 0] if q.ndim == 3 else out
