@@ -69,14 +69,29 @@ def ptr(t: Optional[Tensor]) -> Optional[int]:
     return None if t is None else t.data_ptr()
 
 
+def _whole(x, what: str) -> int:
+    if type(x) is int:
+        return x
+    try:
+        i = int(x)
+    except (TypeError, ValueError, OverflowError):
+        i = None
+    if i is None or i != x:
+        raise ValueError(f"{what} must be a whole number, got {x!r}")
+    return i
+
+
 def check_window(window: Optional[int], sinks: int) -> Tuple[int, int]:
     """Window (0: without end) and first tokens as the C ABI takes them; what lies
     beyond every position (2^31) hides and shows no more than that does."""
-    if window is not None and window <= 0:
-        raise ValueError("window must be positive, or None for no end")
-    if sinks < 0:
+    w, s = 0, _whole(sinks, "sinks")
+    if window is not None:
+        w = _whole(window, "window")
+        if w <= 0:
+            raise ValueError("window must be positive, or None for no end")
+    if s < 0:
         raise ValueError("sinks must be non-negative")
-    return (0 if window is None else min(int(window), 1 << 40)), min(int(sinks), 1 << 40)
+    return min(w, 1 << 40), min(s, 1 << 40)
 
 
 def _raw_stream(index: int) -> int:

@@ -104,3 +104,17 @@ def test_rotary_frequencies():
     f = sa.rotary_frequencies(8, base=100.0)
     assert f.tolist() == pytest.approx([1.0, 100 ** -0.25, 0.1, 100 ** -0.75], rel=1e-15)
     assert sa.rotary_frequencies(0).numel() == 0
+
+
+def test_windows_and_first_tokens_are_whole_numbers():
+    from streaming_attention_b200 import _serving as S
+    nan, inf = float("nan"), float("inf")
+    for window, sinks, match in ((0.5, 0, "window must be a whole"), (1.5, 0, "window must be a whole"), (nan, 0, "window must be a whole"),
+                                 (inf, 0, "window must be a whole"), ("4", 0, "window must be a whole"), (4, 0.5, "sinks must be a whole"),
+                                 (4, None, "sinks must be a whole"), (0, 0, "window must be positive"), (-1.0, 0, "window must be positive"),
+                                 (4, -1, "sinks must be non-negative")):
+        with pytest.raises(ValueError, match=match):
+            S.check_window(window, sinks)
+        with pytest.raises(ValueError, match=match):
+            sa.StreamingWindowAttention(2, 2, 64, max_requests=1, max_length=10, window=window, sinks=sinks)
+    assert S.check_window(None, 3) == (0, 3) and S.check_window(7.0, 0) == (7, 0) and S.check_window(2 ** 64, 2 ** 50) == (1 << 40, 1 << 40)
