@@ -64,6 +64,11 @@ int check_heads(int heads, int kv_heads) {
 int64_t window_of(int64_t window) { return window > 0 ? std::min(window, (int64_t)1 << 40) : (int64_t)1 << 40; }
 int64_t sinks_of(int64_t sinks) { return std::min(sinks, (int64_t)1 << 40); }
 
+// Whether [b, h, n, width] with these strides is contiguous; an axis of one entry may have any.
+bool contiguous(int64_t b, int64_t s_b, int64_t h, int64_t s_h, int64_t n, int64_t s_n, int64_t width) {
+  return (n <= 1 || s_n == width) && (h <= 1 || s_h == n * width) && (b <= 1 || s_b == h * n * width);
+}
+
 int page_shift_of(int page_size) {
   for (int s = 4; s <= 8; ++s)
     if (page_size == 1 << s) return s;
@@ -172,9 +177,9 @@ int sa_window_attention(const void* q, const void* k, const void* v, void* out, 
   const char* simt = getenv("SA_FORCE_SIMT");
   if (window_tc_takes(a) && !(simt && simt[0] == '1')) return launch_window_tc(a, workspace, workspace_bytes, (cudaStream_t)stream);
   // float32 on the tensor cores: contiguous tensors and a workspace
-  if (dtype == SA_REP_FLOAT32 && !cu_q && workspace && a.status && a.q_n == d && a.q_h == n * d && a.q_b == heads * a.q_h &&
-      a.k_n == d && a.k_h == m * d && a.k_b == kv_heads * a.k_h && a.v_n == dv && a.v_h == m * dv &&
-      a.v_b == kv_heads * a.v_h && a.o_n == dv && a.o_h == n * dv && a.o_b == heads * a.o_h &&
+  if (dtype == SA_REP_FLOAT32 && !cu_q && workspace && a.status && contiguous(batch, a.q_b, heads, a.q_h, n, a.q_n, d) &&
+      contiguous(batch, a.k_b, kv_heads, a.k_h, m, a.k_n, d) && contiguous(batch, a.v_b, kv_heads, a.v_h, m, a.v_n, dv) &&
+      contiguous(batch, a.o_b, heads, a.o_h, n, a.o_n, dv) &&
       window_tf32_bytes(batch, heads, kv_heads, n, m, d, dv, window, sinks_of(sinks)) > 0)
     return window_tf32_run(a, workspace, workspace_bytes, (cudaStream_t)stream);
   return launch_window_simt(a, (cudaStream_t)stream);
