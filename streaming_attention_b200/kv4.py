@@ -147,14 +147,15 @@ class Kv4Cache:
             if t.dtype != dt or (shape is not None and t.shape != shape) or not t.is_contiguous():
                 raise ValueError(f"{what} must be contiguous {dt} {list(shape or k_codes.shape)}")
         self.device, self.kv_heads, self.page_size, self.num_pages = device, heads, page, pages
-        self._held, self._args = held, tuple(t.data_ptr() for t in held) + (pages, heads, page, self.dim)
+        self._held, self._ptrs = held, (k_codes.data_ptr(), k_params.data_ptr(), v_codes.data_ptr(), v_params.data_ptr())
+        self._args = (*self._ptrs, pages, heads, page, self.dim)
 
     def _storage(self):
         """Pointers and sizes for a call: the tensors may have been replaced, or their
         memory, since the last one."""
-        a, (k, kp, v, vp) = self._args, self._held
+        k, kp, v, vp = self._held
         if (self.k_codes is not k or self.k_params is not kp or self.v_codes is not v or self.v_params is not vp or
-                k.data_ptr() != a[0] or kp.data_ptr() != a[1] or v.data_ptr() != a[2] or vp.data_ptr() != a[3]):
+                (k.data_ptr(), kp.data_ptr(), v.data_ptr(), vp.data_ptr()) != self._ptrs):
             self._bind()
         return self._args
 
