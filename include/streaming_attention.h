@@ -404,6 +404,7 @@ int sa_kv4_attend(const void* k_codes, const void* k_params, const void* v_codes
  * the last token and where there is no page (per_request > 0: token i of
  * request r stands at r * per_request + i instead, max_tokens is requests *
  * per_request, and -1 fills the rows of requests with fewer new tokens); free_out[0] is what is left.
+ * New tokens beyond the rows are reported; they count, and their pages are entered.
  * Page ids are below free_size.  No output overlaps an input. */
 int sa_plan_kv_pages(const int32_t* lengths, const int32_t* fresh, int32_t* tables, const int32_t* free_pages,
                      const int32_t* free_count, int requests, int width, int free_size, int page_size, int max_tokens,

@@ -43,6 +43,18 @@ __device__ __forceinline__ int64_t pages_of(int64_t tokens, int shift, int width
   return min((tokens + (1 << shift) - 1) >> shift, (int64_t)width);
 }
 
+// The page that entry `row` of a request's table takes, the first of the new ones
+// being `had`: nth from the end of the `have` free ones, `before` taken by the
+// requests before; -1 where there is none.
+__device__ __forceinline__ int32_t fresh_page(const PlanArgs& a, int have, int before, int64_t row, int64_t had) {
+  const int64_t at = (int64_t)have - 1 - before - (row - had);
+  if (at < 0) return -1;
+  const int32_t page = a.free_pages[at];
+  if (page < a.free_size) return page;
+  report(a.status, kBadPage, page);
+  return -1;
+}
+
 __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs a) {
   extern __shared__ int32_t plan_smem[];
   int32_t* sum_new = plan_smem;                       // [requests + 1], exclusive
@@ -157,12 +169,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs a) {
         if (row < had) {
           page = a.tables[(int64_t)lo * a.width + row];
         } else {
-          const int64_t at = (int64_t)have - 1 - sum_pages[lo] - (row - had);
-          page = at >= 0 ? a.free_pages[at] : -1;
-          if (page >= a.free_size) {
-            report(a.status, kBadPage, page);
-            page = -1;
-          }
+          page = fresh_page(a, have, sum_pages[lo], row, had);
           if ((pos & mask) == 0) a.tables[(int64_t)lo * a.width + row] = page;
         }
         if (page >= 0 && page < a.free_size) slot = (page << a.page_shift) | (int32_t)(pos & mask);
@@ -170,6 +177,16 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs a) {
     }
     a.positions[t] = position;
     a.slots[t] = slot;
+  }
+  // pages that are opened by tokens without a row: they are taken, so they are entered too
+  for (int64_t r = (int64_t)blockIdx.x * kPlanThreads + tid; r < a.requests; r += (int64_t)gridDim.x * kPlanThreads) {
+    const int64_t add = a.fresh[r];
+    const int64_t rows = a.per_request > 0 ? a.per_request : max((int64_t)a.max_tokens - sum_new[r], (int64_t)0);
+    if (add <= rows) continue;
+    const int64_t len = max(a.lengths[r], 0), had = pages_of(len, a.page_shift, a.width);
+    const int64_t from = (len + rows + mask) >> a.page_shift;   // the first that no token with a row opens
+    for (int64_t row = max(had, from); row < pages_of(len + add, a.page_shift, a.width); ++row)
+      a.tables[r * a.width + row] = fresh_page(a, have, sum_pages[r], row, had);
   }
 }
 

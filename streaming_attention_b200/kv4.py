@@ -58,8 +58,8 @@ def plan_kv_pages(lengths: Tensor, new: Tensor, tables: Tensor, free_pages: Tens
     the same inputs enters the same).  Positions and
     slots are packed, ``max_tokens`` long, or, with ``per_request=n`` instead,
     [R*n] with n rows for each request.  Too few pages, a row of the table that is too short
-    and more new tokens than rows leave slots at -1 and are reported
-    by ``check_serving_status``."""
+    and more new tokens than rows (they count, and their pages are entered) leave
+    slots at -1 and are reported by ``check_serving_status``."""
     dev = S.device_of(lengths, new, tables, free_pages, free_count)
     _check_page_size(page_size)
     if tables.ndim != 2 or tables.dtype != torch.int32 or not tables.is_contiguous():

@@ -1,0 +1,58 @@
+"""Page plans and releases where something does not fit: what is taken from the free
+list is in the tables, and goes back from there."""
+
+import pytest
+import torch
+
+import serving_ref as R
+import streaming_attention_b200 as sa
+from streaming_attention_b200 import fast
+from test_serving_path_gpu import _i32, _state
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def dev():
+    assert torch.cuda.is_available(), "GPU tests need a CUDA device"
+    return torch.device("cuda:0")
+
+
+@pytest.fixture
+def unchecked(monkeypatch):
+    """Calls as they are without SA_CHECK_STATUS."""
+    monkeypatch.setattr(fast, "_CHECK_STATUS", False)
+
+
+def _reported(match):
+    with pytest.raises(ValueError, match=match):
+        sa.check_serving_status()
+    sa.check_serving_status()
+
+
+@pytest.mark.parametrize("requests,rows", [(1, 0), (3, 17), (40, 333), (1500, 4100)])
+@pytest.mark.parametrize("per_request", [False, True])
+def test_pages_of_tokens_without_rows_are_entered(requests, rows, per_request, unchecked, dev):
+    """The tables and the free count are those of a plan with rows enough; the rows that
+    are there hold what they hold there."""
+    g = R.rng(requests)
+    page, width = 16, 12
+    lengths = torch.randint(0, 60, (requests,), generator=g).tolist()
+    new = torch.randint(60, 130, (requests,), generator=g).tolist()
+    tables, free, count = _state(lengths, page, width, requests)
+    want = R.plan(lengths, new, tables, free, count, page)
+    t = _i32(tables, dev)
+    size = dict(per_request=7) if per_request else dict(max_tokens=rows)
+    got = sa.plan_kv_pages(_i32(lengths, dev), _i32(new, dev), t, _i32(free, dev), _i32([count], dev), page_size=page, **size)
+    _reported("more than the output holds")
+    assert t.tolist() == want[4] and got.free_count.tolist() == [want[5]]
+    assert got.lengths.tolist() == want[0] and got.offsets.tolist() == want[1]
+    if per_request:
+        at = [want[1][r] + i for r in range(requests) for i in range(7)]
+        assert got.slots.tolist() == [want[3][i] for i in at] and got.positions.tolist() == [want[2][i] for i in at]
+    else:
+        assert got.slots.tolist() == want[3][:rows] and got.positions.tolist() == want[2][:rows]
+    # every page is in a table or among the free ones, once
+    held = [p for row in t.tolist() for p in row if p >= 0]
+    assert sorted(held + free[:got.free_count.item()]) == sorted(set(held + free[:got.free_count.item()]))
+    assert len(held) + got.free_count.item() == len(set(sum(([p for p in r if p >= 0] for r in tables), []))) + count
