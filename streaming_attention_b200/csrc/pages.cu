@@ -50,7 +50,7 @@ __device__ __forceinline__ int32_t fresh_page(const PlanArgs& a, int have, int b
   const int64_t at = (int64_t)have - 1 - before - (row - had);
   if (at < 0) return -1;
   const int32_t page = a.free_pages[at];
-  if (page < a.free_size) return page;
+  if (page >= 0 && page < a.free_size) return page;
   report(a.status, kBadPage, page);
   return -1;
 }
@@ -168,6 +168,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs a) {
         int32_t page;
         if (row < had) {
           page = a.tables[(int64_t)lo * a.width + row];
+          if (page < -1 || page >= a.free_size) report(a.status, kBadPage, page);   // -1: taken when none was free
         } else {
           page = fresh_page(a, have, sum_pages[lo], row, had);
           if ((pos & mask) == 0) a.tables[(int64_t)lo * a.width + row] = page;

@@ -56,3 +56,18 @@ def test_pages_of_tokens_without_rows_are_entered(requests, rows, per_request, u
     held = [p for row in t.tolist() for p in row if p >= 0]
     assert sorted(held + free[:got.free_count.item()]) == sorted(set(held + free[:got.free_count.item()]))
     assert len(held) + got.free_count.item() == len(set(sum(([p for p in r if p >= 0] for r in tables), []))) + count
+
+
+def test_page_ids_outside_the_cache_are_reported_wherever_they_stand(unchecked, dev):
+    n, new, c = _i32([20], dev), _i32([1], dev), _i32([2], dev)
+    plan = lambda table, free: sa.plan_kv_pages(n, new, _i32([table], dev), _i32(free, dev), c, page_size=16, max_tokens=1)  # noqa: E731
+    assert plan([0, 1, -1], [2, 3]).slots.tolist() == [1 * 16 + 4]
+    sa.check_serving_status(dev)
+    for bad in (-7, 2, 10 ** 6):
+        assert plan([0, bad, -1], [0, 1]).slots.tolist() == [-1]
+        _reported("outside the cache")
+    n.fill_(16)
+    for bad in (-1, 2):
+        p = plan([0, -1, -1], [0, bad])
+        assert p.slots.tolist() == [-1] and p.tables.tolist() == [[0, -1, -1]]
+        _reported("outside the cache")
