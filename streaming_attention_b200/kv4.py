@@ -79,6 +79,8 @@ def plan_kv_pages(lengths: Tensor, new: Tensor, tables: Tensor, free_pages: Tens
         max_tokens = r * per_request
     elif max_tokens < 0:
         raise ValueError("max_tokens must be non-negative")
+    if max(max_tokens, free_pages.shape[0]) > 2 ** 31 - 1:
+        raise ValueError("a plan takes less than 2^31 rows and pages")
     # one allocation for the outputs
     lens, offsets, positions, slots, free = lengths.new_empty(2 * r + 2 + 2 * max_tokens).split(
         (r, r + 1, max_tokens, max_tokens, 1))

@@ -71,3 +71,11 @@ def test_page_ids_outside_the_cache_are_reported_wherever_they_stand(unchecked, 
         p = plan([0, -1, -1], [0, bad])
         assert p.slots.tolist() == [-1] and p.tables.tolist() == [[0, -1, -1]]
         _reported("outside the cache")
+
+
+def test_rows_past_31_bits_are_refused(dev):
+    n = _i32([1], dev)
+    with pytest.raises(ValueError, match="2\\^31"):
+        sa.plan_kv_pages(n, n, n[:, None], n, n, page_size=16, max_tokens=2 ** 32)
+    with pytest.raises(ValueError, match="2\\^31"):
+        sa.plan_kv_pages(n, n, n[:, None], n, n, page_size=16, per_request=2 ** 31)
