@@ -192,8 +192,9 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs a) {
 }
 
 // Returns the pages of the requests whose `drop` is not 0 to the end of the
-// free list, in request order, and empties their rows of the table.  One CTA:
-// it runs when a request ends.
+// free list, in request order, and empties their rows of the table, whole: entries
+// behind the pages a request holds are of nobody's (a plan whose lengths were not
+// taken over leaves some) and go nowhere.  One CTA: it runs when a request ends.
 __global__ void __launch_bounds__(kPlanThreads)
 release_kernel(int32_t* lengths, int32_t* tables, const uint8_t* drop, int32_t* free_pages, int32_t* free_count,
                int requests, int width, int free_size, int page_shift, int* status) {
@@ -204,6 +205,7 @@ release_kernel(int32_t* lengths, int32_t* tables, const uint8_t* drop, int32_t* 
   for (int r = 0; r < requests; ++r) {
     if (!drop[r]) continue;
     const int64_t held = pages_of(max(lengths[r], 0), page_shift, width);
+    for (int64_t c = held + tid; c < width; c += kPlanThreads) tables[(int64_t)r * width + c] = -1;
     for (int64_t c0 = 0; c0 < held; c0 += kPlanThreads) {
       const int64_t c = c0 + tid;
       int32_t page = -1;

@@ -79,3 +79,14 @@ def test_rows_past_31_bits_are_refused(dev):
         sa.plan_kv_pages(n, n, n[:, None], n, n, page_size=16, max_tokens=2 ** 32)
     with pytest.raises(ValueError, match="2\\^31"):
         sa.plan_kv_pages(n, n, n[:, None], n, n, page_size=16, per_request=2 ** 31)
+
+
+def test_release_empties_whole_rows(unchecked, dev):
+    """Entries behind the held pages, as a plan leaves whose lengths were not taken over, do not go back to the free list."""
+    n, drop = _i32([20, 20], dev), torch.tensor([True, False], device=dev)
+    t = _i32([[0, 1, 5, 6], [2, 3, 7, -1]], dev)
+    f, c = _i32([5, 6, 7, 8, -1, -1, -1, -1, -1], dev), _i32([4], dev)
+    sa.release_kv_pages(n, t, drop, f, c, page_size=16)
+    sa.check_serving_status(dev)
+    assert t.tolist() == [[-1] * 4, [2, 3, 7, -1]] and n.tolist() == [0, 20]
+    assert c.tolist() == [6] and f.tolist()[:6] == [5, 6, 7, 8, 0, 1]
