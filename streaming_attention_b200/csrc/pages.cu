@@ -212,6 +212,10 @@ release_kernel(int32_t* lengths, int32_t* tables, const uint8_t* drop, int32_t* 
       if (c < held) {
         page = tables[(int64_t)r * width + c];
         tables[(int64_t)r * width + c] = -1;
+        if (page < -1 || page >= free_size) {
+          report(status, kBadPage, page);
+          page = -1;
+        }
       }
       const unsigned on = __ballot_sync(0xffffffffu, page >= 0);
       if (lane == 0) part[warp] = __popc(on);

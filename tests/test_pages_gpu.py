@@ -90,3 +90,11 @@ def test_release_empties_whole_rows(unchecked, dev):
     sa.check_serving_status(dev)
     assert t.tolist() == [[-1] * 4, [2, 3, 7, -1]] and n.tolist() == [0, 20]
     assert c.tolist() == [6] and f.tolist()[:6] == [5, 6, 7, 8, 0, 1]
+
+
+def test_release_reports_page_ids_outside_the_cache(unchecked, dev):
+    n, drop = _i32([20, 20], dev), torch.tensor([True, True], device=dev)
+    t, f, c = _i32([[0, 1], [4, 99]], dev), _i32([5, 6, -1, -1, -1, -1, -1], dev), _i32([2], dev)
+    sa.release_kv_pages(n, t, drop, f, c, page_size=16)
+    _reported("page 99 lies outside")
+    assert (t == -1).all() and n.tolist() == [0, 0] and c.tolist() == [5] and f.tolist()[:5] == [5, 6, 0, 1, 4]
