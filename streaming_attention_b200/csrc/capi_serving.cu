@@ -211,8 +211,8 @@ int sa_release_kv_pages(int32_t* lengths, int32_t* tables, const uint8_t* drop, 
   const int shift = page_shift_of(page_size);
   if (shift < 0) return set_error(SA_ERR_INVALID_ARG, "page_size must be 16, 32, 64, 128 or 256");
   if (requests < 0 || width < 0 || free_size < 0) return set_error(SA_ERR_INVALID_ARG, "sizes must be non-negative");
-  if (requests == 0 || width == 0) return SA_OK;
-  if (!lengths || !tables || !drop || !free_pages || !free_count) return set_error(SA_ERR_INVALID_ARG, "null pointer");
+  if (requests == 0) return SA_OK;
+  if (!lengths || !drop || !free_count || (width > 0 && !tables) || (free_size > 0 && !free_pages)) return set_error(SA_ERR_INVALID_ARG, "null pointer");
   return launch_release_pages(lengths, tables, drop, free_pages, free_count, requests, width, free_size, shift,
                               status_word(), (cudaStream_t)stream);
 }

@@ -98,3 +98,10 @@ def test_release_reports_page_ids_outside_the_cache(unchecked, dev):
     sa.release_kv_pages(n, t, drop, f, c, page_size=16)
     _reported("page 99 lies outside")
     assert (t == -1).all() and n.tolist() == [0, 0] and c.tolist() == [5] and f.tolist()[:5] == [5, 6, 0, 1, 4]
+
+
+def test_release_without_table_entries_empties_the_requests(unchecked, dev):
+    n, e = _i32([5, 6], dev), _i32([], dev)
+    sa.release_kv_pages(n, e.reshape(2, 0), torch.tensor([True, False], device=dev), e, _i32([0], dev), page_size=16)
+    assert n.tolist() == [0, 6]
+    sa.check_serving_status(dev)
