@@ -411,6 +411,13 @@ int sa_plan_kv_pages(const int32_t* lengths, const int32_t* fresh, int32_t* tabl
                      int per_request, int32_t* lengths_out, int32_t* offsets, int32_t* positions, int32_t* slots, int32_t* free_out,
                      void* stream);
 
+/* sa_plan_kv_pages for packed prompts, whose tokens see one another and nothing
+ * that their requests hold: new tokens of a request of lengths[r] > 0 are reported. */
+int sa_plan_kv_prompts(const int32_t* lengths, const int32_t* fresh, int32_t* tables, const int32_t* free_pages,
+                       const int32_t* free_count, int requests, int width, int free_size, int page_size, int max_tokens,
+                       int32_t* lengths_out, int32_t* offsets, int32_t* positions, int32_t* slots, int32_t* free_out,
+                       void* stream);
+
 /* Returns the pages of the requests with drop[r] != 0 to the free list and
  * empties those requests (all in place). */
 int sa_release_kv_pages(int32_t* lengths, int32_t* tables, const uint8_t* drop, int32_t* free_pages,

@@ -16,8 +16,8 @@ namespace sa {
 
 int launch_plan_pages(const int32_t* lengths, const int32_t* fresh, int32_t* tables, const int32_t* free_pages,
                       const int32_t* free_count, int requests, int width, int free_size, int page_shift,
-                      int max_tokens, int per_request, int32_t* lengths_out, int32_t* offsets, int32_t* positions, int32_t* slots,
-                      int32_t* free_out, int* status, cudaStream_t s);
+                      int max_tokens, int per_request, int prompts, int32_t* lengths_out, int32_t* offsets, int32_t* positions,
+                      int32_t* slots, int32_t* free_out, int* status, cudaStream_t s);
 int launch_release_pages(int32_t* lengths, int32_t* tables, const uint8_t* drop, int32_t* free_pages,
                          int32_t* free_count, int requests, int width, int free_size, int page_shift, int* status,
                          cudaStream_t s);
@@ -92,6 +92,27 @@ int check_cache(Kv4Cache* c, const void* k_codes, const void* k_params, const vo
   return SA_OK;
 }
 
+int plan_pages(const int32_t* lengths, const int32_t* fresh, int32_t* tables, const int32_t* free_pages,
+               const int32_t* free_count, int requests, int width, int free_size, int page_size, int max_tokens,
+               int per_request, int prompts, int32_t* lengths_out, int32_t* offsets, int32_t* positions, int32_t* slots,
+               int32_t* free_out, void* stream) {
+  const int shift = page_shift_of(page_size);
+  if (shift < 0) return set_error(SA_ERR_INVALID_ARG, "page_size must be 16, 32, 64, 128 or 256");
+  if (requests < 0 || width < 0 || free_size < 0 || max_tokens < 0 || per_request < 0)
+    return set_error(SA_ERR_INVALID_ARG, "sizes must be non-negative");
+  if (per_request > 0 && (int64_t)requests * per_request != max_tokens)
+    return set_error(SA_ERR_INVALID_ARG, "max_tokens must be requests * per_request");
+  if ((int64_t)requests * width > 2147483647LL || free_size > (2147483647 >> shift))
+    return set_error(SA_ERR_UNSUPPORTED, "the page table or the cache is too large");
+  if (!offsets || !free_out || !free_count || (requests > 0 && (!lengths || !fresh || !lengths_out)) ||
+      (requests > 0 && width > 0 && !tables) || (free_size > 0 && !free_pages) ||
+      (max_tokens > 0 && (!positions || !slots)))
+    return set_error(SA_ERR_INVALID_ARG, "null pointer");
+  return launch_plan_pages(lengths, fresh, tables, free_pages, free_count, requests, width, free_size, shift,
+                           max_tokens, per_request, prompts, lengths_out, offsets, positions, slots, free_out, status_word(),
+                           (cudaStream_t)stream);
+}
+
 }  // namespace
 }  // namespace sa
 
@@ -120,6 +141,7 @@ int sa_serving_status(void* stream) {
     case kBadLength: return set_error(SA_ERR_INVALID_ARG, "request %lld is longer than its row of the page table", at);
     case kBadOffsets: return set_error(SA_ERR_INVALID_ARG, "the offsets of request %lld are out of order or out of range", at);
     case kNoPages: return set_error(SA_ERR_INVALID_ARG, "%lld pages wanted, more than are free", at);
+    case kHeld: return set_error(SA_ERR_INVALID_ARG, "request %lld holds tokens already, which its prompt does not see", at);
     case kNoRows: return set_error(SA_ERR_INVALID_ARG, "%lld entries, more than the output holds", at);
     default: break;
   }
@@ -189,21 +211,16 @@ int sa_plan_kv_pages(const int32_t* lengths, const int32_t* fresh, int32_t* tabl
                      const int32_t* free_count, int requests, int width, int free_size, int page_size, int max_tokens,
                      int per_request, int32_t* lengths_out, int32_t* offsets, int32_t* positions, int32_t* slots, int32_t* free_out,
                      void* stream) {
-  const int shift = page_shift_of(page_size);
-  if (shift < 0) return set_error(SA_ERR_INVALID_ARG, "page_size must be 16, 32, 64, 128 or 256");
-  if (requests < 0 || width < 0 || free_size < 0 || max_tokens < 0 || per_request < 0)
-    return set_error(SA_ERR_INVALID_ARG, "sizes must be non-negative");
-  if (per_request > 0 && (int64_t)requests * per_request != max_tokens)
-    return set_error(SA_ERR_INVALID_ARG, "max_tokens must be requests * per_request");
-  if ((int64_t)requests * width > 2147483647LL || free_size > (2147483647 >> shift))
-    return set_error(SA_ERR_UNSUPPORTED, "the page table or the cache is too large");
-  if (!offsets || !free_out || !free_count || (requests > 0 && (!lengths || !fresh || !lengths_out)) ||
-      (requests > 0 && width > 0 && !tables) || (free_size > 0 && !free_pages) ||
-      (max_tokens > 0 && (!positions || !slots)))
-    return set_error(SA_ERR_INVALID_ARG, "null pointer");
-  return launch_plan_pages(lengths, fresh, tables, free_pages, free_count, requests, width, free_size, shift,
-                           max_tokens, per_request, lengths_out, offsets, positions, slots, free_out, status_word(),
-                           (cudaStream_t)stream);
+  return plan_pages(lengths, fresh, tables, free_pages, free_count, requests, width, free_size, page_size, max_tokens,
+                    per_request, 0, lengths_out, offsets, positions, slots, free_out, stream);
+}
+
+int sa_plan_kv_prompts(const int32_t* lengths, const int32_t* fresh, int32_t* tables, const int32_t* free_pages,
+                       const int32_t* free_count, int requests, int width, int free_size, int page_size, int max_tokens,
+                       int32_t* lengths_out, int32_t* offsets, int32_t* positions, int32_t* slots, int32_t* free_out,
+                       void* stream) {
+  return plan_pages(lengths, fresh, tables, free_pages, free_count, requests, width, free_size, page_size, max_tokens, 0,
+                    1, lengths_out, offsets, positions, slots, free_out, stream);
 }
 
 int sa_release_kv_pages(int32_t* lengths, int32_t* tables, const uint8_t* drop, int32_t* free_pages,

@@ -37,6 +37,7 @@ struct PlanArgs {
   int* status;
   int requests, width, free_size, max_tokens, page_shift;
   int per_request;   // > 0: token i of request r stands at r * per_request + i, not packed
+  int prompts;       // new tokens of requests that hold some are reported
 };
 
 __device__ __forceinline__ int64_t pages_of(int64_t tokens, int shift, int width) {
@@ -79,6 +80,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs a) {
       if (first) {
         if (len + add > ((int64_t)a.width << a.page_shift)) report(a.status, kBadLength, r);
         if (a.per_request > 0 && add > a.per_request) report(a.status, kNoRows, add);
+        if (a.prompts && len > 0 && add > 0) report(a.status, kHeld, r);
         a.lengths_out[r] = (int32_t)min(len + add, (int64_t)2147483647);
       }
     }
@@ -245,13 +247,13 @@ release_kernel(int32_t* lengths, int32_t* tables, const uint8_t* drop, int32_t* 
 
 int launch_plan_pages(const int32_t* lengths, const int32_t* fresh, int32_t* tables, const int32_t* free_pages,
                       const int32_t* free_count, int requests, int width, int free_size, int page_shift,
-                      int max_tokens, int per_request, int32_t* lengths_out, int32_t* offsets, int32_t* positions, int32_t* slots,
-                      int32_t* free_out, int* status, cudaStream_t s) {
+                      int max_tokens, int per_request, int prompts, int32_t* lengths_out, int32_t* offsets, int32_t* positions,
+                      int32_t* slots, int32_t* free_out, int* status, cudaStream_t s) {
   if (requests > kPlanMaxRequests)
     return set_error(SA_ERR_UNSUPPORTED, "page plan: more than %d requests", kPlanMaxRequests);
   const PlanArgs a{lengths, fresh,     tables, free_pages, free_count, lengths_out, offsets,    positions,
                    slots,   free_out,  status, requests,   width,      free_size,   max_tokens, page_shift,
-                   per_request};
+                   per_request, prompts};
   const size_t smem = (size_t)(requests + 1) * 8;
   if (smem > 48 * 1024) {
     const cudaError_t e =

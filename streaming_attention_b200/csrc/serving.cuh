@@ -20,6 +20,7 @@ constexpr int kBadLength = 402;   // a request longer than its row of the page t
 constexpr int kBadOffsets = 403;  // offsets that are not monotone or leave the tensors
 constexpr int kNoPages = 404;     // the list of free pages ran out
 constexpr int kNoRows = 405;      // more new tokens than the outputs hold
+constexpr int kHeld = 406;        // a prompt for a request that holds tokens
 
 __device__ __forceinline__ void report(int* status, int code, long long index) {
   if (status && atomicCAS(status, 0, code) == 0) *reinterpret_cast<volatile long long*>(status + 2) = index;

@@ -50,7 +50,8 @@ class PagePlan(NamedTuple):
 
 
 def plan_kv_pages(lengths: Tensor, new: Tensor, tables: Tensor, free_pages: Tensor, free_count: Tensor, *,
-                  page_size: int, max_tokens: Optional[int] = None, per_request: Optional[int] = None) -> PagePlan:
+                  page_size: int, max_tokens: Optional[int] = None, per_request: Optional[int] = None,
+                  prompts: bool = False) -> PagePlan:
     """Makes room for ``new[r]`` tokens of each request behind its ``lengths[r]``
     (int32 [R]).  Pages come in request order from the end of the first
     ``free_count[0]`` entries of ``free_pages`` (int32 [F], ids below F) and are
@@ -59,7 +60,8 @@ def plan_kv_pages(lengths: Tensor, new: Tensor, tables: Tensor, free_pages: Tens
     slots are packed, ``max_tokens`` long, or, with ``per_request=n`` instead,
     [R*n] with n rows for each request.  Too few pages, a row of the table that is too short
     and more new tokens than rows (they count, and their pages are entered) leave
-    slots at -1 and are reported by ``check_serving_status``."""
+    slots at -1 and are reported by ``check_serving_status``; with ``prompts`` (and
+    ``max_tokens``) so are new tokens of requests that hold some already."""
     dev = S.device_of(lengths, new, tables, free_pages, free_count)
     _check_page_size(page_size)
     if tables.ndim != 2 or tables.dtype != torch.int32 or not tables.is_contiguous():
@@ -74,6 +76,8 @@ def plan_kv_pages(lengths: Tensor, new: Tensor, tables: Tensor, free_pages: Tens
     if (max_tokens is None) == (per_request is None):
         raise ValueError("give either max_tokens or per_request")
     if per_request is not None:
+        if prompts:
+            raise ValueError("prompts are packed: give max_tokens")
         if per_request <= 0:
             raise ValueError("per_request must be positive")
         max_tokens = r * per_request
@@ -84,9 +88,10 @@ def plan_kv_pages(lengths: Tensor, new: Tensor, tables: Tensor, free_pages: Tens
     # one allocation for the outputs
     lens, offsets, positions, slots, free = lengths.new_empty(2 * r + 2 + 2 * max_tokens).split(
         (r, r + 1, max_tokens, max_tokens, 1))
-    S.launch(dev, "sa_plan_kv_pages", lengths.data_ptr(), new.data_ptr(), tables.data_ptr(), free_pages.data_ptr(),
-             free_count.data_ptr(), r, width, free_pages.shape[0], page_size, max_tokens, per_request or 0, lens.data_ptr(),
-             offsets.data_ptr(), positions.data_ptr(), slots.data_ptr(), free.data_ptr())
+    S.launch(dev, "sa_plan_kv_prompts" if prompts else "sa_plan_kv_pages", lengths.data_ptr(), new.data_ptr(),
+             tables.data_ptr(), free_pages.data_ptr(), free_count.data_ptr(), r, width, free_pages.shape[0], page_size,
+             max_tokens, *(() if prompts else (per_request or 0,)), lens.data_ptr(), offsets.data_ptr(), positions.data_ptr(),
+             slots.data_ptr(), free.data_ptr())
     return PagePlan(lens, offsets, positions, slots, tables, free)
 
 

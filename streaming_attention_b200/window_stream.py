@@ -79,8 +79,10 @@ class StreamingWindowAttention:
         """Prompts of requests that hold nothing yet: ``new`` (int32
         [max_requests]) tokens of each, packed in request order in q [T,H,D], k
         and v [T,Hkv,D]; T may be larger than their sum (rows behind stay zero).
-        Requests with new[r] = 0 are left alone, whatever they hold."""
-        plan, q, k = self._step(q, k, v, new, max_tokens=q.shape[0])
+        Requests with new[r] = 0 are left alone, whatever they hold; new tokens of
+        one that holds some would not see them, and are reported by
+        ``check_serving_status``."""
+        plan, q, k = self._step(q, k, v, new, max_tokens=q.shape[0], prompts=True)
         return sliding_window_attention_packed(q, k, v, plan.offsets, plan.offsets, window=self.window,
                                                sinks=self.sinks, scale=self.scale)
 

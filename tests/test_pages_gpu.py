@@ -105,3 +105,20 @@ def test_release_without_table_entries_empties_the_requests(unchecked, dev):
     sa.release_kv_pages(n, e.reshape(2, 0), torch.tensor([True, False], device=dev), e, _i32([0], dev), page_size=16)
     assert n.tolist() == [0, 6]
     sa.check_serving_status(dev)
+
+
+def test_prompts_of_requests_that_hold_tokens_are_reported(unchecked, dev):
+    layer = sa.StreamingWindowAttention(2, 2, 64, max_requests=3, max_length=64, window=20, page_size=16, device=dev)
+    x = torch.randn(12, 2, 64, generator=R.rng(1)).to(dev)
+    layer.prefill(x, x, x, _i32([5, 0, 7], dev))
+    layer.prefill(x, x, x, _i32([0, 9, 0], dev))        # the others are left alone
+    layer.decode(x[:3], x[:3], x[:3])
+    sa.check_serving_status(dev)
+    layer.prefill(x, x, x, _i32([0, 0, 4], dev))
+    _reported("request 2 holds tokens already")
+    layer.release(torch.tensor([False, False, True], device=dev))
+    layer.prefill(x, x, x, _i32([0, 0, 4], dev))
+    sa.check_serving_status(dev)
+    n = _i32([1], dev)
+    with pytest.raises(ValueError, match="packed"):
+        sa.plan_kv_pages(n, n, n[:, None], n, n, page_size=16, per_request=1, prompts=True)

@@ -118,3 +118,12 @@ def test_windows_and_first_tokens_are_whole_numbers():
         with pytest.raises(ValueError, match=match):
             sa.StreamingWindowAttention(2, 2, 64, max_requests=1, max_length=10, window=window, sinks=sinks)
     assert S.check_window(None, 3) == (0, 3) and S.check_window(7.0, 0) == (7, 0) and S.check_window(2 ** 64, 2 ** 50) == (1 << 40, 1 << 40)
+
+
+def test_prompt_plan_arguments():
+    plan = lambda requests=2, width=4, free=8, page=16, cap=5, lengths=P, tables=P, slots=P: _lib.load().sa_plan_kv_prompts(  # noqa: E731
+        lengths, P, tables, P, P, requests, width, free, page, cap, P, P, P, slots, P, None)
+    for kw, rc in ((dict(page=17), INV), (dict(requests=-1), INV), (dict(width=-1), INV), (dict(free=-1), INV), (dict(cap=-1), INV),
+                   (dict(lengths=None), INV), (dict(tables=None), INV), (dict(slots=None), INV), (dict(requests=1 << 20, width=1 << 12), UNS),
+                   (dict(free=1 << 28), UNS), (dict(requests=16385), UNS)):
+        assert plan(**kw) == rc, kw
