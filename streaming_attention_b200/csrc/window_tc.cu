@@ -832,9 +832,12 @@ bool window_tc_takes(const WindowArgs& a) {
 
 // Parts of each pair's keys, for a dense call whose pairs fill less than half of
 // the SMs: at most 32 (a lane each in the join), at least four tiles to a part,
-// and from 48 tiles on.  A tile takes 0.85 us, the join's launch and workspace 11 us
-// of the caller's time: 8192 keys 105 us whole and 39 split, 4096 57 and 39, 1024 28
-// and 39.
+// from 48 tiles on, and where the tiles that a pair saves (1.3 us each, 0.9 with few
+// rows) cost more than the parts (15 us for the join's launch and the workspace,
+// 0.9 ns for each part's row of 128 columns, written and read).  32/8 heads of 128,
+// whole and split: 1 query over 8192 keys 106 and 31 us, over 4096 59 and 26; 256
+// over 4096 82 and 51; 512, in two parts, over 4096 82 and 90 (stays whole), over
+// 8192 151 and 126; over 1024 keys 28 whole and 39.
 int window_tc_splits(const WindowArgs& a) {
   if (a.cu_q) return 1;
   WindowTcParams p{};
@@ -843,7 +846,10 @@ int window_tc_splits(const WindowArgs& a) {
   const int64_t rows = std::min<int64_t>(a.n, p.rows_per_cta), span = std::min<int64_t>(a.window, a.m) + rows;
   const int64_t tiles = ceil_div(std::min<int64_t>(a.m, span + std::min<int64_t>(a.sinks, a.m)), kCols);
   const int64_t splits = std::min<int64_t>(std::min<int64_t>(148 / std::max<int64_t>(pairs, 1), tiles / 4), 32);
-  return splits < 2 || tiles < 48 ? 1 : (int)splits;
+  if (splits < 2 || tiles < 48) return 1;
+  const double saved = 1.3 * (double)tiles * (double)(splits - 1) / (double)splits;
+  const double parts = (double)a.batch * a.heads * (double)a.n * (double)splits;
+  return saved > 15.0 + 0.0009 / 132.0 * part_pitch(a.dv) * parts ? (int)splits : 1;
 }
 
 size_t window_tc_bytes(const WindowArgs& a) {

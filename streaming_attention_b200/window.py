@@ -94,7 +94,7 @@ def sliding_window_attention(q: Tensor, k: Tensor, v: Tensor, *, window: Optiona
     if out.numel():
         _check_heads(heads, kv_heads)
         ws = None
-        if q.dtype == torch.float32 or (n * heads <= 4096 and m > 2900):   # 16-bit: few rows have their many keys split
+        if q.dtype == torch.float32 or m > 3008:   # 16 bits: 48 tiles of 64 keys and more may be split
             size = _workspace_size(b, heads, kv_heads, n, m, d, dv, w, s, code)
             if size:
                 ws = torch.empty(size, device=dev, dtype=torch.uint8)

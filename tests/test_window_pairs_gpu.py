@@ -71,3 +71,17 @@ def test_many_short_packed_pairs(dev):
         if x:
             _check(*(y[None, rows].transpose(1, 2) for y in (q, k, v, out)), 20, 49)
         at += x
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=["f16", "bf16"])
+@pytest.mark.parametrize("h,hkv,n,m,d,window,sinks", [(32, 8, 256, 4096, 128, None, 0), (8, 8, 520, 5000, 64, 4500, 3),
+                                                     (32, 8, 512, 9000, 64, None, 0), (4, 2, 1030, 12000, 80, 11000, 70)])
+def test_hundreds_of_queries_over_split_keys(h, hkv, n, m, d, window, sinks, dtype, dev):
+    """Too few pairs for the chip though the rows are many: their keys are split, and joined."""
+    g = torch.Generator(dev).manual_seed(n)
+    q, k, v = (torch.randn(1, x, y, d, generator=g, device=dev).to(dtype) for x, y in ((h, n), (hkv, m), (hkv, m)))
+    out = sa.sliding_window_attention(q, k, v, window=window, sinks=sinks)
+    for x in range(0, h, h // 2):
+        y = x // (h // hkv)
+        _check(q[:, x:x + 1], k[:, y:y + 1], v[:, y:y + 1], out[:, x:x + 1], window, sinks)
+    assert torch.equal(out, sa.sliding_window_attention(q, k, v, window=window, sinks=sinks))
