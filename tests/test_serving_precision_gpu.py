@@ -7,6 +7,7 @@ import math
 import pytest
 import torch
 
+import serving_ref as R
 import streaming_attention_b200 as sa
 
 pytestmark = pytest.mark.gpu
@@ -81,3 +82,25 @@ def test_cache_attention_keeps_its_precision_over_long_caches(length, heads, req
         own = 0.33 * (23.5 if dtype == BF16 else 4.0) * (4 * 2.0 ** -23 + adds * 2.0 ** -24)
     err = _rms(out[0].double() - ref)
     assert err <= math.hypot(rounding, own) * 1.02, (err / size, rounding / size, own / size)
+
+
+@pytest.mark.parametrize("dtype,d,dv", [(F32, 64, 64), (F32, 64, 128), (F32, 40, 32), (F16, 128, 128), (BF16, 128, 128), (BF16, 64, 80)])
+@pytest.mark.parametrize("spread", [0.02, 1.5], ids=["equal", "normal"])
+@pytest.mark.parametrize("n,m,window", [(512, 4608, 4096), (300, 700, 100), (2, 20000, None)], ids=["long", "short", "split"])
+def test_windowed_attention_keeps_its_precision(n, m, window, spread, dtype, d, dv, dev):
+    """float32: 24 truncated additions to a score (a sixth of a step each in the root
+    mean square, of sums as large as the score, 3 in base 2) and 48 to a chain of two
+    tiles of O: 2.7e-6 ln 2 and 1.4e-6 of the result.  16 bits: the probabilities'
+    rounding, at most half a step of the type for all of a row alike, beside the output's own."""
+    g = torch.Generator(dev).manual_seed(n + d)
+    mk = lambda h, rows, w, s: (torch.randn(1, h, rows, w, generator=g, device=dev) * s).to(dtype)  # noqa: E731
+    q, k, v = mk(4, n, d, spread), mk(2, m, d, 1.0), mk(2, m, dv, 1.0)
+    out = sa.sliding_window_attention(q, k, v, window=window, sinks=5)
+    kd, vd = (x[0].double().repeat_interleave(2, 0) for x in (k, v))
+    sees = R.visible(n, m, window, 5).to(dev)
+    x = torch.einsum("hnd,hmd->hnm", q[0].double(), kd) / math.sqrt(d)
+    ref = torch.einsum("hnm,hmd->hnd", torch.softmax(x.masked_fill(~sees, -math.inf), -1), vd)
+    size, rounding = _rms(ref), _rms(ref.to(dtype).double() - ref)
+    own = size * (3.3e-6 if dtype == F32 else R.HALF[dtype])
+    err = _rms(out[0].double() - ref)
+    assert err <= math.hypot(rounding, own), (err / size, rounding / size, own / size)
