@@ -127,7 +127,7 @@ __global__ void __launch_bounds__(kWThreads) window_simt_kernel(const WindowArgs
       float es = 0.0f;
 #pragma unroll
       for (int rr = 0; rr < 8; ++rr) {
-        const float e = on[rr] ? (m_new == -INFINITY ? 0.0f : expf(x[rr] - m_off)) : 0.0f;
+        const float e = on[rr] && x[rr] != -INFINITY ? expf(x[rr] - m_off) : 0.0f;   // NaN before any maximum stays NaN
         E[qi][cg * 8 + rr] = e;
         es += e;
       }

@@ -209,3 +209,23 @@ def test_prefill_with_fewer_rows_than_new_tokens(dtype, unchecked, dev):
     with pytest.raises(ValueError):
         sa.check_serving_status(dev)
     assert (out[10:] == 0).all() and torch.isfinite(out).all() and (out[:10] != 0).any()
+
+
+@pytest.mark.parametrize("packed", [False, True])
+@pytest.mark.parametrize("dtype,d", [(F32, 64), (F32, 128), (F16, 64), (BF16, 128), (BF16, 200)])
+def test_a_row_that_sees_nothing_but_nan_is_nan(dtype, d, packed, dev):
+    """Whatever kernel takes it: a key that is NaN, alone in a window, or before all the others that a row sees."""
+    g = torch.Generator(dev).manual_seed(6)
+    q, k, v = (_make(g, dev, dtype, 1, 2, 300, d) for _ in range(3))
+    k[:, :, 0], k[:, :, 200] = float("nan"), float("nan")
+    cu = torch.tensor([0, 300], dtype=torch.int32, device=dev)
+    rows = lambda x: x[0].transpose(0, 1).contiguous()  # noqa: E731
+    for window, sinks in ((1, 0), (1, 1), (64, 0), (None, 0)):
+        if packed:
+            out = sa.sliding_window_attention_packed(rows(q), rows(k), rows(v), cu, cu, window=window, sinks=sinks)
+            out = out.transpose(0, 1)[None]
+        else:
+            out = sa.sliding_window_attention(q, k, v, window=window, sinks=sinks)
+        sees = R.visible(300, 300, window, sinks)
+        bad = (sees[:, 0] | sees[:, 200]).to(dev)
+        assert torch.isnan(out[:, :, bad]).all() and torch.isfinite(out[:, :, ~bad]).all()
