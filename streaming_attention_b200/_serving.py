@@ -58,6 +58,12 @@ def rows(t: Tensor) -> Tensor:
     return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.detach().contiguous()
 
 
+def repeats(t: Tensor) -> bool:
+    """Whether entries of t share memory along an axis (an expanded tensor), so that
+    a kernel cannot write them."""
+    return any(st == 0 and n > 1 for n, st in zip(t.shape, t.stride()))
+
+
 _ARRAYS = {n: ctypes.c_int64 * n for n in (3, 4, 8, 12)}
 
 

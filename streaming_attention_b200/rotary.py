@@ -66,6 +66,8 @@ def qk_norm_rotary(q: Tensor, k: Tensor, positions: Tensor, q_weight: Optional[T
         for o, x in zip(out, (q, k)):
             if o.shape != x.shape or o.dtype != x.dtype or o.device != dev or (d > 1 and o.stride(-1) != 1):
                 raise ValueError("out must match q and k, its last dimension contiguous")
+            if S.repeats(o):
+                raise ValueError("out must not be an expanded tensor")
     if t:
         q, k, frequencies = S.rows(q), S.rows(k), frequencies.contiguous()
         q_weight, k_weight = (None if w is None else w.contiguous() for w in (q_weight, k_weight))

@@ -138,6 +138,8 @@ def sliding_window_attention_packed(q: Tensor, k: Tensor, v: Tensor, cu_q: Tenso
         out = q.new_empty((t, heads, dv)) if cu_q.size(0) > 1 else q.new_zeros((t, heads, dv))
     elif tuple(out.shape) != (t, heads, dv) or out.dtype != q.dtype or out.device != dev or (dv > 1 and out.stride(-1) != 1):
         raise ValueError(f"out must be [{t},{heads},{dv}] like q, its last dimension contiguous")
+    elif S.repeats(out):
+        raise ValueError("out must not be an expanded tensor")
     if out.numel():
         _check_heads(heads, kv_heads)
         q, k, v = _on_borders(q), _on_borders(k), _on_borders(v)
