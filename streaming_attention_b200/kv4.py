@@ -109,6 +109,8 @@ def release_kv_pages(lengths: Tensor, tables: Tensor, drop: Tensor, free_pages: 
         raise ValueError(f"drop must be bool [{r}]")
     S.int32(lengths, (r,), "lengths")
     S.int32(tables, (r, width), "tables")
+    if free_pages.ndim != 1:
+        raise ValueError("free_pages must be [F]")
     S.int32(free_pages, free_pages.shape, "free_pages")
     S.int32(free_count, (1,), "free_count")
     for t in (lengths, tables, free_pages, free_count):

@@ -22,3 +22,9 @@ def test_results_are_not_written_to_expanded_tensors():
         for pair in ((out, x), (x, out)):
             with pytest.raises(ValueError, match="expanded"):
                 sa.qk_norm_rotary(x, x, torch.zeros(6, dtype=torch.int32), None, None, sa.rotary_frequencies(64), out=pair)
+
+
+def test_release_takes_one_list_of_free_pages():
+    i = torch.zeros(1, dtype=torch.int32)
+    with pytest.raises(ValueError, match=r"free_pages must be \[F\]"):
+        sa.release_kv_pages(i, i[:, None], torch.zeros(1, dtype=torch.bool), i[None], i, page_size=16)
