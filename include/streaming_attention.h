@@ -349,11 +349,13 @@ int sa_serving_status(void* stream);
  * are out of order or range is reported and skipped.  Rows of no request, those
  * between a skipped one's offsets too, stay as they were or are zeroed
  * (zero_behind != 0).  d, dv <= 256.
- * Tensor cores: float16 / bfloat16 of d, dv <= 128 on 16-byte borders (few
- * queries over many keys: split over the SMs, given the workspace); dense
+ * Tensor cores: float16 / bfloat16 of d, dv <= 128 on 16-byte borders; dense
  * contiguous float32 (3xTF32) of d <= 64, dv <= 128 and long enough given a workspace of
  * sa_window_attention_workspace_size bytes (256-byte aligned; 0: none is used).
- * CUDA cores otherwise. */
+ * CUDA cores otherwise.  The 16-bit form does without a workspace, but uses one of
+ * that size (packed: that of a dense call of batch 1 with as many queries and keys
+ * as k has rows) to split few queries' many keys over the SMs, and to fold the sums
+ * over more than 32768 keys, which the matrix units would pull towards zero. */
 int sa_window_attention_workspace_size(int batch, int heads, int kv_heads, int64_t n, int64_t m, int d, int dv,
                                        int64_t window, int64_t sinks, int dtype, size_t* bytes);
 int sa_window_attention(const void* q, const void* k, const void* v, void* out, const int64_t* strides, int batch,

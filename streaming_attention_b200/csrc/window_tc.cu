@@ -43,6 +43,11 @@
 // most 2^14, and 2^-14, where float16 starts to lose bits, is 2^-20 of the
 // row's usual largest).
 //
+// The matrix units truncate as they add, so a chain of products pulls O towards
+// zero by up to 7e-8 of it a step of 16 keys: values of mean 1 came out 5.5e-4 low
+// after 131072 keys.  Given a workspace, O goes to a sum in memory every kFold
+// tiles (32768 keys, at most 1.4e-4) and starts from zero again.
+//
 // A product with a hidden key's value is 0 * v, NaN where v is NaN or infinite.
 // Columns that come out non-finite are computed again by the row's warp from the
 // visible keys alone (repair_row): what a query does not see cannot reach it.
@@ -66,6 +71,8 @@ constexpr int kRows = 128;     // rows of a query tile
 constexpr int kCols = 64;      // keys of a key tile
 constexpr int kSeam = 16;      // rows of a box of the seam tile
 constexpr int kThreads = 352;
+constexpr int kFold = 512;     // key tiles of a chain of products, where there is a workspace
+constexpr int kFoldCtas = 148;
 constexpr float kMove = 8.0f;
 
 constexpr int kErrQ = 501, kErrFull = 502, kErrP = 503, kErrS = 504, kErrEmpty = 505, kErrO = 506, kErrDrain = 507,
@@ -81,6 +88,7 @@ struct WindowTcParams {
   int splits;                // parts that a pair's keys are dealt into
   float* part;               // splits > 1: [row][split][pitch], O (not divided), m, l
   int pitch;
+  float* sums;               // kLong: [cta][query tile][dv + 1][row], folded O and the maximum it goes by
   uint64_t wait_ns;
 };
 
@@ -258,6 +266,53 @@ __device__ __noinline__ void scale_row(uint32_t to, int dv, float alpha) {
   tmem_wait_st();
 }
 
+// A row's place in the folded sums: columns kRows apart, behind them the maximum
+// that they go by.  (All from the thread's index: called rarely, it takes no registers elsewhere.)
+__device__ __forceinline__ float* sums_of(float* sums, int dv) {
+  const int warp = threadIdx.x >> 5, t = (warp - 3) >> 2;
+  return sums + ((blockIdx.x * 2 + t) * (dv + 1)) * kRows + (warp & 3) * 32 + (threadIdx.x & 31);
+}
+
+// O of a row, in TMEM, times alpha; then, with `fold`, into its sum, and zero there.
+__device__ __noinline__ void scale_fold_row(uint32_t to, int dv, float alpha, float m, float* sums, bool fold, bool first) {
+  float* at = sums_of(sums, dv);
+  const float before = first || !fold ? -INFINITY : at[dv * kRows];
+  const float f = before == -INFINITY ? 0.0f : ex2(before - m);
+#pragma unroll 1
+  for (int c = 0; c < dv; c += 16) {
+    float o[16];
+    tmem_ld16(to + c, o);
+    tmem_wait_ld();
+    uint32_t os[16];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      o[e] *= alpha;
+      os[e] = fold ? 0u : __float_as_uint(o[e]);
+      if (fold && c + e < dv) at[(c + e) * kRows] = before == -INFINITY ? o[e] : fmaf(f, at[(c + e) * kRows], o[e]);
+    }
+    tmem_st16(to + c, os);
+  }
+  tmem_wait_st();
+  if (fold) at[dv * kRows] = m;
+}
+
+// The sum of a row back to its O in TMEM.
+__device__ __noinline__ void unfold_row(uint32_t to, int dv, float m, float* sums) {
+  const float* at = sums_of(sums, dv);
+  const float before = at[dv * kRows], f = before == -INFINITY ? 0.0f : ex2(before - m);
+#pragma unroll 1
+  for (int c = 0; c < dv; c += 16) {
+    float o[16];
+    tmem_ld16(to + c, o);
+    tmem_wait_ld();
+    uint32_t os[16];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) os[e] = __float_as_uint(c + e < dv ? fmaf(f, at[(c + e) * kRows], o[e]) : 0.0f);
+    tmem_st16(to + c, os);
+  }
+  tmem_wait_st();
+}
+
 template <int DC, int VC>   // 64-column chunks of the head widths
 struct Layout {
   static constexpr uint32_t kQ = DC * kRows * 128;                              // one query tile
@@ -272,7 +327,7 @@ struct Layout {
   static_assert(kBytes <= 227 * 1024, "shared memory");
 };
 
-template <int DT, int DC, int VC>
+template <int DT, int DC, int VC, bool kLong>   // kLong: chains are folded (the code costs the others registers)
 __global__ void __launch_bounds__(kThreads, 1)
 window_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                  const __grid_constant__ CUtensorMap tm_ks, const __grid_constant__ CUtensorMap tm_kw,
@@ -575,7 +630,8 @@ window_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
         }
         const float top = fmaxf(max32(s0), max32(s1)) * c2;
         const bool move = top > m + kMove;
-        if (__any_sync(0xffffffffu, move)) {
+        const bool fold = kLong && done > 0 && (done & (kFold - 1)) == 0;
+        if (__any_sync(0xffffffffu, move) || fold) {
           const float to = move ? top : m;
           const float alpha = move ? ex2(m - to) : 1.0f;   // m = -inf: 0
           m = to;
@@ -589,7 +645,10 @@ window_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
             }
             if (!ok) break;
             tc_fence_after();
-            scale_row(tO[t] + at, a.dv, alpha);
+            if (kLong)
+              scale_fold_row(tO[t] + at, a.dv, alpha, m, p.sums, fold, done == kFold);
+            else
+              scale_row(tO[t] + at, a.dv, alpha);
           }
         }
         const float off = kShift - (m == -INFINITY ? 0.0f : m);
@@ -610,6 +669,7 @@ window_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
       if (!ok) break;
       tc_fence_after();
       const int h0 = c.hk * p.group + c.g0, nq = c.nq;
+      if (kLong && done > kFold) unfold_row(tO[t] + at, a.dv, m, p.sums);
       const int64_t obase = c.b * a.o_b + (int64_t)h0 * a.o_h + c.q_row * a.o_n;
       // 32 columns at a time pass through shared memory, so that neighbouring
       // lanes store neighbouring pieces of a row (16 bytes; the pitch keeps the
@@ -785,7 +845,7 @@ int encode(CUtensorMap* map, bool bf16, const void* base, int rank, const int64_
 
 template <int DT, int DC, int VC>
 int launch_one(const CUtensorMap* maps, const WindowTcParams& p, dim3 grid, cudaStream_t s) {
-  auto kern = window_tc_kernel<DT, DC, VC>;
+  auto kern = p.sums ? window_tc_kernel<DT, DC, VC, true> : window_tc_kernel<DT, DC, VC, false>;
   const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Layout<DC, VC>::kBytes);
   if (e != cudaSuccess) return set_error(SA_ERR_CUDA, "window_tc smem attribute: %s", cudaGetErrorString(e));
   kern<<<grid, kThreads, Layout<DC, VC>::kBytes, s>>>(maps[0], maps[1], maps[2], maps[3], maps[4], maps[5], maps[6], p);
@@ -838,13 +898,11 @@ bool window_tc_takes(const WindowArgs& a) {
 // whole and split: 1 query over 8192 keys 106 and 31 us, over 4096 59 and 26; 256
 // over 4096 82 and 51; 512, in two parts, over 4096 82 and 90 (stays whole), over
 // 8192 151 and 126; over 1024 keys 28 whole and 39.
-int window_tc_splits(const WindowArgs& a) {
+int window_tc_splits(const WindowArgs& a, int64_t tiles) {
   if (a.cu_q) return 1;
   WindowTcParams p{};
   shape_of(a, p);
   const int64_t pairs = ceil_div(a.n, p.rows_per_cta) * a.batch * (a.heads / p.pack);
-  const int64_t rows = std::min<int64_t>(a.n, p.rows_per_cta), span = std::min<int64_t>(a.window, a.m) + rows;
-  const int64_t tiles = ceil_div(std::min<int64_t>(a.m, span + std::min<int64_t>(a.sinks, a.m)), kCols);
   const int64_t splits = std::min<int64_t>(std::min<int64_t>(148 / std::max<int64_t>(pairs, 1), tiles / 4), 32);
   if (splits < 2 || tiles < 48) return 1;
   const double saved = 1.3 * (double)tiles * (double)(splits - 1) / (double)splits;
@@ -852,10 +910,25 @@ int window_tc_splits(const WindowArgs& a) {
   return saved > 15.0 + 0.0009 / 132.0 * part_pitch(a.dv) * parts ? (int)splits : 1;
 }
 
-size_t window_tc_bytes(const WindowArgs& a) {
-  const int splits = window_tc_splits(a);
-  return splits > 1 ? (size_t)a.batch * a.heads * a.n * splits * part_pitch(a.dv) * sizeof(float) : 0;
+// What a call keeps in its workspace: the parts of split keys, then folded sums.
+struct WindowTcSpace {
+  int splits;
+  size_t sums_at, bytes;   // folded sums, where bytes > sums_at
+};
+WindowTcSpace window_tc_space(const WindowArgs& a) {
+  WindowTcParams p{};
+  shape_of(a, p);
+  // the most key tiles of a pair
+  const int64_t rows = std::min<int64_t>(a.n, p.rows_per_cta), span = std::min<int64_t>(a.window, a.m) + rows;
+  const int64_t tiles = ceil_div(std::min<int64_t>(a.m, span + std::min<int64_t>(a.sinks, a.m)), kCols);
+  WindowTcSpace w{window_tc_splits(a, tiles), 0, 0};
+  if (w.splits > 1) w.sums_at = ((size_t)a.batch * a.heads * a.n * w.splits * part_pitch(a.dv) * sizeof(float) + 255) & ~(size_t)255;
+  w.bytes = w.sums_at;
+  if (tiles / w.splits + 2 > kFold) w.bytes += (size_t)kFoldCtas * 2 * (a.dv + 1) * kRows * sizeof(float);
+  return w;
 }
+
+size_t window_tc_bytes(const WindowArgs& a) { return window_tc_space(a).bytes; }
 
 int launch_window_tc(const WindowArgs& a, void* workspace, size_t workspace_bytes, cudaStream_t s) {
   WindowTcParams p{};
@@ -865,9 +938,12 @@ int launch_window_tc(const WindowArgs& a, void* workspace, size_t workspace_byte
               (a.dv & 7) == 0;
   p.wait_ns = wait_limit_ns();
   p.pitch = part_pitch(a.dv);
-  // without a workspace the keys are not split
-  p.splits = workspace && workspace_bytes >= window_tc_bytes(a) ? window_tc_splits(a) : 1;
+  // without a workspace the keys are not split, nor sums folded
+  const WindowTcSpace space = window_tc_space(a);
+  const bool given = workspace && workspace_bytes >= space.bytes;
+  p.splits = given ? space.splits : 1;
   p.part = static_cast<float*>(workspace);
+  p.sums = given && space.bytes > space.sums_at ? reinterpret_cast<float*>(static_cast<char*>(workspace) + space.sums_at) : nullptr;
   const bool bf16 = a.dtype == SA_REP_BFLOAT16;
   const int64_t batch = a.cu_q ? 1 : a.batch;
   CUtensorMap maps[7];   // q; k in boxes of a tile, of the seam's 16 rows and of the rows behind them; v likewise
@@ -892,6 +968,7 @@ int launch_window_tc(const WindowArgs& a, void* workspace, size_t workspace_byte
   cudaError_t e = cudaGetDevice(&dev);
   if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
   if (e != cudaSuccess) return set_error(SA_ERR_CUDA, "window_tc device query: %s", cudaGetErrorString(e));
+  if (p.sums) sms = std::min(sms, kFoldCtas);
   dim3 grid((unsigned)(items < sms ? items : sms));
   rc = bf16 ? launch_dims<SA_REP_BFLOAT16>(maps, p, grid, s) : launch_dims<SA_REP_FLOAT16>(maps, p, grid, s);
   if (rc || p.splits == 1) return rc;

@@ -94,7 +94,8 @@ def sliding_window_attention(q: Tensor, k: Tensor, v: Tensor, *, window: Optiona
     if out.numel():
         _check_heads(heads, kv_heads)
         ws = None
-        if q.dtype == torch.float32 or m > 3008:   # 16 bits: 48 tiles of 64 keys and more may be split
+        # 16 bits: 48 tiles of 64 keys and more may be split, longer chains folded
+        if q.dtype == torch.float32 or m > 3008:
             size = _workspace_size(b, heads, kv_heads, n, m, d, dv, w, s, code)
             if size:
                 ws = torch.empty(size, device=dev, dtype=torch.uint8)
@@ -142,9 +143,13 @@ def sliding_window_attention_packed(q: Tensor, k: Tensor, v: Tensor, cu_q: Tenso
         raise ValueError("out must not be an expanded tensor")
     if out.numel():
         _check_heads(heads, kv_heads)
+        ws, size = None, 0
+        if code != _lib.REP_DTYPES["float32"] and rows > 32000 and (w == 0 or w + s > 31900):   # long chains are folded
+            size = _workspace_size(1, heads, kv_heads, rows, rows, d, dv, w, s, code)
+            ws = torch.empty(size, device=dev, dtype=torch.uint8) if size else None
         q, k, v = _on_borders(q), _on_borders(k), _on_borders(v)
         S.launch(dev, "sa_window_attention", q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
                  S.strides(0, q.stride(1), q.stride(0), 0, k.stride(1), k.stride(0), 0, v.stride(1), v.stride(0), 0,
                            out.stride(1), out.stride(0)), cu_q.shape[0] - 1, heads, kv_heads, t, rows, d, dv, w, s,
-                 _scale(scale, d), code, cu_q.data_ptr(), cu_k.data_ptr(), int(fresh), None, 0)
+                 _scale(scale, d), code, cu_q.data_ptr(), cu_k.data_ptr(), int(fresh), S.ptr(ws), size)
     return out

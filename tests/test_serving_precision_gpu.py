@@ -104,3 +104,40 @@ def test_windowed_attention_keeps_its_precision(n, m, window, spread, dtype, d, 
     own = size * (3.3e-6 if dtype == F32 else R.HALF[dtype])
     err = _rms(out[0].double() - ref)
     assert err <= math.hypot(rounding, own), (err / size, rounding / size, own / size)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=["f16", "bf16"])
+@pytest.mark.parametrize("form,heads,m,dv,window", [("dense", 80, 131072, 64, None), ("dense", 80, 40000, 100, 30000), ("dense", 2, 300000, 64, None),
+                                                   ("packed", 80, 60000, 64, None), ("packed", 3, 34000, 128, None)])
+def test_windowed_attention_of_long_chains_is_not_low(form, heads, m, dv, window, dtype, dev):
+    """Values of mean 1: the mean of the result beside that of the rounded reference
+    (rounding has a mean of its own here: results crowd around 1, where the type's steps
+    change).  The matrix units cut off 7e-8 for each 16 keys of a chain of at most 32768
+    keys, 1.44e-4 in all.  A shift by that moves the rounded values of a share of
+    1.44e-4 / step of the N elements by one step, so its mean is off by
+    sqrt(1.44e-4 step / N) from it: four of those."""
+    g = torch.Generator(dev).manual_seed(m)
+    n, d = 256, 64
+    q = torch.randn(1, heads, n, d, generator=g, device=dev).to(dtype)
+    k, v = torch.empty(1, heads, m, d, dtype=dtype, device=dev), torch.empty(1, heads, m, dv, dtype=dtype, device=dev)
+    for h in range(heads):
+        k[0, h] = torch.randn(m, d, generator=g, device=dev).to(dtype)
+        v[0, h] = (torch.randn(m, dv, generator=g, device=dev) + 1).to(dtype)
+    if form == "dense":
+        out = sa.sliding_window_attention(q, k, v, window=window)
+    else:
+        rows = lambda x: x[0].transpose(0, 1).contiguous()  # noqa: E731
+        cu_q, cu_k = (torch.tensor([0, x], dtype=torch.int32, device=dev) for x in (n, m))
+        out = sa.sliding_window_attention_packed(rows(q), rows(k), rows(v), cu_q, cu_k, window=window).transpose(0, 1)[None]
+    at = torch.arange(m - n, m, device=dev)[:, None]
+    j = torch.arange(m, device=dev)[None]
+    for h in {0, heads - 1}:
+        x = q[0, h].double() @ k[0, h].double().T / math.sqrt(d)
+        x = torch.softmax(x.masked_fill((j > at) | (j <= at - (window or m)), -math.inf), -1)
+        ref = x @ v[0, h].double()
+        rounded = ref.to(dtype).double()
+        low = 1 - (out[0, h].double().mean() / rounded.mean()).item()
+        most = 2048 * 7e-8
+        assert abs(low) <= most + 4 * math.sqrt(most * 2 * R.HALF[dtype] / ref.numel()), low
+        err = _rms(out[0, h].double() - ref)
+        assert err <= math.hypot(_rms(rounded - ref), _rms(ref) * R.HALF[dtype])

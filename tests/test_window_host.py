@@ -13,7 +13,7 @@ CASES = [
     # b, h, hkv, n, m, d, window, split
     (1, 32, 8, 1, 4096, 128, None, True), (1, 32, 8, 128, 4096, 128, None, True), (1, 32, 8, 256, 4096, 128, None, True),
     (1, 32, 8, 512, 4096, 128, None, False), (1, 32, 8, 512, 8192, 128, None, True), (1, 8, 8, 1024, 32768, 64, None, True),
-    (1, 32, 8, 600, 32768, 128, None, False), (1, 32, 8, 1, 3008, 128, None, False), (1, 32, 8, 1, 8192, 128, 1024, False),
+    (1, 32, 8, 600, 16000, 128, None, False), (1, 32, 8, 1, 3008, 128, None, False), (1, 32, 8, 1, 8192, 128, 1024, False),
     (16, 32, 8, 1, 4096, 128, None, False), (1, 8, 8, 2304, 8192, 128, None, True),
 ]
 
