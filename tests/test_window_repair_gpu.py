@@ -229,3 +229,29 @@ def test_a_row_that_sees_nothing_but_nan_is_nan(dtype, d, packed, dev):
         sees = R.visible(300, 300, window, sinks)
         bad = (sees[:, 0] | sees[:, 200]).to(dev)
         assert torch.isnan(out[:, :, bad]).all() and torch.isfinite(out[:, :, ~bad]).all()
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=["f16", "bf16"])
+@pytest.mark.parametrize("h,hkv,n,m,window,sinks", [(80, 80, 130, 40000, None, 0), (80, 80, 130, 40000, 36000, 4), (32, 8, 512, 70000, None, 0)],
+                         ids=["whole", "window", "split"])
+def test_chains_that_are_folded(h, hkv, n, m, window, sinks, dtype, dev):
+    """Over 32768 keys and more: rising scores late in a chain, which all that was
+    folded is scaled down for, and values that are not finite, seen and hidden."""
+    g = torch.Generator(dev).manual_seed(7)
+    q, k, v = _make(g, dev, dtype, 1, h, n, 64), *(_make(g, dev, dtype, 1, hkv, m, 64) for _ in range(2))
+    k[:, :, m - 3000] *= 4
+    k[:, 0, 34000:] += q[:, 0, :1] * 0.5        # the first query's scores rise by 16 there
+    w = v.clone()
+    w[:, :, 20000, 3] = float("inf")
+    w[:, :, m - 1] = float("nan")                # seen by the last query alone
+    if sinks:
+        w[:, :, 6] = float("nan")                # hidden, beside the first tokens
+    for values, cols in ((v, slice(None)), (w, torch.arange(64) != 3)):
+        out = sa.sliding_window_attention(q, k, values, window=window, sinks=sinks)
+        for at in (0, h - 1):
+            y = at // (h // hkv)
+            ref, bound = _bound(q[0, at:at + 1], k[0, y:y + 1], v[0, y:y + 1], window, sinks, 0.125, dtype)
+            rows = slice(0, n if values is v else n - 1)
+            R.assert_close(out[0, at:at + 1, rows][..., cols], ref[:, rows][..., cols], bound[:, rows][..., cols])
+        if values is w:
+            assert torch.isnan(out[:, :, n - 1]).all() and (out[:, :, :n - 1, 3] == float("inf")).all()
