@@ -16,7 +16,7 @@
 //                                                along the token axis that the product P V contracts
 //   k_params, v_params [pages, heads, page, 2]   scale, least
 // 20011 tokens of 8 heads of 128 (bfloat16): the write 68 us (104 MB; bound by the
-// instructions that find the codes, 69 % of the issue slots), the read of the same
+// instructions that find the codes, 72 % of the issue slots), the read of the same
 // to float32 48 us (186 MB, 3.9 TB/s).
 #include <math.h>
 

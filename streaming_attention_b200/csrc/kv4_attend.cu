@@ -31,7 +31,8 @@
 //
 // What bounds it beside the bytes (94 us of 64 requests x 6000..12000 tokens x 8
 // heads, 611 MB) is instructions: 480 a block and 301 us with every code centred,
-// masks in every block and register double buffers; 228 us now (2.7 TB/s).  Float16 operands (five integer operations for eight codes in place of
+// masks in every block and register double buffers; 228 us now (2.7 TB/s; issue slots
+// and integer pipe half busy, tensor pipe a fifth).  Float16 operands (five integer operations for eight codes in place of
 // eight) took 245: their scales cost more than they saved.  Q is
 // bfloat16 as it is, float16 as two and float32 as three bfloat16 pieces (exact,
 // or to 24 bits); p s_v is split into two pieces (16 bits; three for float32).

@@ -11,7 +11,7 @@
 // second launch), then handles a run of new tokens: it finds a token's request
 // by binary search over the sums, and the token that opens a page writes the
 // page's entry of the table.  The first CTA writes what there is one of per
-// request.  24 requests' next tokens: 5.7 us; 1000 prompts of up to 400 tokens: 9.4 us,
+// request.  24 requests' next tokens: 6.2 us; 1000 prompts of up to 400 tokens: 9.4 us,
 // both latency (a round of sums, a search, the table's and the list's loads).
 #include "serving.cuh"
 

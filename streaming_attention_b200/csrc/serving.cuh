@@ -11,7 +11,7 @@
 namespace sa {
 
 // Codes of the error word that name bad contents of device-side index arrays
-// (the kernels skip what they point at); sa_workspace_status reports them as
+// (the kernels skip what they point at); sa_serving_status reports them as
 // SA_ERR_INVALID_ARG.
 constexpr int kBadFirst = 400, kBadLast = 499;
 constexpr int kBadPage = 400;     // a page id outside the cache

@@ -31,7 +31,8 @@
 // since a parity wait must have seen each phase of its barrier before the next
 // ends: scores' commits are all answered by a P, these by a later one); with one S of 128
 // columns each waited for the other (32 heads x 8192 of 128, window 1024: 184 us, and
-// 174 so; 129 GFLOP, 44 % of the measured GEMM rate, bound by that chain).
+// 174 so, back to back; 188 us of a caller's time with cold caches, 129 GFLOP, 41 % of
+// the measured GEMM rate; bound by that chain: tensor pipe and exponentials 40 % each).
 //
 // Where a dense call has few pairs and many keys, a pair's key tiles are dealt
 // into parts that run as items of their own and are joined by join_kernel.

@@ -6,8 +6,10 @@ One object is one layer's attention: ``prefill`` takes the prompts of new
 requests (packed, ragged), ``decode`` the next tokens of the batch.  Both norm
 and rotate queries and keys, make room in the cache, write the new keys and
 values to it and attend: a prompt over its own keys at full precision, a decode
-step over the cache.  Lengths, page tables and the free list live on the device
-at fixed addresses, so ``decode`` can be captured into a CUDA graph.
+step over the cache.  The window bounds the work of a step, not the cache: a
+request keeps the pages of all its tokens until it is released.  Lengths, page
+tables and the free list live on the device at fixed addresses, so ``decode`` can
+be captured into a CUDA graph.
 """
 
 from __future__ import annotations
