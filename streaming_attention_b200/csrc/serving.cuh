@@ -13,7 +13,6 @@ namespace sa {
 // Codes of the error word that name bad contents of device-side index arrays
 // (the kernels skip what they point at); sa_serving_status reports them as
 // SA_ERR_INVALID_ARG.
-constexpr int kBadFirst = 400, kBadLast = 499;
 constexpr int kBadPage = 400;     // a page id outside the cache
 constexpr int kBadSlot = 401;     // a slot outside the cache
 constexpr int kBadLength = 402;   // a request longer than its row of the page table
