@@ -397,6 +397,79 @@ int sa_kv4_attend(const void* k_codes, const void* k_params, const void* v_codes
                   const int32_t* tables, const int32_t* lengths, int requests, int n, int heads, int width,
                   int64_t window, int64_t sinks, float scale, int dtype, void* stream);
 
+/* sa_kv4_attend over listed pages alone: selected [requests, n, kv_heads, count]
+ * holds, for each query token and key head, rows of the request's table in ascending
+ * order; a query sees the tokens up to its own that stand in them.  Entries from the
+ * first -1 on count as none; so do those from the first that is not above the one
+ * before or leaves the table, which is reported.  requests * n < 65536. */
+int sa_kv4_attend_pages(const void* k_codes, const void* k_params, const void* v_codes, const void* v_params, int64_t pages,
+                        int kv_heads, int page_size, int d, const void* q, void* out, const int64_t* strides,
+                        const int32_t* tables, const int32_t* lengths, const int32_t* selected, int count, int requests, int n,
+                        int heads, int width, float scale, int dtype, void* stream);
+
+/* sa_kv4_attend that also adds to weights [pages, kv_heads, page_size] (float32) what
+ * weight each token had: the sum over the n queries and the heads that read key head h
+ * of its softmax weight, at its slot.  The workspace is 256-byte aligned.  No page
+ * stands in the tables of two requests (else both are added, in any order). */
+int sa_kv4_attend_weigh_workspace_size(int kv_heads, int page_size, int requests, int n, int heads, int width, int64_t window,
+                                       int64_t sinks, size_t* bytes);
+int sa_kv4_attend_weigh(const void* k_codes, const void* k_params, const void* v_codes, const void* v_params, int64_t pages,
+                        int kv_heads, int page_size, int d, const void* q, void* out, const int64_t* strides,
+                        const int32_t* tables, const int32_t* lengths, int requests, int n, int heads, int width,
+                        int64_t window, int64_t sinks, float scale, int dtype, float* weights, void* workspace,
+                        size_t workspace_bytes, void* stream);
+
+/* Sets the weights of slots [tokens] to zero, of every head; a negative slot is left out. */
+int sa_kv4_reset_weights(float* weights, int64_t pages, int kv_heads, int page_size, const int32_t* slots, int64_t tokens,
+                         void* stream);
+
+/* sa_kv4_attend of a batch whose requests share a prefix of prefix_length[0] tokens in
+ * pages prefix_table [prefix_width]: request r's tokens are the prefix's and behind
+ * them its own lengths[r] in tables[r, 0..].  Query i of n is own token lengths[r] - n +
+ * i (zeros where there is none) and stands at prefix_length[0] + lengths[r] - n + i; window
+ * and sinks count over both.  The prefix is read once for all requests.  The workspace
+ * is 256-byte aligned; requests * n * heads <= 400000. */
+int sa_kv4_attend_shared_workspace_size(int kv_heads, int page_size, int d, int requests, int n, int heads, int prefix_width,
+                                        int64_t window, int64_t sinks, int dtype, size_t* bytes);
+int sa_kv4_attend_shared(const void* k_codes, const void* k_params, const void* v_codes, const void* v_params, int64_t pages,
+                         int kv_heads, int page_size, int d, const void* q, void* out, const int64_t* strides,
+                         const int32_t* prefix_table, const int32_t* prefix_length, int prefix_width, const int32_t* tables,
+                         const int32_t* lengths, int requests, int n, int heads, int width, int64_t window, int64_t sinks,
+                         float scale, int dtype, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Bounds of the keys of the pages that the newest fresh[r] tokens of each request
+ * stand in: bounds bfloat16 [pages, kv_heads, 2, dp], 16-byte aligned: the least and the
+ * largest value of each column over the tokens that the page holds (NaN where one is),
+ * rounded to nearest; columns behind d are 0.  Other pages' bounds stay. */
+int sa_kv4_page_bounds(const void* k_codes, const void* k_params, const void* v_codes, const void* v_params, int64_t pages,
+                       int kv_heads, int page_size, int d, void* bounds, const int32_t* tables, const int32_t* lengths,
+                       const int32_t* fresh, int requests, int width, void* stream);
+
+/* For each query token and key head the `count` pages of its request it should read:
+ * selected [requests, n, kv_heads, count], rows of the table in ascending order, -1
+ * behind.  Of the pages up to the query's own: the first `first`, the last `last`, and
+ * between them those of the largest score (of equal ones the lowest),
+ *   score = sum over the heads that read the key head, over columns c, of max(q_c low_c, q_c high_c),
+ * summed in float64; a score that is NaN is the largest.  first + last <= count,
+ * width <= 24576. */
+int sa_kv4_select_pages(const void* bounds, int64_t pages, int kv_heads, int page_size, int d, const void* q,
+                        const int64_t* strides, const int32_t* tables, const int32_t* lengths, int requests, int n, int heads,
+                        int width, int count, int first, int last, int dtype, int32_t* selected, void* stream);
+
+/* Evicts tokens of the requests of more than `limit` tokens: of each key head the first
+ * `first` and the newest `last` stay and, between, those of the largest weights
+ * [pages, kv_heads, page_size] (of equal ones the lowest; NaN counts as the largest),
+ * `keep` in all.  They move up, in order and with their weights, to the request's first
+ * places, in place; weights behind become zero, lengths[r] becomes keep, and the pages behind go to the end
+ * of the free list.  kept [requests, kv_heads, keep]: which tokens stayed (of other
+ * requests 0, 1, .. and -1 behind the last); dropped [requests]: how many did not.
+ * 1 <= keep <= limit, first + last <= keep, requests <= 16384.  No page stands in two
+ * requests' tables. */
+int sa_kv4_evict(void* k_codes, void* k_params, void* v_codes, void* v_params, int64_t pages, int kv_heads, int page_size,
+                 int d, float* weights, int32_t* lengths, int32_t* tables, int32_t* free_pages, int32_t* free_count,
+                 int requests, int width, int free_size, int keep, int limit, int first, int last, int32_t* kept,
+                 int32_t* dropped, void* stream);
+
 /* Room for fresh[r] (>= 0) new tokens of each of `requests` requests (at most
  * 16384): pages are taken in request order from the end of the free_count[0]
  * entries of free_pages and entered in tables [requests, width] (in place;

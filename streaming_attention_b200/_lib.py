@@ -80,6 +80,21 @@ SIGNATURES = {
     "sa_kv4_read": [_vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _vp, _vp, _vp, _i64, _i32, _vp],
     "sa_kv4_attend": [_vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32,
                       _i64, _i64, _f32, _i32, _vp],
+    "sa_kv4_attend_pages": [_vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32,
+                            _i32, _i32, _f32, _i32, _vp],
+    "sa_kv4_attend_weigh_workspace_size": [_i32, _i32, _i32, _i32, _i32, _i32, _i64, _i64, ctypes.POINTER(_sz)],
+    "sa_kv4_attend_weigh": [_vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32,
+                            _i64, _i64, _f32, _i32, _vp, _vp, _sz, _vp],
+    "sa_kv4_reset_weights": [_vp, _i64, _i32, _i32, _vp, _i64, _vp],
+    "sa_kv4_attend_shared_workspace_size": [_i32, _i32, _i32, _i32, _i32, _i32, _i32, _i64, _i64, _i32,
+                                            ctypes.POINTER(_sz)],
+    "sa_kv4_attend_shared": [_vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _i32, _vp, _vp, _i32,
+                             _i32, _i32, _i32, _i64, _i64, _f32, _i32, _vp, _sz, _vp],
+    "sa_kv4_page_bounds": [_vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _i32, _i32, _vp],
+    "sa_kv4_select_pages": [_vp, _i64, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _i32,
+                            _i32, _vp, _vp],
+    "sa_kv4_evict": [_vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32,
+                     _i32, _i32, _vp, _vp, _vp],
     "sa_plan_kv_pages": [_vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _vp],
     "sa_plan_kv_prompts": [_vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _vp],
     "sa_release_kv_pages": [_vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _vp],

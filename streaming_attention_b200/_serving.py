@@ -75,7 +75,7 @@ def ptr(t: Optional[Tensor]) -> Optional[int]:
     return None if t is None else t.data_ptr()
 
 
-def _whole(x, what: str) -> int:
+def whole(x, what: str) -> int:
     if type(x) is int:
         return x
     try:
@@ -90,14 +90,23 @@ def _whole(x, what: str) -> int:
 def check_window(window: Optional[int], sinks: int) -> Tuple[int, int]:
     """Window (0: without end) and first tokens as the C ABI takes them; what lies
     beyond every position (2^31) hides and shows no more than that does."""
-    w, s = 0, _whole(sinks, "sinks")
+    w, s = 0, whole(sinks, "sinks")
     if window is not None:
-        w = _whole(window, "window")
+        w = whole(window, "window")
         if w <= 0:
             raise ValueError("window must be positive, or None for no end")
     if s < 0:
         raise ValueError("sinks must be non-negative")
     return min(w, 1 << 40), min(s, 1 << 40)
+
+
+def workspace(dev: torch.device, name: str, *sizes: int) -> Tensor:
+    """Device memory of the size that the entry point `name` asks for."""
+    nbytes = ctypes.c_size_t(0)
+    rc = getattr(_lib.load(), name)(*sizes, ctypes.byref(nbytes))
+    if rc:
+        _lib.check(rc, name)
+    return torch.empty(nbytes.value, device=dev, dtype=torch.uint8)
 
 
 def _raw_stream(index: int) -> int:

@@ -21,6 +21,9 @@ int launch_plan_pages(const int32_t* lengths, const int32_t* fresh, int32_t* tab
 int launch_release_pages(int32_t* lengths, int32_t* tables, const uint8_t* drop, int32_t* free_pages,
                          int32_t* free_count, int requests, int width, int free_size, int page_shift, int* status,
                          cudaStream_t s);
+int launch_shrink_requests(int32_t* lengths, int32_t* tables, int32_t* free_pages, int32_t* free_count, int32_t* dropped,
+                           int requests, int width, int free_size, int page_shift, int keep, int limit, int* status,
+                           cudaStream_t s);
 int launch_rotary(const void* q, const void* k, void* q_out, void* k_out, const int32_t* positions,
                   const void* q_weight, const void* k_weight, const double* frequencies, const int64_t* strides,
                   int64_t tokens, int heads, int kv_heads, int d, int half, float eps, int interleaved,
@@ -75,6 +78,13 @@ int page_shift_of(int page_size) {
   return -1;
 }
 
+// A head width filled up to 32, 64, 128 or 256.
+int padded_dim(int d) {
+  int dp = 32;
+  while (dp < d) dp *= 2;
+  return dp;
+}
+
 int check_cache(Kv4Cache* c, const void* k_codes, const void* k_params, const void* v_codes, const void* v_params,
                 int64_t pages, int heads, int page_size, int d) {
   if (pages <= 0 || heads <= 0) return set_error(SA_ERR_INVALID_ARG, "the cache needs at least one page and one head");
@@ -85,10 +95,79 @@ int check_cache(Kv4Cache* c, const void* k_codes, const void* k_params, const vo
   if (!k_codes || !k_params || !v_codes || !v_params) return set_error(SA_ERR_INVALID_ARG, "null cache pointer");
   if (((uintptr_t)k_codes | (uintptr_t)k_params | (uintptr_t)v_codes | (uintptr_t)v_params) & 15)
     return set_error(SA_ERR_INVALID_ARG, "the cache's tensors must be 16-byte aligned");
-  int dp = 32;
-  while (dp < d) dp *= 2;
   *c = Kv4Cache{(uint8_t*)k_codes, (__nv_bfloat16*)k_params, (uint8_t*)v_codes, (__nv_bfloat16*)v_params,
-                pages, heads, d, dp, shift};
+                pages, heads, d, padded_dim(d), shift};
+  return SA_OK;
+}
+
+int check_tables(int requests, int width, int page_shift) {
+  if (requests < 0 || width < 0) return set_error(SA_ERR_INVALID_ARG, "sizes must be non-negative");
+  if (requests > 65535) return set_error(SA_ERR_UNSUPPORTED, "more than 65535 requests in one call");
+  if (((int64_t)width << page_shift) > 2147483647LL)
+    return set_error(SA_ERR_UNSUPPORTED, "a row of the page table covers 2^31 tokens or more");
+  return SA_OK;
+}
+
+// The sizes of an attention over the cache.
+int attend_sizes(Kv4AttendArgs* a, int kv_heads, int page_size, int requests, int n, int heads, int width, int64_t window,
+                 int64_t sinks) {
+  int rc = check_heads(heads, kv_heads);
+  if (rc) return rc;
+  const int shift = page_shift_of(page_size);
+  if (shift < 0) return set_error(SA_ERR_INVALID_ARG, "page_size must be 16, 32, 64, 128 or 256");
+  if (requests < 0 || n < 0 || width < 0) return set_error(SA_ERR_INVALID_ARG, "sizes must be non-negative");
+  if (window < 0 || sinks < 0) return set_error(SA_ERR_INVALID_ARG, "window and sinks must be non-negative");
+  if ((int64_t)n * heads > 65535) return set_error(SA_ERR_UNSUPPORTED, "more than 65535 query rows per request");
+  rc = check_tables(requests, width, shift);
+  if (rc) return rc;
+  a->c.heads = kv_heads;
+  a->c.page_shift = shift;
+  a->requests = requests;
+  a->n = n;
+  a->heads = heads;
+  a->width = width;
+  a->window = window_of(window);
+  a->sinks = sinks_of(sinks);
+  return SA_OK;
+}
+
+int attend_args(Kv4AttendArgs* a, const void* k_codes, const void* k_params, const void* v_codes, const void* v_params,
+                int64_t pages, int kv_heads, int page_size, int d, const void* q, void* out, const int64_t* strides,
+                const int32_t* tables, const int32_t* lengths, int requests, int n, int heads, int width, int64_t window,
+                int64_t sinks, float scale, int dtype) {
+  int rc = check_dtype(dtype);
+  if (!rc) rc = check_cache(&a->c, k_codes, k_params, v_codes, v_params, pages, kv_heads, page_size, d);
+  if (!rc) rc = attend_sizes(a, kv_heads, page_size, requests, n, heads, width, window, sinks);
+  if (rc || requests == 0 || n == 0) return rc;
+  if (!q || !out || !strides || !lengths || (width > 0 && !tables)) return set_error(SA_ERR_INVALID_ARG, "null pointer");
+  a->q = q;
+  a->out = out;
+  a->q_r = strides[0];
+  a->q_n = strides[1];
+  a->q_h = strides[2];
+  a->tables = tables;
+  a->lengths = lengths;
+  a->scale = scale;
+  a->dtype = dtype;
+  a->status = status_word();
+  return SA_OK;
+}
+
+// The prefix's table, and the rows of all requests over it.
+int prefix_sizes(Kv4AttendArgs* a, int prefix_width) {
+  if (prefix_width < 0) return set_error(SA_ERR_INVALID_ARG, "sizes must be non-negative");
+  if (((int64_t)prefix_width << a->c.page_shift) > 2147483647LL)
+    return set_error(SA_ERR_UNSUPPORTED, "the prefix's table covers 2^31 tokens or more");
+  if ((int64_t)a->requests * a->n * a->heads > 400000)
+    return set_error(SA_ERR_UNSUPPORTED, "more than 400000 query rows over one prefix");
+  a->prefix_width = prefix_width;
+  return SA_OK;
+}
+
+int check_workspace(const void* workspace, size_t have, size_t want) {
+  if (want == 0) return SA_OK;
+  if (!workspace || have < want) return set_error(SA_ERR_WORKSPACE, "the workspace has %zu bytes, %zu are needed", have, want);
+  if ((uintptr_t)workspace & 255) return set_error(SA_ERR_WORKSPACE, "the workspace must be 256-byte aligned");
   return SA_OK;
 }
 
@@ -142,6 +221,8 @@ int sa_serving_status(void* stream) {
     case kBadOffsets: return set_error(SA_ERR_INVALID_ARG, "the offsets of request %lld are out of order or out of range", at);
     case kNoPages: return set_error(SA_ERR_INVALID_ARG, "%lld pages wanted, more than are free", at);
     case kHeld: return set_error(SA_ERR_INVALID_ARG, "request %lld holds tokens already, which its prompt does not see", at);
+    case kBadList: return set_error(SA_ERR_INVALID_ARG, "entry %lld of a list of pages is not above the one before, or leaves the table", at);
+    case kBadPrefix: return set_error(SA_ERR_INVALID_ARG, "the prefix is longer than its table (request %lld asked first)", at);
     case kNoRows: return set_error(SA_ERR_INVALID_ARG, "%lld entries, more than the output holds", at);
     default: break;
   }
@@ -297,35 +378,193 @@ int sa_kv4_attend(const void* k_codes, const void* k_params, const void* v_codes
                   const int32_t* tables, const int32_t* lengths, int requests, int n, int heads, int width,
                   int64_t window, int64_t sinks, float scale, int dtype, void* stream) {
   Kv4AttendArgs a{};
+  const int rc = attend_args(&a, k_codes, k_params, v_codes, v_params, pages, kv_heads, page_size, d, q, out, strides,
+                             tables, lengths, requests, n, heads, width, window, sinks, scale, dtype);
+  if (rc || requests == 0 || n == 0) return rc;
+  return launch_kv4_attend(a, (cudaStream_t)stream);
+}
+
+int sa_kv4_attend_pages(const void* k_codes, const void* k_params, const void* v_codes, const void* v_params, int64_t pages,
+                        int kv_heads, int page_size, int d, const void* q, void* out, const int64_t* strides,
+                        const int32_t* tables, const int32_t* lengths, const int32_t* selected, int count, int requests, int n,
+                        int heads, int width, float scale, int dtype, void* stream) {
+  Kv4AttendArgs a{};
+  const int rc = attend_args(&a, k_codes, k_params, v_codes, v_params, pages, kv_heads, page_size, d, q, out, strides,
+                             tables, lengths, requests, n, heads, width, 0, 0, scale, dtype);
+  if (rc) return rc;
+  if (count < 0) return set_error(SA_ERR_INVALID_ARG, "sizes must be non-negative");
+  if ((int64_t)requests * n > 65535) return set_error(SA_ERR_UNSUPPORTED, "more than 65535 queries in one call");
+  if (requests == 0 || n == 0) return SA_OK;
+  if (count > 0 && !selected) return set_error(SA_ERR_INVALID_ARG, "null pointer");
+  a.pages = selected;
+  a.count = count;
+  return launch_kv4_attend_pages(a, (cudaStream_t)stream);
+}
+
+int sa_kv4_attend_weigh_workspace_size(int kv_heads, int page_size, int requests, int n, int heads, int width, int64_t window,
+                                       int64_t sinks, size_t* bytes) {
+  if (!bytes) return set_error(SA_ERR_INVALID_ARG, "null output pointer");
+  Kv4AttendArgs a{};
+  const int rc = attend_sizes(&a, kv_heads, page_size, requests, n, heads, width, window, sinks);
+  if (rc) return rc;
+  *bytes = kv4_weigh_bytes(a);
+  return SA_OK;
+}
+
+int sa_kv4_attend_weigh(const void* k_codes, const void* k_params, const void* v_codes, const void* v_params, int64_t pages,
+                        int kv_heads, int page_size, int d, const void* q, void* out, const int64_t* strides,
+                        const int32_t* tables, const int32_t* lengths, int requests, int n, int heads, int width,
+                        int64_t window, int64_t sinks, float scale, int dtype, float* weights, void* workspace,
+                        size_t workspace_bytes, void* stream) {
+  Kv4AttendArgs a{};
+  const int rc = attend_args(&a, k_codes, k_params, v_codes, v_params, pages, kv_heads, page_size, d, q, out, strides,
+                             tables, lengths, requests, n, heads, width, window, sinks, scale, dtype);
+  if (rc || requests == 0 || n == 0) return rc;
+  if (!weights) return set_error(SA_ERR_INVALID_ARG, "null pointer");
+  const int bad = check_workspace(workspace, workspace_bytes, kv4_weigh_bytes(a));
+  if (bad) return bad;
+  a.weights = weights;
+  return launch_kv4_attend_weigh(a, workspace, (cudaStream_t)stream);
+}
+
+int sa_kv4_reset_weights(float* weights, int64_t pages, int kv_heads, int page_size, const int32_t* slots, int64_t tokens,
+                         void* stream) {
+  const int shift = page_shift_of(page_size);
+  if (shift < 0) return set_error(SA_ERR_INVALID_ARG, "page_size must be 16, 32, 64, 128 or 256");
+  if (pages <= 0 || kv_heads <= 0) return set_error(SA_ERR_INVALID_ARG, "the cache needs at least one page and one head");
+  if (tokens < 0) return set_error(SA_ERR_INVALID_ARG, "tokens must be non-negative");
+  if (tokens == 0) return SA_OK;
+  if (!weights || !slots) return set_error(SA_ERR_INVALID_ARG, "null pointer");
+  return launch_kv4_reset_weights(weights, slots, tokens, pages, kv_heads, shift, status_word(), (cudaStream_t)stream);
+}
+
+int sa_kv4_attend_shared_workspace_size(int kv_heads, int page_size, int d, int requests, int n, int heads, int prefix_width,
+                                        int64_t window, int64_t sinks, int dtype, size_t* bytes) {
+  if (!bytes) return set_error(SA_ERR_INVALID_ARG, "null output pointer");
+  Kv4AttendArgs a{};
   int rc = check_dtype(dtype);
-  if (!rc) rc = check_cache(&a.c, k_codes, k_params, v_codes, v_params, pages, kv_heads, page_size, d);
+  if (!rc) rc = attend_sizes(&a, kv_heads, page_size, requests, n, heads, 0, window, sinks);
+  if (!rc) rc = prefix_sizes(&a, prefix_width);
+  if (rc) return rc;
+  if (d <= 0 || d > SA_MAX_DIM) return set_error(SA_ERR_INVALID_ARG, "the cache's head width must lie in [1, %d]", SA_MAX_DIM);
+  a.c.dp = padded_dim(d);
+  a.dtype = dtype;
+  *bytes = kv4_shared_bytes(a);
+  return SA_OK;
+}
+
+int sa_kv4_attend_shared(const void* k_codes, const void* k_params, const void* v_codes, const void* v_params, int64_t pages,
+                         int kv_heads, int page_size, int d, const void* q, void* out, const int64_t* strides,
+                         const int32_t* prefix_table, const int32_t* prefix_length, int prefix_width, const int32_t* tables,
+                         const int32_t* lengths, int requests, int n, int heads, int width, int64_t window, int64_t sinks,
+                         float scale, int dtype, void* workspace, size_t workspace_bytes, void* stream) {
+  Kv4AttendArgs a{};
+  int rc = attend_args(&a, k_codes, k_params, v_codes, v_params, pages, kv_heads, page_size, d, q, out, strides, tables,
+                       lengths, requests, n, heads, width, window, sinks, scale, dtype);
+  if (!rc) rc = prefix_sizes(&a, prefix_width);
+  if (rc || requests == 0 || n == 0) return rc;
+  if (!prefix_length || (prefix_width > 0 && !prefix_table)) return set_error(SA_ERR_INVALID_ARG, "null pointer");
+  rc = check_workspace(workspace, workspace_bytes, kv4_shared_bytes(a));
+  if (rc) return rc;
+  a.prefix_table = prefix_table;
+  a.prefix_length = prefix_length;
+  return launch_kv4_attend_shared(a, workspace, (cudaStream_t)stream);
+}
+
+int sa_kv4_page_bounds(const void* k_codes, const void* k_params, const void* v_codes, const void* v_params, int64_t pages,
+                       int kv_heads, int page_size, int d, void* bounds, const int32_t* tables, const int32_t* lengths,
+                       const int32_t* fresh, int requests, int width, void* stream) {
+  Kv4BoundsArgs a{};
+  int rc = check_cache(&a.c, k_codes, k_params, v_codes, v_params, pages, kv_heads, page_size, d);
+  if (!rc) rc = check_tables(requests, width, a.c.page_shift);
+  if (rc || requests == 0 || width == 0) return rc;
+  if (!bounds || !tables || !lengths || !fresh) return set_error(SA_ERR_INVALID_ARG, "null pointer");
+  if ((uintptr_t)bounds & 15) return set_error(SA_ERR_INVALID_ARG, "the bounds must be 16-byte aligned");
+  a.bounds = static_cast<__nv_bfloat16*>(bounds);
+  a.tables = tables;
+  a.lengths = lengths;
+  a.fresh = fresh;
+  a.requests = requests;
+  a.width = width;
+  a.status = status_word();
+  return launch_kv4_bounds(a, (cudaStream_t)stream);
+}
+
+int sa_kv4_select_pages(const void* bounds, int64_t pages, int kv_heads, int page_size, int d, const void* q,
+                        const int64_t* strides, const int32_t* tables, const int32_t* lengths, int requests, int n, int heads,
+                        int width, int count, int first, int last, int dtype, int32_t* selected, void* stream) {
+  Kv4SelectArgs a{};
+  int rc = check_dtype(dtype);
   if (!rc) rc = check_heads(heads, kv_heads);
   if (rc) return rc;
-  if (requests < 0 || n < 0 || width < 0) return set_error(SA_ERR_INVALID_ARG, "sizes must be non-negative");
-  if (window < 0 || sinks < 0) return set_error(SA_ERR_INVALID_ARG, "window and sinks must be non-negative");
-  if (requests > 65535) return set_error(SA_ERR_UNSUPPORTED, "more than 65535 requests in one call");
-  if ((int64_t)n * heads > 65535) return set_error(SA_ERR_UNSUPPORTED, "more than 65535 query rows per request");
-  if (((int64_t)width << a.c.page_shift) > 2147483647LL)
-    return set_error(SA_ERR_UNSUPPORTED, "a row of the page table covers 2^31 tokens or more");
-  if (requests == 0 || n == 0) return SA_OK;
-  if (!q || !out || !strides || !lengths || (width > 0 && !tables)) return set_error(SA_ERR_INVALID_ARG, "null pointer");
+  const int shift = page_shift_of(page_size);
+  if (shift < 0) return set_error(SA_ERR_INVALID_ARG, "page_size must be 16, 32, 64, 128 or 256");
+  if (pages <= 0) return set_error(SA_ERR_INVALID_ARG, "the cache needs at least one page and one head");
+  if (d <= 0 || d > SA_MAX_DIM) return set_error(SA_ERR_INVALID_ARG, "the cache's head width must lie in [1, %d]", SA_MAX_DIM);
+  if (n < 0 || count < 0) return set_error(SA_ERR_INVALID_ARG, "sizes must be non-negative");
+  if (first < 0 || last < 0 || (int64_t)first + last > count)
+    return set_error(SA_ERR_INVALID_ARG, "first and last must be non-negative, and no more than count together");
+  rc = check_tables(requests, width, shift);
+  if (rc) return rc;
+  if (width > kSelectMaxPages)
+    return set_error(SA_ERR_UNSUPPORTED, "a row of the page table has more than %d pages to select from", kSelectMaxPages);
+  if (requests == 0 || n == 0 || count == 0) return SA_OK;
+  if (!bounds || !q || !strides || !lengths || !selected || (width > 0 && !tables)) return set_error(SA_ERR_INVALID_ARG, "null pointer");
+  if ((uintptr_t)bounds & 15) return set_error(SA_ERR_INVALID_ARG, "the bounds must be 16-byte aligned");
+  a.c.pages = pages;
+  a.c.heads = kv_heads;
+  a.c.d = d;
+  a.c.dp = padded_dim(d);
+  a.c.page_shift = shift;
+  a.bounds = static_cast<const __nv_bfloat16*>(bounds);
   a.q = q;
-  a.out = out;
   a.q_r = strides[0];
   a.q_n = strides[1];
   a.q_h = strides[2];
   a.tables = tables;
   a.lengths = lengths;
+  a.out = selected;
   a.requests = requests;
   a.n = n;
   a.heads = heads;
   a.width = width;
-  a.window = window_of(window);
-  a.sinks = sinks_of(sinks);
-  a.scale = scale;
-  a.dtype = dtype;
+  a.count = count;
+  a.first = first;
+  a.last = last;
   a.status = status_word();
-  return launch_kv4_attend(a, (cudaStream_t)stream);
+  return launch_kv4_select(a, dtype, (cudaStream_t)stream);
+}
+
+int sa_kv4_evict(void* k_codes, void* k_params, void* v_codes, void* v_params, int64_t pages, int kv_heads, int page_size,
+                 int d, float* weights, int32_t* lengths, int32_t* tables, int32_t* free_pages, int32_t* free_count,
+                 int requests, int width, int free_size, int keep, int limit, int first, int last, int32_t* kept,
+                 int32_t* dropped, void* stream) {
+  Kv4EvictArgs a{};
+  int rc = check_cache(&a.c, k_codes, k_params, v_codes, v_params, pages, kv_heads, page_size, d);
+  if (!rc) rc = check_tables(requests, width, a.c.page_shift);
+  if (rc) return rc;
+  if (free_size < 0) return set_error(SA_ERR_INVALID_ARG, "sizes must be non-negative");
+  if (keep < 1 || limit < keep) return set_error(SA_ERR_INVALID_ARG, "keep must be positive, and limit no less");
+  if (first < 0 || last < 0 || (int64_t)first + last > keep)
+    return set_error(SA_ERR_INVALID_ARG, "first and last must be non-negative, and no more than keep together");
+  if (requests == 0) return SA_OK;
+  if (!weights || !lengths || !free_count || !kept || !dropped || (width > 0 && !tables) || (free_size > 0 && !free_pages))
+    return set_error(SA_ERR_INVALID_ARG, "null pointer");
+  a.weights = weights;
+  a.lengths = lengths;
+  a.tables = tables;
+  a.kept = kept;
+  a.requests = requests;
+  a.width = width;
+  a.keep = keep;
+  a.limit = limit;
+  a.first = first;
+  a.last = last;
+  a.status = status_word();
+  rc = launch_kv4_evict(a, (cudaStream_t)stream);
+  if (rc) return rc;
+  return launch_shrink_requests(lengths, tables, free_pages, free_count, dropped, requests, width, free_size,
+                                a.c.page_shift, keep, limit, a.status, (cudaStream_t)stream);
 }
 
 }  // extern "C"

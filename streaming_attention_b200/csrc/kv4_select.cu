@@ -1,0 +1,296 @@
+// Which pages of a long request a query reads: bounds of each page's keys, a score of
+// every page from them, and the pages of the largest scores.
+//
+// Bounds of a page (of one key head): the least and the largest value of each column
+// over the tokens it holds, in bfloat16, [pages, heads, 2, dp] (columns behind d: 0).
+//
+// Score of page w for the group of query heads that reads key head h:
+//   score_w = sum over heads, columns of max(q_c low_c, q_c high_c)
+//           = sum_c up_c high_c + down_c low_c,  up = sum of the heads' max(q, 0), down of min(q, 0),
+// no less than the sum of the heads' scores of any token of the page (but for the
+// bounds' rounding), at the price of one product of 2 d terms for the whole group.
+// The sums are float64: which pages are chosen does not depend on the order of adding.
+#include <cooperative_groups.h>
+#include <math.h>
+
+#include <algorithm>
+
+#include "kv4.cuh"
+
+namespace sa {
+
+namespace {
+
+namespace cg = cooperative_groups;
+
+constexpr int kThreads = 256;
+constexpr int kWarps = kThreads / 32;
+
+// Minimum and maximum that keep NaN.
+__device__ __forceinline__ float least_of(float x, float y) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ float most_of(float x, float y) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(y));
+  return r;
+}
+
+// A warp per (touched page, head): a lane holds eight columns (a word of codes) of
+// every (32 / words of a row)-th token.
+__global__ void __launch_bounds__(kThreads) bounds_kernel(const Kv4BoundsArgs a) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int r = blockIdx.y;
+  const int cap = a.width << a.c.page_shift;
+  const int whole = max(a.lengths[r], 0), length = min(whole, cap);
+  if (whole > cap && blockIdx.x == 0 && threadIdx.x == 0) report(a.status, kBadLength, r);
+  const int from = whole - min(max(a.fresh[r], 0), whole);   // tokens [from, length) are new
+  if (from >= length) return;
+  const int first = from >> a.c.page_shift, last = (length - 1) >> a.c.page_shift;
+  const int words = a.c.dp >> 3, word = lane & (words - 1), sub = lane / words, step = 32 / words;
+  const int64_t units = (int64_t)(last - first + 1) * a.c.heads;
+  for (int64_t u = (int64_t)blockIdx.x * kWarps + warp; u < units; u += (int64_t)gridDim.x * kWarps) {
+    const int row = first + (int)(u / a.c.heads), h = (int)(u % a.c.heads);
+    const int page = a.tables[(int64_t)r * a.width + row];
+    if (page < 0 || page >= a.c.pages) {
+      if (h == 0 && lane == 0) report(a.status, kBadPage, page);
+      continue;
+    }
+    const int held = min(length - (row << a.c.page_shift), 1 << a.c.page_shift);
+    const int64_t cell = (page * (int64_t)a.c.heads + h) << a.c.page_shift;
+    const uint32_t* codes = reinterpret_cast<const uint32_t*>(a.c.k_codes + cell * (a.c.dp >> 1)) + word;
+    const uint32_t* params = reinterpret_cast<const uint32_t*>(a.c.k_params + 2 * cell);
+    float low[8], high[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) low[e] = INFINITY, high[e] = -INFINITY;
+#pragma unroll 4
+    for (int t = sub; t < held; t += step) {
+      const uint32_t w = codes[(int64_t)t * words], p = params[t];
+      const float scale = __uint_as_float(p << 16), least = __uint_as_float(p & 0xffff0000u);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float x = fmaf((float)((w >> (4 * e)) & 15u), scale, least);
+        low[e] = least_of(low[e], x);
+        high[e] = most_of(high[e], x);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      for (int d = words; d < 32; d *= 2) {
+        low[e] = least_of(low[e], __shfl_xor_sync(0xffffffffu, low[e], d));
+        high[e] = most_of(high[e], __shfl_xor_sync(0xffffffffu, high[e], d));
+      }
+    if (sub == 0) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (word * 8 + e >= a.c.d) low[e] = high[e] = 0.0f;
+      __nv_bfloat16* to = a.bounds + (page * (int64_t)a.c.heads + h) * 2 * a.c.dp + word * 8;
+      store8(to, low);
+      store8(to + a.c.dp, high);
+    }
+  }
+}
+
+// A score as a whole number of the same order; NaN is the largest.
+__device__ __forceinline__ uint64_t order_of(double x) {
+  if (x != x) return ~0ull;
+  const uint64_t b = (uint64_t)__double_as_longlong(x + 0.0);   // -0 becomes 0
+  return b >> 63 ? ~b : b | (1ull << 63);
+}
+
+// A cluster of CTAs scores the pages of one (query token, key head); its first CTA
+// then picks the largest scores by their digits and writes them in ascending order.
+template <int DT, int DP>
+__global__ void __launch_bounds__(kThreads) select_kernel(const Kv4SelectArgs a) {
+  using T = typename Elem<DT>::T;
+  constexpr int kCols = DP / 32;   // columns of a lane
+  extern __shared__ __align__(16) uint64_t keys[];   // [width]: of the pages between first and last
+  __shared__ double up[DP], down[DP];
+  __shared__ int count_of[256];
+  __shared__ int part[2][kWarps];
+  __shared__ int digit, below;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int hk = blockIdx.y, r = blockIdx.z / a.n, i = blockIdx.z % a.n;
+  const int group = a.heads / a.c.heads;
+  const int cap = a.width << a.c.page_shift;
+  const int whole = max(a.lengths[r], 0);
+  if (whole > cap && tid == 0) report(a.status, kBadLength, r);
+  const int length = min(whole, cap) - (a.n - 1 - i);   // up to this query
+  const int pages = length > 0 ? (length + (1 << a.c.page_shift) - 1) >> a.c.page_shift : 0;
+  int32_t* out = a.out + ((int64_t)blockIdx.z * a.c.heads + hk) * a.count;
+  if (pages <= a.count) {   // all of them
+    if (blockIdx.x == 0)
+      for (int e = tid; e < a.count; e += kThreads) out[e] = e < pages ? e : -1;
+    return;
+  }
+  const int middle = pages - a.first - a.last, want = a.count - a.first - a.last;
+  cg::cluster_group cluster = cg::this_cluster();
+  if (want > 0) {
+    for (int c = tid; c < DP; c += kThreads) {
+      double x = 0.0, y = 0.0;
+      if (c < a.c.d)
+        for (int e = 0; e < group; ++e) {
+          const double q = to_f32(static_cast<const T*>(a.q)[r * a.q_r + i * a.q_n + (int64_t)(hk * group + e) * a.q_h + c]);
+          x += q > 0.0 || q != q ? q : 0.0;
+          y += q < 0.0 ? q : 0.0;
+        }
+      up[c] = x;
+      down[c] = y;
+    }
+    __syncthreads();
+    double u[kCols], d[kCols];
+#pragma unroll
+    for (int e = 0; e < kCols; ++e) {
+      u[e] = up[lane * kCols + e];
+      d[e] = down[lane * kCols + e];
+    }
+    uint64_t* to = gridDim.x > 1 ? cluster.map_shared_rank(keys, 0) : keys;
+    const int32_t* table = a.tables + (int64_t)r * a.width + a.first;
+    for (int w = blockIdx.x * kWarps + warp; w < middle; w += gridDim.x * kWarps) {
+      const int page = __ldg(table + w);
+      double score = -INFINITY;
+      if (page < 0 || page >= a.c.pages) {
+        if (lane == 0) report(a.status, kBadPage, page);
+      } else {
+        const __nv_bfloat16* b = a.bounds + (page * (int64_t)a.c.heads + hk) * 2 * DP + lane * kCols;
+        score = 0.0;
+#pragma unroll
+        for (int e = 0; e < kCols; ++e) {
+          score = fma(u[e], (double)to_f32(b[DP + e]), score);
+          score = fma(d[e], (double)to_f32(b[e]), score);
+        }
+#pragma unroll
+        for (int x = 16; x >= 1; x >>= 1) score += __shfl_xor_sync(0xffffffffu, score, x);
+      }
+      if (lane == 0) to[w] = order_of(score);
+    }
+  }
+  if (gridDim.x > 1)
+    cluster.sync();
+  else
+    __syncthreads();
+  if (blockIdx.x != 0) return;
+  // the want-th largest key, digit by digit: `border`, of whose equals `ties` are taken
+  uint64_t border = 0, mask = 0;
+  int ties = want;
+  for (int shift = 56; shift >= 0 && want > 0; shift -= 8) {
+    count_of[tid] = 0;
+    __syncthreads();
+    for (int w = tid; w < middle; w += kThreads)
+      if ((keys[w] & mask) == border) atomicAdd(&count_of[(keys[w] >> shift) & 255], 1);
+    __syncthreads();
+    if (warp == 0) {   // a lane eight digits, from the top
+      int sum = 0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sum += count_of[255 - 8 * lane - e];
+      int upto = sum;
+#pragma unroll
+      for (int x = 1; x < 32; x *= 2) {
+        const int y = __shfl_up_sync(0xffffffffu, upto, x);
+        if (lane >= x) upto += y;
+      }
+      int before = upto - sum;
+      if (before < ties && ties <= upto)
+        for (int e = 0; e < 8; ++e) {
+          const int c = count_of[255 - 8 * lane - e];
+          if (before + c >= ties) {
+            digit = 255 - 8 * lane - e;
+            below = before;
+            break;
+          }
+          before += c;
+        }
+    }
+    __syncthreads();
+    border |= (uint64_t)digit << shift;
+    mask |= 255ull << shift;
+    ties -= below;
+    const bool all = count_of[digit] == ties;   // the whole digit is taken
+    __syncthreads();
+    if (all) break;
+  }
+  // ascending: the first pages, those picked between, the last
+  for (int e = tid; e < a.first; e += kThreads) out[e] = e;
+  for (int e = tid; e < a.last; e += kThreads) out[a.first + want + e] = pages - a.last + e;
+  int at = a.first, equal = 0;
+  for (int w0 = 0; w0 < middle && want > 0; w0 += kThreads) {
+    const int w = w0 + tid;
+    const uint64_t k = w < middle ? keys[w] & mask : 0;
+    const bool over = w < middle && k > border, same = w < middle && k == border;
+    const unsigned overs = __ballot_sync(0xffffffffu, over), sames = __ballot_sync(0xffffffffu, same);
+    if (lane == 0) {
+      part[0][warp] = __popc(overs);
+      part[1][warp] = __popc(sames);
+    }
+    __syncthreads();
+    const unsigned before = (1u << lane) - 1;
+    int o = __popc(overs & before), s = equal + __popc(sames & before), o_all = 0, s_all = 0;
+#pragma unroll
+    for (int x = 0; x < kWarps; ++x) {
+      if (x < warp) o += part[0][x], s += part[1][x];
+      o_all += part[0][x];
+      s_all += part[1][x];
+    }
+    // of the equal ones before this one, no more than `ties` were taken
+    if (over || (same && s < ties)) out[at + o + min(s, ties) - min(equal, ties)] = a.first + w;
+    at += o_all + min(equal + s_all, ties) - min(equal, ties);
+    equal += s_all;
+    __syncthreads();
+  }
+}
+
+template <int DT, int DP>
+int launch_select(const Kv4SelectArgs& a, cudaStream_t s) {
+  auto kern = select_kernel<DT, DP>;
+  const int64_t z = (int64_t)a.requests * a.n;
+  if (z > 65535 || a.c.heads > 65535) return set_error(SA_ERR_UNSUPPORTED, "kv4 select: grid too large");
+  const size_t smem = (size_t)a.width * 8;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSelectMaxPages * 8);
+  if (e != cudaSuccess) return set_error(SA_ERR_CUDA, "kv4 select smem attribute: %s", cudaGetErrorString(e));
+  int splits = 1;   // while a warp keeps eight pages and CTAs are few
+  while (splits < 8 && a.width >= splits * 2 * kWarps * 8 && z * a.c.heads * splits < 148) splits *= 2;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)splits, (unsigned)a.c.heads, (unsigned)z);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)splits;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  e = cudaLaunchKernelEx(&cfg, kern, a);
+  if (e != cudaSuccess) return set_error(SA_ERR_CUDA, "kv4 select_kernel: %s", cudaGetErrorString(e));
+  return check_launch("kv4 select_kernel");
+}
+
+template <int DT>
+int launch_select_dim(const Kv4SelectArgs& a, cudaStream_t s) {
+  if (a.c.dp == 32) return launch_select<DT, 32>(a, s);
+  if (a.c.dp == 64) return launch_select<DT, 64>(a, s);
+  if (a.c.dp == 128) return launch_select<DT, 128>(a, s);
+  return launch_select<DT, 256>(a, s);
+}
+
+}  // namespace
+
+int launch_kv4_bounds(const Kv4BoundsArgs& a, cudaStream_t s) {
+  // CTAs that share a request's pages: enough for the GPU when requests are few
+  const int64_t most = ceil_div((int64_t)a.width * a.c.heads, kWarps);
+  const int64_t x = std::min(most, std::max<int64_t>(ceil_div(148 * 8, a.requests), ceil_div(a.c.heads, kWarps)));
+  if (a.requests > 65535) return set_error(SA_ERR_UNSUPPORTED, "kv4 bounds: more than 65535 requests in one call");
+  bounds_kernel<<<dim3((unsigned)x, (unsigned)a.requests), kThreads, 0, s>>>(a);
+  return check_launch("kv4 bounds_kernel");
+}
+
+int launch_kv4_select(const Kv4SelectArgs& a, int dtype, cudaStream_t s) {
+  if (dtype == SA_REP_FLOAT32) return launch_select_dim<SA_REP_FLOAT32>(a, s);
+  if (dtype == SA_REP_FLOAT16) return launch_select_dim<SA_REP_FLOAT16>(a, s);
+  return launch_select_dim<SA_REP_BFLOAT16>(a, s);
+}
+
+}  // namespace sa

@@ -1,5 +1,5 @@
-// Page tables, slots and positions from request lengths, and the return of a
-// request's pages.
+// Page tables, slots and positions from request lengths, and the return of pages
+// of ended requests and of those that an eviction made shorter.
 //
 //   after[r]   = lengths[r] + new[r],   offsets = exclusive sum of new
 //   fresh(r)   = ceil(after[r] / P) - ceil(lengths[r] / P)  pages, in request order, from the end of the free list
@@ -22,6 +22,7 @@ namespace {
 constexpr int kPlanThreads = 1024;              // a batch of 1000 requests is summed in one round (256 threads: 13 us)
 constexpr int kPlanTokens = 2 * kPlanThreads;   // per CTA
 constexpr int kPlanMaxRequests = 16384;
+constexpr int kShrinkThreads = 1024;
 
 struct PlanArgs {
   const int32_t* lengths;
@@ -243,6 +244,89 @@ release_kernel(int32_t* lengths, int32_t* tables, const uint8_t* drop, int32_t* 
   if (tid == 0) free_count[0] = (int)at;
 }
 
+// After an eviction: requests longer than `limit` hold `keep` tokens, and the pages
+// behind those go to the end of the free list, in the order of requests and of their
+// tables.  One CTA: a warp counts a request's pages, and enters them behind the sum of
+// those before.
+__global__ void __launch_bounds__(kShrinkThreads)
+shrink_kernel(int32_t* lengths, int32_t* tables, int32_t* free_pages, int32_t* free_count, int32_t* dropped, int requests,
+              int width, int free_size, int page_shift, int keep, int limit, int* status) {
+  extern __shared__ int sums[];   // [requests]: pages that come free, then the sum of those before
+  __shared__ int part[kShrinkThreads / 32];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int from = (int)pages_of(keep, page_shift, width);
+  // the pages of request r behind `keep`: fn(page or -1, of each lane) for 32 at a time
+  auto each = [&](int r, auto fn) {
+    const int32_t* row = tables + (int64_t)r * width;
+    const int held = (int)pages_of(max(lengths[r], 0), page_shift, width);
+    for (int c0 = from; c0 < held; c0 += 32) {
+      const int c = c0 + lane;
+      int32_t page = c < held ? row[c] : -1;
+      if (page < -1 || page >= free_size) {
+        report(status, kBadPage, page);
+        page = -1;
+      }
+      fn(c, c < held, page);
+    }
+  };
+  // longer than its row allows, a request counts as one that fills it, as for the eviction
+  auto over = [&](int r) { return min((int64_t)lengths[r], (int64_t)width << page_shift) > limit; };
+  for (int r = warp; r < requests; r += kShrinkThreads / 32) {
+    int n = 0;
+    if (over(r)) each(r, [&](int, bool, int32_t page) { n += __popc(__ballot_sync(0xffffffffu, page >= 0)); });
+    if (lane == 0) sums[r] = n;
+  }
+  __syncthreads();
+  // exclusive sums: each thread a run of requests
+  const int run = (requests + kShrinkThreads - 1) / kShrinkThreads, r0 = min(tid * run, requests), r1 = min(r0 + run, requests);
+  int mine = 0;
+  for (int r = r0; r < r1; ++r) mine += sums[r];
+  int upto = mine;
+#pragma unroll
+  for (int d = 1; d < 32; d *= 2) {
+    const int y = __shfl_up_sync(0xffffffffu, upto, d);
+    if (lane >= d) upto += y;
+  }
+  if (lane == 31) part[warp] = upto;
+  __syncthreads();
+  const int had = min(max(free_count[0], 0), free_size);
+  int64_t at = (int64_t)had + upto - mine, total = had;
+  for (int w = 0; w < kShrinkThreads / 32; ++w) {
+    if (w < warp) at += part[w];
+    total += part[w];
+  }
+  for (int r = r0; r < r1; ++r) {   // where request r's pages go; past the list's end they are reported
+    const int n = sums[r];
+    sums[r] = (int)min(at, (int64_t)free_size);
+    at += n;
+  }
+  __syncthreads();
+  for (int r = warp; r < requests; r += kShrinkThreads / 32) {
+    const bool shrinks = over(r);
+    if (shrinks) {
+      int64_t to = sums[r];
+      each(r, [&](int c, bool in, int32_t page) {
+        const unsigned on = __ballot_sync(0xffffffffu, page >= 0);
+        const int64_t place = to + __popc(on & ((1u << lane) - 1));
+        if (in) tables[(int64_t)r * width + c] = -1;
+        if (page >= 0) {
+          if (place < free_size)
+            free_pages[place] = page;
+          else
+            report(status, kNoRows, place);
+        }
+        to += __popc(on);
+      });
+    }
+    __syncwarp();
+    if (lane == 0) {
+      dropped[r] = shrinks ? lengths[r] - keep : 0;
+      if (shrinks) lengths[r] = keep;
+    }
+  }
+  if (tid == 0) free_count[0] = (int)min(total, (int64_t)free_size);
+}
+
 }  // namespace
 
 int launch_plan_pages(const int32_t* lengths, const int32_t* fresh, int32_t* tables, const int32_t* free_pages,
@@ -263,6 +347,21 @@ int launch_plan_pages(const int32_t* lengths, const int32_t* fresh, int32_t* tab
   const int64_t ctas = max_tokens > 0 ? ceil_div(max_tokens, kPlanTokens) : 1;
   plan_kernel<<<(unsigned)ctas, kPlanThreads, smem, s>>>(a);
   return check_launch("plan_kernel");
+}
+
+int launch_shrink_requests(int32_t* lengths, int32_t* tables, int32_t* free_pages, int32_t* free_count, int32_t* dropped,
+                           int requests, int width, int free_size, int page_shift, int keep, int limit, int* status,
+                           cudaStream_t s) {
+  if (requests > kPlanMaxRequests)
+    return set_error(SA_ERR_UNSUPPORTED, "eviction: more than %d requests", kPlanMaxRequests);
+  const size_t smem = (size_t)requests * 4;
+  if (smem > 48 * 1024) {
+    const cudaError_t e = cudaFuncSetAttribute(shrink_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPlanMaxRequests * 4);
+    if (e != cudaSuccess) return set_error(SA_ERR_CUDA, "eviction smem attribute: %s", cudaGetErrorString(e));
+  }
+  shrink_kernel<<<1, kShrinkThreads, smem, s>>>(lengths, tables, free_pages, free_count, dropped, requests, width, free_size,
+                                                page_shift, keep, limit, status);
+  return check_launch("shrink_kernel");
 }
 
 int launch_release_pages(int32_t* lengths, int32_t* tables, const uint8_t* drop, int32_t* free_pages,

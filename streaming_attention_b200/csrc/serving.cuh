@@ -20,6 +20,8 @@ constexpr int kBadOffsets = 403;  // offsets that are not monotone or leave the 
 constexpr int kNoPages = 404;     // the list of free pages ran out
 constexpr int kNoRows = 405;      // more new tokens than the outputs hold
 constexpr int kHeld = 406;        // a prompt for a request that holds tokens
+constexpr int kBadList = 407;     // a list of pages that is not ascending or leaves the table
+constexpr int kBadPrefix = 408;   // a prefix longer than its table
 
 __device__ __forceinline__ void report(int* status, int code, long long index) {
   if (status && atomicCAS(status, 0, code) == 0) *reinterpret_cast<volatile long long*>(status + 2) = index;

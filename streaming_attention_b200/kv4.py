@@ -9,6 +9,11 @@ tokens over its pages, ``Kv4Cache.read`` gives back what slots hold, and
 the free list stay on the device: nothing here reads them on the host, so a
 decode step can be captured into a CUDA graph.
 
+For long requests: ``attend_shared`` computes a prefix that all requests share
+once for all; ``update_page_bounds`` / ``select_pages`` / ``attend_pages`` read, for each
+query, only the pages whose keys may matter most to it; ``attend(weights=...)`` adds up
+what weight each token had, and ``evict`` drops the tokens of little weight.
+
 Every (token, head) row of keys and of values is held as 4-bit codes with a
 scale and a least value in bfloat16 (layout in include/streaming_attention.h):
 
@@ -222,19 +227,10 @@ class Kv4Cache:
                      S.DTYPES[dtype])
         return k, v
 
-    def attend(self, q: Tensor, tables: Tensor, lengths: Tensor, *, window: Optional[int] = None, sinks: int = 0,
-               scale: Optional[float] = None) -> Tensor:
-        """Attention of each request's newest tokens over its cached ones.
-
-        q [R,H,D] (one token each) or [R,N,H,D] (the last N of each request);
-        ``tables`` int32 [R,W], ``lengths`` int32 [R] count the new tokens, which
-        are appended before.  Query i of N stands at lengths[r] - N + i and sees
-        as in ``sliding_window_attention``; a query that sees nothing (a request
-        of length 0, or shorter than N) gives zeros.  Returns q's shape and dtype."""
-        cache = self._storage()
-        S.device_of(self.k_codes, q, tables, lengths)
+    def _queries(self, q: Tensor, tables: Tensor, lengths: Tensor):
+        """q as [R,N,H,D] with contiguous rows, tables and lengths as the kernels read them,
+        the element type's code and a new result."""
         code = S.dtype_code(q)
-        w, s = S.check_window(window, sinks)
         if q.ndim not in (3, 4):
             raise ValueError("q must be [R,H,D] or [R,N,H,D]")
         q4 = q[:, None] if q.ndim == 3 else q
@@ -245,10 +241,208 @@ class Kv4Cache:
             raise ValueError(f"tables must be [{r},W]")
         tables = S.int32(tables, tables.shape, "tables")
         lengths = S.int32(lengths, (r,), "lengths")
+        return S.rows(q4), tables, lengths, code
+
+    def _scale(self, scale: Optional[float]) -> float:
+        return float(1.0 / math.sqrt(self.dim) if scale is None else scale)
+
+    def attend(self, q: Tensor, tables: Tensor, lengths: Tensor, *, window: Optional[int] = None, sinks: int = 0,
+               scale: Optional[float] = None, weights: Optional[Tensor] = None) -> Tensor:
+        """Attention of each request's newest tokens over its cached ones.
+
+        q [R,H,D] (one token each) or [R,N,H,D] (the last N of each request);
+        ``tables`` int32 [R,W], ``lengths`` int32 [R] count the new tokens, which
+        are appended before.  Query i of N stands at lengths[r] - N + i and sees
+        as in ``sliding_window_attention``; a query that sees nothing (a request
+        of length 0, or shorter than N) gives zeros.  Returns q's shape and dtype.
+
+        ``weights`` (``token_weights()``, float32 [P,Hkv,page]) is added to, in place: at each
+        token's slot the softmax weight it had, summed over the N queries and the
+        heads that read the key head.  No page may then stand in two requests' tables."""
+        cache = self._storage()
+        S.device_of(self.k_codes, q, tables, lengths, *(() if weights is None else (weights,)))
+        w, s = S.check_window(window, sinks)
+        q4, tables, lengths, code = self._queries(q, tables, lengths)
+        if weights is not None:
+            self._check_weights(weights)
+        r, n, heads, d = q4.shape
         out = torch.empty((r, n, heads, d), device=self.device, dtype=q.dtype)
         if out.numel():
-            q4 = S.rows(q4)
-            S.launch(self.device, "sa_kv4_attend", *cache, q4.data_ptr(), out.data_ptr(),
-                     S.strides(*q4.stride()[:3]), tables.data_ptr(), lengths.data_ptr(), r, n, heads, tables.shape[1],
-                     w, s, float(1.0 / math.sqrt(d) if scale is None else scale), code)
+            args = (*cache, q4.data_ptr(), out.data_ptr(), S.strides(*q4.stride()[:3]), tables.data_ptr(),
+                    lengths.data_ptr(), r, n, heads, tables.shape[1], w, s, self._scale(scale), code)
+            if weights is None:
+                S.launch(self.device, "sa_kv4_attend", *args)
+            else:
+                ws = S.workspace(self.device, "sa_kv4_attend_weigh_workspace_size", self.kv_heads, self.page_size, r, n,
+                                 heads, tables.shape[1], w, s)
+                S.launch(self.device, "sa_kv4_attend_weigh", *args, weights.data_ptr(), ws.data_ptr(), ws.numel())
         return out[:, 0] if q.ndim == 3 else out
+
+    def attend_shared(self, q: Tensor, prefix_table: Tensor, prefix_length: Tensor, tables: Tensor, lengths: Tensor, *,
+                      window: Optional[int] = None, sinks: int = 0, scale: Optional[float] = None) -> Tensor:
+        """``attend`` of a batch whose requests share a prefix, which is read and computed
+        once for all: request r's tokens are those of the prefix (``prefix_length`` int32 [1]
+        in pages ``prefix_table`` int32 [W0]) and behind them its own (``lengths[r]``
+        in pages ``tables[r]``).  The queries are the last N of its own tokens; one that it does
+        not have (a request of length 0, or shorter than N) gives zeros.  Positions, ``window`` and
+        ``sinks`` count from the prefix's first token."""
+        cache = self._storage()
+        S.device_of(self.k_codes, q, prefix_table, prefix_length, tables, lengths)
+        w, s = S.check_window(window, sinks)
+        q4, tables, lengths, code = self._queries(q, tables, lengths)
+        if prefix_table.ndim != 1:
+            raise ValueError("prefix_table must be [W0]")
+        prefix_table = S.int32(prefix_table, prefix_table.shape, "prefix_table")
+        prefix_length = S.int32(prefix_length, (1,), "prefix_length")
+        r, n, heads, d = q4.shape
+        out = torch.empty((r, n, heads, d), device=self.device, dtype=q.dtype)
+        if out.numel():
+            ws = S.workspace(self.device, "sa_kv4_attend_shared_workspace_size", self.kv_heads, self.page_size, d, r, n, heads,
+                             prefix_table.shape[0], w, s, code)
+            S.launch(self.device, "sa_kv4_attend_shared", *cache, q4.data_ptr(), out.data_ptr(), S.strides(*q4.stride()[:3]),
+                     prefix_table.data_ptr(), prefix_length.data_ptr(), prefix_table.shape[0], tables.data_ptr(),
+                     lengths.data_ptr(), r, n, heads, tables.shape[1], w, s, self._scale(scale), code, ws.data_ptr(),
+                     ws.numel())
+        return out[:, 0] if q.ndim == 3 else out
+
+    def attend_pages(self, q: Tensor, tables: Tensor, lengths: Tensor, pages: Tensor, *,
+                     scale: Optional[float] = None) -> Tensor:
+        """``attend`` over chosen pages alone: ``pages`` int32 [R,Hkv,K] ([R,N,Hkv,K] for q
+        [R,N,H,D]) lists for each query and key head rows of the request's table, in
+        ascending order, -1 behind (as ``select_pages`` gives them).  A query sees the tokens
+        up to its own that stand in them."""
+        cache = self._storage()
+        S.device_of(self.k_codes, q, tables, lengths, pages)
+        q4, tables, lengths, code = self._queries(q, tables, lengths)
+        r, n, heads, d = q4.shape
+        lead = (r, self.kv_heads) if q.ndim == 3 else (r, n, self.kv_heads)
+        if pages.ndim != len(lead) + 1:
+            raise ValueError(f"pages must be {[*lead, 'K']}")
+        pages = S.int32(pages, (*lead, pages.shape[-1]), "pages")
+        out = torch.empty((r, n, heads, d), device=self.device, dtype=q.dtype)
+        if out.numel():
+            S.launch(self.device, "sa_kv4_attend_pages", *cache, q4.data_ptr(), out.data_ptr(), S.strides(*q4.stride()[:3]),
+                     tables.data_ptr(), lengths.data_ptr(), pages.data_ptr(), pages.shape[-1], r, n, heads, tables.shape[1],
+                     self._scale(scale), code)
+        return out[:, 0] if q.ndim == 3 else out
+
+    def page_bounds(self) -> Tensor:
+        """Room for the bounds of every page's keys, bfloat16 [P,Hkv,2,Dp], zeros."""
+        self._storage()
+        shape = (self.num_pages, self.kv_heads, 2, self.padded_dim(self.dim))
+        return torch.zeros(shape, dtype=torch.bfloat16, device=self.device)
+
+    def _check_bounds(self, bounds: Tensor) -> None:
+        shape = (self.num_pages, self.kv_heads, 2, self.padded_dim(self.dim))
+        if bounds.dtype != torch.bfloat16 or bounds.shape != shape or not bounds.is_contiguous():
+            raise ValueError(f"bounds must be contiguous bfloat16 {list(shape)}")
+
+    def update_page_bounds(self, bounds: Tensor, tables: Tensor, lengths: Tensor, new: Tensor) -> None:
+        """Writes to ``bounds`` the least and the largest value of each column of the keys
+        that the pages of each request's newest ``new[r]`` (int32 [R]) tokens hold;
+        ``lengths`` counts them, as after ``append``.  Other pages' bounds stay."""
+        cache = self._storage()
+        S.device_of(self.k_codes, bounds, tables, lengths, new)
+        self._check_bounds(bounds)
+        if tables.ndim != 2:
+            raise ValueError("tables must be [R,W]")
+        tables = S.int32(tables, tables.shape, "tables")
+        r, width = tables.shape
+        lengths = S.int32(lengths, (r,), "lengths")
+        new = S.int32(new, (r,), "new")
+        if r and width:
+            S.launch(self.device, "sa_kv4_page_bounds", *cache, bounds.data_ptr(), tables.data_ptr(), lengths.data_ptr(),
+                     new.data_ptr(), r, width)
+
+    def select_pages(self, q: Tensor, bounds: Tensor, tables: Tensor, lengths: Tensor, *, count: int, first: int = 1,
+                     last: int = 1) -> Tensor:
+        """The ``count`` pages each query should read, int32 [R,Hkv,count] ([R,N,Hkv,count] for
+        q [R,N,H,D]): rows of the request's table, ascending, -1 behind.  Of the pages up
+        to the query's own the ``first`` first and the ``last`` last are always among them; of
+        those between, the ones of the largest
+
+            score = sum over the heads of a key head, columns c, of max(q_c low_c, q_c high_c)
+
+        with the page's ``bounds`` (of equal scores the lowest page; NaN is the largest)."""
+        self._storage()
+        S.device_of(self.k_codes, q, bounds, tables, lengths)
+        self._check_bounds(bounds)
+        q4, tables, lengths, code = self._queries(q, tables, lengths)
+        count, first, last = S.whole(count, "count"), S.whole(first, "first"), S.whole(last, "last")
+        if count < 0 or count > 2 ** 31 - 1:
+            raise ValueError("count must lie in [0, 2^31)")
+        if first < 0 or last < 0 or first + last > count:
+            raise ValueError("first and last must be non-negative, and no more than count together")
+        r, n, heads, _ = q4.shape
+        out = torch.empty((r, n, self.kv_heads, count), device=self.device, dtype=torch.int32)
+        if out.numel():
+            S.launch(self.device, "sa_kv4_select_pages", bounds.data_ptr(), self.num_pages, self.kv_heads, self.page_size,
+                     self.dim, q4.data_ptr(), S.strides(*q4.stride()[:3]), tables.data_ptr(), lengths.data_ptr(), r, n, heads,
+                     tables.shape[1], count, first, last, code, out.data_ptr())
+        return out[:, 0] if q.ndim == 3 else out
+
+    def token_weights(self) -> Tensor:
+        """Room for the weight of every token, float32 [P,Hkv,page], zeros."""
+        self._storage()
+        return torch.zeros((self.num_pages, self.kv_heads, self.page_size), dtype=torch.float32, device=self.device)
+
+    def _check_weights(self, weights: Tensor) -> None:
+        shape = (self.num_pages, self.kv_heads, self.page_size)
+        if weights.dtype != torch.float32 or weights.shape != shape or not weights.is_contiguous():
+            raise ValueError(f"weights must be contiguous float32 {list(shape)}")
+
+    def reset_weights(self, weights: Tensor, slots: Tensor) -> None:
+        """Zeros for the weights of ``slots`` (int32 [T], negative: none): what new tokens start
+        from, where others stood before."""
+        self._storage()
+        S.device_of(self.k_codes, weights, slots)
+        self._check_weights(weights)
+        if slots.ndim != 1:
+            raise ValueError("slots must be [T]")
+        slots = S.int32(slots, slots.shape, "slots")
+        if slots.shape[0]:
+            S.launch(self.device, "sa_kv4_reset_weights", weights.data_ptr(), self.num_pages, self.kv_heads, self.page_size,
+                     slots.data_ptr(), slots.shape[0])
+
+    def evict(self, weights: Tensor, lengths: Tensor, tables: Tensor, free_pages: Tensor, free_count: Tensor, *, keep: int,
+              limit: Optional[int] = None, first: int = 0, last: int = 0) -> Tuple[Tensor, Tensor]:
+        """Drops tokens of little weight, in place: a request of more than ``limit`` tokens
+        (default ``keep``) keeps ``keep`` of each key head -- its ``first`` first ones, its ``last``
+        newest ones and, between, those of the largest ``weights`` (of equal ones the
+        lowest; NaN is the largest) -- moved up in order, with their weights, to its first slots.  Its
+        length becomes ``keep``; the pages behind go to the end of the free list; the weights
+        of the slots behind become zero.
+
+        Returns which tokens each head kept (int32 [R,Hkv,keep]; of a request that was not
+        over 0, 1, .. and -1 behind its last) and how many a request lost (int32 [R]): its next
+        token's position is its length plus all it ever lost.  Heads keep tokens of their
+        own, so ``window`` and ``sinks`` count what is held, and bounds of its pages are to be
+        updated as a whole.  No page may stand in two requests' tables."""
+        cache = self._storage()
+        S.device_of(self.k_codes, weights, lengths, tables, free_pages, free_count)
+        self._check_weights(weights)
+        keep, first, last = S.whole(keep, "keep"), S.whole(first, "first"), S.whole(last, "last")
+        limit = keep if limit is None else S.whole(limit, "limit")
+        if not 1 <= keep <= limit <= 2 ** 31 - 1:
+            raise ValueError("keep must be positive, and limit no less")
+        if first < 0 or last < 0 or first + last > keep:
+            raise ValueError("first and last must be non-negative, and no more than keep together")
+        if tables.ndim != 2:
+            raise ValueError("tables must be [R,W]")
+        if free_pages.ndim != 1:
+            raise ValueError("free_pages must be [F]")
+        r, width = tables.shape
+        S.int32(lengths, (r,), "lengths")
+        S.int32(tables, (r, width), "tables")
+        S.int32(free_pages, free_pages.shape, "free_pages")
+        S.int32(free_count, (1,), "free_count")
+        for t in (lengths, tables, free_pages, free_count):
+            if not t.is_contiguous():
+                raise ValueError("lengths, tables, free_pages and free_count are updated in place: they must be contiguous")
+        kept = torch.empty((r, self.kv_heads, keep), device=self.device, dtype=torch.int32)
+        dropped = torch.empty((r,), device=self.device, dtype=torch.int32)
+        if r:
+            S.launch(self.device, "sa_kv4_evict", *cache, weights.data_ptr(), lengths.data_ptr(), tables.data_ptr(),
+                     free_pages.data_ptr(), free_count.data_ptr(), r, width, free_pages.shape[0], keep, limit, first, last,
+                     kept.data_ptr(), dropped.data_ptr())
+        return kept, dropped
