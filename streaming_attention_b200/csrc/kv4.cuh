@@ -56,7 +56,7 @@ struct Kv4AttendArgs {
   int score_rows;
   float* weights;   // [pages, heads, page]
   // a shared prefix, and the unfinished sums of `parts` parts of it: [parts, key heads,
-  // requests * n * group] (x dp)
+  // dp / 4, rows, 4], maximum and total [parts, key heads, rows], rows = requests * n * group
   const int32_t* prefix_table;
   const int32_t* prefix_length;
   int prefix_width;
@@ -107,6 +107,9 @@ size_t kv4_weigh_bytes(const Kv4AttendArgs& a);
 int launch_kv4_attend_weigh(Kv4AttendArgs a, void* workspace, cudaStream_t s);
 int launch_kv4_reset_weights(float* weights, const int32_t* slots, int64_t tokens, int64_t pages, int heads, int page_shift,
                              int* status, cudaStream_t s);
+bool kv4_prefix_tc_takes(const Kv4AttendArgs& a, int64_t rows);
+int kv4_prefix_tc_parts(const Kv4AttendArgs& a, int64_t rows);
+int launch_kv4_prefix_tc(const Kv4AttendArgs& a, int64_t rows, cudaStream_t s);
 size_t kv4_shared_bytes(const Kv4AttendArgs& a);
 int launch_kv4_attend_shared(Kv4AttendArgs a, void* workspace, cudaStream_t s);
 int launch_kv4_bounds(const Kv4BoundsArgs& a, cudaStream_t s);

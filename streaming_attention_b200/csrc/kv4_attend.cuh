@@ -651,7 +651,9 @@ __global__ void __launch_bounds__(kThreads, (Shape<DT, DP, NT>::kPerSm)) attend_
   // and the cluster's CTAs, each a share of the columns
   const int share = S::kRows * DP / splits;
   for (int x = blockIdx.x * share + threadIdx.x; x < (blockIdx.x + 1) * share; x += kThreads) {
-    const int row = x / DP, col = x - row * DP;
+    // the parts of a prefix stand as [columns / 4][row][4]: threads follow them
+    constexpr bool kParts = kMode == kPrefix || kMode == kTail;
+    const int row = kParts ? (x >> 2) % S::kRows : x / DP, col = kParts ? (x >> 2) / S::kRows * 4 + (x & 3) : x - row * DP;
     float top = -INFINITY, sum = 0.0f, total = 0.0f;
     for (int s = 0; s < splits; ++s) top = fmaxf(top, splits > 1 ? *cluster.map_shared_rank(part_m + row, s) : part_m[row]);
     for (int s = 0; s < splits; ++s) {
@@ -664,19 +666,20 @@ __global__ void __launch_bounds__(kThreads, (Shape<DT, DP, NT>::kPerSm)) attend_
     }
     if (kMode == kPrefix) {   // unfinished: kTail joins the parts
       if (row0 + row < rows) {
-        const int64_t at = ((int64_t)part * a.c.heads + hk) * rows + row0 + row;
-        a.part_o[at * DP + col] = sum;
-        if (col == 0) a.part_ml[at] = make_float2(top, total);
+        const int64_t of = (int64_t)part * a.c.heads + hk;
+        a.part_o[((of * (DP / 4) + (col >> 2)) * rows + row0 + row) * 4 + (col & 3)] = sum;
+        if (col == 0) a.part_ml[of * rows + row0 + row] = make_float2(top, total);
       }
       continue;
     }
     if (row0 + row < rows && col < a.c.d) {
       if (kMode == kTail) {   // the prefix's parts, in order
-        const int64_t all = (int64_t)a.requests * rows, at = (int64_t)hk * all + (int64_t)r * rows + row0 + row;
+        const int64_t all = (int64_t)a.requests * rows, at = (int64_t)r * rows + row0 + row;
+#pragma unroll 4
         for (int s = 0; s < a.parts; ++s) {
-          const int64_t from = at + s * a.c.heads * all;
-          const float2 ml = a.part_ml[from];
-          const float o = a.part_o[from * DP + col], next = fmaxf(top, ml.x);
+          const int64_t of = (int64_t)s * a.c.heads + hk;
+          const float2 ml = a.part_ml[of * all + at];
+          const float o = a.part_o[((of * (DP / 4) + (col >> 2)) * all + at) * 4 + (col & 3)], next = fmaxf(top, ml.x);
           if (next == -INFINITY) {   // nothing seen yet; NaN stays
             sum += o;
             total += ml.y;

@@ -61,6 +61,8 @@ SHARED = [
     (6000, [500, 1], 12, 4, 4, 96, 64, None, 0),
     (0, [40, 3], 4, 2, 1, 64, 16, None, 0),
     (5000, [13] * 70, 8, 2, 1, 32, 64, 3000, 2),
+    (9001, [3] * 40, 64, 8, 1, 64, 64, None, 0),    # long chains of tiles in one part
+    (4100, [5, 6] * 33, 96, 8, 2, 32, 32, None, 0),
 ]
 
 
