@@ -673,21 +673,32 @@ __global__ void __launch_bounds__(kThreads, (Shape<DT, DP, NT>::kPerSm)) attend_
       continue;
     }
     if (row0 + row < rows && col < a.c.d) {
-      if (kMode == kTail) {   // the prefix's parts, in order
+      if (kMode == kTail) {   // the prefix's parts, in order, kBatch of them on their way at a time
+        constexpr int kBatch = 10;
         const int64_t all = (int64_t)a.requests * rows, at = (int64_t)r * rows + row0 + row;
-#pragma unroll 4
-        for (int s = 0; s < a.parts; ++s) {
-          const int64_t of = (int64_t)s * a.c.heads + hk;
-          const float2 ml = a.part_ml[of * all + at];
-          const float o = a.part_o[((of * (DP / 4) + (col >> 2)) * all + at) * 4 + (col & 3)], next = fmaxf(top, ml.x);
-          if (next == -INFINITY) {   // nothing seen yet; NaN stays
-            sum += o;
-            total += ml.y;
-            continue;
+        const int64_t part_ml = a.c.heads * all, part_o = part_ml * DP;
+        const float2* from_ml = a.part_ml + hk * all + at;
+        const float* from_o = a.part_o + ((hk * (DP / 4) + (col >> 2)) * all + at) * 4 + (col & 3);
+        for (int s0 = 0; s0 < a.parts; s0 += kBatch, from_ml += kBatch * part_ml, from_o += kBatch * part_o) {
+          float2 ml[kBatch];
+          float o[kBatch];
+          float next = top;
+#pragma unroll
+          for (int s = 0; s < kBatch; ++s) {
+            ml[s] = s0 + s < a.parts ? from_ml[s * part_ml] : make_float2(-INFINITY, 0.0f);
+            o[s] = s0 + s < a.parts ? from_o[s * part_o] : 0.0f;
           }
-          const float f = top == -INFINITY ? 1.0f : ex2(top - next), g = ml.x == -INFINITY ? 1.0f : ex2(ml.x - next);
-          sum = fmaf(g, o, f * sum);
-          total = fmaf(g, ml.y, f * total);
+#pragma unroll
+          for (int s = 0; s < kBatch; ++s) next = fmaxf(next, ml[s].x);
+          const float f = top == -INFINITY ? 1.0f : ex2(top - next);   // nothing yet: zeros, or NaN that stays
+          sum *= f;
+          total *= f;
+#pragma unroll
+          for (int s = 0; s < kBatch; ++s) {
+            const float g = ml[s].x == -INFINITY ? 1.0f : ex2(ml[s].x - next);
+            sum = fmaf(g, o[s], sum);
+            total = fmaf(g, ml[s].y, total);
+          }
           top = next;
         }
       }

@@ -3,25 +3,34 @@
 // What the prefix of a batch adds to each row: an unfinished sum, its maximum and total
 // for kTail (kv4_attend.cuh), as kPrefix there, which takes the other types and few rows.
 //
-// A code less 8 is exact in bfloat16, so the products take codes and the rows' scales and
-// least values stay outside, in float32.  With x = least + 8 scale,
-//   score_j = s_k (Q K'^T)_j + x_k sum(Q),   O = (p s_v) V' + sum(p x_v),
-// K', V' the centred codes.  Q is one bfloat16 piece (float16: two, exact), and so is p s_v
-// (rounded to bfloat16, as the windowed attention's probabilities; float16: two pieces, 16 bits).
+// Operands are float16.  A scale has 8 bits and a code less 8 at most 3, so their
+// product is exact in float16's 11, and with x = least + 8 scale
+//   score_j = scale (sum_c q_c k'_jc + x_j sum(Q)),   k' = scale (code - 8),
+// the second term as 16 more columns of the same product: x_j and sum(Q) in three pieces
+// each.  Values are rounded once, to float16 (2^-12 of them at most), and so are
+// probabilities.  Powers of two keep all in float16's range: one for each query row, one
+// for the keys and one for the values of a CTA, from their largest (what is 2^-26 of the
+// largest and less may lose bits).
+// (Scales outside the products, bfloat16 codes inside: each score then wants 16 bytes of
+// parameters out of shared memory, 2048 of its cycles a tile, and the kernel took 85 us.)
 //
 // A CTA holds two tiles of 128 query rows of one key head (a row: request, query, head)
 // and a part of the prefix in tiles of 64 tokens; all rows see (nearly) all of it, so a
 // decoded tile serves 256 rows.  Warps: 0..3 and 4..7 are the softmax of a row tile, one
-// row a thread; 8..11 decode: 16 bytes of codes a load, two tiles ahead in registers, to
-// swizzled tiles in shared memory; 12 and 13 issue the products of a row tile, one elected lane.
-// TMEM: of each row tile two S of 64 columns and O; P overwrites its S.  The issuer goes
-// P V(j), S(j + 2), so that scores are there while a softmax runs.
+// row a thread; 8..11 decode keys and 12..15 values, from raw tiles that warp 18 brings
+// in ahead (bulk copies) to swizzled ones; 16 and 17 issue the products of a row tile, one
+// elected lane.  TMEM: of each row tile two S of 64 columns and O; P overwrites the first
+// half of its S.  The issuer goes P V(j), S(j + 2), so that scores are there while a softmax
+// runs.
 //
-// Order inside the tiles.  A word of a key row holds eight columns' codes; one shift and
-// two logical operations give those of columns i and i + 4, so K' and Q hold columns in the
-// order 0 4 1 5 2 6 3 7.  A word of values holds four tokens of two columns, and gives tokens
-// 0 and 2, 1 and 3: V' lies a column to a row, tokens in the order 0 2 1 3, and P's halves
-// are packed to match.
+// Order inside the tiles.  A word of a key row holds eight columns' codes, of which one
+// logical operation gives two (columns i and i + 4) as 1024 + code or 64 + code, so keys and
+// queries hold columns in the order 0 4 1 5 2 6 3 7.  A word of values holds four tokens of
+// two columns, and gives tokens 0 and 2, 1 and 3: values lie a column to a row, tokens in the
+// order 0 2 1 3, and P's halves are packed to match.
+//
+// A token whose value is not finite gets values of 0 and a key that is NaN: whoever sees
+// it comes out NaN, and nobody else.
 #include <math.h>
 
 #include <algorithm>
@@ -39,10 +48,18 @@ constexpr int kTileRows = 128;
 constexpr int kTokens = 64;        // of a tile
 constexpr int kRowTiles = 2;
 constexpr int kSoftmax = kRowTiles * kTileRows;
-constexpr int kDecoders = 128;
-constexpr int kPrefixThreads = kSoftmax + kDecoders + kRowTiles * 32;
+constexpr int kDecoders = 128;     // of keys, and as many of values
+constexpr int kIssuer = (kSoftmax + 2 * kDecoders) / 32;   // the first of two warps
+constexpr int kLoader = kIssuer + kRowTiles;
+constexpr int kPrefixThreads = (kLoader + 2) * 32;          // whole groups of four warps
+// Registers of a thread: launched with 96 (65536 / 640, in steps of 8), then dealt out by groups of four
+// warps: 2 x 136 (a row's 64 scores stay in registers) + 2 x 72 + 64 = 5 x 96.
+constexpr int kSoftmaxRegs = 136, kDecoderRegs = 72, kOtherRegs = 64;
+static_assert(2 * kSoftmaxRegs + 2 * kDecoderRegs + kOtherRegs <= 5 * 96, "more registers than the launch has");
+constexpr float kShiftP = 6.0f;    // P = 2^(x - m + 6), m at most kMove below the largest x: 2^14 at most, and 2^-14,
+                                   // where float16 starts to lose bits, is 2^-20 of a row's usual largest
 
-constexpr int kErrK = 521, kErrV = 522, kErrP = 523, kErrS = 524, kErrEmpty = 525, kErrO = 526, kErrDrain = 527;
+constexpr int kErrK = 521, kErrV = 522, kErrP = 523, kErrS = 524, kErrEmpty = 525, kErrO = 526, kErrDrain = 527, kErrRaw = 528;
 
 struct PrefixParams {
   Kv4AttendArgs a;
@@ -51,22 +68,32 @@ struct PrefixParams {
   uint64_t wait_ns;
 };
 
-template <int DT, int DP>
+template <int DP>
 struct PrefixLayout {
-  static constexpr int kQ = DT == SA_REP_BFLOAT16 ? 1 : 2;   // pieces of q, and of p s_v
   static constexpr int kChunks = (DP + 63) / 64;             // of 64 columns: a row of 128 bytes
-  static constexpr int kQPiece = kChunks * kTileRows * 128;
+  static constexpr int kQ = kChunks * kTileRows * 128;
   static constexpr int kK = kChunks * kTokens * 128;
   static constexpr int kV = DP * 128;
-  static constexpr int kKStages = kQ == 1 ? 4 : 3, kVStages = kQ == 1 ? 3 : 2;
-  static constexpr int kKeys = kRowTiles * kQ * kQPiece;
-  static constexpr int kValues = kKeys + kKStages * kK;
-  static constexpr int kParams = kValues + kVStages * kV;    // of each V stage: 64 keys' and 64 values' scales and offsets
-  static constexpr int kInfo = kParams + kVStages * kTokens * 16;   // and its blocks' first tokens, and whether all see all
-  static constexpr int kBars = kInfo + kVStages * 32;
-  static constexpr int kBytes = kBars + (2 * kKStages + 2 * kVStages + 12) * 8 + 32 + 1024;
+  static constexpr int kStages = 3;
+  // the 16 columns of the sums and of the offsets: rows of 32 bytes
+  static constexpr int kQSum = kTileRows * 32, kKOff = kTokens * 32;
+  // a raw tile: keys, eight tokens' values (16 bytes on: their readers fall into different banks), parameters,
+  // its blocks' first tokens
+  static constexpr int kChunkBytes = 4 * DP, kChunkPitch = kChunkBytes + 16;
+  static constexpr int kRawV = kTokens * DP / 2, kRawKp = kRawV + 8 * kChunkPitch, kRawVp = kRawKp + kTokens * 4;
+  static constexpr int kRawInfo = kRawVp + kTokens * 4, kRaw = kRawInfo + 16;
+  static constexpr int kRawStages = 4;
+  static constexpr int kKeys = kRowTiles * kQ;
+  static constexpr int kValues = kKeys + kStages * kK;
+  static constexpr int kSums = kValues + kStages * kV;
+  static constexpr int kOffsets = kSums + kRowTiles * kQSum;
+  static constexpr int kPowers = kOffsets + kStages * kKOff;   // of the rows
+  static constexpr int kRaws = kPowers + kSoftmax * 4;
+  static constexpr int kBars = kRaws + kRawStages * kRaw;
+  static constexpr int kBytes = kBars + (4 * kStages + 2 * kRawStages + 12) * 8 + 48 + 1024;
   static_assert(kBytes <= 227 * 1024, "shared memory");
-  static_assert(kValues % 1024 == 0 && kKeys % 1024 == 0, "swizzled tiles start on 1024 bytes");
+  static_assert(kValues % 1024 == 0 && kKeys % 1024 == 0 && kSums % 1024 == 0 && kOffsets % 1024 == 0 && kRaws % 16 == 0 &&
+                kRaw % 16 == 0 && kBars % 8 == 0, "alignment of tiles, copies and barriers");
 };
 
 __device__ __forceinline__ uint64_t pack2(float a, float b) {
@@ -80,11 +107,6 @@ __device__ __forceinline__ void unpack2(uint64_t x, float& a, float& b) {
 __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
   uint64_t r;
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
 __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
@@ -102,6 +124,15 @@ __device__ __forceinline__ void tie16(float* v) {
 __device__ __forceinline__ void tie32(float (&v)[32]) {
   tie16(v);
   tie16(v + 16);
+}
+
+template <int N>
+__device__ __forceinline__ void fewer_registers() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void more_registers() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
 }
 
 // O of a row times alpha, in TMEM (rare).
@@ -125,86 +156,117 @@ __device__ __forceinline__ uint32_t low_bits(int x) {
   return x >= 32 ? 0xffffffffu : (x <= 0 ? 0u : (1u << x) - 1u);
 }
 
-// 32 scores in base 2: s_k S + x_k sum(Q); params: {s, s', x, x'} of each pair of tokens.
-__device__ __forceinline__ void finish_scores(float (&s)[32], const float4* params, uint64_t qsum2) {
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+__device__ __forceinline__ uint32_t fma_f16(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t r;
+  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+  return r;
+}
+__device__ __forceinline__ uint32_t mul_f16(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ uint32_t add_f16(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("add.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+// Eight codes less kBias, two at a time (nibble i of each half of w), as float16: a code in a
+// mantissa's low bits is added to 1024, four bits further up to 64.
+template <int kBias>
+__device__ __forceinline__ void codes16(uint32_t w, uint32_t (&c)[4]) {
+  constexpr uint32_t kLow = kBias == 0 ? 0xe400e400u : 0xe408e408u, kHigh = kBias == 0 ? 0xd400d400u : 0xd480d480u;   // -1024, -1032; -64, -72
+  const uint32_t u = w >> 8;
+  c[0] = add_f16((w & 0x000f000fu) | 0x64006400u, kLow);
+  c[1] = add_f16((w & 0x00f000f0u) | 0x54005400u, kHigh);
+  c[2] = add_f16((u & 0x000f000fu) | 0x64006400u, kLow);
+  c[3] = add_f16((u & 0x00f000f0u) | 0x54005400u, kHigh);
+}
+
+// Shared-memory matrix descriptor of rows of 32 bytes, 32-byte swizzle (layout type 6): the 16-byte halves of
+// rows 4..7 of eight are swapped.
+__device__ __forceinline__ uint64_t sdesc_sw32(uint32_t saddr) {
+  return (sdesc_sw128(saddr, 16, 256) & ~(7ull << 61)) | (6ull << 61);
+}
+__device__ __forceinline__ int sw32(int row, int half) { return row * 32 + ((half ^ ((row >> 2) & 1)) << 4); }
+
+// The power of two that brings a value of this size to [2^to, 2^(to + 1)); 1 for zero, infinities and NaN.
+__device__ __forceinline__ int power_for(float size, int to) {
+  const int e = (int)(__float_as_uint(size) >> 23) & 255;
+  return size == 0.0f || e == 255 ? 0 : min(max(to + 127 - e, -126), 126);
+}
+__device__ __forceinline__ float power(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+
+// x in three float16 pieces.
+__device__ __forceinline__ void pieces(float x, float (&y)[3]) {
 #pragma unroll
-  for (int e = 0; e < 16; ++e) {
-    const float4 k = params[e];
-    unpack2(fma2(pack2(s[2 * e], s[2 * e + 1]), pack2(k.x, k.y), mul2(pack2(k.z, k.w), qsum2)), s[2 * e], s[2 * e + 1]);
+  for (int e = 0; e < 3; ++e) {
+    y[e] = __half2float(__float2half_rn(x));
+    x -= y[e];
   }
 }
 
-// P of 32 tokens: p = 2^(s + off), its sum, sum(p x_v), and p s_v in pieces to TMEM.
-// Without kWhole, bit e of `on` says whether token e is seen: a hidden one's parameters may be anything.
-template <int kP, bool kWhole>
-__device__ __forceinline__ void exp_chunk(float (&s)[32], float off, const float4* params, uint32_t on, uint64_t& sum2,
-                                          uint64_t& z2, uint32_t to) {
-  uint32_t pk[kP][16];
-  const uint64_t off2 = pack2(off, off);
+// P of 32 tokens: p = 2^(s c2 + off), its sum, and in float16 to TMEM.
+__device__ __forceinline__ void exp_chunk(const float (&s)[32], uint64_t c22, uint64_t off2, uint64_t (&sum2)[2], uint32_t to) {
+  uint32_t pk[16];
 #pragma unroll
   for (int g = 0; g < 8; ++g) {   // four tokens: pairs 0 2 and 1 3
-    float ps[4];
+    float x[4];
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      const float4 v = params[2 * g + e];
-      const int t = 4 * g + 2 * e;
-      float x, y;
-      unpack2(add2(pack2(s[t], s[t + 1]), off2), x, y);
-      x = ex2(x);
-      y = ex2(y);
-      const uint64_t p2 = pack2(x, y);
-      sum2 = add2(sum2, p2);
-      if (kWhole) {
-        z2 = fma2(p2, pack2(v.z, v.w), z2);
-        unpack2(mul2(p2, pack2(v.x, v.y)), ps[2 * e], ps[2 * e + 1]);
-      } else {
-        const bool a = (on >> t) & 1u, b = (on >> (t + 1)) & 1u;
-        z2 = fma2(p2, pack2(a ? v.z : 0.0f, b ? v.w : 0.0f), z2);
-        unpack2(mul2(p2, pack2(a ? v.x : 0.0f, b ? v.y : 0.0f)), ps[2 * e], ps[2 * e + 1]);
-      }
+      unpack2(fma2(pack2(s[4 * g + 2 * e], s[4 * g + 2 * e + 1]), c22, off2), x[2 * e], x[2 * e + 1]);
+      x[2 * e] = ex2(x[2 * e]);
+      x[2 * e + 1] = ex2(x[2 * e + 1]);
+      sum2[e] = add2(sum2[e], pack2(x[2 * e], x[2 * e + 1]));
     }
-#pragma unroll
-    for (int q = 0; q < kP; ++q) {
-      const uint32_t lo = pack_bf16(ps[0], ps[2]), hi = pack_bf16(ps[1], ps[3]);
-      pk[q][2 * g] = lo;
-      pk[q][2 * g + 1] = hi;
-      if (q + 1 < kP) {
-        ps[0] -= __uint_as_float(lo << 16);
-        ps[2] -= __uint_as_float(lo & 0xffff0000u);
-        ps[1] -= __uint_as_float(hi << 16);
-        ps[3] -= __uint_as_float(hi & 0xffff0000u);
-      }
-    }
+    pk[2 * g] = pack_f16(x[0], x[2]);
+    pk[2 * g + 1] = pack_f16(x[1], x[3]);
   }
-#pragma unroll
-  for (int q = 0; q < kP; ++q) tmem_st16(to + q * (kTokens / 2), pk[q]);
+  tmem_st16(to, pk);
 }
 
 __device__ __forceinline__ float max32(const float (&s)[32]) {
   float t[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-  for (int e = 4; e < 32; ++e) t[e & 3] = fmaxf(t[e & 3], s[e]);
-  return fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
+  for (int e = 4; e < 28; e += 8)
+#pragma unroll
+    for (int x = 0; x < 4; ++x) t[x] = max3(t[x], s[e + 2 * x], s[e + 2 * x + 1]);
+  return fmaxf(max3(t[0], t[1], s[28]), max3(max3(t[2], t[3], s[29]), s[30], s[31]));
 }
 
 template <int DT, int DP>
 __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_tc_kernel(const __grid_constant__ PrefixParams p) {
-  using L = PrefixLayout<DT, DP>;
+  using L = PrefixLayout<DP>;
   using T = typename Elem<DT>::T;
-  constexpr int kQ = L::kQ, kKStages = L::kKStages, kVStages = L::kVStages;
+  constexpr int kStages = L::kStages;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* kfull = reinterpret_cast<uint64_t*>(smem + L::kBars);
-  uint64_t* kempty = kfull + kKStages;
-  uint64_t* vfull = kempty + kKStages;
-  uint64_t* vempty = vfull + kVStages;
-  uint64_t* sfull = vempty + kVStages;   // [row tile][score buffer]
+  uint64_t* kempty = kfull + kStages;
+  uint64_t* vfull = kempty + kStages;
+  uint64_t* vempty = vfull + kStages;
+  uint64_t* rfull = vempty + kStages;
+  uint64_t* rempty = rfull + L::kRawStages;
+  uint64_t* sfull = rempty + L::kRawStages;   // [row tile][score buffer]
   uint64_t* pfull = sfull + 4;           // likewise
   uint64_t* pvdone = pfull + 4;          // [row tile]: a P V has ended
   uint64_t* drain = pvdone + 2;          // [row tile]: every product has
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 2);
   int* abort_word = reinterpret_cast<int*>(tmem_slot + 1);
   int* range = abort_word + 2;           // least and largest position of the CTA's rows
+  uint32_t* size = reinterpret_cast<uint32_t*>(range + 2);   // bits of the largest of its keys and values, whether pages are bad
 
   const Kv4AttendArgs& a = p.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -212,13 +274,15 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_tc_kernel(const __gr
   const int group = a.heads / a.c.heads;
   const int live = p.rows - row0 > kTileRows ? 2 : 1;   // row tiles with rows
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kKStages; ++s) {
+    for (int s = 0; s < kStages; ++s) {
       mbar_init(&kfull[s], kDecoders / 32);
       mbar_init(&kempty[s], live);
-    }
-    for (int s = 0; s < kVStages; ++s) {
       mbar_init(&vfull[s], kDecoders / 32);
       mbar_init(&vempty[s], live);
+    }
+    for (int s = 0; s < L::kRawStages; ++s) {
+      mbar_init(&rfull[s], 1);
+      mbar_init(&rempty[s], 2 * kDecoders / 32);
     }
     for (int i = 0; i < 4; ++i) {
       mbar_init(&sfull[i], 1);
@@ -231,10 +295,11 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_tc_kernel(const __gr
     abort_word[0] = abort_word[1] = 0;
     range[0] = 2147483647;
     range[1] = -1;
+    size[0] = size[1] = size[2] = 0;
     fence_mbar_init();
     fence_proxy_async_smem();
   }
-  if (warp == 12) {
+  if (warp == kIssuer) {
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
   }
@@ -258,42 +323,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_tc_kernel(const __gr
       atomicMax(&range[1], most);
     }
   }
-  // Q: eight columns at a time, in the order 0 4 1 5 2 6 3 7
-  for (int x = threadIdx.x; x < live * kTileRows * (DP / 8); x += kPrefixThreads) {
-    const int r = x / (DP / 8), c8 = x - r * (DP / 8), at = row0 + r;
-    float v[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = 0.0f;
-    if (at < p.rows) {
-      const int y = at / group, q = y / a.n;
-      const T* from = static_cast<const T*>(a.q) + q * a.q_r + (y - q * a.n) * a.q_n + (int64_t)(hk * group + at - y * group) * a.q_h + c8 * 8;
-      if (p.vec_q && c8 * 8 + 8 <= a.c.d) {
-        load8(v, from);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (c8 * 8 + e < a.c.d) v[e] = to_f32(from[e]);
-      }
-    }
-    uint8_t* to = smem + (r / kTileRows) * kQ * L::kQPiece + (c8 >> 3) * (kTileRows * 128) + (r % kTileRows) * 128 +
-                  (((c8 & 7) ^ (r & 7)) << 4);
-#pragma unroll
-    for (int q = 0; q < kQ; ++q) {
-      uint4 w;
-      w.x = pack_bf16(v[0], v[4]);
-      w.y = pack_bf16(v[1], v[5]);
-      w.z = pack_bf16(v[2], v[6]);
-      w.w = pack_bf16(v[3], v[7]);
-      *reinterpret_cast<uint4*>(to + q * L::kQPiece) = w;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] -= __bfloat162float(__float2bfloat16_rn(v[e]));
-    }
-  }
-  fence_proxy_async_smem();
-  tc_fence_before();
   __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
   // the visible blocks of 16 tokens, and this part's tiles of four
   const int p_lo = range[0], p_hi = range[1];
   const int window = (int)min(a.window, (int64_t)2147483647), sinks = (int)min(a.sinks, (int64_t)2147483647);
@@ -304,40 +334,141 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_tc_kernel(const __gr
   const int blocks = sink_blocks + max(win_end - win_begin, 0);
   const int all = (blocks + 3) >> 2;
   const int first = (int)((int64_t)all * part / parts), tiles = (int)((int64_t)all * (part + 1) / parts) - first;
+  auto token_of = [&](int v) { return (v < sink_blocks ? v : win_begin + v - sink_blocks) << 4; };
+  const int64_t cell0 = (int64_t)hk << a.c.page_shift;
+  const int64_t page_step = (int64_t)a.c.heads << a.c.page_shift;
+  const int page_mask = (1 << a.c.page_shift) - 1;
+  // Q: eight columns at a time, the DP / 8 lanes of a row together; loads first, all on their way at once
+  constexpr int kQLoads = (kSoftmax * (DP / 8) + kPrefixThreads - 1) / kPrefixThreads;
+  uint4 q_raw[kQLoads];
+#pragma unroll
+  for (int i = 0; i < kQLoads; ++i) {
+    const int x = i * kPrefixThreads + (int)threadIdx.x, r = x / (DP / 8), c8 = x - r * (DP / 8), at = row0 + r;
+    q_raw[i] = make_uint4(0, 0, 0, 0);
+    if (r < kSoftmax && at < p.rows) {
+      const int y = at / group, q = y / a.n;
+      const T* from = static_cast<const T*>(a.q) + q * a.q_r + (y - q * a.n) * a.q_n + (int64_t)(hk * group + at - y * group) * a.q_h + c8 * 8;
+      if (p.vec_q && c8 * 8 + 8 <= a.c.d) {
+        q_raw[i] = *reinterpret_cast<const uint4*>(from);
+      } else {
+        union {
+          uint4 w;
+          T e[8];
+        } u;
+        u.w = make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (c8 * 8 + e < a.c.d) u.e[e] = from[e];
+        q_raw[i] = u.w;
+      }
+    }
+  }
+  // the largest of the part's keys and values
+  {
+    float k_size = 0.0f, v_size = 0.0f;
+    bool bad = false;
+    const int end = min((first + tiles) * 4, blocks) * 16;
+#pragma unroll 4
+    for (int x = first * kTokens + (int)threadIdx.x; x < end; x += kPrefixThreads) {
+      const int token = token_of(x >> 4) + (x & 15), page = __ldg(a.prefix_table + (token >> a.c.page_shift));
+      const bool out = page < 0 || page >= a.c.pages;
+      if (out) {
+        report(a.status, kBadPage, page);
+        bad = true;
+      }
+      const int64_t cell = (out ? 0 : page) * page_step + cell0 + (token & page_mask);
+      const bool in = !out && token < bound;
+      const float2 k = params(__ldg(reinterpret_cast<const uint32_t*>(a.c.k_params) + cell));
+      const float2 v = params(__ldg(reinterpret_cast<const uint32_t*>(a.c.v_params) + cell));
+      const float ks = fmaxf(8.0f * fabsf(k.x), fabsf(fmaf(8.0f, k.x, k.y))), vs = fmaxf(fabsf(v.y), fabsf(fmaf(15.0f, v.x, v.y)));
+      if (in && ks < INFINITY) k_size = fmaxf(k_size, ks);
+      if (in && vs < INFINITY) v_size = fmaxf(v_size, vs);
+    }
+    const uint32_t k_bits = __reduce_max_sync(0xffffffffu, __float_as_uint(k_size));
+    const uint32_t v_bits = __reduce_max_sync(0xffffffffu, __float_as_uint(v_size));
+    bad = __any_sync(0xffffffffu, bad);
+    if (lane == 0) {
+      atomicMax(&size[0], k_bits);
+      atomicMax(&size[1], v_bits);
+      if (bad) atomicOr(&size[2], 1u);
+    }
+  }
+  // Q in the order 0 4 1 5 2 6 3 7, times the row's power; behind it the sums' pieces, which meet the
+  // offsets' as 1 1 1 2 2 3
+  const float sign = a.scale < 0.0f ? -1.0f : 1.0f;
+#pragma unroll
+  for (int i = 0; i < kQLoads; ++i) {
+    const int x = i * kPrefixThreads + (int)threadIdx.x, r = x / (DP / 8), c8 = x - r * (DP / 8);
+    if (x - lane >= kSoftmax * (DP / 8)) break;   // (whole warps)
+    union {
+      uint4 w;
+      T e[8];
+    } u;
+    u.w = q_raw[i];
+    float v[8], top = 0.0f, sum = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      v[e] = to_f32(u.e[e]);
+      top = fmaxf(top, fabsf(v[e]));
+    }
+#pragma unroll
+    for (int d = 1; d < DP / 8; d *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+    const int e2 = power_for(top, 7);
+    const float f = power(e2) * sign;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      v[e] *= f;
+      sum += v[e];
+    }
+#pragma unroll
+    for (int d = 1; d < DP / 8; d *= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    const int t = r / kTileRows, rt = r % kTileRows;
+    *reinterpret_cast<uint4*>(smem + t * L::kQ + (c8 >> 3) * (kTileRows * 128) + rt * 128 + (((c8 & 7) ^ (rt & 7)) << 4)) =
+        make_uint4(pack_f16(v[0], v[4]), pack_f16(v[1], v[5]), pack_f16(v[2], v[6]), pack_f16(v[3], v[7]));
+    if (c8 < 2) {
+      float y[3];
+      pieces(sum, y);
+      *reinterpret_cast<uint4*>(smem + L::kSums + t * L::kQSum + sw32(rt, c8)) =
+          c8 == 0 ? make_uint4(pack_f16(y[0], y[1]), pack_f16(y[2], y[0]), pack_f16(y[1], y[0]), 0) : make_uint4(0, 0, 0, 0);
+      if (c8 == 0) reinterpret_cast<int*>(smem + L::kPowers)[r] = e2;
+    }
+  }
+  // of the offsets' 16 columns the last eight stay zero
+  for (int x = threadIdx.x; x < kStages * kTokens; x += kPrefixThreads)
+    *reinterpret_cast<uint4*>(smem + L::kOffsets + (x / kTokens) * L::kKOff + sw32(x % kTokens, 1)) = make_uint4(0, 0, 0, 0);
+  fence_proxy_async_smem();
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const int k_power = power_for(__uint_as_float(size[0]), 9), v_power = power_for(__uint_as_float(size[1]), 9);
   const Abort ab{abort_word, a.status, p.wait_ns};
 
   if (threadIdx.x < kSoftmax) {
     // ------------------------------------------------------------ softmax rows
+    more_registers<kSoftmaxRegs>();
     const int t = warp >> 2;
     if (t < live) {
       const uint32_t at = (uint32_t)((warp & 3) * 32) << 16;
       const uint32_t tO = tmem + 256 + t * 128 + at;
-      float qsum = 0.0f;
-      {
-        const int r = threadIdx.x % kTileRows;
-#pragma unroll 1
-        for (int x = 0; x < kQ * (DP / 8); ++x) {
-          const int q = x / (DP / 8), c8 = x - q * (DP / 8);
-          const uint4 w = *reinterpret_cast<const uint4*>(smem + (t * kQ + q) * L::kQPiece + (c8 >> 3) * (kTileRows * 128) +
-                                                          r * 128 + (((c8 & 7) ^ (r & 7)) << 4));
-          const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-          for (int e = 0; e < 4; ++e) qsum += __uint_as_float(ws[e] << 16) + __uint_as_float(ws[e] & 0xffff0000u);
-        }
-      }
-      const uint64_t qsum2 = pack2(qsum, qsum);
-      float m = -INFINITY, l = 0.0f, z = 0.0f;
+      const int q_power = reinterpret_cast<const int*>(smem + L::kPowers)[threadIdx.x];
+      // scores in base 2 from the products; the powers one after the other, since their product may leave the range
+      // (0, of a scale of 0, would make NaN of a hidden score: the least that is none)
+      const float c2s = fabsf(a.scale) * 1.4426950408889634f * power(-q_power) * power(-k_power), c2 = c2s == 0.0f ? 1.17549435e-38f : c2s;
+      const uint64_t c22 = pack2(c2, c2);
+      const bool bad = size[2] != 0;
+      float m = -INFINITY, l = 0.0f;
       bool ok = true;
 #pragma unroll 1
       for (int j = 0; j < tiles; ++j) {
-        const int buf = j & 1, vs = j % kVStages;
-        ok = mbar_wait_warp_lazy(&vfull[vs], (j / kVStages) & 1, ab, kErrV);
-        if (ok) ok = mbar_wait_warp_lazy(&sfull[2 * t + buf], (j >> 1) & 1, ab, kErrS);
+        const int buf = j & 1;
+        // whether every row that sees anything sees all 64 tokens
+        const int v0 = (first + j) * 4, t0 = token_of(v0);
+        const bool whole = !bad && v0 + 4 <= blocks && token_of(v0 + 3) == t0 + 48 && t0 + kTokens <= bound &&
+                           (p_hi - t0 < window || t0 + kTokens <= sinks);
+        ok = mbar_wait_warp_lazy(&sfull[2 * t + buf], (j >> 1) & 1, ab, kErrS);
         if (!ok) break;
         tc_fence_after();
-        const float4* kp = reinterpret_cast<const float4*>(smem + L::kParams + vs * kTokens * 16);
-        const float4* vp = kp + kTokens / 2;
-        const int* info = reinterpret_cast<const int*>(smem + L::kInfo + vs * 32);
         const uint32_t ts = tmem + t * 128 + buf * kTokens + at;
         float s0[32], s1[32];
         tmem_ld32(ts, s0);
@@ -345,34 +476,33 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_tc_kernel(const __gr
         tmem_wait_ld();
         tie32(s0);
         tie32(s1);
-        finish_scores(s0, kp, qsum2);
-        finish_scores(s1, kp + 16, qsum2);
-        uint32_t on0 = 0xffffffffu, on1 = 0xffffffffu;
-        const bool whole = info[4] != 0;
         if (!whole) {
-          // 16 tokens from info[b] on: j < bound and (j > position - window or j < sinks); j <= position always
+          // the 16 tokens of a block: j < bound and (j > position - window or j < sinks); j <= position always
           auto seen = [&](int b) {
-            const int j0 = info[b];
-            if (j0 < 0) return 0u;
+            if (v0 + b >= blocks) return 0u;
+            const int j0 = token_of(v0 + b);
+            if (bad) {
+              const int page = __ldg(a.prefix_table + (j0 >> a.c.page_shift));
+              if (page < 0 || page >= a.c.pages) return 0u;
+            }
             const uint32_t near = position - j0 < window ? 0xffffu : 0xffffu & ~low_bits(position - j0 - window + 1);
             return low_bits(bound - j0) & (near | low_bits(sinks - j0)) & 0xffffu;
           };
-          on0 = seen(0) | seen(1) << 16;
-          on1 = seen(2) | seen(3) << 16;
+          const uint32_t on0 = seen(0) | seen(1) << 16, on1 = seen(2) | seen(3) << 16;
 #pragma unroll
           for (int e = 0; e < 32; ++e) {
             s0[e] = (on0 >> e) & 1u ? s0[e] : -INFINITY;
             s1[e] = (on1 >> e) & 1u ? s1[e] : -INFINITY;
           }
         }
-        const float top = fmaxf(max32(s0), max32(s1));
+        const float raw = fmaxf(max32(s0), max32(s1));
+        const float top = raw * c2;
         const bool move = top > m + kMove;
         if (__any_sync(0xffffffffu, move)) {
           const float to = move ? top : m;
           const float alpha = move ? ex2(m - to) : 1.0f;   // m = -inf: 0
           m = to;
           l *= alpha;
-          z *= alpha;
           if (j > 0) {   // the product of the tile before may still run (that of the one before it ended before S(j))
             ok = mbar_wait_warp_lazy(&pvdone[t], (j - 1) & 1, ab, kErrO);
             if (!ok) break;
@@ -380,34 +510,30 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_tc_kernel(const __gr
             scale_row(tO, DP, alpha);
           }
         }
-        const float off = kShift - (m == -INFINITY ? 0.0f : m);
-        uint64_t sum2 = 0, z2 = 0;
-        if (whole) {
-          exp_chunk<kQ, true>(s0, off, vp, on0, sum2, z2, ts);
-          exp_chunk<kQ, true>(s1, off, vp + 16, on1, sum2, z2, ts + 16);
-        } else {
-          exp_chunk<kQ, false>(s0, off, vp, on0, sum2, z2, ts);
-          exp_chunk<kQ, false>(s1, off, vp + 16, on1, sum2, z2, ts + 16);
-        }
+        const float off = kShiftP - (m == -INFINITY ? 0.0f : m);
+        const uint64_t off2 = pack2(off, off);
+        uint64_t sum2[2] = {0, 0};
+        exp_chunk(s0, c22, off2, sum2, ts);
+        exp_chunk(s1, c22, off2, sum2, ts + 16);
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&pfull[2 * t + buf]);
-        float x, y;
-        unpack2(sum2, x, y);
-        l += x + y;
-        unpack2(z2, x, y);
-        z += x + y;
+        float x0, x1, x2, x3;
+        unpack2(sum2[0], x0, x1);
+        unpack2(sum2[1], x2, x3);
+        l += (x0 + x1) + (x2 + x3);
       }
       if (ok && tiles > 0) {
         // not pvdone: P V of the last tile but one may still run too, and a parity tells only neighbours apart
         ok = mbar_wait_warp_lazy(&drain[t], 0, ab, kErrO);
         tc_fence_after();
       }
-      // this part's sums: [part][key head][columns / 4][row][4]
+      // this part's sums, as kTail's own p has them: [part][key head][columns / 4][row][4]
       const int64_t of = (int64_t)part * a.c.heads + hk;
-      const bool some = ok && tiles > 0 && position >= 0 && m != -INFINITY;
-      if (row < p.rows) a.part_ml[of * p.rows + row] = some || (position >= 0 && !(l == 0.0f)) ? make_float2(m, l) : make_float2(-INFINITY, 0.0f);
+      const bool seen = ok && tiles > 0 && position >= 0, some = seen && m != -INFINITY;
+      const float f = power((int)(kShift - kShiftP)), fo = f * power(-v_power);
+      if (row < p.rows) a.part_ml[of * p.rows + row] = seen ? make_float2(m, l * f) : make_float2(-INFINITY, 0.0f);
 #pragma unroll 1
       for (int c = 0; c < DP; c += 16) {
         float o[16];
@@ -420,217 +546,260 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_tc_kernel(const __gr
         for (int e = 0; e < 16; e += 4)
           if (row < p.rows)
             *reinterpret_cast<float4*>(a.part_o + ((of * (DP / 4) + (c + e) / 4) * p.rows + row) * 4) =
-                some ? make_float4(o[e] + z, o[e + 1] + z, o[e + 2] + z, o[e + 3] + z) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                some ? make_float4(o[e] * fo, o[e + 1] * fo, o[e + 2] * fo, o[e + 3] * fo) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
       }
       tc_fence_before();
     }
-  } else if (threadIdx.x < kSoftmax + kDecoders) {
+  } else if (warp < kIssuer) {
     // ------------------------------------------------------------ codes to tiles
-    constexpr int kPieces = DP / 32;                               // 16-byte pieces of a key row
-    constexpr int kKLoads = (kTokens * kPieces + kDecoders - 1) / kDecoders;
-    const int d = threadIdx.x - kSoftmax;
-    const int v_chunk = d & 7, v_quad = d >> 3;                    // 8 tokens, 8 columns (quad < DP / 8)
-    const int64_t cell0 = (int64_t)hk << a.c.page_shift;
-    const int64_t page_step = (int64_t)a.c.heads << a.c.page_shift;
-    const int page_mask = (1 << a.c.page_shift) - 1;
-    auto token_of = [&](int v) { return (v < sink_blocks ? v : win_begin + v - sink_blocks) << 4; };
-    const float sc = a.scale * 1.4426950408889634f;
-    // first token (-1: none) and page of 32 blocks, one a lane: eight tiles
-    int token_l = -1, page_l = 0;
-    auto fetch = [&](int j) {
-      const int v = (first + j) * 4 + lane;
-      token_l = -1;
-      page_l = 0;
-      if (v < blocks && lane < (tiles - j) * 4) {
-        const int token = token_of(v), page = __ldg(a.prefix_table + (token >> a.c.page_shift));
-        if (page < 0 || page >= a.c.pages) {
-          if (d < 32) report(a.status, kBadPage, page);
-        } else {
-          token_l = token;
-          page_l = page;
-        }
-      }
-    };
-    struct Raw {
-      uint4 k[kKLoads], v[2];
-      uint32_t kp, vp;
-      int block;     // lane b < 4: first token of block b
-    };
-    auto load = [&](Raw& x, int j) {
-      if ((j & 7) == 0) fetch(j);
-      const int b0 = (j & 7) * 4;
-      // a block's first cell in the cache, or that of any valid one where there is none
-      auto cell_of = [&](int b) {
-        const int token = __shfl_sync(0xffffffffu, token_l, b0 + b), page = __shfl_sync(0xffffffffu, page_l, b0 + b);
-        return (int64_t)page * page_step + cell0 + (max(token, 0) & page_mask);
-      };
-      x.block = __shfl_sync(0xffffffffu, token_l, b0 + (lane & 3));
-#pragma unroll
-      for (int i = 0; i < kKLoads; ++i) {
-        const int u = i * kDecoders + d, token = (u / (8 * kPieces)) * 8 + (u & 7), piece = (u >> 3) % kPieces;
-        const int64_t cell = cell_of((token >> 4) & 3);
-        if (token < kTokens)
-          x.k[i] = __ldg(reinterpret_cast<const uint4*>(a.c.k_codes + (cell + (token & 15)) * (DP / 2)) + piece);
-      }
-      const int64_t vc = cell_of(v_chunk >> 1);
-      if (v_quad < DP / 8) {
-        const uint8_t* from = a.c.v_codes + (vc + (v_chunk & 1) * 8) * (DP / 2) + v_quad * 16;
-        x.v[0] = __ldg(reinterpret_cast<const uint4*>(from));
-        x.v[1] = __ldg(reinterpret_cast<const uint4*>(from + 4 * (DP / 2)));
-      }
-      const int64_t pc = cell_of((d >> 4) & 3) + (d & 15);
-      if (d < kTokens) {
-        x.kp = __ldg(reinterpret_cast<const uint32_t*>(a.c.k_params) + pc);
-        x.vp = __ldg(reinterpret_cast<const uint32_t*>(a.c.v_params) + pc);
-      }
-    };
+    fewer_registers<kDecoderRegs>();
+    const bool isv = warp >= (kSoftmax + kDecoders) / 32;
+    const int d = (threadIdx.x - kSoftmax) % kDecoders;
     bool ok = true;
-    auto put = [&](const Raw& x, int j) {
-      const int ks = j % kKStages, vs = j % kVStages;
-      if (j >= kKStages) ok = mbar_wait_warp_lazy(&kempty[ks], ((j / kKStages) - 1) & 1, ab, kErrEmpty);
-      if (!ok) return;
-      uint8_t* kt = smem + L::kKeys + ks * L::kK;
+    if (!isv) {
+      // keys: a thread takes 16 bytes (32 columns) of tokens; eight lanes are eight tokens, so that their
+      // stores fall into different banks
+      constexpr int kPieces = DP / 32;
+      constexpr int kLoads = (kTokens * kPieces + kDecoders - 1) / kDecoders;
+      const float f = power(k_power);
+#pragma unroll 1
+      for (int j = 0; j < tiles; ++j) {
+        const int s = j % kStages, rs = j % L::kRawStages;
+        ok = mbar_wait_warp_lazy(&rfull[rs], (j / L::kRawStages) & 1, ab, kErrRaw);
+        if (!ok) break;
+        const uint8_t* raw = smem + L::kRaws + rs * L::kRaw;
+        uint4 w[kLoads];
+        uint32_t kp[kLoads], vp[kLoads];
+        bool in[kLoads];
 #pragma unroll
-      for (int i = 0; i < kKLoads; ++i) {
-        const int u = i * kDecoders + d, token = (u / (8 * kPieces)) * 8 + (u & 7), piece = (u >> 3) % kPieces;
-        if (token < kTokens) {
-          const uint32_t ws[4] = {x.k[i].x, x.k[i].y, x.k[i].z, x.k[i].w};
+        for (int i = 0; i < kLoads; ++i) {
+          const int u = i * kDecoders + d, token = (u / (8 * kPieces)) * 8 + (u & 7), piece = (u >> 3) % kPieces;
+          if (token >= kTokens) continue;
+          w[i] = *reinterpret_cast<const uint4*>(raw + token * (DP / 2) + piece * 16);
+          kp[i] = *reinterpret_cast<const uint32_t*>(raw + L::kRawKp + token * 4);
+          vp[i] = *reinterpret_cast<const uint32_t*>(raw + L::kRawVp + token * 4);
+          const int block = *reinterpret_cast<const int*>(raw + L::kRawInfo + (token >> 4) * 4);
+          in[i] = block >= 0 && block + (token & 15) < bound;
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&rempty[rs]);
+        if (j >= kStages) ok = mbar_wait_warp_lazy(&kempty[s], ((j / kStages) - 1) & 1, ab, kErrEmpty);
+        if (!ok) break;
+        uint8_t* tile = smem + L::kKeys + s * L::kK;
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+          const int u = i * kDecoders + d, token = (u / (8 * kPieces)) * 8 + (u & 7), piece = (u >> 3) % kPieces;
+          if (token >= kTokens) continue;
+          const float2 k = params(in[i] ? kp[i] : 0u);
+          const uint32_t s2 = pack_f16(k.x * f, k.x * f);
+          const uint32_t ws[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+          uint8_t* to = tile + token * 128;
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const int c8 = piece * 4 + e;
-            uint4 w;
-            w.x = codes<0, -8>(ws[e]);
-            w.y = codes<1, -8>(ws[e]);
-            w.z = codes<2, -8>(ws[e]);
-            w.w = codes<3, -8>(ws[e]);
-            *reinterpret_cast<uint4*>(kt + (c8 >> 3) * (kTokens * 128) + token * 128 + (((c8 & 7) ^ (token & 7)) << 4)) = w;
+            uint32_t c[4];
+            codes16<8>(ws[e], c);
+            *reinterpret_cast<uint4*>(to + (c8 >> 3) * (kTokens * 128) + (((c8 & 7) ^ (token & 7)) << 4)) =
+                make_uint4(mul_f16(c[0], s2), mul_f16(c[1], s2), mul_f16(c[2], s2), mul_f16(c[3], s2));
+          }
+          if (piece == 0) {
+            const float2 v = params(in[i] ? vp[i] : 0u);
+            const bool fine = fabsf(v.x) + fabsf(v.y) < INFINITY;
+            float y[3];
+            pieces(fine ? fmaf(8.0f, k.x, k.y) * f : NAN, y);
+            *reinterpret_cast<uint4*>(smem + L::kOffsets + s * L::kKOff + sw32(token, 0)) =
+                make_uint4(pack_f16(y[0], y[0]), pack_f16(y[0], y[1]), pack_f16(y[1], y[2]), 0);
           }
         }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&kfull[s]);
       }
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&kfull[ks]);
-      if (j >= kVStages) ok = mbar_wait_warp_lazy(&vempty[vs], ((j / kVStages) - 1) & 1, ab, kErrEmpty);
-      if (!ok) return;
-      uint8_t* vt = smem + L::kValues + vs * L::kV;
-      if (v_quad < DP / 8) {
-        const uint32_t w0[4] = {x.v[0].x, x.v[0].y, x.v[0].z, x.v[0].w}, w1[4] = {x.v[1].x, x.v[1].y, x.v[1].z, x.v[1].w};
-#pragma unroll
-        for (int b = 0; b < 4; ++b) {
-          uint8_t* to = vt + (v_quad * 8 + 2 * b) * 128;
-          *reinterpret_cast<uint4*>(to + ((v_chunk ^ (2 * b)) << 4)) =
-              make_uint4(codes<0, -8>(w0[b]), codes<2, -8>(w0[b]), codes<0, -8>(w1[b]), codes<2, -8>(w1[b]));
-          *reinterpret_cast<uint4*>(to + 128 + ((v_chunk ^ (2 * b + 1)) << 4)) =
-              make_uint4(codes<1, -8>(w0[b]), codes<3, -8>(w0[b]), codes<1, -8>(w1[b]), codes<3, -8>(w1[b]));
-        }
-      }
-      const int mine = __shfl_sync(0xffffffffu, x.block, (d >> 4) & 3);
-      if (d < kTokens) {
-        const bool in = mine >= 0 && mine + (d & 15) < bound;
-        const float2 k = params(in ? x.kp : 0u), v = params(in ? x.vp : 0u);
-        float* kp = reinterpret_cast<float*>(smem + L::kParams + vs * kTokens * 16) + (d >> 1) * 4 + (d & 1);
-        kp[0] = k.x * sc;
-        kp[2] = fmaf(8.0f, k.x, k.y) * sc;
-        float* vp = kp + 2 * kTokens;
-        vp[0] = v.x;
-        vp[2] = fmaf(8.0f, v.x, v.y);
-      }
-      // whether every row that sees anything sees all 64 tokens
-      const bool whole = __all_sync(0xffffffffu, x.block >= 0 && x.block + 16 <= bound && (p_hi - x.block < window || x.block + 16 <= sinks));
-      if (d < 4) reinterpret_cast<int*>(smem + L::kInfo + vs * 32)[d] = x.block;
-      if (d == 4) reinterpret_cast<int*>(smem + L::kInfo + vs * 32)[4] = whole;
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&vfull[vs]);
-    };
-    Raw x, y;
-    if (tiles > 0) load(x, 0);
-    if (tiles > 1) load(y, 1);
+    } else {
+      // values: a thread takes 8 columns of 8 tokens; eight lanes are the eight such runs of a tile
+      const int chunk = d & 7, quad = d >> 3;   // quad < DP / 8
+      const float f = power(v_power);
 #pragma unroll 1
-    for (int j = 0; j < tiles && ok; j += 2) {
-      put(x, j);
-      if (j + 2 < tiles) load(x, j + 2);
-      if (j + 1 < tiles && ok) {
-        put(y, j + 1);
-        if (j + 3 < tiles) load(y, j + 3);
+      for (int j = 0; j < tiles; ++j) {
+        const int s = j % kStages, rs = j % L::kRawStages;
+        ok = mbar_wait_warp_lazy(&rfull[rs], (j / L::kRawStages) & 1, ab, kErrRaw);
+        if (!ok) break;
+        const uint8_t* raw = smem + L::kRaws + rs * L::kRaw;
+        uint4 w[2], ps[2];
+        int left = 0;   // how many of the eight are there
+        if (quad < DP / 8) {
+          w[0] = *reinterpret_cast<const uint4*>(raw + L::kRawV + chunk * L::kChunkPitch + quad * 16);
+          w[1] = *reinterpret_cast<const uint4*>(raw + L::kRawV + chunk * L::kChunkPitch + 2 * DP + quad * 16);
+          ps[0] = *reinterpret_cast<const uint4*>(raw + L::kRawVp + chunk * 32);
+          ps[1] = *reinterpret_cast<const uint4*>(raw + L::kRawVp + chunk * 32 + 16);
+          const int block = *reinterpret_cast<const int*>(raw + L::kRawInfo + (chunk >> 1) * 4);
+          left = block < 0 ? 0 : bound - block - (chunk & 1) * 8;
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&rempty[rs]);
+        if (j >= kStages) ok = mbar_wait_warp_lazy(&vempty[s], ((j / kStages) - 1) & 1, ab, kErrEmpty);
+        if (!ok) break;
+        if (quad < DP / 8) {
+          uint32_t s2[4], l2[4];   // tokens 0 2, 1 3, 4 6, 5 7
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const uint32_t p4[4] = {ps[h].x, ps[h].y, ps[h].z, ps[h].w};
+            float2 v[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              v[e] = params(4 * h + e < left ? p4[e] : 0u);
+              if (!(fabsf(v[e].x) + fabsf(v[e].y) < INFINITY)) v[e] = make_float2(0.0f, 0.0f);   // its key is NaN
+            }
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              s2[2 * h + e] = pack_f16(v[e].x * f, v[e + 2].x * f);
+              l2[2 * h + e] = pack_f16(v[e].y * f, v[e + 2].y * f);
+            }
+          }
+          const uint32_t w0[4] = {w[0].x, w[0].y, w[0].z, w[0].w}, w1[4] = {w[1].x, w[1].y, w[1].z, w[1].w};
+          uint8_t* tile = smem + L::kValues + s * L::kV + quad * 8 * 128;
+#pragma unroll
+          for (int b = 0; b < 4; ++b) {
+            uint32_t c[4], e[4];
+            codes16<0>(w0[b], c);
+            codes16<0>(w1[b], e);
+            *reinterpret_cast<uint4*>(tile + 2 * b * 128 + ((chunk ^ (2 * b)) << 4)) =
+                make_uint4(fma_f16(c[0], s2[0], l2[0]), fma_f16(c[2], s2[1], l2[1]), fma_f16(e[0], s2[2], l2[2]),
+                           fma_f16(e[2], s2[3], l2[3]));
+            *reinterpret_cast<uint4*>(tile + (2 * b + 1) * 128 + ((chunk ^ (2 * b + 1)) << 4)) =
+                make_uint4(fma_f16(c[1], s2[0], l2[0]), fma_f16(c[3], s2[1], l2[1]), fma_f16(e[1], s2[2], l2[2]),
+                           fma_f16(e[3], s2[3], l2[3]));
+          }
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&vfull[s]);
       }
     }
   } else {
-    // ------------------------------------------------------------ products of row tile t
-    const int t = warp - 12;
-    if (t < live) {
-      constexpr uint32_t id_s = idesc_f16(kTileRows, kTokens, true, false, false);
-      constexpr uint32_t id_pv = idesc_f16(kTileRows, DP, true, false, false);
-      const uint32_t q_smem = smem_u32(smem) + t * kQ * L::kQPiece, k_smem = smem_u32(smem + L::kKeys), v_smem = smem_u32(smem + L::kValues);
-      const uint32_t tS = tmem + t * 128, tO = tmem + 256 + t * 128;
-      auto scores = [&](int j) {   // by one lane
-        const uint64_t kd = sdesc_sw128(k_smem + (j % kKStages) * L::kK, 16, 1024);
-#pragma unroll
-        for (int q = 0; q < kQ; ++q) {
-          const uint64_t qd = sdesc_sw128(q_smem + q * L::kQPiece, 16, 1024);
-#pragma unroll
-          for (int kk = 0; kk < DP / 16; ++kk)
-            mma_f16_ss(tS + (j & 1) * kTokens, qd + (uint64_t)(((kk >> 2) * (kTileRows * 128) + (kk & 3) * 32) >> 4),
-                       kd + (uint64_t)(((kk >> 2) * (kTokens * 128) + (kk & 3) * 32) >> 4), id_s, q > 0 || kk > 0 ? 1u : 0u);
+    fewer_registers<kOtherRegs>();
+    if (warp == kLoader) {
+      // ---------------------------------------------------------- raw tiles
+      // of a tile lanes 0..3 bring a block's keys, 4..11 eight tokens' values, 12..15 and 16..19 a block's parameters
+      const int b = lane < 4 ? lane : lane < 12 ? (lane - 4) >> 1 : lane & 3;
+      int token_l = -1, page_l = 0;   // first token (-1: none) and page of 32 blocks, one a lane: eight tiles
+      int sent = 0;
+  #pragma unroll 1
+      for (int j = 0; j < tiles; ++j) {
+        const int rs = j % L::kRawStages;
+        if ((j & 7) == 0) {
+          const int v = (first + j) * 4 + lane;
+          token_l = -1;
+          page_l = 0;
+          if (v < blocks && lane < (tiles - j) * 4) {
+            const int token = token_of(v), page = __ldg(a.prefix_table + (token >> a.c.page_shift));
+            if (page >= 0 && page < a.c.pages) token_l = token, page_l = page;   // else reported above
+          }
         }
-        mma_commit(&sfull[2 * t + (j & 1)]);
-        mma_commit(&kempty[j % kKStages]);
-      };
-      bool ok = true;
-#pragma unroll 1
-      for (int j = 0; j < min(tiles, 2) && ok; ++j) {
-        ok = mbar_wait_warp_lazy(&kfull[j % kKStages], (j / kKStages) & 1, ab, kErrK);
-        if (!ok) break;
-        tc_fence_after();
-        if (elect_one()) scores(j);
+        const int token = __shfl_sync(0xffffffffu, token_l, (j & 7) * 4 + b), page = __shfl_sync(0xffffffffu, page_l, (j & 7) * 4 + b);
+        if (j >= L::kRawStages && !mbar_wait_warp_lazy(&rempty[rs], ((j / L::kRawStages) - 1) & 1, ab, kErrRaw)) break;
+        uint8_t* raw = smem + L::kRaws + rs * L::kRaw;
+        if (lane < 4) reinterpret_cast<int*>(raw + L::kRawInfo)[b] = token;
+        __syncwarp();
+        if (lane == 0) mbar_arrive_expect_tx(&rfull[rs], kTokens * DP + 2 * kTokens * 4);
+        __syncwarp();
+        // where there is no block, a valid one's bytes: nobody sees them
+        const int64_t cell = page * page_step + cell0 + (max(token, 0) & page_mask);
+        if (lane < 4)
+          bulk_load(raw + b * 16 * (DP / 2), a.c.k_codes + cell * (DP / 2), 16 * (DP / 2), &rfull[rs]);
+        else if (lane < 12)
+          bulk_load(raw + L::kRawV + (lane - 4) * L::kChunkPitch, a.c.v_codes + (cell + (lane & 1) * 8) * (DP / 2), L::kChunkBytes, &rfull[rs]);
+        else if (lane < 16)
+          bulk_load(raw + L::kRawKp + b * 64, a.c.k_params + 2 * cell, 64, &rfull[rs]);
+        else if (lane < 20)
+          bulk_load(raw + L::kRawVp + b * 64, a.c.v_params + 2 * cell, 64, &rfull[rs]);
+        sent = j + 1;
         __syncwarp();
       }
-#pragma unroll 1
-      for (int j = 0; j < tiles && ok; ++j) {
-        const int vs = j % kVStages;
-        ok = mbar_wait_warp_lazy(&vfull[vs], (j / kVStages) & 1, ab, kErrV);
-        if (ok) ok = mbar_wait_warp_lazy(&pfull[2 * t + (j & 1)], (j >> 1) & 1, ab, kErrP);
-        if (!ok) break;
-        tc_fence_after();
-        if (elect_one()) {
-          const uint64_t vd = sdesc_sw128(v_smem + vs * L::kV, 16, 1024);
-#pragma unroll
-          for (int q = kQ - 1; q >= 0; --q)
-#pragma unroll
-            for (int kk = 0; kk < kTokens / 16; ++kk)
-              mma_f16_ts(tO, tS + (j & 1) * kTokens + q * (kTokens / 2) + kk * 8, vd + (uint64_t)((kk * 32) >> 4), id_pv,
-                         j > 0 || q < kQ - 1 || kk > 0 ? 1u : 0u);
-          mma_commit(&pvdone[t]);
-          mma_commit(&vempty[vs]);
-        }
-        __syncwarp();
-        if (j + 2 < tiles) {
-          ok = mbar_wait_warp_lazy(&kfull[(j + 2) % kKStages], ((j + 2) / kKStages) & 1, ab, kErrK);
-          if (!ok) break;
-          tc_fence_after();
-          if (elect_one()) scores(j + 2);
-          __syncwarp();
-        }
-      }
-      if (elect_one()) mma_commit(&drain[t]);
-      const uint64_t t0 = globaltimer_ns();
-      while (!mbar_try_wait(&drain[t], 0)) {
-        if (globaltimer_ns() - t0 > 2000000000ull) {
-          if (a.status) atomicCAS(a.status, 0, kErrDrain);
-          break;
+      // never leave with copies in flight
+      for (int j = max(0, sent - L::kRawStages); j < sent; ++j) {
+        const uint64_t t0 = globaltimer_ns();
+        while (!mbar_try_wait(&rfull[j % L::kRawStages], (j / L::kRawStages) & 1)) {
+          if (globaltimer_ns() - t0 > 1000000000ull) {
+            if (a.status) atomicCAS(a.status, 0, kErrDrain);
+            break;
+          }
         }
       }
       __syncwarp();
+    } else if (warp < kLoader) {
+      // ---------------------------------------------------------- products of row tile t
+      const int t = warp - kIssuer;
+      if (t < live) {
+        constexpr uint32_t id_s = idesc_f16(kTileRows, kTokens, false, false, false);
+        constexpr uint32_t id_pv = idesc_f16(kTileRows, DP, false, false, false);
+        const uint32_t q_smem = smem_u32(smem) + t * L::kQ, k_smem = smem_u32(smem + L::kKeys), v_smem = smem_u32(smem + L::kValues);
+        const uint32_t sum_smem = smem_u32(smem + L::kSums + t * L::kQSum), off_smem = smem_u32(smem + L::kOffsets);
+        const uint32_t tS = tmem + t * 128, tO = tmem + 256 + t * 128;
+        auto scores = [&](int j) {   // by one lane
+          const uint64_t qd = sdesc_sw128(q_smem, 16, 1024), kd = sdesc_sw128(k_smem + (j % kStages) * L::kK, 16, 1024);
+          const uint32_t to = tS + (j & 1) * kTokens;
+          mma_f16_ss(to, sdesc_sw32(sum_smem), sdesc_sw32(off_smem + (j % kStages) * L::kKOff), id_s, 0u);
+  #pragma unroll
+          for (int kk = 0; kk < DP / 16; ++kk)
+            mma_f16_ss(to, qd + (uint64_t)(((kk >> 2) * (kTileRows * 128) + (kk & 3) * 32) >> 4),
+                       kd + (uint64_t)(((kk >> 2) * (kTokens * 128) + (kk & 3) * 32) >> 4), id_s, 1u);
+          mma_commit(&sfull[2 * t + (j & 1)]);
+          mma_commit(&kempty[j % kStages]);
+        };
+        bool ok = true;
+  #pragma unroll 1
+        for (int j = 0; j < min(tiles, 2) && ok; ++j) {
+          ok = mbar_wait_warp_lazy(&kfull[j], 0, ab, kErrK);
+          if (!ok) break;
+          tc_fence_after();
+          if (elect_one()) scores(j);
+          __syncwarp();
+        }
+  #pragma unroll 1
+        for (int j = 0; j < tiles && ok; ++j) {
+          const int vs = j % kStages;
+          ok = mbar_wait_warp_lazy(&vfull[vs], (j / kStages) & 1, ab, kErrV);
+          if (ok) ok = mbar_wait_warp_lazy(&pfull[2 * t + (j & 1)], (j >> 1) & 1, ab, kErrP);
+          if (!ok) break;
+          tc_fence_after();
+          if (elect_one()) {
+            const uint64_t vd = sdesc_sw128(v_smem + vs * L::kV, 16, 1024);
+  #pragma unroll
+            for (int kk = 0; kk < kTokens / 16; ++kk)
+              mma_f16_ts(tO, tS + (j & 1) * kTokens + kk * 8, vd + (uint64_t)((kk * 32) >> 4), id_pv, j > 0 || kk > 0 ? 1u : 0u);
+            mma_commit(&pvdone[t]);
+            mma_commit(&vempty[vs]);
+          }
+          __syncwarp();
+          if (j + 2 < tiles) {
+            ok = mbar_wait_warp_lazy(&kfull[(j + 2) % kStages], ((j + 2) / kStages) & 1, ab, kErrK);
+            if (!ok) break;
+            tc_fence_after();
+            if (elect_one()) scores(j + 2);
+            __syncwarp();
+          }
+        }
+        if (elect_one()) mma_commit(&drain[t]);
+        const uint64_t t0 = globaltimer_ns();
+        while (!mbar_try_wait(&drain[t], 0)) {
+          if (globaltimer_ns() - t0 > 2000000000ull) {
+            if (a.status) atomicCAS(a.status, 0, kErrDrain);
+            break;
+          }
+        }
+        __syncwarp();
+      }
     }
   }
   __syncthreads();
   tc_fence_after();
-  if (warp == 12) tmem_dealloc(tmem, 512);
+  if (warp == kIssuer) tmem_dealloc(tmem, 512);
 }
 
 template <int DT, int DP>
 int launch_prefix(const Kv4AttendArgs& a, int64_t rows, cudaStream_t s) {
-  using L = PrefixLayout<DT, DP>;
+  using L = PrefixLayout<DP>;
   auto kern = prefix_tc_kernel<DT, DP>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes);
   if (e != cudaSuccess) return set_error(SA_ERR_CUDA, "kv4 prefix smem attribute: %s", cudaGetErrorString(e));
