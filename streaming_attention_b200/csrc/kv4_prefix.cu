@@ -77,10 +77,8 @@ struct PrefixLayout {
   static constexpr int kStages = 3;
   // the 16 columns of the sums and of the offsets: rows of 32 bytes
   static constexpr int kQSum = kTileRows * 32, kKOff = kTokens * 32;
-  // a raw tile: keys, eight tokens' values (16 bytes on: their readers fall into different banks), parameters,
-  // its blocks' first tokens
-  static constexpr int kChunkBytes = 4 * DP, kChunkPitch = kChunkBytes + 16;
-  static constexpr int kRawV = kTokens * DP / 2, kRawKp = kRawV + 8 * kChunkPitch, kRawVp = kRawKp + kTokens * 4;
+  // a raw tile: keys, values, their parameters, and which of its blocks of 16 tokens are there
+  static constexpr int kRawV = kTokens * DP / 2, kRawKp = 2 * kRawV, kRawVp = kRawKp + kTokens * 4;
   static constexpr int kRawInfo = kRawVp + kTokens * 4, kRaw = kRawInfo + 16;
   static constexpr int kRawStages = 4;
   static constexpr int kKeys = kRowTiles * kQ;
@@ -88,7 +86,8 @@ struct PrefixLayout {
   static constexpr int kSums = kValues + kStages * kV;
   static constexpr int kOffsets = kSums + kRowTiles * kQSum;
   static constexpr int kPowers = kOffsets + kStages * kKOff;   // of the rows
-  static constexpr int kRaws = kPowers + kSoftmax * 4;
+  static constexpr int kRows = kPowers + kSoftmax * 4;         // where the rows of q start
+  static constexpr int kRaws = kRows + kSoftmax * 8;
   static constexpr int kBars = kRaws + kRawStages * kRaw;
   static constexpr int kBytes = kBars + (4 * kStages + 2 * kRawStages + 12) * 8 + 48 + 1024;
   static_assert(kBytes <= 227 * 1024, "shared memory");
@@ -311,11 +310,14 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_tc_kernel(const __gr
   int position = -1;
   const int row = row0 + (int)threadIdx.x;
   if (threadIdx.x < kSoftmax) {
+    int64_t start = -1;   // no row
     if (row < p.rows) {
       const int x = row / group, q = x / a.n;
+      start = q * a.q_r + (x - q * a.n) * a.q_n + (int64_t)(hk * group + row - x * group) * a.q_h;
       const int own = max(a.lengths[q], 0) - a.n + (x - q * a.n);   // only a request's own tokens ask
       if (own >= 0) position = (int)min((int64_t)length + own, (int64_t)2147483646);
     }
+    reinterpret_cast<int64_t*>(smem + L::kRows)[threadIdx.x] = start;
     const int least = __reduce_min_sync(0xffffffffu, position < 0 ? 2147483647 : position);
     const int most = __reduce_max_sync(0xffffffffu, position);
     if (lane == 0) {
@@ -324,17 +326,19 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_tc_kernel(const __gr
     }
   }
   __syncthreads();
-  // the visible blocks of 16 tokens, and this part's tiles of four
+  // the tiles of 64 tokens, from multiples of 64 on, that hold what rows see, and this part's of them
   const int p_lo = range[0], p_hi = range[1];
   const int window = (int)min(a.window, (int64_t)2147483647), sinks = (int)min(a.sinks, (int64_t)2147483647);
   KeyRanges kr{0, 0, 0};
   if (p_hi >= 0) kr = key_ranges(p_lo, p_hi, bound, a.window, a.sinks);
-  const int sink_blocks = (int)((kr.first + 15) >> 4);
-  const int win_begin = max((int)(kr.begin >> 4), sink_blocks), win_end = (int)((kr.end + 15) >> 4);
-  const int blocks = sink_blocks + max(win_end - win_begin, 0);
-  const int all = (blocks + 3) >> 2;
+  const int sink_tiles = (int)((kr.first + kTokens - 1) / kTokens);
+  const int win_tile = max((int)(kr.begin / kTokens), sink_tiles);
+  const int all = sink_tiles + max((int)((kr.end + kTokens - 1) / kTokens) - win_tile, 0);
   const int first = (int)((int64_t)all * part / parts), tiles = (int)((int64_t)all * (part + 1) / parts) - first;
-  auto token_of = [&](int v) { return (v < sink_blocks ? v : win_begin + v - sink_blocks) << 4; };
+  auto token_of = [&](int j) {   // of this part's tile j, the first
+    const int v = first + j;
+    return (v < sink_tiles ? v : win_tile + v - sink_tiles) * kTokens;
+  };
   const int64_t cell0 = (int64_t)hk << a.c.page_shift;
   const int64_t page_step = (int64_t)a.c.heads << a.c.page_shift;
   const int page_mask = (1 << a.c.page_shift) - 1;
@@ -343,11 +347,11 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_tc_kernel(const __gr
   uint4 q_raw[kQLoads];
 #pragma unroll
   for (int i = 0; i < kQLoads; ++i) {
-    const int x = i * kPrefixThreads + (int)threadIdx.x, r = x / (DP / 8), c8 = x - r * (DP / 8), at = row0 + r;
+    const int x = i * kPrefixThreads + (int)threadIdx.x, r = x / (DP / 8), c8 = x - r * (DP / 8);
     q_raw[i] = make_uint4(0, 0, 0, 0);
-    if (r < kSoftmax && at < p.rows) {
-      const int y = at / group, q = y / a.n;
-      const T* from = static_cast<const T*>(a.q) + q * a.q_r + (y - q * a.n) * a.q_n + (int64_t)(hk * group + at - y * group) * a.q_h + c8 * 8;
+    const int64_t start = r < kSoftmax ? reinterpret_cast<const int64_t*>(smem + L::kRows)[r] : -1;
+    if (start >= 0) {
+      const T* from = static_cast<const T*>(a.q) + start + c8 * 8;
       if (p.vec_q && c8 * 8 + 8 <= a.c.d) {
         q_raw[i] = *reinterpret_cast<const uint4*>(from);
       } else {
@@ -367,10 +371,10 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_tc_kernel(const __gr
   {
     float k_size = 0.0f, v_size = 0.0f;
     bool bad = false;
-    const int end = min((first + tiles) * 4, blocks) * 16;
 #pragma unroll 4
-    for (int x = first * kTokens + (int)threadIdx.x; x < end; x += kPrefixThreads) {
-      const int token = token_of(x >> 4) + (x & 15), page = __ldg(a.prefix_table + (token >> a.c.page_shift));
+    for (int x = threadIdx.x; x < tiles * kTokens; x += kPrefixThreads) {
+      const int token = token_of(x / kTokens) + x % kTokens;
+      const int page = token < bound ? __ldg(a.prefix_table + (token >> a.c.page_shift)) : 0;
       const bool out = page < 0 || page >= a.c.pages;
       if (out) {
         report(a.status, kBadPage, page);
@@ -399,7 +403,6 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_tc_kernel(const __gr
 #pragma unroll
   for (int i = 0; i < kQLoads; ++i) {
     const int x = i * kPrefixThreads + (int)threadIdx.x, r = x / (DP / 8), c8 = x - r * (DP / 8);
-    if (x - lane >= kSoftmax * (DP / 8)) break;   // (whole warps)
     union {
       uint4 w;
       T e[8];
@@ -423,6 +426,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_tc_kernel(const __gr
 #pragma unroll
     for (int d = 1; d < DP / 8; d *= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
     const int t = r / kTileRows, rt = r % kTileRows;
+    if (r >= kSoftmax) continue;
     *reinterpret_cast<uint4*>(smem + t * L::kQ + (c8 >> 3) * (kTileRows * 128) + rt * 128 + (((c8 & 7) ^ (rt & 7)) << 4)) =
         make_uint4(pack_f16(v[0], v[4]), pack_f16(v[1], v[5]), pack_f16(v[2], v[6]), pack_f16(v[3], v[7]));
     if (c8 < 2) {
@@ -463,9 +467,8 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_tc_kernel(const __gr
       for (int j = 0; j < tiles; ++j) {
         const int buf = j & 1;
         // whether every row that sees anything sees all 64 tokens
-        const int v0 = (first + j) * 4, t0 = token_of(v0);
-        const bool whole = !bad && v0 + 4 <= blocks && token_of(v0 + 3) == t0 + 48 && t0 + kTokens <= bound &&
-                           (p_hi - t0 < window || t0 + kTokens <= sinks);
+        const int t0 = token_of(j);
+        const bool whole = !bad && t0 + kTokens <= bound && (p_hi - t0 < window || t0 + kTokens <= sinks);
         ok = mbar_wait_warp_lazy(&sfull[2 * t + buf], (j >> 1) & 1, ab, kErrS);
         if (!ok) break;
         tc_fence_after();
@@ -477,18 +480,17 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_tc_kernel(const __gr
         tie32(s0);
         tie32(s1);
         if (!whole) {
-          // the 16 tokens of a block: j < bound and (j > position - window or j < sinks); j <= position always
-          auto seen = [&](int b) {
-            if (v0 + b >= blocks) return 0u;
-            const int j0 = token_of(v0 + b);
-            if (bad) {
-              const int page = __ldg(a.prefix_table + (j0 >> a.c.page_shift));
-              if (page < 0 || page >= a.c.pages) return 0u;
+          // token j: j < bound and (j > position - window or j < sinks); j <= position always
+          auto seen = [&](int j0) {
+            const uint32_t near = position - j0 < window ? 0xffffffffu : ~low_bits(position - j0 - window + 1);
+            uint32_t on = low_bits(bound - j0) & (near | low_bits(sinks - j0));
+            for (int b = 0; bad && b < 2; ++b) {   // a page that is not there
+              const int at = j0 + 16 * b, page = at < bound ? __ldg(a.prefix_table + (at >> a.c.page_shift)) : 0;
+              if (page < 0 || page >= a.c.pages) on &= 0xffff0000u >> (16 * b);
             }
-            const uint32_t near = position - j0 < window ? 0xffffu : 0xffffu & ~low_bits(position - j0 - window + 1);
-            return low_bits(bound - j0) & (near | low_bits(sinks - j0)) & 0xffffu;
+            return on;
           };
-          const uint32_t on0 = seen(0) | seen(1) << 16, on1 = seen(2) | seen(3) << 16;
+          const uint32_t on0 = seen(t0), on1 = seen(t0 + 32);
 #pragma unroll
           for (int e = 0; e < 32; ++e) {
             s0[e] = (on0 >> e) & 1u ? s0[e] : -INFINITY;
@@ -578,8 +580,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_tc_kernel(const __gr
           w[i] = *reinterpret_cast<const uint4*>(raw + token * (DP / 2) + piece * 16);
           kp[i] = *reinterpret_cast<const uint32_t*>(raw + L::kRawKp + token * 4);
           vp[i] = *reinterpret_cast<const uint32_t*>(raw + L::kRawVp + token * 4);
-          const int block = *reinterpret_cast<const int*>(raw + L::kRawInfo + (token >> 4) * 4);
-          in[i] = block >= 0 && block + (token & 15) < bound;
+          in[i] = (token & 15) < reinterpret_cast<const int*>(raw + L::kRawInfo)[token >> 4];
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&rempty[rs]);
@@ -617,7 +618,9 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_tc_kernel(const __gr
       }
     } else {
       // values: a thread takes 8 columns of 8 tokens; eight lanes are the eight such runs of a tile
-      const int chunk = d & 7, quad = d >> 3;   // quad < DP / 8
+      // (the columns turned by them, so that neither loads nor stores fall into one bank); quad < DP / 8
+      constexpr int kTurn = DP >= 64 ? 8 : 4;
+      const int chunk = d & 7, quad = ((d >> 3) & ~(kTurn - 1)) + (((d >> 3) + chunk) & (kTurn - 1));
       const float f = power(v_power);
 #pragma unroll 1
       for (int j = 0; j < tiles; ++j) {
@@ -628,12 +631,11 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_tc_kernel(const __gr
         uint4 w[2], ps[2];
         int left = 0;   // how many of the eight are there
         if (quad < DP / 8) {
-          w[0] = *reinterpret_cast<const uint4*>(raw + L::kRawV + chunk * L::kChunkPitch + quad * 16);
-          w[1] = *reinterpret_cast<const uint4*>(raw + L::kRawV + chunk * L::kChunkPitch + 2 * DP + quad * 16);
+          w[0] = *reinterpret_cast<const uint4*>(raw + L::kRawV + chunk * (4 * DP) + quad * 16);
+          w[1] = *reinterpret_cast<const uint4*>(raw + L::kRawV + chunk * (4 * DP) + 2 * DP + quad * 16);
           ps[0] = *reinterpret_cast<const uint4*>(raw + L::kRawVp + chunk * 32);
           ps[1] = *reinterpret_cast<const uint4*>(raw + L::kRawVp + chunk * 32 + 16);
-          const int block = *reinterpret_cast<const int*>(raw + L::kRawInfo + (chunk >> 1) * 4);
-          left = block < 0 ? 0 : bound - block - (chunk & 1) * 8;
+          left = reinterpret_cast<const int*>(raw + L::kRawInfo)[chunk >> 1] - (chunk & 1) * 8;
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&rempty[rs]);
@@ -680,39 +682,39 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_tc_kernel(const __gr
     fewer_registers<kOtherRegs>();
     if (warp == kLoader) {
       // ---------------------------------------------------------- raw tiles
-      // of a tile lanes 0..3 bring a block's keys, 4..11 eight tokens' values, 12..15 and 16..19 a block's parameters
-      const int b = lane < 4 ? lane : lane < 12 ? (lane - 4) >> 1 : lane & 3;
-      int token_l = -1, page_l = 0;   // first token (-1: none) and page of 32 blocks, one a lane: eight tiles
+      // a tile is one run of tokens in a page, or of two or four in pages of 32 and 16: a lane for each and each of
+      // keys, values and their parameters
+      const int runs = max(kTokens >> a.c.page_shift, 1), tokens = kTokens / runs;
+      const int what = lane / runs, run = lane - what * runs;
+      int page_l = 0;   // pages of 32 runs, one a lane: 32 / runs tiles
       int sent = 0;
-  #pragma unroll 1
+#pragma unroll 1
       for (int j = 0; j < tiles; ++j) {
-        const int rs = j % L::kRawStages;
-        if ((j & 7) == 0) {
-          const int v = (first + j) * 4 + lane;
-          token_l = -1;
-          page_l = 0;
-          if (v < blocks && lane < (tiles - j) * 4) {
-            const int token = token_of(v), page = __ldg(a.prefix_table + (token >> a.c.page_shift));
-            if (page >= 0 && page < a.c.pages) token_l = token, page_l = page;   // else reported above
-          }
+        const int rs = j % L::kRawStages, at = j % (32 / runs) * runs;
+        if (at == 0) {
+          const int token = token_of(min(j + lane / runs, tiles - 1)) + lane % runs * tokens;
+          page_l = token < bound ? __ldg(a.prefix_table + (token >> a.c.page_shift)) : -1;
+          if (page_l >= a.c.pages) page_l = -1;   // reported above
         }
-        const int token = __shfl_sync(0xffffffffu, token_l, (j & 7) * 4 + b), page = __shfl_sync(0xffffffffu, page_l, (j & 7) * 4 + b);
+        const int page = __shfl_sync(0xffffffffu, page_l, at + run), token = token_of(j) + run * tokens;
+        // what stands in a block of 16: four lanes say (runs are multiples of that)
+        const int block_page = __shfl_sync(0xffffffffu, page_l, at + (lane & 3) * 16 / tokens);
         if (j >= L::kRawStages && !mbar_wait_warp_lazy(&rempty[rs], ((j / L::kRawStages) - 1) & 1, ab, kErrRaw)) break;
         uint8_t* raw = smem + L::kRaws + rs * L::kRaw;
-        if (lane < 4) reinterpret_cast<int*>(raw + L::kRawInfo)[b] = token;
+        if (lane < 4) reinterpret_cast<int*>(raw + L::kRawInfo)[lane] = block_page < 0 ? 0 : bound - token_of(j) - lane * 16;
         __syncwarp();
         if (lane == 0) mbar_arrive_expect_tx(&rfull[rs], kTokens * DP + 2 * kTokens * 4);
         __syncwarp();
-        // where there is no block, a valid one's bytes: nobody sees them
-        const int64_t cell = page * page_step + cell0 + (max(token, 0) & page_mask);
-        if (lane < 4)
-          bulk_load(raw + b * 16 * (DP / 2), a.c.k_codes + cell * (DP / 2), 16 * (DP / 2), &rfull[rs]);
-        else if (lane < 12)
-          bulk_load(raw + L::kRawV + (lane - 4) * L::kChunkPitch, a.c.v_codes + (cell + (lane & 1) * 8) * (DP / 2), L::kChunkBytes, &rfull[rs]);
-        else if (lane < 16)
-          bulk_load(raw + L::kRawKp + b * 64, a.c.k_params + 2 * cell, 64, &rfull[rs]);
-        else if (lane < 20)
-          bulk_load(raw + L::kRawVp + b * 64, a.c.v_params + 2 * cell, 64, &rfull[rs]);
+        // where there is no page, a valid one's bytes: nobody sees them
+        const int64_t cell = max(page, 0) * page_step + cell0 + (token & page_mask);
+        if (what < 4) {
+          const uint32_t bytes = what < 2 ? tokens * (DP / 2) : tokens * 4;
+          const void* from = what == 0   ? (const void*)(a.c.k_codes + cell * (DP / 2))
+                             : what == 1 ? (const void*)(a.c.v_codes + cell * (DP / 2))
+                             : what == 2 ? (const void*)(a.c.k_params + 2 * cell)
+                                         : (const void*)(a.c.v_params + 2 * cell);
+          bulk_load(raw + (what == 0 ? 0 : what == 1 ? L::kRawV : what == 2 ? L::kRawKp : L::kRawVp) + run * bytes, from, bytes, &rfull[rs]);
+        }
         sent = j + 1;
         __syncwarp();
       }
