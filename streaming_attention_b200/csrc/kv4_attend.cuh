@@ -72,8 +72,6 @@ namespace cg = cooperative_groups;
 
 enum Mode { kPlain, kSelected, kWeigh, kPrefix, kTail };
 
-constexpr int kWarps = 8;
-constexpr int kThreads = kWarps * 32;
 constexpr float kMove = 8.0f;     // how far a maximum may be passed before it is moved (base 2)
 constexpr float kShift = -12.0f;  // p <= 2^-4: 2^16 values of 1e34 still sum below float32's limit
 
@@ -226,14 +224,14 @@ __device__ __forceinline__ int byte_column(int t, int g) {
   return DP >= 64 ? (t >> 2) * 32 + g * 4 + (t & 3) : g * 2 + t;
 }
 
-template <int DT, int DP, int NT>
+template <int DT, int DP, int NT, int kWarps>
 struct Shape {
   static constexpr int kQ = DT == SA_REP_BFLOAT16 ? 1 : (DT == SA_REP_FLOAT16 ? 2 : 3);   // pieces of q
   static constexpr int kP = DT == SA_REP_FLOAT32 ? 3 : 2;                                 // pieces of p s_v
   static constexpr int kRows = 8 * NT;
   // registers of O, Q and a block in a lane: where two CTAs an SM would spill, one
   static constexpr int kHeld = NT * (DP / 4 + kQ * DP / 8) + DP / 8;
-  static constexpr int kPerSm = kHeld <= 96 ? 2 : 1;
+  static constexpr int kPerSm = (kHeld <= 96 ? 2 : 1) * (8 / kWarps);
   static constexpr int kPitch = DP + 4;   // a row of O in shared memory
   // the queues, later the warps' O; then m, l and factors of warps (and CTAs), m, l
   static constexpr int kQueues = kWarps * kDepth * Queue<DP>::kSlot;
@@ -244,6 +242,7 @@ struct Shape {
 
 // How many entries of a list of pages count: those before the first that lies outside
 // the table or is not above the one before it (reported), or is -1.
+template <int kThreads>
 __device__ __forceinline__ int listed_pages(const Kv4AttendArgs& a, const int32_t* list, int* shared) {
   if (threadIdx.x == 0) *shared = a.count;
   __syncthreads();
@@ -258,10 +257,11 @@ __device__ __forceinline__ int listed_pages(const Kv4AttendArgs& a, const int32_
   return n;
 }
 
-template <int DT, int DP, int NT, int kMode>
-__global__ void __launch_bounds__(kThreads, (Shape<DT, DP, NT>::kPerSm)) attend_kernel(const Kv4AttendArgs a) {
+template <int DT, int DP, int NT, int kMode, int kWarps>
+__global__ void __launch_bounds__(kWarps * 32, (Shape<DT, DP, NT, kWarps>::kPerSm)) attend_kernel(const Kv4AttendArgs a) {
   using T = typename Elem<DT>::T;
-  using S = Shape<DT, DP, NT>;
+  using S = Shape<DT, DP, NT, kWarps>;
+  constexpr int kThreads = kWarps * 32;
   // codes of K and V enter the products plus 16, or, where the sums need the bits, less 8
   // (the weights are float32, whatever the inputs)
   constexpr int kOff = DT == SA_REP_FLOAT32 || kMode == kWeigh ? -8 : 16;
@@ -297,7 +297,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<DT, DP, NT>::kPerSm)) attend_
   if (kMode == kSelected) {
     length -= a.n - 1 - (int)(blockIdx.z % a.n);   // up to this query
     list = a.pages + ((int64_t)blockIdx.z * a.c.heads + hk) * a.count;
-    listed = listed_pages(a, list, reinterpret_cast<int*>(sm_f));
+    listed = listed_pages<kThreads>(a, list, reinterpret_cast<int*>(sm_f));
   }
   // positions of this tile's rows (rows behind the last count as the last); -1: sees nothing
   auto position = [&](int row) {
@@ -722,27 +722,37 @@ int64_t rows_of(const Kv4AttendArgs& a) {
   return kMode == kSelected ? group : kMode == kPrefix ? a.requests * a.n * group : a.n * group;
 }
 
-template <int DT, int DP, int NT, int kMode>
+template <int DT, int DP, int NT, int kMode, int kWarps = kMode == kPlain ? 8 : 4>
 int launch_one(const Kv4AttendArgs& a, cudaStream_t s) {
-  using S = Shape<DT, DP, NT>;
-  auto kern = attend_kernel<DT, DP, NT, kMode>;
+  using S = Shape<DT, DP, NT, kWarps>;
+  auto kern = attend_kernel<DT, DP, NT, kMode, kWarps>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
   if (e != cudaSuccess) return set_error(SA_ERR_CUDA, "kv4 attend smem attribute: %s", cudaGetErrorString(e));
   const int64_t y = a.c.heads * ceil_div(rows_of<kMode>(a), S::kRows);
   const int64_t z = kMode == kSelected ? (int64_t)a.requests * a.n : kMode == kPrefix ? a.parts : a.requests;
   if (y > 65535 || z > 65535) return set_error(SA_ERR_UNSUPPORTED, "kv4 attend: grid too large");
-  // CTAs per (request, key head): while a warp keeps at least four blocks of the
-  // longest request the table allows, of what window and first tokens show of it
-  // (8192 first tokens and a window of 64 of one request: 65 us as one CTA, 20 as
-  // eight), and the grid has less than three rounds (the batch above as it was at
-  // 212 us: 232 with six, 231 with one)
   const int64_t held = (int64_t)(kMode == kSelected ? std::min(a.count, a.width) : a.width) << a.c.page_shift;
   const int64_t longest = std::min<int64_t>(held, a.window + a.sinks + a.n);
-  int splits = 1;
-  while (splits < 8 && longest >= (int64_t)splits * 2 * kWarps * 16 * 4 && y * z * splits < 148 * S::kPerSm * 3) splits *= 2;
+  int splits = 1;   // CTAs per (request, key head)
+  if (kMode == kPlain) {
+    // while a warp keeps at least four blocks of the longest request the table allows, of
+    // what window and first tokens show of it (8192 first tokens and a window of 64 of one
+    // request: 65 us as one CTA, 20 as eight), and the grid has less than three rounds (the
+    // batch above as it was at 212 us: 232 with six, 231 with one)
+    while (splits < 8 && longest >= (int64_t)splits * 2 * kWarps * 16 * 4 && y * z * splits < 148 * S::kPerSm * 3) splits *= 2;
+  } else {
+    // while all run at once and a warp has half a block, or, in less than three rounds, it
+    // keeps 32 (48 requests x 8 heads x 2048 selected tokens: 57 us as one, 64 as two, 70 as
+    // four; three queries x 4 heads over 800: 16, 14, 12, 10 as eight; 32 requests of 10000
+    // tokens with weights: 196, 158, 150, 154)
+    auto more = [&](int64_t blocks, int64_t ctas) {
+      return splits < 8 && 2 * longest >= splits * 2 * kWarps * 16 * blocks && y * z * splits * 2 <= ctas;
+    };
+    while (more(1, 148 * S::kPerSm) || more(64, 148 * S::kPerSm * 3)) splits *= 2;
+  }
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)splits, (unsigned)y, (unsigned)z);
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(kWarps * 32);
   cfg.dynamicSmemBytes = S::kSmem;
   cfg.stream = s;
   cudaLaunchAttribute attr[1];

@@ -18,7 +18,7 @@ int parts_of(const Kv4AttendArgs& a) {
   const int64_t tiles = a.c.heads * ceil_div(all_rows(a), 8);
   const int64_t longest = std::min<int64_t>((int64_t)a.prefix_width << a.c.page_shift, a.window + a.sinks + a.n);
   int parts = 1;
-  while (parts < 16 && longest >= (int64_t)parts * 2 * 8 * kWarps * 16 * 4 && tiles * parts * 8 < 148 * 2) parts *= 2;
+  while (parts < 16 && longest >= (int64_t)parts * 2 * 8 * 8 * 16 * 4 && tiles * parts * 8 < 148 * 2) parts *= 2;
   return parts;
 }
 
