@@ -96,6 +96,7 @@ struct Kv4EvictArgs {
   const int32_t* tables;
   int32_t* kept;    // [requests, heads, keep]
   int requests, width, keep, limit, first, last;
+  int fits;         // tokens whose weights stand in shared memory
   int* status;
 };
 

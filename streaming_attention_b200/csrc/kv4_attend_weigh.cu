@@ -13,6 +13,7 @@ namespace sa {
 namespace {
 
 constexpr int kWeightThreads = 256;
+constexpr int kEach = 4;   // tokens of a thread
 
 __global__ void __launch_bounds__(kWeightThreads) weights_kernel(const Kv4AttendArgs a) {
   const int hk = blockIdx.y, r = blockIdx.z;
@@ -23,27 +24,40 @@ __global__ void __launch_bounds__(kWeightThreads) weights_kernel(const Kv4Attend
   const KeyRanges kr = key_ranges(length - a.n, length - 1, min(length, cap), a.window, a.sinks);
   const int sink_blocks = (int)((kr.first + 15) >> 4);
   const int win_begin = max((int)(kr.begin >> 4), sink_blocks), win_end = (int)((kr.end + 15) >> 4);
-  const int64_t t = (int64_t)blockIdx.x * kWeightThreads + threadIdx.x;
-  const int64_t v = t >> 4;
-  if (v >= sink_blocks + max(win_end - win_begin, 0)) return;
-  const int j = (int)(v < sink_blocks ? v : win_begin + v - sink_blocks) * 16 + (int)(t & 15);
-  if (j >= length) return;
-  const int page = __ldg(a.tables + (int64_t)r * a.width + (j >> a.c.page_shift));
-  if (page < 0 || page >= a.c.pages) return;   // reported by the attention
+  const int64_t seen = (int64_t)(sink_blocks + max(win_end - win_begin, 0)) * 16;
   const int64_t of = (int64_t)r * a.c.heads + hk;
-  const float* s = a.scores + (of * a.score_blocks * 16 + t) * a.score_rows;
+  const float* scores = a.scores + of * a.score_blocks * 16 * a.score_rows;
   const float2* ml = a.score_ml + of * a.score_rows;
-  float sum = 0.0f;
+  const int64_t t0 = (int64_t)blockIdx.x * kWeightThreads * kEach + threadIdx.x;
+  float* to[kEach];
+  float sum[kEach];
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    const int64_t t = t0 + i * kWeightThreads;
+    const int v = (int)(t >> 4), j = (v < sink_blocks ? v : win_begin + v - sink_blocks) * 16 + (int)(t & 15);
+    const int page = t < seen && j < length ? __ldg(a.tables + (int64_t)r * a.width + (j >> a.c.page_shift)) : -1;
+    // (a bad page is reported by the attention)
+    to[i] = page < 0 || page >= a.c.pages ? nullptr
+                                          : a.weights + ((page * (int64_t)a.c.heads + hk) << a.c.page_shift) +
+                                                (j & ((1 << a.c.page_shift) - 1));
+    sum[i] = 0.0f;
+  }
   for (int row = 0; row < rows; row += 2) {
-    const float2 x = *reinterpret_cast<const float2*>(s + row);
-    const float2 y = ml[row];
-    if (x.x != -INFINITY) sum += ex2(x.x + y.x) * y.y;
-    if (row + 1 < rows && x.y != -INFINITY) {
-      const float2 z = ml[row + 1];
-      sum += ex2(x.y + z.x) * z.y;
+    const float2 y = ml[row], z = row + 1 < rows ? ml[row + 1] : make_float2(0.0f, 0.0f);
+    float2 x[kEach];
+#pragma unroll
+    for (int i = 0; i < kEach; ++i)
+      x[i] = to[i] ? *reinterpret_cast<const float2*>(scores + (t0 + i * kWeightThreads) * a.score_rows + row)
+                   : make_float2(-INFINITY, -INFINITY);
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      if (x[i].x != -INFINITY) sum[i] += ex2(x[i].x + y.x) * y.y;
+      if (row + 1 < rows && x[i].y != -INFINITY) sum[i] += ex2(x[i].y + z.x) * z.y;
     }
   }
-  atomicAdd(a.weights + ((page * (int64_t)a.c.heads + hk) << a.c.page_shift) + (j & ((1 << a.c.page_shift) - 1)), sum);
+#pragma unroll
+  for (int i = 0; i < kEach; ++i)
+    if (to[i]) atomicAdd(to[i], sum[i]);
 }
 
 // Zero for the weights of slots.
@@ -89,7 +103,7 @@ int launch_kv4_attend_weigh(Kv4AttendArgs a, void* workspace, cudaStream_t s) {
   if (a.c.heads > 65535) return set_error(SA_ERR_UNSUPPORTED, "kv4 weights: grid too large");
   const int rc = launch_mode<kWeigh>(a, s);
   if (rc || a.score_blocks == 0) return rc;
-  weights_kernel<<<dim3((unsigned)ceil_div(a.score_blocks * 16, kWeightThreads), a.c.heads, a.requests), kWeightThreads, 0, s>>>(a);
+  weights_kernel<<<dim3((unsigned)ceil_div(a.score_blocks * 16, kWeightThreads * kEach), a.c.heads, a.requests), kWeightThreads, 0, s>>>(a);
   return check_launch("kv4 weights_kernel");
 }
 

@@ -2,11 +2,12 @@
 // first ones, the newest ones and, between, those of the largest weights (of equal ones
 // the lowest) -- moved up in their order to the request's first places, in place.
 //
-// One CTA per (request, key head).  The border between kept and dropped weights is found
-// by four passes over their digits; a scan in order then writes the list of what is kept.
-// Token j's new place is no higher than j, so places are filled from the first on, a
-// chunk at a time: all of a chunk is read before any of it is written, and what later
-// chunks read lies behind.
+// One CTA per (request, key head).  Its weights stand in shared memory (as whole numbers of
+// the same order) while the border between kept and dropped ones is found by four passes
+// over their digits and a scan in order turns them into the list of what is kept.  Token
+// j's new place is no higher than j, so places are filled from the first on, a chunk at a
+// time: all of a chunk is read before any of it is written, and what later chunks read lies
+// behind, so the next chunk is on its way while one is written.
 #include <algorithm>
 
 #include "kv4.cuh"
@@ -18,10 +19,10 @@ namespace {
 constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 constexpr int kChunk = 64;   // tokens moved at a time
-constexpr int kMaxRow = 128;                                            // bytes of a row's codes
-constexpr int kPieces = kChunk * (kMaxRow / 16) / kThreads;             // 16-byte pieces of keys, a thread
-constexpr int kWords = kChunk / 4 * kMaxRow / kThreads;                 // words of values, a thread
-static_assert(kPieces * kThreads == kChunk * (kMaxRow / 16) && kWords * kThreads == kChunk / 4 * kMaxRow, "whole shares");
+constexpr int kMaxRow = 128;                                   // bytes of a row's codes
+constexpr int kUnits = 2 * kChunk * (kMaxRow / 16) / kThreads; // 16-byte units of keys and of values, a thread
+constexpr int kLoads = 8;                                      // weights on their way, a thread
+static_assert(kUnits * kThreads == 2 * kChunk * (kMaxRow / 16), "whole shares");
 static_assert(3 * kChunk <= kThreads, "a thread moves one of a token's single words");
 
 // A weight as a whole number of the same order; NaN is the largest.
@@ -32,6 +33,7 @@ __device__ __forceinline__ uint32_t order_of(float x) {
 }
 
 __global__ void __launch_bounds__(kThreads) evict_kernel(const Kv4EvictArgs a) {
+  __shared__ int64_t src[4][kChunk], dst[4][kChunk];   // of four chunks' tokens: cells they come from and go to
   __shared__ int count_of[256];
   __shared__ int part[2][kWarps];
   __shared__ int digit, below;
@@ -49,14 +51,27 @@ __global__ void __launch_bounds__(kThreads) evict_kernel(const Kv4EvictArgs a) {
   }
   // the place of token j of this head, -1 without a page
   auto cell = [&](int j) -> int64_t {
-    const int page = table[j >> shift];
+    const int page = __ldg(table + (j >> shift));
     if (page < 0 || page >= a.c.pages) return -1;
     return (((int64_t)page * a.c.heads + h) << shift) + (j & mask);
   };
-  auto key = [&](int j) {
+  // the weights' order, then (in the same memory) the list; what does not fit is read where it stands
+  extern __shared__ uint32_t held[];
+  const int fits = min(a.fits, length);
+  auto key_of = [&](int j) {
     const int64_t at = cell(j);
     return at < 0 ? 0u : order_of(a.weights[at]);
   };
+  for (int j = tid; j < fits; j += kThreads * kLoads) {
+    uint32_t k[kLoads];
+#pragma unroll
+    for (int x = 0; x < kLoads; ++x) k[x] = j + x * kThreads < fits ? key_of(j + x * kThreads) : 0u;
+#pragma unroll
+    for (int x = 0; x < kLoads; ++x)
+      if (j + x * kThreads < fits) held[j + x * kThreads] = k[x];
+  }
+  auto key = [&](int j) { return j < fits ? held[j] : key_of(j); };
+  __syncthreads();
   for (int row = tid; row << shift < length; row += kThreads)
     if (h == 0 && (table[row] < 0 || table[row] >= a.c.pages)) report(a.status, kBadPage, table[row]);
   const int begin = a.first, end = length - a.last, want = a.keep - a.first - a.last;
@@ -123,76 +138,113 @@ __global__ void __launch_bounds__(kThreads) evict_kernel(const Kv4EvictArgs a) {
       s_all += part[1][x];
     }
     // of the equal ones before this one, no more than `ties` were taken
-    if (over || (same && s < ties)) kept[at + o + min(s, ties) - min(equal, ties)] = j;
+    if (over || (same && s < ties)) {
+      const int place = at + o + min(s, ties) - min(equal, ties);   // <= j: every key up to this round's has been read
+      kept[place] = j;
+      if (place < fits) held[place] = j;
+    }
     at += o_all + min(equal + s_all, ties) - min(equal, ties);
     equal += s_all;
     __syncthreads();
   }
   // the tokens, a chunk of new places at a time
-  const int bytes = a.c.dp >> 1, pieces = bytes >> 4;
-  for (int j0 = 0; j0 < a.keep; j0 += kChunk) {
-    const int n = min(kChunk, a.keep - j0);
-    if (kept[j0 + n - 1] == j0 + n - 1) continue;   // all where they were: kept[] ascends
-    uint4 keys[kPieces];
-    uint32_t values[kWords], single = 0;
-#pragma unroll
-    for (int x = 0; x < kPieces; ++x) {
-      const int p = x * kThreads + tid, j = p / pieces;
-      if (j < n) {
-        const int64_t from = cell(kept[j0 + j]);
-        if (from >= 0) keys[x] = reinterpret_cast<const uint4*>(a.c.k_codes + from * bytes)[p - j * pieces];
-      }
+  const int bytes = a.c.dp >> 1, bytes_log = 31 - __clz(bytes);
+  const int which = tid / kChunk, js = tid - which * kChunk;   // keys' parameters, values', weights
+  auto cells = [&](int j0) {
+    if (tid >= kChunk || j0 >= a.keep) return;
+    const int j = j0 + tid, at = j0 / kChunk & 3;
+    int64_t from = -1, to = -1;
+    if (j < ((a.keep + 3) & ~3)) {   // places behind `keep` in its word of values take what they hold
+      to = cell(j);
+      from = j < a.keep ? cell(j < fits ? (int)held[j] : kept[j]) : to;
     }
-    // a word holds four tokens' bytes: of places behind `keep`, what they hold
+    src[at][tid] = from;
+    dst[at][tid] = to;
+  };
+  struct Part {
+    uint4 w[kUnits];
+    uint32_t single;
+  };
+  // unit u: 16 bytes of a key row, or, behind those, four tokens' bytes of four column pairs
+  auto load = [&](Part& c, int j0) {
+    if (j0 >= a.keep) return;
+    const int64_t* from = src[j0 / kChunk & 3];
 #pragma unroll
-    for (int x = 0; x < kWords; ++x) {
-      const int p = x * kThreads + tid, j4 = p / bytes * 4, b = p - j4 / 4 * bytes;
-      uint32_t w = 0;
-      if (j4 < n) {
+    for (int x = 0; x < kUnits; ++x) {
+      const int u = x * kThreads + tid;
+      c.w[x] = make_uint4(0, 0, 0, 0);
+      if (u < 4 * bytes) {
+        const int j = u >> (bytes_log - 4);
+        if (from[j] >= 0) c.w[x] = *reinterpret_cast<const uint4*>(a.c.k_codes + from[j] * bytes + (u & (bytes / 16 - 1)) * 16);
+      } else if (u < 8 * bytes) {
+        const int v = u - 4 * bytes, j = (v >> (bytes_log - 2)) * 4, b = (v & (bytes / 4 - 1)) * 4;
+        uint4 t[4];
+        int byte[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const int64_t from = cell(j4 + e < n ? kept[j0 + j4 + e] : j0 + j4 + e);
-          if (from < 0) continue;
-          w |= (uint32_t)a.c.v_codes[(from & ~3ll) * bytes + b * 4 + (from & 3)] << (8 * e);
+          const int64_t f = from[j + e];
+          t[e] = f < 0 ? make_uint4(0, 0, 0, 0) : *reinterpret_cast<const uint4*>(a.c.v_codes + (f & ~3ll) * bytes + b * 4);
+          byte[e] = (int)(f & 3);
         }
+        const uint32_t lo = byte[0] | (4 + byte[1]) << 4, hi = byte[2] | (4 + byte[3]) << 4;
+        auto join = [&](uint32_t p, uint32_t q, uint32_t r, uint32_t s) {
+          return __byte_perm(__byte_perm(p, q, lo), __byte_perm(r, s, hi), 0x5410);
+        };
+        c.w[x] = make_uint4(join(t[0].x, t[1].x, t[2].x, t[3].x), join(t[0].y, t[1].y, t[2].y, t[3].y),
+                            join(t[0].z, t[1].z, t[2].z, t[3].z), join(t[0].w, t[1].w, t[2].w, t[3].w));
       }
-      values[x] = w;
     }
-    const int which = tid / kChunk, js = tid - which * kChunk;   // keys' parameters, values', weights
-    if (which < 3 && js < n) {
-      const int64_t from = cell(kept[j0 + js]);
-      if (from >= 0)
-        single = which == 0   ? reinterpret_cast<const uint32_t*>(a.c.k_params)[from]
-                 : which == 1 ? reinterpret_cast<const uint32_t*>(a.c.v_params)[from]
-                              : __float_as_uint(a.weights[from]);
-    }
-    __syncthreads();
+    c.single = 0;
+    if (which < 3 && j0 + js < a.keep && from[js] >= 0)
+      c.single = which == 0   ? reinterpret_cast<const uint32_t*>(a.c.k_params)[from[js]]
+                 : which == 1 ? reinterpret_cast<const uint32_t*>(a.c.v_params)[from[js]]
+                              : __float_as_uint(a.weights[from[js]]);
+  };
+  auto store = [&](const Part& c, int j0) {
+    if (j0 >= a.keep) return;
+    const int64_t* from = src[j0 / kChunk & 3];
+    const int64_t* to = dst[j0 / kChunk & 3];
 #pragma unroll
-    for (int x = 0; x < kPieces; ++x) {
-      const int p = x * kThreads + tid, j = p / pieces;
-      if (j < n) {
-        const int64_t to = cell(j0 + j);
-        if (to >= 0 && cell(kept[j0 + j]) >= 0) reinterpret_cast<uint4*>(a.c.k_codes + to * bytes)[p - j * pieces] = keys[x];
+    for (int x = 0; x < kUnits; ++x) {
+      const int u = x * kThreads + tid;
+      if (u < 4 * bytes) {
+        const int j = u >> (bytes_log - 4);
+        if (j0 + j < a.keep && to[j] >= 0 && from[j] >= 0)
+          *reinterpret_cast<uint4*>(a.c.k_codes + to[j] * bytes + (u & (bytes / 16 - 1)) * 16) = c.w[x];
+      } else if (u < 8 * bytes) {
+        const int v = u - 4 * bytes, j = (v >> (bytes_log - 2)) * 4, b = (v & (bytes / 4 - 1)) * 4;
+        if (to[j] >= 0) *reinterpret_cast<uint4*>(a.c.v_codes + to[j] * bytes + b * 4) = c.w[x];
       }
     }
-#pragma unroll
-    for (int x = 0; x < kWords; ++x) {
-      const int p = x * kThreads + tid, j4 = p / bytes * 4, b = p - j4 / 4 * bytes;
-      if (j4 < n) {
-        const int64_t to = cell(j0 + j4);
-        if (to >= 0) *reinterpret_cast<uint32_t*>(a.c.v_codes + to * bytes + b * 4) = values[x];
-      }
+    if (which < 3 && j0 + js < a.keep && to[js] >= 0) {
+      if (which == 0) reinterpret_cast<uint32_t*>(a.c.k_params)[to[js]] = c.single;
+      if (which == 1) reinterpret_cast<uint32_t*>(a.c.v_params)[to[js]] = c.single;
+      if (which == 2) a.weights[to[js]] = __uint_as_float(c.single);
     }
-    if (which < 3 && js < n) {
-      const int64_t to = cell(j0 + js);
-      if (to >= 0) {
-        if (which == 0) reinterpret_cast<uint32_t*>(a.c.k_params)[to] = single;
-        if (which == 1) reinterpret_cast<uint32_t*>(a.c.v_params)[to] = single;
-        if (which == 2) a.weights[to] = __uint_as_float(single);
-      }
-    }
-    __syncthreads();
+  };
+  int begun = 0;   // the first tokens are where they were: the list ascends
+  while (begun + kChunk <= a.keep) {
+    const int last = begun + kChunk - 1;
+    if ((last < fits ? (int)held[last] : kept[last]) != last) break;
+    begun += kChunk;
   }
+  // a barrier stands between a chunk's loads and its stores, and behind what says where it goes
+  Part x, y;
+  cells(begun);
+  cells(begun + kChunk);
+  __syncthreads();
+  load(x, begun);
+  for (int j0 = begun; j0 < a.keep; j0 += 2 * kChunk) {
+    cells(j0 + 2 * kChunk);
+    load(y, j0 + kChunk);
+    __syncthreads();
+    store(x, j0);
+    cells(j0 + 3 * kChunk);
+    load(x, j0 + 2 * kChunk);
+    __syncthreads();
+    store(y, j0 + kChunk);
+  }
+  __syncthreads();
   // whoever stands in the places behind starts from zero
   for (int j = a.keep + tid; j < (((int64_t)length + mask) & ~(int64_t)mask); j += kThreads) {
     const int64_t to = cell(j);
@@ -204,7 +256,13 @@ __global__ void __launch_bounds__(kThreads) evict_kernel(const Kv4EvictArgs a) {
 
 int launch_kv4_evict(const Kv4EvictArgs& a, cudaStream_t s) {
   if (a.requests > 65535) return set_error(SA_ERR_UNSUPPORTED, "kv4 evict: more than 65535 requests in one call");
-  evict_kernel<<<dim3((unsigned)a.c.heads, (unsigned)a.requests), kThreads, 0, s>>>(a);
+  // weights of 24576 tokens at most (96 KB): registers keep it at two CTAs an SM anyway
+  constexpr int kFits = 24576;
+  Kv4EvictArgs b = a;
+  b.fits = (int)std::min<int64_t>((int64_t)a.width << a.c.page_shift, kFits);
+  const cudaError_t e = cudaFuncSetAttribute(evict_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kFits * 4);
+  if (e != cudaSuccess) return set_error(SA_ERR_CUDA, "kv4 evict smem attribute: %s", cudaGetErrorString(e));
+  evict_kernel<<<dim3((unsigned)a.c.heads, (unsigned)a.requests), kThreads, b.fits * 4, s>>>(b);
   return check_launch("kv4 evict_kernel");
 }
 

@@ -38,9 +38,15 @@ __device__ __forceinline__ float most_of(float x, float y) {
   return r;
 }
 
-// A warp per (touched page, head): a lane holds eight columns (a word of codes) of
-// every (32 / words of a row)-th token.
-__global__ void __launch_bounds__(kThreads) bounds_kernel(const Kv4BoundsArgs a) {
+// A CTA per (touched page, head) at a time: a lane holds eight columns (a word of codes) of
+// every (32 / words of a row)-th token of its warp's, kBatch loads on their way at a time;
+// the warps join through shared memory.  (As one warp a page, and four loads, 48 requests' newest
+// pages of 64 tokens x 8 heads, 3.4 MB, took 25 us: the chain of a lane's tokens.)
+constexpr int kBoundWarps = 4;
+constexpr int kBatch = 8;
+
+__global__ void __launch_bounds__(kBoundWarps * 32) bounds_kernel(const Kv4BoundsArgs a) {
+  __shared__ float joined[kBoundWarps][2][256];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int r = blockIdx.y;
   const int cap = a.width << a.c.page_shift;
@@ -49,13 +55,13 @@ __global__ void __launch_bounds__(kThreads) bounds_kernel(const Kv4BoundsArgs a)
   const int from = whole - min(max(a.fresh[r], 0), whole);   // tokens [from, length) are new
   if (from >= length) return;
   const int first = from >> a.c.page_shift, last = (length - 1) >> a.c.page_shift;
-  const int words = a.c.dp >> 3, word = lane & (words - 1), sub = lane / words, step = 32 / words;
+  const int words = a.c.dp >> 3, word = lane & (words - 1), sub = lane / words, step = kBoundWarps * (32 / words);
   const int64_t units = (int64_t)(last - first + 1) * a.c.heads;
-  for (int64_t u = (int64_t)blockIdx.x * kWarps + warp; u < units; u += (int64_t)gridDim.x * kWarps) {
+  for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
     const int row = first + (int)(u / a.c.heads), h = (int)(u % a.c.heads);
     const int page = a.tables[(int64_t)r * a.width + row];
     if (page < 0 || page >= a.c.pages) {
-      if (h == 0 && lane == 0) report(a.status, kBadPage, page);
+      if (h == 0 && threadIdx.x == 0) report(a.status, kBadPage, page);
       continue;
     }
     const int held = min(length - (row << a.c.page_shift), 1 << a.c.page_shift);
@@ -65,15 +71,24 @@ __global__ void __launch_bounds__(kThreads) bounds_kernel(const Kv4BoundsArgs a)
     float low[8], high[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) low[e] = INFINITY, high[e] = -INFINITY;
-#pragma unroll 4
-    for (int t = sub; t < held; t += step) {
-      const uint32_t w = codes[(int64_t)t * words], p = params[t];
-      const float scale = __uint_as_float(p << 16), least = __uint_as_float(p & 0xffff0000u);
+    const int t0 = warp * (32 / words) + sub;
+    for (int b = 0; b < held; b += kBatch * step) {
+      uint32_t w[kBatch], p[kBatch];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float x = fmaf((float)((w >> (4 * e)) & 15u), scale, least);
-        low[e] = least_of(low[e], x);
-        high[e] = most_of(high[e], x);
+      for (int i = 0; i < kBatch; ++i) {
+        const int t = min(b + t0 + i * step, held - 1);   // the last token again changes nothing
+        w[i] = codes[(int64_t)t * words];
+        p[i] = params[t];
+      }
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        const float scale = __uint_as_float(p[i] << 16), least = __uint_as_float(p[i] & 0xffff0000u);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float x = fmaf((float)((w[i] >> (4 * e)) & 15u), scale, least);
+          low[e] = least_of(low[e], x);
+          high[e] = most_of(high[e], x);
+        }
       }
     }
 #pragma unroll
@@ -82,14 +97,25 @@ __global__ void __launch_bounds__(kThreads) bounds_kernel(const Kv4BoundsArgs a)
         low[e] = least_of(low[e], __shfl_xor_sync(0xffffffffu, low[e], d));
         high[e] = most_of(high[e], __shfl_xor_sync(0xffffffffu, high[e], d));
       }
-    if (sub == 0) {
+    if (sub == 0)
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (word * 8 + e >= a.c.d) low[e] = high[e] = 0.0f;
-      __nv_bfloat16* to = a.bounds + (page * (int64_t)a.c.heads + h) * 2 * a.c.dp + word * 8;
-      store8(to, low);
-      store8(to + a.c.dp, high);
+      for (int e = 0; e < 8; ++e) {
+        joined[warp][0][word * 8 + e] = low[e];
+        joined[warp][1][word * 8 + e] = high[e];
+      }
+    __syncthreads();
+    __nv_bfloat16* to = a.bounds + (page * (int64_t)a.c.heads + h) * 2 * a.c.dp;
+    for (int c = threadIdx.x; c < a.c.dp; c += kBoundWarps * 32) {
+      float x = joined[0][0][c], y = joined[0][1][c];
+#pragma unroll
+      for (int w = 1; w < kBoundWarps; ++w) {
+        x = least_of(x, joined[w][0][c]);
+        y = most_of(y, joined[w][1][c]);
+      }
+      to[c] = __float2bfloat16_rn(c < a.c.d ? x : 0.0f);
+      to[a.c.dp + c] = __float2bfloat16_rn(c < a.c.d ? y : 0.0f);
     }
+    __syncthreads();
   }
 }
 
@@ -100,10 +126,35 @@ __device__ __forceinline__ uint64_t order_of(double x) {
   return b >> 63 ? ~b : b | (1ull << 63);
 }
 
+// A lane's columns of a row of bounds.
+template <int N>
+struct Columns {
+  static constexpr int kWords = N > 1 ? N / 2 : 1;
+  uint32_t w[kWords];
+  __device__ __forceinline__ void load(const __nv_bfloat16* p) {
+    if constexpr (N == 8) {
+      const uint4 x = __ldg(reinterpret_cast<const uint4*>(p));
+      w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w;
+    } else if constexpr (N == 4) {
+      const uint2 x = __ldg(reinterpret_cast<const uint2*>(p));
+      w[0] = x.x, w[1] = x.y;
+    } else if constexpr (N == 2) {
+      w[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
+    } else {
+      w[0] = __ldg(reinterpret_cast<const uint16_t*>(p));
+    }
+  }
+  __device__ __forceinline__ float get(int e) const {
+    return __uint_as_float(e & 1 ? w[e >> 1] & 0xffff0000u : w[e >> 1] << 16);
+  }
+};
+
+constexpr int kPages = 8;   // that a warp scores at a time
+
 // A cluster of CTAs scores the pages of one (query token, key head); its first CTA
 // then picks the largest scores by their digits and writes them in ascending order.
 template <int DT, int DP>
-__global__ void __launch_bounds__(kThreads) select_kernel(const Kv4SelectArgs a) {
+__global__ void __launch_bounds__(kThreads, 3) select_kernel(const Kv4SelectArgs a) {
   using T = typename Elem<DT>::T;
   constexpr int kCols = DP / 32;   // columns of a lane
   extern __shared__ __align__(16) uint64_t keys[];   // [width]: of the pages between first and last
@@ -148,23 +199,46 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const Kv4SelectArgs a)
     }
     uint64_t* to = gridDim.x > 1 ? cluster.map_shared_rank(keys, 0) : keys;
     const int32_t* table = a.tables + (int64_t)r * a.width + a.first;
-    for (int w = blockIdx.x * kWarps + warp; w < middle; w += gridDim.x * kWarps) {
-      const int page = __ldg(table + w);
-      double score = -INFINITY;
-      if (page < 0 || page >= a.c.pages) {
-        if (lane == 0) report(a.status, kBadPage, page);
-      } else {
-        const __nv_bfloat16* b = a.bounds + (page * (int64_t)a.c.heads + hk) * 2 * DP + lane * kCols;
-        score = 0.0;
+    // eight pages of a warp at a time, all their loads on their way
+    for (int w0 = (blockIdx.x * kWarps + warp) * kPages; w0 < middle; w0 += gridDim.x * kWarps * kPages) {
+      const int mine = w0 + (lane & (kPages - 1));
+      int page = mine < middle ? __ldg(table + mine) : 0;
+      const bool bad = page < 0 || page >= a.c.pages;
+      if (bad && lane < kPages) report(a.status, kBadPage, page);
+      if (bad) page = -1;
+      Columns<kCols> low[kPages], high[kPages];
+#pragma unroll
+      for (int x = 0; x < kPages; ++x) {
+        const int id = max(__shfl_sync(0xffffffffu, page, x), 0);
+        const __nv_bfloat16* b = a.bounds + (id * (int64_t)a.c.heads + hk) * 2 * DP + lane * kCols;
+        low[x].load(b);
+        high[x].load(b + DP);
+      }
+      double score[kPages];
+#pragma unroll
+      for (int x = 0; x < kPages; ++x) {
+        score[x] = 0.0;
 #pragma unroll
         for (int e = 0; e < kCols; ++e) {
-          score = fma(u[e], (double)to_f32(b[DP + e]), score);
-          score = fma(d[e], (double)to_f32(b[e]), score);
+          score[x] = fma(u[e], (double)high[x].get(e), score[x]);
+          score[x] = fma(d[e], (double)low[x].get(e), score[x]);
         }
-#pragma unroll
-        for (int x = 16; x >= 1; x >>= 1) score += __shfl_xor_sync(0xffffffffu, score, x);
       }
-      if (lane == 0) to[w] = order_of(score);
+      // sums over the lanes: each halving keeps half of the pages, so that in the end four lanes have one page's
+#pragma unroll
+      for (int n = kPages / 2, x = 16; n >= 1; n /= 2, x /= 2) {
+        const bool upper = lane & x;
+#pragma unroll
+        for (int i = 0; i < n; ++i) {
+          const double give = upper ? score[i] : score[i + n], keep = upper ? score[i + n] : score[i];
+          score[i] = keep + __shfl_xor_sync(0xffffffffu, give, x);
+        }
+      }
+      score[0] += __shfl_xor_sync(0xffffffffu, score[0], 2);
+      score[0] += __shfl_xor_sync(0xffffffffu, score[0], 1);
+      const int x = lane >> 2;   // bit 4 chose among pages 0..3 and 4..7, and so on
+      const bool none = __shfl_sync(0xffffffffu, page, x) < 0;
+      if ((lane & 3) == 0 && w0 + x < middle) to[w0 + x] = order_of(none ? -INFINITY : score[0]);
     }
   }
   if (gridDim.x > 1)
@@ -250,7 +324,7 @@ int launch_select(const Kv4SelectArgs& a, cudaStream_t s) {
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSelectMaxPages * 8);
   if (e != cudaSuccess) return set_error(SA_ERR_CUDA, "kv4 select smem attribute: %s", cudaGetErrorString(e));
   int splits = 1;   // while a warp keeps eight pages and CTAs are few
-  while (splits < 8 && a.width >= splits * 2 * kWarps * 8 && z * a.c.heads * splits < 148) splits *= 2;
+  while (splits < 8 && a.width >= splits * 2 * kWarps * kPages && z * a.c.heads * splits < 148) splits *= 2;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)splits, (unsigned)a.c.heads, (unsigned)z);
   cfg.blockDim = dim3(kThreads);
@@ -279,11 +353,12 @@ int launch_select_dim(const Kv4SelectArgs& a, cudaStream_t s) {
 }  // namespace
 
 int launch_kv4_bounds(const Kv4BoundsArgs& a, cudaStream_t s) {
-  // CTAs that share a request's pages: enough for the GPU when requests are few
-  const int64_t most = ceil_div((int64_t)a.width * a.c.heads, kWarps);
-  const int64_t x = std::min(most, std::max<int64_t>(ceil_div(148 * 8, a.requests), ceil_div(a.c.heads, kWarps)));
+  // CTAs that share a request's pages: enough for the GPU when requests are few, and one for
+  // each head of a page
+  const int64_t most = (int64_t)a.width * a.c.heads;
+  const int64_t x = std::min(most, std::max<int64_t>(ceil_div(148 * 8, a.requests), a.c.heads));
   if (a.requests > 65535) return set_error(SA_ERR_UNSUPPORTED, "kv4 bounds: more than 65535 requests in one call");
-  bounds_kernel<<<dim3((unsigned)x, (unsigned)a.requests), kThreads, 0, s>>>(a);
+  bounds_kernel<<<dim3((unsigned)x, (unsigned)a.requests), kBoundWarps * 32, 0, s>>>(a);
   return check_launch("kv4 bounds_kernel");
 }
 

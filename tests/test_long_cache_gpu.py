@@ -43,6 +43,13 @@ def _close(out, ref, spread, score, d, keys, p_half, span=None):
     R.assert_close(out, ref, R.attention_bound(ref, spread, span * score, d, max(keys, 1), dtype, p_half))
 
 
+def _one_step(a, b):
+    """Results of bfloat16 whose sums were added in another order: float32 sums that differ by less than 2^-14 (2^-16 of
+    values below 4), each rounded, are a step apart at most (2^-7 of the value: twice half a step)."""
+    a, b = a.double(), b.double()
+    assert ((a - b).abs() <= 2 * R.HALF[BF16] * torch.maximum(a.abs(), b.abs()) + 2.0 ** -14).all()
+
+
 # ------------------------------------------------------------- shared prefix
 
 SHARED = [
@@ -161,8 +168,8 @@ def test_shared_prefix_of_nothing_is_attend(dev):
     cache, tables, lens, _, _ = _filled(dev, [0, 50, 3], 2, 64, 16, F32, 5)
     q = _queries(2, 1, 4, 64, BF16, 1, dev)
     want = cache.attend(q, tables[1:], lens[1:])
-    assert torch.equal(cache.attend_shared(q, tables[0], lens[:1], tables[1:], lens[1:]), want)
-    assert torch.equal(cache.attend_shared(q, tables[0, :0], lens[:1], tables[1:], lens[1:]), want)
+    _one_step(cache.attend_shared(q, tables[0], lens[:1], tables[1:], lens[1:]), want)
+    _one_step(cache.attend_shared(q, tables[0, :0], lens[:1], tables[1:], lens[1:]), want)
     empty = cache.attend_shared(q[:0], tables[0], lens[:1], tables[:0], lens[:0])
     assert empty.shape == (0, 1, 4, 64)
 
@@ -224,7 +231,7 @@ def test_attend_pages_all_and_none(dev):
     q = _queries(3, 1, 4, 64, BF16, 1, dev)
     every = torch.arange(10, dtype=torch.int32).expand(3, 1, 2, 10).contiguous()
     every = torch.where(every < torch.tensor([10, 3, 0])[:, None, None, None], every, -1).to(torch.int32).to(dev)
-    assert torch.equal(cache.attend_pages(q, tables, lens, every), cache.attend(q, tables, lens))
+    _one_step(cache.attend_pages(q, tables, lens, every), cache.attend(q, tables, lens))
     none = torch.full((3, 1, 2, 4), -1, dtype=torch.int32, device=dev)
     assert (cache.attend_pages(q, tables, lens, none) == 0).all()
     assert (cache.attend_pages(q, tables, lens, none[..., :0]) == 0).all()
@@ -429,6 +436,7 @@ EVICT = [
     ([257, 2], 4, 31, 16, 2, 200, 1, 0),
     ([3000], 1, 128, 256, 130, 256, 0, 0),
     ([90] * 40, 1, 32, 16, 70, 70, 2, 3),
+    ([25600, 26000], 1, 32, 256, 24900, 25599, 10, 300),   # more than stand in shared memory
 ]
 
 
@@ -590,7 +598,7 @@ def test_sparse_attention_with_every_page_is_attend(dev):
     bounds = cache.page_bounds()
     cache.update_page_bounds(bounds, tables, lens, lens)
     pages = cache.select_pages(q, bounds, tables, lens, count=32)
-    assert torch.equal(cache.attend_pages(q, tables, lens, pages), cache.attend(q, tables, lens))
+    _one_step(cache.attend_pages(q, tables, lens, pages), cache.attend(q, tables, lens))
 
 
 def test_calls_on_other_streams_with_workspaces(dev):
