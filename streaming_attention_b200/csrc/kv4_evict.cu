@@ -16,13 +16,12 @@ namespace sa {
 
 namespace {
 
-constexpr int kThreads = 512;
+constexpr int kThreads = 384;
 constexpr int kWarps = kThreads / 32;
 constexpr int kChunk = 64;   // tokens moved at a time
 constexpr int kMaxRow = 128;                                   // bytes of a row's codes
-constexpr int kUnits = 2 * kChunk * (kMaxRow / 16) / kThreads; // 16-byte units of keys and of values, a thread
+constexpr int kUnits = (2 * kChunk * (kMaxRow / 16) + kThreads - 1) / kThreads; // 16-byte units of keys and of values, a thread
 constexpr int kLoads = 8;                                      // weights on their way, a thread
-static_assert(kUnits * kThreads == 2 * kChunk * (kMaxRow / 16), "whole shares");
 static_assert(3 * kChunk <= kThreads, "a thread moves one of a token's single words");
 
 // A weight as a whole number of the same order; NaN is the largest.
@@ -32,7 +31,7 @@ __device__ __forceinline__ uint32_t order_of(float x) {
   return b >> 31 ? ~b : b | 0x80000000u;
 }
 
-__global__ void __launch_bounds__(kThreads) evict_kernel(const Kv4EvictArgs a) {
+__global__ void __launch_bounds__(kThreads, 3) evict_kernel(const Kv4EvictArgs a) {
   __shared__ int64_t src[4][kChunk], dst[4][kChunk];   // of four chunks' tokens: cells they come from and go to
   __shared__ int count_of[256];
   __shared__ int part[2][kWarps];
