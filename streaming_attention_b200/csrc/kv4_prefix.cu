@@ -16,10 +16,11 @@
 //
 // A CTA holds two tiles of 128 query rows of one key head (a row: request, query, head)
 // and a part of the prefix in tiles of 64 tokens; all rows see (nearly) all of it, so a
-// decoded tile serves 256 rows.  Warps: 0..3 and 4..7 are the softmax of a row tile, one
-// row a thread; 8..11 decode keys and 12..15 values, from raw tiles that warp 18 brings
-// in ahead (bulk copies) to swizzled ones; 16 and 17 issue the products of a row tile, one
-// elected lane.  TMEM: of each row tile two S of 64 columns and O; P overwrites the first
+// decoded tile serves 256 rows.  Warps: 0..7 and 8..15 are the softmax of a row tile, two
+// threads a row (the exponentials' unit is shared, and four warps beside it keep it busy where
+// two, in step, left it idle half of the time); 16..19 decode keys and 20..23 values, from raw tiles
+// that warp 26 brings in ahead (bulk copies) to swizzled ones; 24 and 25 issue the products of a
+// row tile, one elected lane.  TMEM: of each row tile two S of 64 columns and O; P overwrites the first
 // half of its S.  The issuer goes P V(j), S(j + 2), so that scores are there while a softmax
 // runs.
 //
@@ -47,15 +48,17 @@ using namespace tc;
 constexpr int kTileRows = 128;
 constexpr int kTokens = 64;        // of a tile
 constexpr int kRowTiles = 2;
-constexpr int kSoftmax = kRowTiles * kTileRows;
+constexpr int kCtaRows = kRowTiles * kTileRows;
+constexpr int kHalf = kTokens / 2;
+constexpr int kSoftmax = 2 * kCtaRows;   // two threads a row, each of half of a tile's tokens
 constexpr int kDecoders = 128;     // of keys, and as many of values
 constexpr int kIssuer = (kSoftmax + 2 * kDecoders) / 32;   // the first of two warps
 constexpr int kLoader = kIssuer + kRowTiles;
 constexpr int kPrefixThreads = (kLoader + 2) * 32;          // whole groups of four warps
-// Registers of a thread: launched with 96 (65536 / 640, in steps of 8), then dealt out by groups of four
-// warps: 2 x 136 (a row's 64 scores stay in registers) + 2 x 72 + 64 = 5 x 96.
-constexpr int kSoftmaxRegs = 136, kDecoderRegs = 72, kOtherRegs = 64;
-static_assert(2 * kSoftmaxRegs + 2 * kDecoderRegs + kOtherRegs <= 5 * 96, "more registers than the launch has");
+// Registers of a thread: launched with 72 (65536 / 896, in steps of 8), then dealt out by groups of four
+// warps: 4 x 80 + 2 x 64 + 56 = 7 x 72.
+constexpr int kSoftmaxRegs = 80, kDecoderRegs = 64, kOtherRegs = 56;
+static_assert(4 * kSoftmaxRegs + 2 * kDecoderRegs + kOtherRegs <= 7 * 72, "more registers than the launch has");
 constexpr float kShiftP = 6.0f;    // P = 2^(x - m + 6), m at most kMove below the largest x: 2^14 at most, and 2^-14,
                                    // where float16 starts to lose bits, is 2^-20 of a row's usual largest
 
@@ -86,10 +89,12 @@ struct PrefixLayout {
   static constexpr int kSums = kValues + kStages * kV;
   static constexpr int kOffsets = kSums + kRowTiles * kQSum;
   static constexpr int kPowers = kOffsets + kStages * kKOff;   // of the rows
-  static constexpr int kRows = kPowers + kSoftmax * 4;         // where the rows of q start
-  static constexpr int kRaws = kRows + kSoftmax * 8;
+  static constexpr int kRows = kPowers + kCtaRows * 4;         // where the rows of q start
+  static constexpr int kTops = kRows + kCtaRows * 8;           // what a row's threads tell each other: [two turns][half][row]
+  static constexpr int kPositions = kTops + 4 * kCtaRows * 4;
+  static constexpr int kRaws = kPositions + kCtaRows * 4;
   static constexpr int kBars = kRaws + kRawStages * kRaw;
-  static constexpr int kBytes = kBars + (4 * kStages + 2 * kRawStages + 12) * 8 + 48 + 1024;
+  static constexpr int kBytes = kBars + (4 * kStages + 2 * kRawStages + 12) * 8 + 64 + 1024;
   static_assert(kBytes <= 227 * 1024, "shared memory");
   static_assert(kValues % 1024 == 0 && kKeys % 1024 == 0 && kSums % 1024 == 0 && kOffsets % 1024 == 0 && kRaws % 16 == 0 &&
                 kRaw % 16 == 0 && kBars % 8 == 0, "alignment of tiles, copies and barriers");
@@ -125,6 +130,11 @@ __device__ __forceinline__ void tie32(float (&v)[32]) {
   tie16(v + 16);
 }
 
+// The barrier of two warps.  A warp that gives up arrives there once more, so that its
+// mate, should it wait, goes on to find the abort word set.
+__device__ __forceinline__ void pair_sync(int id) { asm volatile("bar.sync %0, 64;" ::"r"(id) : "memory"); }
+__device__ __forceinline__ void pair_leave(int id) { asm volatile("bar.arrive %0, 64;" ::"r"(id) : "memory"); }
+
 template <int N>
 __device__ __forceinline__ void fewer_registers() {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
@@ -149,6 +159,22 @@ __device__ __noinline__ void scale_row(uint32_t to, int columns, float alpha) {
   }
   tmem_wait_st();
 }
+
+// What the roles need of the set-up, in shared memory: what a register held from there on would be spilled,
+// and beside this much shared memory a spilled one is read from L2.
+struct Span {
+  int p_lo, p_hi;              // least and largest position of the CTA's rows
+  uint32_t k_size, v_size;     // bits of the largest of its keys and values
+  uint32_t bad;                // whether pages are not there
+  int bound;                   // no token stands there or behind
+  int first, tiles;            // this part's tiles
+  int sink_tiles, win_tile;    // tile t of all is the t-th of the sequence, or from sink_tiles on the (win_tile + t - sink_tiles)-th
+  // the first token of this part's tile j
+  __device__ __forceinline__ int token_of(int j) const {
+    const int t = first + j;
+    return (t < sink_tiles ? t : win_tile + t - sink_tiles) * kTokens;
+  }
+};
 
 // The x lowest bits set (x may be anything).
 __device__ __forceinline__ uint32_t low_bits(int x) {
@@ -264,12 +290,12 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_tc_kernel(const __gr
   uint64_t* drain = pvdone + 2;          // [row tile]: every product has
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 2);
   int* abort_word = reinterpret_cast<int*>(tmem_slot + 1);
-  int* range = abort_word + 2;           // least and largest position of the CTA's rows
-  uint32_t* size = reinterpret_cast<uint32_t*>(range + 2);   // bits of the largest of its keys and values, whether pages are bad
+  Span* span = reinterpret_cast<Span*>(abort_word + 2);
+  static_assert(sizeof(Span) + 12 <= 64, "behind the barriers");
 
   const Kv4AttendArgs& a = p.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int part = blockIdx.x, parts = gridDim.x, row0 = blockIdx.y * kSoftmax, hk = blockIdx.z;
+  const int part = blockIdx.x, parts = gridDim.x, row0 = blockIdx.y * kCtaRows, hk = blockIdx.z;
   const int group = a.heads / a.c.heads;
   const int live = p.rows - row0 > kTileRows ? 2 : 1;   // row tiles with rows
   if (threadIdx.x == 0) {
@@ -285,16 +311,14 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_tc_kernel(const __gr
     }
     for (int i = 0; i < 4; ++i) {
       mbar_init(&sfull[i], 1);
-      mbar_init(&pfull[i], 4);
+      mbar_init(&pfull[i], 8);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&pvdone[i], 1);
       mbar_init(&drain[i], 1);
     }
     abort_word[0] = abort_word[1] = 0;
-    range[0] = 2147483647;
-    range[1] = -1;
-    size[0] = size[1] = size[2] = 0;
+    *span = Span{2147483647, -1, 0, 0, 0, 0, 0, 0, 0, 0};
     fence_mbar_init();
     fence_proxy_async_smem();
   }
@@ -307,9 +331,10 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_tc_kernel(const __gr
   const int length = max(a.prefix_length[0], 0), bound = min(length, cap);
   if (length > cap && threadIdx.x == 0) report(a.status, kBadPrefix, 0);
   // a softmax thread's row: where it stands, -1 where it sees nothing
-  int position = -1;
-  const int row = row0 + (int)threadIdx.x;
+  const int half = (warp >> 2) & 1, rt = (warp >> 3) * kTileRows + (warp & 3) * 32 + lane;   // (of the softmax's threads)
+  const int row = row0 + rt;
   if (threadIdx.x < kSoftmax) {
+    int position = -1;
     int64_t start = -1;   // no row
     if (row < p.rows) {
       const int x = row / group, q = x / a.n;
@@ -317,39 +342,39 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_tc_kernel(const __gr
       const int own = max(a.lengths[q], 0) - a.n + (x - q * a.n);   // only a request's own tokens ask
       if (own >= 0) position = (int)min((int64_t)length + own, (int64_t)2147483646);
     }
-    reinterpret_cast<int64_t*>(smem + L::kRows)[threadIdx.x] = start;
+    if (half == 0) {
+      reinterpret_cast<int64_t*>(smem + L::kRows)[rt] = start;
+      reinterpret_cast<int*>(smem + L::kPositions)[rt] = position;
+    }
     const int least = __reduce_min_sync(0xffffffffu, position < 0 ? 2147483647 : position);
     const int most = __reduce_max_sync(0xffffffffu, position);
     if (lane == 0) {
-      atomicMin(&range[0], least);
-      atomicMax(&range[1], most);
+      atomicMin(&span->p_lo, least);
+      atomicMax(&span->p_hi, most);
     }
   }
   __syncthreads();
   // the tiles of 64 tokens, from multiples of 64 on, that hold what rows see, and this part's of them
-  const int p_lo = range[0], p_hi = range[1];
-  const int window = (int)min(a.window, (int64_t)2147483647), sinks = (int)min(a.sinks, (int64_t)2147483647);
+  Span all_of = *span;
   KeyRanges kr{0, 0, 0};
-  if (p_hi >= 0) kr = key_ranges(p_lo, p_hi, bound, a.window, a.sinks);
-  const int sink_tiles = (int)((kr.first + kTokens - 1) / kTokens);
-  const int win_tile = max((int)(kr.begin / kTokens), sink_tiles);
-  const int all = sink_tiles + max((int)((kr.end + kTokens - 1) / kTokens) - win_tile, 0);
-  const int first = (int)((int64_t)all * part / parts), tiles = (int)((int64_t)all * (part + 1) / parts) - first;
-  auto token_of = [&](int j) {   // of this part's tile j, the first
-    const int v = first + j;
-    return (v < sink_tiles ? v : win_tile + v - sink_tiles) * kTokens;
-  };
+  if (all_of.p_hi >= 0) kr = key_ranges(all_of.p_lo, all_of.p_hi, bound, a.window, a.sinks);
+  all_of.bound = bound;
+  all_of.sink_tiles = (int)((kr.first + kTokens - 1) / kTokens);
+  all_of.win_tile = max((int)(kr.begin / kTokens), all_of.sink_tiles);
+  const int all = all_of.sink_tiles + max((int)((kr.end + kTokens - 1) / kTokens) - all_of.win_tile, 0);
+  all_of.first = (int)((int64_t)all * part / parts);
+  all_of.tiles = (int)((int64_t)all * (part + 1) / parts) - all_of.first;
   const int64_t cell0 = (int64_t)hk << a.c.page_shift;
   const int64_t page_step = (int64_t)a.c.heads << a.c.page_shift;
   const int page_mask = (1 << a.c.page_shift) - 1;
   // Q: eight columns at a time, the DP / 8 lanes of a row together; loads first, all on their way at once
-  constexpr int kQLoads = (kSoftmax * (DP / 8) + kPrefixThreads - 1) / kPrefixThreads;
+  constexpr int kQLoads = (kCtaRows * (DP / 8) + kPrefixThreads - 1) / kPrefixThreads;
   uint4 q_raw[kQLoads];
 #pragma unroll
   for (int i = 0; i < kQLoads; ++i) {
     const int x = i * kPrefixThreads + (int)threadIdx.x, r = x / (DP / 8), c8 = x - r * (DP / 8);
     q_raw[i] = make_uint4(0, 0, 0, 0);
-    const int64_t start = r < kSoftmax ? reinterpret_cast<const int64_t*>(smem + L::kRows)[r] : -1;
+    const int64_t start = r < kCtaRows ? reinterpret_cast<const int64_t*>(smem + L::kRows)[r] : -1;
     if (start >= 0) {
       const T* from = static_cast<const T*>(a.q) + start + c8 * 8;
       if (p.vec_q && c8 * 8 + 8 <= a.c.d) {
@@ -372,8 +397,8 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_tc_kernel(const __gr
     float k_size = 0.0f, v_size = 0.0f;
     bool bad = false;
 #pragma unroll 4
-    for (int x = threadIdx.x; x < tiles * kTokens; x += kPrefixThreads) {
-      const int token = token_of(x / kTokens) + x % kTokens;
+    for (int x = threadIdx.x; x < all_of.tiles * kTokens; x += kPrefixThreads) {
+      const int token = all_of.token_of(x / kTokens) + x % kTokens;
       const int page = token < bound ? __ldg(a.prefix_table + (token >> a.c.page_shift)) : 0;
       const bool out = page < 0 || page >= a.c.pages;
       if (out) {
@@ -392,10 +417,17 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_tc_kernel(const __gr
     const uint32_t v_bits = __reduce_max_sync(0xffffffffu, __float_as_uint(v_size));
     bad = __any_sync(0xffffffffu, bad);
     if (lane == 0) {
-      atomicMax(&size[0], k_bits);
-      atomicMax(&size[1], v_bits);
-      if (bad) atomicOr(&size[2], 1u);
+      atomicMax(&span->k_size, k_bits);
+      atomicMax(&span->v_size, v_bits);
+      if (bad) atomicOr(&span->bad, 1u);
     }
+  }
+  if (threadIdx.x == 0) {
+    span->bound = all_of.bound;
+    span->first = all_of.first;
+    span->tiles = all_of.tiles;
+    span->sink_tiles = all_of.sink_tiles;
+    span->win_tile = all_of.win_tile;
   }
   // Q in the order 0 4 1 5 2 6 3 7, times the row's power; behind it the sums' pieces, which meet the
   // offsets' as 1 1 1 2 2 3
@@ -426,7 +458,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_tc_kernel(const __gr
 #pragma unroll
     for (int d = 1; d < DP / 8; d *= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
     const int t = r / kTileRows, rt = r % kTileRows;
-    if (r >= kSoftmax) continue;
+    if (r >= kCtaRows) continue;
     *reinterpret_cast<uint4*>(smem + t * L::kQ + (c8 >> 3) * (kTileRows * 128) + rt * 128 + (((c8 & 7) ^ (rt & 7)) << 4)) =
         make_uint4(pack_f16(v[0], v[4]), pack_f16(v[1], v[5]), pack_f16(v[2], v[6]), pack_f16(v[3], v[7]));
     if (c8 < 2) {
@@ -445,60 +477,65 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_tc_kernel(const __gr
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  const int k_power = power_for(__uint_as_float(size[0]), 9), v_power = power_for(__uint_as_float(size[1]), 9);
+  const volatile Span* now = span;
+  const int tiles = now->tiles;
   const Abort ab{abort_word, a.status, p.wait_ns};
 
   if (threadIdx.x < kSoftmax) {
     // ------------------------------------------------------------ softmax rows
     more_registers<kSoftmaxRegs>();
-    const int t = warp >> 2;
+    const int t = warp >> 3;
     if (t < live) {
       const uint32_t at = (uint32_t)((warp & 3) * 32) << 16;
-      const uint32_t tO = tmem + 256 + t * 128 + at;
-      const int q_power = reinterpret_cast<const int*>(smem + L::kPowers)[threadIdx.x];
+      const uint32_t tO = tmem + 256 + t * 128 + at + half * (DP / 2);
+      const int q_power = reinterpret_cast<const volatile int*>(smem + L::kPowers)[rt];
+      const int position = reinterpret_cast<const volatile int*>(smem + L::kPositions)[rt];
+      const int k_power = power_for(__uint_as_float(now->k_size), 9);
+      const Span sp{0, now->p_hi, 0, now->v_size, now->bad, now->bound, now->first, tiles, now->sink_tiles, now->win_tile};
+      const int window = (int)min(a.window, (int64_t)2147483647), sinks = (int)min(a.sinks, (int64_t)2147483647);
+      float* tops = reinterpret_cast<float*>(smem + L::kTops);
+      const int pair = 1 + t * 4 + (warp & 3);   // the barrier of the two warps of 32 rows
       // scores in base 2 from the products; the powers one after the other, since their product may leave the range
       // (0, of a scale of 0, would make NaN of a hidden score: the least that is none)
       const float c2s = fabsf(a.scale) * 1.4426950408889634f * power(-q_power) * power(-k_power), c2 = c2s == 0.0f ? 1.17549435e-38f : c2s;
       const uint64_t c22 = pack2(c2, c2);
-      const bool bad = size[2] != 0;
       float m = -INFINITY, l = 0.0f;
       bool ok = true;
 #pragma unroll 1
       for (int j = 0; j < tiles; ++j) {
         const int buf = j & 1;
         // whether every row that sees anything sees all 64 tokens
-        const int t0 = token_of(j);
-        const bool whole = !bad && t0 + kTokens <= bound && (p_hi - t0 < window || t0 + kTokens <= sinks);
+        const int t0 = sp.token_of(j);
+        const bool whole = !sp.bad && t0 + kTokens <= sp.bound && (sp.p_hi - t0 < window || t0 + kTokens <= sinks);
         ok = mbar_wait_warp_lazy(&sfull[2 * t + buf], (j >> 1) & 1, ab, kErrS);
         if (!ok) break;
         tc_fence_after();
         const uint32_t ts = tmem + t * 128 + buf * kTokens + at;
-        float s0[32], s1[32];
-        tmem_ld32(ts, s0);
-        tmem_ld32(ts + 32, s1);
+        float s[32];
+        tmem_ld32(ts + half * kHalf, s);
         tmem_wait_ld();
-        tie32(s0);
-        tie32(s1);
+        tie32(s);
         if (!whole) {
           // token j: j < bound and (j > position - window or j < sinks); j <= position always
-          auto seen = [&](int j0) {
-            const uint32_t near = position - j0 < window ? 0xffffffffu : ~low_bits(position - j0 - window + 1);
-            uint32_t on = low_bits(bound - j0) & (near | low_bits(sinks - j0));
-            for (int b = 0; bad && b < 2; ++b) {   // a page that is not there
-              const int at = j0 + 16 * b, page = at < bound ? __ldg(a.prefix_table + (at >> a.c.page_shift)) : 0;
-              if (page < 0 || page >= a.c.pages) on &= 0xffff0000u >> (16 * b);
-            }
-            return on;
-          };
-          const uint32_t on0 = seen(t0), on1 = seen(t0 + 32);
-#pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            s0[e] = (on0 >> e) & 1u ? s0[e] : -INFINITY;
-            s1[e] = (on1 >> e) & 1u ? s1[e] : -INFINITY;
+          const int j0 = t0 + half * kHalf;
+          const uint32_t near = position - j0 < window ? 0xffffffffu : ~low_bits(position - j0 - window + 1);
+          uint32_t on = low_bits(sp.bound - j0) & (near | low_bits(sinks - j0));
+          for (int b = 0; sp.bad && b < 2; ++b) {   // a page that is not there
+            const int first16 = j0 + 16 * b, page = first16 < sp.bound ? __ldg(a.prefix_table + (first16 >> a.c.page_shift)) : 0;
+            if (page < 0 || page >= a.c.pages) on &= 0xffff0000u >> (16 * b);
           }
+#pragma unroll
+          for (int e = 0; e < 32; ++e) s[e] = (on >> e) & 1u ? s[e] : -INFINITY;
         }
-        const float raw = fmaxf(max32(s0), max32(s1));
-        const float top = raw * c2;
+        // the row's maximum: both its threads hear of both halves (and have read their scores, which P overwrites)
+        const float mine = max32(s);
+        tops[(buf * 2 + half) * kCtaRows + rt] = mine;
+        pair_sync(pair);
+        if (*ab.cta) {   // the other warp may be gone
+          ok = false;
+          break;
+        }
+        const float top = fmaxf(mine, tops[(buf * 2 + (half ^ 1)) * kCtaRows + rt]) * c2;
         const bool move = top > m + kMove;
         if (__any_sync(0xffffffffu, move)) {
           const float to = move ? top : m;
@@ -509,14 +546,12 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_tc_kernel(const __gr
             ok = mbar_wait_warp_lazy(&pvdone[t], (j - 1) & 1, ab, kErrO);
             if (!ok) break;
             tc_fence_after();
-            scale_row(tO, DP, alpha);
+            scale_row(tO, DP / 2, alpha);
           }
         }
         const float off = kShiftP - (m == -INFINITY ? 0.0f : m);
-        const uint64_t off2 = pack2(off, off);
         uint64_t sum2[2] = {0, 0};
-        exp_chunk(s0, c22, off2, sum2, ts);
-        exp_chunk(s1, c22, off2, sum2, ts + 16);
+        exp_chunk(s, c22, pack2(off, off), sum2, ts + half * (kHalf / 2));
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
@@ -526,6 +561,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_tc_kernel(const __gr
         unpack2(sum2[1], x2, x3);
         l += (x0 + x1) + (x2 + x3);
       }
+      if (!ok) pair_leave(pair);   // nobody waits for this warp
       if (ok && tiles > 0) {
         // not pvdone: P V of the last tile but one may still run too, and a parity tells only neighbours apart
         ok = mbar_wait_warp_lazy(&drain[t], 0, ab, kErrO);
@@ -533,11 +569,10 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_tc_kernel(const __gr
       }
       // this part's sums, as kTail's own p has them: [part][key head][columns / 4][row][4]
       const int64_t of = (int64_t)part * a.c.heads + hk;
-      const bool seen = ok && tiles > 0 && position >= 0, some = seen && m != -INFINITY;
-      const float f = power((int)(kShift - kShiftP)), fo = f * power(-v_power);
-      if (row < p.rows) a.part_ml[of * p.rows + row] = seen ? make_float2(m, l * f) : make_float2(-INFINITY, 0.0f);
+      const bool some = ok && tiles > 0 && position >= 0 && m != -INFINITY;
+      const float f = power((int)(kShift - kShiftP)), fo = f * power(-power_for(__uint_as_float(sp.v_size), 9));
 #pragma unroll 1
-      for (int c = 0; c < DP; c += 16) {
+      for (int c = 0; c < DP / 2; c += 16) {
         float o[16];
         if (tiles > 0) {
           tmem_ld16(tO + c, o);
@@ -547,10 +582,16 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_tc_kernel(const __gr
 #pragma unroll
         for (int e = 0; e < 16; e += 4)
           if (row < p.rows)
-            *reinterpret_cast<float4*>(a.part_o + ((of * (DP / 4) + (c + e) / 4) * p.rows + row) * 4) =
+            *reinterpret_cast<float4*>(a.part_o + ((of * (DP / 4) + (half * (DP / 2) + c + e) / 4) * p.rows + row) * 4) =
                 some ? make_float4(o[e] * fo, o[e + 1] * fo, o[e + 2] * fo, o[e + 3] * fo) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
       }
       tc_fence_before();
+      // maximum and total: the other half's through shared memory, behind the last barrier
+      const bool seen = ok && tiles > 0 && position >= 0;
+      if (half == 0)   // (where rows of q start, and positions, are not needed any more)
+        reinterpret_cast<float2*>(smem + L::kRows)[rt] = seen ? make_float2(m, l * f) : make_float2(-INFINITY, 0.0f);
+      else
+        reinterpret_cast<float*>(smem + L::kPositions)[rt] = seen ? l * f : 0.0f;
     }
   } else if (warp < kIssuer) {
     // ------------------------------------------------------------ codes to tiles
@@ -563,7 +604,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_tc_kernel(const __gr
       // stores fall into different banks
       constexpr int kPieces = DP / 32;
       constexpr int kLoads = (kTokens * kPieces + kDecoders - 1) / kDecoders;
-      const float f = power(k_power);
+      const float f = power(power_for(__uint_as_float(now->k_size), 9));
 #pragma unroll 1
       for (int j = 0; j < tiles; ++j) {
         const int s = j % kStages, rs = j % L::kRawStages;
@@ -621,7 +662,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_tc_kernel(const __gr
       // (the columns turned by them, so that neither loads nor stores fall into one bank); quad < DP / 8
       constexpr int kTurn = DP >= 64 ? 8 : 4;
       const int chunk = d & 7, quad = ((d >> 3) & ~(kTurn - 1)) + (((d >> 3) + chunk) & (kTurn - 1));
-      const float f = power(v_power);
+      const float f = power(power_for(__uint_as_float(now->v_size), 9));
 #pragma unroll 1
       for (int j = 0; j < tiles; ++j) {
         const int s = j % kStages, rs = j % L::kRawStages;
@@ -685,6 +726,9 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_tc_kernel(const __gr
       // a tile is one run of tokens in a page, or of two or four in pages of 32 and 16: a lane for each and each of
       // keys, values and their parameters
       const int runs = max(kTokens >> a.c.page_shift, 1), tokens = kTokens / runs;
+      const Span sp{0, 0, 0, 0, 0, now->bound, now->first, tiles, now->sink_tiles, now->win_tile};
+      const int64_t cell0 = (int64_t)hk << a.c.page_shift, page_step = (int64_t)a.c.heads << a.c.page_shift;
+      const int page_mask = (1 << a.c.page_shift) - 1;
       const int what = lane / runs, run = lane - what * runs;
       int page_l = 0;   // pages of 32 runs, one a lane: 32 / runs tiles
       int sent = 0;
@@ -692,16 +736,16 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_tc_kernel(const __gr
       for (int j = 0; j < tiles; ++j) {
         const int rs = j % L::kRawStages, at = j % (32 / runs) * runs;
         if (at == 0) {
-          const int token = token_of(min(j + lane / runs, tiles - 1)) + lane % runs * tokens;
-          page_l = token < bound ? __ldg(a.prefix_table + (token >> a.c.page_shift)) : -1;
+          const int token = sp.token_of(min(j + lane / runs, tiles - 1)) + lane % runs * tokens;
+          page_l = token < sp.bound ? __ldg(a.prefix_table + (token >> a.c.page_shift)) : -1;
           if (page_l >= a.c.pages) page_l = -1;   // reported above
         }
-        const int page = __shfl_sync(0xffffffffu, page_l, at + run), token = token_of(j) + run * tokens;
+        const int page = __shfl_sync(0xffffffffu, page_l, at + run), token = sp.token_of(j) + run * tokens;
         // what stands in a block of 16: four lanes say (runs are multiples of that)
         const int block_page = __shfl_sync(0xffffffffu, page_l, at + (lane & 3) * 16 / tokens);
         if (j >= L::kRawStages && !mbar_wait_warp_lazy(&rempty[rs], ((j / L::kRawStages) - 1) & 1, ab, kErrRaw)) break;
         uint8_t* raw = smem + L::kRaws + rs * L::kRaw;
-        if (lane < 4) reinterpret_cast<int*>(raw + L::kRawInfo)[lane] = block_page < 0 ? 0 : bound - token_of(j) - lane * 16;
+        if (lane < 4) reinterpret_cast<int*>(raw + L::kRawInfo)[lane] = block_page < 0 ? 0 : sp.bound - sp.token_of(j) - lane * 16;
         __syncwarp();
         if (lane == 0) mbar_arrive_expect_tx(&rfull[rs], kTokens * DP + 2 * kTokens * 4);
         __syncwarp();
@@ -796,6 +840,11 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_tc_kernel(const __gr
   }
   __syncthreads();
   tc_fence_after();
+  if (threadIdx.x < kCtaRows && blockIdx.y * kCtaRows + threadIdx.x < p.rows) {
+    const float2 ml = reinterpret_cast<const float2*>(smem + L::kRows)[threadIdx.x];
+    a.part_ml[((int64_t)blockIdx.x * a.c.heads + blockIdx.z) * p.rows + blockIdx.y * kCtaRows + threadIdx.x] =
+        make_float2(ml.x, ml.y + reinterpret_cast<const float*>(smem + L::kPositions)[threadIdx.x]);
+  }
   if (warp == kIssuer) tmem_dealloc(tmem, 512);
 }
 
@@ -810,7 +859,7 @@ int launch_prefix(const Kv4AttendArgs& a, int64_t rows, cudaStream_t s) {
   p.rows = (int)rows;
   p.vec_q = rows_aligned(a.q, elem_size(a.dtype), a.q_r | a.q_n, a.q_h);
   p.wait_ns = wait_limit_ns();
-  const int64_t pairs = ceil_div(rows, kSoftmax);
+  const int64_t pairs = ceil_div(rows, kCtaRows);
   if (a.c.heads > 65535 || pairs > 65535) return set_error(SA_ERR_UNSUPPORTED, "kv4 prefix: grid too large");
   kern<<<dim3((unsigned)a.parts, (unsigned)pairs, (unsigned)a.c.heads), kPrefixThreads, L::kBytes, s>>>(p);
   return check_launch("kv4 prefix_tc_kernel");
@@ -826,7 +875,7 @@ bool kv4_prefix_tc_takes(const Kv4AttendArgs& a, int64_t rows) {
 // fill the GPU, of two tiles at least.
 int kv4_prefix_tc_parts(const Kv4AttendArgs& a, int64_t rows) {
   const int64_t longest = std::min<int64_t>((int64_t)a.prefix_width << a.c.page_shift, a.window + a.sinks + a.n);
-  const int64_t ctas = ceil_div(rows, kSoftmax) * a.c.heads;
+  const int64_t ctas = ceil_div(rows, kCtaRows) * a.c.heads;
   return (int)std::max<int64_t>(1, std::min(148 / ctas, ceil_div(longest, 2 * kTokens)));
 }
 
