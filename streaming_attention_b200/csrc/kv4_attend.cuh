@@ -629,7 +629,8 @@ __global__ void __launch_bounds__(kWarps * 32, (Shape<DT, DP, NT, kWarps>::kPerS
   }
   __syncthreads();
   // warp 0's place takes the CTA's: each thread a row's four columns, warps in order
-  for (int x = threadIdx.x; x < S::kRows * DP / 4; x += kThreads) {
+  const int valid = min(S::kRows, rows - row0);
+  for (int x = threadIdx.x; x < valid * (DP / 4); x += kThreads) {
     const int row = x / (DP / 4), col = (x - row * (DP / 4)) * 4;
     float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
@@ -648,69 +649,76 @@ __global__ void __launch_bounds__(kWarps * 32, (Shape<DT, DP, NT, kWarps>::kPerS
     cluster.sync();
   else
     __syncthreads();
-  // and the cluster's CTAs, each a share of the columns
-  const int share = S::kRows * DP / splits;
-  for (int x = blockIdx.x * share + threadIdx.x; x < (blockIdx.x + 1) * share; x += kThreads) {
-    // the parts of a prefix stand as [columns / 4][row][4]: threads follow them
-    constexpr bool kParts = kMode == kPrefix || kMode == kTail;
-    const int row = kParts ? (x >> 2) % S::kRows : x / DP, col = kParts ? (x >> 2) / S::kRows * 4 + (x & 3) : x - row * DP;
-    float top = -INFINITY, sum = 0.0f, total = 0.0f;
+  // and the cluster's CTAs, each a share of the rows' four columns (where a prefix's parts are read or written,
+  // neighbouring threads take neighbouring rows, as they stand there)
+  constexpr bool kParts = kMode == kPrefix || kMode == kTail;
+  const int share = (valid * (DP / 4) + splits - 1) / splits, share_end = min((int)(blockIdx.x + 1) * share, valid * (DP / 4));
+  for (int x = blockIdx.x * share + threadIdx.x; x < share_end; x += kThreads) {
+    const int row = kParts ? x % valid : x / (DP / 4), col = (kParts ? x / valid : x - row * (DP / 4)) * 4;
+    float top = -INFINITY, total = 0.0f;
+    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    auto add = [&](float f, const float4& o) {
+      sum[0] = fmaf(f, o.x, sum[0]);
+      sum[1] = fmaf(f, o.y, sum[1]);
+      sum[2] = fmaf(f, o.z, sum[2]);
+      sum[3] = fmaf(f, o.w, sum[3]);
+    };
     for (int s = 0; s < splits; ++s) top = fmaxf(top, splits > 1 ? *cluster.map_shared_rank(part_m + row, s) : part_m[row]);
     for (int s = 0; s < splits; ++s) {
       const float ms = splits > 1 ? *cluster.map_shared_rank(part_m + row, s) : part_m[row];
       const float ls = splits > 1 ? *cluster.map_shared_rank(part_l + row, s) : part_l[row];
-      const float os = splits > 1 ? *cluster.map_shared_rank(sm_o + row * S::kPitch + col, s) : sm_o[row * S::kPitch + col];
+      const float* from = sm_o + row * S::kPitch + col;
+      const float4 os = *reinterpret_cast<const float4*>(splits > 1 ? cluster.map_shared_rank(from, s) : from);
       const float f = ms == -INFINITY ? 0.0f : ex2(ms - top);
-      sum = fmaf(f, os, sum);
+      add(f, os);
       total = fmaf(f, ls, total);
     }
     if (kMode == kPrefix) {   // unfinished: kTail joins the parts
-      if (row0 + row < rows) {
-        const int64_t of = (int64_t)part * a.c.heads + hk;
-        a.part_o[((of * (DP / 4) + (col >> 2)) * rows + row0 + row) * 4 + (col & 3)] = sum;
-        if (col == 0) a.part_ml[of * rows + row0 + row] = make_float2(top, total);
-      }
+      const int64_t of = (int64_t)part * a.c.heads + hk;
+      reinterpret_cast<float4*>(a.part_o)[(of * (DP / 4) + (col >> 2)) * rows + row0 + row] = make_float4(sum[0], sum[1], sum[2], sum[3]);
+      if (col == 0) a.part_ml[of * rows + row0 + row] = make_float2(top, total);
       continue;
     }
-    if (row0 + row < rows && col < a.c.d) {
-      if (kMode == kTail) {   // the prefix's parts, in order, kBatch of them on their way at a time
-        constexpr int kBatch = 10;
-        const int64_t all = (int64_t)a.requests * rows, at = (int64_t)r * rows + row0 + row;
-        const int64_t part_ml = a.c.heads * all, part_o = part_ml * DP;
-        const float2* from_ml = a.part_ml + hk * all + at;
-        const float* from_o = a.part_o + ((hk * (DP / 4) + (col >> 2)) * all + at) * 4 + (col & 3);
-        for (int s0 = 0; s0 < a.parts; s0 += kBatch, from_ml += kBatch * part_ml, from_o += kBatch * part_o) {
-          float2 ml[kBatch];
-          float o[kBatch];
-          float next = top;
+    if (kMode == kTail) {   // the prefix's parts, in order, kBatch of them on their way at a time
+      constexpr int kBatch = 6;
+      const int64_t all = (int64_t)a.requests * rows, at = (int64_t)r * rows + row0 + row;
+      const int64_t ml_step = a.c.heads * all, o_step = ml_step * (DP / 4);
+      const float2* from_ml = a.part_ml + hk * all + at;
+      const float4* from_o = reinterpret_cast<const float4*>(a.part_o) + (hk * (DP / 4) + (col >> 2)) * all + at;
+      for (int s0 = 0; s0 < a.parts; s0 += kBatch, from_ml += kBatch * ml_step, from_o += kBatch * o_step) {
+        float2 ml[kBatch];
+        float4 o[kBatch];
+        float next = top;
 #pragma unroll
-          for (int s = 0; s < kBatch; ++s) {
-            ml[s] = s0 + s < a.parts ? from_ml[s * part_ml] : make_float2(-INFINITY, 0.0f);
-            o[s] = s0 + s < a.parts ? from_o[s * part_o] : 0.0f;
-          }
-#pragma unroll
-          for (int s = 0; s < kBatch; ++s) next = fmaxf(next, ml[s].x);
-          const float f = top == -INFINITY ? 1.0f : ex2(top - next);   // nothing yet: zeros, or NaN that stays
-          sum *= f;
-          total *= f;
-#pragma unroll
-          for (int s = 0; s < kBatch; ++s) {
-            const float g = ml[s].x == -INFINITY ? 1.0f : ex2(ml[s].x - next);
-            sum = fmaf(g, o[s], sum);
-            total = fmaf(g, ml[s].y, total);
-          }
-          top = next;
+        for (int s = 0; s < kBatch; ++s) {
+          ml[s] = s0 + s < a.parts ? from_ml[s * ml_step] : make_float2(-INFINITY, 0.0f);
+          o[s] = s0 + s < a.parts ? from_o[s * o_step] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         }
+#pragma unroll
+        for (int s = 0; s < kBatch; ++s) next = fmaxf(next, ml[s].x);
+        const float f = top == -INFINITY ? 1.0f : ex2(top - next);   // nothing yet: zeros, or NaN that stays
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum[e] *= f;
+        total *= f;
+#pragma unroll
+        for (int s = 0; s < kBatch; ++s) {
+          const float g = ml[s].x == -INFINITY ? 1.0f : ex2(ml[s].x - next);
+          add(g, o[s]);
+          total = fmaf(g, ml[s].y, total);
+        }
+        top = next;
       }
-      const int i = kMode == kSelected ? (int)(blockIdx.z % a.n) : (row0 + row) / group;
-      const int h = hk * group + row0 + row - (kMode == kSelected ? 0 : i * group);
-      T* out = static_cast<T*>(a.out) + (((int64_t)r * a.n + i) * a.heads + h) * a.c.d;
-      out[col] = from_f32<T>(total == 0.0f ? 0.0f : sum / total);
-      // p = 2^(s + kShift - top) / total
-      if (kMode == kWeigh && col == 0)
-        a.score_ml[((int64_t)r * a.c.heads + hk) * a.score_rows + row0 + row] =
-            make_float2(kShift - top, total == 0.0f ? 0.0f : 1.0f / total);
     }
+    const int i = kMode == kSelected ? (int)(blockIdx.z % a.n) : (row0 + row) / group;
+    const int h = hk * group + row0 + row - (kMode == kSelected ? 0 : i * group);
+    T* out = static_cast<T*>(a.out) + (((int64_t)r * a.n + i) * a.heads + h) * a.c.d + col;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (col + e < a.c.d) out[e] = from_f32<T>(total == 0.0f ? 0.0f : sum[e] / total);
+    // p = 2^(s + kShift - top) / total
+    if (kMode == kWeigh && col == 0)
+      a.score_ml[((int64_t)r * a.c.heads + hk) * a.score_rows + row0 + row] =
+          make_float2(kShift - top, total == 0.0f ? 0.0f : 1.0f / total);
   }
   if (splits > 1) cluster.sync();   // nobody leaves while its shared memory is read
 }
