@@ -4,6 +4,7 @@ and the device's error word."""
 from __future__ import annotations
 
 import ctypes
+import functools
 from typing import Optional, Tuple
 
 import torch
@@ -100,13 +101,18 @@ def check_window(window: Optional[int], sinks: int) -> Tuple[int, int]:
     return min(w, 1 << 40), min(s, 1 << 40)
 
 
-def workspace(dev: torch.device, name: str, *sizes: int) -> Tensor:
-    """Device memory of the size that the entry point `name` asks for."""
+@functools.lru_cache(maxsize=1024)
+def _workspace_size(name: str, *sizes: int) -> int:
     nbytes = ctypes.c_size_t(0)
     rc = getattr(_lib.load(), name)(*sizes, ctypes.byref(nbytes))
     if rc:
         _lib.check(rc, name)
-    return torch.empty(nbytes.value, device=dev, dtype=torch.uint8)
+    return nbytes.value
+
+
+def workspace(dev: torch.device, name: str, *sizes: int) -> Tensor:
+    """Device memory of the size that the entry point `name` asks for."""
+    return torch.empty(_workspace_size(name, *sizes), device=dev, dtype=torch.uint8)
 
 
 def _raw_stream(index: int) -> int:

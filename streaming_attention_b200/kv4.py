@@ -143,9 +143,10 @@ class Kv4Cache:
     def _bind(self) -> None:
         """Checks the four tensors as they are now and keeps what the calls need of them."""
         held = k_codes, k_params, v_codes, v_params = self.k_codes, self.k_params, self.v_codes, self.v_params
-        if k_codes.ndim != 4:
+        shape = k_codes.shape
+        if len(shape) != 4:
             raise ValueError("k_codes must be [P,Hkv,page,Dp/2]")
-        pages, heads, page, half = k_codes.shape
+        pages, heads, page, half = shape
         if page not in PAGE_SIZES:
             _check_page_size(page)
         if pages == 0 or heads == 0:
@@ -154,12 +155,12 @@ class Kv4Cache:
             raise ValueError(f"a row of codes of dim {self.dim} takes {self.padded_dim(self.dim) // 2} bytes, got {half}")
         device = S.device_of(k_codes, k_params, v_codes, v_params)
         params = (pages, heads, page, 2)
-        for t, shape, dt, what in ((k_codes, None, torch.uint8, "k_codes"),
-                                   (v_codes, (pages, heads, page // 4, half, 4), torch.uint8, "v_codes"),
-                                   (k_params, params, torch.bfloat16, "k_params"),
-                                   (v_params, params, torch.bfloat16, "v_params")):
-            if t.dtype != dt or (shape is not None and t.shape != shape) or not t.is_contiguous():
-                raise ValueError(f"{what} must be contiguous {dt} {list(shape or k_codes.shape)}")
+        for t, want, dt, what in ((k_codes, shape, torch.uint8, "k_codes"),
+                                  (v_codes, (pages, heads, page // 4, half, 4), torch.uint8, "v_codes"),
+                                  (k_params, params, torch.bfloat16, "k_params"),
+                                  (v_params, params, torch.bfloat16, "v_params")):
+            if t.dtype != dt or t.shape != want or not t.is_contiguous():
+                raise ValueError(f"{what} must be contiguous {dt} {list(want)}")
         self.device, self.kv_heads, self.page_size, self.num_pages = device, heads, page, pages
         self._held, self._ptrs = held, (k_codes.data_ptr(), k_params.data_ptr(), v_codes.data_ptr(), v_params.data_ptr())
         self._args = (*self._ptrs, pages, heads, page, self.dim)
@@ -228,20 +229,33 @@ class Kv4Cache:
         return k, v
 
     def _queries(self, q: Tensor, tables: Tensor, lengths: Tensor):
-        """q as [R,N,H,D] with contiguous rows, tables and lengths as the kernels read them,
-        the element type's code and a new result."""
-        code = S.dtype_code(q)
-        if q.ndim not in (3, 4):
+        """q [R,H,D] or [R,N,H,D], tables and lengths as the kernels read them: pointers and
+        sizes for a call (q, its strides, tables, lengths; R, N, H, W; the element type's code), and
+        the tensors that they are of."""
+        shape = q.shape
+        if len(shape) == 4:
+            r, n, heads, d = shape
+        elif len(shape) == 3:
+            r, heads, d = shape
+            n = 1
+        else:
             raise ValueError("q must be [R,H,D] or [R,N,H,D]")
-        q4 = q[:, None] if q.ndim == 3 else q
-        r, n, heads, d = q4.shape
+        code = S.DTYPES.get(q.dtype)
+        if code is None:
+            code = S.dtype_code(q)
         if d != self.dim or heads == 0 or heads % self.kv_heads:
             raise ValueError(f"q must have head width {self.dim} and a multiple of {self.kv_heads} heads")
-        if tables.ndim != 2 or tables.shape[0] != r:
+        table_shape = tables.shape
+        if len(table_shape) != 2 or table_shape[0] != r:
             raise ValueError(f"tables must be [{r},W]")
-        tables = S.int32(tables, tables.shape, "tables")
+        tables = S.int32(tables, table_shape, "tables")
         lengths = S.int32(lengths, (r,), "lengths")
-        return S.rows(q4), tables, lengths, code
+        st = q.stride()
+        if st[-1] != 1 and d > 1:
+            q = q.detach().contiguous()
+            st = q.stride()
+        st = S.strides(st[0], st[1], st[2]) if len(shape) == 4 else S.strides(st[0], 0, st[1])
+        return ((q.data_ptr(), st, tables.data_ptr(), lengths.data_ptr()), (r, n, heads, table_shape[1]), code, (q, tables, lengths))
 
     def _scale(self, scale: Optional[float]) -> float:
         return float(1.0 / math.sqrt(self.dim) if scale is None else scale)
@@ -260,23 +274,24 @@ class Kv4Cache:
         token's slot the softmax weight it had, summed over the N queries and the
         heads that read the key head.  No page may then stand in two requests' tables."""
         cache = self._storage()
-        S.device_of(self.k_codes, q, tables, lengths, *(() if weights is None else (weights,)))
-        w, s = S.check_window(window, sinks)
-        q4, tables, lengths, code = self._queries(q, tables, lengths)
-        if weights is not None:
+        if weights is None:
+            S.device_of(self.k_codes, q, tables, lengths)
+        else:
+            S.device_of(self.k_codes, q, tables, lengths, weights)
             self._check_weights(weights)
-        r, n, heads, d = q4.shape
-        out = torch.empty((r, n, heads, d), device=self.device, dtype=q.dtype)
-        if out.numel():
-            args = (*cache, q4.data_ptr(), out.data_ptr(), S.strides(*q4.stride()[:3]), tables.data_ptr(),
-                    lengths.data_ptr(), r, n, heads, tables.shape[1], w, s, self._scale(scale), code)
+        w, s = S.check_window(window, sinks)
+        (qp, st, tp, lp), (r, n, heads, width), code, held = self._queries(q, tables, lengths)
+        out = q.new_empty(q.shape)
+        if r and n:
             if weights is None:
-                S.launch(self.device, "sa_kv4_attend", *args)
+                S.launch(self.device, "sa_kv4_attend", *cache, qp, out.data_ptr(), st, tp, lp, r, n, heads, width, w, s,
+                         self._scale(scale), code)
             else:
                 ws = S.workspace(self.device, "sa_kv4_attend_weigh_workspace_size", self.kv_heads, self.page_size, r, n,
-                                 heads, tables.shape[1], w, s)
-                S.launch(self.device, "sa_kv4_attend_weigh", *args, weights.data_ptr(), ws.data_ptr(), ws.numel())
-        return out[:, 0] if q.ndim == 3 else out
+                                 heads, width, w, s)
+                S.launch(self.device, "sa_kv4_attend_weigh", *cache, qp, out.data_ptr(), st, tp, lp, r, n, heads, width, w, s,
+                         self._scale(scale), code, weights.data_ptr(), ws.data_ptr(), ws.numel())
+        return out
 
     def attend_shared(self, q: Tensor, prefix_table: Tensor, prefix_length: Tensor, tables: Tensor, lengths: Tensor, *,
                       window: Optional[int] = None, sinks: int = 0, scale: Optional[float] = None) -> Tensor:
@@ -289,21 +304,20 @@ class Kv4Cache:
         cache = self._storage()
         S.device_of(self.k_codes, q, prefix_table, prefix_length, tables, lengths)
         w, s = S.check_window(window, sinks)
-        q4, tables, lengths, code = self._queries(q, tables, lengths)
-        if prefix_table.ndim != 1:
+        (qp, st, tp, lp), (r, n, heads, width), code, held = self._queries(q, tables, lengths)
+        prefix_shape = prefix_table.shape
+        if len(prefix_shape) != 1:
             raise ValueError("prefix_table must be [W0]")
-        prefix_table = S.int32(prefix_table, prefix_table.shape, "prefix_table")
+        prefix_table = S.int32(prefix_table, prefix_shape, "prefix_table")
         prefix_length = S.int32(prefix_length, (1,), "prefix_length")
-        r, n, heads, d = q4.shape
-        out = torch.empty((r, n, heads, d), device=self.device, dtype=q.dtype)
-        if out.numel():
-            ws = S.workspace(self.device, "sa_kv4_attend_shared_workspace_size", self.kv_heads, self.page_size, d, r, n, heads,
-                             prefix_table.shape[0], w, s, code)
-            S.launch(self.device, "sa_kv4_attend_shared", *cache, q4.data_ptr(), out.data_ptr(), S.strides(*q4.stride()[:3]),
-                     prefix_table.data_ptr(), prefix_length.data_ptr(), prefix_table.shape[0], tables.data_ptr(),
-                     lengths.data_ptr(), r, n, heads, tables.shape[1], w, s, self._scale(scale), code, ws.data_ptr(),
-                     ws.numel())
-        return out[:, 0] if q.ndim == 3 else out
+        out = q.new_empty(q.shape)
+        if r and n:
+            ws = S.workspace(self.device, "sa_kv4_attend_shared_workspace_size", self.kv_heads, self.page_size, self.dim, r, n,
+                             heads, prefix_shape[0], w, s, code)
+            S.launch(self.device, "sa_kv4_attend_shared", *cache, qp, out.data_ptr(), st, prefix_table.data_ptr(),
+                     prefix_length.data_ptr(), prefix_shape[0], tp, lp, r, n, heads, width, w, s, self._scale(scale), code,
+                     ws.data_ptr(), ws.numel())
+        return out
 
     def attend_pages(self, q: Tensor, tables: Tensor, lengths: Tensor, pages: Tensor, *,
                      scale: Optional[float] = None) -> Tensor:
@@ -313,18 +327,17 @@ class Kv4Cache:
         up to its own that stand in them."""
         cache = self._storage()
         S.device_of(self.k_codes, q, tables, lengths, pages)
-        q4, tables, lengths, code = self._queries(q, tables, lengths)
-        r, n, heads, d = q4.shape
+        (qp, st, tp, lp), (r, n, heads, width), code, held = self._queries(q, tables, lengths)
         lead = (r, self.kv_heads) if q.ndim == 3 else (r, n, self.kv_heads)
         if pages.ndim != len(lead) + 1:
             raise ValueError(f"pages must be {[*lead, 'K']}")
-        pages = S.int32(pages, (*lead, pages.shape[-1]), "pages")
-        out = torch.empty((r, n, heads, d), device=self.device, dtype=q.dtype)
-        if out.numel():
-            S.launch(self.device, "sa_kv4_attend_pages", *cache, q4.data_ptr(), out.data_ptr(), S.strides(*q4.stride()[:3]),
-                     tables.data_ptr(), lengths.data_ptr(), pages.data_ptr(), pages.shape[-1], r, n, heads, tables.shape[1],
-                     self._scale(scale), code)
-        return out[:, 0] if q.ndim == 3 else out
+        count = pages.shape[-1]
+        pages = S.int32(pages, (*lead, count), "pages")
+        out = q.new_empty(q.shape)
+        if r and n:
+            S.launch(self.device, "sa_kv4_attend_pages", *cache, qp, out.data_ptr(), st, tp, lp, pages.data_ptr(), count, r, n,
+                     heads, width, self._scale(scale), code)
+        return out
 
     def page_bounds(self) -> Tensor:
         """Room for the bounds of every page's keys, bfloat16 [P,Hkv,2,Dp], zeros."""
@@ -367,19 +380,17 @@ class Kv4Cache:
         self._storage()
         S.device_of(self.k_codes, q, bounds, tables, lengths)
         self._check_bounds(bounds)
-        q4, tables, lengths, code = self._queries(q, tables, lengths)
+        (qp, st, tp, lp), (r, n, heads, width), code, held = self._queries(q, tables, lengths)
         count, first, last = S.whole(count, "count"), S.whole(first, "first"), S.whole(last, "last")
         if count < 0 or count > 2 ** 31 - 1:
             raise ValueError("count must lie in [0, 2^31)")
         if first < 0 or last < 0 or first + last > count:
             raise ValueError("first and last must be non-negative, and no more than count together")
-        r, n, heads, _ = q4.shape
-        out = torch.empty((r, n, self.kv_heads, count), device=self.device, dtype=torch.int32)
-        if out.numel():
+        out = lengths.new_empty((r, self.kv_heads, count) if q.ndim == 3 else (r, n, self.kv_heads, count))
+        if r and n and count:
             S.launch(self.device, "sa_kv4_select_pages", bounds.data_ptr(), self.num_pages, self.kv_heads, self.page_size,
-                     self.dim, q4.data_ptr(), S.strides(*q4.stride()[:3]), tables.data_ptr(), lengths.data_ptr(), r, n, heads,
-                     tables.shape[1], count, first, last, code, out.data_ptr())
-        return out[:, 0] if q.ndim == 3 else out
+                     self.dim, qp, st, tp, lp, r, n, heads, width, count, first, last, code, out.data_ptr())
+        return out
 
     def token_weights(self) -> Tensor:
         """Room for the weight of every token, float32 [P,Hkv,page], zeros."""
@@ -439,8 +450,7 @@ class Kv4Cache:
         for t in (lengths, tables, free_pages, free_count):
             if not t.is_contiguous():
                 raise ValueError("lengths, tables, free_pages and free_count are updated in place: they must be contiguous")
-        kept = torch.empty((r, self.kv_heads, keep), device=self.device, dtype=torch.int32)
-        dropped = torch.empty((r,), device=self.device, dtype=torch.int32)
+        kept, dropped = lengths.new_empty((r, self.kv_heads, keep)), lengths.new_empty((r,))
         if r:
             S.launch(self.device, "sa_kv4_evict", *cache, weights.data_ptr(), lengths.data_ptr(), tables.data_ptr(),
                      free_pages.data_ptr(), free_count.data_ptr(), r, width, free_pages.shape[0], keep, limit, first, last,
