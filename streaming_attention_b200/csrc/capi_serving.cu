@@ -145,6 +145,7 @@ int attend_args(Kv4AttendArgs* a, const void* k_codes, const void* k_params, con
   a->q_r = strides[0];
   a->q_n = strides[1];
   a->q_h = strides[2];
+  a->vec_q = rows_aligned(q, elem_size(dtype), strides[0] | strides[1], strides[2]);
   a->tables = tables;
   a->lengths = lengths;
   a->scale = scale;

@@ -38,6 +38,7 @@ struct Kv4AttendArgs {
   const void* q;   // [requests, n, heads, d]
   void* out;
   int64_t q_r, q_n, q_h;   // strides of q in elements (out is contiguous)
+  int vec_q;               // rows of q start on 16-byte borders
   const int32_t* tables;
   const int32_t* lengths;
   int requests, n, heads, width;

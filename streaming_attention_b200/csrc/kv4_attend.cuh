@@ -240,6 +240,11 @@ struct Shape {
   static constexpr int kSmem = kFirst + (3 * kWarps * kRows + 2 * kRows) * 4;
 };
 
+// A kernel that the next one in the stream need not wait for to start, and the place
+// where that one needs what it wrote.
+__device__ __forceinline__ void next_may_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void previous_has_ended() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // How many entries of a list of pages count: those before the first that lies outside
 // the table or is not above the one before it (reported), or is -1.
 template <int kThreads>
@@ -267,6 +272,7 @@ __global__ void __launch_bounds__(kWarps * 32, (Shape<DT, DP, NT, kWarps>::kPerS
   constexpr int kOff = DT == SA_REP_FLOAT32 || kMode == kWeigh ? -8 : 16;
   constexpr int kOffV = DT == SA_REP_BFLOAT16 ? 16 : -8;
   constexpr int kKS = DP / 16;   // k steps of the first product, 16-column tiles of the second
+  if (kMode == kPrefix || kMode == kWeigh) next_may_start();
   extern __shared__ __align__(16) uint8_t smem[];
   float* sm_o = reinterpret_cast<float*>(smem);                // [warps][rows][pitch]
   float* sm_m = reinterpret_cast<float*>(smem + S::kFirst);    // [warps][rows]
@@ -403,12 +409,15 @@ __global__ void __launch_bounds__(kWarps * 32, (Shape<DT, DP, NT, kWarps>::kPerS
 #pragma unroll
     for (int w = 0; w < kKS / 2; ++w) {
       float x[8];
+      const int col = cc * (DP / 4) + w * 8;
+      if (in && a.vec_q && col + 8 <= a.c.d) {
+        load8(x, q + col);
+      } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int col = cc * (DP / 4) + w * 8 + e;
-        x[e] = in && col < a.c.d ? to_f32(q[col]) : 0.0f;
-        sum += x[e];
+        for (int e = 0; e < 8; ++e) x[e] = in && col + e < a.c.d ? to_f32(q[col + e]) : 0.0f;
       }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sum += x[e];
 #pragma unroll
       for (int s = 0; s < S::kQ; ++s) {
         float hi[8];
@@ -652,6 +661,7 @@ __global__ void __launch_bounds__(kWarps * 32, (Shape<DT, DP, NT, kWarps>::kPerS
   // and the cluster's CTAs, each a share of the rows' four columns (where a prefix's parts are read or written,
   // neighbouring threads take neighbouring rows, as they stand there)
   constexpr bool kParts = kMode == kPrefix || kMode == kTail;
+  if (kMode == kTail) previous_has_ended();
   const int share = (valid * (DP / 4) + splits - 1) / splits, share_end = min((int)(blockIdx.x + 1) * share, valid * (DP / 4));
   for (int x = blockIdx.x * share + threadIdx.x; x < share_end; x += kThreads) {
     const int row = kParts ? x % valid : x / (DP / 4), col = (kParts ? x / valid : x - row * (DP / 4)) * 4;
@@ -679,7 +689,7 @@ __global__ void __launch_bounds__(kWarps * 32, (Shape<DT, DP, NT, kWarps>::kPerS
       if (col == 0) a.part_ml[of * rows + row0 + row] = make_float2(top, total);
       continue;
     }
-    if (kMode == kTail) {   // the prefix's parts, in order, kBatch of them on their way at a time
+    if (kMode == kTail) {   // the prefix's parts (in before this loop), in order, kBatch of them on their way at a time
       constexpr int kBatch = 6;
       const int64_t all = (int64_t)a.requests * rows, at = (int64_t)r * rows + row0 + row;
       const int64_t ml_step = a.c.heads * all, o_step = ml_step * (DP / 4);
@@ -763,13 +773,15 @@ int launch_one(const Kv4AttendArgs& a, cudaStream_t s) {
   cfg.blockDim = dim3(kWarps * 32);
   cfg.dynamicSmemBytes = S::kSmem;
   cfg.stream = s;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = (unsigned)splits;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;   // kTail: its own tokens beside the prefix's last CTAs
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = kMode == kTail ? 2 : 1;
   e = cudaLaunchKernelEx(&cfg, kern, a);
   if (e != cudaSuccess) return set_error(SA_ERR_CUDA, "kv4 attend_kernel: %s", cudaGetErrorString(e));
   return check_launch("kv4 attend_kernel");

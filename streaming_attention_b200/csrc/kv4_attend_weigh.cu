@@ -42,6 +42,7 @@ __global__ void __launch_bounds__(kWeightThreads) weights_kernel(const Kv4Attend
                                                 (j & ((1 << a.c.page_shift) - 1));
     sum[i] = 0.0f;
   }
+  previous_has_ended();
   for (int row = 0; row < rows; row += 2) {
     const float2 y = ml[row], z = row + 1 < rows ? ml[row + 1] : make_float2(0.0f, 0.0f);
     float2 x[kEach];
@@ -103,7 +104,17 @@ int launch_kv4_attend_weigh(Kv4AttendArgs a, void* workspace, cudaStream_t s) {
   if (a.c.heads > 65535) return set_error(SA_ERR_UNSUPPORTED, "kv4 weights: grid too large");
   const int rc = launch_mode<kWeigh>(a, s);
   if (rc || a.score_blocks == 0) return rc;
-  weights_kernel<<<dim3((unsigned)ceil_div(a.score_blocks * 16, kWeightThreads * kEach), a.c.heads, a.requests), kWeightThreads, 0, s>>>(a);
+  cudaLaunchConfig_t cfg{};   // what needs no scores of it, and its launch, run beside the attention's last CTAs
+  cfg.gridDim = dim3((unsigned)ceil_div(a.score_blocks * 16, kWeightThreads * kEach), a.c.heads, a.requests);
+  cfg.blockDim = dim3(kWeightThreads);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, weights_kernel, a);
+  if (e != cudaSuccess) return set_error(SA_ERR_CUDA, "kv4 weights_kernel: %s", cudaGetErrorString(e));
   return check_launch("kv4 weights_kernel");
 }
 

@@ -67,7 +67,6 @@ constexpr int kErrK = 521, kErrV = 522, kErrP = 523, kErrS = 524, kErrEmpty = 52
 struct PrefixParams {
   Kv4AttendArgs a;
   int rows;      // requests * n * group
-  int vec_q;     // rows of q take 16-byte loads
   uint64_t wait_ns;
 };
 
@@ -276,6 +275,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_tc_kernel(const __gr
   using L = PrefixLayout<DP>;
   using T = typename Elem<DT>::T;
   constexpr int kStages = L::kStages;
+  next_may_start();
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* kfull = reinterpret_cast<uint64_t*>(smem + L::kBars);
@@ -377,7 +377,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_tc_kernel(const __gr
     const int64_t start = r < kCtaRows ? reinterpret_cast<const int64_t*>(smem + L::kRows)[r] : -1;
     if (start >= 0) {
       const T* from = static_cast<const T*>(a.q) + start + c8 * 8;
-      if (p.vec_q && c8 * 8 + 8 <= a.c.d) {
+      if (a.vec_q && c8 * 8 + 8 <= a.c.d) {
         q_raw[i] = *reinterpret_cast<const uint4*>(from);
       } else {
         union {
@@ -857,7 +857,6 @@ int launch_prefix(const Kv4AttendArgs& a, int64_t rows, cudaStream_t s) {
   PrefixParams p{};
   p.a = a;
   p.rows = (int)rows;
-  p.vec_q = rows_aligned(a.q, elem_size(a.dtype), a.q_r | a.q_n, a.q_h);
   p.wait_ns = wait_limit_ns();
   const int64_t pairs = ceil_div(rows, kCtaRows);
   if (a.c.heads > 65535 || pairs > 65535) return set_error(SA_ERR_UNSUPPORTED, "kv4 prefix: grid too large");
