@@ -5,6 +5,11 @@
 
 namespace sa {
 
+// A kernel that the next one in the stream need not wait for to start, and the place
+// where that one needs what it wrote.
+__device__ __forceinline__ void next_may_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void previous_has_ended() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 struct Kv4Cache {
   uint8_t* k_codes;
   __nv_bfloat16* k_params;

@@ -240,11 +240,6 @@ struct Shape {
   static constexpr int kSmem = kFirst + (3 * kWarps * kRows + 2 * kRows) * 4;
 };
 
-// A kernel that the next one in the stream need not wait for to start, and the place
-// where that one needs what it wrote.
-__device__ __forceinline__ void next_may_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-__device__ __forceinline__ void previous_has_ended() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-
 // How many entries of a list of pages count: those before the first that lies outside
 // the table or is not above the one before it (reported), or is -1.
 template <int kThreads>

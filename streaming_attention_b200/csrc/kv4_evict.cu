@@ -19,10 +19,11 @@ namespace {
 constexpr int kThreads = 384;
 constexpr int kWarps = kThreads / 32;
 constexpr int kChunk = 64;   // tokens moved at a time
-constexpr int kMaxRow = 128;                                   // bytes of a row's codes
-constexpr int kUnits = (2 * kChunk * (kMaxRow / 16) + kThreads - 1) / kThreads; // 16-byte units of keys and of values, a thread
-constexpr int kLoads = 8;                                      // weights on their way, a thread
+constexpr int kAhead = 3;    // chunks on their way
+constexpr int kLoads = 8;    // weights on their way, a thread
+constexpr int kDigits = 2048;
 static_assert(3 * kChunk <= kThreads, "a thread moves one of a token's single words");
+static_assert(kDigits % 8 == 0 && kDigits / 8 <= kThreads && kDigits / 8 % 32 == 0, "eight digits a thread, in whole warps");
 
 // A weight as a whole number of the same order; NaN is the largest.
 __device__ __forceinline__ uint32_t order_of(float x) {
@@ -31,9 +32,14 @@ __device__ __forceinline__ uint32_t order_of(float x) {
   return b >> 31 ? ~b : b | 0x80000000u;
 }
 
+template <int DP>
 __global__ void __launch_bounds__(kThreads, 3) evict_kernel(const Kv4EvictArgs a) {
-  __shared__ int64_t src[4][kChunk], dst[4][kChunk];   // of four chunks' tokens: cells they come from and go to
-  __shared__ int count_of[256];
+  constexpr int bytes = DP / 2;                                      // of a row's codes
+  constexpr int kUnits = (8 * bytes + kThreads - 1) / kThreads;      // 16-byte units of a chunk's keys and values, a thread
+  constexpr int kRing = kAhead + 3;
+  __shared__ int64_t src[kRing][kChunk], dst[kRing][kChunk];   // of chunks' tokens: cells they come from and go to
+  __shared__ int count_of[kDigits];
+  __shared__ int warp_sum[kDigits / 256];
   __shared__ int part[2][kWarps];
   __shared__ int digit, below;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -76,30 +82,38 @@ __global__ void __launch_bounds__(kThreads, 3) evict_kernel(const Kv4EvictArgs a
   const int begin = a.first, end = length - a.last, want = a.keep - a.first - a.last;
   uint32_t border = 0, top = 0;
   int ties = want;
-  for (int at = 24; at >= 0 && want > 0; at -= 8) {
-    if (tid < 256) count_of[tid] = 0;
+  // digits of 11, 11 and 10 bits: a weight's exponent alone would send most of them to a few counters
+  for (int at = 21; want > 0; at = at > 11 ? at - 11 : 0) {
+    const uint32_t digits = at == 0 ? 1023u : 2047u;
+    for (int x = tid; x < kDigits; x += kThreads) count_of[x] = 0;
     __syncthreads();
     for (int j = begin + tid; j < end; j += kThreads) {
       const uint32_t k = key(j);
-      if ((k & top) == border) atomicAdd(&count_of[(k >> at) & 255], 1);
+      if ((k & top) == border) atomicAdd(&count_of[(k >> at) & digits], 1);
     }
     __syncthreads();
-    if (warp == 0) {   // a lane eight digits, from the top
-      int sum = 0;
+    // eight digits a thread, from the top, and the sums before them
+    int sum = 0, upto = 0;
+    if (tid < kDigits / 8) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) sum += count_of[255 - 8 * lane - e];
-      int upto = sum;
+      for (int e = 0; e < 8; ++e) sum += count_of[kDigits - 1 - 8 * tid - e];
+      upto = sum;
 #pragma unroll
       for (int x = 1; x < 32; x *= 2) {
         const int y = __shfl_up_sync(0xffffffffu, upto, x);
         if (lane >= x) upto += y;
       }
+      if (lane == 31) warp_sum[warp] = upto;
+    }
+    __syncthreads();
+    if (tid < kDigits / 8) {
+      for (int w = 0; w < warp; ++w) upto += warp_sum[w];
       int before = upto - sum;
       if (before < ties && ties <= upto)
         for (int e = 0; e < 8; ++e) {
-          const int c = count_of[255 - 8 * lane - e];
+          const int c = count_of[kDigits - 1 - 8 * tid - e];
           if (before + c >= ties) {
-            digit = 255 - 8 * lane - e;
+            digit = kDigits - 1 - 8 * tid - e;
             below = before;
             break;
           }
@@ -108,11 +122,11 @@ __global__ void __launch_bounds__(kThreads, 3) evict_kernel(const Kv4EvictArgs a
     }
     __syncthreads();
     border |= (uint32_t)digit << at;
-    top |= 255u << at;
+    top |= digits << at;
     ties -= below;
     const bool all = count_of[digit] == ties;   // the whole digit is kept
     __syncthreads();
-    if (all) break;
+    if (all || at == 0) break;
   }
   // the list, in order
   int at = 0, equal = 0;
@@ -147,11 +161,10 @@ __global__ void __launch_bounds__(kThreads, 3) evict_kernel(const Kv4EvictArgs a
     __syncthreads();
   }
   // the tokens, a chunk of new places at a time
-  const int bytes = a.c.dp >> 1, bytes_log = 31 - __clz(bytes);
   const int which = tid / kChunk, js = tid - which * kChunk;   // keys' parameters, values', weights
   auto cells = [&](int j0) {
     if (tid >= kChunk || j0 >= a.keep) return;
-    const int j = j0 + tid, at = j0 / kChunk & 3;
+    const int j = j0 + tid, at = j0 / kChunk % kRing;
     int64_t from = -1, to = -1;
     if (j < ((a.keep + 3) & ~3)) {   // places behind `keep` in its word of values take what they hold
       to = cell(j);
@@ -167,16 +180,16 @@ __global__ void __launch_bounds__(kThreads, 3) evict_kernel(const Kv4EvictArgs a
   // unit u: 16 bytes of a key row, or, behind those, four tokens' bytes of four column pairs
   auto load = [&](Part& c, int j0) {
     if (j0 >= a.keep) return;
-    const int64_t* from = src[j0 / kChunk & 3];
+    const int64_t* from = src[j0 / kChunk % kRing];
 #pragma unroll
     for (int x = 0; x < kUnits; ++x) {
       const int u = x * kThreads + tid;
       c.w[x] = make_uint4(0, 0, 0, 0);
       if (u < 4 * bytes) {
-        const int j = u >> (bytes_log - 4);
-        if (from[j] >= 0) c.w[x] = *reinterpret_cast<const uint4*>(a.c.k_codes + from[j] * bytes + (u & (bytes / 16 - 1)) * 16);
+        const int j = u / (bytes / 16);
+        if (from[j] >= 0) c.w[x] = *reinterpret_cast<const uint4*>(a.c.k_codes + from[j] * bytes + u % (bytes / 16) * 16);
       } else if (u < 8 * bytes) {
-        const int v = u - 4 * bytes, j = (v >> (bytes_log - 2)) * 4, b = (v & (bytes / 4 - 1)) * 4;
+        const int v = u - 4 * bytes, j = v / (bytes / 4) * 4, b = v % (bytes / 4) * 4;
         uint4 t[4];
         int byte[4];
 #pragma unroll
@@ -201,17 +214,17 @@ __global__ void __launch_bounds__(kThreads, 3) evict_kernel(const Kv4EvictArgs a
   };
   auto store = [&](const Part& c, int j0) {
     if (j0 >= a.keep) return;
-    const int64_t* from = src[j0 / kChunk & 3];
-    const int64_t* to = dst[j0 / kChunk & 3];
+    const int64_t* from = src[j0 / kChunk % kRing];
+    const int64_t* to = dst[j0 / kChunk % kRing];
 #pragma unroll
     for (int x = 0; x < kUnits; ++x) {
       const int u = x * kThreads + tid;
       if (u < 4 * bytes) {
-        const int j = u >> (bytes_log - 4);
+        const int j = u / (bytes / 16);
         if (j0 + j < a.keep && to[j] >= 0 && from[j] >= 0)
-          *reinterpret_cast<uint4*>(a.c.k_codes + to[j] * bytes + (u & (bytes / 16 - 1)) * 16) = c.w[x];
+          *reinterpret_cast<uint4*>(a.c.k_codes + to[j] * bytes + u % (bytes / 16) * 16) = c.w[x];
       } else if (u < 8 * bytes) {
-        const int v = u - 4 * bytes, j = (v >> (bytes_log - 2)) * 4, b = (v & (bytes / 4 - 1)) * 4;
+        const int v = u - 4 * bytes, j = v / (bytes / 4) * 4, b = v % (bytes / 4) * 4;
         if (to[j] >= 0) *reinterpret_cast<uint4*>(a.c.v_codes + to[j] * bytes + b * 4) = c.w[x];
       }
     }
@@ -227,21 +240,23 @@ __global__ void __launch_bounds__(kThreads, 3) evict_kernel(const Kv4EvictArgs a
     if ((last < fits ? (int)held[last] : kept[last]) != last) break;
     begun += kChunk;
   }
-  // a barrier stands between a chunk's loads and its stores, and behind what says where it goes
-  Part x, y;
-  cells(begun);
-  cells(begun + kChunk);
+  // A barrier stands between a chunk's loads and its stores, and behind what says where it goes: of round i,
+  // chunk i + kAhead + 1's cells, chunk i + kAhead's loads, barrier, chunk i's stores.
+  Part parts[kAhead + 1];
+#pragma unroll
+  for (int x = 0; x <= kAhead; ++x) cells(begun + x * kChunk);
   __syncthreads();
-  load(x, begun);
-  for (int j0 = begun; j0 < a.keep; j0 += 2 * kChunk) {
-    cells(j0 + 2 * kChunk);
-    load(y, j0 + kChunk);
-    __syncthreads();
-    store(x, j0);
-    cells(j0 + 3 * kChunk);
-    load(x, j0 + 2 * kChunk);
-    __syncthreads();
-    store(y, j0 + kChunk);
+#pragma unroll
+  for (int x = 0; x < kAhead; ++x) load(parts[x], begun + x * kChunk);
+  for (int j0 = begun; j0 < a.keep; j0 += (kAhead + 1) * kChunk) {
+#pragma unroll
+    for (int x = 0; x <= kAhead; ++x) {
+      const int j1 = j0 + x * kChunk;
+      cells(j1 + (kAhead + 1) * kChunk);
+      load(parts[(x + kAhead) % (kAhead + 1)], j1 + kAhead * kChunk);
+      __syncthreads();
+      store(parts[x], j1);
+    }
   }
   __syncthreads();
   // whoever stands in the places behind starts from zero
@@ -255,13 +270,14 @@ __global__ void __launch_bounds__(kThreads, 3) evict_kernel(const Kv4EvictArgs a
 
 int launch_kv4_evict(const Kv4EvictArgs& a, cudaStream_t s) {
   if (a.requests > 65535) return set_error(SA_ERR_UNSUPPORTED, "kv4 evict: more than 65535 requests in one call");
-  // weights of 24576 tokens at most (96 KB): registers keep it at two CTAs an SM anyway
-  constexpr int kFits = 24576;
+  // weights of 16384 tokens at most (64 KB): three CTAs an SM
+  constexpr int kFits = 16384;
   Kv4EvictArgs b = a;
   b.fits = (int)std::min<int64_t>((int64_t)a.width << a.c.page_shift, kFits);
-  const cudaError_t e = cudaFuncSetAttribute(evict_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kFits * 4);
+  auto kern = a.c.dp == 32 ? evict_kernel<32> : a.c.dp == 64 ? evict_kernel<64> : a.c.dp == 128 ? evict_kernel<128> : evict_kernel<256>;
+  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kFits * 4);
   if (e != cudaSuccess) return set_error(SA_ERR_CUDA, "kv4 evict smem attribute: %s", cudaGetErrorString(e));
-  evict_kernel<<<dim3((unsigned)a.c.heads, (unsigned)a.requests), kThreads, b.fits * 4, s>>>(b);
+  kern<<<dim3((unsigned)a.c.heads, (unsigned)a.requests), kThreads, b.fits * 4, s>>>(b);
   return check_launch("kv4 evict_kernel");
 }
 

@@ -46,6 +46,7 @@ constexpr int kBoundWarps = 4;
 constexpr int kBatch = 8;
 
 __global__ void __launch_bounds__(kBoundWarps * 32) bounds_kernel(const Kv4BoundsArgs a) {
+  next_may_start();
   __shared__ float joined[kBoundWarps][2][256];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int r = blockIdx.y;
@@ -131,17 +132,18 @@ template <int N>
 struct Columns {
   static constexpr int kWords = N > 1 ? N / 2 : 1;
   uint32_t w[kWords];
+  // (not __ldg: the kernel before may still write them when this one starts)
   __device__ __forceinline__ void load(const __nv_bfloat16* p) {
     if constexpr (N == 8) {
-      const uint4 x = __ldg(reinterpret_cast<const uint4*>(p));
+      const uint4 x = *reinterpret_cast<const uint4*>(p);
       w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w;
     } else if constexpr (N == 4) {
-      const uint2 x = __ldg(reinterpret_cast<const uint2*>(p));
+      const uint2 x = *reinterpret_cast<const uint2*>(p);
       w[0] = x.x, w[1] = x.y;
     } else if constexpr (N == 2) {
-      w[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
+      w[0] = *reinterpret_cast<const uint32_t*>(p);
     } else {
-      w[0] = __ldg(reinterpret_cast<const uint16_t*>(p));
+      w[0] = *reinterpret_cast<const uint16_t*>(p);
     }
   }
   __device__ __forceinline__ float get(int e) const {
@@ -174,6 +176,7 @@ __global__ void __launch_bounds__(kThreads, 3) select_kernel(const Kv4SelectArgs
   if (pages <= a.count) {   // all of them
     if (blockIdx.x == 0)
       for (int e = tid; e < a.count; e += kThreads) out[e] = e < pages ? e : -1;
+    previous_has_ended();   // on every way out: who comes next counts on it
     return;
   }
   const int middle = pages - a.first - a.last, want = a.count - a.first - a.last;
@@ -200,13 +203,20 @@ __global__ void __launch_bounds__(kThreads, 3) select_kernel(const Kv4SelectArgs
     uint64_t* to = gridDim.x > 1 ? cluster.map_shared_rank(keys, 0) : keys;
     const int32_t* table = a.tables + (int64_t)r * a.width + a.first;
     // eight pages of a warp at a time, all their loads on their way
-    for (int w0 = (blockIdx.x * kWarps + warp) * kPages; w0 < middle; w0 += gridDim.x * kWarps * kPages) {
+    const int step = gridDim.x * kWarps * kPages;
+    int page = 0;
+    Columns<kCols> low[kPages], high[kPages];
+    auto fetch = [&](int w0) {
       const int mine = w0 + (lane & (kPages - 1));
-      int page = mine < middle ? __ldg(table + mine) : 0;
+      page = mine < middle ? __ldg(table + mine) : 0;
       const bool bad = page < 0 || page >= a.c.pages;
       if (bad && lane < kPages) report(a.status, kBadPage, page);
       if (bad) page = -1;
-      Columns<kCols> low[kPages], high[kPages];
+    };
+    const int begin = (blockIdx.x * kWarps + warp) * kPages;
+    if (begin < middle) fetch(begin);
+    previous_has_ended();   // the bounds may be on their way
+    for (int w0 = begin; w0 < middle; w0 += step) {
 #pragma unroll
       for (int x = 0; x < kPages; ++x) {
         const int id = max(__shfl_sync(0xffffffffu, page, x), 0);
@@ -214,6 +224,8 @@ __global__ void __launch_bounds__(kThreads, 3) select_kernel(const Kv4SelectArgs
         low[x].load(b);
         high[x].load(b + DP);
       }
+      const int here = page;
+      if (w0 + step < middle) fetch(w0 + step);
       double score[kPages];
 #pragma unroll
       for (int x = 0; x < kPages; ++x) {
@@ -237,10 +249,11 @@ __global__ void __launch_bounds__(kThreads, 3) select_kernel(const Kv4SelectArgs
       score[0] += __shfl_xor_sync(0xffffffffu, score[0], 2);
       score[0] += __shfl_xor_sync(0xffffffffu, score[0], 1);
       const int x = lane >> 2;   // bit 4 chose among pages 0..3 and 4..7, and so on
-      const bool none = __shfl_sync(0xffffffffu, page, x) < 0;
+      const bool none = __shfl_sync(0xffffffffu, here, x) < 0;
       if ((lane & 3) == 0 && w0 + x < middle) to[w0 + x] = order_of(none ? -INFINITY : score[0]);
     }
   }
+  previous_has_ended();
   if (gridDim.x > 1)
     cluster.sync();
   else
@@ -330,13 +343,15 @@ int launch_select(const Kv4SelectArgs& a, cudaStream_t s) {
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = (unsigned)splits;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;   // its set-up beside the bounds' last CTAs
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = 2;
   e = cudaLaunchKernelEx(&cfg, kern, a);
   if (e != cudaSuccess) return set_error(SA_ERR_CUDA, "kv4 select_kernel: %s", cudaGetErrorString(e));
   return check_launch("kv4 select_kernel");
