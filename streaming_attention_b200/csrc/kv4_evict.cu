@@ -18,7 +18,7 @@ namespace {
 
 constexpr int kThreads = 384;
 constexpr int kWarps = kThreads / 32;
-constexpr int kChunk = 64;   // tokens moved at a time
+constexpr int kChunk = 96;   // tokens moved at a time: of width 128, two units a thread
 constexpr int kAhead = 3;    // chunks on their way
 constexpr int kLoads = 8;    // weights on their way, a thread
 constexpr int kDigits = 2048;
@@ -35,7 +35,8 @@ __device__ __forceinline__ uint32_t order_of(float x) {
 template <int DP>
 __global__ void __launch_bounds__(kThreads, 3) evict_kernel(const Kv4EvictArgs a) {
   constexpr int bytes = DP / 2;                                      // of a row's codes
-  constexpr int kUnits = (8 * bytes + kThreads - 1) / kThreads;      // 16-byte units of a chunk's keys and values, a thread
+  constexpr int kSide = kChunk * bytes / 16;                         // 16-byte units of a chunk's keys, or of its values
+  constexpr int kUnits = (2 * kSide + kThreads - 1) / kThreads;      // of a thread
   constexpr int kRing = kAhead + 3;
   __shared__ int64_t src[kRing][kChunk], dst[kRing][kChunk];   // of chunks' tokens: cells they come from and go to
   __shared__ int count_of[kDigits];
@@ -128,38 +129,47 @@ __global__ void __launch_bounds__(kThreads, 3) evict_kernel(const Kv4EvictArgs a
     __syncthreads();
     if (all || at == 0) break;
   }
-  // the list, in order
-  int at = 0, equal = 0;
-  for (int j0 = 0; j0 < length; j0 += kThreads) {
-    const int j = j0 + tid;
-    const bool fixed = j < begin || (j >= end && j < length);
-    const uint32_t k = j >= begin && j < end ? key(j) & top : 0;
-    const bool over = fixed || (j >= begin && j < end && want > 0 && k > border);
-    const bool same = j >= begin && j < end && want > 0 && k == border;
-    const unsigned overs = __ballot_sync(0xffffffffu, over), sames = __ballot_sync(0xffffffffu, same);
-    if (lane == 0) {
-      part[0][warp] = __popc(overs);
-      part[1][warp] = __popc(sames);
-    }
-    __syncthreads();
-    const unsigned before = (1u << lane) - 1;
-    int o = __popc(overs & before), s = equal + __popc(sames & before), o_all = 0, s_all = 0;
-#pragma unroll
-    for (int x = 0; x < kWarps; ++x) {
-      if (x < warp) o += part[0][x], s += part[1][x];
-      o_all += part[0][x];
-      s_all += part[1][x];
-    }
-    // of the equal ones before this one, no more than `ties` were taken
-    if (over || (same && s < ties)) {
-      const int place = at + o + min(s, ties) - min(equal, ties);   // <= j: every key up to this round's has been read
-      kept[place] = j;
-      if (place < fits) held[place] = j;
-    }
-    at += o_all + min(equal + s_all, ties) - min(equal, ties);
-    equal += s_all;
-    __syncthreads();
+  // the list, in order: each warp counts what stays of a run of tokens, and, when all have, writes it
+  const int run = (((length + kWarps - 1) / kWarps) + 31) & ~31, run_end = min((warp + 1) * run, length);
+  auto stays = [&](int j, bool& over, bool& same) {
+    const bool fixed = j < begin || j >= end;
+    const uint32_t k = fixed || j >= run_end ? 0u : key(j) & top;
+    over = j < run_end && (fixed || (want > 0 && k > border));
+    same = j < run_end && !fixed && want > 0 && k == border;
+  };
+  int overs = 0, equal = 0;
+  for (int j0 = warp * run; j0 < run_end; j0 += 32) {
+    bool over, same;
+    stays(j0 + lane, over, same);
+    overs += __popc(__ballot_sync(0xffffffffu, over));
+    equal += __popc(__ballot_sync(0xffffffffu, same));
   }
+  if (lane == 0) {
+    part[0][warp] = overs;
+    part[1][warp] = equal;
+  }
+  __syncthreads();
+  int at = 0;
+  equal = 0;
+  for (int w = 0; w < warp; ++w) {
+    at += part[0][w];
+    equal += part[1][w];
+  }
+  at += min(equal, ties);   // of the equal ones the first `ties` stay
+  for (int j0 = warp * run; j0 < run_end; j0 += 32) {
+    bool over, same;
+    stays(j0 + lane, over, same);
+    const unsigned all_over = __ballot_sync(0xffffffffu, over), all_same = __ballot_sync(0xffffffffu, same);
+    const unsigned before = (1u << lane) - 1;
+    const int s = equal + __popc(all_same & before);
+    if (over || (same && s < ties)) kept[at + __popc(all_over & before) + min(s, ties) - min(equal, ties)] = j0 + lane;
+    at += __popc(all_over) - min(equal, ties);
+    equal += __popc(all_same);
+    at += min(equal, ties);
+  }
+  __syncthreads();
+  for (int j = tid; j < min(fits, a.keep); j += kThreads) held[j] = kept[j];   // the weights are done with
+  __syncthreads();
   // the tokens, a chunk of new places at a time
   const int which = tid / kChunk, js = tid - which * kChunk;   // keys' parameters, values', weights
   auto cells = [&](int j0) {
@@ -185,11 +195,11 @@ __global__ void __launch_bounds__(kThreads, 3) evict_kernel(const Kv4EvictArgs a
     for (int x = 0; x < kUnits; ++x) {
       const int u = x * kThreads + tid;
       c.w[x] = make_uint4(0, 0, 0, 0);
-      if (u < 4 * bytes) {
+      if (u < kSide) {
         const int j = u / (bytes / 16);
         if (from[j] >= 0) c.w[x] = *reinterpret_cast<const uint4*>(a.c.k_codes + from[j] * bytes + u % (bytes / 16) * 16);
-      } else if (u < 8 * bytes) {
-        const int v = u - 4 * bytes, j = v / (bytes / 4) * 4, b = v % (bytes / 4) * 4;
+      } else if (u < 2 * kSide) {
+        const int v = u - kSide, j = v / (bytes / 4) * 4, b = v % (bytes / 4) * 4;
         uint4 t[4];
         int byte[4];
 #pragma unroll
@@ -219,12 +229,12 @@ __global__ void __launch_bounds__(kThreads, 3) evict_kernel(const Kv4EvictArgs a
 #pragma unroll
     for (int x = 0; x < kUnits; ++x) {
       const int u = x * kThreads + tid;
-      if (u < 4 * bytes) {
+      if (u < kSide) {
         const int j = u / (bytes / 16);
         if (j0 + j < a.keep && to[j] >= 0 && from[j] >= 0)
           *reinterpret_cast<uint4*>(a.c.k_codes + to[j] * bytes + u % (bytes / 16) * 16) = c.w[x];
-      } else if (u < 8 * bytes) {
-        const int v = u - 4 * bytes, j = v / (bytes / 4) * 4, b = v % (bytes / 4) * 4;
+      } else if (u < 2 * kSide) {
+        const int v = u - kSide, j = v / (bytes / 4) * 4, b = v % (bytes / 4) * 4;
         if (to[j] >= 0) *reinterpret_cast<uint4*>(a.c.v_codes + to[j] * bytes + b * 4) = c.w[x];
       }
     }
