@@ -34,8 +34,9 @@ def dtype_code(*ts: Tensor) -> int:
 def device_of(first: Tensor, *others: Tensor) -> torch.device:
     """The CUDA device that all tensors are on."""
     dev = first.device
+    index = first.get_device()
     for t in others:
-        if t.device != dev:
+        if t.get_device() != index:
             for x in (first, *others):
                 if not x.is_cuda:
                     raise ValueError("the B200 kernels require CUDA tensors")

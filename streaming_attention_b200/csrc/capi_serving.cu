@@ -41,12 +41,22 @@ struct alignas(16) StatusWord {
 static_assert(alignof(StatusWord) % alignof(long long) == 0 && offsetof(StatusWord, index) == 2 * sizeof(int), "report() stores the index as one 8-byte word");
 __device__ StatusWord g_serving_status;
 
+// (where it lies is asked once for each device: 1 us)
 int* status_word() {
+  static std::atomic<int*> words[64];
+  int device = -1;
+  if (cudaGetDevice(&device) != cudaSuccess) {
+    cudaGetLastError();
+    return nullptr;
+  }
+  if (device >= 0 && device < 64)
+    if (int* known = words[device].load(std::memory_order_relaxed)) return known;
   void* p = nullptr;
   if (cudaGetSymbolAddress(&p, g_serving_status) != cudaSuccess) {
     cudaGetLastError();
     return nullptr;
   }
+  if (device >= 0 && device < 64) words[device].store(static_cast<int*>(p), std::memory_order_relaxed);
   return static_cast<int*>(p);
 }
 
@@ -546,6 +556,7 @@ int sa_kv4_evict(void* k_codes, void* k_params, void* v_codes, void* v_params, i
   if (rc) return rc;
   if (free_size < 0) return set_error(SA_ERR_INVALID_ARG, "sizes must be non-negative");
   if (keep < 1 || limit < keep) return set_error(SA_ERR_INVALID_ARG, "keep must be positive, and limit no less");
+  if (keep > 1 << 30) return set_error(SA_ERR_UNSUPPORTED, "keep must not pass 2^30");
   if (first < 0 || last < 0 || (int64_t)first + last > keep)
     return set_error(SA_ERR_INVALID_ARG, "first and last must be non-negative, and no more than keep together");
   if (requests == 0) return SA_OK;

@@ -739,8 +739,9 @@ template <int DT, int DP, int NT, int kMode, int kWarps = kMode == kPlain ? 8 : 
 int launch_one(const Kv4AttendArgs& a, cudaStream_t s) {
   using S = Shape<DT, DP, NT, kWarps>;
   auto kern = attend_kernel<DT, DP, NT, kMode, kWarps>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
-  if (e != cudaSuccess) return set_error(SA_ERR_CUDA, "kv4 attend smem attribute: %s", cudaGetErrorString(e));
+  static std::atomic<uint64_t> allowed{0};
+  const int rc = allow_shared(kern, S::kSmem, allowed, "kv4 attend");
+  if (rc) return rc;
   const int64_t y = a.c.heads * ceil_div(rows_of<kMode>(a), S::kRows);
   const int64_t z = kMode == kSelected ? (int64_t)a.requests * a.n : kMode == kPrefix ? a.parts : a.requests;
   if (y > 65535 || z > 65535) return set_error(SA_ERR_UNSUPPORTED, "kv4 attend: grid too large");
@@ -769,15 +770,18 @@ int launch_one(const Kv4AttendArgs& a, cudaStream_t s) {
   cfg.dynamicSmemBytes = S::kSmem;
   cfg.stream = s;
   cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = (unsigned)splits;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;   // kTail: its own tokens beside the prefix's last CTAs
-  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = kMode == kTail ? 2 : 1;
-  e = cudaLaunchKernelEx(&cfg, kern, a);
+  if (splits > 1) {
+    attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+    attr[cfg.numAttrs].val.clusterDim.x = (unsigned)splits;
+    attr[cfg.numAttrs].val.clusterDim.y = 1;
+    attr[cfg.numAttrs++].val.clusterDim.z = 1;
+  }
+  if (kMode == kTail) {   // its own tokens beside the prefix's last CTAs
+    attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, a);
   if (e != cudaSuccess) return set_error(SA_ERR_CUDA, "kv4 attend_kernel: %s", cudaGetErrorString(e));
   return check_launch("kv4 attend_kernel");
 }

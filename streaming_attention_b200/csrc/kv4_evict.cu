@@ -276,19 +276,26 @@ __global__ void __launch_bounds__(kThreads, 3) evict_kernel(const Kv4EvictArgs a
   }
 }
 
+constexpr int kFits = 16384;   // tokens whose weights shared memory holds (64 KB): three CTAs an SM
+
+template <int DP>
+int launch_evict(const Kv4EvictArgs& a, cudaStream_t s) {
+  static std::atomic<uint64_t> allowed{0};
+  const int rc = allow_shared(evict_kernel<DP>, kFits * 4, allowed, "kv4 evict");
+  if (rc) return rc;
+  evict_kernel<DP><<<dim3((unsigned)a.c.heads, (unsigned)a.requests), kThreads, a.fits * 4, s>>>(a);
+  return check_launch("kv4 evict_kernel");
+}
+
 }  // namespace
 
 int launch_kv4_evict(const Kv4EvictArgs& a, cudaStream_t s) {
   if (a.requests > 65535) return set_error(SA_ERR_UNSUPPORTED, "kv4 evict: more than 65535 requests in one call");
-  // weights of 16384 tokens at most (64 KB): three CTAs an SM
-  constexpr int kFits = 16384;
   Kv4EvictArgs b = a;
   b.fits = (int)std::min<int64_t>((int64_t)a.width << a.c.page_shift, kFits);
-  auto kern = a.c.dp == 32 ? evict_kernel<32> : a.c.dp == 64 ? evict_kernel<64> : a.c.dp == 128 ? evict_kernel<128> : evict_kernel<256>;
-  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kFits * 4);
-  if (e != cudaSuccess) return set_error(SA_ERR_CUDA, "kv4 evict smem attribute: %s", cudaGetErrorString(e));
-  kern<<<dim3((unsigned)a.c.heads, (unsigned)a.requests), kThreads, b.fits * 4, s>>>(b);
-  return check_launch("kv4 evict_kernel");
+  if (a.c.dp == 32) return launch_evict<32>(b, s);
+  if (a.c.dp == 64) return launch_evict<64>(b, s);
+  return a.c.dp == 128 ? launch_evict<128>(b, s) : launch_evict<256>(b, s);
 }
 
 }  // namespace sa

@@ -9,8 +9,10 @@
 // the second term as 16 more columns of the same product: x_j and sum(Q) in three pieces
 // each.  Values are rounded once, to float16 (2^-12 of them at most), and so are
 // probabilities.  Powers of two keep all in float16's range: one for each query row, one
-// for the keys and one for the values of a CTA, from their largest (what is 2^-26 of the
-// largest and less may lose bits).
+// for the keys and one for the values of a CTA, from the largest of what some row sees.
+// Where a token's are so much smaller than the largest that they would lose bits (2^-16 for
+// keys, 2^-13 for values), the CTA's rows go over their tokens in float32 instead (plain_rows),
+// a warp a row: right, and slow.
 // (Scales outside the products, bfloat16 codes inside: each score then wants 16 bytes of
 // parameters out of shared memory, 2048 of its cycles a tile, and the kernel took 85 us.)
 //
@@ -79,7 +81,7 @@ struct PrefixLayout {
   static constexpr int kStages = 3;
   // the 16 columns of the sums and of the offsets: rows of 32 bytes
   static constexpr int kQSum = kTileRows * 32, kKOff = kTokens * 32;
-  // a raw tile: keys, values, their parameters, and which of its blocks of 16 tokens are there
+  // a raw tile: keys, values, their parameters, and which tokens of each block of 16 some row sees
   static constexpr int kRawV = kTokens * DP / 2, kRawKp = 2 * kRawV, kRawVp = kRawKp + kTokens * 4;
   static constexpr int kRawInfo = kRawVp + kTokens * 4, kRaw = kRawInfo + 16;
   static constexpr int kRawStages = 4;
@@ -164,7 +166,9 @@ __device__ __noinline__ void scale_row(uint32_t to, int columns, float alpha) {
 struct Span {
   int p_lo, p_hi;              // least and largest position of the CTA's rows
   uint32_t k_size, v_size;     // bits of the largest of its keys and values
+  uint32_t k_least, v_least;   // and of the smallest that are not zero
   uint32_t bad;                // whether pages are not there
+  int low;                     // no row's window begins before
   int bound;                   // no token stands there or behind
   int first, tiles;            // this part's tiles
   int sink_tiles, win_tile;    // tile t of all is the t-th of the sequence, or from sink_tiles on the (win_tile + t - sink_tiles)-th
@@ -172,6 +176,10 @@ struct Span {
   __device__ __forceinline__ int token_of(int j) const {
     const int t = first + j;
     return (t < sink_tiles ? t : win_tile + t - sink_tiles) * kTokens;
+  }
+  // whether what a token holds may be so small beside the largest that float16 loses bits of it
+  __device__ __forceinline__ bool wide() const {
+    return __uint_as_float(k_size) > 65536.0f * __uint_as_float(k_least) || __uint_as_float(v_size) > 8192.0f * __uint_as_float(v_least);
   }
 };
 
@@ -270,6 +278,60 @@ __device__ __forceinline__ float max32(const float (&s)[32]) {
   return fmaxf(max3(t[0], t[1], s[28]), max3(max3(t[2], t[3], s[29]), s[30], s[31]));
 }
 
+// A part's rows over its tokens in float32, a warp a row and a token at a time: where float16 would not do.
+template <int DT, int DP>
+__device__ __noinline__ void plain_rows(const Kv4AttendArgs& a, int rows, const Span& sp, const int64_t* starts, const int* positions) {
+  using T = typename Elem<DT>::T;
+  constexpr int kCols = DP / 32;   // column lane + 32 i
+  const int lane = threadIdx.x & 31;
+  const float sc = a.scale * 1.4426950408889634f;
+  const int64_t of = (int64_t)blockIdx.x * a.c.heads + blockIdx.z;
+  for (int r = threadIdx.x >> 5; r < kCtaRows; r += kPrefixThreads / 32) {
+    const int row = blockIdx.y * kCtaRows + r;
+    if (row >= rows) break;
+    const int position = positions[r];
+    float q[kCols], o[kCols], m = -INFINITY, l = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kCols; ++i) {
+      const int c = lane + 32 * i;
+      q[i] = c < a.c.d ? to_f32(static_cast<const T*>(a.q)[starts[r] + c]) : 0.0f;
+      o[i] = 0.0f;
+    }
+#pragma unroll 1
+    for (int x = 0; position >= 0 && x < sp.tiles * kTokens; ++x) {
+      const int j = sp.token_of(x / kTokens) + x % kTokens;
+      if (j >= sp.bound || !(position - j < a.window || j < a.sinks)) continue;
+      const int page = __ldg(a.prefix_table + (j >> a.c.page_shift));
+      if (page < 0 || page >= a.c.pages) continue;
+      const int64_t cell = ((page * (int64_t)a.c.heads + blockIdx.z) << a.c.page_shift) + (j & ((1 << a.c.page_shift) - 1));
+      const float2 k = params(__ldg(reinterpret_cast<const uint32_t*>(a.c.k_params) + cell));
+      const float2 v = params(__ldg(reinterpret_cast<const uint32_t*>(a.c.v_params) + cell));
+      float s = 0.0f, value[kCols];
+#pragma unroll
+      for (int i = 0; i < kCols; ++i) {
+        const int c = lane + 32 * i, shift = 4 * (c & 1);
+        s = fmaf(q[i], fmaf((float)((a.c.k_codes[cell * (DP / 2) + (c >> 1)] >> shift) & 15), k.x, k.y), s);
+        value[i] = fmaf((float)((a.c.v_codes[(cell & ~(int64_t)3) * (DP / 2) + (c >> 1) * 4 + (cell & 3)] >> shift) & 15), v.x, v.y);
+      }
+#pragma unroll
+      for (int d = 16; d >= 1; d /= 2) s += __shfl_xor_sync(0xffffffffu, s, d);
+      s *= sc;
+      const float top = fmaxf(m, s), alpha = top == -INFINITY ? 1.0f : ex2(m - top);
+      const float p = ex2(s + kShift - (top == -INFINITY ? 0.0f : top));
+      m = top;
+      l = fmaf(l, alpha, p);
+#pragma unroll
+      for (int i = 0; i < kCols; ++i) o[i] = fmaf(o[i], alpha, p * value[i]);
+    }
+    if (lane == 0) a.part_ml[of * rows + row] = make_float2(m, l);
+#pragma unroll
+    for (int i = 0; i < kCols; ++i) {
+      const int c = lane + 32 * i;
+      a.part_o[((of * (DP / 4) + c / 4) * rows + row) * 4 + c % 4] = m == -INFINITY ? 0.0f : o[i];
+    }
+  }
+}
+
 template <int DT, int DP>
 __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_tc_kernel(const __grid_constant__ PrefixParams p) {
   using L = PrefixLayout<DP>;
@@ -318,7 +380,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_tc_kernel(const __gr
       mbar_init(&drain[i], 1);
     }
     abort_word[0] = abort_word[1] = 0;
-    *span = Span{2147483647, -1, 0, 0, 0, 0, 0, 0, 0, 0};
+    *span = Span{2147483647, -1, 0, 0, 0x7f800000u, 0x7f800000u, 0, 0, 0, 0, 0, 0, 0};
     fence_mbar_init();
     fence_proxy_async_smem();
   }
@@ -359,6 +421,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_tc_kernel(const __gr
   KeyRanges kr{0, 0, 0};
   if (all_of.p_hi >= 0) kr = key_ranges(all_of.p_lo, all_of.p_hi, bound, a.window, a.sinks);
   all_of.bound = bound;
+  all_of.low = (int)max((int64_t)all_of.p_lo - a.window + 1, (int64_t)0);
   all_of.sink_tiles = (int)((kr.first + kTokens - 1) / kTokens);
   all_of.win_tile = max((int)(kr.begin / kTokens), all_of.sink_tiles);
   const int all = all_of.sink_tiles + max((int)((kr.end + kTokens - 1) / kTokens) - all_of.win_tile, 0);
@@ -394,9 +457,9 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_tc_kernel(const __gr
   }
   // the largest of the part's keys and values
   {
-    float k_size = 0.0f, v_size = 0.0f;
+    float k_size = 0.0f, v_size = 0.0f, k_least = INFINITY, v_least = INFINITY;
     bool bad = false;
-#pragma unroll 4
+#pragma unroll 2
     for (int x = threadIdx.x; x < all_of.tiles * kTokens; x += kPrefixThreads) {
       const int token = all_of.token_of(x / kTokens) + x % kTokens;
       const int page = token < bound ? __ldg(a.prefix_table + (token >> a.c.page_shift)) : 0;
@@ -406,24 +469,35 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_tc_kernel(const __gr
         bad = true;
       }
       const int64_t cell = (out ? 0 : page) * page_step + cell0 + (token & page_mask);
-      const bool in = !out && token < bound;
+      const bool in = !out && token < bound && (token >= all_of.low || token < a.sinks);   // some row sees it
       const float2 k = params(__ldg(reinterpret_cast<const uint32_t*>(a.c.k_params) + cell));
       const float2 v = params(__ldg(reinterpret_cast<const uint32_t*>(a.c.v_params) + cell));
       const float ks = fmaxf(8.0f * fabsf(k.x), fabsf(fmaf(8.0f, k.x, k.y))), vs = fmaxf(fabsf(v.y), fabsf(fmaf(15.0f, v.x, v.y)));
-      if (in && ks < INFINITY) k_size = fmaxf(k_size, ks);
-      if (in && vs < INFINITY) v_size = fmaxf(v_size, vs);
+      if (in && ks < INFINITY && ks > 0.0f) {
+        k_size = fmaxf(k_size, ks);
+        k_least = fminf(k_least, ks);
+      }
+      if (in && vs < INFINITY && vs > 0.0f) {
+        v_size = fmaxf(v_size, vs);
+        v_least = fminf(v_least, vs);
+      }
     }
     const uint32_t k_bits = __reduce_max_sync(0xffffffffu, __float_as_uint(k_size));
     const uint32_t v_bits = __reduce_max_sync(0xffffffffu, __float_as_uint(v_size));
+    const uint32_t k_low = __reduce_min_sync(0xffffffffu, __float_as_uint(k_least));
+    const uint32_t v_low = __reduce_min_sync(0xffffffffu, __float_as_uint(v_least));
     bad = __any_sync(0xffffffffu, bad);
     if (lane == 0) {
       atomicMax(&span->k_size, k_bits);
       atomicMax(&span->v_size, v_bits);
+      atomicMin(&span->k_least, k_low);
+      atomicMin(&span->v_least, v_low);
       if (bad) atomicOr(&span->bad, 1u);
     }
   }
   if (threadIdx.x == 0) {
     span->bound = all_of.bound;
+    span->low = all_of.low;
     span->first = all_of.first;
     span->tiles = all_of.tiles;
     span->sink_tiles = all_of.sink_tiles;
@@ -477,6 +551,11 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_tc_kernel(const __gr
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  if (span->wide()) {
+    if (warp == kIssuer) tmem_dealloc(tmem, 512);
+    plain_rows<DT, DP>(a, p.rows, *span, reinterpret_cast<const int64_t*>(smem + L::kRows), reinterpret_cast<const int*>(smem + L::kPositions));
+    return;
+  }
   const volatile Span* now = span;
   const int tiles = now->tiles;
   const Abort ab{abort_word, a.status, p.wait_ns};
@@ -491,7 +570,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_tc_kernel(const __gr
       const int q_power = reinterpret_cast<const volatile int*>(smem + L::kPowers)[rt];
       const int position = reinterpret_cast<const volatile int*>(smem + L::kPositions)[rt];
       const int k_power = power_for(__uint_as_float(now->k_size), 9);
-      const Span sp{0, now->p_hi, 0, now->v_size, now->bad, now->bound, now->first, tiles, now->sink_tiles, now->win_tile};
+      const Span sp{0, now->p_hi, 0, now->v_size, 0, 0, now->bad, 0, now->bound, now->first, tiles, now->sink_tiles, now->win_tile};
       const int window = (int)min(a.window, (int64_t)2147483647), sinks = (int)min(a.sinks, (int64_t)2147483647);
       float* tops = reinterpret_cast<float*>(smem + L::kTops);
       const int pair = 1 + t * 4 + (warp & 3);   // the barrier of the two warps of 32 rows
@@ -535,7 +614,9 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_tc_kernel(const __gr
           ok = false;
           break;
         }
-        const float top = fmaxf(mine, tops[(buf * 2 + (half ^ 1)) * kCtaRows + rt]) * c2;
+        // no less than the product that exp_chunk takes it from, which is not rounded (NaN, where nothing is seen, moves nothing)
+        const float rounded = fmaxf(mine, tops[(buf * 2 + (half ^ 1)) * kCtaRows + rt]) * c2;
+        const float top = fmaf(fabsf(rounded), 0x1p-23f, rounded);
         const bool move = top > m + kMove;
         if (__any_sync(0xffffffffu, move)) {
           const float to = move ? top : m;
@@ -621,7 +702,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_tc_kernel(const __gr
           w[i] = *reinterpret_cast<const uint4*>(raw + token * (DP / 2) + piece * 16);
           kp[i] = *reinterpret_cast<const uint32_t*>(raw + L::kRawKp + token * 4);
           vp[i] = *reinterpret_cast<const uint32_t*>(raw + L::kRawVp + token * 4);
-          in[i] = (token & 15) < reinterpret_cast<const int*>(raw + L::kRawInfo)[token >> 4];
+          in[i] = (reinterpret_cast<const uint32_t*>(raw + L::kRawInfo)[token >> 4] >> (token & 15)) & 1u;
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&rempty[rs]);
@@ -670,13 +751,13 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_tc_kernel(const __gr
         if (!ok) break;
         const uint8_t* raw = smem + L::kRaws + rs * L::kRaw;
         uint4 w[2], ps[2];
-        int left = 0;   // how many of the eight are there
+        uint32_t on = 0;   // bit e: some row sees the e-th of the eight
         if (quad < DP / 8) {
           w[0] = *reinterpret_cast<const uint4*>(raw + L::kRawV + chunk * (4 * DP) + quad * 16);
           w[1] = *reinterpret_cast<const uint4*>(raw + L::kRawV + chunk * (4 * DP) + 2 * DP + quad * 16);
           ps[0] = *reinterpret_cast<const uint4*>(raw + L::kRawVp + chunk * 32);
           ps[1] = *reinterpret_cast<const uint4*>(raw + L::kRawVp + chunk * 32 + 16);
-          left = reinterpret_cast<const int*>(raw + L::kRawInfo)[chunk >> 1] - (chunk & 1) * 8;
+          on = reinterpret_cast<const uint32_t*>(raw + L::kRawInfo)[chunk >> 1] >> (chunk & 1) * 8;
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&rempty[rs]);
@@ -690,7 +771,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_tc_kernel(const __gr
             float2 v[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              v[e] = params(4 * h + e < left ? p4[e] : 0u);
+              v[e] = params((on >> (4 * h + e)) & 1u ? p4[e] : 0u);
               if (!(fabsf(v[e].x) + fabsf(v[e].y) < INFINITY)) v[e] = make_float2(0.0f, 0.0f);   // its key is NaN
             }
 #pragma unroll
@@ -726,7 +807,8 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_tc_kernel(const __gr
       // a tile is one run of tokens in a page, or of two or four in pages of 32 and 16: a lane for each and each of
       // keys, values and their parameters
       const int runs = max(kTokens >> a.c.page_shift, 1), tokens = kTokens / runs;
-      const Span sp{0, 0, 0, 0, 0, now->bound, now->first, tiles, now->sink_tiles, now->win_tile};
+      const Span sp{0, 0, 0, 0, 0, 0, 0, now->low, now->bound, now->first, tiles, now->sink_tiles, now->win_tile};
+      const int sinks = (int)min(a.sinks, (int64_t)2147483647);
       const int64_t cell0 = (int64_t)hk << a.c.page_shift, page_step = (int64_t)a.c.heads << a.c.page_shift;
       const int page_mask = (1 << a.c.page_shift) - 1;
       const int what = lane / runs, run = lane - what * runs;
@@ -745,7 +827,11 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_tc_kernel(const __gr
         const int block_page = __shfl_sync(0xffffffffu, page_l, at + (lane & 3) * 16 / tokens);
         if (j >= L::kRawStages && !mbar_wait_warp_lazy(&rempty[rs], ((j / L::kRawStages) - 1) & 1, ab, kErrRaw)) break;
         uint8_t* raw = smem + L::kRaws + rs * L::kRaw;
-        if (lane < 4) reinterpret_cast<int*>(raw + L::kRawInfo)[lane] = block_page < 0 ? 0 : sp.bound - sp.token_of(j) - lane * 16;
+        if (lane < 4) {   // which tokens of block `lane` some row sees
+          const int j0 = sp.token_of(j) + lane * 16;
+          reinterpret_cast<uint32_t*>(raw + L::kRawInfo)[lane] =
+              block_page < 0 ? 0u : low_bits(sp.bound - j0) & (~low_bits(sp.low - j0) | low_bits(sinks - j0));
+        }
         __syncwarp();
         if (lane == 0) mbar_arrive_expect_tx(&rfull[rs], kTokens * DP + 2 * kTokens * 4);
         __syncwarp();
@@ -852,8 +938,9 @@ template <int DT, int DP>
 int launch_prefix(const Kv4AttendArgs& a, int64_t rows, cudaStream_t s) {
   using L = PrefixLayout<DP>;
   auto kern = prefix_tc_kernel<DT, DP>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes);
-  if (e != cudaSuccess) return set_error(SA_ERR_CUDA, "kv4 prefix smem attribute: %s", cudaGetErrorString(e));
+  static std::atomic<uint64_t> allowed{0};
+  const int rc = allow_shared(kern, L::kBytes, allowed, "kv4 prefix");
+  if (rc) return rc;
   PrefixParams p{};
   p.a = a;
   p.rows = (int)rows;

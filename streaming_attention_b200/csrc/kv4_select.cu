@@ -193,7 +193,10 @@ __global__ void __launch_bounds__(kThreads, 3) select_kernel(const Kv4SelectArgs
       up[c] = x;
       down[c] = y;
     }
-    __syncthreads();
+    if (gridDim.x > 1)
+      cluster.sync();   // the first CTA has begun: its shared memory may be written
+    else
+      __syncthreads();
     double u[kCols], d[kCols];
 #pragma unroll
     for (int e = 0; e < kCols; ++e) {
@@ -334,8 +337,9 @@ int launch_select(const Kv4SelectArgs& a, cudaStream_t s) {
   const int64_t z = (int64_t)a.requests * a.n;
   if (z > 65535 || a.c.heads > 65535) return set_error(SA_ERR_UNSUPPORTED, "kv4 select: grid too large");
   const size_t smem = (size_t)a.width * 8;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSelectMaxPages * 8);
-  if (e != cudaSuccess) return set_error(SA_ERR_CUDA, "kv4 select smem attribute: %s", cudaGetErrorString(e));
+  static std::atomic<uint64_t> allowed{0};
+  const int rc = allow_shared(kern, kSelectMaxPages * 8, allowed, "kv4 select");
+  if (rc) return rc;
   int splits = 1;   // while a warp keeps eight pages and CTAs are few
   while (splits < 8 && a.width >= splits * 2 * kWarps * kPages && z * a.c.heads * splits < 148) splits *= 2;
   cudaLaunchConfig_t cfg{};
@@ -352,7 +356,7 @@ int launch_select(const Kv4SelectArgs& a, cudaStream_t s) {
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  e = cudaLaunchKernelEx(&cfg, kern, a);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, a);
   if (e != cudaSuccess) return set_error(SA_ERR_CUDA, "kv4 select_kernel: %s", cudaGetErrorString(e));
   return check_launch("kv4 select_kernel");
 }

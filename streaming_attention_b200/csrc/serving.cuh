@@ -6,6 +6,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <atomic>
+
 #include "sa_common.cuh"
 
 namespace sa {
@@ -99,6 +101,20 @@ __device__ __forceinline__ void store8(T* p, const float (&x)[8]) {
 // Whether every row of a tensor with these strides starts on a 16-byte border.
 __host__ inline bool rows_aligned(const void* p, int elem, int64_t s0, int64_t s1) {
   return (((uintptr_t)p | (uintptr_t)(s0 * elem) | (uintptr_t)(s1 * elem)) & 15) == 0;
+}
+
+// Lets `kern` take `bytes` of dynamic shared memory on the current device; `done`, one for each kernel, remembers
+// for which devices that has been said (a call of 0.5 us that a decode step would make for every kernel).
+template <typename Kernel>
+__host__ int allow_shared(Kernel kern, int bytes, std::atomic<uint64_t>& done, const char* what) {
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  const uint64_t bit = device < 64 ? 1ull << device : 0;
+  if (e == cudaSuccess && (done.load(std::memory_order_relaxed) & bit)) return SA_OK;
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != cudaSuccess) return set_error(SA_ERR_CUDA, "%s smem attribute: %s", what, cudaGetErrorString(e));
+  done.fetch_or(bit, std::memory_order_relaxed);
+  return SA_OK;
 }
 
 __host__ inline int elem_size(int dtype) { return dtype == SA_REP_FLOAT32 ? 4 : 2; }

@@ -17,10 +17,10 @@ pytestmark = pytest.mark.gpu
 
 F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
 TYPES = pytest.mark.parametrize("dtype", [F32, F16, BF16], ids=["f32", "f16", "bf16"])
-# rounding of the probabilities: 16 bits kept; behind a shared prefix those of bfloat16
-# queries may be rounded to bfloat16
+# rounding of the probabilities: 16 bits kept; over a shared prefix those of 16-bit queries and the
+# values are rounded to float16: half a step (2^-11) of each term p v from either, 2^-10 in all
 P_HALF = {F32: 0.0, F16: 2.0 ** -16, BF16: 2.0 ** -16}
-P_SHARED = {F32: 0.0, F16: 2.0 ** -16, BF16: 2.0 ** -8}
+P_SHARED = {F32: 0.0, F16: 2.0 ** -10, BF16: 2.0 ** -10}
 
 
 @pytest.fixture(scope="module")
@@ -162,6 +162,97 @@ def test_shared_prefix_bad_pages_and_nan(requests, dev):
         cache.attend_shared(q, table, lens[:1], tables[1:], lens[1:])
     with pytest.raises(ValueError, match="longer than its table"):
         cache.attend_shared(q, tables[0, :3], lens[:1], tables[1:], lens[1:])
+
+
+def _shared_case(dev, requests, k, v, window, sinks, dtype, q_scale=1.0, own=5, seed=1):
+    """Prefix rows k, v [P,1,64] and `own` tokens of each request, of the same size; checks every request."""
+    prefix, g = k.shape[0], R.rng(seed)
+    pages = -(-prefix // 64)
+    cache = sa.Kv4Cache.empty(pages + requests, 1, 64, page_size=64, device=dev)
+    own_k, own_v = (torch.randn(requests * own, 1, 64, generator=g) * x[:3].abs().median() for x in (k, v))
+    slots = torch.cat([torch.arange(prefix), ((pages + torch.arange(requests))[:, None] * 64 + torch.arange(own)).flatten()]).to(torch.int32)
+    cache.append(torch.cat([k, own_k]).to(dev), torch.cat([v, own_v]).to(dev), slots.to(dev))
+    rk, rv = (x.cpu().double() for x in cache.read(slots.to(dev)))
+    q = (_queries(requests, 1, 2, 64, F32, seed + 1, dev) * q_scale).to(dtype)
+    out = cache.attend_shared(q, torch.arange(pages, dtype=torch.int32, device=dev), _i32([prefix], dev),
+                              (pages + torch.arange(requests, dtype=torch.int32, device=dev))[:, None], _i32([own] * requests, dev),
+                              window=window, sinks=sinks)
+    for r in range(requests):
+        at = list(range(prefix)) + list(range(prefix + r * own, prefix + (r + 1) * own))
+        ref, spread, score, _ = L.attend(q[r].cpu().double(), torch.nan_to_num(rk[at]), torch.nan_to_num(rv[at]),
+                                         R.visible(1, prefix + own, window, sinks), 0.125)
+        _close(out[r], ref, spread, score, 64, prefix + own, P_SHARED[dtype])
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=["f16", "bf16"])
+@pytest.mark.parametrize("k_size,v_size,q_size", [(1e-15, 1e20, 1.0), (1e15, 1e-20, 1e-4), (1e-30, 1e-30, 1.0), (1.0, 1.0, 1e-5)])
+def test_shared_prefix_of_any_size(k_size, v_size, q_size, dtype, dev):
+    if dtype == F16 and v_size > 1:
+        v_size = 1e3   # float16 results
+    g = R.rng(4)
+    _shared_case(dev, 40, torch.randn(500, 1, 64, generator=g) * k_size, torch.randn(500, 1, 64, generator=g) * v_size, None, 0,
+                 dtype, q_size)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=["f16", "bf16"])
+@pytest.mark.parametrize("which", ["k", "v"])
+def test_shared_prefix_of_sizes_far_apart(which, dtype, dev):
+    """One token's row a million times the others, and one a millionth of them: seen, with little weight."""
+    g = R.rng(4)
+    k, v = torch.randn(500, 1, 64, generator=g), torch.randn(500, 1, 64, generator=g)
+    if which == "k":
+        k[100] *= 1e-3   # scores that say nothing, beside those of the others
+        k[200] *= 1e-7
+    else:
+        v[100] *= 1e4
+        v[200] *= 1e-6
+    _shared_case(dev, 40, k, v, None, 0, dtype)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=["f16", "bf16"])
+@pytest.mark.parametrize("value", [1e30, 3e38, float("inf"), float("nan")])
+def test_shared_prefix_hidden_rows_of_any_size(value, dtype, dev):
+    """What no query sees, in a tile whose other tokens are seen, changes nothing."""
+    g = R.rng(4)
+    k, v = torch.randn(500, 1, 64, generator=g), torch.randn(500, 1, 64, generator=g)
+    k[3:390], v[3:390] = value, value   # 505 - 110 = 395: visible from there on, and tokens 0..2
+    _shared_case(dev, 40, k, v, 110, 3, dtype)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=["f16", "bf16"])
+def test_shared_prefix_rows_that_only_some_see(dtype, dev):
+    """Requests of other lengths: the shorter see a token of 1e25 or NaN, the longer ones' windows end behind it."""
+    g, requests, prefix, d = R.rng(9), 40, 700, 64
+    for bad in (1e25, float("nan")):
+        lengths = [3 + 2 * (r % 2) * 40 for r in range(requests)]   # 3 or 83: positions 702 and 782
+        window = 200                                                # tokens 503.. and 583..
+        k, v = torch.randn(prefix, 1, d, generator=g), torch.randn(prefix, 1, d, generator=g)
+        v[560] = bad
+        pages = -(-prefix // 64)
+        cache = sa.Kv4Cache.empty(pages + 2 * requests, 1, d, page_size=64, device=dev)
+        slots = torch.arange(prefix, dtype=torch.int32)
+        cache.append(k.to(dev), v.to(dev), slots.to(dev))
+        tables = pages + 2 * torch.arange(requests, dtype=torch.int32)[:, None] + torch.tensor([0, 1], dtype=torch.int32)
+        ks, vs = [], []
+        for r, x in enumerate(lengths):
+            j = torch.arange(x)
+            s = tables[r][j // 64] * 64 + (j % 64).to(torch.int32)
+            cache.append(torch.randn(x, 1, d, generator=g).to(dev), torch.randn(x, 1, d, generator=g).to(dev), s.to(dev))
+            a, b = cache.read(s.to(dev))
+            ks.append(a.cpu().double())
+            vs.append(b.cpu().double())
+        pk, pv = (x.cpu().double() for x in cache.read(slots.to(dev)))
+        q = _queries(requests, 1, 2, d, dtype, 3, dev)
+        out = cache.attend_shared(q, torch.arange(pages, dtype=torch.int32, device=dev), _i32([prefix], dev), tables.to(dev),
+                                  _i32(lengths, dev), window=window)
+        for r, x in enumerate(lengths):
+            if x == 3:
+                assert not torch.isfinite(out[r]).any() if bad != bad or dtype == F16 else (out[r].abs() > 1e10).any()
+                continue
+            sees = R.visible(1, prefix + x, window, 0)
+            ref, spread, score, _ = L.attend(q[r].cpu().double(), torch.cat([pk, ks[r]]), torch.nan_to_num(torch.cat([pv, vs[r]])),
+                                             sees, 0.125)
+            _close(out[r], ref, spread, score, d, prefix + x, P_SHARED[dtype])
 
 
 def test_shared_prefix_of_nothing_is_attend(dev):
