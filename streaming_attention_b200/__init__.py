@@ -10,7 +10,8 @@ and the segment-mean variant of ``triton_article_attention.py``
 attention with a sliding window and first tokens that stay visible, a paged
 cache held in 4 bits with the attention that reads it, its page tables, the
 norm and rotation of queries and keys, and ``StreamingWindowAttention``, which
-runs them together.  There is no CPU compute path.
+runs them together; on that cache also attention behind a shared prefix, over
+selected pages, and eviction by accumulated weight.  There is no CPU compute path.
 """
 
 from .fast import (  # noqa: F401

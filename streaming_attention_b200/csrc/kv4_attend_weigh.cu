@@ -6,6 +6,9 @@
 // width 128, most of them still in L2) and a second launch turns them into weights.
 // Each slot is added to by one thread, its rows in order: the same bits every time as
 // long as no page stands in two requests' tables; where one does, both are added.
+//
+// 32 requests of 5000..10000 tokens, 32 heads over 8 of 128: 117 us and 14 (275 MB, 42 us):
+// the attention's instructions; a token a thread took the second 19.
 #include "kv4_attend.cuh"
 
 namespace sa {

@@ -15,6 +15,9 @@
 // a warp a row: right, and slow.
 // (Scales outside the products, bfloat16 codes inside: each score then wants 16 bytes of
 // parameters out of shared memory, 2048 of its cycles a tile, and the kernel took 85 us.)
+// 64 requests of 32 heads over 8 of 128 behind 32000 tokens: 59 us (33 GFLOP, 20 us at the
+// measured GEMM rate).  A tile's chain of waits, about 1 us of 64 tokens, bounds it: left out in turn,
+// products were worth 4 us, decoding 7, the exponentials none, all of them together 11.
 //
 // A CTA holds two tiles of 128 query rows of one key head (a row: request, query, head)
 // and a part of the prefix in tiles of 64 tokens; all rows see (nearly) all of it, so a

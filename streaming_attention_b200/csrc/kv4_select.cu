@@ -10,6 +10,10 @@
 // no less than the sum of the heads' scores of any token of the page (but for the
 // bounds' rounding), at the price of one product of 2 d terms for the whole group.
 // The sums are float64: which pages are chosen does not depend on the order of adding.
+//
+// 48 requests of 12000..24000 tokens, 8 key heads of 128, pages of 64, 32 chosen: 24 us
+// (52 MB of bounds, 8 us): latency, of six rounds of loads and five of digits; one page a
+// warp at a time took 51, with every load waited for.
 #include <cooperative_groups.h>
 #include <math.h>
 
@@ -40,8 +44,8 @@ __device__ __forceinline__ float most_of(float x, float y) {
 
 // A CTA per (touched page, head) at a time: a lane holds eight columns (a word of codes) of
 // every (32 / words of a row)-th token of its warp's, kBatch loads on their way at a time;
-// the warps join through shared memory.  (As one warp a page, and four loads, 48 requests' newest
-// pages of 64 tokens x 8 heads, 3.4 MB, took 25 us: the chain of a lane's tokens.)
+// the warps join through shared memory.  (48 requests' newest pages of 64 tokens x 8 heads, 3.4 MB: 10 us,
+// latency; as one warp a page, with four loads, 25: the chain of a lane's tokens.)
 constexpr int kBoundWarps = 4;
 constexpr int kBatch = 8;
 
