@@ -40,6 +40,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <cmath>
 
 #include "kv4_attend.cuh"
 #include "tc_util.cuh"
@@ -956,16 +957,28 @@ int launch_prefix(const Kv4AttendArgs& a, int64_t rows, cudaStream_t s) {
 
 }  // namespace
 
+// From how many query rows of a key head on the tensor cores' tile of 128 rows pays.  One call
+// with its tails and join, this kernel / warps with mma.sync, us, D 128, bf16:
+//   prefix    key heads   16 rows       32 rows       64 rows       256 rows
+//   500       8           18.4 / 14.4   17.2 / 18.5   18.5 / 20.5   24.7 / 22.7
+//   500       1           16.4 / 12.3   16.4 / 12.4   16.5 / 14.4   20.5 / 14.8
+//   4000      8           25.9 / 20.5   25.8 / 24.6   26.7 / 28.7   30.8 / 53.4
+//   4000      1           20.5 / 18.5   20.5 / 20.4   20.5 / 20.5   23.0 / 24.6
+//   32000     8           53.5 / 37.3   53.8 / 55.4   55.0 / 92.8   64.6 / 305
+//   32000     1           28.7 / 24.6   28.7 / 26.7   28.7 / 32.8   33.2 / 52.2
 bool kv4_prefix_tc_takes(const Kv4AttendArgs& a, int64_t rows) {
   return a.dtype != SA_REP_FLOAT32 && a.c.dp <= 128 && rows > 32;
 }
 
-// Parts of the prefix, each a CTA for every pair of row tiles and key head: as many as
-// fill the GPU, of two tiles at least.
+// Parts of the prefix, each a CTA for every pair of row tiles and key head: no more than
+// fill the GPU, and no more than pay.  A tile takes 1 us, and a part 0.09 us of the join that
+// reads it: tiles / parts + 0.09 parts is least at sqrt(11 tiles).  With a part of two tiles at
+// least and no other limit, one key head took 44.1 us for 256 rows of a prefix of 32000, not 33.2.
 int kv4_prefix_tc_parts(const Kv4AttendArgs& a, int64_t rows) {
   const int64_t longest = std::min<int64_t>((int64_t)a.prefix_width << a.c.page_shift, a.window + a.sinks + a.n);
-  const int64_t ctas = ceil_div(rows, kCtaRows) * a.c.heads;
-  return (int)std::max<int64_t>(1, std::min(148 / ctas, ceil_div(longest, 2 * kTokens)));
+  const int64_t ctas = ceil_div(rows, kCtaRows) * a.c.heads, tiles = ceil_div(longest, kTokens);
+  const int64_t pays = std::min(tiles, (int64_t)std::sqrt(11.0 * (double)tiles) + 1);
+  return (int)std::max<int64_t>(1, std::min(148 / ctas, pays));
 }
 
 int launch_kv4_prefix_tc(const Kv4AttendArgs& a, int64_t rows, cudaStream_t s) {
