@@ -272,7 +272,8 @@ class Kv4Cache:
 
         ``weights`` (``token_weights()``, float32 [P,Hkv,page]) is added to, in place: at each
         token's slot the softmax weight it had, summed over the N queries and the
-        heads that read the key head.  No page may then stand in two requests' tables."""
+        heads that read the key head.  No page may then stand in two requests' tables; the call
+        takes a workspace of 4 bytes for each query row and token that ``tables`` (and the window) allow."""
         cache = self._storage()
         if weights is None:
             S.device_of(self.k_codes, q, tables, lengths)

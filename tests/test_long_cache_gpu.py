@@ -70,6 +70,9 @@ SHARED = [
     (5000, [13] * 70, 8, 2, 1, 32, 64, 3000, 2),
     (9001, [3] * 40, 64, 8, 1, 64, 64, None, 0),    # long chains of tiles in one part
     (4100, [5, 6] * 33, 96, 8, 2, 32, 32, None, 0),
+    (900, [5] * 40, 8, 1, 1, 64, 256, None, 0),
+    (700, [9] * 40, 5, 1, 1, 127, 64, 300, 33),
+    (200, [9, 30] * 9, 10, 2, 1, 50, 16, 60, 3),
 ]
 
 
