@@ -6,7 +6,8 @@
 namespace sa {
 
 // A kernel that the next one in the stream need not wait for to start, and the place
-// where that one needs what it wrote.
+// where that one needs what it wrote.  Only for two kernels of one call, the first of them launched
+// in the ordinary way: of other neighbours in the stream nothing is known.
 __device__ __forceinline__ void next_may_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void previous_has_ended() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 

@@ -50,7 +50,6 @@ constexpr int kBoundWarps = 4;
 constexpr int kBatch = 8;
 
 __global__ void __launch_bounds__(kBoundWarps * 32) bounds_kernel(const Kv4BoundsArgs a) {
-  next_may_start();
   __shared__ float joined[kBoundWarps][2][256];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int r = blockIdx.y;
@@ -136,7 +135,6 @@ template <int N>
 struct Columns {
   static constexpr int kWords = N > 1 ? N / 2 : 1;
   uint32_t w[kWords];
-  // (not __ldg: the kernel before may still write them when this one starts)
   __device__ __forceinline__ void load(const __nv_bfloat16* p) {
     if constexpr (N == 8) {
       const uint4 x = *reinterpret_cast<const uint4*>(p);
@@ -180,7 +178,6 @@ __global__ void __launch_bounds__(kThreads, 3) select_kernel(const Kv4SelectArgs
   if (pages <= a.count) {   // all of them
     if (blockIdx.x == 0)
       for (int e = tid; e < a.count; e += kThreads) out[e] = e < pages ? e : -1;
-    previous_has_ended();   // on every way out: who comes next counts on it
     return;
   }
   const int middle = pages - a.first - a.last, want = a.count - a.first - a.last;
@@ -222,7 +219,6 @@ __global__ void __launch_bounds__(kThreads, 3) select_kernel(const Kv4SelectArgs
     };
     const int begin = (blockIdx.x * kWarps + warp) * kPages;
     if (begin < middle) fetch(begin);
-    previous_has_ended();   // the bounds may be on their way
     for (int w0 = begin; w0 < middle; w0 += step) {
 #pragma unroll
       for (int x = 0; x < kPages; ++x) {
@@ -260,7 +256,6 @@ __global__ void __launch_bounds__(kThreads, 3) select_kernel(const Kv4SelectArgs
       if ((lane & 3) == 0 && w0 + x < middle) to[w0 + x] = order_of(none ? -INFINITY : score[0]);
     }
   }
-  previous_has_ended();
   if (gridDim.x > 1)
     cluster.sync();
   else
@@ -351,15 +346,15 @@ int launch_select(const Kv4SelectArgs& a, cudaStream_t s) {
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
-  cudaLaunchAttribute attr[2];
+  // An ordinary launch, behind all of the stream: what a caller put there before may write q, lengths or tables, or
+  // still read the memory that `selected` lies in, and whether that kernel lets others start early is not known here.
+  cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = (unsigned)splits;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
-  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;   // its set-up beside the bounds' last CTAs
-  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 2;
+  cfg.numAttrs = 1;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, a);
   if (e != cudaSuccess) return set_error(SA_ERR_CUDA, "kv4 select_kernel: %s", cudaGetErrorString(e));
   return check_launch("kv4 select_kernel");
