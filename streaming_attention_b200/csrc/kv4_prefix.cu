@@ -974,11 +974,19 @@ bool kv4_prefix_tc_takes(const Kv4AttendArgs& a, int64_t rows) {
 // fill the GPU, and no more than pay.  A tile takes 1 us, and a part 0.09 us of the join that
 // reads it: tiles / parts + 0.09 parts is least at sqrt(11 tiles).  With a part of two tiles at
 // least and no other limit, one key head took 44.1 us for 256 rows of a prefix of 32000, not 33.2.
+// And no fewer than keep a chain of products short: the matrix units cut off what they add,
+// 7e-8 of O for each 16 tokens, always to the same side, so a part is kChain tiles at most and what
+// parts hold is added rounded.  (80 pairs, one part each, over 131072 / 500000 tokens of mean 1: float16
+// results 8e-4 / 3e-3 low; so 1.6e-4 / 1.2e-4, and 10.4 / 37.6 ms, not 12.0 / 44.9.)
+// Every query stands behind the prefix, so rows see no more of it than window and first tokens
+// allow, however far apart they stand.
+constexpr int kChain = 32768 / kTokens;
+
 int kv4_prefix_tc_parts(const Kv4AttendArgs& a, int64_t rows) {
   const int64_t longest = std::min<int64_t>((int64_t)a.prefix_width << a.c.page_shift, a.window + a.sinks + a.n);
   const int64_t ctas = ceil_div(rows, kCtaRows) * a.c.heads, tiles = ceil_div(longest, kTokens);
   const int64_t pays = std::min(tiles, (int64_t)std::sqrt(11.0 * (double)tiles) + 1);
-  return (int)std::max<int64_t>(1, std::min(148 / ctas, pays));
+  return (int)std::max({(int64_t)1, std::min(148 / ctas, pays), ceil_div(tiles, kChain)});
 }
 
 int launch_kv4_prefix_tc(const Kv4AttendArgs& a, int64_t rows, cudaStream_t s) {
