@@ -21,6 +21,7 @@ int launch_plan_pages(const int32_t* lengths, const int32_t* fresh, int32_t* tab
 int launch_release_pages(int32_t* lengths, int32_t* tables, const uint8_t* drop, int32_t* free_pages,
                          int32_t* free_count, int requests, int width, int free_size, int page_shift, int* status,
                          cudaStream_t s);
+int prepare_shrink_requests(int requests);
 int launch_shrink_requests(int32_t* lengths, int32_t* tables, int32_t* free_pages, int32_t* free_count, int32_t* dropped,
                            int requests, int width, int free_size, int page_shift, int keep, int limit, int* status,
                            cudaStream_t s);
@@ -573,7 +574,8 @@ int sa_kv4_evict(void* k_codes, void* k_params, void* v_codes, void* v_params, i
   a.first = first;
   a.last = last;
   a.status = status_word();
-  rc = launch_kv4_evict(a, (cudaStream_t)stream);
+  rc = prepare_shrink_requests(requests);   // what it refuses leaves the cache as it is
+  if (!rc) rc = launch_kv4_evict(a, (cudaStream_t)stream);
   if (rc) return rc;
   return launch_shrink_requests(lengths, tables, free_pages, free_count, dropped, requests, width, free_size,
                                 a.c.page_shift, keep, limit, a.status, (cudaStream_t)stream);

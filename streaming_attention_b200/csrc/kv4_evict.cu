@@ -295,7 +295,6 @@ int launch_evict(const Kv4EvictArgs& a, cudaStream_t s) {
 }  // namespace
 
 int launch_kv4_evict(const Kv4EvictArgs& a, cudaStream_t s) {
-  if (a.requests > 65535) return set_error(SA_ERR_UNSUPPORTED, "kv4 evict: more than 65535 requests in one call");
   Kv4EvictArgs b = a;
   b.fits = (int)std::min<int64_t>((int64_t)a.width << a.c.page_shift, kFits);
   if (a.c.dp == 32) return launch_evict<32>(b, s);

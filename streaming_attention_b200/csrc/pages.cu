@@ -349,16 +349,22 @@ int launch_plan_pages(const int32_t* lengths, const int32_t* fresh, int32_t* tab
   return check_launch("plan_kernel");
 }
 
-int launch_shrink_requests(int32_t* lengths, int32_t* tables, int32_t* free_pages, int32_t* free_count, int32_t* dropped,
-                           int requests, int width, int free_size, int page_shift, int keep, int limit, int* status,
-                           cudaStream_t s) {
+// What may refuse launch_shrink_requests, before anything of an eviction runs: once tokens have moved up, the
+// lengths and tables have to follow.
+int prepare_shrink_requests(int requests) {
   if (requests > kPlanMaxRequests)
     return set_error(SA_ERR_UNSUPPORTED, "eviction: more than %d requests", kPlanMaxRequests);
-  const size_t smem = (size_t)requests * 4;
-  if (smem > 48 * 1024) {
+  if (requests * 4 > 48 * 1024) {
     const cudaError_t e = cudaFuncSetAttribute(shrink_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPlanMaxRequests * 4);
     if (e != cudaSuccess) return set_error(SA_ERR_CUDA, "eviction smem attribute: %s", cudaGetErrorString(e));
   }
+  return SA_OK;
+}
+
+int launch_shrink_requests(int32_t* lengths, int32_t* tables, int32_t* free_pages, int32_t* free_count, int32_t* dropped,
+                           int requests, int width, int free_size, int page_shift, int keep, int limit, int* status,
+                           cudaStream_t s) {
+  const size_t smem = (size_t)requests * 4;
   shrink_kernel<<<1, kShrinkThreads, smem, s>>>(lengths, tables, free_pages, free_count, dropped, requests, width, free_size,
                                                 page_shift, keep, limit, status);
   return check_launch("shrink_kernel");

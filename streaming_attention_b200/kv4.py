@@ -429,7 +429,7 @@ class Kv4Cache:
         over 0, 1, .. and -1 behind its last) and how many a request lost (int32 [R]): its next
         token's position is its length plus all it ever lost.  Heads keep tokens of their
         own, so ``window`` and ``sinks`` count what is held, and bounds of its pages are to be
-        updated as a whole.  No page may stand in two requests' tables."""
+        updated as a whole.  No page may stand in two requests' tables.  Up to 16384 requests a call."""
         cache = self._storage()
         S.device_of(self.k_codes, weights, lengths, tables, free_pages, free_count)
         self._check_weights(weights)
