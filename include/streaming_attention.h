@@ -450,7 +450,7 @@ int sa_kv4_page_bounds(const void* k_codes, const void* k_params, const void* v_
  * behind.  Of the pages up to the query's own: the first `first`, the last `last`, and
  * between them those of the largest score (of equal ones the lowest),
  *   score = sum over the heads that read the key head, over columns c, of max(q_c low_c, q_c high_c),
- * summed in float64; a score that is NaN is the largest.  first + last <= count,
+ * summed in float64; a score that is NaN (0 times an infinite bound is) is the largest.  first + last <= count,
  * width <= 24576. */
 int sa_kv4_select_pages(const void* bounds, int64_t pages, int kv_heads, int page_size, int d, const void* q,
                         const int64_t* strides, const int32_t* tables, const int32_t* lengths, int requests, int n, int heads,

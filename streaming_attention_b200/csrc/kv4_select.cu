@@ -9,6 +9,8 @@
 //           = sum_c up_c high_c + down_c low_c,  up = sum of the heads' max(q, 0), down of min(q, 0),
 // no less than the sum of the heads' scores of any token of the page (but for the
 // bounds' rounding), at the price of one product of 2 d terms for the whole group.
+// The second line is the first where bounds are finite; beside an infinite one it has 0 times
+// infinity for a side that no head uses.  What is not finite is computed by the first line.
 // The sums are float64: which pages are chosen does not depend on the order of adding.
 //
 // 48 requests of 12000..24000 tokens, 8 key heads of 128, pages of 64, 32 chosen: 24 us
@@ -153,6 +155,24 @@ struct Columns {
   }
 };
 
+// A lane's columns of a page's score by the definition, head by head: where the short form is not finite (rare).
+template <typename T, int N>
+__device__ __forceinline__ double score_by_heads(const T* q, int64_t q_h, int group, int columns, const Columns<N>& low,
+                                                 const Columns<N>& high) {
+  double sum = 0.0;
+#pragma unroll
+  for (int e = 0; e < N; ++e)
+#pragma unroll 1
+    for (int h = 0; e < columns && h < group; ++h) {
+      const double x = to_f32(q[h * q_h + e]), at_low = x * (double)low.get(e), at_high = x * (double)high.get(e);
+      sum += at_low != at_low ? at_low : (at_low > at_high ? at_low : at_high);   // (a NaN of either side stays)
+    }
+  return sum;
+}
+
+// Whether a number is no finite one.
+__device__ __forceinline__ bool endless(double x) { return (__double2hiint(x) & 0x7ff00000) == 0x7ff00000; }
+
 constexpr int kPages = 8;   // that a warp scores at a time
 
 // A cluster of CTAs scores the pages of one (query token, key head); its first CTA
@@ -217,6 +237,7 @@ __global__ void __launch_bounds__(kThreads, 3) select_kernel(const Kv4SelectArgs
       if (bad && lane < kPages) report(a.status, kBadPage, page);
       if (bad) page = -1;
     };
+    bool odd = false;   // a share of a score that is not finite
     const int begin = (blockIdx.x * kWarps + warp) * kPages;
     if (begin < middle) fetch(begin);
     for (int w0 = begin; w0 < middle; w0 += step) {
@@ -238,6 +259,7 @@ __global__ void __launch_bounds__(kThreads, 3) select_kernel(const Kv4SelectArgs
           score[x] = fma(u[e], (double)high[x].get(e), score[x]);
           score[x] = fma(d[e], (double)low[x].get(e), score[x]);
         }
+        odd |= endless(score[x]);
       }
       // sums over the lanes: each halving keeps half of the pages, so that in the end four lanes have one page's
 #pragma unroll
@@ -254,6 +276,29 @@ __global__ void __launch_bounds__(kThreads, 3) select_kernel(const Kv4SelectArgs
       const int x = lane >> 2;   // bit 4 chose among pages 0..3 and 4..7, and so on
       const bool none = __shfl_sync(0xffffffffu, here, x) < 0;
       if ((lane & 3) == 0 && w0 + x < middle) to[w0 + x] = order_of(none ? -INFINITY : score[0]);
+    }
+    if (__any_sync(0xffffffffu, odd)) {   // again, a page at a time, those scores alone
+      const T* q = static_cast<const T*>(a.q) + r * a.q_r + i * a.q_n + (int64_t)hk * group * a.q_h + lane * kCols;
+      for (int w = begin; w < middle; w = (w & (kPages - 1)) == kPages - 1 ? w + 1 - kPages + step : w + 1) {
+        const int id = __ldg(table + w);
+        if (id < 0 || id >= a.c.pages) continue;
+        const __nv_bfloat16* b = a.bounds + (id * (int64_t)a.c.heads + hk) * 2 * DP + lane * kCols;
+        Columns<kCols> l, h;
+        l.load(b);
+        h.load(b + DP);
+        double score = 0.0;
+#pragma unroll
+        for (int e = 0; e < kCols; ++e) {
+          score = fma(u[e], (double)h.get(e), score);
+          score = fma(d[e], (double)l.get(e), score);
+        }
+        odd = endless(score);
+        if (!__any_sync(0xffffffffu, odd)) continue;
+        if (odd) score = score_by_heads<T>(q, a.q_h, group, a.c.d - lane * kCols, l, h);
+#pragma unroll
+        for (int x = 16; x >= 1; x /= 2) score += __shfl_xor_sync(0xffffffffu, score, x);
+        if (lane == 4 * (w & (kPages - 1))) to[w] = order_of(score);   // the lane that wrote it above
+      }
     }
   }
   if (gridDim.x > 1)

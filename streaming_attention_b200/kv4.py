@@ -377,7 +377,8 @@ class Kv4Cache:
 
             score = sum over the heads of a key head, columns c, of max(q_c low_c, q_c high_c)
 
-        with the page's ``bounds`` (of equal scores the lowest page; NaN is the largest)."""
+        with the page's ``bounds`` (of equal scores the lowest page; NaN, which 0 times an infinite
+        bound gives, is the largest)."""
         self._storage()
         S.device_of(self.k_codes, q, bounds, tables, lengths)
         self._check_bounds(bounds)
