@@ -589,7 +589,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_tc_kernel(const __gr
         const int buf = j & 1;
         // whether every row that sees anything sees all 64 tokens
         const int t0 = sp.token_of(j);
-        const bool whole = !sp.bad && t0 + kTokens <= sp.bound && (sp.p_hi - t0 < window || t0 + kTokens <= sinks);
+        const bool whole = !sp.bad && t0 <= sp.bound - kTokens && (sp.p_hi - t0 < window || t0 <= sinks - kTokens);   // (t0 + kTokens may be 2^31)
         ok = mbar_wait_warp_lazy(&sfull[2 * t + buf], (j >> 1) & 1, ab, kErrS);
         if (!ok) break;
         tc_fence_after();
