@@ -401,7 +401,7 @@ int sa_kv4_attend(const void* k_codes, const void* k_params, const void* v_codes
  * holds, for each query token and key head, rows of the request's table in ascending
  * order; a query sees the tokens up to its own that stand in them.  Entries from the
  * first -1 on count as none; so do those from the first that is not above the one
- * before or leaves the table, which is reported.  requests * n < 65536. */
+ * before or leaves the table, which is reported.  requests * n < 65536, count <= 2^30. */
 int sa_kv4_attend_pages(const void* k_codes, const void* k_params, const void* v_codes, const void* v_params, int64_t pages,
                         int kv_heads, int page_size, int d, const void* q, void* out, const int64_t* strides,
                         const int32_t* tables, const int32_t* lengths, const int32_t* selected, int count, int requests, int n,
@@ -450,8 +450,8 @@ int sa_kv4_page_bounds(const void* k_codes, const void* k_params, const void* v_
  * behind.  Of the pages up to the query's own: the first `first`, the last `last`, and
  * between them those of the largest score (of equal ones the lowest),
  *   score = sum over the heads that read the key head, over columns c, of max(q_c low_c, q_c high_c),
- * summed in float64; a score that is NaN (0 times an infinite bound is) is the largest.  first + last <= count,
- * width <= 24576. */
+ * summed in float64; a score that is NaN (0 times an infinite bound is) is the largest.  first + last <= count
+ * <= 2^30, width <= 24576, requests * n < 65536. */
 int sa_kv4_select_pages(const void* bounds, int64_t pages, int kv_heads, int page_size, int d, const void* q,
                         const int64_t* strides, const int32_t* tables, const int32_t* lengths, int requests, int n, int heads,
                         int width, int count, int first, int last, int dtype, int32_t* selected, void* stream);
@@ -463,7 +463,7 @@ int sa_kv4_select_pages(const void* bounds, int64_t pages, int kv_heads, int pag
  * places, in place; weights behind become zero, lengths[r] becomes keep, and the pages behind go to the end
  * of the free list.  kept [requests, kv_heads, keep]: which tokens stayed (of other
  * requests 0, 1, .. and -1 behind the last); dropped [requests]: how many did not.
- * 1 <= keep <= limit, first + last <= keep, requests <= 16384.  No page stands in two
+ * 1 <= keep <= limit, first + last <= keep, requests <= 16384, width * page_size <= 2^30.  No page stands in two
  * requests' tables. */
 int sa_kv4_evict(void* k_codes, void* k_params, void* v_codes, void* v_params, int64_t pages, int kv_heads, int page_size,
                  int d, float* weights, int32_t* lengths, int32_t* tables, int32_t* free_pages, int32_t* free_count,

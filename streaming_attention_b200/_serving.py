@@ -55,6 +55,13 @@ def int32(t: Tensor, shape: Tuple[int, ...], what: str) -> Tensor:
     return t if t.is_contiguous() else t.contiguous()
 
 
+def below_2_31(**sizes: int) -> None:
+    """Refuses sizes that the C ABI's 32-bit arguments would cut off."""
+    for what, n in sizes.items():
+        if n >= 1 << 31:
+            raise ValueError(f"{what} must be below 2^31, got {n}")
+
+
 def rows(t: Tensor) -> Tensor:
     """t, or a copy of it, with a contiguous last dimension."""
     return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.detach().contiguous()

@@ -176,6 +176,9 @@ int prefix_sizes(Kv4AttendArgs* a, int prefix_width) {
   return SA_OK;
 }
 
+// Entries that a CTA's threads take in turns, in steps of 31 bits that may pass the last entry by a CTA's width.
+constexpr int kMostCounted = 1 << 30;
+
 int check_workspace(const void* workspace, size_t have, size_t want) {
   if (want == 0) return SA_OK;
   if (!workspace || have < want) return set_error(SA_ERR_WORKSPACE, "the workspace has %zu bytes, %zu are needed", have, want);
@@ -405,6 +408,7 @@ int sa_kv4_attend_pages(const void* k_codes, const void* k_params, const void* v
                              tables, lengths, requests, n, heads, width, 0, 0, scale, dtype);
   if (rc) return rc;
   if (count < 0) return set_error(SA_ERR_INVALID_ARG, "sizes must be non-negative");
+  if (count > kMostCounted) return set_error(SA_ERR_UNSUPPORTED, "count must not pass 2^30");
   if ((int64_t)requests * n > 65535) return set_error(SA_ERR_UNSUPPORTED, "more than 65535 queries in one call");
   if (requests == 0 || n == 0) return SA_OK;
   if (count > 0 && !selected) return set_error(SA_ERR_INVALID_ARG, "null pointer");
@@ -516,6 +520,7 @@ int sa_kv4_select_pages(const void* bounds, int64_t pages, int kv_heads, int pag
   if (n < 0 || count < 0) return set_error(SA_ERR_INVALID_ARG, "sizes must be non-negative");
   if (first < 0 || last < 0 || (int64_t)first + last > count)
     return set_error(SA_ERR_INVALID_ARG, "first and last must be non-negative, and no more than count together");
+  if (count > kMostCounted) return set_error(SA_ERR_UNSUPPORTED, "count must not pass 2^30");
   rc = check_tables(requests, width, shift);
   if (rc) return rc;
   if (width > kSelectMaxPages)
@@ -557,7 +562,9 @@ int sa_kv4_evict(void* k_codes, void* k_params, void* v_codes, void* v_params, i
   if (rc) return rc;
   if (free_size < 0) return set_error(SA_ERR_INVALID_ARG, "sizes must be non-negative");
   if (keep < 1 || limit < keep) return set_error(SA_ERR_INVALID_ARG, "keep must be positive, and limit no less");
-  if (keep > 1 << 30) return set_error(SA_ERR_UNSUPPORTED, "keep must not pass 2^30");
+  if (keep > kMostCounted) return set_error(SA_ERR_UNSUPPORTED, "keep must not pass 2^30");
+  if (((int64_t)width << a.c.page_shift) > kMostCounted)
+    return set_error(SA_ERR_UNSUPPORTED, "eviction: a row of the page table covers more than 2^30 tokens");
   if (first < 0 || last < 0 || (int64_t)first + last > keep)
     return set_error(SA_ERR_INVALID_ARG, "first and last must be non-negative, and no more than keep together");
   if (requests == 0) return SA_OK;

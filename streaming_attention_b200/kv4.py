@@ -248,6 +248,8 @@ class Kv4Cache:
         table_shape = tables.shape
         if len(table_shape) != 2 or table_shape[0] != r:
             raise ValueError(f"tables must be [{r},W]")
+        if max(r, n, heads, table_shape[1]) >= 1 << 31:
+            S.below_2_31(R=r, N=n, H=heads, W=table_shape[1])
         tables = S.int32(tables, table_shape, "tables")
         lengths = S.int32(lengths, (r,), "lengths")
         st = q.stride()
@@ -309,6 +311,7 @@ class Kv4Cache:
         prefix_shape = prefix_table.shape
         if len(prefix_shape) != 1:
             raise ValueError("prefix_table must be [W0]")
+        S.below_2_31(W0=prefix_shape[0])
         prefix_table = S.int32(prefix_table, prefix_shape, "prefix_table")
         prefix_length = S.int32(prefix_length, (1,), "prefix_length")
         out = q.new_empty(q.shape)
@@ -333,6 +336,7 @@ class Kv4Cache:
         if pages.ndim != len(lead) + 1:
             raise ValueError(f"pages must be {[*lead, 'K']}")
         count = pages.shape[-1]
+        S.below_2_31(K=count)
         pages = S.int32(pages, (*lead, count), "pages")
         out = q.new_empty(q.shape)
         if r and n:
@@ -360,6 +364,7 @@ class Kv4Cache:
         self._check_bounds(bounds)
         if tables.ndim != 2:
             raise ValueError("tables must be [R,W]")
+        S.below_2_31(R=tables.shape[0], W=tables.shape[1])
         tables = S.int32(tables, tables.shape, "tables")
         r, width = tables.shape
         lengths = S.int32(lengths, (r,), "lengths")
@@ -384,8 +389,8 @@ class Kv4Cache:
         self._check_bounds(bounds)
         (qp, st, tp, lp), (r, n, heads, width), code, held = self._queries(q, tables, lengths)
         count, first, last = S.whole(count, "count"), S.whole(first, "first"), S.whole(last, "last")
-        if count < 0 or count > 2 ** 31 - 1:
-            raise ValueError("count must lie in [0, 2^31)")
+        if not 0 <= count <= 1 << 30:
+            raise ValueError("count must lie in [0, 2^30]")
         if first < 0 or last < 0 or first + last > count:
             raise ValueError("first and last must be non-negative, and no more than count together")
         out = lengths.new_empty((r, self.kv_heads, count) if q.ndim == 3 else (r, n, self.kv_heads, count))
@@ -430,7 +435,8 @@ class Kv4Cache:
         over 0, 1, .. and -1 behind its last) and how many a request lost (int32 [R]): its next
         token's position is its length plus all it ever lost.  Heads keep tokens of their
         own, so ``window`` and ``sinks`` count what is held, and bounds of its pages are to be
-        updated as a whole.  No page may stand in two requests' tables.  Up to 16384 requests a call."""
+        updated as a whole.  No page may stand in two requests' tables.  Up to 16384 requests a call, of tables of
+        up to 2^30 tokens."""
         cache = self._storage()
         S.device_of(self.k_codes, weights, lengths, tables, free_pages, free_count)
         self._check_weights(weights)
@@ -445,6 +451,7 @@ class Kv4Cache:
         if free_pages.ndim != 1:
             raise ValueError("free_pages must be [F]")
         r, width = tables.shape
+        S.below_2_31(R=r, W=width, F=free_pages.shape[0])
         S.int32(lengths, (r,), "lengths")
         S.int32(tables, (r, width), "tables")
         S.int32(free_pages, free_pages.shape, "free_pages")

@@ -6,8 +6,9 @@ import pytest
 import torch
 
 import streaming_attention_b200 as sa
-from streaming_attention_b200 import _lib
+from streaming_attention_b200 import _lib, _serving
 from test_kv4_gpu import _filled
+from test_kv4_host import _tensors
 from test_long_cache_gpu import F32
 
 
@@ -22,6 +23,40 @@ def test_evict_refuses_many_requests_before_it_moves_anything():
         assert _evict(requests) == _lib.SA_ERR_UNSUPPORTED
         assert "16384 requests" in _lib.load().sa_last_error().decode()
     assert _evict(65536) == _lib.SA_ERR_UNSUPPORTED
+
+
+def test_sizes_near_31_bits_are_refused():
+    assert _evict(1, width=(1 << 26) + 1) == _lib.SA_ERR_UNSUPPORTED and "2^30 tokens" in _lib.load().sa_last_error().decode()
+    assert _evict(1, keep=(1 << 30) + 1, limit=2 ** 31 - 1) == _lib.SA_ERR_UNSUPPORTED
+    lib, p = _lib.load(), ctypes.c_void_p(0x10000)
+    strides = (ctypes.c_int64 * 3)(64, 64, 64)
+    for count in ((1 << 30) + 1, 2 ** 31 - 1):
+        assert lib.sa_kv4_select_pages(p, 4, 1, 16, 64, p, strides, p, p, 1, 1, 1, 1, count, 0, 0, 0, p, None) == _lib.SA_ERR_UNSUPPORTED
+        assert lib.sa_kv4_attend_pages(p, p, p, p, 4, 1, 16, 64, p, p, strides, p, p, p, count, 1, 1, 1, 1, 1.0, 0, None) == _lib.SA_ERR_UNSUPPORTED
+        assert "2^30" in lib.sa_last_error().decode()
+
+
+def test_sizes_past_31_bits_do_not_reach_the_library(monkeypatch):
+    """Expanded tensors of a size that a 32-bit argument would cut off to 3."""
+    monkeypatch.setattr(_serving, "device_of", lambda first, *others: first.device)
+    monkeypatch.setattr(_serving, "launch", lambda *a: pytest.fail("launched"))
+    far = 2 ** 32 + 3
+    cache = sa.Kv4Cache(*_tensors(4), 64)
+    i = lambda *shape: torch.zeros(shape, dtype=torch.int32)  # noqa: E731
+    q, wide = torch.zeros(1, 2, 64), i(1, 1).expand(1, far)
+    weights, bounds = cache.token_weights(), cache.page_bounds()
+    for call in (lambda: cache.attend(q, wide, i(1)), lambda: cache.attend(q, wide, i(1), weights=weights),
+                 lambda: cache.attend_shared(q, wide[0], i(1), i(1, 1), i(1)), lambda: cache.attend_shared(q, i(1), i(1), wide, i(1)),
+                 lambda: cache.attend_pages(q, i(1, 1), i(1), i(1, 2, 1).expand(1, 2, far)),
+                 lambda: cache.attend_pages(q, wide, i(1), i(1, 2, 1)),
+                 lambda: cache.update_page_bounds(bounds, wide, i(1), i(1)),
+                 lambda: cache.select_pages(q, bounds, wide, i(1), count=2),
+                 lambda: cache.evict(weights, i(1), wide, i(1), i(1), keep=1),
+                 lambda: cache.evict(weights, i(1), i(1, 1), i(1).expand(far), i(1), keep=1)):
+        with pytest.raises(ValueError, match=r"below 2\^31"):
+            call()
+    with pytest.raises(ValueError, match="count must lie"):
+        cache.select_pages(q, bounds, i(1, 1), i(1), count=(1 << 30) + 1)
 
 
 @pytest.mark.gpu
