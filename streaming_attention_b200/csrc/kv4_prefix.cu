@@ -245,6 +245,16 @@ __device__ __forceinline__ int power_for(float size, int to) {
 }
 __device__ __forceinline__ float power(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 
+// Whether both parameters of a row are finite (their halves' sum is then).
+__device__ __forceinline__ bool finite(const float2& params) {
+  return fmaf(0.5f, fabsf(params.x), 0.5f * fabsf(params.y)) < INFINITY;
+}
+
+// The size of a row of these parameters: of finite ones finite, of others none (NaN).
+__device__ __forceinline__ float size_of(const float2& params, float size) {
+  return finite(params) ? fminf(size, 3.40282347e38f) : NAN;
+}
+
 // x in three float16 pieces.
 __device__ __forceinline__ void pieces(float x, float (&y)[3]) {
 #pragma unroll
@@ -476,7 +486,9 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_tc_kernel(const __gr
       const bool in = !out && token < bound && (token >= all_of.low || token < a.sinks);   // some row sees it
       const float2 k = params(__ldg(reinterpret_cast<const uint32_t*>(a.c.k_params) + cell));
       const float2 v = params(__ldg(reinterpret_cast<const uint32_t*>(a.c.v_params) + cell));
-      const float ks = fmaxf(8.0f * fabsf(k.x), fabsf(fmaf(8.0f, k.x, k.y))), vs = fmaxf(fabsf(v.y), fabsf(fmaf(15.0f, v.x, v.y)));
+      // (a row's parameters may be finite where a code that it does not have would pass float32: it is as large as any)
+      const float ks = size_of(k, fmaxf(8.0f * fabsf(k.x), fabsf(fmaf(8.0f, k.x, k.y))));
+      const float vs = size_of(v, fmaxf(fabsf(v.y), fabsf(fmaf(15.0f, v.x, v.y))));
       if (in && ks < INFINITY && ks > 0.0f) {
         k_size = fmaxf(k_size, ks);
         k_least = fminf(k_least, ks);
@@ -731,9 +743,8 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_tc_kernel(const __gr
           }
           if (piece == 0) {
             const float2 v = params(in[i] ? vp[i] : 0u);
-            const bool fine = fabsf(v.x) + fabsf(v.y) < INFINITY;
             float y[3];
-            pieces(fine ? fmaf(8.0f, k.x, k.y) * f : NAN, y);
+            pieces(finite(v) ? fmaf(8.0f, k.x * f, k.y * f) : NAN, y);
             *reinterpret_cast<uint4*>(smem + L::kOffsets + s * L::kKOff + sw32(token, 0)) =
                 make_uint4(pack_f16(y[0], y[0]), pack_f16(y[0], y[1]), pack_f16(y[1], y[2]), 0);
           }
@@ -776,7 +787,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_tc_kernel(const __gr
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               v[e] = params((on >> (4 * h + e)) & 1u ? p4[e] : 0u);
-              if (!(fabsf(v[e].x) + fabsf(v[e].y) < INFINITY)) v[e] = make_float2(0.0f, 0.0f);   // its key is NaN
+              if (!finite(v[e])) v[e] = make_float2(0.0f, 0.0f);   // its key is NaN
             }
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
