@@ -8,7 +8,9 @@
 // long as no page stands in two requests' tables; where one does, both are added.
 //
 // 32 requests of 5000..10000 tokens, 32 heads over 8 of 128: 117 us and 14 (275 MB, 42 us):
-// the attention's instructions; a token a thread took the second 19.
+// the attention's instructions; a token a thread took the second 19.  A thread takes a token's rows one after the
+// other, so a prompt's many rows are slow: 512 tokens at once over 8000, 4 heads a key head, 3245 us, of which
+// attention without weights is 340.
 #include "kv4_attend.cuh"
 
 namespace sa {

@@ -7,17 +7,21 @@
 // product is exact in float16's 11, and with x = least + 8 scale
 //   score_j = scale (sum_c q_c k'_jc + x_j sum(Q)),   k' = scale (code - 8),
 // the second term as 16 more columns of the same product: x_j and sum(Q) in three pieces
-// each.  Values are rounded once, to float16 (2^-12 of them at most), and so are
-// probabilities.  Powers of two keep all in float16's range: one for each query row, one
+// each.  Values are rounded once, to float16 (half a step, 2^-11 of them at most), and so are
+// probabilities: fewer bits than kv4_attend.cuh keeps (16 of a probability, codes as they are), which
+// bfloat16's rounding hides and float16's does not quite (errors of 2.5e-4, not 2.1e-4, of the result);
+// two pieces of either would be twice the products.  Powers of two keep all in float16's range: one for each query row, one
 // for the keys and one for the values of a CTA, from the largest of what some row sees.
 // Where a token's are so much smaller than the largest that they would lose bits (2^-16 for
 // keys, 2^-13 for values), the CTA's rows go over their tokens in float32 instead (plain_rows),
-// a warp a row: right, and slow.
+// a warp a row and a token at a time: right, and slow (64 requests of 32 heads over 8 of 128, one such token: behind
+// 4000 tokens 39 -> 2150 us, behind 32000 72 -> 14400).
 // (Scales outside the products, bfloat16 codes inside: each score then wants 16 bytes of
 // parameters out of shared memory, 2048 of its cycles a tile, and the kernel took 85 us.)
-// 64 requests of 32 heads over 8 of 128 behind 32000 tokens: 59 us (33 GFLOP, 20 us at the
-// measured GEMM rate).  A tile's chain of waits, about 1 us of 64 tokens, bounds it: left out in turn,
-// products were worth 4 us, decoding 7, the exponentials none, all of them together 11.
+// 64 requests of 32 heads over 8 of 128 behind 32000 tokens: 60 us (33 GFLOP, 20 us at the
+// measured GEMM rate).  Its 28 tiles a CTA take about 1 us each, a chain of waits, and set-up and end 8: of the
+// other 24 us the cause is not known.  Left out in turn, products were worth 4 us, decoding 7, the
+// exponentials none, all of them together 11.
 //
 // A CTA holds two tiles of 128 query rows of one key head (a row: request, query, head)
 // and a part of the prefix in tiles of 64 tokens; all rows see (nearly) all of it, so a
@@ -968,8 +972,9 @@ int launch_prefix(const Kv4AttendArgs& a, int64_t rows, cudaStream_t s) {
 
 }  // namespace
 
-// From how many query rows of a key head on the tensor cores' tile of 128 rows pays.  One call
-// with its tails and join, this kernel / warps with mma.sync, us, D 128, bf16:
+// From how many query rows of a key head on the tensor cores' tile of 128 rows pays behind prefixes
+// of thousands of tokens; behind some hundreds warps with mma.sync stay ahead by up to 6 us a call,
+// which the rule leaves.  One call with its tails and join, this kernel / warps with mma.sync, us, D 128, bf16:
 //   prefix    key heads   16 rows       32 rows       64 rows       256 rows
 //   500       8           18.4 / 14.4   17.2 / 18.5   18.5 / 20.5   24.7 / 22.7
 //   500       1           16.4 / 12.3   16.4 / 12.4   16.5 / 14.4   20.5 / 14.8
@@ -977,6 +982,9 @@ int launch_prefix(const Kv4AttendArgs& a, int64_t rows, cudaStream_t s) {
 //   4000      1           20.5 / 18.5   20.5 / 20.4   20.5 / 20.5   23.0 / 24.6
 //   32000     8           53.5 / 37.3   53.8 / 55.4   55.0 / 92.8   64.6 / 305
 //   32000     1           28.7 / 24.6   28.7 / 26.7   28.7 / 32.8   33.2 / 52.2
+// Float32 and widths above 128 have no form here (three pieces of either operand; O of two row tiles would not
+// fit TMEM) and go to mma.sync whatever the rows: 64 requests of 32 heads over 8 behind 32000 tokens, float32 of
+// width 128 539 us, bfloat16 of width 256 809, where bfloat16 of width 128 takes 72.
 bool kv4_prefix_tc_takes(const Kv4AttendArgs& a, int64_t rows) {
   return a.dtype != SA_REP_FLOAT32 && a.c.dp <= 128 && rows > 32;
 }

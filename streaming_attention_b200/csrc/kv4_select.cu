@@ -11,9 +11,10 @@
 // bounds' rounding), at the price of one product of 2 d terms for the whole group.
 // The second line is the first where bounds are finite; beside an infinite one it has 0 times
 // infinity for a side that no head uses.  What is not finite is computed by the first line.
-// The sums are float64: which pages are chosen does not depend on the order of adding.
+// The sums are float64: products of 16-bit queries with bounds are exact and their sums nearly so, and which pages are
+// chosen hardly depends on the order of adding (scores have to agree to some 2^-50; float32 queries' products are rounded there).
 //
-// 48 requests of 12000..24000 tokens, 8 key heads of 128, pages of 64, 32 chosen: 24 us
+// 48 requests of 12000..24000 tokens, 8 key heads of 128, pages of 64, 32 chosen: 25 us
 // (52 MB of bounds, 8 us): latency, of six rounds of loads and five of digits; one page a
 // warp at a time took 51, with every load waited for.
 #include <cooperative_groups.h>

@@ -303,7 +303,13 @@ class Kv4Cache:
         in pages ``prefix_table`` int32 [W0]) and behind them its own (``lengths[r]``
         in pages ``tables[r]``).  The queries are the last N of its own tokens; one that it does
         not have (a request of length 0, or shorter than N) gives zeros.  Positions, ``window`` and
-        ``sinks`` count from the prefix's first token."""
+        ``sinks`` count from the prefix's first token.
+
+        16-bit queries of width up to 128 and more than 32 rows a key head go over the prefix with
+        probabilities and values rounded to float16 (2^-11 of each).  Where one visible token's
+        keys are 2^-16 of the largest of its part, or its values 2^-13, and not zero, float32
+        takes over, up to 200 times slower.  The call takes a workspace of 4 bytes for each row and
+        padded column, times the parts the prefix is cut into (at least one for each 32768 tokens)."""
         cache = self._storage()
         S.device_of(self.k_codes, q, prefix_table, prefix_length, tables, lengths)
         w, s = S.check_window(window, sinks)
@@ -358,7 +364,8 @@ class Kv4Cache:
     def update_page_bounds(self, bounds: Tensor, tables: Tensor, lengths: Tensor, new: Tensor) -> None:
         """Writes to ``bounds`` the least and the largest value of each column of the keys
         that the pages of each request's newest ``new[r]`` (int32 [R]) tokens hold;
-        ``lengths`` counts them, as after ``append``.  Other pages' bounds stay."""
+        ``lengths`` counts them, as after ``append``.  Other pages' bounds stay.  A page in two
+        requests' tables holds the same tokens of both."""
         cache = self._storage()
         S.device_of(self.k_codes, bounds, tables, lengths, new)
         self._check_bounds(bounds)
