@@ -777,7 +777,7 @@ int launch_one(const Kv4AttendArgs& a, cudaStream_t s) {
     attr[cfg.numAttrs].val.clusterDim.y = 1;
     attr[cfg.numAttrs++].val.clusterDim.z = 1;
   }
-  if (kMode == kTail) {   // its own tokens beside the prefix's last CTAs
+  if (kMode == kTail) {   // its launch, and its own tokens on SMs without a CTA of the prefix, beside that kernel
     attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
   }
