@@ -70,7 +70,10 @@ constexpr int kPrefixThreads = (kLoader + 2) * 32;          // whole groups of f
 constexpr int kSoftmaxRegs = 80, kDecoderRegs = 64, kOtherRegs = 56;
 static_assert(4 * kSoftmaxRegs + 2 * kDecoderRegs + kOtherRegs <= 7 * 72, "more registers than the launch has");
 constexpr float kShiftP = 6.0f;    // P = 2^(x - m + 6), m at most kMove below the largest x: 2^14 at most, and 2^-14,
-                                   // where float16 starts to lose bits, is 2^-20 of a row's usual largest
+                                   // where float16 starts to lose bits, is 2^-20 of a row's usual largest.  It shows where a token
+                                   // of value 0 has nearly all weight: results of others that have 2^-26 / 2^-28 of it each are 0.3 /
+                                   // 1 % off.  With m moved at 4, and P up to 2^15, that is 0.05 / 0.07 %, and 64 requests behind 32000
+                                   // tokens 72 -> 80 us.
 
 constexpr int kErrK = 521, kErrV = 522, kErrP = 523, kErrS = 524, kErrEmpty = 525, kErrO = 526, kErrDrain = 527, kErrRaw = 528;
 
