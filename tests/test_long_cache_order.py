@@ -9,7 +9,7 @@ import torch
 
 import streaming_attention_b200 as sa
 from test_kv4_gpu import _filled
-from test_long_cache_gpu import BF16, F32, _i32, _queries
+from test_long_cache_gpu import BF16, F32, _queries
 
 CSRC = os.path.join(os.path.dirname(sa.__file__), "csrc")
 
@@ -23,7 +23,7 @@ def test_only_second_kernels_of_a_call_start_early():
     assert early == {"kv4_attend.cuh", "kv4_attend_weigh.cu"}
     # and there it is asked for in the one mode that always follows the prefix's kernel
     text = open(os.path.join(CSRC, "kv4_attend.cuh")).read()
-    before, after = text.split("attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization")
+    before, _ = text.split("attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization")
     assert before.rstrip().splitlines()[-1].strip().startswith("if (kMode == kTail) {")
 
 
